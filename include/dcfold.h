@@ -445,6 +445,104 @@ int dcf_hash_many_async(const dcf_hash_piece* pieces, size_t n,
 /* Read a device dcf_status back into a dcf_result (synchronises stream). */
 int dcf_status_read(const dcf_status* status, void* stream, dcf_result* res);
 
+/* ---- operators on learned tensors ------------------------------------
+ *
+ * Functions of a model's learned tensors alone, which a module holds as
+ * constants: the relative position bias expanded from its table, the
+ * gradient of that table, and the orthogonalisation of a dense matrix.
+ * The reference folds none of them: an exported bias is iota, sub, log,
+ * min, gather and transpose of constants, and its math.log stays in place
+ * (src/patterns/math/canonicalize.rs:6-52 calls the host's libm).  They
+ * never refuse: `folded` is always 1. */
+
+#define DCF_BIAS_MAX_BUCKETS 256
+#define DCF_BIAS_BIDIRECTIONAL 1u /* half of the buckets for keys after the query */
+#define DCF_BIAS_CAUSAL 2u        /* keys after the query: -inf; no gradient from them */
+#define DCF_BIAS_ACCUMULATE 4u    /* gradient: add to the table gradient */
+
+/* A relative position bias: out[h][i][j] = table[bucket(j - pos(i))][h],
+ * pos(i) = first_query + i, or positions[i] where positions are given.
+ * With d = j - pos(i):
+ *   bidirectional: half = num_buckets / 2 (rounded down), n = |d|, and
+ *                  keys after the query (d > 0) use buckets half ..
+ *                  2 * half - 1;
+ *   otherwise      half = num_buckets, n = max(-d, 0).
+ * With e = half / 2 (rounded down), a distance n < e has bucket n, and a
+ * larger one min(half - 1, e + floor((half - e) * log(n / e) /
+ * log(max_distance / e))), evaluated exactly (by comparing integer
+ * powers, so a distance at which a bucket begins belongs to it).  half = 1
+ * has bucket 0 alone.
+ * The table and its gradient are dense [num_buckets][heads].  Strides are
+ * in elements, 0 means dense; keys are contiguous. */
+typedef struct dcf_bias_desc {
+  uint32_t dtype;       /* of the bias (its gradient): DCF_F16, BF16, F32, F64 */
+  uint32_t table_dtype; /* of the table: dtype, or DCF_F32 beside f16 / bf16.
+                         * Table gradients are f32, f64 for a f64 bias,
+                         * whatever this says */
+  uint32_t num_buckets; /* 1 (bidirectional: 2) .. DCF_BIAS_MAX_BUCKETS */
+  uint32_t max_distance; /* > half / 2, < 2^31 */
+  uint32_t flags;       /* DCF_BIAS_* */
+  uint32_t heads;
+  uint64_t batch;       /* gradient only: the bias is shared by the batch */
+  uint64_t queries, keys; /* < 2^31 each */
+  int64_t first_query;  /* position of query 0 where key 0 has position 0; |.| <= 2^40 */
+  int64_t row_stride, head_stride, batch_stride;
+} dcf_bias_desc;
+
+#define DCF_ORTH_MAX_STEPS 16
+
+/* Newton-Schulz orthogonalisation of `batch` matrices G, rows x cols.  On
+ * the side with fewer rows m <= n (a matrix with rows > cols is taken
+ * transposed): X = G / (||G||_F + eps), then per step, with the step's
+ * coefficients (a, b, c),
+ *     A = X X^T,  X <- a X + (b A + c A A) X,
+ * which maps every singular value s of X to a s + b s^3 + c s^5.  The
+ * iterate is kept in two fp16 halves of a scaled value (22 bits or more)
+ * and products are accumulated in 32 bits; the norm is summed in 64.
+ * The coefficients must keep every singular value from [0, 1] within
+ * [-64, 64] (checked). */
+typedef struct dcf_orth_desc {
+  uint32_t dtype, out_dtype; /* DCF_F16, DCF_BF16 or DCF_F32 */
+  uint32_t steps;            /* 0 .. DCF_ORTH_MAX_STEPS */
+  uint32_t reserved;         /* 0 */
+  uint64_t batch, rows, cols; /* rows, cols <= 65536 */
+  int64_t row_stride, batch_stride;         /* of the input, in elements; 0: dense */
+  int64_t out_row_stride, out_batch_stride; /* of the output */
+  double eps;                               /* >= 0 */
+  double coef[DCF_ORTH_MAX_STEPS][3];
+} dcf_orth_desc;
+
+/* Host forms: host pointers, dense tensors (strides 0). */
+int dcf_position_bias(const dcf_bias_desc* desc, const void* table,
+                      const int32_t* positions, void* out, dcf_result* res);
+int dcf_position_bias_grad(const dcf_bias_desc* desc, const void* grad,
+                           const int32_t* positions, void* table_grad,
+                           dcf_result* res);
+int dcf_orthogonalize(const dcf_orth_desc* desc, const void* in, void* out,
+                      dcf_result* res);
+
+/* Device forms: device pointers of one device, work queued on `stream` of
+ * that device, the caller's current device kept.  `positions` (queries
+ * int32 values, any order) may be NULL.  Elements between rows that a
+ * stride leaves out are not written.  The workspace (256-byte aligned) is
+ * of the size the *_workspace call gives; calls that may overlap on the
+ * GPU (two streams, two captured graphs) need one each.  Sums run in a
+ * fixed order: the same call gives the same bits. */
+int dcf_position_bias_async(const dcf_bias_desc* desc, const void* table,
+                            const int32_t* positions, void* out, void* stream);
+int dcf_position_bias_grad_workspace(const dcf_bias_desc* desc, size_t* bytes);
+int dcf_position_bias_grad_async(const dcf_bias_desc* desc, const void* grad,
+                                 const int32_t* positions, void* table_grad,
+                                 void* workspace, size_t workspace_bytes,
+                                 void* stream);
+/* `out` may be `in` (same strides and element type).  Kernels that give up a
+ * bounded wait set status->error (reset it first; dcf_status_read). */
+int dcf_orthogonalize_workspace(const dcf_orth_desc* desc, size_t* bytes);
+int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in,
+                            void* out, void* workspace,
+                            size_t workspace_bytes, dcf_status* status,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

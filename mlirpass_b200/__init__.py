@@ -90,9 +90,29 @@ class Job(ctypes.Structure):
                 ("rhs_splat", ctypes.c_uint8), ("reserved", ctypes.c_uint8 * 6), ("result", Result)]
 
 
+class BiasDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("table_dtype", ctypes.c_uint32), ("num_buckets", ctypes.c_uint32),
+                ("max_distance", ctypes.c_uint32), ("flags", ctypes.c_uint32), ("heads", ctypes.c_uint32),
+                ("batch", ctypes.c_uint64), ("queries", ctypes.c_uint64), ("keys", ctypes.c_uint64),
+                ("first_query", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("batch_stride", ctypes.c_int64)]
+
+
+ORTH_MAX_STEPS = 16
+
+
+class OrthDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("out_dtype", ctypes.c_uint32), ("steps", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32), ("batch", ctypes.c_uint64), ("rows", ctypes.c_uint64),
+                ("cols", ctypes.c_uint64), ("row_stride", ctypes.c_int64), ("batch_stride", ctypes.c_int64),
+                ("out_row_stride", ctypes.c_int64), ("out_batch_stride", ctypes.c_int64), ("eps", ctypes.c_double),
+                ("coef", (ctypes.c_double * 3) * ORTH_MAX_STEPS)]
+
+
 # Every symbol include/dcfold.h declares, with its ctypes signature.
 _VP, _U64, _I, _U32, _SZ = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t
 _RP, _SP = ctypes.POINTER(Result), ctypes.POINTER(Status)
+_BP, _OP, _SZP = ctypes.POINTER(BiasDesc), ctypes.POINTER(OrthDesc), ctypes.POINTER(ctypes.c_size_t)
 SIGNATURES = {
     "dcf_init": (_I, [_I]),
     "dcf_shutdown": (_I, []),
@@ -127,6 +147,14 @@ SIGNATURES = {
     "dcf_hex_decode_many_async": (_I, [_VP, _SZ, _U64, _VP, _VP]),
     "dcf_hash_many_async": (_I, [_VP, _SZ, _U64, _VP, _VP]),
     "dcf_status_read": (_I, [_VP, _VP, _RP]),
+    "dcf_position_bias": (_I, [_BP, _VP, _VP, _VP, _RP]),
+    "dcf_position_bias_grad": (_I, [_BP, _VP, _VP, _VP, _RP]),
+    "dcf_orthogonalize": (_I, [_OP, _VP, _VP, _RP]),
+    "dcf_position_bias_async": (_I, [_BP, _VP, _VP, _VP, _VP]),
+    "dcf_position_bias_grad_workspace": (_I, [_BP, _SZP]),
+    "dcf_position_bias_grad_async": (_I, [_BP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "dcf_orthogonalize_workspace": (_I, [_OP, _SZP]),
+    "dcf_orthogonalize_async": (_I, [_OP, _VP, _VP, _VP, _SZ, _VP, _VP]),
 }
 
 _lib = None
@@ -441,3 +469,233 @@ def status_read(status, stream=None) -> Fold:
     res = Result()
     _check(lib().dcf_status_read(_tptr(status), _stream(stream), ctypes.byref(res)))
     return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), None)
+
+
+# ------------------------------------------- operators on learned tensors
+
+BIAS_BIDIRECTIONAL, BIAS_CAUSAL, BIAS_ACCUMULATE = 1, 2, 4
+# The quintic whose singular values settle between about 0.7 and 1.2 in five steps.
+ORTH_COEF = (3.4445, -4.7750, 2.0315)
+
+
+class BiasPlan:
+    """The sizes, types and strides of one position bias: a dcf_bias_desc
+    that calls reuse.  Validated when made."""
+
+    def __init__(self, desc: BiasDesc, dtype: str, table_dtype: str):
+        self.desc, self.dtype, self.table_dtype = desc, dtype, table_dtype
+        self.ref = ctypes.byref(desc)
+        d = desc
+        row = d.row_stride or d.keys
+        head = d.head_stride or d.queries * row
+        batch = d.batch_stride or d.heads * head
+        some = d.queries and d.keys and d.heads
+        span = (d.queries - 1) * row + (d.heads - 1) * head + d.keys if some else 0
+        self.out_elements = span                     # elements from a bias's first to its last
+        self.grad_elements = span + (d.batch - 1) * batch if some and d.batch else 0
+        self.entries = d.num_buckets * d.heads
+        ws = ctypes.c_size_t(0)
+        _check(lib().dcf_position_bias_grad_workspace(self.ref, ctypes.byref(ws)))
+        self.workspace = ws.value
+
+
+def position_bias_plan(dtype: str, heads: int, queries: int, keys: int, *, num_buckets: int = 32,
+                       max_distance: int = 128, bidirectional: bool = True, causal: bool = False,
+                       first_query: int = 0, batch: int = 1, table_dtype: str | None = None, row_stride: int = 0,
+                       head_stride: int = 0, batch_stride: int = 0, accumulate: bool = False) -> BiasPlan:
+    """Describe a relative position bias (dcf_bias_desc, include/dcfold.h).
+
+    The bias is [heads, queries, keys] of `dtype`, its gradient [batch,
+    heads, queries, keys]; the table is [num_buckets, heads] of table_dtype
+    (dtype, or f32 beside f16 / bf16).  Strides are in elements, 0 is dense.
+    `accumulate` makes the gradient add to what its output holds.
+    """
+    for name, v in (("heads", heads), ("queries", queries), ("keys", keys), ("batch", batch),
+                    ("num_buckets", num_buckets), ("max_distance", max_distance)):
+        if not 0 <= v < 1 << 31:
+            raise ValueError(f"{name} {v} out of range")
+    for name, v in (("first_query", first_query), ("row_stride", row_stride), ("head_stride", head_stride),
+                    ("batch_stride", batch_stride)):
+        if not -(1 << 62) < v < 1 << 62:
+            raise ValueError(f"{name} {v} out of range")
+    table_dtype = table_dtype or dtype
+    flags = (BIAS_BIDIRECTIONAL if bidirectional else 0) | (BIAS_CAUSAL if causal else 0) | \
+        (BIAS_ACCUMULATE if accumulate else 0)
+    desc = BiasDesc(DTYPES[dtype], DTYPES[table_dtype], num_buckets, max_distance, flags, heads, batch, queries, keys,
+                    first_query, row_stride, head_stride, batch_stride)
+    return BiasPlan(desc, dtype, table_dtype)
+
+
+def position_bias(plan: BiasPlan, table, *, positions=None, out: np.ndarray | None = None) -> Fold:
+    """The bias [heads, queries, keys] of a table on host buffers."""
+    d = plan.desc
+    t = as_storage(table, plan.table_dtype)
+    if len(t) != plan.entries:
+        raise ValueError(f"table has {len(t)} elements, {plan.entries} expected")
+    n = d.heads * d.queries * d.keys
+    out = _host_out(out, n, plan.dtype)
+    p = _host_positions(positions, d.queries)
+    res = Result()
+    _check(lib().dcf_position_bias(plan.ref, _ptr(t), _ptr(p) if p is not None else None, _ptr(out),
+                                   ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index),
+                out.reshape(d.heads, d.queries, d.keys))
+
+
+def position_bias_grad(plan: BiasPlan, grad, *, positions=None, out: np.ndarray | None = None) -> Fold:
+    """The table's gradient [num_buckets, heads] on host buffers: f32, f64
+    for a f64 bias.  With an accumulating plan `out` is added to."""
+    d = plan.desc
+    g = as_storage(grad, plan.dtype)
+    n = d.batch * d.heads * d.queries * d.keys
+    if len(g) != n:
+        raise ValueError(f"gradient has {len(g)} elements, {n} expected")
+    wide = np.float64 if plan.dtype == "f64" else np.float32
+    if out is None:
+        if d.flags & BIAS_ACCUMULATE:
+            raise ValueError("an accumulating plan needs `out`")
+        out = np.empty((d.num_buckets, d.heads), wide)
+    elif out.dtype != wide or out.size != plan.entries or not out.flags.c_contiguous:
+        raise ValueError("out must be a contiguous f32 (f64 for f64) array of the table's size")
+    p = _host_positions(positions, d.queries)
+    res = Result()
+    _check(lib().dcf_position_bias_grad(plan.ref, _ptr(g), _ptr(p) if p is not None else None, _ptr(out),
+                                        ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), out)
+
+
+def _host_positions(positions, queries: int):
+    if positions is None:
+        return None
+    p = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
+    if len(p) != queries:
+        raise ValueError(f"{len(p)} positions for {queries} queries")
+    return p
+
+
+def _host_out(out, n: int, dtype: str) -> np.ndarray:
+    if out is None:
+        return np.empty(n, dtype=storage(dtype))
+    if out.size != n or out.dtype.itemsize != DTYPE_SIZE[dtype] or not out.flags.c_contiguous:
+        raise ValueError(f"out must be a contiguous array of {n} {dtype} elements")
+    return out.reshape(-1)
+
+
+def _own_stream(stream, t) -> int:
+    """The given stream, or the current one of the tensor's device."""
+    if stream is None:
+        import torch
+        return torch.cuda.current_stream(t.device).cuda_stream
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _room(t) -> int:
+    """Elements from a tensor's first one to the end of its storage."""
+    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+
+
+def _need(t, what: str, elements: int, size: int) -> int:
+    if t.element_size() != size:
+        raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
+    if _room(t) < elements:
+        raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
+    return t.data_ptr()
+
+
+def position_bias_async(plan: BiasPlan, table, out, *, positions=None, stream=None) -> None:
+    """Launch a position bias on device tensors.  `out` starts at the bias's
+    first element; the plan's strides say where the rest lies."""
+    _check(lib().dcf_position_bias_async(
+        plan.ref, _need(table, "table", plan.entries, DTYPE_SIZE[plan.table_dtype]),
+        None if positions is None else _need(positions, "positions", plan.desc.queries, 4),
+        _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.dtype]), _own_stream(stream, out)))
+
+
+def position_bias_grad_workspace(plan: BiasPlan) -> int:
+    """Bytes of device workspace that a gradient call of this plan needs."""
+    return plan.workspace
+
+
+def position_bias_grad_async(plan: BiasPlan, grad, out, workspace, *, positions=None, stream=None) -> None:
+    """Launch the table gradient on device tensors: `out` is the dense
+    [num_buckets, heads] gradient, `workspace` uint8 (may be empty when
+    position_bias_grad_workspace says 0)."""
+    _check(lib().dcf_position_bias_grad_async(
+        plan.ref, _need(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype]),
+        None if positions is None else _need(positions, "positions", plan.desc.queries, 4),
+        _need(out, "out", plan.entries, 8 if plan.dtype == "f64" else 4), workspace.data_ptr(),
+        _room(workspace) * workspace.element_size(), _own_stream(stream, out)))
+
+
+class OrthPlan:
+    """The sizes, strides and coefficients of one orthogonalisation: a
+    dcf_orth_desc that calls reuse.  Validated when made."""
+
+    def __init__(self, desc: OrthDesc, dtype: str, out_dtype: str):
+        self.desc, self.dtype, self.out_dtype = desc, dtype, out_dtype
+        self.ref = ctypes.byref(desc)
+        d = desc
+
+        def span(row, batch):
+            if not (d.rows and d.cols and d.batch):
+                return 0
+            row = row or d.cols
+            return (d.rows - 1) * row + d.cols + (d.batch - 1) * (batch or d.rows * row)
+        self.in_elements = span(d.row_stride, d.batch_stride)
+        self.out_elements = span(d.out_row_stride, d.out_batch_stride)
+        ws = ctypes.c_size_t(0)
+        _check(lib().dcf_orthogonalize_workspace(self.ref, ctypes.byref(ws)))
+        self.workspace = ws.value
+
+
+def orthogonalize_plan(dtype: str, rows: int, cols: int, *, batch: int = 1, steps: int = 5, coef=ORTH_COEF,
+                       eps: float = 1e-7, out_dtype: str | None = None, row_stride: int = 0, batch_stride: int = 0,
+                       out_row_stride: int = 0, out_batch_stride: int = 0) -> OrthPlan:
+    """Describe a Newton-Schulz orthogonalisation (dcf_orth_desc,
+    include/dcfold.h).  `coef` is one (a, b, c) for every step, or one per step."""
+    for name, v in (("rows", rows), ("cols", cols), ("batch", batch)):
+        if not 0 <= v < 1 << 31:
+            raise ValueError(f"{name} {v} out of range")
+    for name, v in (("row_stride", row_stride), ("batch_stride", batch_stride), ("out_row_stride", out_row_stride),
+                    ("out_batch_stride", out_batch_stride)):
+        if not -(1 << 62) < v < 1 << 62:
+            raise ValueError(f"{name} {v} out of range")
+    if not 0 <= steps <= ORTH_MAX_STEPS:
+        raise ValueError(f"steps must be 0 .. {ORTH_MAX_STEPS}")
+    per_step = [coef] * steps if len(coef) == 0 or not hasattr(coef[0], "__len__") else list(coef)
+    if len(per_step) != steps or any(len(c) != 3 for c in per_step):
+        raise ValueError("coef is three numbers, or three for each step")
+    out_dtype = out_dtype or dtype
+    desc = OrthDesc(DTYPES[dtype], DTYPES[out_dtype], steps, 0, batch, rows, cols, row_stride, batch_stride,
+                    out_row_stride, out_batch_stride, eps)
+    for i, c in enumerate(per_step):
+        for j in range(3):
+            desc.coef[i][j] = float(c[j])
+    return OrthPlan(desc, dtype, out_dtype)
+
+
+def orthogonalize(plan: OrthPlan, x, *, out: np.ndarray | None = None) -> Fold:
+    """Orthogonalise [batch, rows, cols] on host buffers."""
+    d = plan.desc
+    a = as_storage(x, plan.dtype)
+    n = d.batch * d.rows * d.cols
+    if len(a) != n:
+        raise ValueError(f"input has {len(a)} elements, {n} expected")
+    out = _host_out(out, n, plan.out_dtype)
+    res = Result()
+    _check(lib().dcf_orthogonalize(plan.ref, _ptr(a), _ptr(out), ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), out.reshape(d.batch, d.rows, d.cols))
+
+
+def orthogonalize_workspace(plan: OrthPlan) -> int:
+    """Bytes of device workspace that a call of this plan needs."""
+    return plan.workspace
+
+
+def orthogonalize_async(plan: OrthPlan, x, out, workspace, status, *, stream=None) -> None:
+    """Launch an orthogonalisation on device tensors; `out` may be `x`.
+    `status` (16 bytes, reset first) takes a kernel's error report."""
+    _check(lib().dcf_orthogonalize_async(
+        plan.ref, _need(x, "x", plan.in_elements, DTYPE_SIZE[plan.dtype]),
+        _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.out_dtype]), workspace.data_ptr(),
+        _room(workspace) * workspace.element_size(), status.data_ptr(), _own_stream(stream, out)))

@@ -30,7 +30,7 @@ GEN_LIB = os.path.join(PKG, "libdcfgen.so")
 SOURCES = ["dcf_ew_float.cu", "dcf_ew_float_f32.cu", "dcf_ew_float_f64.cu", "dcf_ew_float_h.cu",
            "dcf_ew_float_f8.cu", "dcf_ew_int.cu", "dcf_ew_convert.cu", "dcf_ew_convert_ff.cu",
            "dcf_ew_convert_if.cu", "dcf_ew_convert_fi.cu", "dcf_ew_math.cu", "dcf_misc.cu", "dcf_transpose_tma.cu", "dcf_runtime.cu",
-           "dcf_noalloc.cu", "dcf_rt.cu"]
+           "dcf_noalloc.cu", "dcf_rt.cu", "dcf_bias.cu", "dcf_orth.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,557 @@
+// dcf_bias.cu — the relative position bias expanded from a learned table of
+// buckets, and the gradient of that table.
+//
+//   bias:      out[h][i][j] = table[bucket(j - pos(i))][h]
+//   gradient:  d table[v][h] = sum of g[b][h][i][j] over b and the (i, j)
+//              whose bucket is v
+//
+// An exported model holds the first as iota, sub, abs, log, floor, min,
+// select, gather and transpose; here the bucket of a distance is a search
+// in the sorted list of distances at which buckets begin.  That list is
+// made on the host by comparing integer powers (bias_starts), so no device
+// log decides a border.
+//
+// Both are bound by HBM: one write, or one read, per element of the bias,
+// against one table value or one addition.  What has to be kept small is the
+// work per element around that, above all finding its bucket: a thread owns
+// one 16-byte vector of a row, looks up its first and last distance, and
+// where they agree (nearly everywhere: buckets widen with distance)
+// the vector is one value; the lookup is shared by all heads.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "dcf_launch.h"
+
+namespace dcf {
+
+namespace {
+
+constexpr int kMaxB = DCF_BIAS_MAX_BUCKETS;
+constexpr int kSms = 148;
+
+// How a distance maps to its bucket; a kernel parameter.
+struct Buckets {
+  int half;           // buckets per direction
+  int both;           // keys after the query have buckets half .. 2 half - 1
+  int causal;
+  int last;           // distances >= last have bucket half - 1
+  int start[kMaxB];   // first distance of each bucket, sorted
+};
+
+struct BiasArgs {
+  uint64_t queries, keys;
+  int64_t first;
+  int64_t rs, hs, bs;   // strides in elements
+  int heads, nb;
+  uint64_t batch;
+  const int32_t* pos;
+};
+
+__device__ __forceinline__ int64_t query_position(const BiasArgs& a, uint64_t i) {
+  return a.pos ? (int64_t)a.pos[i] : a.first + (int64_t)i;
+}
+
+// Bucket of the distance d = key - query; `start` is in shared memory.
+__device__ __forceinline__ int bucket_of(const Buckets& t, const int* start, int64_t d) {
+  int base = 0;
+  int64_t n64 = -d;
+  if (t.both) {
+    if (d > 0) {
+      base = t.half;
+      n64 = d;
+    }
+  } else if (n64 < 0) {
+    n64 = 0;
+  }
+  if (n64 >= t.last) return base + t.half - 1;
+  const int n = (int)n64;
+  int lo = 0, hi = t.half;  // start[lo] <= n < start[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start[mid] <= n) lo = mid;
+    else hi = mid;
+  }
+  return base + lo;
+}
+
+template <class T> __device__ __forceinline__ T minus_infinity();
+template <> __device__ __forceinline__ float minus_infinity<float>() { return -INFINITY; }
+template <> __device__ __forceinline__ double minus_infinity<double>() { return -(double)INFINITY; }
+template <> __device__ __forceinline__ __half minus_infinity<__half>() { return __ushort_as_half(0xFC00); }
+template <> __device__ __forceinline__ __nv_bfloat16 minus_infinity<__nv_bfloat16>() {
+  return __ushort_as_bfloat16(0xFF80);
+}
+
+// The table's value in the bias's type: the same bits, or one rounding to
+// nearest from a f32 table.
+template <class T, class S> __device__ __forceinline__ T cast(S v) { return v; }
+template <> __device__ __forceinline__ __half cast<__half, float>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 cast<__nv_bfloat16, float>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+template <class T> struct alignas(16) Vec {
+  static constexpr int N = 16 / sizeof(T);
+  T e[N];
+};
+
+// Whether a vector of N distances from d0 on lies in one bucket (then
+// *which), the masked ones counting as bucket nb (the table's -inf row).
+template <int N>
+__device__ __forceinline__ bool one_bucket(const Buckets& t, const int* start, int nb, int64_t d0, int* which) {
+  if (t.causal && d0 > 0) {
+    *which = nb;
+    return true;
+  }
+  const int a = bucket_of(t, start, d0);
+  *which = a;
+  if (N == 1) return true;
+  const int64_t d1 = d0 + N - 1;
+  if (t.causal && d1 > 0) return false;
+  // The two directions are two runs of buckets: a vector that crosses
+  // distance 0 is never one bucket, unless each direction has only one and
+  // only the query side counts.
+  if (t.both && d0 <= 0 && d1 > 0) return false;
+  return a == bucket_of(t, start, d1);
+}
+
+__device__ __forceinline__ int bucket_or_masked(const Buckets& t, const int* start, int nb, int64_t d) {
+  return t.causal && d > 0 ? nb : bucket_of(t, start, d);
+}
+
+// ---------------------------------------------------------------- bias
+
+constexpr int kFwdThreads = 256;
+
+// A thread owns one 16-byte vector of a row and writes it for `hc` heads.
+// Rows need not be aligned: vectors sit on 16-byte addresses, the ones at a
+// row's ends are written element by element.
+template <class T, class S>
+__global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
+                                                           const __grid_constant__ BiasArgs a,
+                                                           const S* __restrict__ table, T* __restrict__ out, int hc,
+                                                           uint64_t vecs, uint64_t items) {
+  constexpr int N = Vec<T>::N;
+  extern __shared__ __align__(16) uint8_t smem[];
+  T* tab = (T*)smem;                       // [hc][nb + 1]
+  const int pitch = a.nb + 1;
+  int* start = (int*)(smem + (((size_t)hc * pitch * sizeof(T) + 15) & ~(size_t)15));
+  const int h0 = blockIdx.y * hc;
+  const int hn = min(hc, a.heads - h0);
+  for (int i = threadIdx.x; i < t.half; i += kFwdThreads) start[i] = t.start[i];
+  for (int i = threadIdx.x; i < a.nb * hn; i += kFwdThreads) {
+    const int v = i / hn, h = i - v * hn;
+    tab[h * pitch + v] = cast<T, S>(table[(size_t)v * a.heads + h0 + h]);
+  }
+  for (int h = threadIdx.x; h < hn; h += kFwdThreads) tab[h * pitch + a.nb] = minus_infinity<T>();
+  __syncthreads();
+
+  for (uint64_t item = (uint64_t)blockIdx.x * kFwdThreads + threadIdx.x; item < items;
+       item += (uint64_t)gridDim.x * kFwdThreads) {
+    uint64_t row, v;
+    if (items < (1ull << 32)) {
+      row = (uint32_t)item / (uint32_t)vecs;
+      v = (uint32_t)item - (uint32_t)row * (uint32_t)vecs;
+    } else {
+      row = item / vecs;
+      v = item - row * vecs;
+    }
+    const int64_t q = query_position(a, row);
+    int shift = -1;          // elements of the row before its first 16-byte boundary's vector
+    int which[N];
+    bool one = false;
+    int64_t c0 = 0;
+    for (int h = 0; h < hn; h++) {
+      T* line = out + (int64_t)(h0 + h) * a.hs + (int64_t)row * a.rs;
+      const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
+      if (s != shift) {      // the first head, or rows of another alignment
+        shift = s;
+        c0 = (int64_t)v * N - s;
+        one = one_bucket<N>(t, start, a.nb, c0 - q, &which[0]);
+        if (!one) {
+#pragma unroll
+          for (int k = 0; k < N; k++) which[k] = bucket_or_masked(t, start, a.nb, c0 + k - q);
+        }
+      }
+      if (c0 >= (int64_t)a.keys) continue;
+      const T* ht = tab + h * pitch;
+      Vec<T> x;
+      if (one) {
+        const T e = ht[which[0]];
+#pragma unroll
+        for (int k = 0; k < N; k++) x.e[k] = e;
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) x.e[k] = ht[which[k]];
+      }
+      if (c0 >= 0 && c0 + N <= (int64_t)a.keys) {
+        *(uint4*)(line + c0) = *(const uint4*)&x;
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; k++)
+          if (c0 + k >= 0 && c0 + k < (int64_t)a.keys) line[c0 + k] = x.e[k];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ gradient
+
+template <class T> struct AccOf { using type = float; };
+template <> struct AccOf<double> { using type = double; };
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ double widen(double x) { return x; }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+constexpr int kRows = 4;            // rows of a warp's tile
+constexpr uint64_t kBatchTile = 8;  // batch entries of a tile
+constexpr size_t kAccBytes = 64 << 10;
+
+// How the gradient is split: `splits` CTAs per head, each with `warps`
+// warps, every warp taking tiles (kRows rows x 32 vectors x kBatchTile batch
+// entries) in turn.  Fixed by the sizes alone, so sums keep their order.
+struct GradPlan {
+  int warps, splits;
+  uint64_t vecs, tiles_v, tiles_r, tiles_b;
+};
+
+GradPlan grad_plan(const dcf_bias_desc& d) {
+  GradPlan p;
+  const size_t es = dtype_size((int)d.dtype), acc = d.dtype == DCF_F64 ? 8 : 4;
+  const uint64_t n = 16 / es;
+  p.warps = (int)(kAccBytes / (d.num_buckets * 32 * acc));
+  p.warps = p.warps > 8 ? 8 : p.warps < 1 ? 1 : p.warps;
+  p.vecs = d.keys ? (d.keys + 2 * n - 2) / n : 0;
+  p.tiles_v = (p.vecs + 31) / 32;
+  p.tiles_r = (d.queries + kRows - 1) / kRows;
+  p.tiles_b = (d.batch + kBatchTile - 1) / kBatchTile;
+  const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
+  const uint64_t most = (tiles + p.warps - 1) / p.warps;
+  uint64_t want = d.heads ? (uint64_t)(kSms * 4 + d.heads - 1) / d.heads : 1;
+  if (want > most) want = most;
+  p.splits = (int)(want < 1 ? 1 : want);
+  return p;
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) bias_grad_kernel(const __grid_constant__ Buckets t,
+                                                        const __grid_constant__ BiasArgs a, const T* __restrict__ g,
+                                                        const __grid_constant__ GradPlan p,
+                                                        typename AccOf<T>::type* __restrict__ part,
+                                                        typename AccOf<T>::type* __restrict__ dtable, int add) {
+  using A = typename AccOf<T>::type;
+  constexpr int N = Vec<T>::N;
+  extern __shared__ __align__(16) uint8_t smem[];
+  A* acc = (A*)smem;   // [warp][bucket][lane]: every lane adds into its own column, in its own order
+  __shared__ int start[kMaxB];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int threads = p.warps * 32;
+  for (int i = threadIdx.x; i < t.half; i += threads) start[i] = t.start[i];
+  for (int i = threadIdx.x; i < p.warps * a.nb * 32; i += threads) acc[i] = 0;
+  __syncthreads();
+  A* mine = acc + (size_t)warp * a.nb * 32 + lane;
+
+  const int h = blockIdx.y;
+  const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
+  int cur = 0;        // the bucket that `sum` belongs to
+  A sum = 0;
+  auto into = [&](int v, A x) {
+    if (v != cur) {
+      mine[cur * 32] += sum;
+      cur = v;
+      sum = 0;
+    }
+    sum += x;
+  };
+  for (uint64_t tile = (uint64_t)blockIdx.x * p.warps + warp; tile < tiles; tile += (uint64_t)gridDim.x * p.warps) {
+    const uint64_t tv = tile % p.tiles_v, rest = tile / p.tiles_v;
+    const uint64_t r0 = (rest % p.tiles_r) * kRows, b0 = (rest / p.tiles_r) * kBatchTile;
+    const uint64_t v = tv * 32 + lane;
+    const uint64_t b1 = min(a.batch, b0 + kBatchTile);
+    for (uint64_t b = b0; b < b1; b++) {
+      const T* head = g + (int64_t)b * a.bs + (int64_t)h * a.hs;
+      Vec<T> x[kRows];
+      int64_t c0[kRows], q[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; r++) {
+        const uint64_t row = r0 + r;
+        c0[r] = (int64_t)a.keys;
+        q[r] = 0;
+        if (row < a.queries) {
+          q[r] = query_position(a, row);
+          const T* line = head + (int64_t)row * a.rs;
+          const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
+          int64_t c = (int64_t)v * N - s;
+          // A vector whose keys all come after the query is not read.
+          if (t.causal && max(c, (int64_t)0) > q[r]) c = (int64_t)a.keys;
+          c0[r] = c;
+          if (c >= 0 && c + N <= (int64_t)a.keys) {
+            *(uint4*)&x[r] = __ldg((const uint4*)(line + c));
+          } else {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+              if (c + k >= 0 && c + k < (int64_t)a.keys) x[r].e[k] = line[c + k];
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; r++) {
+        if (c0[r] >= (int64_t)a.keys) continue;
+        const int64_t d0 = c0[r] - q[r];
+        int which;
+        const bool whole = c0[r] >= 0 && c0[r] + N <= (int64_t)a.keys;
+        if (whole && one_bucket<N>(t, start, a.nb, d0, &which)) {
+          A s[N];
+#pragma unroll
+          for (int k = 0; k < N; k++) s[k] = widen(x[r].e[k]);
+#pragma unroll
+          for (int w = N / 2; w > 0; w >>= 1)
+#pragma unroll
+            for (int k = 0; k < w; k++) s[k] += s[k + w];
+          into(which, s[0]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k++) {
+            const int64_t c = c0[r] + k;
+            if (c < 0 || c >= (int64_t)a.keys || (t.causal && d0 + k > 0)) continue;
+            into(bucket_of(t, start, d0 + k), widen(x[r].e[k]));
+          }
+        }
+      }
+    }
+  }
+  mine[cur * 32] += sum;
+  __syncthreads();
+  for (int v = warp; v < a.nb; v += p.warps) {
+    A s = 0;
+    for (int w = 0; w < p.warps; w++) s += acc[((size_t)w * a.nb + v) * 32 + lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    if (lane == 0) {
+      if (gridDim.x == 1) {
+        A* d = dtable + (size_t)v * a.heads + h;
+        *d = add ? *d + s : s;
+      } else {
+        part[((size_t)h * gridDim.x + blockIdx.x) * a.nb + v] = s;
+      }
+    }
+  }
+}
+
+// One warp per table entry adds the splits' parts, always in the same order.
+template <class A>
+__global__ void __launch_bounds__(256) bias_grad_join_kernel(const A* __restrict__ part, int splits, int nb, int heads,
+                                                             A* __restrict__ dtable, int add) {
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= nb * heads) return;
+  const int h = e / nb, v = e - h * nb;
+  A s = 0;
+  for (int k = lane; k < splits; k += 32) s += part[((size_t)h * splits + k) * nb + v];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  if (lane == 0) {
+    A* d = dtable + (size_t)v * heads + h;
+    *d = add ? *d + s : s;
+  }
+}
+
+// -------------------------------------------------------------- host
+
+// A non-negative whole number of up to 31 * DCF_BIAS_MAX_BUCKETS bits.
+struct Big {
+  uint32_t w[kMaxB + 4];
+  int n = 1;
+  Big() { w[0] = 1; }
+  void times(uint32_t f) {
+    uint64_t carry = 0;
+    for (int i = 0; i < n; i++) {
+      carry += (uint64_t)w[i] * f;
+      w[i] = (uint32_t)carry;
+      carry >>= 32;
+    }
+    if (carry) w[n++] = (uint32_t)carry;
+  }
+  bool at_least(const Big& o) const {
+    if (n != o.n) return n > o.n;
+    for (int i = n - 1; i >= 0; i--)
+      if (w[i] != o.w[i]) return w[i] > o.w[i];
+    return true;
+  }
+};
+
+// The first distance of each of `half` buckets.  Bucket e + k (k >= 1)
+// begins at the smallest n with n^m >= last^k e^(m - k), m = half - e: at
+// x = e (last / e)^(k / m), rounded up.  x in 64 bits is off by some 1e-14 of
+// itself (an exponential of a product below 22), so unless a whole number
+// lies within 1e-13 of it the integers need not be asked.
+void bias_starts(int half, uint32_t last, int* start) {
+  const int e = half / 2, m = half - e;
+  for (int v = 0; v <= e && v < half; v++) start[v] = v;
+  for (int k = 1; k < m; k++) {
+    const double x = e * exp((double)k / m * log((double)last / e));
+    const double near = floor(x * (1 + 1e-13));
+    uint32_t n = (uint32_t)floor(x) + 1;
+    if (near != floor(x * (1 - 1e-13))) {
+      Big l, r;
+      n = (uint32_t)near;
+      for (int i = 0; i < m; i++) l.times(n);
+      for (int i = 0; i < k; i++) r.times(last);
+      for (int i = k; i < m; i++) r.times((uint32_t)e);
+      if (!l.at_least(r)) n++;
+    }
+    start[e + k] = (int)n;
+  }
+}
+
+Buckets buckets_of(const dcf_bias_desc& d) {
+  Buckets t;
+  t.both = (d.flags & DCF_BIAS_BIDIRECTIONAL) != 0;
+  t.causal = (d.flags & DCF_BIAS_CAUSAL) != 0;
+  t.half = (int)(t.both ? d.num_buckets / 2 : d.num_buckets);
+  bias_starts(t.half, d.max_distance, t.start);
+  t.last = t.start[t.half - 1];
+  return t;
+}
+
+BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
+  BiasArgs a;
+  a.queries = d.queries;
+  a.keys = d.keys;
+  a.first = d.first_query;
+  a.rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
+  a.hs = d.head_stride ? d.head_stride : (int64_t)d.queries * a.rs;
+  a.bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * a.hs;
+  a.heads = (int)d.heads;
+  a.nb = (int)d.num_buckets;
+  a.batch = d.batch;
+  a.pos = pos;
+  return a;
+}
+
+template <class T, class S>
+int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos, void* out, cudaStream_t stream) {
+  constexpr uint64_t N = Vec<T>::N;
+  const Buckets t = buckets_of(d);
+  const BiasArgs a = args_of(d, pos);
+  const uint64_t vecs = (d.keys + 2 * N - 2) / N, items = vecs * d.queries;
+  const uint64_t blocks = (items + kFwdThreads - 1) / kFwdThreads;
+  // Heads per block: as many as share the bucket lookup without leaving SMs
+  // idle, within 16 KB of table.
+  const uint64_t room = (16 << 10) / ((d.num_buckets + 1) * sizeof(T));
+  uint64_t hc = blocks >= kSms * 8 ? d.heads : (d.heads * blocks + kSms * 8 - 1) / (kSms * 8);
+  if (hc > room) hc = room;
+  if (hc < 1) hc = 1;
+  uint64_t groups = (d.heads + hc - 1) / hc;
+  hc = (d.heads + groups - 1) / groups;
+  groups = (d.heads + hc - 1) / hc;
+  const size_t smem = ((hc * (d.num_buckets + 1) * sizeof(T) + 15) & ~(size_t)15) + (size_t)t.half * 4;
+  const dim3 grid((unsigned)(blocks < (1u << 30) ? blocks : (1u << 30)), (unsigned)groups);
+  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, vecs, items);
+  note_launch();
+  return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
+}
+
+template <class T>
+int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, void* dtable, void* ws,
+                  cudaStream_t stream) {
+  using A = typename AccOf<T>::type;
+  const Buckets t = buckets_of(d);
+  const BiasArgs a = args_of(d, pos);
+  const GradPlan p = grad_plan(d);
+  const int add = (d.flags & DCF_BIAS_ACCUMULATE) != 0;
+  const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A);
+  if (cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAccBytes) !=
+      cudaSuccess)
+    return DCF_ECUDA;
+  bias_grad_kernel<T><<<dim3((unsigned)p.splits, d.heads), p.warps * 32, smem, stream>>>(
+      t, a, (const T*)g, p, (A*)ws, (A*)dtable, add);
+  note_launch();
+  if (p.splits > 1) {
+    const unsigned entries = d.num_buckets * d.heads;
+    bias_grad_join_kernel<A><<<(entries + 7) / 8, 256, 0, stream>>>((const A*)ws, p.splits, a.nb, a.heads, (A*)dtable,
+                                                                    add);
+    note_launch();
+  }
+  return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
+}
+
+}  // namespace
+
+int bias_desc_check(const dcf_bias_desc* d, bool grad) {
+  auto bad = [](const char* m) { return record_error(DCF_EINVAL, m); };
+  if (!d) return bad("null descriptor");
+  if (d->dtype != DCF_F16 && d->dtype != DCF_BF16 && d->dtype != DCF_F32 && d->dtype != DCF_F64)
+    return bad("position bias: dtype must be f16, bf16, f32 or f64");
+  if (!grad && d->table_dtype != d->dtype &&
+      !(d->table_dtype == DCF_F32 && (d->dtype == DCF_F16 || d->dtype == DCF_BF16)))
+    return bad("position bias: table_dtype must be dtype, or f32 beside f16 / bf16");
+  if (d->flags & ~(DCF_BIAS_BIDIRECTIONAL | DCF_BIAS_CAUSAL | (grad ? DCF_BIAS_ACCUMULATE : 0u)))
+    return bad("position bias: unknown flag");
+  const uint32_t both = d->flags & DCF_BIAS_BIDIRECTIONAL;
+  if (d->num_buckets < (both ? 2u : 1u) || d->num_buckets > DCF_BIAS_MAX_BUCKETS)
+    return bad("position bias: num_buckets out of range");
+  const uint32_t half = both ? d->num_buckets / 2 : d->num_buckets;
+  if (d->max_distance <= half / 2 || d->max_distance >= 1u << 31)
+    return bad("position bias: max_distance must be above the exact buckets and below 2^31");
+  if (d->heads > 65535) return bad("position bias: at most 65535 heads");
+  const uint64_t lim = 1ull << 31;
+  if (d->queries >= lim || d->keys >= lim || (grad && d->batch >= lim))
+    return bad("position bias: queries, keys and batch must be below 2^31");
+  if (d->first_query > (1ll << 40) || d->first_query < -(1ll << 40)) return bad("position bias: first_query out of range");
+  if (d->row_stride < 0 || d->head_stride < 0 || d->batch_stride < 0) return bad("position bias: negative stride");
+  // Extents in 128 bits, so that no product of the checks wraps.
+  const __int128 rs = d->row_stride ? d->row_stride : (int64_t)d->keys;
+  const __int128 hs = d->head_stride ? d->head_stride : (__int128)d->queries * rs;
+  const __int128 bs = d->batch_stride ? d->batch_stride : (__int128)d->heads * hs;
+  const uint64_t batch = grad ? d->batch : 1;
+  if (!d->queries || !d->keys || !d->heads || !batch) return DCF_OK;
+  const __int128 span = (__int128)(d->queries - 1) * rs + (__int128)(d->heads - 1) * hs + (__int128)(batch - 1) * bs +
+                        (__int128)d->keys;
+  if (span > ((__int128)1 << 46)) return bad("position bias: tensor too large");
+  if (!grad) {
+    // Rows that overlap would be written twice.  Either dim may be the outer one.
+    const __int128 nq = d->queries, nh = d->heads, nk = d->keys;
+    const bool rows_in_heads = (nq == 1 || rs >= nk) && (nh == 1 || hs >= (nq - 1) * rs + nk);
+    const bool heads_in_rows = (nh == 1 || hs >= nk) && (nq == 1 || rs >= (nh - 1) * hs + nk);
+    if (!rows_in_heads && !heads_in_rows) return bad("position bias: strides make rows overlap");
+  }
+  return DCF_OK;
+}
+
+size_t bias_grad_workspace(const dcf_bias_desc& d) {
+  const GradPlan p = grad_plan(d);
+  const size_t acc = d.dtype == DCF_F64 ? 8 : 4;
+  const size_t bytes = p.splits > 1 ? (size_t)p.splits * d.heads * d.num_buckets * acc : 0;
+  return (bytes + 255) / 256 * 256;
+}
+
+int launch_position_bias(const dcf_bias_desc& d, const void* table, const int32_t* pos, void* out,
+                         cudaStream_t stream) {
+  const bool from32 = d.table_dtype == DCF_F32;
+  switch (d.dtype) {
+    case DCF_F16:
+      return from32 ? launch_bias_t<__half, float>(d, table, pos, out, stream)
+                    : launch_bias_t<__half, __half>(d, table, pos, out, stream);
+    case DCF_BF16:
+      return from32 ? launch_bias_t<__nv_bfloat16, float>(d, table, pos, out, stream)
+                    : launch_bias_t<__nv_bfloat16, __nv_bfloat16>(d, table, pos, out, stream);
+    case DCF_F32: return launch_bias_t<float, float>(d, table, pos, out, stream);
+    case DCF_F64: return launch_bias_t<double, double>(d, table, pos, out, stream);
+    default: return DCF_EUNSUPPORTED;
+  }
+}
+
+int launch_position_bias_grad(const dcf_bias_desc& d, const void* g, const int32_t* pos, void* dtable, void* ws,
+                              cudaStream_t stream) {
+  switch (d.dtype) {
+    case DCF_F16: return launch_grad_t<__half>(d, g, pos, dtable, ws, stream);
+    case DCF_BF16: return launch_grad_t<__nv_bfloat16>(d, g, pos, dtable, ws, stream);
+    case DCF_F32: return launch_grad_t<float>(d, g, pos, dtable, ws, stream);
+    case DCF_F64: return launch_grad_t<double>(d, g, pos, dtable, ws, stream);
+    default: return DCF_EUNSUPPORTED;
+  }
+}
+
+}  // namespace dcf

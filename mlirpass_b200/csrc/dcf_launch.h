@@ -100,6 +100,21 @@ int launch_select(size_t elem_size, const void* cond, int cond_splat, const void
                   int f_splat, uint64_t n, void* out, dcf_status* st, cudaStream_t stream);
 int launch_splat_check(const void* in, size_t elem_size, uint64_t n, dcf_status* st, cudaStream_t stream);
 
+
+// Operators on learned tensors.  The *_check functions validate a
+// descriptor (DCF_OK, or a recorded DCF_EINVAL) and need no GPU; the launches
+// take checked descriptors with at least one element.
+int bias_desc_check(const dcf_bias_desc* d, bool grad);
+size_t bias_grad_workspace(const dcf_bias_desc& d);
+int launch_position_bias(const dcf_bias_desc& d, const void* table, const int32_t* pos, void* out,
+                         cudaStream_t stream);
+int launch_position_bias_grad(const dcf_bias_desc& d, const void* g, const int32_t* pos, void* dtable, void* ws,
+                              cudaStream_t stream);
+int orth_desc_check(const dcf_orth_desc* d);
+size_t orth_workspace(const dcf_orth_desc& d);
+int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void* ws, dcf_status* st,
+                         cudaStream_t stream);
+
 // Set the per-thread text dcf_last_error() returns; returns `code`.
 int record_error(int code, const char* msg);
 

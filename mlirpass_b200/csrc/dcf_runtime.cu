@@ -24,10 +24,12 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <mutex>
 #include <string>
 #include <thread>
+#include <utility>
 #include <vector>
 
 #include "dcf_launch.h"
@@ -1159,6 +1161,231 @@ int dcf_status_read(const dcf_status* status, void* stream, dcf_result* res) {
   res->folded = h.first_fail == ~0ull;
   res->is_splat = res->folded && h.splat_word != 0;
   return DCF_OK;
+}
+
+// ------------------------------------------- operators on learned tensors
+
+}  // extern "C"
+
+namespace {
+
+// Makes the device that owns the given pointers current for one call.
+struct OnDevice {
+  int prev = -1;
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  // Every non-null pointer must be device memory of one device, aligned to
+  // `align` bytes.
+  int enter(std::initializer_list<std::pair<const void*, size_t>> ptrs) {
+    int dev = -1;
+    for (const auto& [p, align] : ptrs) {
+      if (!p) continue;
+      if ((uintptr_t)p % align) return set_err(DCF_EINVAL, "pointer %p is not aligned to %zu bytes", p, align);
+      cudaPointerAttributes at;
+      if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return set_err(DCF_EINVAL, "pointer %p is not known to CUDA", p);
+      }
+      if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+        return set_err(DCF_EINVAL, "pointer %p is not device memory", p);
+      if (dev >= 0 && at.device != dev) return set_err(DCF_EINVAL, "pointers of more than one device");
+      dev = at.device;
+    }
+    int cur = 0;
+    CK(cudaGetDevice(&cur));
+    if (cur != dev) {
+      CK(cudaSetDevice(dev));
+      prev = cur;
+    }
+    return DCF_OK;
+  }
+};
+
+int learned_launch_failed(int rc, const char* what) {
+  return set_err(rc, "%s launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+}
+
+void learned_result(dcf_result* res, bool splat) {
+  if (!res) return;
+  memset(res, 0, sizeof *res);
+  res->folded = 1;
+  res->is_splat = splat;
+  res->first_fail_index = UINT64_MAX;
+}
+
+// The splat test of a host form's result, on the device buffer it is in.
+int learned_splat(Dev& d, const void* out, size_t es, uint64_t n, cudaStream_t s, dcf_result* res) {
+  CK(cudaMemsetAsync(d.st, 0xFF, sizeof(dcf_status), s));
+  if (int rc = launch_splat_check(out, es, n, d.st, s)) return learned_launch_failed(rc, "splat");
+  dcf_status st;
+  if (int rc = read_status(d, s, &st)) return rc;
+  learned_result(res, n <= 1 || st.splat_word != 0);
+  return DCF_OK;
+}
+
+bool dense_strides(std::initializer_list<int64_t> strides) {
+  for (int64_t s : strides)
+    if (s) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dcf_position_bias(const dcf_bias_desc* desc, const void* table, const int32_t* positions, void* out,
+                      dcf_result* res) {
+  int rc = bias_desc_check(desc, false);
+  if (rc) return rc;
+  const dcf_bias_desc& q = *desc;
+  if (!dense_strides({q.row_stride, q.head_stride, q.batch_stride}))
+    return set_err(DCF_EINVAL, "position bias: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = (uint64_t)q.heads * q.queries * q.keys;
+  if (n == 0) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if (!table || !out) return set_err(DCF_EINVAL, "null buffer");
+  const size_t es = dtype_size((int)q.dtype);
+  const size_t tb = (size_t)q.num_buckets * q.heads * dtype_size((int)q.table_dtype);
+  Dev& d = *g_devs[0];
+  std::lock_guard<std::mutex> g(d.mu);
+  CK(cudaSetDevice(d.id));
+  if ((rc = ensure_big(d, 0, tb)) || (rc = ensure_big(d, 1, n * es)) || (rc = ensure_big(d, 2, q.queries * 4))) return rc;
+  cudaStream_t s = d.s[0];
+  if ((rc = h2d_full(d, d.big[0], table, tb, s))) return rc;
+  if (positions && (rc = h2d_full(d, d.big[2], positions, q.queries * 4, s))) return rc;
+  rc = launch_position_bias(q, d.big[0], positions ? (const int32_t*)d.big[2] : nullptr, d.big[1], s);
+  if (rc) return learned_launch_failed(rc, "position bias");
+  if ((rc = d2h_full(d, out, d.big[1], n * es, s))) return rc;
+  return learned_splat(d, d.big[1], es, n, s, res);
+}
+
+int dcf_position_bias_grad(const dcf_bias_desc* desc, const void* grad, const int32_t* positions, void* table_grad,
+                           dcf_result* res) {
+  int rc = bias_desc_check(desc, true);
+  if (rc) return rc;
+  const dcf_bias_desc& q = *desc;
+  if (!dense_strides({q.row_stride, q.head_stride, q.batch_stride}))
+    return set_err(DCF_EINVAL, "position bias: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = q.batch * q.heads * q.queries * q.keys, entries = (uint64_t)q.num_buckets * q.heads;
+  if (entries == 0) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if ((n && !grad) || !table_grad) return set_err(DCF_EINVAL, "null buffer");
+  const size_t es = dtype_size((int)q.dtype), as = q.dtype == DCF_F64 ? 8 : 4, ob = entries * as;
+  const size_t ws = bias_grad_workspace(q);
+  Dev& d = *g_devs[0];
+  std::lock_guard<std::mutex> g(d.mu);
+  CK(cudaSetDevice(d.id));
+  if ((rc = ensure_big(d, 0, n * es)) || (rc = ensure_big(d, 1, ob)) || (rc = ensure_big(d, 2, q.queries * 4)) ||
+      (rc = ensure_big(d, 3, ws)))
+    return rc;
+  cudaStream_t s = d.s[0];
+  if ((rc = h2d_full(d, d.big[0], grad, n * es, s))) return rc;
+  if (positions && (rc = h2d_full(d, d.big[2], positions, q.queries * 4, s))) return rc;
+  if ((q.flags & DCF_BIAS_ACCUMULATE) && (rc = h2d_full(d, d.big[1], table_grad, ob, s))) return rc;
+  rc = launch_position_bias_grad(q, d.big[0], positions ? (const int32_t*)d.big[2] : nullptr, d.big[1], d.big[3], s);
+  if (rc) return learned_launch_failed(rc, "position bias gradient");
+  if ((rc = d2h_full(d, table_grad, d.big[1], ob, s))) return rc;
+  return learned_splat(d, d.big[1], as, entries, s, res);
+}
+
+int dcf_position_bias_async(const dcf_bias_desc* desc, const void* table, const int32_t* positions, void* out,
+                            void* stream) {
+  int rc = bias_desc_check(desc, false);
+  if (rc) return rc;
+  const dcf_bias_desc& q = *desc;
+  if (!q.heads || !q.queries || !q.keys) return DCF_OK;
+  if (!table || !out) return set_err(DCF_EINVAL, "null pointer");
+  OnDevice on;
+  if ((rc = on.enter({{out, dtype_size((int)q.dtype)}, {table, dtype_size((int)q.table_dtype)}, {positions, 4}}))) return rc;
+  rc = launch_position_bias(q, table, positions, out, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "position bias") : DCF_OK;
+}
+
+int dcf_position_bias_grad_workspace(const dcf_bias_desc* desc, size_t* bytes) {
+  int rc = bias_desc_check(desc, true);
+  if (rc) return rc;
+  if (!bytes) return set_err(DCF_EINVAL, "null result");
+  *bytes = bias_grad_workspace(*desc);
+  return DCF_OK;
+}
+
+int dcf_position_bias_grad_async(const dcf_bias_desc* desc, const void* grad, const int32_t* positions,
+                                 void* table_grad, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = bias_desc_check(desc, true);
+  if (rc) return rc;
+  const dcf_bias_desc& q = *desc;
+  if (!q.heads) return DCF_OK;
+  const size_t ws = bias_grad_workspace(q);
+  if (!table_grad || (!grad && q.batch && q.queries && q.keys) || (ws && !workspace))
+    return set_err(DCF_EINVAL, "null pointer");
+  if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
+  OnDevice on;
+  if ((rc = on.enter({{table_grad, q.dtype == DCF_F64 ? 8 : 4}, {grad, dtype_size((int)q.dtype)}, {positions, 4},
+                      {ws ? workspace : nullptr, 256}})))
+    return rc;
+  rc = launch_position_bias_grad(q, grad, positions, table_grad, workspace, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "position bias gradient") : DCF_OK;
+}
+
+int dcf_orthogonalize(const dcf_orth_desc* desc, const void* in, void* out, dcf_result* res) {
+  int rc = orth_desc_check(desc);
+  if (rc) return rc;
+  const dcf_orth_desc& q = *desc;
+  if (!dense_strides({q.row_stride, q.batch_stride, q.out_row_stride, q.out_batch_stride}))
+    return set_err(DCF_EINVAL, "orthogonalize: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = q.batch * q.rows * q.cols;
+  if (n == 0) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if (!in || !out) return set_err(DCF_EINVAL, "null buffer");
+  const size_t ies = dtype_size((int)q.dtype), oes = dtype_size((int)q.out_dtype), ws = orth_workspace(q);
+  Dev& d = *g_devs[0];
+  std::lock_guard<std::mutex> g(d.mu);
+  CK(cudaSetDevice(d.id));
+  if ((rc = ensure_big(d, 0, n * ies)) || (rc = ensure_big(d, 1, n * oes)) || (rc = ensure_big(d, 2, ws))) return rc;
+  cudaStream_t s = d.s[0];
+  if ((rc = h2d_full(d, d.big[0], in, n * ies, s))) return rc;
+  CK(cudaMemsetAsync(d.st, 0xFF, sizeof(dcf_status), s));
+  if ((rc = launch_orthogonalize(q, d.big[0], d.big[1], d.big[2], d.st, s)))
+    return learned_launch_failed(rc, "orthogonalize");
+  dcf_status st;
+  if ((rc = read_status(d, s, &st))) return rc;
+  if ((rc = d2h_full(d, out, d.big[1], n * oes, s))) return rc;
+  return learned_splat(d, d.big[1], oes, n, s, res);
+}
+
+int dcf_orthogonalize_workspace(const dcf_orth_desc* desc, size_t* bytes) {
+  int rc = orth_desc_check(desc);
+  if (rc) return rc;
+  if (!bytes) return set_err(DCF_EINVAL, "null result");
+  *bytes = orth_workspace(*desc);
+  return DCF_OK;
+}
+
+int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in, void* out, void* workspace,
+                            size_t workspace_bytes, dcf_status* status, void* stream) {
+  int rc = orth_desc_check(desc);
+  if (rc) return rc;
+  const dcf_orth_desc& q = *desc;
+  if (!q.batch || !q.rows || !q.cols) return DCF_OK;
+  const size_t ws = orth_workspace(q);
+  if (!in || !out || !status || (ws && !workspace)) return set_err(DCF_EINVAL, "null pointer");
+  if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
+  OnDevice on;
+  if ((rc = on.enter({{out, dtype_size((int)q.out_dtype)}, {in, dtype_size((int)q.dtype)},
+                      {ws ? workspace : nullptr, 256}, {status, 8}})))
+    return rc;
+  rc = launch_orthogonalize(q, in, out, workspace, status, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "orthogonalize") : DCF_OK;
 }
 
 }  // extern "C"

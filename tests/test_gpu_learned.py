@@ -1,0 +1,509 @@
+"""The operators on learned tensors on the GPU against 64-bit statements."""
+import numpy as np
+import pytest
+
+import learned_oracle as lo
+
+pytestmark = pytest.mark.gpu
+
+WIDE = {"f16": np.float16, "f32": np.float32, "f64": np.float64}
+
+
+def tdtype(name):
+    import torch
+    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32, "f64": torch.float64}[name]
+
+
+def values(t) -> np.ndarray:
+    return t.double().cpu().numpy()
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, device="cuda", generator=gen, dtype=torch.float64) * scale).to(tdtype(dtype))
+
+
+# ------------------------------------------------------------------ bias
+
+
+def bias_want(table, ids, hidden):
+    want = table.T[:, ids]
+    return np.where(hidden, -np.inf, want) if hidden is not None else want
+
+
+def run_bias(dcf, table, dtype, heads, queries, keys, *, given=None, table_dtype=None, fill=7.0, **kw):
+    import torch
+    plan = dcf.position_bias_plan(dtype, heads, queries, keys, table_dtype=table_dtype, **kw)
+    flat = torch.full((plan.out_elements + 3,), fill, dtype=tdtype(dtype), device="cuda")
+    pos = torch.tensor(given, dtype=torch.int32, device="cuda") if given is not None else None
+    dcf.position_bias_async(plan, table, flat, positions=pos)
+    torch.cuda.synchronize()
+    d = plan.desc
+    row = d.row_stride or keys
+    head = d.head_stride or queries * row
+    assert (flat[plan.out_elements:] == fill).all()      # nothing behind the last row
+    return flat.as_strided((heads, queries, keys), (head, row, 1)), flat
+
+
+SIZES = [(1, 1), (1, 7), (1, 300), (2, 1), (5, 8), (9, 31), (33, 64), (64, 129), (130, 257)]
+
+
+@pytest.mark.parametrize("queries,keys", SIZES)
+@pytest.mark.parametrize("both,causal", [(True, False), (False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16", "f64"])
+def test_bias_sizes(dcf, queries, keys, both, causal, dtype):
+    heads = 3
+    table = randn((32, heads), dtype, 1)
+    first = keys - queries if causal else 0
+    got, _ = run_bias(dcf, table, dtype, heads, queries, keys, bidirectional=both, causal=causal, first_query=first)
+    q = lo.positions(queries, first)
+    ids = lo.buckets(q, keys, 32, 128, both)
+    want = bias_want(values(table), ids, lo.masked(q, keys) if causal else None)
+    assert np.array_equal(values(got), want)
+
+
+@pytest.mark.parametrize("num_buckets,max_distance,both", [
+    (1, 1, False), (2, 2, False), (2, 1, True), (3, 2, False), (4, 2, True), (5, 3, False), (7, 5, True),
+    (8, 64, True), (16, 1000, False), (32, 128, True), (32, 128, False), (33, 200, True), (64, 33, True),
+    (128, 1 << 20, False), (256, 2000, False), (256, (1 << 31) - 1, False), (255, 128, False), (32, 256, True),
+    (32, 512, False), (48, 4096, True)])
+def test_bias_every_border(dcf, num_buckets, max_distance, both):
+    """A table of its own row numbers returns the buckets themselves."""
+    import torch
+    table = torch.arange(num_buckets, dtype=torch.float32, device="cuda").reshape(-1, 1)
+    keys, mid = 5000, 2500
+    far = [mid, 0, keys - 1, -1, -(1 << 30), (1 << 31) - 1, -(1 << 31), max_distance, max_distance - mid]
+    far = [min(max(f, -(1 << 31)), (1 << 31) - 1) for f in far]
+    got, _ = run_bias(dcf, table, "f32", 1, len(far), keys, given=far, num_buckets=num_buckets,
+                      max_distance=max_distance, bidirectional=both)
+    assert np.array_equal(values(got)[0], lo.buckets(far, keys, num_buckets, max_distance, both))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f64"])
+@pytest.mark.parametrize("row,head,off", [(40, 0, 0), (37, 0, 0), (38, 5 * 38 + 3, 0), (3 * 37, 37, 0), (131, 41, 1),
+                                          (64, 1024, 5)])
+def test_bias_strides_alignments_and_what_lies_between(dcf, dtype, row, head, off):
+    import torch
+    heads, queries, keys = 3, 5, 37
+    table = randn((32, heads), dtype, 2)
+    plan = dcf.position_bias_plan(dtype, heads, queries, keys, row_stride=row, head_stride=head, bidirectional=False,
+                                  causal=True, first_query=20)
+    h = head or queries * row
+    flat = torch.full((plan.out_elements + off + 9,), 3.0, dtype=tdtype(dtype), device="cuda")
+    dcf.position_bias_async(plan, table, flat[off:])
+    got = flat[off:].as_strided((heads, queries, keys), (h, row, 1))
+    q = lo.positions(queries, 20)
+    want = bias_want(values(table), lo.buckets(q, keys, 32, 128, False), lo.masked(q, keys))
+    assert np.array_equal(values(got), want)
+    got.fill_(3.0)
+    assert (flat == 3.0).all()
+
+
+def test_bias_positions_of_their_own_and_rows_with_no_key(dcf):
+    heads, keys = 4, 100
+    given = [0, 99, 50, 50, -1, 1000, -(1 << 31), 7]
+    table = randn((32, heads), "bf16", 3)
+    got, _ = run_bias(dcf, table, "bf16", heads, len(given), keys, given=given, bidirectional=False, causal=True)
+    ids = lo.buckets(given, keys, 32, 128, False)
+    hidden = lo.masked(given, keys)
+    assert hidden[4].all() and hidden[6].all()
+    assert np.array_equal(values(got), bias_want(values(table), ids, hidden))
+
+
+def test_bias_far_first_query(dcf):
+    table = randn((32, 2), "f32", 4)
+    for first in (1 << 40, -(1 << 40), (1 << 31) + 5):
+        got, _ = run_bias(dcf, table, "f32", 2, 3, 20, first_query=first)
+        q = lo.positions(3, first)
+        assert np.array_equal(values(got), bias_want(values(table), lo.buckets(q, 20, 32, 128, True), None))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_bias_from_a_f32_table_rounds_once(dcf, dtype):
+    import torch
+    table = randn((32, 5), "f32", 5)
+    table[0, 0], table[1, 0], table[2, 1], table[3, 2] = float("nan"), float("inf"), 1e-40, 70000.0
+    got, _ = run_bias(dcf, table, dtype, 5, 40, 50, table_dtype="f32")
+    ids = torch.from_numpy(lo.buckets(lo.positions(40, 0), 50, 32, 128, True)).cuda()
+    want = table.to(tdtype(dtype))[ids].permute(2, 0, 1)
+    assert torch.equal(got.nan_to_num(123.0), want.nan_to_num(123.0))
+    assert torch.equal(got.isnan(), want.isnan())
+
+
+def test_bias_keeps_the_bits_of_a_table(dcf):
+    import torch
+    bits = torch.randint(-(1 << 15), 1 << 15, (32, 6), dtype=torch.int32, device="cuda").to(torch.int16)
+    got, _ = run_bias(dcf, bits.view(torch.bfloat16), "bf16", 6, 70, 90)
+    ids = torch.from_numpy(lo.buckets(lo.positions(70, 0), 90, 32, 128, True)).cuda()
+    assert torch.equal(got.contiguous().view(torch.int16), bits[ids].permute(2, 0, 1).contiguous())
+
+
+def test_bias_many_heads_and_buckets(dcf):
+    """More heads than one block's table holds."""
+    table = randn((256, 70), "f32", 6)
+    got, _ = run_bias(dcf, table, "f32", 70, 6, 700, num_buckets=256, max_distance=600, first_query=300)
+    ids = lo.buckets(lo.positions(6, 300), 700, 256, 600, True)
+    assert np.array_equal(values(got), bias_want(values(table), ids, None))
+
+
+def test_bias_past_32_bits_of_elements(dcf):
+    """Row offsets beyond 2^32 elements, through a stride."""
+    import torch
+    keys, row = 19, (1 << 32) + 40
+    plan = dcf.position_bias_plan("f16", 1, 2, keys, row_stride=row)
+    flat = torch.zeros(plan.out_elements, dtype=torch.float16, device="cuda")
+    table = randn((32, 1), "f16", 7)
+    dcf.position_bias_async(plan, table, flat)
+    ids = lo.buckets(lo.positions(2, 0), keys, 32, 128, True)
+    got = torch.stack([flat[:keys], flat[row:row + keys]])
+    assert np.array_equal(values(got)[None], bias_want(values(table), ids, None))
+    assert int(flat[keys:row].count_nonzero()) == 0
+
+
+# -------------------------------------------------------------- gradient
+
+
+def run_grad(dcf, g, dtype, *, given=None, out=None, **kw):
+    import torch
+    batch, heads, queries, keys = g.shape
+    strides = dict(batch_stride=g.stride(0), head_stride=g.stride(1), row_stride=g.stride(2)) if g.numel() else {}
+    plan = dcf.position_bias_plan(dtype, heads, queries, keys, batch=batch, accumulate=out is not None, **strides,
+                                  **kw)
+    wide = torch.float64 if dtype == "f64" else torch.float32
+    if out is None:
+        out = torch.full((kw.get("num_buckets", 32), heads), float("nan"), dtype=wide, device="cuda")
+    work = torch.full((dcf.position_bias_grad_workspace(plan) + 256,), 255, dtype=torch.uint8, device="cuda")
+    pos = torch.tensor(given, dtype=torch.int32, device="cuda") if given is not None else None
+    dcf.position_bias_grad_async(plan, g, out, work[:plan.workspace], positions=pos)
+    torch.cuda.synchronize()
+    assert (work[plan.workspace:] == 255).all()
+    return out
+
+
+def check_grad(got, g, dtype, ids, hidden, num_buckets=32, start=0.0):
+    batch, heads, queries, keys = g.shape
+    want, mag = lo.bias_grad(values(g), ids, num_buckets, hidden)
+    step = lo.HALF_STEP["f64" if dtype == "f64" else "f32"]
+    bound = lo.bias_grad_bound(mag + abs(start), batch, queries, keys, 16 // g.element_size(), step)
+    err = np.abs(values(got) - (want + start))
+    assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("batch,queries,keys", [(1, 1, 1), (2, 1, 9), (1, 3, 40), (3, 17, 33), (1, 64, 64),
+                                                (9, 50, 131), (2, 257, 513)])
+@pytest.mark.parametrize("both,causal", [(True, False), (False, True)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16", "f64"])
+def test_grad_sizes(dcf, batch, queries, keys, both, causal, dtype):
+    g = randn((batch, 3, queries, keys), dtype, 11)
+    first = max(0, keys - queries)
+    got = run_grad(dcf, g, dtype, bidirectional=both, causal=causal, first_query=first)
+    q = lo.positions(queries, first)
+    check_grad(got, g, dtype, lo.buckets(q, keys, 32, 128, both), lo.masked(q, keys) if causal else None)
+
+
+@pytest.mark.parametrize("num_buckets,max_distance,both", [(1, 1, False), (2, 1, True), (5, 3, False), (64, 300, True),
+                                                           (100, 300, False), (128, 70, True), (256, 400, False)])
+@pytest.mark.parametrize("dtype", ["f16", "f64"])
+def test_grad_buckets(dcf, num_buckets, max_distance, both, dtype):
+    g = randn((2, 2, 90, 210), dtype, 12)
+    got = run_grad(dcf, g, dtype, num_buckets=num_buckets, max_distance=max_distance, bidirectional=both,
+                   first_query=60)
+    ids = lo.buckets(lo.positions(90, 60), 210, num_buckets, max_distance, both)
+    check_grad(got, g, dtype, ids, None, num_buckets)
+
+
+def test_grad_does_not_read_masked_places(dcf):
+    """NaN and infinities after the query, and rows that see nothing."""
+    import torch
+    given = [5, -1, 63, 0, 200, -(1 << 31)]
+    g = randn((2, 3, len(given), 64), "bf16", 13)
+    hidden = lo.masked(given, 64)
+    g[:, :, torch.from_numpy(hidden).cuda()] = float("nan")
+    got = run_grad(dcf, g, "bf16", given=given, bidirectional=False, causal=True)
+    check_grad(got, g.nan_to_num(0.0), "bf16", lo.buckets(given, 64, 32, 128, False), hidden)
+
+
+def test_grad_passes_on_what_is_not_finite(dcf):
+    g = randn((1, 2, 20, 20), "f32", 14)
+    g[0, 1, 3, 3] = float("inf")
+    got = values(run_grad(dcf, g, "f32"))
+    assert got[0, 1] == np.inf and np.isfinite(np.delete(got.reshape(-1), 1)).all()
+
+
+@pytest.mark.parametrize("shape,strides,off", [((2, 3, 20, 45), (8000, 2000, 50, 1), 0), ((2, 3, 20, 45), (3 * 20 * 45 + 1, 45, 135, 1), 0),
+                                               ((1, 2, 30, 70), (9999, 2101, 70, 1), 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_grad_strides(dcf, shape, strides, off, dtype):
+    n = sum((s - 1) * t for s, t in zip(shape, strides)) + 1
+    flat = randn((n + off,), dtype, 15)
+    g = flat[off:].as_strided(shape, strides, off)
+    got = run_grad(dcf, g, dtype, first_query=3)
+    check_grad(got, g, dtype, lo.buckets(lo.positions(shape[2], 3), shape[3], 32, 128, True), None)
+
+
+def test_grad_accumulates_and_overwrites(dcf):
+    import torch
+    g = randn((1, 2, 300, 300), "bf16", 16)
+    ids = lo.buckets(lo.positions(300, 0), 300, 32, 128, True)
+    out = torch.full((32, 2), 5.0, device="cuda")
+    got = run_grad(dcf, g, "bf16", out=out)
+    assert got is out
+    check_grad(got, g, "bf16", ids, None, start=5.0)
+    small = g[:, :, :1, :3].contiguous()      # one split: written by the first kernel
+    out = torch.full((32, 2), 5.0, device="cuda")
+    check_grad(run_grad(dcf, small, "bf16", out=out), small, "bf16", ids[:1, :3], None, start=5.0)
+
+
+@pytest.mark.parametrize("shape", [(0, 2, 3, 4), (1, 2, 0, 4), (1, 2, 3, 0)])
+def test_grad_of_nothing_is_zero(dcf, shape):
+    import torch
+    g = torch.empty(shape, dtype=torch.float32, device="cuda")
+    assert (run_grad(dcf, g, "f32") == 0).all()
+    out = torch.full((32, 2), 2.0, device="cuda")
+    assert (run_grad(dcf, g, "f32", out=out) == 2.0).all()
+
+
+def test_grad_same_bits_every_time(dcf):
+    import torch
+    g = randn((2, 4, 500, 700), "bf16", 17)
+    first = run_grad(dcf, g, "bf16")
+    for _ in range(3):
+        assert torch.equal(run_grad(dcf, g, "bf16"), first)
+
+
+def test_grad_against_differences(dcf):
+    """d/dt sum(g * bias(t)) by differences in 64 bits: the bias is linear in
+    its table, so a difference of any width is exact up to rounding."""
+    import torch
+    heads, queries, keys = 2, 40, 55
+    g = randn((1, heads, queries, keys), "f64", 18)
+    table = randn((32, heads), "f64", 19)
+    grad = values(run_grad(dcf, g, "f64"))
+    mag = lo.bias_grad(values(g), lo.buckets(lo.positions(queries, 0), keys, 32, 128, True), 32)[1]
+    for v, h in ((0, 0), (3, 1), (8, 0), (17, 1), (24, 0)):
+        sums = []
+        for sign in (1, -1):
+            t = table.clone()
+            t[v, h] += sign
+            got, _ = run_bias(dcf, t, "f64", heads, queries, keys)
+            sums.append(float((got * g[0]).sum()))
+        scale = float((g.abs() * 5).sum()) + mag[v, h]
+        assert abs((sums[0] - sums[1]) / 2 - grad[v, h]) <= 4400 * 2 * lo.HALF_STEP["f64"] * scale
+
+
+# ---------------------------------------------------------- orthogonalize
+
+COEF = (3.4445, -4.7750, 2.0315)
+
+
+def run_orth(dcf, x, dtype, *, out=None, **kw):
+    import torch
+    batch, rows, cols = x.shape
+    plan = dcf.orthogonalize_plan(dtype, rows, cols, batch=batch, **kw)
+    if out is None:
+        out = torch.full((batch, rows, cols), float("nan"), dtype=tdtype(plan.out_dtype), device="cuda")
+    # A workspace full of NaN: what is read has been written.
+    work = torch.full((dcf.orthogonalize_workspace(plan) + 256,), 255, dtype=torch.uint8, device="cuda")
+    status = torch.empty(2, dtype=torch.int64, device="cuda")
+    dcf.status_reset(status)
+    dcf.orthogonalize_async(plan, x, out, work[:plan.workspace], status)
+    assert dcf.status_read(status).folded
+    assert (work[plan.workspace:] == 255).all()
+    return out
+
+
+def check_orth(got, x, out_dtype, coef, eps=1e-7):
+    got, x = values(got), values(x)
+    for k in range(x.shape[0]):
+        want = lo.newton_schulz(x[k], coef, eps)
+        tol = lo.orth_tolerance(x[k], coef, eps) + lo.HALF_STEP[out_dtype]
+        # fp16 results below its normal range round to half of 2^-24
+        small = 2.0 ** -25 * np.sqrt(want.size) if out_dtype == "f16" else 0.0
+        err = np.linalg.norm(got[k] - want)
+        assert err <= tol * np.linalg.norm(want) + small, (err / np.linalg.norm(want), tol)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7), (7, 1), (3, 5), (16, 16), (31, 65), (64, 64), (96, 96),
+                                       (65, 31), (127, 129), (128, 128), (129, 128), (128, 500), (200, 333), (333, 200),
+                                       (257, 257), (1, 1000), (300, 2)])
+def test_orth_sizes(dcf, rows, cols):
+    x = randn((1, rows, cols), "f32", 21)
+    check_orth(run_orth(dcf, x, "f32"), x, "f32", [COEF] * 5)
+
+
+@pytest.mark.parametrize("dtype,out_dtype", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16"), ("bf16", "f32"),
+                                             ("f16", "f32"), ("f32", "f16")])
+@pytest.mark.parametrize("rows,cols", [(40, 72), (150, 90)])
+def test_orth_types(dcf, dtype, out_dtype, rows, cols):
+    x = randn((3, rows, cols), dtype, 22)
+    check_orth(run_orth(dcf, x, dtype, out_dtype=out_dtype), x, out_dtype, [COEF] * 5)
+
+
+@pytest.mark.parametrize("steps", [0, 1, 2, 7])
+def test_orth_steps(dcf, steps):
+    for shape in ((2, 50, 80), (1, 150, 140)):
+        x = randn(shape, "f32", 23)
+        check_orth(run_orth(dcf, x, "f32", steps=steps), x, "f32", [COEF] * steps)
+
+
+def test_orth_coefficients_of_each_step(dcf):
+    coef = [(4.0, -6.0, 2.9), (3.0, -3.2, 1.2), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0)]
+    x = randn((1, 70, 180), "f32", 24)
+    check_orth(run_orth(dcf, x, "f32", steps=4, coef=coef), x, "f32", coef)
+
+
+@pytest.mark.parametrize("rows,cols", [(100, 120), (260, 200)])
+def test_orth_low_rank(dcf, rows, cols):
+    """What rounding leaves in the null space is amplified the most."""
+    import torch
+    x = randn((1, rows, 4), "f32", 25) @ randn((1, 4, cols), "f32", 26)
+    # the f32 product itself is the input: its own noise is part of it
+    check_orth(run_orth(dcf, x, "f32"), x, "f32", [COEF] * 5)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e30])
+def test_orth_scales(dcf, scale):
+    x = randn((1, 60, 50), "f32", 27, scale)
+    check_orth(run_orth(dcf, x, "f32", eps=0.0), x, "f32", [COEF] * 5, eps=0.0)
+
+
+def test_orth_zero_and_not_finite(dcf):
+    import torch
+    x = randn((4, 33, 40), "f32", 28)
+    x[0] = 0
+    x[2, 3, 3] = float("nan")
+    got = run_orth(dcf, x, "f32")
+    assert (got[0] == 0).all()
+    assert got[2].isnan().all()
+    check_orth(got[[1, 3]], x[[1, 3]], "f32", [COEF] * 5)
+
+
+@pytest.mark.parametrize("rows,cols", [(45, 61), (150, 131)])
+def test_orth_strides_and_what_lies_between(dcf, rows, cols):
+    import torch
+    for dtype in ("bf16", "f32"):
+        flat = randn((3 * 200 * 200 + 7,), dtype, 29)
+        x = flat[5:].as_strided((2, rows, cols), (rows * 183 + 11, 183, 1), 5)
+        out = torch.full((2 * 200 * 200,), 9.0, dtype=tdtype(dtype), device="cuda")
+        view = out.as_strided((2, rows, cols), (rows * 171 + 1, 171, 1), 3)
+        run_orth(dcf, x, dtype, out=view, row_stride=183, batch_stride=rows * 183 + 11, out_row_stride=171,
+                 out_batch_stride=rows * 171 + 1)
+        check_orth(view, x, dtype, [COEF] * 5)
+        view.fill_(9.0)
+        assert (out == 9.0).all()
+
+
+@pytest.mark.parametrize("steps", [0, 5])
+def test_orth_in_place(dcf, steps):
+    import torch
+    for shape in ((2, 40, 30), (1, 200, 140)):
+        x = randn(shape, "f32", 30)
+        want = run_orth(dcf, x, "f32", steps=steps)
+        run_orth(dcf, x, "f32", steps=steps, out=x)
+        assert torch.equal(x, want)
+
+
+def test_orth_same_bits_every_time_and_alone_or_in_a_batch(dcf):
+    import torch
+    for rows, cols in ((50, 60), (140, 300)):
+        x = randn((5, rows, cols), "bf16", 31)
+        first = run_orth(dcf, x, "bf16")
+        assert torch.equal(run_orth(dcf, x, "bf16"), first)
+        assert torch.equal(run_orth(dcf, x[3:4].contiguous(), "bf16"), first[3:4])
+
+
+# ------------------------------------------------------------- together
+
+
+def test_device_pointer_checks(dcf):
+    import torch
+    plan = dcf.position_bias_plan("f32", 2, 4, 8)
+    out = torch.zeros(64, device="cuda")
+    table = torch.zeros(32, 2)                     # host memory
+    with pytest.raises(dcf.DcfError):
+        dcf.position_bias_async(plan, table, out)
+    with pytest.raises(ValueError):
+        dcf.position_bias_async(plan, table.cuda(), out[1:])
+    with pytest.raises(ValueError):
+        dcf.position_bias_async(plan, table.cuda().double(), out)
+    odd = torch.zeros(300, dtype=torch.uint8, device="cuda")[1:257].view(torch.uint8)
+    with pytest.raises(dcf.DcfError):
+        dcf._check(dcf.lib().dcf_position_bias_async(plan.ref, table.cuda().data_ptr(), None, odd.data_ptr(), None))
+
+
+def test_host_forms(dcf):
+    rng = np.random.default_rng(41)
+    plan = dcf.position_bias_plan("f32", 3, 20, 30, bidirectional=False, causal=True, first_query=10, batch=2)
+    table = rng.standard_normal((32, 3)).astype(np.float32)
+    q = lo.positions(20, 10)
+    ids, hidden = lo.buckets(q, 30, 32, 128, False), lo.masked(q, 30)
+    f = dcf.position_bias(plan, table)
+    assert f.folded and not f.is_splat
+    assert np.array_equal(f.out.view(np.float32), bias_want(table, ids, hidden).astype(np.float32))
+    assert dcf.position_bias(dcf.position_bias_plan("f32", 3, 20, 30), np.full((32, 3), 2.5, np.float32)).is_splat
+    g = rng.standard_normal((2, 3, 20, 30)).astype(np.float32)
+    want, mag = lo.bias_grad(g, ids, 32, hidden)
+    got = dcf.position_bias_grad(plan, g)
+    assert (np.abs(got.out - want) <= lo.bias_grad_bound(mag, 2, 20, 30, 4, lo.U32)).all()
+    given = rng.integers(0, 30, 20).astype(np.int32)
+    f = dcf.position_bias(plan, table, positions=given)
+    assert np.array_equal(f.out.view(np.float32),
+                          bias_want(table, lo.buckets(given, 30, 32, 128, False), lo.masked(given, 30)).astype(np.float32))
+    x = rng.standard_normal((2, 30, 25)).astype(np.float32)
+    o = dcf.orthogonalize(dcf.orthogonalize_plan("f32", 30, 25, batch=2), x)
+    for k in range(2):
+        want = lo.newton_schulz(x[k], [COEF] * 5, 1e-7)
+        tol = lo.orth_tolerance(x[k], [COEF] * 5, 1e-7) + lo.U32
+        assert np.linalg.norm(o.out[k].view(np.float32) - want) <= tol * np.linalg.norm(want)
+
+
+def test_another_stream_and_captured_graph(dcf):
+    """Bias, its gradient and the orthogonalised gradient as one captured step,
+    replayed on new inputs."""
+    import torch
+    heads, queries, keys = 4, 100, 120
+    bias = dcf.position_bias_plan("f32", heads, queries, keys)
+    orth = dcf.orthogonalize_plan("f32", 32, heads)
+    table = randn((32, heads), "f32", 51)
+    g = torch.empty(1, heads, queries, keys, device="cuda")
+    dtable, step = torch.empty(32, heads, device="cuda"), torch.empty(32, heads, device="cuda")
+    out = torch.empty(heads, queries, keys, device="cuda")
+    w1 = torch.empty(dcf.position_bias_grad_workspace(bias) + 1, dtype=torch.uint8, device="cuda")
+    w2 = torch.empty(dcf.orthogonalize_workspace(orth), dtype=torch.uint8, device="cuda")
+    status = torch.empty(2, dtype=torch.int64, device="cuda")
+    dcf.status_reset(status)
+
+    def run():
+        dcf.position_bias_async(bias, table, out)
+        g.copy_(out[None] - 1.0)                # the gradient of |bias - 1|^2 / 2
+        dcf.position_bias_grad_async(bias, g, dtable, w1)
+        dcf.orthogonalize_async(orth, dtable, step, w2, status)
+        table.sub_(step, alpha=0.1)
+
+    start = table.clone()
+    eager = []
+    for _ in range(3):
+        run()
+        eager.append((table.clone(), dtable.clone(), out.clone()))
+    table.copy_(start)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(table, eager[0][0])
+    table.copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    assert torch.equal(table, start)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((table, dtable, out), eager[k]):
+            assert torch.equal(a, b)
+    assert dcf.status_read(status).folded
+    # and the step means what it says: the table's rows move against the gradient
+    ids = lo.buckets(lo.positions(queries, 0), keys, 32, 128, True)
+    check_grad(dtable, g, "f32", ids, None)

@@ -1,0 +1,177 @@
+"""Operators on learned tensors, on the CPU: descriptors that are refused,
+workspace sizes, and that a call without a GPU says so."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+import learned_oracle as lo
+import mlirpass_b200 as m
+from conftest import have_gpu
+
+
+def refused(make, *args, **kw):
+    with pytest.raises(m.DcfError) as e:
+        make(*args, **kw)
+    assert e.value.code == -1, e.value
+    return str(e.value)
+
+
+def bias(**kw):
+    base = dict(dtype="bf16", heads=4, queries=8, keys=16)
+    base.update(kw)
+    return m.position_bias_plan(base.pop("dtype"), base.pop("heads"), base.pop("queries"), base.pop("keys"), **base)
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dtype="i32"), "dtype"), (dict(dtype="f8E4M3"), "dtype"),
+    (dict(num_buckets=0), "num_buckets"), (dict(num_buckets=1), "num_buckets"), (dict(num_buckets=257), "num_buckets"),
+    (dict(max_distance=8), "max_distance"),                       # 32 buckets, 16 a side: 8 are exact
+    (dict(max_distance=16, bidirectional=False), "max_distance"),
+    (dict(heads=65536), "heads"),
+    (dict(first_query=(1 << 40) + 1), "first_query"), (dict(first_query=-(1 << 40) - 1), "first_query"),
+    (dict(row_stride=-1), "stride"), (dict(head_stride=-128), "stride"), (dict(batch_stride=-1), "stride"),
+    (dict(row_stride=1 << 45), "large"), (dict(head_stride=1 << 45), "large"),
+])
+def test_bias_plans_that_are_refused(kw, word):
+    assert word in refused(bias, **kw)
+
+
+def test_bias_calls_that_are_refused():
+    call = m.lib().dcf_position_bias_async
+
+    def rc(plan, table=256, out=256):
+        return call(plan.ref, table, None, out, None)
+
+    for kw in (dict(dtype="f32", table_dtype="bf16"), dict(dtype="f64", table_dtype="f32"),
+               dict(accumulate=True),                       # the gradient's flag
+               dict(row_stride=15), dict(head_stride=127),  # rows that overlap
+               dict(row_stride=16, head_stride=64)):
+        plan = bias(**kw)
+        assert rc(plan) == -1, kw
+    # heads inside rows is a layout, not an overlap: refused only for its pointers
+    assert rc(bias(row_stride=64, head_stride=16), table=None) == -1
+    assert b"null" in m.lib().dcf_last_error()
+    # nothing to write: no pointer is looked at
+    for kw in (dict(heads=0), dict(queries=0), dict(keys=0)):
+        assert rc(bias(**kw), None, None) == 0
+    assert call(None, 256, None, 256, None) == -1
+
+
+def test_bias_grad_workspace_and_its_checks():
+    plan = bias(heads=16, queries=1000, keys=1000)
+    assert plan.workspace > 0 and plan.workspace % 256 == 0
+    assert bias(queries=1, keys=4).workspace == 0
+    call = m.lib().dcf_position_bias_grad_async
+    assert call(plan.ref, 256, None, 256, 256, plan.workspace - 1, None) == -1
+    assert b"workspace" in m.lib().dcf_last_error()
+    assert call(plan.ref, 256, None, 256, None, plan.workspace, None) == -1
+    assert call(plan.ref, None, None, 256, 256, plan.workspace, None) == -1
+    assert call(plan.ref, 256, None, None, 256, plan.workspace, None) == -1
+    assert m.lib().dcf_position_bias_grad_workspace(plan.ref, None) == -1
+    assert m.lib().dcf_position_bias_grad_workspace(None, ctypes.byref(ctypes.c_size_t())) == -1
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(dtype="f64"), "dtype"), (dict(dtype="i8"), "dtype"), (dict(out_dtype="f64"), "dtype"),
+    (dict(rows=65537), "65536"), (dict(cols=65537), "65536"), (dict(batch=65536), "65535"),
+    (dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"), (dict(eps=math.inf), "eps"),
+    (dict(row_stride=-1), "stride"), (dict(out_row_stride=-1), "stride"), (dict(batch_stride=-1), "stride"),
+    (dict(out_row_stride=15), "overlap"), (dict(batch=2, out_batch_stride=127), "overlap"),
+    (dict(row_stride=1 << 45), "large"),
+    (dict(coef=(math.nan, 0, 0)), "coefficient"), (dict(coef=(1e5, 0, 0)), "coefficient"),
+    (dict(coef=(3.0, 0, 0)), "past 64"),                    # 3^5 = 243
+    (dict(coef=(3.4445, 4.7750, 2.0315)), "past 64"),
+    (dict(rows=65536, cols=65536, batch=65535), "tiles"),
+])
+def test_orth_plans_that_are_refused(kw, word):
+    base = dict(dtype="bf16", rows=8, cols=16)
+    base.update(kw)
+    assert word in refused(m.orthogonalize_plan, base.pop("dtype"), base.pop("rows"), base.pop("cols"), **base)
+
+
+def test_orth_bound_follows_the_interior_of_the_interval():
+    # 4 s - 4 s^3 is 0 at 0 and at 1; its largest value lies between (1.54), and grows from there
+    m.orthogonalize_plan("f32", 8, 8, steps=2, coef=(4, -4, 0))
+    assert "past 64" in refused(m.orthogonalize_plan, "f32", 8, 8, steps=4, coef=(4, -4, 0))
+    # the quintic used by default settles for any number of steps
+    m.orthogonalize_plan("f32", 8, 8, steps=16)
+    # a step of its own for each
+    m.orthogonalize_plan("f32", 8, 8, steps=3, coef=[(4, -4, 0), (1, 0, 0), (0.25, 0, 0)])
+
+
+def test_orth_calls_that_are_refused():
+    plan = m.orthogonalize_plan("f32", 40, 50)
+    assert plan.workspace > 0
+    call = m.lib().dcf_orthogonalize_async
+    assert call(plan.ref, 256, 256, 256, plan.workspace - 1, 256, None) == -1
+    for ptrs in ((None, 256, 256, 256), (256, None, 256, 256), (256, 256, None, 256), (256, 256, 256, None)):
+        i, o, w, s = ptrs
+        assert call(plan.ref, i, o, w, plan.workspace, s, None) == -1
+    bad = m.OrthDesc.from_buffer_copy(plan.desc)
+    bad.reserved = 1
+    assert call(ctypes.byref(bad), 256, 256, 256, plan.workspace, 256, None) == -1
+    bad = m.OrthDesc.from_buffer_copy(plan.desc)
+    bad.steps = 17
+    assert call(ctypes.byref(bad), 256, 256, 256, plan.workspace, 256, None) == -1
+    for kw in (dict(rows=0, cols=5), dict(rows=5, cols=0), dict(rows=5, cols=5, batch=0)):
+        empty = m.orthogonalize_plan("f32", **kw)
+        assert empty.workspace == 0
+        assert call(empty.ref, None, None, None, 0, None, None) == 0
+
+
+@pytest.mark.parametrize("args", [dict(steps=17), dict(steps=-1), dict(coef=(1, 2)), dict(coef=[(1, 2, 3)] * 4),
+                                  dict(rows=-1)])
+def test_orth_python_arguments(args):
+    base = dict(rows=8, cols=8)
+    base.update(args)
+    with pytest.raises(ValueError):
+        m.orthogonalize_plan("f32", **base)
+
+
+def test_host_forms_take_dense_tensors_of_the_right_size():
+    plan = bias(dtype="f32")
+    with pytest.raises(ValueError):
+        m.position_bias(plan, np.zeros((32, 3), np.float32))
+    with pytest.raises(ValueError):
+        m.position_bias(plan, np.zeros((32, 4), np.float32), positions=[1, 2])
+    with pytest.raises(ValueError):
+        m.position_bias_grad(plan, np.zeros(7, np.float32))
+    with pytest.raises(ValueError):
+        m.position_bias_grad(bias(dtype="f32", accumulate=True), np.zeros((1, 4, 8, 16), np.float32))
+    with pytest.raises(ValueError):
+        m.orthogonalize(m.orthogonalize_plan("f32", 4, 4), np.zeros(15, np.float32))
+    assert "dense" in refused(m.position_bias, bias(dtype="f32", row_stride=32), np.zeros((32, 4), np.float32))
+    assert "dense" in refused(m.orthogonalize, m.orthogonalize_plan("f32", 4, 4, row_stride=8),
+                              np.zeros((4, 4), np.float32))
+
+
+@pytest.mark.skipif(have_gpu(), reason="checks the no-GPU failure path")
+def test_no_cpu_fallback():
+    for call in (lambda: m.position_bias(bias(dtype="f32"), np.zeros((32, 4), np.float32)),
+                 lambda: m.position_bias_grad(bias(dtype="f32"), np.zeros((1, 4, 8, 16), np.float32)),
+                 lambda: m.orthogonalize(m.orthogonalize_plan("f32", 4, 4), np.zeros((4, 4), np.float32))):
+        with pytest.raises(m.DcfError) as e:
+            call()
+        assert e.value.code == -2
+
+
+def test_oracle_buckets_at_the_borders():
+    # 32 buckets both ways, distance 128: exact to 7, then 8 * 2^(k/2) rounded up
+    b = [lo.bucket(-n, 32, 128, True) for n in range(200)]
+    starts = [b.index(v) for v in range(16)]
+    assert starts == lo.starts(32, 128, True) == [0, 1, 2, 3, 4, 5, 6, 7, 8, 12, 16, 23, 32, 46, 64, 91]
+    assert b[127] == b[128] == b[199] == 15
+    assert lo.bucket(1, 32, 128, True) == 17 and lo.bucket(5, 32, 128, False) == 0
+    # plain floating point agrees away from the borders
+    for n in (9, 13, 25, 50, 100):
+        assert b[n] == 8 + int(math.log(n / 8) / math.log(16) * 8)
+
+
+@pytest.mark.parametrize("num_buckets,max_distance,both", [(1, 1, False), (2, 1, True), (3, 2, False), (7, 5, True),
+                                                           (33, 200, True), (64, 33, True), (32, 512, False)])
+def test_oracle_starts_and_buckets_agree(num_buckets, max_distance, both):
+    reach = max_distance + 30
+    ids = lo.buckets([reach], 2 * reach + 1, num_buckets, max_distance, both)[0]
+    assert list(ids) == [lo.bucket(d, num_buckets, max_distance, both) for d in range(-reach, reach + 1)]
