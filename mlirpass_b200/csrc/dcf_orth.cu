@@ -33,8 +33,14 @@ namespace dcf {
 
 namespace {
 
-constexpr int kBM = 128, kBK = 64;      // tile rows; k extent of a stage: one 128-byte swizzle row
-constexpr int kGemmThreads = 192;       // warp 0 loads, warp 1 multiplies, warps 2-5 write out
+constexpr int kSide = 128, kBK = 64;  // rows of an operand a CTA loads; k extent of a stage: one 128-byte swizzle row
+constexpr int kPlane = kSide * kBK * 2;  // bytes of one plane of one operand in a stage
+constexpr int kStage = 4 * kPlane;       // P hi, P lo, Q hi, Q lo
+constexpr int kOrthStages = 3;
+constexpr int kOutWarps = 8;             // warps that add up and write out
+constexpr int kGemmThreads = 64 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+constexpr int kTurn = 16 * 36;           // words of a warp's 16 x 32 turning buffer (rows of 36: no bank conflicts)
+constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kTurn * 4 + 256 + 1024;
 
 // ------------------------------------------------------- PTX wrappers
 
@@ -45,16 +51,91 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
+// The forms for one CTA and for a pair of CTAs that share one product.
+template <int CTAS> struct Tc;
 
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-               : "memory");
+template <> struct Tc<1> {
+  static __device__ __forceinline__ void alloc(uint32_t* at, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  static __device__ __forceinline__ void free(uint32_t at, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+  static __device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+  }
+  static __device__ __forceinline__ uint32_t rank() { return 0; }
+  static __device__ __forceinline__ void sync() { __syncthreads(); }
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+  }
+};
+
+template <> struct Tc<2> {
+  static __device__ __forceinline__ void alloc(uint32_t* at, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  static __device__ __forceinline__ void free(uint32_t at, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
+  }
+  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+  // Arrives on the barrier of both CTAs.
+  static __device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  }
+  static __device__ __forceinline__ uint32_t rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+  }
+  static __device__ __forceinline__ void sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  // Arrives on the first CTA's barrier, from either.
+  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n"
+        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}\n" ::"r"(smem_addr(bar))
+        : "memory");
+  }
+};
+
+// Bounded wait that also sees what the other CTA of a pair did before its
+// arrival.
+__device__ __forceinline__ bool pair_wait_bounded(uint64_t* bar, unsigned parity) {
+  for (long spins = 0; spins <= kWaitLimit; spins++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
+        "p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
@@ -102,11 +183,12 @@ enum Mode {
 };
 
 struct GemmArgs {
-  int m, n, k;            // rows, columns, length of the product
-  int tiles_m, tiles_n;   // tiles of kBM x BN
-  int tiles;              // per matrix (of the upper triangle for GRAM, POLY)
+  int m, n, k;              // rows, columns, length of the product
+  int tiles_m, tiles_n;     // tiles of 128 CTAS x 128 CTAS
+  int tiles;                // per matrix (of the upper triangle for GRAM, POLY)
+  int total;                // of the batch
   float alpha, beta, diag;  // v = alpha acc [+ beta A + diag I]
-  Planes to, to_t, from;  // results; POLY: A
+  Planes to, to_t, from;    // results; POLY: A
   void* out;
   int out_dtype, transposed;
   int64_t out_rs, out_bs;
@@ -119,184 +201,303 @@ __device__ __forceinline__ void store_typed(void* out, int64_t at, int dtype, fl
   else ((__nv_bfloat16*)out)[at] = __float2bfloat16_rn(v);
 }
 
-template <int BN, int STAGES> struct GemmSmem {
-  static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2;  // one plane of one stage
-  static constexpr int kStage = 2 * (kA + kB);
-  static constexpr int kBytes = STAGES * kStage + 1024 + (2 * STAGES + 1) * 8 + 16;
+__device__ __forceinline__ uint32_t split_word(float v) {
+  __half hi, lo;
+  split(v, hi, lo);
+  return (uint32_t)__half_as_ushort(hi) | ((uint32_t)__half_as_ushort(lo) << 16);
+}
+
+// Eight split words as eight his and eight los.
+__device__ __forceinline__ void part_words(const uint32_t (&w)[8], uint4& hi, uint4& lo) {
+  hi = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[4], w[5], 0x5410),
+                  __byte_perm(w[6], w[7], 0x5410));
+  lo = make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632), __byte_perm(w[4], w[5], 0x7632),
+                  __byte_perm(w[6], w[7], 0x7632));
+}
+
+template <int CTAS, Mode MODE> struct TileOf {
+  uint32_t z;
+  int row0, col0;
+  __device__ __forceinline__ TileOf(const GemmArgs& g, int t) {
+    constexpr int side = kSide * CTAS;
+    z = (uint32_t)(t / g.tiles);
+    int tile = t - (int)z * g.tiles, tm, tn;
+    if (MODE == GRAM || MODE == POLY) {
+      for (tm = 0; tile >= g.tiles_n - tm; tm++) tile -= g.tiles_n - tm;  // row tm keeps tm .. tiles_n - 1
+      tn = tm + tile;
+    } else {
+      tm = tile % g.tiles_m;
+      tn = tile / g.tiles_m;
+    }
+    row0 = tm * side;
+    col0 = tn * side;
+  }
 };
 
-// One kBM x BN tile of D = P Q^T per CTA, P and Q given as two fp16 planes each,
-// K-major.  A stage holds 64 columns of all four planes, which three products
-// share: hi hi, hi lo and lo hi.
-template <int BN, int STAGES, Mode MODE>
-__global__ void __launch_bounds__(kGemmThreads) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
-                                                                 const __grid_constant__ CUtensorMap map_q,
-                                                                 const __grid_constant__ GemmArgs g) {
-  using L = GemmSmem<BN, STAGES>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = (uint64_t*)(base + STAGES * L::kStage);
-  uint64_t* empty = full + STAGES;
-  uint64_t* done = empty + STAGES;
-  uint32_t* tmem_at = (uint32_t*)(done + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  const uint32_t z = blockIdx.x / (uint32_t)g.tiles;
-  int tile = (int)(blockIdx.x % (uint32_t)g.tiles);
-  int tm, tn;
-  if (MODE == GRAM || MODE == POLY) {
-    // Row tm keeps the tiles that reach the diagonal or lie right of it.
-    for (tm = 0;; tm++) {
-      const int first = tm * kBM / BN, count = g.tiles_n - first;
-      if (tile < count) {
-        tn = first + tile;
-        break;
+// Writes a warp's 32 rows x 16 columns (one row per lane, v[j] in column c0 + j).
+template <Mode MODE>
+__device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint32_t* turn,
+                                          int lane) {
+  const int r = r0 + lane;
+  if (MODE == FINAL) {
+    if (g.transposed) {  // rows are contiguous in the result
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (r < g.m && c0 + j < g.n) store_typed(g.out, (int64_t)z * g.out_bs + (int64_t)(c0 + j) * g.out_rs + r, g.out_dtype, __fmul_rn(g.alpha, v[j]));
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 16; j++) turn[j * 36 + lane] = __float_as_uint(__fmul_rn(g.alpha, v[j]));
+      __syncwarp();
+      const int c = c0 + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int rr = 2 * i + (lane >> 4);
+        if (r0 + rr < g.m && c < g.n)
+          store_typed(g.out, (int64_t)z * g.out_bs + (int64_t)(r0 + rr) * g.out_rs + c, g.out_dtype,
+                      __uint_as_float(turn[(lane & 15) * 36 + rr]));
       }
-      tile -= count;
+    }
+    return;
+  }
+  constexpr bool sym = MODE == GRAM || MODE == POLY;
+  uint32_t w[16];
+  if (MODE == POLY) {
+    // A's 16 values of this row, whole vectors: rows are padded to 64 columns
+    uint4 a[4] = {};
+    if (r < g.m) {
+      const uint4* h = (const uint4*)(g.from.row(z, 0, r) + c0);
+      const uint4* l = (const uint4*)(g.from.row(z, 1, r) + c0);
+      a[0] = h[0], a[1] = h[1], a[2] = l[0], a[3] = l[1];
+    }
+    const __half* h = (const __half*)&a[0];
+    const __half* l = (const __half*)&a[2];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      float x = __fmul_rn(g.alpha, v[j]);
+      x = __fmaf_rn(g.beta, __fadd_rn(__half2float(h[j]), __half2float(l[j])), x);
+      if (r == c0 + j) x = __fadd_rn(x, g.diag);
+      w[j] = split_word(x);
     }
   } else {
-    tm = tile % g.tiles_m;
-    tn = tile / g.tiles_m;
+#pragma unroll
+    for (int j = 0; j < 16; j++) w[j] = split_word(__fmul_rn(g.alpha, v[j]));
   }
-  const int row0 = tm * kBM, col0 = tn * BN;
+  if (r < g.m) {
+    __half* ph = g.to.row(z, 0, r) + c0;
+    __half* pl = g.to.row(z, 1, r) + c0;
+    if (!sym || c0 >= r) {
+      uint4 h, l;
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const uint32_t x[8] = {w[8 * k], w[8 * k + 1], w[8 * k + 2], w[8 * k + 3], w[8 * k + 4], w[8 * k + 5], w[8 * k + 6], w[8 * k + 7]};
+        part_words(x, h, l);
+        *(uint4*)(ph + 8 * k) = h;
+        *(uint4*)(pl + 8 * k) = l;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; j++)
+        if (c0 + j >= r) {
+          ph[j] = __ushort_as_half((unsigned short)w[j]);
+          pl[j] = __ushort_as_half((unsigned short)(w[j] >> 16));
+        }
+    }
+  }
+  // The same turned: eight rows of one column per vector.
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; j++) turn[j * 36 + lane] = w[j];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int c = c0 + i * 8 + (lane >> 2), rr = (lane & 3) * 8;
+    if (c >= g.n || r0 + rr >= g.m) continue;
+    uint32_t x[8];
+    *(uint4*)&x[0] = *(const uint4*)&turn[(i * 8 + (lane >> 2)) * 36 + rr];
+    *(uint4*)&x[4] = *(const uint4*)&turn[(i * 8 + (lane >> 2)) * 36 + rr + 4];
+    __half* ph = g.to_t.row(z, 0, c) + r0 + rr;
+    __half* pl = g.to_t.row(z, 1, c) + r0 + rr;
+    if (!sym || c >= r0 + rr + 8) {
+      uint4 h, l;
+      part_words(x, h, l);
+      *(uint4*)ph = h;
+      *(uint4*)pl = l;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (c > r0 + rr + k) {
+          ph[k] = __ushort_as_half((unsigned short)x[k]);
+          pl[k] = __ushort_as_half((unsigned short)(x[k] >> 16));
+        }
+    }
+  }
+}
+
+// D = P Q^T in square tiles of 128 CTAS, P and Q given as two fp16 planes
+// each, K-major.  Persistent CTAs (pairs of CTAs): warp 0 keeps a ring of stages
+// full, 64 columns of all four planes each, which three products share; one
+// thread issues these; eight warps add up and write out.
+//
+// The tensor core truncates as it accumulates, which shows as a bias of some
+// 2^-25 per instruction: 1e-4 over k = 8192.  So TMEM sums one stage
+// only (the two small products first, then the large one), in two buffers
+// in turn, and the eight warps add the stages in registers, rounding to
+// nearest.
+//
+// A pair works on one 256 x 256 tile: each CTA loads 128 rows of P and of Q
+// and multiplies its rows of P with all of Q, so that a stage feeds twice the
+// arithmetic.  The second CTA reports its full stages to the first, which
+// issues for both.
+template <int CTAS, Mode MODE>
+__global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
+                                                                    const __grid_constant__ CUtensorMap map_q,
+                                                                    const __grid_constant__ GemmArgs g) {
+  using T = Tc<CTAS>;
+  constexpr int kCols = kSide * CTAS, kTmem = 2 * kCols, kMine = kCols / 2;  // columns of one out warp
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint32_t* turn_all = (uint32_t*)(base + kOrthStages * kStage);
+  uint64_t* full = (uint64_t*)(turn_all + kOutWarps * kTurn);
+  uint64_t* empty = full + kOrthStages;
+  uint64_t* peer = empty + kOrthStages;   // the first CTA's: the second's stage is full
+  uint64_t* sum_full = peer + kOrthStages;
+  uint64_t* sum_empty = sum_full + 2;     // the first CTA's
+  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = T::rank();
+  const int first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
   const int blocks = (g.k + kBK - 1) / kBK;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < STAGES; s++) {
+    for (int s = 0; s < kOrthStages; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&peer[s], 1);
     }
-    mbar_init(done, 1);
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&sum_full[b], 1);
+      mbar_init(&sum_empty[b], CTAS * kOutWarps);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_at)), "r"(BN)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == 1) T::alloc(tmem_at, kTmem);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  T::sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t*)tmem_at;
 
   bool fail = false;
   if (warp == 0) {
     if (lane == 0) {
-      int issued = 0;
-      for (int i = 0; i < blocks; i++) {
-        const int s = i % STAGES;
-        if (i >= STAGES && !mbar_wait_bounded(&empty[s], (unsigned)((i / STAGES - 1) & 1))) {
-          fail = true;
-          break;
+      int64_t i = 0;  // stages so far
+      for (int t = first; t < g.total && !fail; t += step) {
+        const TileOf<CTAS, MODE> at(g, t);
+        const int row = at.row0 + (int)rank * kSide, col = at.col0 + (int)rank * kSide, z = (int)(2 * at.z);
+        for (int b = 0; b < blocks; b++, i++) {
+          const int s = (int)(i % kOrthStages);
+          if (i >= kOrthStages && !mbar_wait_bounded(&empty[s], (unsigned)((i / kOrthStages - 1) & 1))) {
+            fail = true;
+            break;
+          }
+          const uint32_t to = smem_addr(base + s * kStage);
+          mbar_expect_tx(&full[s], kStage);
+          tma_load_3d(to, &map_p, b * kBK, row, z, &full[s]);
+          tma_load_3d(to + kPlane, &map_p, b * kBK, row, z + 1, &full[s]);
+          tma_load_3d(to + 2 * kPlane, &map_q, b * kBK, col, z, &full[s]);
+          tma_load_3d(to + 3 * kPlane, &map_q, b * kBK, col, z + 1, &full[s]);
         }
-        const uint32_t at = smem_addr(base + s * L::kStage);
-        mbar_expect_tx(&full[s], L::kStage);
-        for (int p = 0; p < 2; p++) {
-          tma_load_3d(at + p * L::kA, &map_p, i * kBK, row0, (int)(2 * z + p), &full[s]);
-          for (int r = 0; r < BN; r += 128)
-            tma_load_3d(at + 2 * L::kA + p * L::kB + r * kBK * 2, &map_q, i * kBK, col0 + r, (int)(2 * z + p), &full[s]);
-        }
-        issued = i + 1;
       }
-      // Give up only with no copy of ours left in flight.
-      if (fail)
-        for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; i++)
-          mbar_wait_bounded(&full[i % STAGES], (unsigned)((i / STAGES) & 1));
+      // Leave only with no copy of ours and no arrival for us left in flight.
+      for (int64_t j = i > kOrthStages ? i - kOrthStages : 0; j < i; j++) {
+        const unsigned turn = (unsigned)((j / kOrthStages) & 1);
+        if (!mbar_wait_bounded(&full[j % kOrthStages], turn)) fail = true;
+        if (!fail && !mbar_wait_bounded(&empty[j % kOrthStages], turn)) fail = true;
+      }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-      for (int i = 0; i < blocks; i++) {
-        const int s = i % STAGES;
-        if (!mbar_wait_bounded(&full[s], (unsigned)((i / STAGES) & 1))) {
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kCols >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
+      int64_t i = 0;
+      for (int t = first; t < g.total && !fail; t += step) {
+        for (int b = 0; b < blocks; b++, i++) {
+          const int s = (int)(i % kOrthStages), d = (int)(i & 1);
+          const unsigned turn = (unsigned)((i / kOrthStages) & 1);
+          if (!mbar_wait_bounded(&full[s], turn)) {
+            fail = true;
+            break;
+          }
+          if (CTAS == 2 && rank) {
+            T::arrive_first(&peer[s]);
+            continue;
+          }
+          if ((CTAS == 2 && !pair_wait_bounded(&peer[s], turn)) ||
+              (i >= 2 && !pair_wait_bounded(&sum_empty[d], (unsigned)((i / 2 - 1) & 1)))) {
+            fail = true;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t at = smem_addr(base + s * kStage), to = tmem + d * kCols;
+          const uint64_t ph = smem_desc(at), pl = smem_desc(at + kPlane);
+          const uint64_t qh = smem_desc(at + 2 * kPlane), ql = smem_desc(at + 3 * kPlane);
+#pragma unroll
+          for (int j = 0; j < kBK / 16; j++) {  // 16 columns: 32 bytes on
+            T::mma(to, ph + 2 * j, ql + 2 * j, idesc, j != 0);
+            T::mma(to, pl + 2 * j, qh + 2 * j, idesc, 1);
+          }
+#pragma unroll
+          for (int j = 0; j < kBK / 16; j++) T::mma(to, ph + 2 * j, qh + 2 * j, idesc, 1);
+          T::commit(&empty[s]);
+          T::commit(&sum_full[d]);
+        }
+      }
+    }
+  } else {
+    const int part = warp & 3;                  // the 32 TMEM lanes this warp may read
+    const int col = (warp - 2) / 4 * kMine;     // and the half of the columns it takes
+    uint32_t* turn = turn_all + (warp - 2) * kTurn;
+    int64_t i = 0;
+    for (int t = first; t < g.total && !fail; t += step) {
+      const TileOf<CTAS, MODE> at(g, t);
+      float acc[kMine];
+#pragma unroll
+      for (int j = 0; j < kMine; j++) acc[j] = 0;
+      for (int b = 0; b < blocks; b++, i++) {
+        const int d = (int)(i & 1);
+        if (__any_sync(0xFFFFFFFFu, !pair_wait_bounded(&sum_full[d], (unsigned)((i >> 1) & 1)))) {
           fail = true;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t at = smem_addr(base + s * L::kStage);
-        const uint64_t ph = smem_desc(at), pl = smem_desc(at + L::kA);
-        const uint64_t qh = smem_desc(at + 2 * L::kA), ql = smem_desc(at + 2 * L::kA + L::kB);
 #pragma unroll
-        for (int j = 0; j < kBK / 16; j++) {  // 16 columns: 32 bytes on
-          mma_f16(tmem, ph + 2 * j, qh + 2 * j, idesc, (i | j) != 0);
-          mma_f16(tmem, ph + 2 * j, ql + 2 * j, idesc, 1);
-          mma_f16(tmem, pl + 2 * j, qh + 2 * j, idesc, 1);
+        for (int c = 0; c < kMine; c += 32) {
+          uint32_t x[32];
+          tmem_load32(tmem + ((uint32_t)(part * 32) << 16) + d * kCols + col + c, x);
+#pragma unroll
+          for (int j = 0; j < 32; j++) acc[c + j] = __fadd_rn(acc[c + j], __uint_as_float(x[j]));
         }
-        mma_commit(&empty[s]);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        if (lane == 0) T::arrive_first(&sum_empty[d]);
       }
-      mma_commit(done);
-    }
-  } else {
-    fail = __any_sync(0xFFFFFFFFu, !mbar_wait_bounded(done, 0));
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const int part = warp & 3;  // the 32 TMEM lanes this warp may read
-    const int r = row0 + part * 32 + lane;
-    for (int c = 0; c < BN && !fail; c += 32) {
-      const int c0 = col0 + c;
-      if (c0 >= g.n) break;
-      uint32_t acc[32];
-      tmem_load32(tmem + ((uint32_t)(part * 32) << 16) + c, acc);
-      if (MODE == FINAL) {
-        for (int j = 0; j < 32; j++) {
-          const int cc = c0 + j;
-          if (r < g.m && cc < g.n) {
-            const int64_t at = (int64_t)z * g.out_bs + (g.transposed ? (int64_t)cc * g.out_rs + r : (int64_t)r * g.out_rs + cc);
-            store_typed(g.out, at, g.out_dtype, __fmul_rn(g.alpha, __uint_as_float(acc[j])));
-          }
-        }
-        continue;
-      }
-      constexpr bool sym = MODE == GRAM || MODE == POLY;
-      if (sym && c0 + 31 < row0 + part * 32) continue;  // below the diagonal: written by its mirror image
-      __half hi[32], lo[32];
+      if (fail) break;
+      const int r0 = at.row0 + (int)rank * kSide + part * 32;
 #pragma unroll
-      for (int j = 0; j < 32; j++) {
-        float v = __fmul_rn(g.alpha, __uint_as_float(acc[j]));
-        if (MODE == POLY) {
-          const int cc = c0 + j;
-          if (r < g.m && cc < g.n) {
-            const float x = __fadd_rn(__half2float(g.from.row(z, 0, r)[cc]), __half2float(g.from.row(z, 1, r)[cc]));
-            v = __fmaf_rn(g.beta, x, v);
-            if (r == cc) v = __fadd_rn(v, g.diag);
-          }
-        }
-        split(v, hi[j], lo[j]);
-      }
-      if (r < g.m) {
-        __half* h = g.to.row(z, 0, r) + c0;
-        __half* l = g.to.row(z, 1, r) + c0;
-        if (!sym || c0 >= r) {  // rows are padded to 64 columns, so whole chunks fit
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            *(uint4*)(h + j) = *(const uint4*)(hi + j);
-            *(uint4*)(l + j) = *(const uint4*)(lo + j);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; j++)
-            if (c0 + j >= r) {
-              h[j] = hi[j];
-              l[j] = lo[j];
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-          const int cc = c0 + j;
-          if (cc < g.n && (!sym || cc > r)) {
-            g.to_t.row(z, 0, cc)[r] = hi[j];
-            g.to_t.row(z, 1, cc)[r] = lo[j];
-          }
-        }
+      for (int c = 0; c < kMine; c += 16) {
+        const int c0 = at.col0 + col + c;
+        // beyond the matrix, or below the diagonal: written by its mirror image
+        if (r0 >= g.m || c0 >= g.n || ((MODE == GRAM || MODE == POLY) && c0 + 15 < r0)) continue;
+        write_out<MODE>(g, at.z, r0, c0, acc + c, turn, lane);
       }
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   if (fail) atomicExch(&g.st->error, 1u);
   __syncthreads();
+  T::sync();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN) : "memory");
+    T::free(tmem, kTmem);
   }
 }
 
@@ -455,6 +656,7 @@ int scale_of(double bound) {
 }
 
 constexpr double kMostSingular = 64;
+constexpr int kPairRows = 1536;
 
 struct Layout {
   Planes x, xt[2], a, b;
@@ -493,22 +695,35 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
   return l;
 }
 
-template <int BN, int STAGES, Mode MODE>
-int gemm(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
-  using L = GemmSmem<BN, STAGES>;
-  g.tiles_m = (g.m + kBM - 1) / kBM;
-  g.tiles_n = (g.n + BN - 1) / BN;
-  g.tiles = 0;
-  if (MODE == GRAM || MODE == POLY)
-    for (int t = 0; t < g.tiles_m; t++) g.tiles += g.tiles_n - t * kBM / BN;
-  else
-    g.tiles = g.tiles_m * g.tiles_n;
-  auto kernel = orth_gemm_kernel<BN, STAGES, MODE>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+template <int CTAS, Mode MODE>
+int gemm_with(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
+  constexpr int side = kSide * CTAS;
+  g.tiles_m = (g.m + side - 1) / side;
+  g.tiles_n = (g.n + side - 1) / side;
+  g.tiles = MODE == GRAM || MODE == POLY ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
+  g.total = (int)(g.tiles * batch);
+  auto kernel = orth_gemm_kernel<CTAS, MODE>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
     return DCF_ECUDA;
-  kernel<<<(unsigned)(g.tiles * batch), kGemmThreads, L::kBytes, s>>>(p, q, g);
+  const int most = sm_count_current() / CTAS;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((unsigned)((g.total < most ? g.total : most) * CTAS));
+  c.blockDim = dim3(kGemmThreads);
+  c.dynamicSmemBytes = kGemmSmem;
+  c.stream = s;
+  cudaLaunchAttribute a[1];
+  a[0].id = cudaLaunchAttributeClusterDimension;
+  a[0].val.clusterDim.x = CTAS;
+  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  c.attrs = a;
+  c.numAttrs = 1;
   note_launch();
-  return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
+  return cudaLaunchKernelEx(&c, kernel, p, q, g) == cudaSuccess ? DCF_OK : DCF_ECUDA;
+}
+
+template <Mode MODE>
+int gemm(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, uint64_t batch, cudaStream_t s) {
+  return g.m >= kPairRows ? gemm_with<2, MODE>(p, q, g, batch, s) : gemm_with<1, MODE>(p, q, g, batch, s);
 }
 
 }  // namespace
@@ -593,7 +808,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.k = n;
     g.alpha = (float)ldexp(1.0, sa - 2 * sx);
     g.to = g.to_t = l.a;
-    int rc = gemm<128, 3, GRAM>(mx, mx, g, d.batch, s);
+    int rc = gemm<GRAM>(mx, mx, g, d.batch, s);
     if (rc) return rc;
     g.k = m;
     g.alpha = (float)ldexp(k[2], sb - 2 * sa);
@@ -601,7 +816,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
     g.to = g.to_t = l.b;
-    if ((rc = gemm<128, 3, POLY>(ma, ma, g, d.batch, s))) return rc;
+    if ((rc = gemm<POLY>(ma, ma, g, d.batch, s))) return rc;
     const int sn = scale_of(next);
     g.n = n;
     g.beta = g.diag = 0;
@@ -609,7 +824,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
       g.alpha = (float)ldexp(1.0, sn - sb - sx);
       g.to = l.x;
       g.to_t = l.xt[(i + 1) & 1];
-      if ((rc = gemm<128, 3, APPLY>(mb, mxt[i & 1], g, d.batch, s))) return rc;
+      if ((rc = gemm<APPLY>(mb, mxt[i & 1], g, d.batch, s))) return rc;
     } else {
       g.alpha = (float)ldexp(1.0, -sb - sx);
       g.out = out;
@@ -617,7 +832,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
       g.transposed = t;
       g.out_rs = out_rs;
       g.out_bs = out_bs;
-      if ((rc = gemm<128, 3, FINAL>(mb, mxt[i & 1], g, d.batch, s))) return rc;
+      if ((rc = gemm<FINAL>(mb, mxt[i & 1], g, d.batch, s))) return rc;
     }
     bound = next;
     sx = sn;
