@@ -39,8 +39,8 @@ constexpr int kStage = 4 * kPlane;       // P hi, P lo, Q hi, Q lo
 constexpr int kOrthStages = 3;
 constexpr int kOutWarps = 8;             // warps that add up and write out
 constexpr int kGemmThreads = 64 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
-constexpr int kTurn = 16 * 36;           // words of a warp's 16 x 32 turning buffer (rows of 36: no bank conflicts)
-constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kTurn * 4 + 256 + 1024;
+constexpr int kBuffer = 4096;            // bytes through which an out warp reorders 32 rows
+constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kBuffer + 256 + 1024;
 
 // ------------------------------------------------------- PTX wrappers
 
@@ -117,26 +117,10 @@ template <> struct Tc<2> {
   static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
     asm volatile(
         "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n"
-        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}\n" ::"r"(smem_addr(bar))
+        " mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(smem_addr(bar))
         : "memory");
   }
 };
-
-// Bounded wait that also sees what the other CTA of a pair did before its
-// arrival.
-__device__ __forceinline__ bool pair_wait_bounded(uint64_t* bar, unsigned parity) {
-  for (long spins = 0; spins <= kWaitLimit; spins++) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
-        "p;\n}\n"
-        : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
@@ -151,11 +135,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// Shared-memory descriptor of a K-major operand tile with the 128-byte
-// swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+// Shared-memory descriptor of one plane of an operand with the 128-byte
+// swizzle: groups of eight 128-byte rows lie 1024 bytes apart.  A K-major
+// plane has a row of 64 k for each of 128 rows of the operand; one whose rows
+// run along the operand (MN) has two blocks of 64 of these, 8192 bytes apart,
+// with a row for each of 64 k.
+template <bool MN> __device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((MN ? 512ull : 1ull) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
+// From one 16-k slice to the next: 32 bytes along a row, or 16 rows.
+template <bool MN> constexpr uint32_t kSlice = (MN ? 2048 : 32) >> 4;
 
 // -------------------------------------------------------------- planes
 
@@ -178,8 +167,8 @@ __device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
 enum Mode {
   GRAM,   // A = X X^T: planes, both triangles
   POLY,   // B = a I + b A + c A A: planes, both triangles
-  APPLY,  // X <- B X: planes of X and of X^T
-  FINAL   // the result, in the caller's type and orientation
+  APPLY,  // X <- B X: planes
+  FINAL   // the result, in the caller's type
 };
 
 struct GemmArgs {
@@ -188,9 +177,9 @@ struct GemmArgs {
   int tiles;                // per matrix (of the upper triangle for GRAM, POLY)
   int total;                // of the batch
   float alpha, beta, diag;  // v = alpha acc [+ beta A + diag I]
-  Planes to, to_t, from;    // results; POLY: A
+  Planes to, from;          // result; POLY: A
   void* out;
-  int out_dtype, transposed;
+  int out_dtype, vectors;   // vectors: rows of out start on 16-byte boundaries
   int64_t out_rs, out_bs;
   dcf_status* st;
 };
@@ -207,12 +196,29 @@ __device__ __forceinline__ uint32_t split_word(float v) {
   return (uint32_t)__half_as_ushort(hi) | ((uint32_t)__half_as_ushort(lo) << 16);
 }
 
-// Eight split words as eight his and eight los.
-__device__ __forceinline__ void part_words(const uint32_t (&w)[8], uint4& hi, uint4& lo) {
-  hi = make_uint4(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[2], w[3], 0x5410), __byte_perm(w[4], w[5], 0x5410),
-                  __byte_perm(w[6], w[7], 0x5410));
-  lo = make_uint4(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632), __byte_perm(w[4], w[5], 0x7632),
-                  __byte_perm(w[6], w[7], 0x7632));
+// The his (los) of eight split words.
+template <int LO> __device__ __forceinline__ uint4 plane_of(const uint32_t* w) {
+  constexpr uint32_t pick = LO ? 0x7632 : 0x5410;
+  return make_uint4(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick), __byte_perm(w[4], w[5], pick),
+                    __byte_perm(w[6], w[7], pick));
+}
+
+// A warp holds 32 rows x 64 columns with a row in each lane.  Going through
+// 4 KB of shared memory, eight lanes then take one row's 128 bytes; the
+// 16-byte chunks of a row are exchanged so that neither side has bank conflicts.
+__device__ __forceinline__ uint4& chunk(uint4* buf, int row, int k) { return buf[row * 8 + (k ^ (row & 7))]; }
+
+// Eight fp16 values to one place in a plane of a symmetric matrix: those on
+// and right of the diagonal (`row` counts along `at`'s matrix row).
+__device__ __forceinline__ void put_upper(__half* at, const uint4& v, int row, int col) {
+  if (col >= row) {
+    *(uint4*)at = v;
+  } else if (col + 7 >= row) {
+    const __half* e = (const __half*)&v;
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (col + j >= row) at[j] = e[j];
+  }
 }
 
 template <int CTAS, Mode MODE> struct TileOf {
@@ -234,108 +240,164 @@ template <int CTAS, Mode MODE> struct TileOf {
   }
 };
 
-// Writes a warp's 32 rows x 16 columns (one row per lane, v[j] in column c0 + j).
+// Writes a warp's 32 rows x 64 columns, v[j] in row r0 + lane, column c0 + j.
 template <Mode MODE>
-__device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint32_t* turn,
+__device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
                                           int lane) {
-  const int r = r0 + lane;
+  const int sub = lane >> 3, k = lane & 7;  // of a pass over four rows: row and chunk
   if (MODE == FINAL) {
-    if (g.transposed) {  // rows are contiguous in the result
+    char* out = (char*)g.out;
+    if (g.out_dtype == DCF_F32) {
 #pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (r < g.m && c0 + j < g.n) store_typed(g.out, (int64_t)z * g.out_bs + (int64_t)(c0 + j) * g.out_rs + r, g.out_dtype, __fmul_rn(g.alpha, v[j]));
+      for (int half = 0; half < 2; half++) {  // 32 columns of 4 bytes fill the buffer
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          const float* x = v + half * 32 + j * 4;
+          chunk(buf, lane, j) = make_uint4(__float_as_uint(__fmul_rn(g.alpha, x[0])), __float_as_uint(__fmul_rn(g.alpha, x[1])),
+                                           __float_as_uint(__fmul_rn(g.alpha, x[2])), __float_as_uint(__fmul_rn(g.alpha, x[3])));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int row = 4 * i + sub, c = c0 + half * 32 + k * 4;
+          const uint4 x = chunk(buf, row, k);
+          if (r0 + row >= g.m) continue;
+          float* at = (float*)out + (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
+          if (g.vectors && c + 4 <= g.n) {
+            *(uint4*)at = x;
+          } else {
+            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              if (c + j < g.n) at[j] = __uint_as_float(e[j]);
+          }
+        }
+      }
     } else {
       __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 16; j++) turn[j * 36 + lane] = __float_as_uint(__fmul_rn(g.alpha, v[j]));
-      __syncwarp();
-      const int c = c0 + (lane & 15);
+      for (int j = 0; j < 8; j++) {
+        uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int rr = 2 * i + (lane >> 4);
-        if (r0 + rr < g.m && c < g.n)
-          store_typed(g.out, (int64_t)z * g.out_bs + (int64_t)(r0 + rr) * g.out_rs + c, g.out_dtype,
-                      __uint_as_float(turn[(lane & 15) * 36 + rr]));
+        for (int e = 0; e < 4; e++) {
+          const float x = __fmul_rn(g.alpha, v[8 * j + 2 * e]), y = __fmul_rn(g.alpha, v[8 * j + 2 * e + 1]);
+          if (g.out_dtype == DCF_F16) {
+            const __half2 p = __floats2half2_rn(x, y);
+            w[e] = *(const uint32_t*)&p;
+          } else {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+            w[e] = *(const uint32_t*)&p;
+          }
+        }
+        chunk(buf, lane, j) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int row = 4 * i + sub, c = c0 + k * 8;
+        const uint4 x = chunk(buf, row, k);
+        if (r0 + row >= g.m) continue;
+        uint16_t* at = (uint16_t*)out + (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
+        if (g.vectors && c + 8 <= g.n) {
+          *(uint4*)at = x;
+        } else {
+          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 8; j++)
+            if (c + j < g.n) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
+        }
       }
     }
     return;
   }
   constexpr bool sym = MODE == GRAM || MODE == POLY;
-  uint32_t w[16];
+  uint32_t w[64];
   if (MODE == POLY) {
-    // A's 16 values of this row, whole vectors: rows are padded to 64 columns
-    uint4 a[4] = {};
-    if (r < g.m) {
-      const uint4* h = (const uint4*)(g.from.row(z, 0, r) + c0);
-      const uint4* l = (const uint4*)(g.from.row(z, 1, r) + c0);
-      a[0] = h[0], a[1] = h[1], a[2] = l[0], a[3] = l[1];
-    }
-    const __half* h = (const __half*)&a[0];
-    const __half* l = (const __half*)&a[2];
+    float x[64];
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-      float x = __fmul_rn(g.alpha, v[j]);
-      x = __fmaf_rn(g.beta, __fadd_rn(__half2float(h[j]), __half2float(l[j])), x);
-      if (r == c0 + j) x = __fadd_rn(x, g.diag);
-      w[j] = split_word(x);
+    for (int j = 0; j < 64; j++) x[j] = __fmul_rn(g.alpha, v[j]);
+#pragma unroll
+    for (int plane = 0; plane < 2; plane++) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int row = 4 * i + sub;
+        if (r0 + row < g.m) chunk(buf, row, k) = *(const uint4*)(g.from.row(z, plane, r0 + row) + c0 + 8 * k);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const uint4 a = chunk(buf, lane, i);
+        const __half2* h = (const __half2*)&a;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 f = __half22float2(h[j]);
+          x[8 * i + 2 * j] = __fmaf_rn(g.beta, f.x, x[8 * i + 2 * j]);
+          x[8 * i + 2 * j + 1] = __fmaf_rn(g.beta, f.y, x[8 * i + 2 * j + 1]);
+        }
+      }
     }
+#pragma unroll
+    for (int j = 0; j < 64; j++) w[j] = split_word(c0 + j == r0 + lane ? __fadd_rn(x[j], g.diag) : x[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; j++) w[j] = split_word(__fmul_rn(g.alpha, v[j]));
+    for (int j = 0; j < 64; j++) w[j] = split_word(__fmul_rn(g.alpha, v[j]));
   }
-  if (r < g.m) {
-    __half* ph = g.to.row(z, 0, r) + c0;
-    __half* pl = g.to.row(z, 1, r) + c0;
-    if (!sym || c0 >= r) {
-      uint4 h, l;
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const uint32_t x[8] = {w[8 * k], w[8 * k + 1], w[8 * k + 2], w[8 * k + 3], w[8 * k + 4], w[8 * k + 5], w[8 * k + 6], w[8 * k + 7]};
-        part_words(x, h, l);
-        *(uint4*)(ph + 8 * k) = h;
-        *(uint4*)(pl + 8 * k) = l;
-      }
-    } else {
+  for (int plane = 0; plane < 2; plane++) {  // rows are padded to 64 columns: whole vectors fit
+    __syncwarp();
 #pragma unroll
-      for (int j = 0; j < 16; j++)
-        if (c0 + j >= r) {
-          ph[j] = __ushort_as_half((unsigned short)w[j]);
-          pl[j] = __ushort_as_half((unsigned short)(w[j] >> 16));
-        }
+    for (int j = 0; j < 8; j++) chunk(buf, lane, j) = plane ? plane_of<1>(w + 8 * j) : plane_of<0>(w + 8 * j);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int row = 4 * i + sub, c = c0 + k * 8;
+      const uint4 x = chunk(buf, row, k);
+      if (r0 + row >= g.m) continue;
+      __half* at = g.to.row(z, plane, r0 + row) + c;
+      if (sym) put_upper(at, x, r0 + row, c);
+      else *(uint4*)at = x;
     }
   }
-  // The same turned: eight rows of one column per vector.
-  __syncwarp();
+  if (!sym || c0 + 63 <= r0) return;
+  // The mirror image: eight rows of one column per vector, strictly below
+  // the diagonal.
+  uint32_t* turn = (uint32_t*)buf;  // [32 columns][32 rows], groups of four rows exchanged
 #pragma unroll
-  for (int j = 0; j < 16; j++) turn[j * 36 + lane] = w[j];
-  __syncwarp();
+  for (int half = 0; half < 2; half++) {
+    __syncwarp();
 #pragma unroll
-  for (int i = 0; i < 2; i++) {
-    const int c = c0 + i * 8 + (lane >> 2), rr = (lane & 3) * 8;
-    if (c >= g.n || r0 + rr >= g.m) continue;
-    uint32_t x[8];
-    *(uint4*)&x[0] = *(const uint4*)&turn[(i * 8 + (lane >> 2)) * 36 + rr];
-    *(uint4*)&x[4] = *(const uint4*)&turn[(i * 8 + (lane >> 2)) * 36 + rr + 4];
-    __half* ph = g.to_t.row(z, 0, c) + r0 + rr;
-    __half* pl = g.to_t.row(z, 1, c) + r0 + rr;
-    if (!sym || c >= r0 + rr + 8) {
-      uint4 h, l;
-      part_words(x, h, l);
-      *(uint4*)ph = h;
-      *(uint4*)pl = l;
-    } else {
+    for (int j = 0; j < 32; j++) turn[j * 32 + (((lane >> 2) ^ (j & 7)) << 2) + (lane & 3)] = w[half * 32 + j];
+    __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 8; k++)
-        if (c > r0 + rr + k) {
-          ph[k] = __ushort_as_half((unsigned short)x[k]);
-          pl[k] = __ushort_as_half((unsigned short)(x[k] >> 16));
-        }
+    for (int i = 0; i < 4; i++) {
+      const int j = i * 8 + (lane >> 2), q = (lane & 3) * 2, c = c0 + half * 32 + j, r = r0 + q * 4;
+      uint32_t x[8];
+      *(uint4*)&x[0] = *(const uint4*)&turn[j * 32 + ((q ^ (j & 7)) << 2)];
+      *(uint4*)&x[4] = *(const uint4*)&turn[j * 32 + (((q + 1) ^ (j & 7)) << 2)];
+      if (c >= g.n || r >= g.m) continue;
+      __half* hi = g.to.row(z, 0, c) + r;
+      __half* lo = g.to.row(z, 1, c) + r;
+      const uint4 h = plane_of<0>(x), l = plane_of<1>(x);
+      if (c >= r + 8) {
+        *(uint4*)hi = h;
+        *(uint4*)lo = l;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (c > r + e) {
+            hi[e] = ((const __half*)&h)[e];
+            lo[e] = ((const __half*)&l)[e];
+          }
+      }
     }
   }
 }
 
 // D = P Q^T in square tiles of 128 CTAS, P and Q given as two fp16 planes
-// each, K-major.  Persistent CTAs (pairs of CTAs): warp 0 keeps a ring of stages
+// each; P_MN, Q_MN: its memory has rows of k and runs along the operand, so
+// that no operand is ever written transposed.  Persistent CTAs (pairs of CTAs): warp 0 keeps a ring of stages
 // full, 64 columns of all four planes each, which three products share; one
 // thread issues these; eight warps add up and write out.
 //
@@ -349,7 +411,7 @@ __device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0,
 // and multiplies its rows of P with all of Q, so that a stage feeds twice the
 // arithmetic.  The second CTA reports its full stages to the first, which
 // issues for both.
-template <int CTAS, Mode MODE>
+template <int CTAS, Mode MODE, bool P_MN, bool Q_MN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
                                                                     const __grid_constant__ GemmArgs g) {
@@ -357,8 +419,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   constexpr int kCols = kSide * CTAS, kTmem = 2 * kCols, kMine = kCols / 2;  // columns of one out warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint32_t* turn_all = (uint32_t*)(base + kOrthStages * kStage);
-  uint64_t* full = (uint64_t*)(turn_all + kOutWarps * kTurn);
+  uint8_t* buffers = base + kOrthStages * kStage;
+  uint64_t* full = (uint64_t*)(buffers + kOutWarps * kBuffer);
   uint64_t* empty = full + kOrthStages;
   uint64_t* peer = empty + kOrthStages;   // the first CTA's: the second's stage is full
   uint64_t* sum_full = peer + kOrthStages;
@@ -404,10 +466,15 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
           }
           const uint32_t to = smem_addr(base + s * kStage);
           mbar_expect_tx(&full[s], kStage);
-          tma_load_3d(to, &map_p, b * kBK, row, z, &full[s]);
-          tma_load_3d(to + kPlane, &map_p, b * kBK, row, z + 1, &full[s]);
-          tma_load_3d(to + 2 * kPlane, &map_q, b * kBK, col, z, &full[s]);
-          tma_load_3d(to + 3 * kPlane, &map_q, b * kBK, col, z + 1, &full[s]);
+#pragma unroll
+          for (int half = 0; half < 2; half++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+              const uint32_t at = to + p * kPlane + half * (kPlane / 2);
+              const int r = row + half * 64, c = col + half * 64, k = b * kBK;
+              tma_load_3d(at, &map_p, P_MN ? r : k, P_MN ? k : r, z + p, &full[s]);
+              tma_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, &full[s]);
+            }
         }
       }
       // Leave only with no copy of ours and no arrival for us left in flight.
@@ -419,7 +486,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(kCols >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
+      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)P_MN << 15) | ((uint32_t)Q_MN << 16) |
+                                 ((uint32_t)(kCols >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
       int64_t i = 0;
       for (int t = first; t < g.total && !fail; t += step) {
         for (int b = 0; b < blocks; b++, i++) {
@@ -433,22 +501,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             T::arrive_first(&peer[s]);
             continue;
           }
-          if ((CTAS == 2 && !pair_wait_bounded(&peer[s], turn)) ||
-              (i >= 2 && !pair_wait_bounded(&sum_empty[d], (unsigned)((i / 2 - 1) & 1)))) {
+          if ((CTAS == 2 && !mbar_wait_bounded(&peer[s], turn)) ||
+              (i >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((i / 2 - 1) & 1)))) {
             fail = true;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint32_t at = smem_addr(base + s * kStage), to = tmem + d * kCols;
-          const uint64_t ph = smem_desc(at), pl = smem_desc(at + kPlane);
-          const uint64_t qh = smem_desc(at + 2 * kPlane), ql = smem_desc(at + 3 * kPlane);
+          const uint64_t ph = smem_desc<P_MN>(at), pl = smem_desc<P_MN>(at + kPlane);
+          const uint64_t qh = smem_desc<Q_MN>(at + 2 * kPlane), ql = smem_desc<Q_MN>(at + 3 * kPlane);
+          constexpr uint32_t ps = kSlice<P_MN>, qs = kSlice<Q_MN>;
 #pragma unroll
-          for (int j = 0; j < kBK / 16; j++) {  // 16 columns: 32 bytes on
-            T::mma(to, ph + 2 * j, ql + 2 * j, idesc, j != 0);
-            T::mma(to, pl + 2 * j, qh + 2 * j, idesc, 1);
+          for (uint32_t j = 0; j < kBK / 16; j++) {
+            T::mma(to, ph + ps * j, ql + qs * j, idesc, j != 0);
+            T::mma(to, pl + ps * j, qh + qs * j, idesc, 1);
           }
 #pragma unroll
-          for (int j = 0; j < kBK / 16; j++) T::mma(to, ph + 2 * j, qh + 2 * j, idesc, 1);
+          for (uint32_t j = 0; j < kBK / 16; j++) T::mma(to, ph + ps * j, qh + qs * j, idesc, 1);
           T::commit(&empty[s]);
           T::commit(&sum_full[d]);
         }
@@ -457,7 +526,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   } else {
     const int part = warp & 3;                  // the 32 TMEM lanes this warp may read
     const int col = (warp - 2) / 4 * kMine;     // and the half of the columns it takes
-    uint32_t* turn = turn_all + (warp - 2) * kTurn;
+    uint4* buf = (uint4*)(buffers + (warp - 2) * kBuffer);
     int64_t i = 0;
     for (int t = first; t < g.total && !fail; t += step) {
       const TileOf<CTAS, MODE> at(g, t);
@@ -466,7 +535,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
       for (int j = 0; j < kMine; j++) acc[j] = 0;
       for (int b = 0; b < blocks; b++, i++) {
         const int d = (int)(i & 1);
-        if (__any_sync(0xFFFFFFFFu, !pair_wait_bounded(&sum_full[d], (unsigned)((i >> 1) & 1)))) {
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[d], (unsigned)((i >> 1) & 1)))) {
           fail = true;
           break;
         }
@@ -484,11 +553,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
       if (fail) break;
       const int r0 = at.row0 + (int)rank * kSide + part * 32;
 #pragma unroll
-      for (int c = 0; c < kMine; c += 16) {
+      for (int c = 0; c < kMine; c += 64) {
         const int c0 = at.col0 + col + c;
         // beyond the matrix, or below the diagonal: written by its mirror image
-        if (r0 >= g.m || c0 >= g.n || ((MODE == GRAM || MODE == POLY) && c0 + 15 < r0)) continue;
-        write_out<MODE>(g, at.z, r0, c0, acc + c, turn, lane);
+        if (r0 >= g.m || c0 >= g.n || ((MODE == GRAM || MODE == POLY) && c0 + 63 < r0)) continue;
+        write_out<MODE>(g, at.z, r0, c0, acc + c, buf, lane);
       }
     }
   }
@@ -506,14 +575,38 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
 struct MatArgs {
   const void* in;
   int dtype;
-  int rows, cols;        // as the caller has them
+  int rows, cols;
   int64_t rs, bs;
+  int vectors;           // rows start on 16-byte boundaries
 };
 
-__device__ __forceinline__ float load_typed(const void* p, int dtype, int64_t at) {
-  if (dtype == DCF_F32) return ((const float*)p)[at];
-  if (dtype == DCF_F16) return __half2float(((const __half*)p)[at]);
-  return __bfloat162float(((const __nv_bfloat16*)p)[at]);
+// Eight columns of a row from column c (a multiple of 8) on, zeros behind the
+// row; with `vectors`, whole ones are read as 16-byte vectors.
+__device__ __forceinline__ void load_row8(const MatArgs& a, uint32_t z, int r, int c, float (&v)[8]) {
+  const int64_t at = (int64_t)z * a.bs + (int64_t)r * a.rs + c;
+  if (a.vectors && c + 8 <= a.cols) {
+    if (a.dtype == DCF_F32) {
+      const float4 x = *(const float4*)((const float*)a.in + at), y = *(const float4*)((const float*)a.in + at + 4);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+      const uint4 x = *(const uint4*)((const uint16_t*)a.in + at);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const unsigned short b = (unsigned short)(w[j >> 1] >> ((j & 1) * 16));
+        v[j] = a.dtype == DCF_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    v[j] = 0;
+    if (c + j >= a.cols) continue;
+    if (a.dtype == DCF_F32) v[j] = ((const float*)a.in)[at + j];
+    else if (a.dtype == DCF_F16) v[j] = __half2float(((const __half*)a.in)[at + j]);
+    else v[j] = __bfloat162float(((const __nv_bfloat16*)a.in)[at + j]);
+  }
 }
 
 constexpr int kNormThreads = 256;
@@ -521,14 +614,14 @@ constexpr int kNormThreads = 256;
 // Sums of squares in 64 bits (a f32 element's square can pass 32), one part
 // per block.
 __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_constant__ MatArgs a, double* part) {
-  const uint32_t z = blockIdx.y;
+  const uint32_t z = blockIdx.y, groups = (uint32_t)(a.cols + 7) / 8;
+  const uint64_t total = (uint64_t)groups * a.rows;
   double s = 0;
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const int64_t at = (int64_t)z * a.bs + (int64_t)r * a.rs;
-    for (int c = threadIdx.x; c < a.cols; c += kNormThreads) {
-      const double v = load_typed(a.in, a.dtype, at + c);
-      s = __fma_rn(v, v, s);
-    }
+  for (uint64_t i = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kNormThreads) {
+    float v[8];
+    load_row8(a, z, (int)(i / groups), (int)(i % groups) * 8, v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s = __fma_rn((double)v[j], (double)v[j], s);
   }
   __shared__ double sh[kNormThreads / 32];
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
@@ -540,15 +633,14 @@ __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_co
   }
 }
 
-// X = G / (norm + eps), 64 x 64 elements per block, into the planes of X and
-// of its transpose; or, with no steps to take, straight to the result.
-__global__ void __launch_bounds__(256) orth_split_kernel(const __grid_constant__ MatArgs a, const double* part,
-                                                         int parts, double eps, double scale, Planes x, Planes xt,
-                                                         int transposed, void* out, int out_dtype, int64_t out_rs,
-                                                         int64_t out_bs) {
-  __shared__ float tile[64][65];
+// X = G / (norm + eps) into its planes, or, with no steps to take, straight
+// to the result.  A thread takes eight columns of a row.
+__global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_constant__ MatArgs a, const double* part,
+                                                                  int parts, double eps, double scale, Planes x,
+                                                                  void* out, int out_dtype, int64_t out_rs,
+                                                                  int64_t out_bs) {
   __shared__ double factor;
-  const uint32_t z = blockIdx.z;
+  const uint32_t z = blockIdx.y;
   if (threadIdx.x < 32) {
     double s = 0;
     for (int i = threadIdx.x; i < parts; i += 32) s += part[(size_t)z * parts + i];
@@ -556,32 +648,24 @@ __global__ void __launch_bounds__(256) orth_split_kernel(const __grid_constant__
     if (threadIdx.x == 0) factor = scale / (sqrt(s) + eps);
   }
   __syncthreads();
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int r = r0 + i / 64, c = c0 + i % 64;
-    float v = 0;
-    if (r < a.rows && c < a.cols) {
-      v = (float)((double)load_typed(a.in, a.dtype, (int64_t)z * a.bs + (int64_t)r * a.rs + c) * factor);
-      if (out) store_typed(out, (int64_t)z * out_bs + (int64_t)r * out_rs + c, out_dtype, v);
-    }
-    tile[i / 64][i % 64] = v;
-  }
-  if (out) return;
-  __syncthreads();
-  const Planes& same = transposed ? xt : x;    // rows as the caller has them
-  const Planes& other = transposed ? x : xt;
-  for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-    const int u = i / 64, v = i % 64;
-    __half hi, lo;
-    if (r0 + u < a.rows && c0 + v < a.cols) {
-      split(tile[u][v], hi, lo);
-      same.row(z, 0, r0 + u)[c0 + v] = hi;
-      same.row(z, 1, r0 + u)[c0 + v] = lo;
-    }
-    if (c0 + u < a.cols && r0 + v < a.rows) {
-      split(tile[v][u], hi, lo);
-      other.row(z, 0, c0 + u)[r0 + v] = hi;
-      other.row(z, 1, c0 + u)[r0 + v] = lo;
+  const double f = factor;
+  const uint32_t groups = (uint32_t)(a.cols + 7) / 8;
+  const uint64_t total = (uint64_t)groups * a.rows;
+  for (uint64_t i = (uint64_t)blockIdx.x * kNormThreads + threadIdx.x; i < total; i += (uint64_t)gridDim.x * kNormThreads) {
+    const int r = (int)(i / groups), c = (int)(i % groups) * 8;
+    float v[8];
+    load_row8(a, z, r, c, v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = (float)((double)v[j] * f);
+    if (out) {
+      for (int j = 0; j < 8 && c + j < a.cols; j++)
+        store_typed(out, (int64_t)z * out_bs + (int64_t)r * out_rs + c + j, out_dtype, v[j]);
+    } else {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) w[j] = split_word(v[j]);
+      *(uint4*)(x.row(z, 0, r) + c) = plane_of<0>(w);  // rows are padded to 64 columns
+      *(uint4*)(x.row(z, 1, r) + c) = plane_of<1>(w);
     }
   }
 }
@@ -606,12 +690,12 @@ EncodeTiled encoder() {
   return fn;
 }
 
-// Boxes of 64 columns x 128 rows of one plane; what lies beyond the matrix
+// Boxes of 64 columns x 64 rows of one plane; what lies beyond the matrix
 // reads as zero.
 bool encode(CUtensorMap* map, const Planes& x, int cols, uint64_t batch) {
   const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)x.rows, 2 * batch};
   const cuuint64_t strides[2] = {(cuuint64_t)x.ld * 2, (cuuint64_t)x.ld * 2 * (cuuint64_t)x.rows};
-  const cuuint32_t box[3] = {kBK, 128, 1};
+  const cuuint32_t box[3] = {64, 64, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.p, dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -658,8 +742,15 @@ int scale_of(double bound) {
 constexpr double kMostSingular = 64;
 constexpr int kPairRows = 1536;
 
+// Blocks of the norm's sum: 32 KB of a f32 matrix each, 256 at most.
+int norm_parts(const dcf_orth_desc& d) {
+  const uint64_t p = (d.rows * d.cols + 8191) / 8192;
+  return (int)(p < 256 ? p : 256);
+}
+
+// The workspace: X twice (a step reads one and writes the other), A, B.
 struct Layout {
-  Planes x, xt[2], a, b;
+  Planes x[2], a, b;
   double* part;
   int parts;
   size_t bytes;
@@ -667,8 +758,7 @@ struct Layout {
 
 Layout layout_of(const dcf_orth_desc& d, void* ws) {
   Layout l;
-  const bool t = d.rows > d.cols;
-  const int m = (int)(t ? d.cols : d.rows), n = (int)(t ? d.rows : d.cols);
+  const int m = (int)(d.rows < d.cols ? d.rows : d.cols);
   uint8_t* at = (uint8_t*)ws;
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -680,29 +770,27 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
     const int ld = round64((uint64_t)cols);
     return Planes{(__half*)take((size_t)d.batch * 2 * rows * ld * 2), rows, ld};
   };
-  l.parts = (int)(d.rows < 256 ? d.rows : 256);
+  l.parts = norm_parts(d);
   l.part = (double*)take(d.batch * l.parts * 8);
+  l.x[0] = l.x[1] = l.a = l.b = Planes{nullptr, 0, 0};
   if (d.steps) {
-    l.x = planes(m, n);
-    l.xt[0] = planes(n, m);
-    l.xt[1] = planes(n, m);
+    l.x[0] = planes((int)d.rows, (int)d.cols);
     l.a = planes(m, m);
     l.b = planes(m, m);
-  } else {
-    l.x = l.xt[0] = l.xt[1] = l.a = l.b = Planes{nullptr, 0, 0};
   }
+  if (d.steps > 1) l.x[1] = planes((int)d.rows, (int)d.cols);
   l.bytes = off;
   return l;
 }
 
-template <int CTAS, Mode MODE>
+template <int CTAS, Mode MODE, bool P_MN, bool Q_MN>
 int gemm_with(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
   constexpr int side = kSide * CTAS;
   g.tiles_m = (g.m + side - 1) / side;
   g.tiles_n = (g.n + side - 1) / side;
   g.tiles = MODE == GRAM || MODE == POLY ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
   g.total = (int)(g.tiles * batch);
-  auto kernel = orth_gemm_kernel<CTAS, MODE>;
+  auto kernel = orth_gemm_kernel<CTAS, MODE, P_MN, Q_MN>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
     return DCF_ECUDA;
   const int most = sm_count_current() / CTAS;
@@ -721,9 +809,10 @@ int gemm_with(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t b
   return cudaLaunchKernelEx(&c, kernel, p, q, g) == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
 
-template <Mode MODE>
+template <Mode MODE, bool P_MN, bool Q_MN>
 int gemm(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, uint64_t batch, cudaStream_t s) {
-  return g.m >= kPairRows ? gemm_with<2, MODE>(p, q, g, batch, s) : gemm_with<1, MODE>(p, q, g, batch, s);
+  return (g.m < g.n ? g.m : g.n) >= kPairRows ? gemm_with<2, MODE, P_MN, Q_MN>(p, q, g, batch, s)
+                                              : gemm_with<1, MODE, P_MN, Q_MN>(p, q, g, batch, s);
 }
 
 }  // namespace
@@ -770,70 +859,75 @@ size_t orth_workspace(const dcf_orth_desc& d) {
 
 int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void* ws, dcf_status* st, cudaStream_t s) {
   const Layout l = layout_of(d, ws);
-  const int t = d.rows > d.cols;
-  const int m = (int)(t ? d.cols : d.rows), n = (int)(t ? d.rows : d.cols);
+  const int rows = (int)d.rows, cols = (int)d.cols;
+  const bool tall = rows > cols;  // then the memory is X^T, and X <- B X is X^T <- X^T B
+  const int m = tall ? cols : rows, n = tall ? rows : cols;
   MatArgs a;
   a.in = in;
   a.dtype = (int)d.dtype;
-  a.rows = (int)d.rows;
-  a.cols = (int)d.cols;
+  a.rows = rows;
+  a.cols = cols;
   a.rs = d.row_stride ? d.row_stride : (int64_t)d.cols;
   a.bs = d.batch_stride ? d.batch_stride : (int64_t)d.rows * a.rs;
+  auto vectors = [](const void* p, int64_t rs, int64_t bs, size_t es) {
+    return (uintptr_t)p % 16 == 0 && (rs * es) % 16 == 0 && (bs * es) % 16 == 0;
+  };
+  a.vectors = vectors(in, a.rs, a.bs, dtype_size(a.dtype));
   const int64_t out_rs = d.out_row_stride ? d.out_row_stride : (int64_t)d.cols;
   const int64_t out_bs = d.out_batch_stride ? d.out_batch_stride : (int64_t)d.rows * out_rs;
   orth_norm_kernel<<<dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, s>>>(a, l.part);
   note_launch();
   int sx = d.steps ? scale_of(1) : 0;
-  const dim3 blocks((unsigned)((d.cols + 63) / 64), (unsigned)((d.rows + 63) / 64), (unsigned)d.batch);
-  orth_split_kernel<<<blocks, 256, 0, s>>>(a, l.part, l.parts, d.eps, ldexp(1.0, sx), l.x, l.xt[0], t,
-                                           d.steps ? nullptr : out, (int)d.out_dtype, out_rs, out_bs);
+  const uint64_t groups = (d.cols + 7) / 8 * d.rows, blocks = (groups + kNormThreads - 1) / kNormThreads;
+  orth_split_kernel<<<dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch), kNormThreads, 0, s>>>(
+      a, l.part, l.parts, d.eps, ldexp(1.0, sx), l.x[0], d.steps ? nullptr : out, (int)d.out_dtype, out_rs, out_bs);
   note_launch();
   if (cudaPeekAtLastError() != cudaSuccess) return DCF_ECUDA;
   if (!d.steps) return DCF_OK;
 
   if (!encoder()) return DCF_EUNSUPPORTED;
-  CUtensorMap mx, mxt[2], ma, mb;
-  if (!encode(&mx, l.x, n, d.batch) || !encode(&mxt[0], l.xt[0], m, d.batch) || !encode(&mxt[1], l.xt[1], m, d.batch) ||
-      !encode(&ma, l.a, m, d.batch) || !encode(&mb, l.b, m, d.batch))
+  CUtensorMap mx[2], ma, mb;
+  if (!encode(&mx[0], l.x[0], cols, d.batch) || !encode(&ma, l.a, m, d.batch) || !encode(&mb, l.b, m, d.batch) ||
+      (d.steps > 1 && !encode(&mx[1], l.x[1], cols, d.batch)))
     return DCF_ECUDA;
   double bound = 1;
   for (uint32_t i = 0; i < d.steps; i++) {
     const double* k = d.coef[i];
     double next, q;
     step_bounds(k, bound, &next, &q);
-    const int sa = scale_of(bound * bound), sb = scale_of(q);
+    const int sa = scale_of(bound * bound), sb = scale_of(q), sn = scale_of(next);
+    const CUtensorMap& x = mx[i & 1];
     GemmArgs g = {};
     g.st = st;
     g.m = g.n = m;
     g.k = n;
     g.alpha = (float)ldexp(1.0, sa - 2 * sx);
-    g.to = g.to_t = l.a;
-    int rc = gemm<GRAM>(mx, mx, g, d.batch, s);
+    g.to = l.a;
+    int rc = tall ? gemm<GRAM, true, true>(x, x, g, d.batch, s) : gemm<GRAM, false, false>(x, x, g, d.batch, s);
     if (rc) return rc;
     g.k = m;
     g.alpha = (float)ldexp(k[2], sb - 2 * sa);
     g.beta = (float)ldexp(k[1], sb - sa);
     g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
-    g.to = g.to_t = l.b;
-    if ((rc = gemm<POLY>(ma, ma, g, d.batch, s))) return rc;
-    const int sn = scale_of(next);
-    g.n = n;
-    g.beta = g.diag = 0;
+    g.to = l.b;
+    if ((rc = gemm<POLY, false, false>(ma, ma, g, d.batch, s))) return rc;
+    g.m = rows;
+    g.n = cols;
     if (i + 1 < d.steps) {
       g.alpha = (float)ldexp(1.0, sn - sb - sx);
-      g.to = l.x;
-      g.to_t = l.xt[(i + 1) & 1];
-      if ((rc = gemm<APPLY>(mb, mxt[i & 1], g, d.batch, s))) return rc;
+      g.to = l.x[(i + 1) & 1];
+      rc = tall ? gemm<APPLY, false, false>(x, mb, g, d.batch, s) : gemm<APPLY, false, true>(mb, x, g, d.batch, s);
     } else {
       g.alpha = (float)ldexp(1.0, -sb - sx);
       g.out = out;
       g.out_dtype = (int)d.out_dtype;
-      g.transposed = t;
+      g.vectors = vectors(out, out_rs, out_bs, dtype_size(g.out_dtype));
       g.out_rs = out_rs;
       g.out_bs = out_bs;
-      if ((rc = gemm<FINAL>(mb, mxt[i & 1], g, d.batch, s))) return rc;
+      rc = tall ? gemm<FINAL, false, false>(x, mb, g, d.batch, s) : gemm<FINAL, false, true>(mb, x, g, d.batch, s);
     }
+    if (rc) return rc;
     bound = next;
     sx = sn;
   }

@@ -507,3 +507,10 @@ def test_another_stream_and_captured_graph(dcf):
     # and the step means what it says: the table's rows move against the gradient
     ids = lo.buckets(lo.positions(queries, 0), keys, 32, 128, True)
     check_grad(dtable, g, "f32", ids, None)
+
+
+@pytest.mark.parametrize("rows,cols,dtype", [(1601, 1550, "f32"), (1540, 1603, "bf16"), (1536, 2100, "f32")])
+def test_orth_large(dcf, rows, cols, dtype):
+    """Sizes that pairs of CTAs take."""
+    x = randn((1, rows, cols), dtype, 61)
+    check_orth(run_orth(dcf, x, dtype, steps=2), x, dtype, [COEF] * 2)
