@@ -38,7 +38,12 @@ constexpr int kPlane = kSide * kBK * 2;  // bytes of one plane of one operand in
 constexpr int kStage = 4 * kPlane;       // P hi, P lo, Q hi, Q lo
 constexpr int kOrthStages = 3;
 constexpr int kOutWarps = 8;             // warps that add up and write out
-constexpr int kGemmThreads = 64 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies, 2 and 3 lend their registers
+constexpr int kTile = 2 * kSide;         // a pair's tile: 256 x 256
+constexpr int kTmem = 2 * kTile;         // TMEM columns: two sums
+constexpr int kMine = kTile / 2;         // columns of one out warp
+constexpr int kBlock = 32 * 64;          // values an out warp writes at a time: 32 rows x 64 columns
+constexpr int kTileBlocks = kTile * kTile / kBlock;
 constexpr int kBuffer = 4096;            // bytes through which an out warp reorders 32 rows
 constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kBuffer + 256 + 1024;
 
@@ -51,76 +56,41 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// The forms for one CTA and for a pair of CTAs that share one product.
-template <int CTAS> struct Tc;
+// Products are made by pairs of CTAs (clusters of two): one instruction
+// multiplies what both have loaded, into the TMEM of both.
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 
-template <> struct Tc<1> {
-  static __device__ __forceinline__ void alloc(uint32_t* at, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  static __device__ __forceinline__ void free(uint32_t at, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
-  }
-  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  }
-  static __device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-  }
-  static __device__ __forceinline__ uint32_t rank() { return 0; }
-  static __device__ __forceinline__ void sync() { __syncthreads(); }
-  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-  }
-};
+// Arrives on this barrier of both CTAs once the products issued before are done.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
 
-template <> struct Tc<2> {
-  static __device__ __forceinline__ void alloc(uint32_t* at, uint32_t cols) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-  }
-  static __device__ __forceinline__ void free(uint32_t at, uint32_t cols) {
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(cols) : "memory");
-  }
-  static __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-  }
-  // Arrives on the barrier of both CTAs.
-  static __device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_addr(bar)),
-        "h"((uint16_t)3)
-        : "memory");
-  }
-  static __device__ __forceinline__ uint32_t rank() {
-    uint32_t r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-  }
-  static __device__ __forceinline__ void sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-  }
-  // Arrives on the first CTA's barrier, from either.
-  static __device__ __forceinline__ void arrive_first(uint64_t* bar) {
-    asm volatile(
-        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n"
-        " mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(smem_addr(bar))
-        : "memory");
-  }
-};
+__device__ __forceinline__ uint32_t pair_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Arrives on the first CTA's barrier, from either.
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(
+          smem_addr(bar))
+      : "memory");
+}
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
@@ -132,8 +102,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+
+// Until the loads issued before have arrived; `r` is named so that no use of it moves ahead.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[j]));
+}
+
+// 384 threads start with 168 registers each; the first four warps keep 40 and
+// the eight that add up get 232: 128 * 40 + 256 * 232 = 384 * 168.
+__device__ __forceinline__ void shrink_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
+__device__ __forceinline__ void grow_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
 
 // Shared-memory descriptor of one plane of an operand with the 128-byte
 // swizzle: groups of eight 128-byte rows lie 1024 bytes apart.  A K-major
@@ -158,26 +139,25 @@ struct Planes {
   }
 };
 
-__device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
-  hi = __float2half_rn(v);
-  lo = __float2half_rn(__fsub_rn(v, __half2float(hi)));
-}
-
-// What the epilogue of a product does with its accumulators.
+// What becomes of a product.
 enum Mode {
   GRAM,   // A = X X^T: planes, both triangles
   POLY,   // B = a I + b A + c A A: planes, both triangles
   APPLY,  // X <- B X: planes
-  FINAL   // the result, in the caller's type
+  FINAL,  // the result, in the caller's type
+  PART    // of a symmetric product cut along k: fp32 sums to be joined
 };
 
 struct GemmArgs {
   int m, n, k;              // rows, columns, length of the product
-  int tiles_m, tiles_n;     // tiles of 128 CTAS x 128 CTAS
-  int tiles;                // per matrix (of the upper triangle for GRAM, POLY)
-  int total;                // of the batch
+  int tiles_m, tiles_n;     // tiles of 256 x 256
+  int tiles;                // per matrix (of a symmetric product: of the upper triangle)
+  int total;                // work items: tiles of the batch, times splits
+  int splits, split_k;      // PART: parts of k, stages of each
+  int sum;                  // stages that TMEM sums before registers do
   float alpha, beta, diag;  // v = alpha acc [+ beta A + diag I]
   Planes to, from;          // result; POLY: A
+  float* part;              // PART
   void* out;
   int out_dtype, vectors;   // vectors: rows of out start on 16-byte boundaries
   int64_t out_rs, out_bs;
@@ -190,17 +170,13 @@ __device__ __forceinline__ void store_typed(void* out, int64_t at, int dtype, fl
   else ((__nv_bfloat16*)out)[at] = __float2bfloat16_rn(v);
 }
 
-__device__ __forceinline__ uint32_t split_word(float v) {
-  __half hi, lo;
-  split(v, hi, lo);
-  return (uint32_t)__half_as_ushort(hi) | ((uint32_t)__half_as_ushort(lo) << 16);
-}
-
-// The his (los) of eight split words.
-template <int LO> __device__ __forceinline__ uint4 plane_of(const uint32_t* w) {
-  constexpr uint32_t pick = LO ? 0x7632 : 0x5410;
-  return make_uint4(__byte_perm(w[0], w[1], pick), __byte_perm(w[2], w[3], pick), __byte_perm(w[4], w[5], pick),
-                    __byte_perm(w[6], w[7], pick));
+// Two values split at once: the his in one word, the los in another.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(__fsub_rn(a, f.x), __fsub_rn(b, f.y));
+  hi = *(const uint32_t*)&h;
+  lo = *(const uint32_t*)&l;
 }
 
 // A warp holds 32 rows x 64 columns with a row in each lane.  Going through
@@ -208,123 +184,116 @@ template <int LO> __device__ __forceinline__ uint4 plane_of(const uint32_t* w) {
 // 16-byte chunks of a row are exchanged so that neither side has bank conflicts.
 __device__ __forceinline__ uint4& chunk(uint4* buf, int row, int k) { return buf[row * 8 + (k ^ (row & 7))]; }
 
-// Eight fp16 values to one place in a plane of a symmetric matrix: those on
-// and right of the diagonal (`row` counts along `at`'s matrix row).
-__device__ __forceinline__ void put_upper(__half* at, const uint4& v, int row, int col) {
-  if (col >= row) {
-    *(uint4*)at = v;
-  } else if (col + 7 >= row) {
-    const __half* e = (const __half*)&v;
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-      if (col + j >= row) at[j] = e[j];
-  }
-}
-
-template <int CTAS, Mode MODE> struct TileOf {
+// Where a work item lies.
+struct Tile {
   uint32_t z;
   int row0, col0;
-  __device__ __forceinline__ TileOf(const GemmArgs& g, int t) {
-    constexpr int side = kSide * CTAS;
+  __device__ __forceinline__ Tile(const GemmArgs& g, int t, bool symmetric) {
     z = (uint32_t)(t / g.tiles);
     int tile = t - (int)z * g.tiles, tm, tn;
-    if (MODE == GRAM || MODE == POLY) {
+    if (symmetric) {
       for (tm = 0; tile >= g.tiles_n - tm; tm++) tile -= g.tiles_n - tm;  // row tm keeps tm .. tiles_n - 1
       tn = tm + tile;
     } else {
       tm = tile % g.tiles_m;
       tn = tile / g.tiles_m;
     }
-    row0 = tm * side;
-    col0 = tn * side;
+    row0 = tm * kTile;
+    col0 = tn * kTile;
   }
 };
 
-// Writes a warp's 32 rows x 64 columns, v[j] in row r0 + lane, column c0 + j.
-template <Mode MODE>
-__device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
-                                          int lane) {
+// Writes a warp's 32 rows x 64 columns of the result, v[j] in row r0 + lane,
+// column c0 + j.
+__device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
+                                            int lane) {
   const int sub = lane >> 3, k = lane & 7;  // of a pass over four rows: row and chunk
-  if (MODE == FINAL) {
-    char* out = (char*)g.out;
-    if (g.out_dtype == DCF_F32) {
+  const int64_t row = (int64_t)z * g.out_bs + (int64_t)(r0 + sub) * g.out_rs;
+  if (g.out_dtype == DCF_F32) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {  // 32 columns of 4 bytes fill the buffer
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float* x = v + half * 32 + j * 4;
-          chunk(buf, lane, j) = make_uint4(__float_as_uint(__fmul_rn(g.alpha, x[0])), __float_as_uint(__fmul_rn(g.alpha, x[1])),
-                                           __float_as_uint(__fmul_rn(g.alpha, x[2])), __float_as_uint(__fmul_rn(g.alpha, x[3])));
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int row = 4 * i + sub, c = c0 + half * 32 + k * 4;
-          const uint4 x = chunk(buf, row, k);
-          if (r0 + row >= g.m) continue;
-          float* at = (float*)out + (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
-          if (g.vectors && c + 4 <= g.n) {
-            *(uint4*)at = x;
-          } else {
-            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (c + j < g.n) at[j] = __uint_as_float(e[j]);
-          }
-        }
-      }
-    } else {
+    for (int half = 0; half < 2; half++) {  // 32 columns of 4 bytes fill the buffer
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float x = __fmul_rn(g.alpha, v[8 * j + 2 * e]), y = __fmul_rn(g.alpha, v[8 * j + 2 * e + 1]);
-          if (g.out_dtype == DCF_F16) {
-            const __half2 p = __floats2half2_rn(x, y);
-            w[e] = *(const uint32_t*)&p;
-          } else {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
-            w[e] = *(const uint32_t*)&p;
-          }
-        }
-        chunk(buf, lane, j) = make_uint4(w[0], w[1], w[2], w[3]);
+        const float* x = v + half * 32 + j * 4;
+        chunk(buf, lane, j) = make_uint4(__float_as_uint(__fmul_rn(g.alpha, x[0])), __float_as_uint(__fmul_rn(g.alpha, x[1])),
+                                         __float_as_uint(__fmul_rn(g.alpha, x[2])), __float_as_uint(__fmul_rn(g.alpha, x[3])));
       }
       __syncwarp();
+      const int c = c0 + half * 32 + k * 4;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int row = 4 * i + sub, c = c0 + k * 8;
-        const uint4 x = chunk(buf, row, k);
-        if (r0 + row >= g.m) continue;
-        uint16_t* at = (uint16_t*)out + (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
-        if (g.vectors && c + 8 <= g.n) {
+        const uint4 x = chunk(buf, 4 * i + sub, k);
+        if (r0 + sub + 4 * i >= g.m) break;
+        float* at = (float*)g.out + row + 4 * i * g.out_rs + c;
+        if (g.vectors && c + 4 <= g.n) {
           *(uint4*)at = x;
         } else {
           const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int j = 0; j < 8; j++)
-            if (c + j < g.n) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
+          for (int j = 0; j < 4; j++)
+            if (c + j < g.n) at[j] = __uint_as_float(e[j]);
         }
       }
     }
     return;
   }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float x = __fmul_rn(g.alpha, v[8 * j + 2 * e]), y = __fmul_rn(g.alpha, v[8 * j + 2 * e + 1]);
+      if (g.out_dtype == DCF_F16) {
+        const __half2 p = __floats2half2_rn(x, y);
+        w[e] = *(const uint32_t*)&p;
+      } else {
+        const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+        w[e] = *(const uint32_t*)&p;
+      }
+    }
+    chunk(buf, lane, j) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncwarp();
+  const int c = c0 + k * 8;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint4 x = chunk(buf, 4 * i + sub, k);
+    if (r0 + sub + 4 * i >= g.m) break;
+    uint16_t* at = (uint16_t*)g.out + row + 4 * i * g.out_rs + c;
+    if (g.vectors && c + 8 <= g.n) {
+      *(uint4*)at = x;
+    } else {
+      const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (c + j < g.n) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
+    }
+  }
+}
+
+// The same as planes; for GRAM and POLY on and above the diagonal, with
+// the mirror image strictly below it.
+template <Mode MODE>
+__device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
+                                             int lane) {
   constexpr bool sym = MODE == GRAM || MODE == POLY;
-  uint32_t w[64];
+  const int sub = lane >> 3, k = lane & 7;
+  const size_t plane_size = (size_t)g.to.rows * g.to.ld;
+  uint32_t w[2][32];  // his, los of two columns each
   if (MODE == POLY) {
     float x[64];
 #pragma unroll
     for (int j = 0; j < 64; j++) x[j] = __fmul_rn(g.alpha, v[j]);
+    const __half* from = g.from.row(z, 0, r0 + sub) + c0 + 8 * k;
 #pragma unroll
     for (int plane = 0; plane < 2; plane++) {
       __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const int row = 4 * i + sub;
-        if (r0 + row < g.m) chunk(buf, row, k) = *(const uint4*)(g.from.row(z, plane, r0 + row) + c0 + 8 * k);
-      }
+      for (int i = 0; i < 8; i++)
+        if (r0 + sub + 4 * i < g.m)
+          chunk(buf, 4 * i + sub, k) = *(const uint4*)(from + plane * plane_size + (size_t)(4 * i) * g.from.ld);
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -338,85 +307,106 @@ __device__ __forceinline__ void write_out(const GemmArgs& g, uint32_t z, int r0,
         }
       }
     }
+    if (c0 < r0 + 32)
 #pragma unroll
-    for (int j = 0; j < 64; j++) w[j] = split_word(c0 + j == r0 + lane ? __fadd_rn(x[j], g.diag) : x[j]);
+      for (int j = 0; j < 64; j++)
+        if (c0 + j == r0 + lane) x[j] = __fadd_rn(x[j], g.diag);
+#pragma unroll
+    for (int j = 0; j < 32; j++) split2(x[2 * j], x[2 * j + 1], w[0][j], w[1][j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < 64; j++) w[j] = split_word(__fmul_rn(g.alpha, v[j]));
+    for (int j = 0; j < 32; j++)
+      split2(__fmul_rn(g.alpha, v[2 * j]), __fmul_rn(g.alpha, v[2 * j + 1]), w[0][j], w[1][j]);
   }
+  __half* to = g.to.row(z, 0, r0 + sub) + c0 + 8 * k;
 #pragma unroll
   for (int plane = 0; plane < 2; plane++) {  // rows are padded to 64 columns: whole vectors fit
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 8; j++) chunk(buf, lane, j) = plane ? plane_of<1>(w + 8 * j) : plane_of<0>(w + 8 * j);
+    for (int j = 0; j < 8; j++) chunk(buf, lane, j) = make_uint4(w[plane][4 * j], w[plane][4 * j + 1], w[plane][4 * j + 2], w[plane][4 * j + 3]);
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const int row = 4 * i + sub, c = c0 + k * 8;
-      const uint4 x = chunk(buf, row, k);
-      if (r0 + row >= g.m) continue;
-      __half* at = g.to.row(z, plane, r0 + row) + c;
-      if (sym) put_upper(at, x, r0 + row, c);
-      else *(uint4*)at = x;
+      const uint4 x = chunk(buf, 4 * i + sub, k);
+      const int over = r0 + sub + 4 * i - (c0 + 8 * k);  // columns of the vector left of the diagonal
+      if (r0 + sub + 4 * i >= g.m) break;
+      __half* at = to + plane * plane_size + (size_t)(4 * i) * g.to.ld;
+      if (!sym || over <= 0) {
+        *(uint4*)at = x;
+      } else if (over < 8) {
+        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (j >= over) at[j] = __ushort_as_half((unsigned short)(e[j >> 1] >> ((j & 1) * 16)));
+      }
     }
   }
   if (!sym || c0 + 63 <= r0) return;
-  // The mirror image: eight rows of one column per vector, strictly below
-  // the diagonal.
-  uint32_t* turn = (uint32_t*)buf;  // [32 columns][32 rows], groups of four rows exchanged
+  // Eight rows of one column per vector.
+  uint32_t* turn = (uint32_t*)buf;  // [32 column pairs][32 rows], groups of four rows exchanged
+  const int q = (lane & 3) * 2, r = r0 + q * 4;
 #pragma unroll
-  for (int half = 0; half < 2; half++) {
+  for (int plane = 0; plane < 2; plane++) {
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 32; j++) turn[j * 32 + (((lane >> 2) ^ (j & 7)) << 2) + (lane & 3)] = w[half * 32 + j];
+    for (int j = 0; j < 32; j++) turn[j * 32 + (((lane >> 2) ^ (j & 7)) << 2) + (lane & 3)] = w[plane][j];
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const int j = i * 8 + (lane >> 2), q = (lane & 3) * 2, c = c0 + half * 32 + j, r = r0 + q * 4;
-      uint32_t x[8];
-      *(uint4*)&x[0] = *(const uint4*)&turn[j * 32 + ((q ^ (j & 7)) << 2)];
-      *(uint4*)&x[4] = *(const uint4*)&turn[j * 32 + (((q + 1) ^ (j & 7)) << 2)];
-      if (c >= g.n || r >= g.m) continue;
-      __half* hi = g.to.row(z, 0, c) + r;
-      __half* lo = g.to.row(z, 1, c) + r;
-      const uint4 h = plane_of<0>(x), l = plane_of<1>(x);
-      if (c >= r + 8) {
-        *(uint4*)hi = h;
-        *(uint4*)lo = l;
-      } else {
+      const int j = i * 8 + (lane >> 2), c = c0 + 2 * j;
+      const uint4 x = *(const uint4*)&turn[j * 32 + ((q ^ (j & 7)) << 2)];
+      const uint4 y = *(const uint4*)&turn[j * 32 + (((q + 1) ^ (j & 7)) << 2)];
+      if (r >= g.m) continue;
+      __half* at = g.to.row(z, plane, c) + r;
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (c > r + e) {
-            hi[e] = ((const __half*)&h)[e];
-            lo[e] = ((const __half*)&l)[e];
-          }
+      for (int b = 0; b < 2; b++) {  // column c, c + 1
+        const uint32_t pick = b ? 0x7632 : 0x5410;
+        const uint4 e = make_uint4(__byte_perm(x.x, x.y, pick), __byte_perm(x.z, x.w, pick), __byte_perm(y.x, y.y, pick),
+                                   __byte_perm(y.z, y.w, pick));
+        if (c + b >= g.n) continue;
+        const int below = c + b - r;  // rows of the vector above the diagonal
+        if (below >= 8) {
+          *(uint4*)(at + b * g.to.ld) = e;
+        } else {
+          const uint32_t f[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+          for (int u = 0; u < 8; u++)
+            if (u < below) at[b * g.to.ld + u] = __ushort_as_half((unsigned short)(f[u >> 1] >> ((u & 1) * 16)));
+        }
       }
     }
   }
 }
 
-// D = P Q^T in square tiles of 128 CTAS, P and Q given as two fp16 planes
-// each; P_MN, Q_MN: its memory has rows of k and runs along the operand, so
-// that no operand is ever written transposed.  Persistent CTAs (pairs of CTAs): warp 0 keeps a ring of stages
-// full, 64 columns of all four planes each, which three products share; one
-// thread issues these; eight warps add up and write out.
+// Values of PART: per item and block of 32 x 64, [column][row].
+__device__ __forceinline__ float* part_block(float* part, int64_t item, int block) {
+  return part + (item * kTileBlocks + block) * kBlock;
+}
+
+// D = P Q^T in 256 x 256 tiles, P and Q given as two fp16 planes each; P_MN,
+// Q_MN: its memory has rows of k and runs along the operand, so that no
+// operand is ever written transposed.
 //
-// The tensor core truncates as it accumulates, which shows as a bias of some
-// 2^-25 per instruction: 1e-4 over k = 8192.  So TMEM sums one stage
-// only (the two small products first, then the large one), in two buffers
-// in turn, and the eight warps add the stages in registers, rounding to
-// nearest.
+// Persistent pairs of CTAs; each CTA loads 128 rows of P and of Q and keeps the
+// result of its rows of P with all of Q: 64 KB of loads feed 12 instructions of
+// 128 cycles (one CTA by itself with 128 x 128 tiles waits for its loads and
+// for shared memory: twice the time per product, measured).  Warp 0 keeps a ring
+// of stages full, 64 columns of all four planes, which three products share.
+// One thread of the first CTA issues these for both; the second CTA reports
+// its full stages to it.  Eight warps add up and write out.
 //
-// A pair works on one 256 x 256 tile: each CTA loads 128 rows of P and of Q
-// and multiplies its rows of P with all of Q, so that a stage feeds twice the
-// arithmetic.  The second CTA reports its full stages to the first, which
-// issues for both.
-template <int CTAS, Mode MODE, bool P_MN, bool Q_MN>
+// The tensor core truncates as it accumulates, a bias of some 2^-25 per
+// instruction: 1e-4 in the result over k = 8192.  So TMEM sums `sum` stages
+// only (the two small products of a stage first, then the large one), in two
+// buffers in turn, and the eight warps add the sums in registers, rounding to
+// nearest: 2 stages where the result is f32 (3e-6 there), 16 where it is rounded to
+// 16 bits anyway (1e-5), which leaves the warps time to write a tile while the
+// next is multiplied.
+template <Mode MODE, bool P_MN, bool Q_MN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
                                                                     const __grid_constant__ GemmArgs g) {
-  using T = Tc<CTAS>;
-  constexpr int kCols = kSide * CTAS, kTmem = 2 * kCols, kMine = kCols / 2;  // columns of one out warp
+  constexpr bool symmetric = MODE == GRAM || MODE == POLY || MODE == PART;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* buffers = base + kOrthStages * kStage;
@@ -427,9 +417,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   uint64_t* sum_empty = sum_full + 2;     // the first CTA's
   uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = T::rank();
-  const int first = (int)(blockIdx.x / CTAS), step = (int)(gridDim.x / CTAS);
-  const int blocks = (g.k + kBK - 1) / kBK;
+  const uint32_t rank = pair_rank();
+  const int first = (int)(blockIdx.x / 2), step = (int)(gridDim.x / 2);
+  const int all = (g.k + kBK - 1) / kBK;
+  // The stages of a work item.
+  auto begin_of = [&](int t) { return MODE == PART ? t % g.splits * g.split_k : 0; };
+  auto count_of = [&](int t) { return MODE == PART ? min(g.split_k, all - begin_of(t)) : all; };
+  auto tile_of = [&](int t) { return Tile(g, MODE == PART ? t / g.splits : t, symmetric); };
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < kOrthStages; s++) {
@@ -439,25 +433,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
-      mbar_init(&sum_empty[b], CTAS * kOutWarps);
+      mbar_init(&sum_empty[b], 2 * kOutWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) T::alloc(tmem_at, kTmem);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_at)), "r"(kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  T::sync();
+  pair_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t*)tmem_at;
+  pdl_begin();
 
   bool fail = false;
+  if (warp < 4) shrink_registers();
   if (warp == 0) {
     if (lane == 0) {
       int64_t i = 0;  // stages so far
       for (int t = first; t < g.total && !fail; t += step) {
-        const TileOf<CTAS, MODE> at(g, t);
+        const Tile at = tile_of(t);
         const int row = at.row0 + (int)rank * kSide, col = at.col0 + (int)rank * kSide, z = (int)(2 * at.z);
+        const int b0 = begin_of(t), blocks = count_of(t);
         for (int b = 0; b < blocks; b++, i++) {
           const int s = (int)(i % kOrthStages);
           if (i >= kOrthStages && !mbar_wait_bounded(&empty[s], (unsigned)((i / kOrthStages - 1) & 1))) {
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
 #pragma unroll
             for (int p = 0; p < 2; p++) {
               const uint32_t at = to + p * kPlane + half * (kPlane / 2);
-              const int r = row + half * 64, c = col + half * 64, k = b * kBK;
+              const int r = row + half * 64, c = col + half * 64, k = (b0 + b) * kBK;
               tma_load_3d(at, &map_p, P_MN ? r : k, P_MN ? k : r, z + p, &full[s]);
               tma_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, &full[s]);
             }
@@ -487,87 +488,134 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = (1u << 4) | ((uint32_t)P_MN << 15) | ((uint32_t)Q_MN << 16) |
-                                 ((uint32_t)(kCols >> 3) << 17) | ((uint32_t)(kCols >> 4) << 24);
-      int64_t i = 0;
+                                 ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+      int64_t i = 0, u = 0;  // stages and sums so far
       for (int t = first; t < g.total && !fail; t += step) {
+        const int blocks = count_of(t);
+        int in_sum = 0;
         for (int b = 0; b < blocks; b++, i++) {
-          const int s = (int)(i % kOrthStages), d = (int)(i & 1);
+          const int s = (int)(i % kOrthStages), d = (int)(u & 1);
           const unsigned turn = (unsigned)((i / kOrthStages) & 1);
           if (!mbar_wait_bounded(&full[s], turn)) {
             fail = true;
             break;
           }
-          if (CTAS == 2 && rank) {
-            T::arrive_first(&peer[s]);
+          if (rank) {
+            arrive_first(&peer[s]);
             continue;
           }
-          if ((CTAS == 2 && !mbar_wait_bounded(&peer[s], turn)) ||
-              (i >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((i / 2 - 1) & 1)))) {
+          if (!mbar_wait_bounded(&peer[s], turn) ||
+              (in_sum == 0 && u >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((u / 2 - 1) & 1)))) {
             fail = true;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t at = smem_addr(base + s * kStage), to = tmem + d * kCols;
+          const uint32_t at = smem_addr(base + s * kStage), to = tmem + d * kTile;
           const uint64_t ph = smem_desc<P_MN>(at), pl = smem_desc<P_MN>(at + kPlane);
           const uint64_t qh = smem_desc<Q_MN>(at + 2 * kPlane), ql = smem_desc<Q_MN>(at + 3 * kPlane);
           constexpr uint32_t ps = kSlice<P_MN>, qs = kSlice<Q_MN>;
 #pragma unroll
           for (uint32_t j = 0; j < kBK / 16; j++) {
-            T::mma(to, ph + ps * j, ql + qs * j, idesc, j != 0);
-            T::mma(to, pl + ps * j, qh + qs * j, idesc, 1);
+            pair_mma(to, ph + ps * j, ql + qs * j, idesc, in_sum | (int)j);
+            pair_mma(to, pl + ps * j, qh + qs * j, idesc, 1);
           }
 #pragma unroll
-          for (uint32_t j = 0; j < kBK / 16; j++) T::mma(to, ph + ps * j, qh + qs * j, idesc, 1);
-          T::commit(&empty[s]);
-          T::commit(&sum_full[d]);
+          for (uint32_t j = 0; j < kBK / 16; j++) pair_mma(to, ph + ps * j, qh + qs * j, idesc, 1);
+          pair_commit(&empty[s]);
+          if (++in_sum == g.sum || b == blocks - 1) {
+            pair_commit(&sum_full[d]);
+            u++;
+            in_sum = 0;
+          }
         }
       }
     }
-  } else {
-    const int part = warp & 3;                  // the 32 TMEM lanes this warp may read
-    const int col = (warp - 2) / 4 * kMine;     // and the half of the columns it takes
-    uint4* buf = (uint4*)(buffers + (warp - 2) * kBuffer);
-    int64_t i = 0;
+  } else if (warp >= 4) {
+    grow_registers();
+    const int part = warp & 3;               // the 32 TMEM lanes this warp may read
+    const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
+    uint4* buf = (uint4*)(buffers + (warp - 4) * kBuffer);
+    const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
+    int64_t u = 0;  // sums so far
     for (int t = first; t < g.total && !fail; t += step) {
-      const TileOf<CTAS, MODE> at(g, t);
+      const Tile at = tile_of(t);
+      const int sums = (count_of(t) + g.sum - 1) / g.sum;
       float acc[kMine];
 #pragma unroll
       for (int j = 0; j < kMine; j++) acc[j] = 0;
-      for (int b = 0; b < blocks; b++, i++) {
-        const int d = (int)(i & 1);
-        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[d], (unsigned)((i >> 1) & 1)))) {
+      for (int b = 0; b < sums; b++, u++) {
+        const int d = (int)(u & 1);
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[d], (unsigned)((u >> 1) & 1)))) {
           fail = true;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t x[2][32];  // one part is added while the next arrives
+        tmem_load32(lanes + d * kTile, x[0]);
 #pragma unroll
         for (int c = 0; c < kMine; c += 32) {
-          uint32_t x[32];
-          tmem_load32(tmem + ((uint32_t)(part * 32) << 16) + d * kCols + col + c, x);
+          tmem_wait(x[c / 32 & 1]);
+          if (c + 32 < kMine) {
+            tmem_load32(lanes + d * kTile + c + 32, x[(c / 32 + 1) & 1]);
+          } else {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) arrive_first(&sum_empty[d]);
+          }
 #pragma unroll
-          for (int j = 0; j < 32; j++) acc[c + j] = __fadd_rn(acc[c + j], __uint_as_float(x[j]));
+          for (int j = 0; j < 32; j++) acc[c + j] = __fadd_rn(acc[c + j], __uint_as_float(x[c / 32 & 1][j]));
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        if (lane == 0) T::arrive_first(&sum_empty[d]);
       }
       if (fail) break;
-      const int r0 = at.row0 + (int)rank * kSide + part * 32;
+      const int row = (int)rank * kSide + part * 32, r0 = at.row0 + row;
 #pragma unroll
       for (int c = 0; c < kMine; c += 64) {
         const int c0 = at.col0 + col + c;
         // beyond the matrix, or below the diagonal: written by its mirror image
-        if (r0 >= g.m || c0 >= g.n || ((MODE == GRAM || MODE == POLY) && c0 + 63 < r0)) continue;
-        write_out<MODE>(g, at.z, r0, c0, acc + c, buf, lane);
+        if (r0 >= g.m || c0 >= g.n || (symmetric && c0 + 63 < r0)) continue;
+        if (MODE == PART) {
+          float* p = part_block(g.part, t, row / 32 * (kTile / 64) + (col + c) / 64) + lane;
+#pragma unroll
+          for (int j = 0; j < 64; j++) p[j * 32] = acc[c + j];
+        } else if (MODE == FINAL) {
+          write_final(g, at.z, r0, c0, acc + c, buf, lane);
+        } else {
+          write_planes<MODE>(g, at.z, r0, c0, acc + c, buf, lane);
+        }
       }
     }
   }
   if (fail) atomicExch(&g.st->error, 1u);
   __syncthreads();
-  T::sync();
+  pair_sync();
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    T::free(tmem, kTmem);
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
   }
+}
+
+// Joins the parts of a symmetric product, always in the same order; a warp
+// takes a block of 32 x 64.
+constexpr int kJoinWarps = 4;
+template <Mode MODE>
+__global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const __grid_constant__ GemmArgs g) {
+  __shared__ uint4 buffers[kJoinWarps][kBuffer / 16];
+  pdl_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + warp;
+  const int block = (int)(id % kTileBlocks);
+  if (id / kTileBlocks >= g.total) return;
+  const Tile at(g, (int)(id / kTileBlocks), true);
+  const int r0 = at.row0 + block / (kTile / 64) * 32, c0 = at.col0 + block % (kTile / 64) * 64;
+  if (r0 >= g.m || c0 >= g.n || c0 + 63 < r0) return;
+  float v[64];
+#pragma unroll
+  for (int j = 0; j < 64; j++) v[j] = 0;
+  for (int s = 0; s < g.splits; s++) {
+    const float* p = part_block(g.part, id / kTileBlocks * g.splits + s, block) + lane;
+#pragma unroll
+    for (int j = 0; j < 64; j++) v[j] = __fadd_rn(v[j], p[j * 32]);
+  }
+  write_planes<MODE>(g, at.z, r0, c0, v, buffers[warp], lane);
 }
 
 // ------------------------------------------------------- norm and split
@@ -614,6 +662,7 @@ constexpr int kNormThreads = 256;
 // Sums of squares in 64 bits (a f32 element's square can pass 32), one part
 // per block.
 __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_constant__ MatArgs a, double* part) {
+  pdl_begin();
   const uint32_t z = blockIdx.y, groups = (uint32_t)(a.cols + 7) / 8;
   const uint64_t total = (uint64_t)groups * a.rows;
   double s = 0;
@@ -640,6 +689,7 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
                                                                   void* out, int out_dtype, int64_t out_rs,
                                                                   int64_t out_bs) {
   __shared__ double factor;
+  pdl_begin();
   const uint32_t z = blockIdx.y;
   if (threadIdx.x < 32) {
     double s = 0;
@@ -661,11 +711,11 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
       for (int j = 0; j < 8 && c + j < a.cols; j++)
         store_typed(out, (int64_t)z * out_bs + (int64_t)r * out_rs + c + j, out_dtype, v[j]);
     } else {
-      uint32_t w[8];
+      uint32_t h[4], l[4];
 #pragma unroll
-      for (int j = 0; j < 8; j++) w[j] = split_word(v[j]);
-      *(uint4*)(x.row(z, 0, r) + c) = plane_of<0>(w);  // rows are padded to 64 columns
-      *(uint4*)(x.row(z, 1, r) + c) = plane_of<1>(w);
+      for (int j = 0; j < 4; j++) split2(v[2 * j], v[2 * j + 1], h[j], l[j]);
+      *(uint4*)(x.row(z, 0, r) + c) = make_uint4(h[0], h[1], h[2], h[3]);  // rows are padded to 64 columns
+      *(uint4*)(x.row(z, 1, r) + c) = make_uint4(l[0], l[1], l[2], l[3]);
     }
   }
 }
@@ -740,7 +790,7 @@ int scale_of(double bound) {
 }
 
 constexpr double kMostSingular = 64;
-constexpr int kPairRows = 1536;
+constexpr int kPairs = 74;  // pairs of SMs
 
 // Blocks of the norm's sum: 32 KB of a f32 matrix each, 256 at most.
 int norm_parts(const dcf_orth_desc& d) {
@@ -748,9 +798,40 @@ int norm_parts(const dcf_orth_desc& d) {
   return (int)(p < 256 ? p : 256);
 }
 
-// The workspace: X twice (a step reads one and writes the other), A, B.
+// Parts into which the k of a symmetric product is cut, `stages` stages each.
+// One part keeps a tile in registers until it is written; more keep
+// pairs of SMs busy that would have no tile.  In units of a stage (0.85 us):
+// every round of tiles costs its stages and some 4 to start and write,
+// and a join some 8.
+struct Cut {
+  int splits, stages;
+};
+
+Cut cut_of(int64_t tiles, int stages) {
+  Cut best = {1, stages};
+  int64_t least = (tiles + kPairs - 1) / kPairs * (stages + 4);
+  for (int s = 2; s <= stages && tiles * s <= kPairs; s++) {
+    const int each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
+    const int64_t cost = each + 4 + 8;
+    if (cost < least) {
+      least = cost;
+      best = {parts, each};
+    }
+  }
+  return best;
+}
+
+int64_t upper_tiles(int m) {
+  const int64_t t = (m + kTile - 1) / kTile;
+  return t * (t + 1) / 2;
+}
+
+// The workspace: X twice (a step reads one and writes the other), A, B, and
+// the parts of A or B.
 struct Layout {
   Planes x[2], a, b;
+  float* sums;
+  Cut gram, poly;
   double* part;
   int parts;
   size_t bytes;
@@ -779,40 +860,69 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
     l.b = planes(m, m);
   }
   if (d.steps > 1) l.x[1] = planes((int)d.rows, (int)d.cols);
+  const int n = (int)(d.rows < d.cols ? d.cols : d.rows);
+  const int64_t tiles = upper_tiles(m) * (int64_t)d.batch;
+  l.gram = cut_of(tiles, (n + kBK - 1) / kBK);
+  l.poly = cut_of(tiles, (m + kBK - 1) / kBK);
+  const int most = l.gram.splits > l.poly.splits ? l.gram.splits : l.poly.splits;
+  l.sums = d.steps && most > 1 ? (float*)take((size_t)(tiles * most) * kTile * kTile * 4) : nullptr;
   l.bytes = off;
   return l;
 }
 
-template <int CTAS, Mode MODE, bool P_MN, bool Q_MN>
-int gemm_with(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
-  constexpr int side = kSide * CTAS;
-  g.tiles_m = (g.m + side - 1) / side;
-  g.tiles_n = (g.n + side - 1) / side;
-  g.tiles = MODE == GRAM || MODE == POLY ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-  g.total = (int)(g.tiles * batch);
-  auto kernel = orth_gemm_kernel<CTAS, MODE, P_MN, Q_MN>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
-    return DCF_ECUDA;
-  const int most = sm_count_current() / CTAS;
+// Launches as a programmatic dependent: the kernel's start overlaps the end of
+// the one before it, whose results it reads only after griddepcontrol.wait.
+template <class... P, class... A>
+int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((unsigned)((g.total < most ? g.total : most) * CTAS));
-  c.blockDim = dim3(kGemmThreads);
-  c.dynamicSmemBytes = kGemmSmem;
+  c.gridDim = grid;
+  c.blockDim = dim3((unsigned)threads);
+  c.dynamicSmemBytes = (size_t)smem;
   c.stream = s;
-  cudaLaunchAttribute a[1];
-  a[0].id = cudaLaunchAttributeClusterDimension;
-  a[0].val.clusterDim.x = CTAS;
-  a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute a[2];
+  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a[0].val.programmaticStreamSerializationAllowed = 1;
+  a[1].id = cudaLaunchAttributeClusterDimension;
+  a[1].val.clusterDim.x = (unsigned)cluster;
+  a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;
   c.attrs = a;
-  c.numAttrs = 1;
+  c.numAttrs = cluster > 1 ? 2 : 1;
   note_launch();
-  return cudaLaunchKernelEx(&c, kernel, p, q, g) == cudaSuccess ? DCF_OK : DCF_ECUDA;
+  return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
 
 template <Mode MODE, bool P_MN, bool Q_MN>
-int gemm(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, uint64_t batch, cudaStream_t s) {
-  return (g.m < g.n ? g.m : g.n) >= kPairRows ? gemm_with<2, MODE, P_MN, Q_MN>(p, q, g, batch, s)
-                                              : gemm_with<1, MODE, P_MN, Q_MN>(p, q, g, batch, s);
+int gemm_run(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, cudaStream_t s) {
+  auto kernel = orth_gemm_kernel<MODE, P_MN, Q_MN>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
+    return DCF_ECUDA;
+  const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
+  return launch(kernel, dim3(2 * pairs), kGemmThreads, kGemmSmem, 2, s, p, q, g);
+}
+
+template <Mode MODE, bool P_MN, bool Q_MN>
+int gemm(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
+  g.tiles_m = (g.m + kTile - 1) / kTile;
+  g.tiles_n = (g.n + kTile - 1) / kTile;
+  g.tiles = g.tiles_m * g.tiles_n;
+  g.total = (int)(g.tiles * batch);
+  return gemm_run<MODE, P_MN, Q_MN>(p, q, g, s);
+}
+
+// A symmetric product, cut along k where that pays.
+template <Mode MODE, bool MN>
+int gemm_symmetric(const CUtensorMap& x, GemmArgs g, const Cut& cut, uint64_t batch, cudaStream_t s) {
+  g.tiles_m = g.tiles_n = (g.m + kTile - 1) / kTile;
+  g.tiles = (int)upper_tiles(g.m);
+  g.total = (int)(g.tiles * batch);
+  g.splits = cut.splits;
+  g.split_k = cut.stages;
+  if (cut.splits == 1) return gemm_run<MODE, MN, MN>(x, x, g, s);
+  GemmArgs parts = g;
+  parts.total *= cut.splits;
+  if (int rc = gemm_run<PART, MN, MN>(x, x, parts, s)) return rc;
+  const int64_t warps = (int64_t)g.total * kTileBlocks;
+  return launch(orth_join_kernel<MODE>, dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps)), 32 * kJoinWarps, 0, 1, s, g);
 }
 
 }  // namespace
@@ -875,14 +985,14 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
   a.vectors = vectors(in, a.rs, a.bs, dtype_size(a.dtype));
   const int64_t out_rs = d.out_row_stride ? d.out_row_stride : (int64_t)d.cols;
   const int64_t out_bs = d.out_batch_stride ? d.out_batch_stride : (int64_t)d.rows * out_rs;
-  orth_norm_kernel<<<dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, s>>>(a, l.part);
-  note_launch();
+  int rc = launch(orth_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, 1, s, a, l.part);
+  if (rc) return rc;
   int sx = d.steps ? scale_of(1) : 0;
   const uint64_t groups = (d.cols + 7) / 8 * d.rows, blocks = (groups + kNormThreads - 1) / kNormThreads;
-  orth_split_kernel<<<dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch), kNormThreads, 0, s>>>(
-      a, l.part, l.parts, d.eps, ldexp(1.0, sx), l.x[0], d.steps ? nullptr : out, (int)d.out_dtype, out_rs, out_bs);
-  note_launch();
-  if (cudaPeekAtLastError() != cudaSuccess) return DCF_ECUDA;
+  rc = launch(orth_split_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch), kNormThreads, 0, 1, s, a,
+              (const double*)l.part, l.parts, d.eps, ldexp(1.0, sx), l.x[0], d.steps ? (void*)nullptr : out,
+              (int)d.out_dtype, out_rs, out_bs);
+  if (rc) return rc;
   if (!d.steps) return DCF_OK;
 
   if (!encoder()) return DCF_EUNSUPPORTED;
@@ -899,11 +1009,13 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     const CUtensorMap& x = mx[i & 1];
     GemmArgs g = {};
     g.st = st;
+    g.sum = d.out_dtype == DCF_F32 ? 2 : 16;
+    g.part = l.sums;
     g.m = g.n = m;
     g.k = n;
     g.alpha = (float)ldexp(1.0, sa - 2 * sx);
     g.to = l.a;
-    int rc = tall ? gemm<GRAM, true, true>(x, x, g, d.batch, s) : gemm<GRAM, false, false>(x, x, g, d.batch, s);
+    rc = tall ? gemm_symmetric<GRAM, true>(x, g, l.gram, d.batch, s) : gemm_symmetric<GRAM, false>(x, g, l.gram, d.batch, s);
     if (rc) return rc;
     g.k = m;
     g.alpha = (float)ldexp(k[2], sb - 2 * sa);
@@ -911,7 +1023,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
     g.to = l.b;
-    if ((rc = gemm<POLY, false, false>(ma, ma, g, d.batch, s))) return rc;
+    if ((rc = gemm_symmetric<POLY, false>(ma, g, l.poly, d.batch, s))) return rc;
     g.m = rows;
     g.n = cols;
     if (i + 1 < d.steps) {
