@@ -42,7 +42,7 @@ constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 mult
 constexpr int kTile = 2 * kSide;         // a pair's tile: 256 x 256
 constexpr int kTmem = 2 * kTile;         // TMEM columns: two sums
 constexpr int kMine = kTile / 2;         // columns of one out warp
-constexpr int kBlock = 32 * 64;          // values an out warp writes at a time: 32 rows x 64 columns
+constexpr int kBlock = 32 * 32;          // values an out warp writes at a time: 32 rows x 32 columns
 constexpr int kTileBlocks = kTile * kTile / kBlock;
 constexpr int kBuffer = 4096;            // bytes through which an out warp reorders 32 rows
 constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kBuffer + 256 + 1024;
@@ -179,11 +179,6 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = *(const uint32_t*)&l;
 }
 
-// A warp holds 32 rows x 64 columns with a row in each lane.  Going through
-// 4 KB of shared memory, eight lanes then take one row's 128 bytes; the
-// 16-byte chunks of a row are exchanged so that neither side has bank conflicts.
-__device__ __forceinline__ uint4& chunk(uint4* buf, int row, int k) { return buf[row * 8 + (k ^ (row & 7))]; }
-
 // Where a work item lies.
 struct Tile {
   uint32_t z;
@@ -203,182 +198,145 @@ struct Tile {
   }
 };
 
-// Writes a warp's 32 rows x 64 columns of the result, v[j] in row r0 + lane,
-// column c0 + j.
-__device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
-                                            int lane) {
-  const int sub = lane >> 3, k = lane & 7;  // of a pass over four rows: row and chunk
-  const int64_t row = (int64_t)z * g.out_bs + (int64_t)(r0 + sub) * g.out_rs;
-  if (g.out_dtype == DCF_F32) {
-#pragma unroll
-    for (int half = 0; half < 2; half++) {  // 32 columns of 4 bytes fill the buffer
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float* x = v + half * 32 + j * 4;
-        chunk(buf, lane, j) = make_uint4(__float_as_uint(__fmul_rn(g.alpha, x[0])), __float_as_uint(__fmul_rn(g.alpha, x[1])),
-                                         __float_as_uint(__fmul_rn(g.alpha, x[2])), __float_as_uint(__fmul_rn(g.alpha, x[3])));
-      }
-      __syncwarp();
-      const int c = c0 + half * 32 + k * 4;
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const uint4 x = chunk(buf, 4 * i + sub, k);
-        if (r0 + sub + 4 * i >= g.m) break;
-        float* at = (float*)g.out + row + 4 * i * g.out_rs + c;
-        if (g.vectors && c + 4 <= g.n) {
-          *(uint4*)at = x;
-        } else {
-          const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (c + j < g.n) at[j] = __uint_as_float(e[j]);
-        }
-      }
-    }
-    return;
-  }
+// A block of 32 rows x 32 columns on its way out: from rows in lanes, through
+// 4 KB of shared memory, to eight columns of a row, or eight rows of a column,
+// in each lane.  Groups of four rows are exchanged so that none of the three
+// has bank conflicts.  (The code is short on purpose: unrolled over a
+// warp's 128 columns it ran once per tile, and fetching it took 15 us.)
+__device__ __forceinline__ uint32_t place(int col, int row) {
+  return (uint32_t)(col * 32 + ((((row >> 2) ^ (col & 7) ^ ((col >> 2) & 6)) << 2) | (row & 3)));
+}
+
+__device__ __forceinline__ void block_in(float* buf, const float* v, int lane) {
   __syncwarp();
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
+  for (int j = 0; j < 32; j++) buf[place(j, lane)] = v[j];
+  __syncwarp();
+}
+
+// Eight values as his and los.
+__device__ __forceinline__ void split8(const float (&v)[8], uint4& hi, uint4& lo) {
+  split2(v[0], v[1], hi.x, lo.x);
+  split2(v[2], v[3], hi.y, lo.y);
+  split2(v[4], v[5], hi.z, lo.z);
+  split2(v[6], v[7], hi.w, lo.w);
+}
+
+// Those of eight 16-bit values with from <= index < to.
+__device__ __forceinline__ void put_some(uint16_t* at, const uint4& v, int from, int to) {
+  const uint32_t e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 8; j++)
+    if (j >= from && j < to) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
+}
+
+// Writes the block at row r0, column c0 of the result in the caller's type.
+__device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* buf, int lane) {
+  const int o = (lane & 3) * 8, c = c0 + o, have = g.n - c;
+  if (have <= 0) return;
+#pragma unroll 1
+  for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[place(o + e, row)]);
+    const int64_t at = (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
+    if (g.out_dtype == DCF_F32) {
+      float* to = (float*)g.out + at;
+      if (g.vectors && have >= 8) {
+        *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (e < have) to[e] = v[e];
+      }
+      continue;
+    }
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float x = __fmul_rn(g.alpha, v[8 * j + 2 * e]), y = __fmul_rn(g.alpha, v[8 * j + 2 * e + 1]);
       if (g.out_dtype == DCF_F16) {
-        const __half2 p = __floats2half2_rn(x, y);
+        const __half2 p = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
         w[e] = *(const uint32_t*)&p;
       } else {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
+        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
         w[e] = *(const uint32_t*)&p;
       }
     }
-    chunk(buf, lane, j) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  __syncwarp();
-  const int c = c0 + k * 8;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint4 x = chunk(buf, 4 * i + sub, k);
-    if (r0 + sub + 4 * i >= g.m) break;
-    uint16_t* at = (uint16_t*)g.out + row + 4 * i * g.out_rs + c;
-    if (g.vectors && c + 8 <= g.n) {
-      *(uint4*)at = x;
-    } else {
-      const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int j = 0; j < 8; j++)
-        if (c + j < g.n) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
-    }
+    const uint4 x = make_uint4(w[0], w[1], w[2], w[3]);
+    uint16_t* to = (uint16_t*)g.out + at;
+    if (g.vectors && have >= 8) *(uint4*)to = x;
+    else put_some(to, x, 0, have);
   }
 }
 
 // The same as planes; for GRAM and POLY on and above the diagonal, with
 // the mirror image strictly below it.
 template <Mode MODE>
-__device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int r0, int c0, const float* v, uint4* buf,
-                                             int lane) {
+__device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int r0, int c0, float* buf, int lane) {
   constexpr bool sym = MODE == GRAM || MODE == POLY;
-  const int sub = lane >> 3, k = lane & 7;
-  const size_t plane_size = (size_t)g.to.rows * g.to.ld;
-  uint32_t w[2][32];  // his, los of two columns each
-  if (MODE == POLY) {
-    float x[64];
+  const int o = (lane & 3) * 8, c = c0 + o;
+  const size_t plane = (size_t)g.to.rows * g.to.ld;
+#pragma unroll 1
+  for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
+    const int r = r0 + row;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 64; j++) x[j] = __fmul_rn(g.alpha, v[j]);
-    const __half* from = g.from.row(z, 0, r0 + sub) + c0 + 8 * k;
+    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[place(o + e, row)]);
+    if (MODE == POLY) {
+      const __half* from = g.from.row(z, 0, r) + c;
+      const uint4 x = *(const uint4*)from, y = *(const uint4*)(from + plane);
+      const __half2* h = (const __half2*)&x;
+      const __half2* l = (const __half2*)&y;
 #pragma unroll
-    for (int plane = 0; plane < 2; plane++) {
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (r0 + sub + 4 * i < g.m)
-          chunk(buf, 4 * i + sub, k) = *(const uint4*)(from + plane * plane_size + (size_t)(4 * i) * g.from.ld);
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const uint4 a = chunk(buf, lane, i);
-        const __half2* h = (const __half2*)&a;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 f = __half22float2(h[j]);
-          x[8 * i + 2 * j] = __fmaf_rn(g.beta, f.x, x[8 * i + 2 * j]);
-          x[8 * i + 2 * j + 1] = __fmaf_rn(g.beta, f.y, x[8 * i + 2 * j + 1]);
-        }
+      for (int e = 0; e < 4; e++) {
+        const float2 p = __half22float2(h[e]), q = __half22float2(l[e]);
+        v[2 * e] = __fmaf_rn(g.beta, __fadd_rn(p.x, q.x), v[2 * e]);
+        v[2 * e + 1] = __fmaf_rn(g.beta, __fadd_rn(p.y, q.y), v[2 * e + 1]);
       }
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (c + e == r) v[e] = __fadd_rn(v[e], g.diag);
     }
-    if (c0 < r0 + 32)
+    if (sym) {  // as the mirror image has them
 #pragma unroll
-      for (int j = 0; j < 64; j++)
-        if (c0 + j == r0 + lane) x[j] = __fadd_rn(x[j], g.diag);
-#pragma unroll
-    for (int j = 0; j < 32; j++) split2(x[2 * j], x[2 * j + 1], w[0][j], w[1][j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; j++)
-      split2(__fmul_rn(g.alpha, v[2 * j]), __fmul_rn(g.alpha, v[2 * j + 1]), w[0][j], w[1][j]);
-  }
-  __half* to = g.to.row(z, 0, r0 + sub) + c0 + 8 * k;
-#pragma unroll
-  for (int plane = 0; plane < 2; plane++) {  // rows are padded to 64 columns: whole vectors fit
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 8; j++) chunk(buf, lane, j) = make_uint4(w[plane][4 * j], w[plane][4 * j + 1], w[plane][4 * j + 2], w[plane][4 * j + 3]);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const uint4 x = chunk(buf, 4 * i + sub, k);
-      const int over = r0 + sub + 4 * i - (c0 + 8 * k);  // columns of the vector left of the diagonal
-      if (r0 + sub + 4 * i >= g.m) break;
-      __half* at = to + plane * plane_size + (size_t)(4 * i) * g.to.ld;
-      if (!sym || over <= 0) {
-        *(uint4*)at = x;
-      } else if (over < 8) {
-        const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-          if (j >= over) at[j] = __ushort_as_half((unsigned short)(e[j >> 1] >> ((j & 1) * 16)));
-      }
+      for (int e = 0; e < 8; e++) buf[place(o + e, row)] = v[e];
+    }
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    __half* to = g.to.row(z, 0, r) + c;  // rows are padded to 64 columns: whole vectors fit
+    const int left = sym ? r - c : 0;    // of the diagonal
+    if (left <= 0) {
+      *(uint4*)to = hi;
+      *(uint4*)(to + plane) = lo;
+    } else if (left < 8) {
+      put_some((uint16_t*)to, hi, left, 8);
+      put_some((uint16_t*)(to + plane), lo, left, 8);
     }
   }
-  if (!sym || c0 + 63 <= r0) return;
-  // Eight rows of one column per vector.
-  uint32_t* turn = (uint32_t*)buf;  // [32 column pairs][32 rows], groups of four rows exchanged
-  const int q = (lane & 3) * 2, r = r0 + q * 4;
-#pragma unroll
-  for (int plane = 0; plane < 2; plane++) {
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 32; j++) turn[j * 32 + (((lane >> 2) ^ (j & 7)) << 2) + (lane & 3)] = w[plane][j];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int j = i * 8 + (lane >> 2), c = c0 + 2 * j;
-      const uint4 x = *(const uint4*)&turn[j * 32 + ((q ^ (j & 7)) << 2)];
-      const uint4 y = *(const uint4*)&turn[j * 32 + (((q + 1) ^ (j & 7)) << 2)];
-      if (r >= g.m) continue;
-      __half* at = g.to.row(z, plane, c) + r;
-#pragma unroll
-      for (int b = 0; b < 2; b++) {  // column c, c + 1
-        const uint32_t pick = b ? 0x7632 : 0x5410;
-        const uint4 e = make_uint4(__byte_perm(x.x, x.y, pick), __byte_perm(x.z, x.w, pick), __byte_perm(y.x, y.y, pick),
-                                   __byte_perm(y.z, y.w, pick));
-        if (c + b >= g.n) continue;
-        const int below = c + b - r;  // rows of the vector above the diagonal
-        if (below >= 8) {
-          *(uint4*)(at + b * g.to.ld) = e;
-        } else {
-          const uint32_t f[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-          for (int u = 0; u < 8; u++)
-            if (u < below) at[b * g.to.ld + u] = __ushort_as_half((unsigned short)(f[u >> 1] >> ((u & 1) * 16)));
-        }
-      }
+  if (!sym || c0 + 31 <= r0) return;
+  __syncwarp();
+  const int r = r0 + o;  // eight rows of one column
+  if (r >= g.m) return;
+#pragma unroll 1
+  for (int col = lane >> 2; col < 32 && c0 + col < g.n; col += 8) {
+    const float4 x = *(const float4*)&buf[place(col, o)], y = *(const float4*)&buf[place(col, o + 4)];
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    __half* to = g.to.row(z, 0, c0 + col) + r;
+    const int above = c0 + col - r;
+    if (above >= 8) {
+      *(uint4*)to = hi;
+      *(uint4*)(to + plane) = lo;
+    } else if (above > 0) {
+      put_some((uint16_t*)to, hi, 0, above);
+      put_some((uint16_t*)(to + plane), lo, 0, above);
     }
   }
 }
 
-// Values of PART: per item and block of 32 x 64, [column][row].
+// Values of PART: per item and block, [column][row].
 __device__ __forceinline__ float* part_block(float* part, int64_t item, int block) {
   return part + (item * kTileBlocks + block) * kBlock;
 }
@@ -534,7 +492,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     grow_registers();
     const int part = warp & 3;               // the 32 TMEM lanes this warp may read
     const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
-    uint4* buf = (uint4*)(buffers + (warp - 4) * kBuffer);
+    float* buf = (float*)(buffers + (warp - 4) * kBuffer);
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     int64_t u = 0;  // sums so far
     for (int t = first; t < g.total && !fail; t += step) {
@@ -567,20 +525,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
       }
       if (fail) break;
       const int row = (int)rank * kSide + part * 32, r0 = at.row0 + row;
-#pragma unroll
-      for (int c = 0; c < kMine; c += 64) {
+#pragma unroll 1
+      for (int c = 0; c < kMine; c += 32) {
         const int c0 = at.col0 + col + c;
         // beyond the matrix, or below the diagonal: written by its mirror image
-        if (r0 >= g.m || c0 >= g.n || (symmetric && c0 + 63 < r0)) continue;
-        if (MODE == PART) {
-          float* p = part_block(g.part, t, row / 32 * (kTile / 64) + (col + c) / 64) + lane;
+        if (r0 < g.m && c0 < g.n && !(symmetric && c0 + 31 < r0)) {
+          if (MODE == PART) {
+            float* p = part_block(g.part, t, row / 32 * (kTile / 32) + (col + c) / 32) + lane;
 #pragma unroll
-          for (int j = 0; j < 64; j++) p[j * 32] = acc[c + j];
-        } else if (MODE == FINAL) {
-          write_final(g, at.z, r0, c0, acc + c, buf, lane);
-        } else {
-          write_planes<MODE>(g, at.z, r0, c0, acc + c, buf, lane);
+            for (int j = 0; j < 32; j++) p[j * 32] = acc[j];
+          } else {
+            block_in(buf, acc, lane);
+            if (MODE == FINAL) write_final(g, at.z, r0, c0, buf, lane);
+            else write_planes<MODE>(g, at.z, r0, c0, buf, lane);
+          }
         }
+#pragma unroll
+        for (int j = 0; j < kMine - 32; j++) acc[j] = acc[j + 32];
       }
     }
   }
@@ -594,28 +555,30 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
 }
 
 // Joins the parts of a symmetric product, always in the same order; a warp
-// takes a block of 32 x 64.
+// takes a block.
 constexpr int kJoinWarps = 4;
 template <Mode MODE>
 __global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const __grid_constant__ GemmArgs g) {
-  __shared__ uint4 buffers[kJoinWarps][kBuffer / 16];
+  __shared__ __align__(16) float buffers[kJoinWarps][kBlock];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + warp;
+  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + warp, item = id / kTileBlocks;
   const int block = (int)(id % kTileBlocks);
-  if (id / kTileBlocks >= g.total) return;
-  const Tile at(g, (int)(id / kTileBlocks), true);
-  const int r0 = at.row0 + block / (kTile / 64) * 32, c0 = at.col0 + block % (kTile / 64) * 64;
-  if (r0 >= g.m || c0 >= g.n || c0 + 63 < r0) return;
-  float v[64];
+  if (item >= g.total) return;
+  const Tile at(g, (int)item, true);
+  const int r0 = at.row0 + block / (kTile / 32) * 32, c0 = at.col0 + block % (kTile / 32) * 32;
+  if (r0 >= g.m || c0 >= g.n || c0 + 31 < r0) return;
+  float v[32];
 #pragma unroll
-  for (int j = 0; j < 64; j++) v[j] = 0;
+  for (int j = 0; j < 32; j++) v[j] = 0;
+#pragma unroll 2
   for (int s = 0; s < g.splits; s++) {
-    const float* p = part_block(g.part, id / kTileBlocks * g.splits + s, block) + lane;
+    const float* p = part_block(g.part, item * g.splits + s, block) + lane;
 #pragma unroll
-    for (int j = 0; j < 64; j++) v[j] = __fadd_rn(v[j], p[j * 32]);
+    for (int j = 0; j < 32; j++) v[j] = __fadd_rn(v[j], p[j * 32]);
   }
-  write_planes<MODE>(g, at.z, r0, c0, v, buffers[warp], lane);
+  block_in(buffers[warp], v, lane);
+  write_planes<MODE>(g, at.z, r0, c0, buffers[warp], lane);
 }
 
 // ------------------------------------------------------- norm and split
