@@ -13,10 +13,10 @@
 //
 // Both are bound by HBM: one write, or one read, per element of the bias,
 // against one table value or one addition.  What has to be kept small is the
-// work per element around that, above all finding its bucket: a thread owns
-// one 16-byte vector of a row, looks up its first and last distance, and
-// where they agree (nearly everywhere: buckets widen with distance)
-// the vector is one value; the lookup is shared by all heads.
+// work per element around that, above all finding its bucket: a row is
+// cut once into the two far ranges, which have one bucket each, and the near
+// columns between, whose buckets come from a table of distances in shared memory;
+// a thread owns one 16-byte vector, and in the bias its lookup serves all heads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -40,7 +40,8 @@ struct Buckets {
 };
 
 struct BiasArgs {
-  uint64_t queries, keys;
+  uint64_t queries;
+  int keys;
   int64_t first;
   int64_t rs, hs, bs;   // strides in elements
   int heads, nb;
@@ -48,31 +49,55 @@ struct BiasArgs {
   const int32_t* pos;
 };
 
-__device__ __forceinline__ int64_t query_position(const BiasArgs& a, uint64_t i) {
-  return a.pos ? (int64_t)a.pos[i] : a.first + (int64_t)i;
+// A row's columns: those up to `left` have the last bucket of the query's
+// side, those from `right` on one bucket as well (the last of the other side, or,
+// with one direction only, bucket 0), those from `end` on are masked or not there.
+// Between left and right the bucket depends on the distance, column - query,
+// which fits 32 bits there.
+struct Row {
+  int left, right, end, query;
+};
+
+__device__ __forceinline__ int clip(int64_t x, int lo, int hi) { return (int)(x < lo ? lo : x > hi ? hi : x); }
+
+__device__ __forceinline__ Row row_of(const Buckets& t, const BiasArgs& a, uint64_t i) {
+  const int64_t q = a.pos ? (int64_t)a.pos[i] : a.first + (int64_t)i;
+  Row r;
+  r.left = clip(q - t.last, -1, a.keys);
+  r.right = clip(q + (t.both && t.last > 1 ? t.last : 1), 0, a.keys);
+  r.end = t.causal ? clip(q + 1, 0, a.keys) : a.keys;
+  r.query = (int)q;
+  return r;
 }
 
-// Bucket of the distance d = key - query; `start` is in shared memory.
-__device__ __forceinline__ int bucket_of(const Buckets& t, const int* start, int64_t d) {
-  int base = 0;
-  int64_t n64 = -d;
-  if (t.both) {
-    if (d > 0) {
-      base = t.half;
-      n64 = d;
-    }
-  } else if (n64 < 0) {
-    n64 = 0;
-  }
-  if (n64 >= t.last) return base + t.half - 1;
-  const int n = (int)n64;
-  int lo = 0, hi = t.half;  // start[lo] <= n < start[hi]
+constexpr int kTable = 2048;  // distances whose bucket is looked up rather than searched
+
+// The bucket number of every near distance, in shared memory.
+struct Near {
+  uint8_t of[kTable];
+  int start[kMaxB];
+};
+
+__device__ __forceinline__ int search(const int* start, int half, int n) {
+  int lo = 0, hi = half;  // start[lo] <= n < start[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (start[mid] <= n) lo = mid;
     else hi = mid;
   }
-  return base + lo;
+  return lo;
+}
+
+// By all threads of the block; the caller synchronises.
+__device__ __forceinline__ void fill_near(Near& near, const Buckets& t, int threads) {
+  for (int i = threadIdx.x; i < t.half; i += threads) near.start[i] = t.start[i];
+  for (int n = threadIdx.x; n < kTable && n < t.last; n += threads) near.of[n] = (uint8_t)search(t.start, t.half, n);
+}
+
+// Bucket of a column between a row's left and right.
+__device__ __forceinline__ int near_bucket(const Near& near, const Buckets& t, const Row& r, int col) {
+  const int d = (int)((unsigned)col - (unsigned)r.query), n = d < 0 ? -d : d;
+  return (t.both && d > 0 ? t.half : 0) + (n < kTable ? near.of[n] : search(near.start, t.half, n));
 }
 
 template <class T> __device__ __forceinline__ T minus_infinity();
@@ -96,85 +121,70 @@ template <class T> struct alignas(16) Vec {
   T e[N];
 };
 
-// Whether a vector of N distances from d0 on lies in one bucket (then
-// *which), the masked ones counting as bucket nb (the table's -inf row).
-template <int N>
-__device__ __forceinline__ bool one_bucket(const Buckets& t, const int* start, int nb, int64_t d0, int* which) {
-  if (t.causal && d0 > 0) {
-    *which = nb;
-    return true;
-  }
-  const int a = bucket_of(t, start, d0);
-  *which = a;
-  if (N == 1) return true;
-  const int64_t d1 = d0 + N - 1;
-  if (t.causal && d1 > 0) return false;
-  // The two directions are two runs of buckets: a vector that crosses
-  // distance 0 is never one bucket, unless each direction has only one and
-  // only the query side counts.
-  if (t.both && d0 <= 0 && d1 > 0) return false;
-  return a == bucket_of(t, start, d1);
-}
-
-__device__ __forceinline__ int bucket_or_masked(const Buckets& t, const int* start, int nb, int64_t d) {
-  return t.causal && d > 0 ? nb : bucket_of(t, start, d);
-}
-
 // ---------------------------------------------------------------- bias
 
 constexpr int kFwdThreads = 256;
 
 // A thread owns one 16-byte vector of a row and writes it for `hc` heads.
 // Rows need not be aligned: vectors sit on 16-byte addresses, the ones at a
-// row's ends are written element by element.
+// row's ends are written element by element.  Masked columns read the
+// table's row nb, which holds -inf.
 template <class T, class S>
 __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a,
                                                            const S* __restrict__ table, T* __restrict__ out, int hc,
-                                                           uint64_t vecs, uint64_t items) {
+                                                           uint32_t vecs, uint64_t items) {
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ Near near;
   T* tab = (T*)smem;                       // [hc][nb + 1]
   const int pitch = a.nb + 1;
-  int* start = (int*)(smem + (((size_t)hc * pitch * sizeof(T) + 15) & ~(size_t)15));
   const int h0 = blockIdx.y * hc;
   const int hn = min(hc, a.heads - h0);
-  for (int i = threadIdx.x; i < t.half; i += kFwdThreads) start[i] = t.start[i];
+  fill_near(near, t, kFwdThreads);
   for (int i = threadIdx.x; i < a.nb * hn; i += kFwdThreads) {
     const int v = i / hn, h = i - v * hn;
     tab[h * pitch + v] = cast<T, S>(table[(size_t)v * a.heads + h0 + h]);
   }
   for (int h = threadIdx.x; h < hn; h += kFwdThreads) tab[h * pitch + a.nb] = minus_infinity<T>();
   __syncthreads();
+  const int far_left = t.half - 1, far_right = t.both ? 2 * t.half - 1 : 0;
 
   for (uint64_t item = (uint64_t)blockIdx.x * kFwdThreads + threadIdx.x; item < items;
        item += (uint64_t)gridDim.x * kFwdThreads) {
-    uint64_t row, v;
-    if (items < (1ull << 32)) {
-      row = (uint32_t)item / (uint32_t)vecs;
-      v = (uint32_t)item - (uint32_t)row * (uint32_t)vecs;
-    } else {
-      row = item / vecs;
-      v = item - row * vecs;
-    }
-    const int64_t q = query_position(a, row);
-    int shift = -1;          // elements of the row before its first 16-byte boundary's vector
+    uint64_t row;
+    if (items < (1ull << 32)) row = (uint32_t)item / vecs;
+    else row = item / vecs;
+    const int v = (int)(item - row * vecs);
+    const Row r = row_of(t, a, row);
+    T* line = out + (int64_t)h0 * a.hs + (int64_t)row * a.rs;
+    int shift = -1;          // elements by which this head's rows lie behind a 16-byte boundary
     int which[N];
-    bool one = false;
-    int64_t c0 = 0;
-    for (int h = 0; h < hn; h++) {
-      T* line = out + (int64_t)(h0 + h) * a.hs + (int64_t)row * a.rs;
+    bool one = false, whole = false;
+    int c0 = 0;
+    for (int h = 0; h < hn; h++, line += a.hs) {
       const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
       if (s != shift) {      // the first head, or rows of another alignment
         shift = s;
-        c0 = (int64_t)v * N - s;
-        one = one_bucket<N>(t, start, a.nb, c0 - q, &which[0]);
+        c0 = v * N - s;
+        whole = c0 >= 0 && c0 + N <= a.keys;
+        one = true;
+        if (c0 >= r.end) which[0] = a.nb;
+        else if (c0 + N - 1 <= r.left) which[0] = far_left;
+        else if (c0 >= r.right && c0 + N <= r.end) which[0] = far_right;
+        else one = false;
         if (!one) {
+          bool same = true;
 #pragma unroll
-          for (int k = 0; k < N; k++) which[k] = bucket_or_masked(t, start, a.nb, c0 + k - q);
+          for (int k = 0; k < N; k++) {
+            const int c = c0 + k;
+            which[k] = c >= r.end ? a.nb : c <= r.left ? far_left : c >= r.right ? far_right : near_bucket(near, t, r, c);
+            same = same && which[k] == which[0];
+          }
+          one = same;
         }
       }
-      if (c0 >= (int64_t)a.keys) continue;
+      if (c0 >= a.keys) continue;
       const T* ht = tab + h * pitch;
       Vec<T> x;
       if (one) {
@@ -185,12 +195,12 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
 #pragma unroll
         for (int k = 0; k < N; k++) x.e[k] = ht[which[k]];
       }
-      if (c0 >= 0 && c0 + N <= (int64_t)a.keys) {
+      if (whole) {
         *(uint4*)(line + c0) = *(const uint4*)&x;
       } else {
 #pragma unroll
         for (int k = 0; k < N; k++)
-          if (c0 + k >= 0 && c0 + k < (int64_t)a.keys) line[c0 + k] = x.e[k];
+          if (c0 + k >= 0 && c0 + k < a.keys) line[c0 + k] = x.e[k];
       }
     }
   }
@@ -207,7 +217,7 @@ __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162floa
 
 constexpr int kRows = 4;            // rows of a warp's tile
 constexpr uint64_t kBatchTile = 8;  // batch entries of a tile
-constexpr size_t kAccBytes = 64 << 10;
+constexpr size_t kAccBytes = 48 << 10;
 
 // How the gradient is split: `splits` CTAs per head, each with `warps`
 // warps, every warp taking tiles (kRows rows x 32 vectors x kBatchTile batch
@@ -236,93 +246,103 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) bias_grad_kernel(const __grid_constant__ Buckets t,
-                                                        const __grid_constant__ BiasArgs a, const T* __restrict__ g,
-                                                        const __grid_constant__ GradPlan p,
-                                                        typename AccOf<T>::type* __restrict__ part,
-                                                        typename AccOf<T>::type* __restrict__ dtable, int add) {
+__global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant__ Buckets t,
+                                                           const __grid_constant__ BiasArgs a, const T* __restrict__ g,
+                                                           const __grid_constant__ GradPlan p,
+                                                           typename AccOf<T>::type* __restrict__ part,
+                                                           typename AccOf<T>::type* __restrict__ dtable, int add) {
   using A = typename AccOf<T>::type;
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) uint8_t smem[];
   A* acc = (A*)smem;   // [warp][bucket][lane]: every lane adds into its own column, in its own order
-  __shared__ int start[kMaxB];
+  __shared__ Near near;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int threads = p.warps * 32;
-  for (int i = threadIdx.x; i < t.half; i += threads) start[i] = t.start[i];
+  fill_near(near, t, threads);
   for (int i = threadIdx.x; i < p.warps * a.nb * 32; i += threads) acc[i] = 0;
   __syncthreads();
   A* mine = acc + (size_t)warp * a.nb * 32 + lane;
 
   const int h = blockIdx.y;
   const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
-  int cur = 0;        // the bucket that `sum` belongs to
-  A sum = 0;
-  auto into = [&](int v, A x) {
-    if (v != cur) {
-      mine[cur * 32] += sum;
-      cur = v;
-      sum = 0;
-    }
-    sum += x;
-  };
+  int cur = 0;                      // the bucket that `sum` belongs to
+  A sum = 0, far_left = 0, far_right = 0;
   for (uint64_t tile = (uint64_t)blockIdx.x * p.warps + warp; tile < tiles; tile += (uint64_t)gridDim.x * p.warps) {
-    const uint64_t tv = tile % p.tiles_v, rest = tile / p.tiles_v;
-    const uint64_t r0 = (rest % p.tiles_r) * kRows, b0 = (rest / p.tiles_r) * kBatchTile;
-    const uint64_t v = tv * 32 + lane;
+    uint32_t tv;
+    uint64_t rest;
+    if (tiles < (1ull << 32)) rest = (uint32_t)tile / (uint32_t)p.tiles_v;
+    else rest = tile / p.tiles_v;
+    tv = (uint32_t)(tile - rest * p.tiles_v);
+    const uint64_t tb = p.tiles_b == 1 ? 0 : rest / p.tiles_r;
+    const uint64_t r0 = (rest - tb * p.tiles_r) * kRows, b0 = tb * kBatchTile;
+    const int v = (int)(tv * 32 + lane);
     const uint64_t b1 = min(a.batch, b0 + kBatchTile);
-    for (uint64_t b = b0; b < b1; b++) {
-      const T* head = g + (int64_t)b * a.bs + (int64_t)h * a.hs;
+    Row rows[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; r++) {
+      rows[r].end = 0;              // no row there: nothing is read
+      if (r0 + r < a.queries) rows[r] = row_of(t, a, r0 + r);
+    }
+    const T* line = g + (int64_t)b0 * a.bs + (int64_t)h * a.hs + (int64_t)r0 * a.rs;
+    for (uint64_t b = b0; b < b1; b++, line += a.bs) {
       Vec<T> x[kRows];
-      int64_t c0[kRows], q[kRows];
+      int c0[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
-        const uint64_t row = r0 + r;
-        c0[r] = (int64_t)a.keys;
-        q[r] = 0;
-        if (row < a.queries) {
-          q[r] = query_position(a, row);
-          const T* line = head + (int64_t)row * a.rs;
-          const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
-          int64_t c = (int64_t)v * N - s;
-          // A vector whose keys all come after the query is not read.
-          if (t.causal && max(c, (int64_t)0) > q[r]) c = (int64_t)a.keys;
-          c0[r] = c;
-          if (c >= 0 && c + N <= (int64_t)a.keys) {
-            *(uint4*)&x[r] = __ldg((const uint4*)(line + c));
-          } else {
+        const T* at = line + r * a.rs;
+        const int c = v * N - (int)(((uintptr_t)at / sizeof(T)) % N);
+        c0[r] = c;
+        if (c >= rows[r].end) continue;   // past the row, or masked: not read
+        if (c >= 0 && c + N <= a.keys) {
+          *(uint4*)&x[r] = __ldg((const uint4*)(at + c));
+        } else {
 #pragma unroll
-            for (int k = 0; k < N; k++)
-              if (c + k >= 0 && c + k < (int64_t)a.keys) x[r].e[k] = line[c + k];
-          }
+          for (int k = 0; k < N; k++)
+            if (c + k >= 0 && c + k < a.keys) x[r].e[k] = at[c + k];
         }
       }
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
-        if (c0[r] >= (int64_t)a.keys) continue;
-        const int64_t d0 = c0[r] - q[r];
-        int which;
-        const bool whole = c0[r] >= 0 && c0[r] + N <= (int64_t)a.keys;
-        if (whole && one_bucket<N>(t, start, a.nb, d0, &which)) {
+        const Row& w = rows[r];
+        const int c = c0[r];
+        if (c >= w.end) continue;
+        const bool left = c >= 0 && c + N - 1 <= w.left && c + N <= w.end;
+        if (left || (c >= 0 && c >= w.right && c + N <= w.end)) {
           A s[N];
 #pragma unroll
           for (int k = 0; k < N; k++) s[k] = widen(x[r].e[k]);
 #pragma unroll
-          for (int w = N / 2; w > 0; w >>= 1)
+          for (int u = N / 2; u > 0; u >>= 1)
 #pragma unroll
-            for (int k = 0; k < w; k++) s[k] += s[k + w];
-          into(which, s[0]);
+            for (int k = 0; k < u; k++) s[k] += s[k + u];
+          far_left += left ? s[0] : 0;
+          far_right += left ? 0 : s[0];
         } else {
 #pragma unroll
           for (int k = 0; k < N; k++) {
-            const int64_t c = c0[r] + k;
-            if (c < 0 || c >= (int64_t)a.keys || (t.causal && d0 + k > 0)) continue;
-            into(bucket_of(t, start, d0 + k), widen(x[r].e[k]));
+            if (c + k < 0 || c + k >= w.end) continue;
+            const A e = widen(x[r].e[k]);
+            if (c + k <= w.left) {
+              far_left += e;
+            } else if (c + k >= w.right) {
+              far_right += e;
+            } else {
+              const int bucket = near_bucket(near, t, w, c + k);
+              if (bucket != cur) {
+                mine[cur * 32] += sum;
+                cur = bucket;
+                sum = 0;
+              }
+              sum += e;
+            }
           }
         }
       }
     }
   }
   mine[cur * 32] += sum;
+  mine[(t.half - 1) * 32] += far_left;
+  mine[(t.both ? 2 * t.half - 1 : 0) * 32] += far_right;
   __syncthreads();
   for (int v = warp; v < a.nb; v += p.warps) {
     A s = 0;
@@ -418,7 +438,7 @@ Buckets buckets_of(const dcf_bias_desc& d) {
 BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
   BiasArgs a;
   a.queries = d.queries;
-  a.keys = d.keys;
+  a.keys = (int)d.keys;
   a.first = d.first_query;
   a.rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
   a.hs = d.head_stride ? d.head_stride : (int64_t)d.queries * a.rs;
@@ -446,9 +466,9 @@ int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos,
   uint64_t groups = (d.heads + hc - 1) / hc;
   hc = (d.heads + groups - 1) / groups;
   groups = (d.heads + hc - 1) / hc;
-  const size_t smem = ((hc * (d.num_buckets + 1) * sizeof(T) + 15) & ~(size_t)15) + (size_t)t.half * 4;
+  const size_t smem = hc * (d.num_buckets + 1) * sizeof(T);
   const dim3 grid((unsigned)(blocks < (1u << 30) ? blocks : (1u << 30)), (unsigned)groups);
-  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, vecs, items);
+  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, (uint32_t)vecs, items);
   note_launch();
   return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
@@ -462,8 +482,8 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
   const GradPlan p = grad_plan(d);
   const int add = (d.flags & DCF_BIAS_ACCUMULATE) != 0;
   const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A);
-  if (cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAccBytes) !=
-      cudaSuccess)
+  if (smem > kAccBytes - 4096 &&
+      cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10) != cudaSuccess)
     return DCF_ECUDA;
   bias_grad_kernel<T><<<dim3((unsigned)p.splits, d.heads), p.warps * 32, smem, stream>>>(
       t, a, (const T*)g, p, (A*)ws, (A*)dtable, add);
@@ -497,8 +517,8 @@ int bias_desc_check(const dcf_bias_desc* d, bool grad) {
     return bad("position bias: max_distance must be above the exact buckets and below 2^31");
   if (d->heads > 65535) return bad("position bias: at most 65535 heads");
   const uint64_t lim = 1ull << 31;
-  if (d->queries >= lim || d->keys >= lim || (grad && d->batch >= lim))
-    return bad("position bias: queries, keys and batch must be below 2^31");
+  if (d->queries >= lim || d->keys >= lim - 64 || (grad && d->batch >= lim))
+    return bad("position bias: queries and batch must be below 2^31, keys below 2^31 - 64");
   if (d->first_query > (1ll << 40) || d->first_query < -(1ll << 40)) return bad("position bias: first_query out of range");
   if (d->row_stride < 0 || d->head_stride < 0 || d->batch_stride < 0) return bad("position bias: negative stride");
   // Extents in 128 bits, so that no product of the checks wraps.
