@@ -215,7 +215,7 @@ __device__ __forceinline__ double widen(double x) { return x; }
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-constexpr int kRows = 4;            // rows of a warp's tile
+constexpr int kRows = 4;            // rows of a warp's tile (their four loads are in flight together)
 constexpr uint64_t kBatchTile = 8;  // batch entries of a tile
 constexpr size_t kAccBytes = 48 << 10;
 
@@ -265,14 +265,15 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
 
   const int h = blockIdx.y;
   const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
-  int cur = 0;                      // the bucket that `sum` belongs to
-  A sum = 0, far_left = 0, far_right = 0;
+  A far_left = 0, far_right = 0;
   for (uint64_t tile = (uint64_t)blockIdx.x * p.warps + warp; tile < tiles; tile += (uint64_t)gridDim.x * p.warps) {
     uint32_t tv;
     uint64_t rest;
     if (tiles < (1ull << 32)) rest = (uint32_t)tile / (uint32_t)p.tiles_v;
     else rest = tile / p.tiles_v;
-    tv = (uint32_t)(tile - rest * p.tiles_v);
+    // Turned by one per row of tiles: a warp's step through the tiles then does not
+    // keep it at the same columns, of which some are near and some masked.
+    tv = (uint32_t)((tile - rest * p.tiles_v + rest) % p.tiles_v);
     const uint64_t tb = p.tiles_b == 1 ? 0 : rest / p.tiles_r;
     const uint64_t r0 = (rest - tb * p.tiles_r) * kRows, b0 = tb * kBatchTile;
     const int v = (int)(tv * 32 + lane);
@@ -285,29 +286,23 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
     }
     const T* line = g + (int64_t)b0 * a.bs + (int64_t)h * a.hs + (int64_t)r0 * a.rs;
     for (uint64_t b = b0; b < b1; b++, line += a.bs) {
+      // Vectors that lie wholly in a far range; the others are noted.
       Vec<T> x[kRows];
       int c0[kRows];
+      unsigned slow[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
         const T* at = line + r * a.rs;
-        const int c = v * N - (int)(((uintptr_t)at / sizeof(T)) % N);
-        c0[r] = c;
-        if (c >= rows[r].end) continue;   // past the row, or masked: not read
-        if (c >= 0 && c + N <= a.keys) {
-          *(uint4*)&x[r] = __ldg((const uint4*)(at + c));
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; k++)
-            if (c + k >= 0 && c + k < a.keys) x[r].e[k] = at[c + k];
-        }
+        c0[r] = v * N - (int)(((uintptr_t)at / sizeof(T)) % N);
+        if (c0[r] >= 0 && c0[r] < rows[r].end && c0[r] + N <= a.keys) *(uint4*)&x[r] = __ldg((const uint4*)(at + c0[r]));
       }
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
         const Row& w = rows[r];
         const int c = c0[r];
-        if (c >= w.end) continue;
-        const bool left = c >= 0 && c + N - 1 <= w.left && c + N <= w.end;
-        if (left || (c >= 0 && c >= w.right && c + N <= w.end)) {
+        const bool whole = c >= 0 && c + N <= w.end;
+        const bool left = whole && c + N - 1 <= w.left, right = whole && c >= w.right;
+        if (left || right) {
           A s[N];
 #pragma unroll
           for (int k = 0; k < N; k++) s[k] = widen(x[r].e[k]);
@@ -315,32 +310,36 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
           for (int u = N / 2; u > 0; u >>= 1)
 #pragma unroll
             for (int k = 0; k < u; k++) s[k] += s[k + u];
-          far_left += left ? s[0] : 0;
-          far_right += left ? 0 : s[0];
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; k++) {
-            if (c + k < 0 || c + k >= w.end) continue;
-            const A e = widen(x[r].e[k]);
-            if (c + k <= w.left) {
-              far_left += e;
-            } else if (c + k >= w.right) {
-              far_right += e;
-            } else {
-              const int bucket = near_bucket(near, t, w, c + k);
-              if (bucket != cur) {
-                mine[cur * 32] += sum;
-                cur = bucket;
-                sum = 0;
-              }
-              sum += e;
-            }
-          }
+          if (left) far_left += s[0];
+          else far_right += s[0];
+        }
+        slow[r] = __ballot_sync(0xFFFFFFFFu, max(c, 0) < w.end && !left && !right);
+      }
+      // Their elements, one to a lane: near ones each into its bucket.  (One copy
+      // of this code: unrolled over rows and vectors, fetching it took longer than
+      // running it.)
+#pragma unroll 1
+      for (int r = 0; r < kRows; r++) {
+        unsigned todo = r == 0 ? slow[0] : r == 1 ? slow[1] : r == 2 ? slow[2] : slow[3];
+        if (!todo) continue;
+        const Row w = row_of(t, a, r0 + r);
+        const T* at = line + r * a.rs;
+        const int base = (int)tv * 32 * N - (int)(((uintptr_t)at / sizeof(T)) % N);
+#pragma unroll 1
+        while (todo) {
+          const int first = __ffs(todo) - 1, vec = first + lane / N, c = base + first * N + lane;
+          const bool here = vec < 32 && (todo >> (vec & 31) & 1) && c >= 0 && c < w.end;
+          const unsigned upto = first + 32 / N;
+          todo = upto < 32 ? todo >> upto << upto : 0;
+          if (!here) continue;
+          const A e = widen(__ldg(at + c));
+          if (c <= w.left) far_left += e;
+          else if (c >= w.right) far_right += e;
+          else mine[near_bucket(near, t, w, c) * 32] += e;
         }
       }
     }
   }
-  mine[cur * 32] += sum;
   mine[(t.half - 1) * 32] += far_left;
   mine[(t.both ? 2 * t.half - 1 : 0) * 32] += far_right;
   __syncthreads();
