@@ -133,7 +133,7 @@ template <class T, class S>
 __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a,
                                                            const S* __restrict__ table, T* __restrict__ out, int hc,
-                                                           uint32_t vecs, uint64_t items) {
+                                                           int aligned, uint32_t vecs, uint64_t items) {
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Near near;
@@ -158,44 +158,63 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
     const int v = (int)(item - row * vecs);
     const Row r = row_of(t, a, row);
     T* line = out + (int64_t)h0 * a.hs + (int64_t)row * a.rs;
-    int shift = -1;          // elements by which this head's rows lie behind a 16-byte boundary
-    int which[N];
-    bool one = false, whole = false;
-    int c0 = 0;
+    int which[N];            // the bucket of each of the vector's columns
+    bool one;                // whether it is one for all
+#define LOOK_UP(c0)                                                                                                      \
+  which[0] = (c0) >= r.end ? a.nb : (c0) + N - 1 <= r.left ? far_left : far_right;                                       \
+  one = (c0) >= r.end || (c0) + N - 1 <= r.left || ((c0) >= r.right && (c0) + N <= r.end);                               \
+  if (!one) {                                                                                                            \
+    _Pragma("unroll") for (int k = 0; k < N; k++) {                                                                      \
+      const int c = (c0) + k;                                                                                            \
+      which[k] = c >= r.end ? a.nb : c <= r.left ? far_left : c >= r.right ? far_right : near_bucket(near, t, r, c);     \
+    }                                                                                                                    \
+  }
+    if (aligned) {           // every head's rows start on a 16-byte boundary: one lookup serves all
+      const int c0 = v * N;
+      LOOK_UP(c0)
+      line += c0;
+      if (c0 + N > a.keys) {
+        for (int h = 0; h < hn; h++, line += a.hs)
+#pragma unroll
+          for (int k = 0; k < N; k++)
+            if (c0 + k < a.keys) line[k] = tab[h * pitch + (one ? which[0] : which[k])];
+      } else if (one) {
+        const T* ht = tab + which[0];
+#pragma unroll 4
+        for (int h = 0; h < hn; h++, line += a.hs, ht += pitch) {
+          const T e = *ht;
+          Vec<T> x;
+#pragma unroll
+          for (int k = 0; k < N; k++) x.e[k] = e;
+          *(uint4*)line = *(const uint4*)&x;
+        }
+      } else {
+        const T* ht = tab;
+#pragma unroll 2
+        for (int h = 0; h < hn; h++, line += a.hs, ht += pitch) {
+          Vec<T> x;
+#pragma unroll
+          for (int k = 0; k < N; k++) x.e[k] = ht[which[k]];
+          *(uint4*)line = *(const uint4*)&x;
+        }
+      }
+      continue;
+    }
+    int shift = -1, c0 = 0;  // elements by which this head's rows lie behind a 16-byte boundary
+    one = false;
     for (int h = 0; h < hn; h++, line += a.hs) {
       const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
-      if (s != shift) {      // the first head, or rows of another alignment
+      if (s != shift) {
         shift = s;
         c0 = v * N - s;
-        whole = c0 >= 0 && c0 + N <= a.keys;
-        one = true;
-        if (c0 >= r.end) which[0] = a.nb;
-        else if (c0 + N - 1 <= r.left) which[0] = far_left;
-        else if (c0 >= r.right && c0 + N <= r.end) which[0] = far_right;
-        else one = false;
-        if (!one) {
-          bool same = true;
-#pragma unroll
-          for (int k = 0; k < N; k++) {
-            const int c = c0 + k;
-            which[k] = c >= r.end ? a.nb : c <= r.left ? far_left : c >= r.right ? far_right : near_bucket(near, t, r, c);
-            same = same && which[k] == which[0];
-          }
-          one = same;
-        }
+        LOOK_UP(c0)
       }
       if (c0 >= a.keys) continue;
       const T* ht = tab + h * pitch;
       Vec<T> x;
-      if (one) {
-        const T e = ht[which[0]];
 #pragma unroll
-        for (int k = 0; k < N; k++) x.e[k] = e;
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; k++) x.e[k] = ht[which[k]];
-      }
-      if (whole) {
+      for (int k = 0; k < N; k++) x.e[k] = ht[one ? which[0] : which[k]];
+      if (c0 >= 0 && c0 + N <= a.keys) {
         *(uint4*)(line + c0) = *(const uint4*)&x;
       } else {
 #pragma unroll
@@ -203,6 +222,7 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
           if (c0 + k >= 0 && c0 + k < a.keys) line[c0 + k] = x.e[k];
       }
     }
+#undef LOOK_UP
   }
 }
 
@@ -216,16 +236,40 @@ __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 constexpr int kRows = 4;            // rows of a warp's tile (their four loads are in flight together)
-constexpr uint64_t kBatchTile = 8;  // batch entries of a tile
 constexpr size_t kAccBytes = 48 << 10;
 
+BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
+  BiasArgs a;
+  a.queries = d.queries;
+  a.keys = (int)d.keys;
+  a.first = d.first_query;
+  a.rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
+  a.hs = d.head_stride ? d.head_stride : (int64_t)d.queries * a.rs;
+  a.bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * a.hs;
+  a.heads = (int)d.heads;
+  a.nb = (int)d.num_buckets;
+  a.batch = d.batch;
+  a.pos = pos;
+  return a;
+}
+
 // How the gradient is split: `splits` CTAs per head, each with `warps`
-// warps, every warp taking tiles (kRows rows x 32 vectors x kBatchTile batch
-// entries) in turn.  Fixed by the sizes alone, so sums keep their order.
+// warps, every warp taking items (four rows of one batch entry x `chunk` times
+// 32 vectors) in turn.  Fixed by the sizes and strides alone, so sums keep
+// their order.
 struct GradPlan {
   int warps, splits;
-  uint64_t vecs, tiles_v, tiles_r, tiles_b;
+  uint32_t tiles_v, chunk, chunks;
+  uint64_t items;
 };
+
+// Vectors that a row of `keys` elements can touch: one more where rows need
+// not start on a 16-byte boundary.
+uint64_t vectors_of_row(uint64_t keys, uint64_t n, bool aligned) { return (keys + (aligned ? n - 1 : 2 * n - 2)) / n; }
+
+bool strides_aligned(const BiasArgs& a, uint64_t n) {
+  return a.rs % (int64_t)n == 0 && a.hs % (int64_t)n == 0 && a.bs % (int64_t)n == 0;
+}
 
 GradPlan grad_plan(const dcf_bias_desc& d) {
   GradPlan p;
@@ -233,20 +277,25 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
   const uint64_t n = 16 / es;
   p.warps = (int)(kAccBytes / (d.num_buckets * 32 * acc));
   p.warps = p.warps > 8 ? 8 : p.warps < 1 ? 1 : p.warps;
-  p.vecs = d.keys ? (d.keys + 2 * n - 2) / n : 0;
-  p.tiles_v = (p.vecs + 31) / 32;
-  p.tiles_r = (d.queries + kRows - 1) / kRows;
-  p.tiles_b = (d.batch + kBatchTile - 1) / kBatchTile;
-  const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
-  const uint64_t most = (tiles + p.warps - 1) / p.warps;
-  uint64_t want = d.heads ? (uint64_t)(kSms * 4 + d.heads - 1) / d.heads : 1;
-  if (want > most) want = most;
+  p.tiles_v = d.keys ? (uint32_t)((vectors_of_row(d.keys, n, false) + 31) / 32) : 0;
+  const uint64_t groups = (d.queries + kRows - 1) / kRows * d.batch;
+  const uint64_t ctas = d.heads ? (uint64_t)(kSms * 3 + d.heads - 1) / d.heads : 1;  // per head: three to an SM
+  const uint64_t slots = ctas * p.warps;
+  // Whole rows where there are enough of them for every warp, else parts.
+  uint64_t cuts = groups ? slots / groups : 1;
+  cuts = cuts < 1 ? 1 : cuts > p.tiles_v ? p.tiles_v : cuts;
+  p.chunk = cuts ? (uint32_t)((p.tiles_v + cuts - 1) / cuts) : 1;
+  p.chunks = p.chunk ? (p.tiles_v + p.chunk - 1) / p.chunk : 0;
+  p.items = groups * p.chunks;
+  // As few CTAs as take no more turns than the most would.
+  const uint64_t turns = (p.items + slots - 1) / slots;
+  const uint64_t want = turns ? (p.items + turns * p.warps - 1) / (turns * p.warps) : 1;
   p.splits = (int)(want < 1 ? 1 : want);
   return p;
 }
 
 template <class T>
-__global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant__ Buckets t,
+__global__ void __launch_bounds__(256, 3) bias_grad_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a, const T* __restrict__ g,
                                                            const __grid_constant__ GradPlan p,
                                                            typename AccOf<T>::type* __restrict__ part,
@@ -264,45 +313,58 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
   A* mine = acc + (size_t)warp * a.nb * 32 + lane;
 
   const int h = blockIdx.y;
-  const uint64_t tiles = p.tiles_v * p.tiles_r * p.tiles_b;
   A far_left = 0, far_right = 0;
-  for (uint64_t tile = (uint64_t)blockIdx.x * p.warps + warp; tile < tiles; tile += (uint64_t)gridDim.x * p.warps) {
-    uint32_t tv;
-    uint64_t rest;
-    if (tiles < (1ull << 32)) rest = (uint32_t)tile / (uint32_t)p.tiles_v;
-    else rest = tile / p.tiles_v;
-    // Turned by one per row of tiles: a warp's step through the tiles then does not
-    // keep it at the same columns, of which some are near and some masked.
-    tv = (uint32_t)((tile - rest * p.tiles_v + rest) % p.tiles_v);
-    const uint64_t tb = p.tiles_b == 1 ? 0 : rest / p.tiles_r;
-    const uint64_t r0 = (rest - tb * p.tiles_r) * kRows, b0 = tb * kBatchTile;
-    const int v = (int)(tv * 32 + lane);
-    const uint64_t b1 = min(a.batch, b0 + kBatchTile);
-    Row rows[kRows];
+  const uint64_t warps = (uint64_t)gridDim.x * p.warps, self = (uint64_t)blockIdx.x * p.warps + warp;
+  for (uint64_t turn = 0; turn * warps < p.items; turn++) {
+    // Forth and back: with a causal mask later rows are longer.
+    const uint64_t item = turn * warps + (turn & 1 ? warps - 1 - self : self);
+    if (item >= p.items) continue;
+    uint64_t group, b;
+    uint32_t part_v;
+    if (p.items < (1ull << 32)) {
+      group = (uint32_t)item / p.chunks;
+      part_v = (uint32_t)item - (uint32_t)group * p.chunks;
+      const uint32_t batch = (uint32_t)a.batch, g4 = (uint32_t)group / batch;
+      b = (uint32_t)group - g4 * batch;
+      group = g4;
+    } else {
+      group = item / p.chunks;
+      part_v = (uint32_t)(item - group * p.chunks);
+      b = group % a.batch;
+      group /= a.batch;
+    }
+    const uint64_t r0 = group * kRows;
+    Row own = {-1, 0, 0, 0};        // of row r0 + lane; no row there: nothing is read
+    if (lane < kRows && r0 + lane < a.queries) own = row_of(t, a, r0 + lane);
+    const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)r0 * a.rs;
+    int left[kRows], right[kRows], end[kRows], shift[kRows];
+    int reach = 0;
 #pragma unroll
     for (int r = 0; r < kRows; r++) {
-      rows[r].end = 0;              // no row there: nothing is read
-      if (r0 + r < a.queries) rows[r] = row_of(t, a, r0 + r);
+      left[r] = __shfl_sync(0xFFFFFFFFu, own.left, r);
+      right[r] = __shfl_sync(0xFFFFFFFFu, own.right, r);
+      end[r] = __shfl_sync(0xFFFFFFFFu, own.end, r);
+      // elements by which the row lies behind a 16-byte boundary
+      shift[r] = (int)(((uintptr_t)(line + r * a.rs) / sizeof(T)) % N);
+      reach = max(reach, end[r]);
     }
-    const T* line = g + (int64_t)b0 * a.bs + (int64_t)h * a.hs + (int64_t)r0 * a.rs;
-    for (uint64_t b = b0; b < b1; b++, line += a.bs) {
+    const uint32_t last = min(p.tiles_v, (part_v + 1) * p.chunk);
+    for (uint32_t tv = part_v * p.chunk; tv < last && (int)tv * 32 * N - (N - 1) < reach; tv++) {
+      const int v0 = (int)(tv * 32 + lane) * N;
       // Vectors that lie wholly in a far range; the others are noted.
       Vec<T> x[kRows];
-      int c0[kRows];
       unsigned slow[kRows];
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
-        const T* at = line + r * a.rs;
-        c0[r] = v * N - (int)(((uintptr_t)at / sizeof(T)) % N);
-        if (c0[r] >= 0 && c0[r] < rows[r].end && c0[r] + N <= a.keys) *(uint4*)&x[r] = __ldg((const uint4*)(at + c0[r]));
+        const int c = v0 - shift[r];
+        if (c >= 0 && c < end[r] && c + N <= a.keys) *(uint4*)&x[r] = __ldg((const uint4*)(line + r * a.rs + c));
       }
 #pragma unroll
       for (int r = 0; r < kRows; r++) {
-        const Row& w = rows[r];
-        const int c = c0[r];
-        const bool whole = c >= 0 && c + N <= w.end;
-        const bool left = whole && c + N - 1 <= w.left, right = whole && c >= w.right;
-        if (left || right) {
+        const int c = v0 - shift[r];
+        const bool whole = c >= 0 && c + N <= end[r];
+        const bool is_left = whole && c + N - 1 <= left[r], is_right = whole && c >= right[r];
+        if (is_left || is_right) {
           A s[N];
 #pragma unroll
           for (int k = 0; k < N; k++) s[k] = widen(x[r].e[k]);
@@ -310,10 +372,10 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
           for (int u = N / 2; u > 0; u >>= 1)
 #pragma unroll
             for (int k = 0; k < u; k++) s[k] += s[k + u];
-          if (left) far_left += s[0];
+          if (is_left) far_left += s[0];
           else far_right += s[0];
         }
-        slow[r] = __ballot_sync(0xFFFFFFFFu, max(c, 0) < w.end && !left && !right);
+        slow[r] = __ballot_sync(0xFFFFFFFFu, max(c, 0) < end[r] && !is_left && !is_right);
       }
       // Their elements, one to a lane: near ones each into its bucket.  (One copy
       // of this code: unrolled over rows and vectors, fetching it took longer than
@@ -322,12 +384,13 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
       for (int r = 0; r < kRows; r++) {
         unsigned todo = r == 0 ? slow[0] : r == 1 ? slow[1] : r == 2 ? slow[2] : slow[3];
         if (!todo) continue;
-        const Row w = row_of(t, a, r0 + r);
+        const Row w = {__shfl_sync(0xFFFFFFFFu, own.left, r), __shfl_sync(0xFFFFFFFFu, own.right, r),
+                       __shfl_sync(0xFFFFFFFFu, own.end, r), __shfl_sync(0xFFFFFFFFu, own.query, r)};
         const T* at = line + r * a.rs;
-        const int base = (int)tv * 32 * N - (int)(((uintptr_t)at / sizeof(T)) % N);
+        const int base = (int)tv * 32 * N - (int)(((uintptr_t)at / sizeof(T)) % N) + lane;
 #pragma unroll 1
         while (todo) {
-          const int first = __ffs(todo) - 1, vec = first + lane / N, c = base + first * N + lane;
+          const int first = __ffs(todo) - 1, vec = first + lane / N, c = base + first * N;
           const bool here = vec < 32 && (todo >> (vec & 31) & 1) && c >= 0 && c < w.end;
           const unsigned upto = first + 32 / N;
           todo = upto < 32 ? todo >> upto << upto : 0;
@@ -434,27 +497,15 @@ Buckets buckets_of(const dcf_bias_desc& d) {
   return t;
 }
 
-BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
-  BiasArgs a;
-  a.queries = d.queries;
-  a.keys = (int)d.keys;
-  a.first = d.first_query;
-  a.rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
-  a.hs = d.head_stride ? d.head_stride : (int64_t)d.queries * a.rs;
-  a.bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * a.hs;
-  a.heads = (int)d.heads;
-  a.nb = (int)d.num_buckets;
-  a.batch = d.batch;
-  a.pos = pos;
-  return a;
-}
-
 template <class T, class S>
 int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos, void* out, cudaStream_t stream) {
   constexpr uint64_t N = Vec<T>::N;
   const Buckets t = buckets_of(d);
-  const BiasArgs a = args_of(d, pos);
-  const uint64_t vecs = (d.keys + 2 * N - 2) / N, items = vecs * d.queries;
+  BiasArgs a = args_of(d, pos);
+  a.bs = 0;
+  const bool aligned = (uintptr_t)out % 16 == 0 && strides_aligned(a, N);
+  const uint64_t vecs = vectors_of_row(d.keys, N, aligned);
+  const uint64_t items = vecs * d.queries;
   const uint64_t blocks = (items + kFwdThreads - 1) / kFwdThreads;
   // Heads per block: as many as share the bucket lookup without leaving SMs
   // idle, within 16 KB of table.
@@ -466,8 +517,10 @@ int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos,
   hc = (d.heads + groups - 1) / groups;
   groups = (d.heads + hc - 1) / hc;
   const size_t smem = hc * (d.num_buckets + 1) * sizeof(T);
-  const dim3 grid((unsigned)(blocks < (1u << 30) ? blocks : (1u << 30)), (unsigned)groups);
-  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, (uint32_t)vecs, items);
+  // A block's table and near buckets serve several items.
+  const uint64_t most = (kSms * 12 + groups - 1) / groups;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)groups);
+  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, aligned, (uint32_t)vecs, items);
   note_launch();
   return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
@@ -478,7 +531,9 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
   using A = typename AccOf<T>::type;
   const Buckets t = buckets_of(d);
   const BiasArgs a = args_of(d, pos);
-  const GradPlan p = grad_plan(d);
+  GradPlan p = grad_plan(d);
+  if ((uintptr_t)g % 16 == 0 && strides_aligned(a, Vec<T>::N))
+    p.tiles_v = (uint32_t)((vectors_of_row(d.keys, Vec<T>::N, true) + 31) / 32);
   const int add = (d.flags & DCF_BIAS_ACCUMULATE) != 0;
   const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A);
   if (smem > kAccBytes - 4096 &&
