@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kMaxB = DCF_BIAS_MAX_BUCKETS;
 constexpr int kSms = 148;
+constexpr int kTable = 256;  // distances whose bucket is looked up rather than searched
 
 // How a distance maps to its bucket; a kernel parameter.
 struct Buckets {
@@ -37,6 +38,7 @@ struct Buckets {
   int causal;
   int last;           // distances >= last have bucket half - 1
   int start[kMaxB];   // first distance of each bucket, sorted
+  alignas(4) uint8_t near[kTable];  // bucket number of each distance below min(last, kTable)
 };
 
 struct BiasArgs {
@@ -66,15 +68,13 @@ __device__ __forceinline__ Row row_of(const Buckets& t, const BiasArgs& a, uint6
   r.left = clip(q - t.last, -1, a.keys);
   r.right = clip(q + (t.both && t.last > 1 ? t.last : 1), 0, a.keys);
   r.end = t.causal ? clip(q + 1, 0, a.keys) : a.keys;
-  r.query = (int)q;
+  r.query = (int)q;  // near columns: their distance is right modulo 2^32
   return r;
 }
 
-constexpr int kTable = 2048;  // distances whose bucket is looked up rather than searched
-
 // The bucket number of every near distance, in shared memory.
 struct Near {
-  uint8_t of[kTable];
+  alignas(4) uint8_t of[kTable];
   int start[kMaxB];
 };
 
@@ -91,7 +91,7 @@ __device__ __forceinline__ int search(const int* start, int half, int n) {
 // By all threads of the block; the caller synchronises.
 __device__ __forceinline__ void fill_near(Near& near, const Buckets& t, int threads) {
   for (int i = threadIdx.x; i < t.half; i += threads) near.start[i] = t.start[i];
-  for (int n = threadIdx.x; n < kTable && n < t.last; n += threads) near.of[n] = (uint8_t)search(t.start, t.half, n);
+  for (int i = threadIdx.x; i < kTable / 4; i += threads) ((uint32_t*)near.of)[i] = ((const uint32_t*)t.near)[i];
 }
 
 // Bucket of a column between a row's left and right.
@@ -123,106 +123,86 @@ template <class T> struct alignas(16) Vec {
 
 // ---------------------------------------------------------------- bias
 
-constexpr int kFwdThreads = 256;
+constexpr int kFwdThreads = 256, kFwdWarps = kFwdThreads / 32;
 
-// A thread owns one 16-byte vector of a row and writes it for `hc` heads.
-// Rows need not be aligned: vectors sit on 16-byte addresses, the ones at a
-// row's ends are written element by element.  Masked columns read the
-// table's row nb, which holds -inf.
+// A block writes rows of one head, one after the other, a warp to a row or to a
+// part of one: what is being written at any time then lies close
+// together (blocks that wrote one row of many heads, sharing the lookup of buckets, reached
+// 3.3 - 5.5 TB/s, the less the more heads).  Vectors sit on 16-byte addresses, rows
+// need not; the ones at a row's ends are written element by element.  Vectors that
+// lie in a far range, or behind the mask, are one of three constants;
+// a near column reads its value from a table by distance.
 template <class T, class S>
 __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a,
-                                                           const S* __restrict__ table, T* __restrict__ out, int hc,
-                                                           int aligned, uint32_t vecs, uint64_t items) {
+                                                           const S* __restrict__ table, T* __restrict__ out,
+                                                           uint32_t chunk, uint32_t chunks, uint64_t items, int turns) {
   constexpr int N = Vec<T>::N;
-  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ Near near;
-  T* tab = (T*)smem;                       // [hc][nb + 1]
-  const int pitch = a.nb + 1;
-  const int h0 = blockIdx.y * hc;
-  const int hn = min(hc, a.heads - h0);
+  __shared__ T tab[kMaxB], value[2 * kTable];  // by bucket; by distance + last
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   fill_near(near, t, kFwdThreads);
-  for (int i = threadIdx.x; i < a.nb * hn; i += kFwdThreads) {
-    const int v = i / hn, h = i - v * hn;
-    tab[h * pitch + v] = cast<T, S>(table[(size_t)v * a.heads + h0 + h]);
-  }
-  for (int h = threadIdx.x; h < hn; h += kFwdThreads) tab[h * pitch + a.nb] = minus_infinity<T>();
+  for (int v = threadIdx.x; v < a.nb; v += kFwdThreads) tab[v] = cast<T, S>(table[(size_t)v * a.heads + h]);
   __syncthreads();
-  const int far_left = t.half - 1, far_right = t.both ? 2 * t.half - 1 : 0;
-
-  for (uint64_t item = (uint64_t)blockIdx.x * kFwdThreads + threadIdx.x; item < items;
-       item += (uint64_t)gridDim.x * kFwdThreads) {
-    uint64_t row;
-    if (items < (1ull << 32)) row = (uint32_t)item / vecs;
-    else row = item / vecs;
-    const int v = (int)(item - row * vecs);
-    const Row r = row_of(t, a, row);
-    T* line = out + (int64_t)h0 * a.hs + (int64_t)row * a.rs;
-    int which[N];            // the bucket of each of the vector's columns
-    bool one;                // whether it is one for all
-#define LOOK_UP(c0)                                                                                                      \
-  which[0] = (c0) >= r.end ? a.nb : (c0) + N - 1 <= r.left ? far_left : far_right;                                       \
-  one = (c0) >= r.end || (c0) + N - 1 <= r.left || ((c0) >= r.right && (c0) + N <= r.end);                               \
-  if (!one) {                                                                                                            \
-    _Pragma("unroll") for (int k = 0; k < N; k++) {                                                                      \
-      const int c = (c0) + k;                                                                                            \
-      which[k] = c >= r.end ? a.nb : c <= r.left ? far_left : c >= r.right ? far_right : near_bucket(near, t, r, c);     \
-    }                                                                                                                    \
-  }
-    if (aligned) {           // every head's rows start on a 16-byte boundary: one lookup serves all
-      const int c0 = v * N;
-      LOOK_UP(c0)
-      line += c0;
-      if (c0 + N > a.keys) {
-        for (int h = 0; h < hn; h++, line += a.hs)
-#pragma unroll
-          for (int k = 0; k < N; k++)
-            if (c0 + k < a.keys) line[k] = tab[h * pitch + (one ? which[0] : which[k])];
-      } else if (one) {
-        const T* ht = tab + which[0];
-#pragma unroll 4
-        for (int h = 0; h < hn; h++, line += a.hs, ht += pitch) {
-          const T e = *ht;
-          Vec<T> x;
-#pragma unroll
-          for (int k = 0; k < N; k++) x.e[k] = e;
-          *(uint4*)line = *(const uint4*)&x;
-        }
-      } else {
-        const T* ht = tab;
-#pragma unroll 2
-        for (int h = 0; h < hn; h++, line += a.hs, ht += pitch) {
-          Vec<T> x;
-#pragma unroll
-          for (int k = 0; k < N; k++) x.e[k] = ht[which[k]];
-          *(uint4*)line = *(const uint4*)&x;
-        }
-      }
-      continue;
+  const bool tabled = t.last <= kTable;
+  if (tabled) {
+    for (int i = threadIdx.x; i < 2 * t.last; i += kFwdThreads) {
+      const int d = i - t.last, n = d < 0 ? -d : d;
+      if (d != -t.last) value[i] = tab[(d > 0 ? (t.both ? t.half : 0) : 0) + (d > 0 && !t.both ? 0 : near.of[n])];
     }
-    int shift = -1, c0 = 0;  // elements by which this head's rows lie behind a 16-byte boundary
-    one = false;
-    for (int h = 0; h < hn; h++, line += a.hs) {
-      const int s = (int)(((uintptr_t)line / sizeof(T)) % N);
-      if (s != shift) {
-        shift = s;
-        c0 = v * N - s;
-        LOOK_UP(c0)
-      }
-      if (c0 >= a.keys) continue;
-      const T* ht = tab + h * pitch;
-      Vec<T> x;
+    __syncthreads();
+  }
+  Vec<T> left, right, masked;
 #pragma unroll
-      for (int k = 0; k < N; k++) x.e[k] = ht[one ? which[0] : which[k]];
-      if (c0 >= 0 && c0 + N <= a.keys) {
-        *(uint4*)(line + c0) = *(const uint4*)&x;
+  for (int k = 0; k < N; k++) {
+    left.e[k] = tab[t.half - 1];
+    right.e[k] = tab[t.both ? 2 * t.half - 1 : 0];
+    masked.e[k] = minus_infinity<T>();
+  }
+
+  for (int turn = 0; turn < turns; turn++) {
+    const uint64_t item = ((uint64_t)blockIdx.x * turns + turn) * kFwdWarps + warp;
+    if (item >= items) return;
+    uint64_t row;
+    uint32_t part;
+    if (items < (1ull << 32)) {
+      row = (uint32_t)item / chunks;
+      part = (uint32_t)item - (uint32_t)row * chunks;
+    } else {
+      row = item / chunks;
+      part = (uint32_t)(item - row * chunks);
+    }
+    const Row r = row_of(t, a, row);
+    T* line = out + (int64_t)h * a.hs + (int64_t)row * a.rs;
+    int c = (int)(part * chunk * 32 + lane) * N - (int)(((uintptr_t)line / sizeof(T)) % N);
+    line += c;
+    for (uint32_t i = 0; i < chunk && c < a.keys; i++, c += 32 * N, line += 32 * N) {
+      Vec<T> x;
+      if (c >= r.end) {
+        x = masked;
+      } else if (c + N - 1 <= r.left) {
+        x = left;
+      } else if (c >= r.right && c + N <= r.end) {
+        x = right;
+      } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+          const int e = c + k;
+          x.e[k] = e >= r.end    ? masked.e[0]
+                   : e <= r.left ? left.e[0]
+                   : e >= r.right ? right.e[0]
+                   : tabled       ? value[(int)((unsigned)e - (unsigned)r.query) + t.last]
+                                  : tab[near_bucket(near, t, r, e)];
+        }
+      }
+      if (c >= 0 && c + N <= a.keys) {
+        *(uint4*)line = *(const uint4*)&x;
       } else {
 #pragma unroll
         for (int k = 0; k < N; k++)
-          if (c0 + k >= 0 && c0 + k < a.keys) line[c0 + k] = x.e[k];
+          if (c + k >= 0 && c + k < a.keys) line[k] = x.e[k];
       }
     }
-#undef LOOK_UP
   }
 }
 
@@ -235,8 +215,8 @@ __device__ __forceinline__ double widen(double x) { return x; }
 __device__ __forceinline__ float widen(__half x) { return __half2float(x); }
 __device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-constexpr int kRows = 4;            // rows of a warp's tile (their four loads are in flight together)
 constexpr size_t kAccBytes = 48 << 10;
+constexpr int kOffsets = 2048;  // distances (each way) for which a block tables where their sums are
 
 BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
   BiasArgs a;
@@ -254,13 +234,13 @@ BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
 }
 
 // How the gradient is split: `splits` CTAs per head, each with `warps`
-// warps, every warp taking items (four rows of one batch entry x `chunk` times
-// 32 vectors) in turn.  Fixed by the sizes and strides alone, so sums keep
+// warps, every warp taking items (`batch` entries of one row, or `chunk` steps of
+// 32 vectors of it) in turn.  Fixed by the sizes and strides alone, so sums keep
 // their order.
 struct GradPlan {
   int warps, splits;
-  uint32_t tiles_v, chunk, chunks;
-  uint64_t items;
+  uint32_t chunk, chunks, batches;
+  uint64_t batch, items;
 };
 
 // Vectors that a row of `keys` elements can touch: one more where rows need
@@ -277,39 +257,75 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
   const uint64_t n = 16 / es;
   p.warps = (int)(kAccBytes / (d.num_buckets * 32 * acc));
   p.warps = p.warps > 8 ? 8 : p.warps < 1 ? 1 : p.warps;
-  p.tiles_v = d.keys ? (uint32_t)((vectors_of_row(d.keys, n, false) + 31) / 32) : 0;
-  const uint64_t groups = (d.queries + kRows - 1) / kRows * d.batch;
-  const uint64_t ctas = d.heads ? (uint64_t)(kSms * 3 + d.heads - 1) / d.heads : 1;  // per head: three to an SM
+  const uint64_t steps = (vectors_of_row(d.keys, n, false) + 31) / 32, rows = d.queries;
+  const uint64_t ctas = d.heads ? (uint64_t)(kSms * 4 + d.heads - 1) / d.heads : 1;  // per head: four to an SM
   const uint64_t slots = ctas * p.warps;
-  // Whole rows where there are enough of them for every warp, else parts.
-  uint64_t cuts = groups ? slots / groups : 1;
-  cuts = cuts < 1 ? 1 : cuts > p.tiles_v ? p.tiles_v : cuts;
-  p.chunk = cuts ? (uint32_t)((p.tiles_v + cuts - 1) / cuts) : 1;
-  p.chunks = p.chunk ? (p.tiles_v + p.chunk - 1) / p.chunk : 0;
-  p.items = groups * p.chunks;
+  if (rows == 0 || d.batch == 0 || steps == 0) {
+    p.chunk = p.chunks = p.batches = 1;
+    p.batch = 1;
+    p.items = 0;
+    p.splits = 1;
+    return p;
+  }
+  // A row's look at its position serves several batch entries where there are
+  // four items per warp all the same; short of items, rows are cut.
+  uint64_t batch = rows * d.batch / (slots * 4);
+  p.batch = batch < 1 ? 1 : batch > d.batch ? d.batch : batch;
+  p.batches = (uint32_t)((d.batch + p.batch - 1) / p.batch);
+  uint64_t cuts = slots / (rows * p.batches);
+  cuts = cuts < 1 ? 1 : cuts > steps ? steps : cuts;
+  p.chunk = (uint32_t)((steps + cuts - 1) / cuts);
+  p.chunks = (uint32_t)((steps + p.chunk - 1) / p.chunk);
+  p.items = rows * p.batches * p.chunks;
   // As few CTAs as take no more turns than the most would.
   const uint64_t turns = (p.items + slots - 1) / slots;
-  const uint64_t want = turns ? (p.items + turns * p.warps - 1) / (turns * p.warps) : 1;
+  const uint64_t want = (p.items + turns * p.warps - 1) / (turns * p.warps);
   p.splits = (int)(want < 1 ? 1 : want);
   return p;
 }
 
+template <class T> __device__ __forceinline__ typename AccOf<T>::type sum_of(const Vec<T>& x) {
+  constexpr int N = Vec<T>::N;
+  typename AccOf<T>::type s[N];
+#pragma unroll
+  for (int k = 0; k < N; k++) s[k] = widen(x.e[k]);
+#pragma unroll
+  for (int u = N / 2; u > 0; u >>= 1)
+#pragma unroll
+    for (int k = 0; k < u; k++) s[k] += s[k + u];
+  return s[0];
+}
+
+// A warp walks along a row in steps of 32 vectors.  Steps that lie wholly in a
+// far range are only summed (18 instructions for 512 bytes of f16); in the others
+// every element adds into its bucket's sum, which each lane has for itself in
+// shared memory, found by a table of distances.
 template <class T>
-__global__ void __launch_bounds__(256, 3) bias_grad_kernel(const __grid_constant__ Buckets t,
+__global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a, const T* __restrict__ g,
                                                            const __grid_constant__ GradPlan p,
                                                            typename AccOf<T>::type* __restrict__ part,
                                                            typename AccOf<T>::type* __restrict__ dtable, int add) {
   using A = typename AccOf<T>::type;
-  constexpr int N = Vec<T>::N;
+  constexpr int N = Vec<T>::N, kStep = 32 * N;
   extern __shared__ __align__(16) uint8_t smem[];
   A* acc = (A*)smem;   // [warp][bucket][lane]: every lane adds into its own column, in its own order
   __shared__ Near near;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int threads = p.warps * 32;
+  uint16_t* offset = (uint16_t*)(acc + (size_t)p.warps * a.nb * 32);  // by distance + far: 32 x bucket
+  const bool tabled = t.last <= kOffsets;
+  const int far = max(t.last, 1);
   fill_near(near, t, threads);
   for (int i = threadIdx.x; i < p.warps * a.nb * 32; i += threads) acc[i] = 0;
   __syncthreads();
+  if (tabled) {
+    for (int i = threadIdx.x; i <= 2 * far; i += threads) {
+      const int d = i - far, n = d < 0 ? -d : t.both ? d : 0;
+      offset[i] = (uint16_t)(32 * ((t.both && d > 0 ? t.half : 0) + (n < kTable ? near.of[n] : search(near.start, t.half, n))));
+    }
+    __syncthreads();
+  }
   A* mine = acc + (size_t)warp * a.nb * 32 + lane;
 
   const int h = blockIdx.y;
@@ -319,86 +335,81 @@ __global__ void __launch_bounds__(256, 3) bias_grad_kernel(const __grid_constant
     // Forth and back: with a causal mask later rows are longer.
     const uint64_t item = turn * warps + (turn & 1 ? warps - 1 - self : self);
     if (item >= p.items) continue;
-    uint64_t group, b;
-    uint32_t part_v;
+    uint64_t row, b;
+    uint32_t cut;
     if (p.items < (1ull << 32)) {
-      group = (uint32_t)item / p.chunks;
-      part_v = (uint32_t)item - (uint32_t)group * p.chunks;
-      const uint32_t batch = (uint32_t)a.batch, g4 = (uint32_t)group / batch;
-      b = (uint32_t)group - g4 * batch;
-      group = g4;
+      const uint32_t x = (uint32_t)item / p.chunks;
+      cut = (uint32_t)item - x * p.chunks;
+      row = x / p.batches;
+      b = x - (uint32_t)row * p.batches;
     } else {
-      group = item / p.chunks;
-      part_v = (uint32_t)(item - group * p.chunks);
-      b = group % a.batch;
-      group /= a.batch;
+      const uint64_t x = item / p.chunks;
+      cut = (uint32_t)(item - x * p.chunks);
+      row = x / p.batches;
+      b = x - row * p.batches;
     }
-    const uint64_t r0 = group * kRows;
-    Row own = {-1, 0, 0, 0};        // of row r0 + lane; no row there: nothing is read
-    if (lane < kRows && r0 + lane < a.queries) own = row_of(t, a, r0 + lane);
-    const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)r0 * a.rs;
-    int left[kRows], right[kRows], end[kRows], shift[kRows];
-    int reach = 0;
+    const Row r = row_of(t, a, row);
+    b *= p.batch;
+    const uint64_t b_end = min(a.batch, b + p.batch);
+    const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)row * a.rs;
+    for (; b < b_end; b++, line += a.bs) {
+      const int shift = (int)(((uintptr_t)line / sizeof(T)) % N);  // elements behind a 16-byte boundary
+      const T* lane_at = line - shift + lane * N;
+      // Steps [l0, l1) lie in the left range, [r0, r1) in the right one.
+      const int l0 = shift ? 1 : 0, l1 = (min(r.left + 1, r.end) + shift) / kStep;
+      const int r0 = (r.right + shift + kStep - 1) / kStep, r1 = (r.end + shift) / kStep;
+      const int stop = min((int)((cut + 1) * p.chunk), r.end > 0 ? (r.end + shift + kStep - 1) / kStep : 0);
+      int i = (int)(cut * p.chunk);
+      while (i < stop) {
+        const bool left = i >= l0 && i < l1;
+        if (left || (i >= r0 && i < r1 && (i >= l0))) {
+          const int to = min(stop, left ? l1 : r1);
+          A s = 0;
+          for (; i + 4 <= to; i += 4) {
+            Vec<T> x[4];
 #pragma unroll
-    for (int r = 0; r < kRows; r++) {
-      left[r] = __shfl_sync(0xFFFFFFFFu, own.left, r);
-      right[r] = __shfl_sync(0xFFFFFFFFu, own.right, r);
-      end[r] = __shfl_sync(0xFFFFFFFFu, own.end, r);
-      // elements by which the row lies behind a 16-byte boundary
-      shift[r] = (int)(((uintptr_t)(line + r * a.rs) / sizeof(T)) % N);
-      reach = max(reach, end[r]);
-    }
-    const uint32_t last = min(p.tiles_v, (part_v + 1) * p.chunk);
-    for (uint32_t tv = part_v * p.chunk; tv < last && (int)tv * 32 * N - (N - 1) < reach; tv++) {
-      const int v0 = (int)(tv * 32 + lane) * N;
-      // Vectors that lie wholly in a far range; the others are noted.
-      Vec<T> x[kRows];
-      unsigned slow[kRows];
-#pragma unroll
-      for (int r = 0; r < kRows; r++) {
-        const int c = v0 - shift[r];
-        if (c >= 0 && c < end[r] && c + N <= a.keys) *(uint4*)&x[r] = __ldg((const uint4*)(line + r * a.rs + c));
-      }
-#pragma unroll
-      for (int r = 0; r < kRows; r++) {
-        const int c = v0 - shift[r];
-        const bool whole = c >= 0 && c + N <= end[r];
-        const bool is_left = whole && c + N - 1 <= left[r], is_right = whole && c >= right[r];
-        if (is_left || is_right) {
-          A s[N];
-#pragma unroll
-          for (int k = 0; k < N; k++) s[k] = widen(x[r].e[k]);
-#pragma unroll
-          for (int u = N / 2; u > 0; u >>= 1)
-#pragma unroll
-            for (int k = 0; k < u; k++) s[k] += s[k + u];
-          if (is_left) far_left += s[0];
-          else far_right += s[0];
+            for (int k = 0; k < 4; k++) *(uint4*)&x[k] = __ldg((const uint4*)(lane_at + (int64_t)(i + k) * kStep));
+            s += (sum_of(x[0]) + sum_of(x[1])) + (sum_of(x[2]) + sum_of(x[3]));
+          }
+          for (; i < to; i++) {
+            Vec<T> x;
+            *(uint4*)&x = __ldg((const uint4*)(lane_at + (int64_t)i * kStep));
+            s += sum_of(x);
+          }
+          if (left) far_left += s;
+          else far_right += s;
+          continue;
         }
-        slow[r] = __ballot_sync(0xFFFFFFFFu, max(c, 0) < end[r] && !is_left && !is_right);
-      }
-      // Their elements, one to a lane: near ones each into its bucket.  (One copy
-      // of this code: unrolled over rows and vectors, fetching it took longer than
-      // running it.)
-#pragma unroll 1
-      for (int r = 0; r < kRows; r++) {
-        unsigned todo = r == 0 ? slow[0] : r == 1 ? slow[1] : r == 2 ? slow[2] : slow[3];
-        if (!todo) continue;
-        const Row w = {__shfl_sync(0xFFFFFFFFu, own.left, r), __shfl_sync(0xFFFFFFFFu, own.right, r),
-                       __shfl_sync(0xFFFFFFFFu, own.end, r), __shfl_sync(0xFFFFFFFFu, own.query, r)};
-        const T* at = line + r * a.rs;
-        const int base = (int)tv * 32 * N - (int)(((uintptr_t)at / sizeof(T)) % N) + lane;
-#pragma unroll 1
-        while (todo) {
-          const int first = __ffs(todo) - 1, vec = first + lane / N, c = base + first * N;
-          const bool here = vec < 32 && (todo >> (vec & 31) & 1) && c >= 0 && c < w.end;
-          const unsigned upto = first + 32 / N;
-          todo = upto < 32 ? todo >> upto << upto : 0;
-          if (!here) continue;
-          const A e = widen(__ldg(at + c));
-          if (c <= w.left) far_left += e;
-          else if (c >= w.right) far_right += e;
-          else mine[near_bucket(near, t, w, c) * 32] += e;
+        const int c = i * kStep + lane * N - shift;
+        i++;
+        if (max(c, 0) >= r.end) continue;
+        Vec<T> x;
+        if (c >= 0 && c + N <= a.keys) {
+          *(uint4*)&x = __ldg((const uint4*)(line + c));
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k++)
+            if (c + k >= 0 && c + k < r.end) x.e[k] = line[c + k];
+        }
+        const bool whole = c >= 0 && c + N <= r.end;
+        if (whole && c + N - 1 <= r.left) {
+          far_left += sum_of(x);
+        } else if (whole && c >= r.right) {
+          far_right += sum_of(x);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k++) {
+            const int e = c + k;
+            if (!whole && (e < 0 || e >= r.end)) continue;
+            int at;
+            if (tabled) {
+              const int d = (int)((unsigned)e - (unsigned)r.query);
+              at = offset[(e <= r.left ? -far : e >= r.right ? far : d) + far];
+            } else {
+              at = 32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e));
+            }
+            mine[at] += widen(x.e[k]);
+          }
         }
       }
     }
@@ -494,6 +505,10 @@ Buckets buckets_of(const dcf_bias_desc& d) {
   t.half = (int)(t.both ? d.num_buckets / 2 : d.num_buckets);
   bias_starts(t.half, d.max_distance, t.start);
   t.last = t.start[t.half - 1];
+  for (int n = 0, v = 0; n < kTable; n++) {
+    while (v + 1 < t.half && t.start[v + 1] <= n) v++;
+    t.near[n] = (uint8_t)v;
+  }
   return t;
 }
 
@@ -504,23 +519,20 @@ int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos,
   BiasArgs a = args_of(d, pos);
   a.bs = 0;
   const bool aligned = (uintptr_t)out % 16 == 0 && strides_aligned(a, N);
-  const uint64_t vecs = vectors_of_row(d.keys, N, aligned);
-  const uint64_t items = vecs * d.queries;
-  const uint64_t blocks = (items + kFwdThreads - 1) / kFwdThreads;
-  // Heads per block: as many as share the bucket lookup without leaving SMs
-  // idle, within 16 KB of table.
-  const uint64_t room = (16 << 10) / ((d.num_buckets + 1) * sizeof(T));
-  uint64_t hc = blocks >= kSms * 8 ? d.heads : (d.heads * blocks + kSms * 8 - 1) / (kSms * 8);
-  if (hc > room) hc = room;
-  if (hc < 1) hc = 1;
-  uint64_t groups = (d.heads + hc - 1) / hc;
-  hc = (d.heads + groups - 1) / groups;
-  groups = (d.heads + hc - 1) / hc;
-  const size_t smem = hc * (d.num_buckets + 1) * sizeof(T);
-  // A block's table and near buckets serve several items.
-  const uint64_t most = (kSms * 12 + groups - 1) / groups;
-  const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)groups);
-  bias_kernel<T, S><<<grid, kFwdThreads, smem, stream>>>(t, a, (const S*)table, (T*)out, (int)hc, aligned, (uint32_t)vecs, items);
+  // A warp's steps along a row; whole rows, or parts where there are few.
+  const uint64_t steps = (vectors_of_row(d.keys, N, aligned) + 31) / 32, rows = d.queries * d.heads;
+  uint64_t cuts = kSms * 32 / rows;
+  cuts = cuts < 1 ? 1 : cuts > steps ? steps : cuts;
+  const uint32_t chunk = (uint32_t)((steps + cuts - 1) / cuts), chunks = (uint32_t)((steps + chunk - 1) / chunk);
+  const uint64_t items = d.queries * chunks;
+  // Up to 32 KB for the tables that a block sets up, where there is enough to do.
+  uint64_t turns = (32 << 10) / (kFwdWarps * chunk * 512);
+  const uint64_t most = items * d.heads / (kFwdWarps * kSms * 8);
+  if (turns > most) turns = most;
+  if (turns < 1) turns = 1;
+  const uint64_t blocks = (items + kFwdWarps * turns - 1) / (kFwdWarps * turns);
+  bias_kernel<T, S><<<dim3((unsigned)blocks, d.heads), kFwdThreads, 0, stream>>>(t, a, (const S*)table, (T*)out, chunk,
+                                                                                chunks, items, (int)turns);
   note_launch();
   return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
@@ -531,13 +543,11 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
   using A = typename AccOf<T>::type;
   const Buckets t = buckets_of(d);
   const BiasArgs a = args_of(d, pos);
-  GradPlan p = grad_plan(d);
-  if ((uintptr_t)g % 16 == 0 && strides_aligned(a, Vec<T>::N))
-    p.tiles_v = (uint32_t)((vectors_of_row(d.keys, Vec<T>::N, true) + 31) / 32);
+  const GradPlan p = grad_plan(d);
   const int add = (d.flags & DCF_BIAS_ACCUMULATE) != 0;
-  const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A);
+  const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A) + (t.last <= kOffsets ? (2 * (size_t)(t.last < 1 ? 1 : t.last) + 1) * 2 : 0);
   if (smem > kAccBytes - 4096 &&
-      cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 << 10) != cudaSuccess)
+      cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) != cudaSuccess)
     return DCF_ECUDA;
   bias_grad_kernel<T><<<dim3((unsigned)p.splits, d.heads), p.warps * 32, smem, stream>>>(
       t, a, (const T*)g, p, (A*)ws, (A*)dtable, add);
