@@ -136,7 +136,7 @@ template <class T, class S>
 __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a,
                                                            const S* __restrict__ table, T* __restrict__ out,
-                                                           uint32_t chunk, uint32_t chunks, uint64_t items, int turns) {
+                                                           uint32_t chunk, uint32_t chunks, uint64_t items, int turns, int team) {
   constexpr int N = Vec<T>::N;
   __shared__ Near near;
   __shared__ T tab[kMaxB], value[2 * kTable];  // by bucket; by distance + last
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
   }
 
   for (int turn = 0; turn < turns; turn++) {
-    const uint64_t item = ((uint64_t)blockIdx.x * turns + turn) * kFwdWarps + warp;
+    const uint64_t item = ((uint64_t)blockIdx.x * turns + turn) * (kFwdWarps / team) + warp / team;
     if (item >= items) return;
     uint64_t row;
     uint32_t part;
@@ -174,9 +174,9 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
     }
     const Row r = row_of(t, a, row);
     T* line = out + (int64_t)h * a.hs + (int64_t)row * a.rs;
-    int c = (int)(part * chunk * 32 + lane) * N - (int)(((uintptr_t)line / sizeof(T)) % N);
+    int c = (int)((part * chunk + warp % team) * 32 + lane) * N - (int)(((uintptr_t)line / sizeof(T)) % N);
     line += c;
-    for (uint32_t i = 0; i < chunk && c < a.keys; i++, c += 32 * N, line += 32 * N) {
+    for (uint32_t i = warp % team; i < chunk && c < a.keys; i += team, c += team * 32 * N, line += team * 32 * N) {
       Vec<T> x;
       if (c >= r.end) {
         x = masked;
@@ -349,6 +349,9 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
       b = x - row * p.batches;
     }
     const Row r = row_of(t, a, row);
+    // Near enough for every distance to fit 32 bits, far enough to change no bucket
+    // that the table has.
+    const int query = clip(a.pos ? (int64_t)a.pos[row] : a.first + (int64_t)row, -kOffsets - 1, (int64_t)a.keys + kOffsets + 1);
     b *= p.batch;
     const uint64_t b_end = min(a.batch, b + p.batch);
     const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)row * a.rs;
@@ -391,25 +394,18 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
           for (int k = 0; k < N; k++)
             if (c + k >= 0 && c + k < r.end) x.e[k] = line[c + k];
         }
+        // (Lanes in a far range add into its bucket the same way: a branch of
+        // their own cost the warp more.)
         const bool whole = c >= 0 && c + N <= r.end;
-        if (whole && c + N - 1 <= r.left) {
-          far_left += sum_of(x);
-        } else if (whole && c >= r.right) {
-          far_right += sum_of(x);
-        } else {
+        const int d0 = c - query + far;
 #pragma unroll
-          for (int k = 0; k < N; k++) {
-            const int e = c + k;
-            if (!whole && (e < 0 || e >= r.end)) continue;
-            int at;
-            if (tabled) {
-              const int d = (int)((unsigned)e - (unsigned)r.query);
-              at = offset[(e <= r.left ? -far : e >= r.right ? far : d) + far];
-            } else {
-              at = 32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e));
-            }
-            mine[at] += widen(x.e[k]);
-          }
+        for (int k = 0; k < N; k++) {
+          const int e = c + k;
+          if (!whole && (e < 0 || e >= r.end)) continue;
+          int at;
+          if (tabled) at = offset[min(max(d0 + k, 0), 2 * far)];
+          else at = 32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e));
+          mine[at] += widen(x.e[k]);
         }
       }
     }
@@ -526,13 +522,18 @@ int launch_bias_t(const dcf_bias_desc& d, const void* table, const int32_t* pos,
   const uint32_t chunk = (uint32_t)((steps + cuts - 1) / cuts), chunks = (uint32_t)((steps + chunk - 1) / chunk);
   const uint64_t items = d.queries * chunks;
   // Up to 32 KB for the tables that a block sets up, where there is enough to do.
-  uint64_t turns = (32 << 10) / (kFwdWarps * chunk * 512);
-  const uint64_t most = items * d.heads / (kFwdWarps * kSms * 8);
+  // Warps that share a row, by turns of a step: long rows then keep a block's writes
+  // together (250 scattered rows of 8192, 32 heads: 24.8 us with two, 29.3 us with one), short
+  // ones pay for every warp's look at the row (4001: 180 and 196 us).
+  int team = 1;
+  while (team < kFwdWarps && chunk >= 32u * team) team *= 2;
+  uint64_t turns = (32 << 10) / (kFwdWarps / team * chunk * 512);
+  const uint64_t most = items * d.heads / (kFwdWarps / team * kSms * 8);
   if (turns > most) turns = most;
   if (turns < 1) turns = 1;
-  const uint64_t blocks = (items + kFwdWarps * turns - 1) / (kFwdWarps * turns);
+  const uint64_t blocks = (items + kFwdWarps / team * turns - 1) / (kFwdWarps / team * turns);
   bias_kernel<T, S><<<dim3((unsigned)blocks, d.heads), kFwdThreads, 0, stream>>>(t, a, (const S*)table, (T*)out, chunk,
-                                                                                chunks, items, (int)turns);
+                                                                                chunks, items, (int)turns, team);
   note_launch();
   return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
@@ -581,8 +582,8 @@ int bias_desc_check(const dcf_bias_desc* d, bool grad) {
     return bad("position bias: max_distance must be above the exact buckets and below 2^31");
   if (d->heads > 65535) return bad("position bias: at most 65535 heads");
   const uint64_t lim = 1ull << 31;
-  if (d->queries >= lim || d->keys >= lim - 64 || (grad && d->batch >= lim))
-    return bad("position bias: queries and batch must be below 2^31, keys below 2^31 - 64");
+  if (d->queries >= lim || d->keys > lim - 65536 || (grad && d->batch >= lim))
+    return bad("position bias: queries and batch must be below 2^31, keys at most 2^31 - 65536");
   if (d->first_query > (1ll << 40) || d->first_query < -(1ll << 40)) return bad("position bias: first_query out of range");
   if (d->row_stride < 0 || d->head_stride < 0 || d->batch_stride < 0) return bad("position bias: negative stride");
   // Extents in 128 bits, so that no product of the checks wraps.
