@@ -267,15 +267,20 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
     p.splits = 1;
     return p;
   }
-  // A row's look at its position serves several batch entries where there are
-  // four items per warp all the same; short of items, rows are cut.
-  uint64_t batch = rows * d.batch / (slots * 4);
-  p.batch = batch < 1 ? 1 : batch > d.batch ? d.batch : batch;
-  p.batches = (uint32_t)((d.batch + p.batch - 1) / p.batch);
-  uint64_t cuts = slots / (rows * p.batches);
+  // Batch entries of a row share the buckets, as long as their rows are aligned
+  // alike; where that leaves fewer than three items per warp, rows are cut into
+  // parts, then the batch.
+  const int64_t rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
+  const int64_t hs = d.head_stride ? d.head_stride : (int64_t)d.queries * rs;
+  const int64_t bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * hs;
+  uint64_t cuts = slots * 3 / rows;
   cuts = cuts < 1 ? 1 : cuts > steps ? steps : cuts;
   p.chunk = (uint32_t)((steps + cuts - 1) / cuts);
   p.chunks = (uint32_t)((steps + p.chunk - 1) / p.chunk);
+  uint64_t batches = (slots * 3 + rows * p.chunks - 1) / (rows * p.chunks);
+  if (batches > d.batch || bs % (int64_t)n) batches = d.batch;
+  p.batch = (d.batch + batches - 1) / batches;
+  p.batches = (uint32_t)((d.batch + p.batch - 1) / p.batch);
   p.items = rows * p.batches * p.chunks;
   // As few CTAs as take no more turns than the most would.
   const uint64_t turns = (p.items + slots - 1) / slots;
@@ -297,9 +302,10 @@ template <class T> __device__ __forceinline__ typename AccOf<T>::type sum_of(con
 }
 
 // A warp walks along a row in steps of 32 vectors.  Steps that lie wholly in a
-// far range are only summed (18 instructions for 512 bytes of f16); in the others
-// every element adds into its bucket's sum, which each lane has for itself in
-// shared memory, found by a table of distances.
+// far range are only summed (18 instructions for 512 bytes of f16); the others
+// are summed over the batch entries, then every element adds into its bucket's
+// sum, which each lane has for itself in shared memory, found by a table of
+// distances.
 template <class T>
 __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a, const T* __restrict__ g,
@@ -355,57 +361,80 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
     b *= p.batch;
     const uint64_t b_end = min(a.batch, b + p.batch);
     const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)row * a.rs;
-    for (; b < b_end; b++, line += a.bs) {
-      const int shift = (int)(((uintptr_t)line / sizeof(T)) % N);  // elements behind a 16-byte boundary
-      const T* lane_at = line - shift + lane * N;
-      // Steps [l0, l1) lie in the left range, [r0, r1) in the right one.
-      const int l0 = shift ? 1 : 0, l1 = (min(r.left + 1, r.end) + shift) / kStep;
-      const int r0 = (r.right + shift + kStep - 1) / kStep, r1 = (r.end + shift) / kStep;
-      const int stop = min((int)((cut + 1) * p.chunk), r.end > 0 ? (r.end + shift + kStep - 1) / kStep : 0);
-      int i = (int)(cut * p.chunk);
-      while (i < stop) {
-        const bool left = i >= l0 && i < l1;
-        if (left || (i >= r0 && i < r1 && (i >= l0))) {
-          const int to = min(stop, left ? l1 : r1);
-          A s = 0;
-          for (; i + 4 <= to; i += 4) {
+    const int entries = (int)(b_end - b);
+    const int shift = (int)(((uintptr_t)line / sizeof(T)) % N);  // elements behind a 16-byte boundary, for all entries
+    const T* lane_at = line - shift + lane * N;
+    // Steps [l0, l1) lie in the left range, [r0, r1) in the right one.
+    const int l0 = shift ? 1 : 0, l1 = (min(r.left + 1, r.end) + shift) / kStep;
+    const int r0 = max(l0, (r.right + shift + kStep - 1) / kStep), r1 = (r.end + shift) / kStep;
+    const int stop = min((int)((cut + 1) * p.chunk), r.end > 0 ? (r.end + shift + kStep - 1) / kStep : 0);
+    int i = (int)(cut * p.chunk);
+    while (i < stop) {
+      const bool left = i >= l0 && i < l1;
+      if (left || (i >= r0 && i < r1)) {
+        const int to = min(stop, left ? l1 : r1);
+        A s = 0;
+        const T* at = lane_at;
+        for (int e = 0; e < entries; e++, at += a.bs) {
+          int j = i;
+          for (; j + 4 <= to; j += 4) {
             Vec<T> x[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) *(uint4*)&x[k] = __ldg((const uint4*)(lane_at + (int64_t)(i + k) * kStep));
+            for (int k = 0; k < 4; k++) *(uint4*)&x[k] = __ldg((const uint4*)(at + (int64_t)(j + k) * kStep));
             s += (sum_of(x[0]) + sum_of(x[1])) + (sum_of(x[2]) + sum_of(x[3]));
           }
-          for (; i < to; i++) {
+          for (; j < to; j++) {
             Vec<T> x;
-            *(uint4*)&x = __ldg((const uint4*)(lane_at + (int64_t)i * kStep));
+            *(uint4*)&x = __ldg((const uint4*)(at + (int64_t)j * kStep));
             s += sum_of(x);
           }
-          if (left) far_left += s;
-          else far_right += s;
-          continue;
         }
-        const int c = i * kStep + lane * N - shift;
-        i++;
-        if (max(c, 0) >= r.end) continue;
-        Vec<T> x;
-        if (c >= 0 && c + N <= a.keys) {
-          *(uint4*)&x = __ldg((const uint4*)(line + c));
-        } else {
+        if (left) far_left += s;
+        else far_right += s;
+        i = to;
+        continue;
+      }
+      const int c = i * kStep + lane * N - shift;
+      i++;
+      if (max(c, 0) >= r.end) continue;
+      A sum[N];
+#pragma unroll
+      for (int k = 0; k < N; k++) sum[k] = 0;
+      const T* at = line + c;
+      if (c >= 0 && c + N <= a.keys) {
+        int e = 0;
+        for (; e + 4 <= entries; e += 4, at += 4 * a.bs) {
+          Vec<T> x[4];
+#pragma unroll
+          for (int u = 0; u < 4; u++) *(uint4*)&x[u] = __ldg((const uint4*)(at + u * a.bs));
 #pragma unroll
           for (int k = 0; k < N; k++)
-            if (c + k >= 0 && c + k < r.end) x.e[k] = line[c + k];
+            sum[k] += (widen(x[0].e[k]) + widen(x[1].e[k])) + (widen(x[2].e[k]) + widen(x[3].e[k]));
         }
-        // (Lanes in a far range add into its bucket the same way: a branch of
-        // their own cost the warp more.)
-        const bool whole = c >= 0 && c + N <= r.end;
+        for (; e < entries; e++, at += a.bs) {
+          Vec<T> x;
+          *(uint4*)&x = __ldg((const uint4*)at);
+#pragma unroll
+          for (int k = 0; k < N; k++) sum[k] += widen(x.e[k]);
+        }
+      } else {
+        for (int e = 0; e < entries; e++, at += a.bs)
+#pragma unroll
+          for (int k = 0; k < N; k++)
+            if (c + k >= 0 && c + k < r.end) sum[k] += widen(at[k]);
+      }
+      // (Lanes in a far range add into its bucket the same way: a branch of
+      // their own cost the warp more.)
+      if (tabled && c >= 0 && c + N <= r.end) {
         const int d0 = c - query + far;
+#pragma unroll
+        for (int k = 0; k < N; k++) mine[offset[min(max(d0 + k, 0), 2 * far)]] += sum[k];
+      } else {
 #pragma unroll
         for (int k = 0; k < N; k++) {
           const int e = c + k;
-          if (!whole && (e < 0 || e >= r.end)) continue;
-          int at;
-          if (tabled) at = offset[min(max(d0 + k, 0), 2 * far)];
-          else at = 32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e));
-          mine[at] += widen(x.e[k]);
+          if (e >= 0 && e < r.end)
+            mine[32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e))] += sum[k];
         }
       }
     }
