@@ -595,11 +595,18 @@ def _room(t) -> int:
 
 
 def _need(t, what: str, elements: int, size: int) -> int:
+    """The tensor's pointer, once `elements` of `size` bytes are known to lie behind it."""
     if t.element_size() != size:
         raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
-    if _room(t) < elements:
+    if not (t.is_contiguous() and t.numel() >= elements) and _room(t) < elements:
         raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
     return t.data_ptr()
+
+
+def _bytes(workspace) -> int:
+    if not workspace.is_contiguous():
+        raise ValueError("workspace: not contiguous")
+    return workspace.numel() * workspace.element_size()
 
 
 def position_bias_async(plan: BiasPlan, table, out, *, positions=None, stream=None) -> None:
@@ -624,7 +631,7 @@ def position_bias_grad_async(plan: BiasPlan, grad, out, workspace, *, positions=
         plan.ref, _need(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype]),
         None if positions is None else _need(positions, "positions", plan.desc.queries, 4),
         _need(out, "out", plan.entries, 8 if plan.dtype == "f64" else 4), workspace.data_ptr(),
-        _room(workspace) * workspace.element_size(), _own_stream(stream, out)))
+        _bytes(workspace), _own_stream(stream, out)))
 
 
 class OrthPlan:
@@ -698,4 +705,4 @@ def orthogonalize_async(plan: OrthPlan, x, out, workspace, status, *, stream=Non
     _check(lib().dcf_orthogonalize_async(
         plan.ref, _need(x, "x", plan.in_elements, DTYPE_SIZE[plan.dtype]),
         _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.out_dtype]), workspace.data_ptr(),
-        _room(workspace) * workspace.element_size(), status.data_ptr(), _own_stream(stream, out)))
+        _bytes(workspace), _need(status, "status", 2, 8), _own_stream(stream, out)))

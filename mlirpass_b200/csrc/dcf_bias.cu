@@ -376,17 +376,14 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
         A s = 0;
         const T* at = lane_at;
         for (int e = 0; e < entries; e++, at += a.bs) {
-          int j = i;
-          for (; j + 4 <= to; j += 4) {
+          for (int j = i; j < to; j += 4) {  // four in flight, the last ones too
             Vec<T> x[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) *(uint4*)&x[k] = __ldg((const uint4*)(at + (int64_t)(j + k) * kStep));
+            for (int k = 0; k < 4; k++) {
+              *(uint4*)&x[k] = make_uint4(0, 0, 0, 0);
+              if (j + k < to) *(uint4*)&x[k] = __ldg((const uint4*)(at + (int64_t)(j + k) * kStep));
+            }
             s += (sum_of(x[0]) + sum_of(x[1])) + (sum_of(x[2]) + sum_of(x[3]));
-          }
-          for (; j < to; j++) {
-            Vec<T> x;
-            *(uint4*)&x = __ldg((const uint4*)(at + (int64_t)j * kStep));
-            s += sum_of(x);
           }
         }
         if (left) far_left += s;
@@ -402,20 +399,16 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
       for (int k = 0; k < N; k++) sum[k] = 0;
       const T* at = line + c;
       if (c >= 0 && c + N <= a.keys) {
-        int e = 0;
-        for (; e + 4 <= entries; e += 4, at += 4 * a.bs) {
+        for (int e = 0; e < entries; e += 4, at += 4 * a.bs) {
           Vec<T> x[4];
 #pragma unroll
-          for (int u = 0; u < 4; u++) *(uint4*)&x[u] = __ldg((const uint4*)(at + u * a.bs));
+          for (int u = 0; u < 4; u++) {
+            *(uint4*)&x[u] = make_uint4(0, 0, 0, 0);
+            if (e + u < entries) *(uint4*)&x[u] = __ldg((const uint4*)(at + u * a.bs));
+          }
 #pragma unroll
           for (int k = 0; k < N; k++)
             sum[k] += (widen(x[0].e[k]) + widen(x[1].e[k])) + (widen(x[2].e[k]) + widen(x[3].e[k]));
-        }
-        for (; e < entries; e++, at += a.bs) {
-          Vec<T> x;
-          *(uint4*)&x = __ldg((const uint4*)at);
-#pragma unroll
-          for (int k = 0; k < N; k++) sum[k] += widen(x.e[k]);
         }
       } else {
         for (int e = 0; e < entries; e++, at += a.bs)
@@ -423,9 +416,14 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
           for (int k = 0; k < N; k++)
             if (c + k >= 0 && c + k < r.end) sum[k] += widen(at[k]);
       }
+      if (c < 0 || c + N > r.end) {  // what lies outside adds nothing
+#pragma unroll
+        for (int k = 0; k < N; k++)
+          if (c + k < 0 || c + k >= r.end) sum[k] = 0;
+      }
       // (Lanes in a far range add into its bucket the same way: a branch of
       // their own cost the warp more.)
-      if (tabled && c >= 0 && c + N <= r.end) {
+      if (tabled) {
         const int d0 = c - query + far;
 #pragma unroll
         for (int k = 0; k < N; k++) mine[offset[min(max(d0 + k, 0), 2 * far)]] += sum[k];
@@ -433,8 +431,7 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
 #pragma unroll
         for (int k = 0; k < N; k++) {
           const int e = c + k;
-          if (e >= 0 && e < r.end)
-            mine[32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e))] += sum[k];
+          mine[32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e))] += sum[k];
         }
       }
     }
