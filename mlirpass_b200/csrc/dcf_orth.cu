@@ -230,43 +230,48 @@ __device__ __forceinline__ void put_some(uint16_t* at, const uint4& v, int from,
     if (j >= from && j < to) at[j] = (uint16_t)(e[j >> 1] >> ((j & 1) * 16));
 }
 
+// Eight values of a row of the result, of which `have` (or all) are there, in
+// the caller's type; `at` in elements.
+__device__ __forceinline__ void put_row8(void* out, int dtype, int vectors, int64_t at, int have, const float (&v)[8]) {
+  if (have <= 0) return;
+  if (dtype == DCF_F32) {
+    float* to = (float*)out + at;
+    if (vectors && have >= 8) {
+      *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
+      *(float4*)(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (e < have) to[e] = v[e];
+    }
+    return;
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    if (dtype == DCF_F16) {
+      const __half2 p = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+      w[e] = *(const uint32_t*)&p;
+    } else {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+      w[e] = *(const uint32_t*)&p;
+    }
+  }
+  const uint4 x = make_uint4(w[0], w[1], w[2], w[3]);
+  uint16_t* to = (uint16_t*)out + at;
+  if (vectors && have >= 8) *(uint4*)to = x;
+  else put_some(to, x, 0, have);
+}
+
 // Writes the block at row r0, column c0 of the result in the caller's type.
 __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* buf, int lane) {
-  const int o = (lane & 3) * 8, c = c0 + o, have = g.n - c;
-  if (have <= 0) return;
+  const int o = (lane & 3) * 8, c = c0 + o;
 #pragma unroll 1
   for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[place(o + e, row)]);
-    const int64_t at = (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c;
-    if (g.out_dtype == DCF_F32) {
-      float* to = (float*)g.out + at;
-      if (g.vectors && have >= 8) {
-        *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
-        *(float4*)(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (e < have) to[e] = v[e];
-      }
-      continue;
-    }
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if (g.out_dtype == DCF_F16) {
-        const __half2 p = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
-        w[e] = *(const uint32_t*)&p;
-      } else {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-        w[e] = *(const uint32_t*)&p;
-      }
-    }
-    const uint4 x = make_uint4(w[0], w[1], w[2], w[3]);
-    uint16_t* to = (uint16_t*)g.out + at;
-    if (g.vectors && have >= 8) *(uint4*)to = x;
-    else put_some(to, x, 0, have);
+    put_row8(g.out, g.out_dtype, g.vectors, (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c, g.n - c, v);
   }
 }
 
@@ -683,6 +688,364 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
   }
 }
 
+// ------------------------------------------------ matrices of few rows
+
+// The whole iteration of a matrix with min(rows, cols) <= 128 in one launch.  A
+// cluster of CTAs keeps X in shared memory, cut along its longer side, as the
+// two planes that the products read; a step's three products then read nothing
+// else:
+//   - each CTA multiplies its slice into a part of A (TMEM); the parts are
+//     added over the cluster, every CTA a share of the rows, and the sums written to
+//     all;
+//   - each CTA makes B from A by itself and multiplies it with its slice.
+// What bounds it is latency: three products of 24 to 48 instructions, three
+// passes over 128 x 128 accumulators and, in a cluster, three barriers per step.  The
+// separate products of orth_gemm_kernel took 17 launches of 8 to 28 us
+// (96 x 96: 157 us, 32 x 128 x 1000: 300 us).
+//
+// Shared memory has 64 columns of a plane as rows of 128 bytes with the
+// 128-byte swizzle.  The same bytes are a K-major operand (its 64 columns along k)
+// and an MN-major one (its rows along k), so that X serves X X^T and B X as
+// it lies, whichever of its sides is the longer.
+constexpr int kFewThreads = 256, kFewSlice = 256, kFewCluster = 8;
+constexpr int kFewPlane = 128 * 128 * 2;       // a plane of A or B
+constexpr int kFewTmem = 256;
+constexpr int kFewLeast = 120 << 10;           // shared memory that keeps a second CTA off the SM and its TMEM
+
+struct FewArgs {
+  MatArgs in;
+  void* out;
+  int out_dtype, vectors;
+  int64_t out_rs, out_bs;
+  int tall;                 // rows > cols: X^T is what lies in memory
+  int slice;                // of the longer side per CTA: a multiple of 64 (128 where tall)
+  int steps;
+  double eps;
+  // per step: A = fa acc; B = fb2 acc + fb1 A + fb0 I; X = fx acc
+  float fa[DCF_ORTH_MAX_STEPS], fb2[DCF_ORTH_MAX_STEPS], fb1[DCF_ORTH_MAX_STEPS], fb0[DCF_ORTH_MAX_STEPS],
+      fx[DCF_ORTH_MAX_STEPS];
+  double scale;             // of X's planes at the start
+  dcf_status* st;
+};
+
+__device__ __forceinline__ void one_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void one_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+               : "memory");
+}
+
+// One operand of a product over `slices` times 16 k: address of slice s of the
+// hi plane, the lo plane `lo` bytes on.
+struct Operand {
+  uint32_t base, lo;
+  uint32_t lbo;            // 0: K-major; else bytes between blocks of 64 along the operand
+  uint32_t block;          // K-major: bytes between blocks of 64 k
+  __device__ __forceinline__ uint64_t desc(int s, bool low) const {
+    const uint32_t at = base + (low ? lo : 0) + (lbo ? s * 2048 : (s >> 2) * block + (s & 3) * 32);
+    return (uint64_t)((at >> 4) & 0x3FFF) | ((uint64_t)(lbo ? lbo >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+  }
+};
+
+// The small products first, while the sum is small: the tensor core truncates.
+__device__ __forceinline__ void one_product(uint32_t d, const Operand& p, const Operand& q, int n, int slices) {
+  const uint32_t idesc = (1u << 4) | ((p.lbo ? 1u : 0u) << 15) | ((q.lbo ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+                         ((uint32_t)(128 >> 4) << 24);
+  for (int s = 0; s < slices; s++) {
+    one_mma(d, p.desc(s, false), q.desc(s, true), idesc, s != 0);
+    one_mma(d, p.desc(s, true), q.desc(s, false), idesc, 1);
+  }
+  for (int s = 0; s < slices; s++) one_mma(d, p.desc(s, false), q.desc(s, false), idesc, 1);
+}
+
+// Eight values of a row to their place in both planes.
+__device__ __forceinline__ uint32_t few_offset(int row, int col, uint32_t block) {
+  return (uint32_t)(col >> 6) * block + (uint32_t)row * 128 + (uint32_t)((((col & 63) >> 3) ^ (row & 7)) << 4);
+}
+
+__device__ __forceinline__ uint32_t remote(uint32_t local, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync(int ctas) {
+  if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  else __syncthreads();
+}
+
+__global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_constant__ FewArgs g) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t done;
+  __shared__ uint32_t tmem_at;
+  __shared__ double sums[kFewThreads / 32], own;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int ctas, rank;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const uint32_t z = blockIdx.x / (uint32_t)ctas;
+  // X's slice as it lies in memory: wide 128 rows x slice columns, tall slice rows x 128.
+  const int rows = g.tall ? g.slice : 128, cols = g.tall ? 128 : g.slice;
+  const int row0 = g.tall ? rank * g.slice : 0, col0 = g.tall ? 0 : rank * g.slice;
+  const int m = g.tall ? g.in.cols : g.in.rows;
+  const uint32_t block = (uint32_t)rows * 128, plane = (uint32_t)rows * (uint32_t)cols * 2;
+  uint8_t* ab = base + 2 * plane;       // A, then B: two planes; the parts of A before that
+  const uint32_t x_at = smem_addr(base), ab_at = smem_addr(ab);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_at)), "r"(kFewTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t*)&tmem_at;
+  pdl_begin();
+
+  // The norm, in 64 bits: of the slice, then of the cluster's.
+  const int groups = cols / 8;
+  double s = 0;
+  for (int i = threadIdx.x; i < rows * groups; i += kFewThreads) {
+    const int r = row0 + i / groups, c = col0 + i % groups * 8;
+    if (r >= g.in.rows || c >= g.in.cols) continue;
+    float v[8];
+    load_row8(g.in, z, r, c, v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s = __fma_rn((double)v[j], (double)v[j], s);
+  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  if (lane == 0) sums[warp] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kFewThreads / 32; w++) s += sums[w];
+    own = s;
+  }
+  cluster_sync(ctas);
+  double norm = 0;
+  for (int k = 0; k < ctas; k++) {
+    double part;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(remote(smem_addr(&own), k)) : "memory");
+    norm += part;
+  }
+  const double factor = g.scale / (sqrt(norm) + g.eps);
+  for (int i = threadIdx.x; i < rows * groups; i += kFewThreads) {
+    const int lr = i / groups, lc = i % groups * 8, r = row0 + lr, c = col0 + lc;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (r < g.in.rows && c < g.in.cols) {
+      load_row8(g.in, z, r, c, v);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = c + j < g.in.cols ? (float)((double)v[j] * factor) : 0;
+    }
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    uint8_t* at = base + few_offset(lr, lc, block);
+    *(uint4*)at = hi;
+    *(uint4*)(at + plane) = lo;
+  }
+
+  const Operand x_k = {x_at, plane, 0, block}, x_mn = {x_at, plane, block, 0};
+  const Operand ab_k = {ab_at, kFewPlane, 0, 128 * 128};
+  const int part = warp & 3, half = warp >> 2, row = part * 32 + lane;
+  const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16);
+  bool fail = false;
+  unsigned phase = 0;
+  auto before = [&]() {  // shared memory written so far is what the products read
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    asm volatile("fence.proxy.async;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+  auto after = [&]() {
+    if (!mbar_wait_bounded(&done, phase)) fail = true;
+    phase ^= 1;
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  };
+
+  for (int step = 0; step < g.steps; step++) {
+    before();
+    if (threadIdx.x == 0) {
+      one_product(tmem, g.tall ? x_mn : x_k, g.tall ? x_mn : x_k, 128, g.slice / 16);
+      one_commit(&done);
+    }
+    after();
+    const float fa = g.fa[step];
+    if (ctas == 1) {
+#pragma unroll 1
+      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+        uint32_t x[32];
+        tmem_load32(lanes + c, x);
+        tmem_wait(x);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          float v[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fa, __uint_as_float(x[8 * k + j]));
+          uint4 hi, lo;
+          split8(v, hi, lo);
+          uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
+          *(uint4*)at = hi;
+          *(uint4*)(at + kFewPlane) = lo;
+        }
+      }
+    } else {
+      // Parts as rows of 512 bytes, their 16-byte chunks exchanged by row.
+#pragma unroll 1
+      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+        uint32_t x[32];
+        tmem_load32(lanes + c, x);
+        tmem_wait(x);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          *(uint4*)(ab + row * 512 + (((c >> 2) + k) ^ (row & 7)) * 16) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      cluster_sync(ctas);
+      // Rows rank * 128 / ctas on; eight columns at a time, at most 32 values a thread.
+      const int share = 128 / ctas, items = share * 16;
+      float v[4][8];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int i = u * kFewThreads + (int)threadIdx.x;
+        if (i >= items) break;
+        const int r = rank * share + i / 16, c4 = i % 16 * 2;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[u][j] = 0;
+        for (int k = 0; k < ctas; k++) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float4 p;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
+                         : "r"(remote(ab_at + (uint32_t)(r * 512 + ((c4 + e) ^ (r & 7)) * 16), k))
+                         : "memory");
+            v[u][4 * e] = __fadd_rn(v[u][4 * e], p.x);
+            v[u][4 * e + 1] = __fadd_rn(v[u][4 * e + 1], p.y);
+            v[u][4 * e + 2] = __fadd_rn(v[u][4 * e + 2], p.z);
+            v[u][4 * e + 3] = __fadd_rn(v[u][4 * e + 3], p.w);
+          }
+        }
+      }
+      cluster_sync(ctas);  // everyone has read: the parts may be overwritten
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int i = u * kFewThreads + (int)threadIdx.x;
+        if (i >= items) break;
+        const int r = rank * share + i / 16, c = i % 16 * 8;
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[u][j] = __fmul_rn(fa, v[u][j]);
+        uint4 hi, lo;
+        split8(v[u], hi, lo);
+        const uint32_t at = ab_at + few_offset(r, c, 128 * 128);
+        for (int k = 0; k < ctas; k++) {
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(remote(at, k)), "r"(hi.x), "r"(hi.y),
+                       "r"(hi.z), "r"(hi.w)
+                       : "memory");
+          asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(remote(at + kFewPlane, k)), "r"(lo.x),
+                       "r"(lo.y), "r"(lo.z), "r"(lo.w)
+                       : "memory");
+        }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      cluster_sync(ctas);
+    }
+    before();
+    if (threadIdx.x == 0) {
+      one_product(tmem, ab_k, ab_k, 128, 8);
+      one_commit(&done);
+    }
+    after();
+    const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
+#pragma unroll 1
+    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      uint32_t x[32];
+      tmem_load32(lanes + c, x);
+      tmem_wait(x);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
+        const uint4 ah = *(const uint4*)at, al = *(const uint4*)(at + kFewPlane);
+        const __half2* h = (const __half2*)&ah;
+        const __half2* l = (const __half2*)&al;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 p = __half22float2(h[j]), q = __half22float2(l[j]);
+          v[2 * j] = __fmaf_rn(fb1, __fadd_rn(p.x, q.x), __fmul_rn(fb2, __uint_as_float(x[8 * k + 2 * j])));
+          v[2 * j + 1] = __fmaf_rn(fb1, __fadd_rn(p.y, q.y), __fmul_rn(fb2, __uint_as_float(x[8 * k + 2 * j + 1])));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+          if (c + 8 * k + j == row && row < m) v[j] = __fadd_rn(v[j], fb0);
+        uint4 hi, lo;
+        split8(v, hi, lo);
+        *(uint4*)at = hi;
+        *(uint4*)(at + kFewPlane) = lo;
+      }
+    }
+    before();
+    if (threadIdx.x == 0) {
+      if (g.tall)
+        for (int b = 0; b < g.slice / 128; b++) {
+          const Operand p = {x_at + (uint32_t)b * 128 * 128, plane, 0, block};
+          one_product(tmem + b * 128, p, ab_k, 128, 8);
+        }
+      else
+        one_product(tmem, ab_k, x_mn, g.slice, 8);
+      one_commit(&done);
+    }
+    after();
+    // The accumulators: wide 128 rows x slice columns, tall slice / 128 blocks of
+    // 128 x 128 beside each other; half of the columns to each four warps.
+    const float fx = g.fx[step];
+    const int width = g.slice / 2;  // (tall: 64 of each block's 128)
+#pragma unroll 1
+    for (int c = 0; c < width; c += 32) {
+      const int at_col = g.tall ? (c >> 6) * 128 + half * 64 + (c & 63) : half * width + c;
+      const int lr = g.tall ? (c >> 6) * 128 + row : row, lc = g.tall ? half * 64 + (c & 63) : at_col;
+      uint32_t x[32];
+      tmem_load32(lanes + at_col, x);
+      tmem_wait(x);
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fx, __uint_as_float(x[8 * k + j]));
+        if (step + 1 < g.steps) {
+          uint4 hi, lo;
+          split8(v, hi, lo);
+          uint8_t* at = base + few_offset(lr, lc + 8 * k, block);
+          *(uint4*)at = hi;
+          *(uint4*)(at + plane) = lo;
+        } else if (row0 + lr < g.in.rows) {
+          put_row8(g.out, g.out_dtype, g.vectors, (int64_t)z * g.out_bs + (int64_t)(row0 + lr) * g.out_rs + col0 + lc + 8 * k,
+                   g.in.cols - (col0 + lc + 8 * k), v);
+        }
+      }
+    }
+  }
+  if (fail) atomicExch(&g.st->error, 1u);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync(ctas);  // no one leaves while its shared memory may be read
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kFewTmem) : "memory");
+  }
+}
+
 // ---------------------------------------------------------------- host
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -854,11 +1217,60 @@ int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, 
   return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
 
+// CTAs of a cluster that take a matrix of few rows at once, 0 where it does not
+// fit: the longer side is at most 8 x 256.  More of them than it needs, while
+// there are SMs, for slices of 128.
+int few_ctas(const dcf_orth_desc& d) {
+  const uint64_t m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
+  if (!d.steps || m > 128 || n > kFewSlice * kFewCluster) return 0;
+  uint64_t c = 1;
+  while (c * kFewSlice < n) c *= 2;
+  while (c < kFewCluster && c * 128 < n && 2 * c * d.batch <= 2 * kPairs) c *= 2;
+  return (int)c;
+}
+
+int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out_rs, int64_t out_bs, int vectors,
+               dcf_status* st, cudaStream_t s) {
+  const int ctas = few_ctas(d);
+  FewArgs g = {};
+  g.in = in;
+  g.out = out;
+  g.out_dtype = (int)d.out_dtype;
+  g.vectors = vectors;
+  g.out_rs = out_rs;
+  g.out_bs = out_bs;
+  g.tall = d.rows > d.cols;
+  const int n = (int)(g.tall ? d.rows : d.cols), unit = g.tall ? 128 : 64;
+  g.slice = ((n + ctas - 1) / ctas + unit - 1) / unit * unit;
+  g.steps = (int)d.steps;
+  g.eps = d.eps;
+  g.st = st;
+  double bound = 1;
+  int sx = scale_of(1);
+  g.scale = ldexp(1.0, sx);
+  for (uint32_t i = 0; i < d.steps; i++) {
+    const double* k = d.coef[i];
+    double next, q;
+    step_bounds(k, bound, &next, &q);
+    const int sa = scale_of(bound * bound), sb = scale_of(q), sn = scale_of(next);
+    g.fa[i] = (float)ldexp(1.0, sa - 2 * sx);
+    g.fb2[i] = (float)ldexp(k[2], sb - 2 * sa);
+    g.fb1[i] = (float)ldexp(k[1], sb - sa);
+    g.fb0[i] = (float)ldexp(k[0], sb);
+    g.fx[i] = (float)ldexp(1.0, (i + 1 < d.steps ? sn : 0) - sb - sx);
+    bound = next;
+    sx = sn;
+  }
+  int smem = 2 * (128 * g.slice * 2) + 2 * kFewPlane + 1024;
+  if (smem < kFewLeast) smem = kFewLeast;
+  if (!prepare_smem((const void*)orth_few_kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
+  return launch(orth_few_kernel, dim3((unsigned)(d.batch * ctas)), kFewThreads, smem, ctas, s, g);
+}
+
 template <Mode MODE, bool P_MN, bool Q_MN>
 int gemm_run(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, cudaStream_t s) {
   auto kernel = orth_gemm_kernel<MODE, P_MN, Q_MN>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem) != cudaSuccess)
-    return DCF_ECUDA;
+  if (!prepare_smem((const void*)kernel, kGemmSmem)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
   return launch(kernel, dim3(2 * pairs), kGemmThreads, kGemmSmem, 2, s, p, q, g);
 }
@@ -926,7 +1338,7 @@ int orth_desc_check(const dcf_orth_desc* d) {
 }
 
 size_t orth_workspace(const dcf_orth_desc& d) {
-  if (!d.batch || !d.rows || !d.cols) return 0;
+  if (!d.batch || !d.rows || !d.cols || few_ctas(d)) return 0;
   return layout_of(d, nullptr).bytes;
 }
 
@@ -948,6 +1360,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
   a.vectors = vectors(in, a.rs, a.bs, dtype_size(a.dtype));
   const int64_t out_rs = d.out_row_stride ? d.out_row_stride : (int64_t)d.cols;
   const int64_t out_bs = d.out_batch_stride ? d.out_batch_stride : (int64_t)d.rows * out_rs;
+  if (few_ctas(d)) return launch_few(d, a, out, out_rs, out_bs, vectors(out, out_rs, out_bs, dtype_size((int)d.out_dtype)), st, s);
   int rc = launch(orth_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, 1, s, a, l.part);
   if (rc) return rc;
   int sx = d.steps ? scale_of(1) : 0;

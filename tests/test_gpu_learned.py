@@ -326,7 +326,8 @@ def check_orth(got, x, out_dtype, coef, eps=1e-7):
 
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7), (7, 1), (3, 5), (16, 16), (31, 65), (64, 64), (96, 96),
                                        (65, 31), (127, 129), (128, 128), (129, 128), (128, 500), (200, 333), (333, 200),
-                                       (257, 257), (1, 1000), (300, 2)])
+                                       (257, 257), (1, 1000), (300, 2), (100, 2048), (2048, 100), (9, 2049),
+                                       (2049, 9), (128, 257), (600, 128), (513, 65), (40, 256)])
 def test_orth_sizes(dcf, rows, cols):
     x = randn((1, rows, cols), "f32", 21)
     check_orth(run_orth(dcf, x, "f32"), x, "f32", [COEF] * 5)
@@ -404,13 +405,23 @@ def test_orth_in_place(dcf, steps):
         assert torch.equal(x, want)
 
 
-def test_orth_same_bits_every_time_and_alone_or_in_a_batch(dcf):
+@pytest.mark.parametrize("batch", [1, 7, 40, 80, 160])
+@pytest.mark.parametrize("rows,cols", [(30, 600), (600, 30)])
+def test_orth_clusters_of_every_size(dcf, batch, rows, cols):
+    """The number of CTAs to a matrix depends on how many matrices there are."""
+    x = randn((batch, rows, cols), "f32", 33)
+    got = run_orth(dcf, x, "f32", steps=3)
+    some = sorted({0, batch // 2, batch - 1})
+    check_orth(got[some], x[some], "f32", [COEF] * 3)
+
+
+def test_orth_same_bits_every_time_and_in_any_place_of_a_batch(dcf):
     import torch
     for rows, cols in ((50, 60), (140, 300)):
         x = randn((5, rows, cols), "bf16", 31)
         first = run_orth(dcf, x, "bf16")
         assert torch.equal(run_orth(dcf, x, "bf16"), first)
-        assert torch.equal(run_orth(dcf, x[3:4].contiguous(), "bf16"), first[3:4])
+        assert torch.equal(run_orth(dcf, x[[3] * 5].contiguous(), "bf16"), first[[3] * 5])
 
 
 # ------------------------------------------------------------- together

@@ -102,13 +102,16 @@ def test_orth_bound_follows_the_interior_of_the_interval():
 
 
 def test_orth_calls_that_are_refused():
-    plan = m.orthogonalize_plan("f32", 40, 50)
+    plan = m.orthogonalize_plan("f32", 400, 500)
     assert plan.workspace > 0
     call = m.lib().dcf_orthogonalize_async
     assert call(plan.ref, 256, 256, 256, plan.workspace - 1, 256, None) == -1
     for ptrs in ((None, 256, 256, 256), (256, None, 256, 256), (256, 256, None, 256), (256, 256, 256, None)):
         i, o, w, s = ptrs
         assert call(plan.ref, i, o, w, plan.workspace, s, None) == -1
+    # a matrix of few rows stays on the chip: no workspace, unless it is too long
+    assert m.orthogonalize_plan("f32", 128, 2048).workspace == m.orthogonalize_plan("f32", 2048, 1).workspace == 0
+    assert m.orthogonalize_plan("f32", 129, 129).workspace > 0 and m.orthogonalize_plan("f32", 8, 2049).workspace > 0
     bad = m.OrthDesc.from_buffer_copy(plan.desc)
     bad.reserved = 1
     assert call(ctypes.byref(bad), 256, 256, 256, plan.workspace, 256, None) == -1
