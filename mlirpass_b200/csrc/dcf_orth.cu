@@ -362,9 +362,9 @@ __device__ __forceinline__ float* part_block(float* part, int64_t item, int bloc
 // instruction: 1e-4 in the result over k = 8192.  So TMEM sums `sum` stages
 // only (the two small products of a stage first, then the large one), in two
 // buffers in turn, and the eight warps add the sums in registers, rounding to
-// nearest: 2 stages where the result is f32 (3e-6 there), 16 where it is rounded to
-// 16 bits anyway (1e-5), which leaves the warps time to write a tile while the
-// next is multiplied.
+// nearest: every stage where the result is f32 (3e-6 there; two stages: 6e-6,
+// and plain fp32 products 5e-6), 16 where it is rounded to 16 bits anyway (1e-5),
+// which leaves the warps time to write a tile while the next is multiplied.
 template <Mode MODE, bool P_MN, bool Q_MN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
 // it lies, whichever of its sides is the longer.
 constexpr int kFewThreads = 256, kFewSlice = 256, kFewCluster = 8;
 constexpr int kFewPlane = 128 * 128 * 2;       // a plane of A or B
-constexpr int kFewTmem = 256;
+constexpr int kFewTmem = 512;
 constexpr int kFewLeast = 120 << 10;           // shared memory that keeps a second CTA off the SM and its TMEM
 
 struct FewArgs {
@@ -753,15 +753,36 @@ struct Operand {
   }
 };
 
-// The small products first, while the sum is small: the tensor core truncates.
-__device__ __forceinline__ void one_product(uint32_t d, const Operand& p, const Operand& q, int n, int slices) {
+// Each 64 k have an accumulator of their own, `pitch` columns after the last, and
+// the small products come first, while its sum is small: the tensor core truncates.
+constexpr int kFewChunk = 4;  // slices of 16
+__device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int slices) {
   const uint32_t idesc = (1u << 4) | ((p.lbo ? 1u : 0u) << 15) | ((q.lbo ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
                          ((uint32_t)(128 >> 4) << 24);
-  for (int s = 0; s < slices; s++) {
-    one_mma(d, p.desc(s, false), q.desc(s, true), idesc, s != 0);
-    one_mma(d, p.desc(s, true), q.desc(s, false), idesc, 1);
+  for (int c = 0; c < slices; c += kFewChunk, d += pitch) {
+    for (int s = c; s < c + kFewChunk; s++) {
+      one_mma(d, p.desc(s, false), q.desc(s, true), idesc, s != c);
+      one_mma(d, p.desc(s, true), q.desc(s, false), idesc, 1);
+    }
+    for (int s = c; s < c + kFewChunk; s++) one_mma(d, p.desc(s, false), q.desc(s, false), idesc, 1);
   }
-  for (int s = 0; s < slices; s++) one_mma(d, p.desc(s, false), q.desc(s, false), idesc, 1);
+}
+
+// 32 columns of a product: its accumulators' sum.
+__device__ __forceinline__ void product_of(uint32_t addr, int pitch, int chunks, float (&v)[32]) {
+  uint32_t x[32];
+  tmem_load32(addr, x);
+  tmem_wait(x);
+#pragma unroll
+  for (int j = 0; j < 32; j++) v[j] = __uint_as_float(x[j]);
+#pragma unroll 1
+  for (int c = 1; c < chunks; c++) {
+    addr += pitch;
+    tmem_load32(addr, x);
+    tmem_wait(x);
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = __fadd_rn(v[j], __uint_as_float(x[j]));
+  }
 }
 
 // Eight values of a row to their place in both planes.
@@ -877,7 +898,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   for (int step = 0; step < g.steps; step++) {
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, g.tall ? x_mn : x_k, g.tall ? x_mn : x_k, 128, g.slice / 16);
+      one_product(tmem, 128, g.tall ? x_mn : x_k, g.tall ? x_mn : x_k, 128, g.slice / 16);
       one_commit(&done);
     }
     after();
@@ -885,14 +906,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     if (ctas == 1) {
 #pragma unroll 1
       for (int c = half * 64; c < half * 64 + 64; c += 32) {
-        uint32_t x[32];
-        tmem_load32(lanes + c, x);
-        tmem_wait(x);
+        float x[32];
+        product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           float v[8];
 #pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fa, __uint_as_float(x[8 * k + j]));
+          for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fa, x[8 * k + j]);
           uint4 hi, lo;
           split8(v, hi, lo);
           uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
@@ -904,12 +924,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
       // Parts as rows of 512 bytes, their 16-byte chunks exchanged by row.
 #pragma unroll 1
       for (int c = half * 64; c < half * 64 + 64; c += 32) {
-        uint32_t x[32];
-        tmem_load32(lanes + c, x);
-        tmem_wait(x);
+        float x[32];
+        product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          *(uint4*)(ab + row * 512 + (((c >> 2) + k) ^ (row & 7)) * 16) = make_uint4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+          *(float4*)(ab + row * 512 + (((c >> 2) + k) ^ (row & 7)) * 16) =
+              make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       cluster_sync(ctas);
@@ -963,16 +983,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     }
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, ab_k, ab_k, 128, 8);
+      one_product(tmem, 128, ab_k, ab_k, 128, 8);
       one_commit(&done);
     }
     after();
     const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
 #pragma unroll 1
     for (int c = half * 64; c < half * 64 + 64; c += 32) {
-      uint32_t x[32];
-      tmem_load32(lanes + c, x);
-      tmem_wait(x);
+      float x[32];
+      product_of(lanes + c, 128, 2, x);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
@@ -983,8 +1002,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const float2 p = __half22float2(h[j]), q = __half22float2(l[j]);
-          v[2 * j] = __fmaf_rn(fb1, __fadd_rn(p.x, q.x), __fmul_rn(fb2, __uint_as_float(x[8 * k + 2 * j])));
-          v[2 * j + 1] = __fmaf_rn(fb1, __fadd_rn(p.y, q.y), __fmul_rn(fb2, __uint_as_float(x[8 * k + 2 * j + 1])));
+          v[2 * j] = __fmaf_rn(fb1, __fadd_rn(p.x, q.x), __fmul_rn(fb2, x[8 * k + 2 * j]));
+          v[2 * j + 1] = __fmaf_rn(fb1, __fadd_rn(p.y, q.y), __fmul_rn(fb2, x[8 * k + 2 * j + 1]));
         }
 #pragma unroll
         for (int j = 0; j < 8; j++)
@@ -1000,10 +1019,10 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
       if (g.tall)
         for (int b = 0; b < g.slice / 128; b++) {
           const Operand p = {x_at + (uint32_t)b * 128 * 128, plane, 0, block};
-          one_product(tmem + b * 128, p, ab_k, 128, 8);
+          one_product(tmem + b * 128, g.slice, p, ab_k, 128, 8);
         }
       else
-        one_product(tmem, ab_k, x_mn, g.slice, 8);
+        one_product(tmem, g.slice, ab_k, x_mn, g.slice, 8);
       one_commit(&done);
     }
     after();
@@ -1015,14 +1034,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     for (int c = 0; c < width; c += 32) {
       const int at_col = g.tall ? (c >> 6) * 128 + half * 64 + (c & 63) : half * width + c;
       const int lr = g.tall ? (c >> 6) * 128 + row : row, lc = g.tall ? half * 64 + (c & 63) : at_col;
-      uint32_t x[32];
-      tmem_load32(lanes + at_col, x);
-      tmem_wait(x);
+      float x[32];
+      product_of(lanes + at_col, g.slice, 2, x);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fx, __uint_as_float(x[8 * k + j]));
+        for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fx, x[8 * k + j]);
         if (step + 1 < g.steps) {
           uint4 hi, lo;
           split8(v, hi, lo);
@@ -1385,7 +1403,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     const CUtensorMap& x = mx[i & 1];
     GemmArgs g = {};
     g.st = st;
-    g.sum = d.out_dtype == DCF_F32 ? 2 : 16;
+    g.sum = d.out_dtype == DCF_F32 ? 1 : 16;
     g.part = l.sums;
     g.m = g.n = m;
     g.k = n;
