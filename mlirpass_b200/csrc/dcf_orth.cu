@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
 // 128-byte swizzle.  The same bytes are a K-major operand (its 64 columns along k)
 // and an MN-major one (its rows along k), so that X serves X X^T and B X as
 // it lies, whichever of its sides is the longer.
-constexpr int kFewThreads = 256, kFewSlice = 256, kFewCluster = 8;
+constexpr int kFewThreads = 512, kFewSlice = 256, kFewCluster = 8;
 constexpr int kFewPlane = 128 * 128 * 2;       // a plane of A or B
 constexpr int kFewTmem = 512;
 constexpr int kFewLeast = 120 << 10;           // shared memory that keeps a second CTA off the SM and its TMEM
@@ -740,31 +740,40 @@ __device__ __forceinline__ void one_commit(uint64_t* bar) {
                : "memory");
 }
 
-// One operand of a product over `slices` times 16 k: address of slice s of the
-// hi plane, the lo plane `lo` bytes on.
+// One operand of a product: descriptors of its first 16 k in both planes, and
+// how far on the next 16 and the next 64 are.
 struct Operand {
-  uint32_t base, lo;
-  uint32_t lbo;            // 0: K-major; else bytes between blocks of 64 along the operand
-  uint32_t block;          // K-major: bytes between blocks of 64 k
-  __device__ __forceinline__ uint64_t desc(int s, bool low) const {
-    const uint32_t at = base + (low ? lo : 0) + (lbo ? s * 2048 : (s >> 2) * block + (s & 3) * 32);
-    return (uint64_t)((at >> 4) & 0x3FFF) | ((uint64_t)(lbo ? lbo >> 4 : 1) << 16) | (64ull << 32) | (1ull << 46) |
-           (2ull << 61);
-  }
+  uint64_t hi, lo;
+  uint32_t step, chunk, mn;
 };
+
+__device__ __forceinline__ Operand k_major(uint32_t at, uint32_t plane, uint32_t block) {  // blocks of 64 k
+  return {smem_desc<false>(at), smem_desc<false>(at + plane), 32 >> 4, block >> 4, 0};
+}
+
+__device__ __forceinline__ Operand mn_major(uint32_t at, uint32_t plane, uint32_t block) {  // blocks of 64 along the operand
+  const uint64_t far = ((uint64_t)(block >> 4) << 16) - (1ull << 16);
+  return {smem_desc<false>(at) + far, smem_desc<false>(at + plane) + far, 2048 >> 4, 4 * (2048 >> 4), 1};
+}
 
 // Each 64 k have an accumulator of their own, `pitch` columns after the last, and
 // the small products come first, while its sum is small: the tensor core truncates.
-constexpr int kFewChunk = 4;  // slices of 16
-__device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int slices) {
-  const uint32_t idesc = (1u << 4) | ((p.lbo ? 1u : 0u) << 15) | ((q.lbo ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
-                         ((uint32_t)(128 >> 4) << 24);
-  for (int c = 0; c < slices; c += kFewChunk, d += pitch) {
-    for (int s = c; s < c + kFewChunk; s++) {
-      one_mma(d, p.desc(s, false), q.desc(s, true), idesc, s != c);
-      one_mma(d, p.desc(s, true), q.desc(s, false), idesc, 1);
+__device__ __forceinline__ void one_product(uint32_t d, int pitch, Operand p, Operand q, int n, int chunks) {
+  const uint32_t idesc =
+      (1u << 4) | (p.mn << 15) | (q.mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+#pragma unroll 1
+  for (int c = 0; c < chunks; c++, d += pitch) {
+#pragma unroll
+    for (uint32_t s = 0; s < 4; s++) {
+      one_mma(d, p.hi + s * p.step, q.lo + s * q.step, idesc, s);
+      one_mma(d, p.lo + s * p.step, q.hi + s * q.step, idesc, 1);
     }
-    for (int s = c; s < c + kFewChunk; s++) one_mma(d, p.desc(s, false), q.desc(s, false), idesc, 1);
+#pragma unroll
+    for (uint32_t s = 0; s < 4; s++) one_mma(d, p.hi + s * p.step, q.hi + s * q.step, idesc, 1);
+    p.hi += p.chunk;
+    p.lo += p.chunk;
+    q.hi += q.chunk;
+    q.lo += q.chunk;
   }
 }
 
@@ -838,6 +847,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   // The norm, in 64 bits: of the slice, then of the cluster's.
   const int groups = cols / 8;
   double s = 0;
+#pragma unroll 2
   for (int i = threadIdx.x; i < rows * groups; i += kFewThreads) {
     const int r = row0 + i / groups, c = col0 + i % groups * 8;
     if (r >= g.in.rows || c >= g.in.cols) continue;
@@ -876,9 +886,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     *(uint4*)(at + plane) = lo;
   }
 
-  const Operand x_k = {x_at, plane, 0, block}, x_mn = {x_at, plane, block, 0};
-  const Operand ab_k = {ab_at, kFewPlane, 0, 128 * 128};
-  const int part = warp & 3, half = warp >> 2, row = part * 32 + lane;
+  const Operand x_mn = mn_major(x_at, plane, block), ab_k = k_major(ab_at, kFewPlane, 128 * 128);
+  const Operand x_gram = g.tall ? x_mn : k_major(x_at, plane, block);
+  const int part = warp & 3, quarter = warp >> 2, row = part * 32 + lane;  // TMEM lanes; columns
   const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16);
   bool fail = false;
   unsigned phase = 0;
@@ -898,14 +908,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   for (int step = 0; step < g.steps; step++) {
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, 128, g.tall ? x_mn : x_k, g.tall ? x_mn : x_k, 128, g.slice / 16);
+      one_product(tmem, 128, x_gram, x_gram, 128, g.slice / 64);
       one_commit(&done);
     }
     after();
     const float fa = g.fa[step];
+    const int c = quarter * 32;
     if (ctas == 1) {
-#pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      {
         float x[32];
         product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
@@ -922,8 +932,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
       }
     } else {
       // Parts as rows of 512 bytes, their 16-byte chunks exchanged by row.
-#pragma unroll 1
-      for (int c = half * 64; c < half * 64 + 64; c += 32) {
+      {
         float x[32];
         product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
@@ -933,34 +942,36 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
       }
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       cluster_sync(ctas);
-      // Rows rank * 128 / ctas on; eight columns at a time, at most 32 values a thread.
+      // Rows rank * 128 / ctas on, eight columns at a time: 16 values a thread at most.
       const int share = 128 / ctas, items = share * 16;
-      float v[4][8];
+      float v[2][8];
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
+      for (int u = 0; u < 2; u++) {
         const int i = u * kFewThreads + (int)threadIdx.x;
         if (i >= items) break;
         const int r = rank * share + i / 16, c4 = i % 16 * 2;
+        const uint32_t at0 = ab_at + (uint32_t)(r * 512 + (c4 ^ (r & 7)) * 16), at1 = ab_at + (uint32_t)(r * 512 + ((c4 + 1) ^ (r & 7)) * 16);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[u][j] = 0;
-        for (int k = 0; k < ctas; k++) {
+        for (int k = 0; k < ctas; k += 2) {  // four loads in flight
+          float4 p[4];
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float4 p;
+          for (int e = 0; e < 4; e++)
             asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(p.x), "=f"(p.y), "=f"(p.z), "=f"(p.w)
-                         : "r"(remote(ab_at + (uint32_t)(r * 512 + ((c4 + e) ^ (r & 7)) * 16), k))
-                         : "memory");
-            v[u][4 * e] = __fadd_rn(v[u][4 * e], p.x);
-            v[u][4 * e + 1] = __fadd_rn(v[u][4 * e + 1], p.y);
-            v[u][4 * e + 2] = __fadd_rn(v[u][4 * e + 2], p.z);
-            v[u][4 * e + 3] = __fadd_rn(v[u][4 * e + 3], p.w);
+                         : "=f"(p[e].x), "=f"(p[e].y), "=f"(p[e].z), "=f"(p[e].w)
+                         : "r"(remote(e & 1 ? at1 : at0, k + (e >> 1))));
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            v[u][4 * (e & 1)] = __fadd_rn(v[u][4 * (e & 1)], p[e].x);
+            v[u][4 * (e & 1) + 1] = __fadd_rn(v[u][4 * (e & 1) + 1], p[e].y);
+            v[u][4 * (e & 1) + 2] = __fadd_rn(v[u][4 * (e & 1) + 2], p[e].z);
+            v[u][4 * (e & 1) + 3] = __fadd_rn(v[u][4 * (e & 1) + 3], p[e].w);
           }
         }
       }
       cluster_sync(ctas);  // everyone has read: the parts may be overwritten
 #pragma unroll
-      for (int u = 0; u < 4; u++) {
+      for (int u = 0; u < 2; u++) {
         const int i = u * kFewThreads + (int)threadIdx.x;
         if (i >= items) break;
         const int r = rank * share + i / 16, c = i % 16 * 8;
@@ -983,13 +994,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     }
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, 128, ab_k, ab_k, 128, 8);
+      one_product(tmem, 128, ab_k, ab_k, 128, 2);
       one_commit(&done);
     }
     after();
     const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
-#pragma unroll 1
-    for (int c = half * 64; c < half * 64 + 64; c += 32) {
+    {
       float x[32];
       product_of(lanes + c, 128, 2, x);
 #pragma unroll
@@ -1017,23 +1027,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     before();
     if (threadIdx.x == 0) {
       if (g.tall)
-        for (int b = 0; b < g.slice / 128; b++) {
-          const Operand p = {x_at + (uint32_t)b * 128 * 128, plane, 0, block};
-          one_product(tmem + b * 128, g.slice, p, ab_k, 128, 8);
-        }
+        for (int b = 0; b < g.slice / 128; b++)
+          one_product(tmem + b * 128, g.slice, k_major(x_at + (uint32_t)b * 128 * 128, plane, block), ab_k, 128, 2);
       else
-        one_product(tmem, g.slice, ab_k, x_mn, g.slice, 8);
+        one_product(tmem, g.slice, ab_k, x_mn, g.slice, 2);
       one_commit(&done);
     }
     after();
     // The accumulators: wide 128 rows x slice columns, tall slice / 128 blocks of
-    // 128 x 128 beside each other; half of the columns to each four warps.
+    // 128 x 128 beside each other.
     const float fx = g.fx[step];
-    const int width = g.slice / 2;  // (tall: 64 of each block's 128)
 #pragma unroll 1
-    for (int c = 0; c < width; c += 32) {
-      const int at_col = g.tall ? (c >> 6) * 128 + half * 64 + (c & 63) : half * width + c;
-      const int lr = g.tall ? (c >> 6) * 128 + row : row, lc = g.tall ? half * 64 + (c & 63) : at_col;
+    for (int at_col = quarter * 32; at_col < g.slice; at_col += 128) {
+      const int lr = g.tall ? (at_col & ~127) + row : row, lc = g.tall ? at_col & 127 : at_col;
       float x[32];
       product_of(lanes + at_col, g.slice, 2, x);
 #pragma unroll
