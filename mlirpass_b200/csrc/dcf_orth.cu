@@ -368,10 +368,11 @@ __device__ __forceinline__ float* part_block(float* part, int64_t item, int bloc
 template <Mode MODE, bool P_MN, bool Q_MN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
-                                                                    const __grid_constant__ GemmArgs g) {
+                                                                    const GemmArgs args) {
+  const GemmArgs g = args;  // a reference to the parameter itself would be read through memory
   constexpr bool symmetric = MODE == GRAM || MODE == POLY || MODE == PART;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);  // (a cast through an integer would make every access generic)
   uint8_t* buffers = base + kOrthStages * kStage;
   uint64_t* full = (uint64_t*)(buffers + kOutWarps * kBuffer);
   uint64_t* empty = full + kOrthStages;
@@ -561,9 +562,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
 
 // Joins the parts of a symmetric product, always in the same order; a warp
 // takes a block.
-constexpr int kJoinWarps = 4;
+constexpr int kJoinWarps = 1;  // (four to a block: 255 us instead of 206 at 256 x 2500, three steps)
 template <Mode MODE>
-__global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const __grid_constant__ GemmArgs g) {
+__global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const GemmArgs args) {
+  const GemmArgs g = args;
   __shared__ __align__(16) float buffers[kJoinWarps][kBlock];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -576,7 +578,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const __grid
   float v[32];
 #pragma unroll
   for (int j = 0; j < 32; j++) v[j] = 0;
-#pragma unroll 2
+#pragma unroll 4
   for (int s = 0; s < g.splits; s++) {
     const float* p = part_block(g.part, item * g.splits + s, block) + lane;
 #pragma unroll
@@ -812,7 +814,7 @@ __device__ __forceinline__ void cluster_sync(int ctas) {
 
 __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_constant__ FewArgs g) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);  // (a cast through an integer would make every access generic)
   __shared__ uint64_t done;
   __shared__ uint32_t tmem_at;
   __shared__ double sums[kFewThreads / 32], own;
@@ -1151,18 +1153,18 @@ int norm_parts(const dcf_orth_desc& d) {
 // Parts into which the k of a symmetric product is cut, `stages` stages each.
 // One part keeps a tile in registers until it is written; more keep
 // pairs of SMs busy that would have no tile.  In units of a stage (0.85 us):
-// every round of tiles costs its stages and some 4 to start and write,
-// and a join some 8.
+// every round of tiles costs its stages, a launch some 16 to start and to write
+// both triangles, or 10 to write parts and 14 to join them.
 struct Cut {
   int splits, stages;
 };
 
 Cut cut_of(int64_t tiles, int stages) {
   Cut best = {1, stages};
-  int64_t least = (tiles + kPairs - 1) / kPairs * (stages + 4);
+  int64_t least = (tiles + kPairs - 1) / kPairs * stages + 16;
   for (int s = 2; s <= stages && tiles * s <= kPairs; s++) {
     const int each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
-    const int64_t cost = each + 4 + 8;
+    const int64_t cost = each + 24;
     if (cost < least) {
       least = cost;
       best = {parts, each};
@@ -1242,15 +1244,15 @@ int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, 
 }
 
 // CTAs of a cluster that take a matrix of few rows at once, 0 where it does not
-// fit: the longer side is at most 8 x 256.  More of them than it needs, while
-// there are SMs, for slices of 128.
+// fit: the longer side is at most 8 x 256.  As few as hold it: more of them have
+// less to multiply, but joining their parts of A costs a step 7 us, and a product
+// of 256 k 2 us (128 x 256: 48 us with two, 35 us with one, 3 steps).
 int few_ctas(const dcf_orth_desc& d) {
   const uint64_t m = d.rows < d.cols ? d.rows : d.cols, n = d.rows < d.cols ? d.cols : d.rows;
   if (!d.steps || m > 128 || n > kFewSlice * kFewCluster) return 0;
-  uint64_t c = 1;
-  while (c * kFewSlice < n) c *= 2;
-  while (c < kFewCluster && c * 128 < n && 2 * c * d.batch <= 2 * kPairs) c *= 2;
-  return (int)c;
+  int c = 1;
+  while ((uint64_t)c * kFewSlice < n) c *= 2;
+  return c;
 }
 
 int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out_rs, int64_t out_bs, int vectors,
