@@ -41,9 +41,7 @@ constexpr int kOutWarps = 8;             // warps that add up and write out
 constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies, 2 and 3 lend their registers
 constexpr int kTile = 2 * kSide;         // a pair's tile: 256 x 256
 constexpr int kTmem = 2 * kTile;         // TMEM columns: two sums
-constexpr int kMine = kTile / 2;         // columns of one out warp
 constexpr int kBlock = 32 * 32;          // values an out warp writes at a time: 32 rows x 32 columns
-constexpr int kTileBlocks = kTile * kTile / kBlock;
 constexpr int kBuffer = 4096;            // bytes through which an out warp reorders 32 rows
 constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kBuffer + 256 + 1024;
 
@@ -150,7 +148,8 @@ enum Mode {
 
 struct GemmArgs {
   int m, n, k;              // rows, columns, length of the product
-  int tiles_m, tiles_n;     // tiles of 256 x 256
+  int tile_n;               // 256 or 128: columns of a tile of 256 rows
+  int tiles_m, tiles_n;
   int tiles;                // per matrix (of a symmetric product: of the upper triangle)
   int total;                // work items: tiles of the batch, times splits
   int splits, split_k;      // PART: parts of k, stages of each
@@ -187,14 +186,15 @@ struct Tile {
     z = (uint32_t)(t / g.tiles);
     int tile = t - (int)z * g.tiles, tm, tn;
     if (symmetric) {
-      for (tm = 0; tile >= g.tiles_n - tm; tm++) tile -= g.tiles_n - tm;  // row tm keeps tm .. tiles_n - 1
-      tn = tm + tile;
+      const int per = kTile / g.tile_n;  // row tm keeps the tiles that reach the diagonal or lie right of it
+      for (tm = 0; tile >= g.tiles_n - tm * per; tm++) tile -= g.tiles_n - tm * per;
+      tn = tm * per + tile;
     } else {
       tm = tile % g.tiles_m;
       tn = tile / g.tiles_m;
     }
     row0 = tm * kTile;
-    col0 = tn * kTile;
+    col0 = tn * g.tile_n;
   }
 };
 
@@ -342,11 +342,11 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
 }
 
 // Values of PART: per item and block, [column][row].
-__device__ __forceinline__ float* part_block(float* part, int64_t item, int block) {
-  return part + (item * kTileBlocks + block) * kBlock;
+__device__ __forceinline__ float* part_block(const GemmArgs& g, int64_t item, int block) {
+  return g.part + (item * (kTile / 32 * (g.tile_n / 32)) + block) * kBlock;
 }
 
-// D = P Q^T in 256 x 256 tiles, P and Q given as two fp16 planes each; P_MN,
+// D = P Q^T in tiles of 256 x 256 (256 x 128 where these are few), P and Q given as two fp16 planes each; P_MN,
 // Q_MN: its memory has rows of k and runs along the operand, so that no
 // operand is ever written transposed.
 //
@@ -365,10 +365,11 @@ __device__ __forceinline__ float* part_block(float* part, int64_t item, int bloc
 // nearest: every stage where the result is f32 (3e-6 there; two stages: 6e-6,
 // and plain fp32 products 5e-6), 16 where it is rounded to 16 bits anyway (1e-5),
 // which leaves the warps time to write a tile while the next is multiplied.
-template <Mode MODE, bool P_MN, bool Q_MN>
+template <Mode MODE, bool P_MN, bool Q_MN, int TN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
                                                                     const GemmArgs args) {
+  constexpr int kMine = TN / 2;  // columns of one out warp
   const GemmArgs g = args;  // a reference to the parameter itself would be read through memory
   constexpr bool symmetric = MODE == GRAM || MODE == POLY || MODE == PART;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -412,6 +413,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   pair_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t*)tmem_at;
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_p) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_q) : "memory");
+  }
   pdl_begin();
 
   bool fail = false;
@@ -421,7 +426,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
       int64_t i = 0;  // stages so far
       for (int t = first; t < g.total && !fail; t += step) {
         const Tile at = tile_of(t);
-        const int row = at.row0 + (int)rank * kSide, col = at.col0 + (int)rank * kSide, z = (int)(2 * at.z);
+        const int row = at.row0 + (int)rank * kSide, col = at.col0 + (int)rank * (TN / 2), z = (int)(2 * at.z);
         const int b0 = begin_of(t), blocks = count_of(t);
         for (int b = 0; b < blocks; b++, i++) {
           const int s = (int)(i % kOrthStages);
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             break;
           }
           const uint32_t to = smem_addr(base + s * kStage);
-          mbar_expect_tx(&full[s], kStage);
+          mbar_expect_tx(&full[s], 2 * (kSide + TN / 2) * kBK * 2);
 #pragma unroll
           for (int half = 0; half < 2; half++)
 #pragma unroll
@@ -438,7 +443,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
               const uint32_t at = to + p * kPlane + half * (kPlane / 2);
               const int r = row + half * 64, c = col + half * 64, k = (b0 + b) * kBK;
               tma_load_3d(at, &map_p, P_MN ? r : k, P_MN ? k : r, z + p, &full[s]);
-              tma_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, &full[s]);
+              if (half * 128 < TN) tma_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, &full[s]);
             }
         }
       }
@@ -451,8 +456,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t idesc = (1u << 4) | ((uint32_t)P_MN << 15) | ((uint32_t)Q_MN << 16) |
-                                 ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+      const uint32_t idesc = (1u << 4) | ((uint32_t)P_MN << 15) | ((uint32_t)Q_MN << 16) |
+                             ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
       int64_t i = 0, u = 0;  // stages and sums so far
       for (int t = first; t < g.total && !fail; t += step) {
         const int blocks = count_of(t);
@@ -537,7 +542,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
         // beyond the matrix, or below the diagonal: written by its mirror image
         if (r0 < g.m && c0 < g.n && !(symmetric && c0 + 31 < r0)) {
           if (MODE == PART) {
-            float* p = part_block(g.part, t, row / 32 * (kTile / 32) + (col + c) / 32) + lane;
+            float* p = part_block(g, t, row / 32 * (TN / 32) + (col + c) / 32) + lane;
 #pragma unroll
             for (int j = 0; j < 32; j++) p[j * 32] = acc[j];
           } else {
@@ -569,18 +574,19 @@ __global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const GemmAr
   __shared__ __align__(16) float buffers[kJoinWarps][kBlock];
   pdl_begin();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + warp, item = id / kTileBlocks;
-  const int block = (int)(id % kTileBlocks);
+  const int wide = g.tile_n / 32, blocks = kTile / 32 * wide;
+  const int64_t id = (int64_t)blockIdx.x * kJoinWarps + warp, item = id / blocks;
+  const int block = (int)(id % blocks);
   if (item >= g.total) return;
   const Tile at(g, (int)item, true);
-  const int r0 = at.row0 + block / (kTile / 32) * 32, c0 = at.col0 + block % (kTile / 32) * 32;
+  const int r0 = at.row0 + block / wide * 32, c0 = at.col0 + block % wide * 32;
   if (r0 >= g.m || c0 >= g.n || c0 + 31 < r0) return;
   float v[32];
 #pragma unroll
   for (int j = 0; j < 32; j++) v[j] = 0;
 #pragma unroll 4
   for (int s = 0; s < g.splits; s++) {
-    const float* p = part_block(g.part, item * g.splits + s, block) + lane;
+    const float* p = part_block(g, item * g.splits + s, block) + lane;
 #pragma unroll
     for (int j = 0; j < 32; j++) v[j] = __fadd_rn(v[j], p[j * 32]);
   }
@@ -1150,32 +1156,42 @@ int norm_parts(const dcf_orth_desc& d) {
   return (int)(p < 256 ? p : 256);
 }
 
-// Parts into which the k of a symmetric product is cut, `stages` stages each.
-// One part keeps a tile in registers until it is written; more keep
-// pairs of SMs busy that would have no tile.  In units of a stage (0.85 us):
-// every round of tiles costs its stages, a launch some 16 to start and to write
-// both triangles, or 10 to write parts and 14 to join them.
+// How a product is laid out: columns of a tile, and for a symmetric one the
+// parts into which its k is cut, `stages` stages each.
 struct Cut {
-  int splits, stages;
+  int tile_n, splits, stages;
 };
 
-Cut cut_of(int64_t tiles, int stages) {
-  Cut best = {1, stages};
-  int64_t least = (tiles + kPairs - 1) / kPairs * stages + 16;
-  for (int s = 2; s <= stages && tiles * s <= kPairs; s++) {
-    const int each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
-    const int64_t cost = each + 24;
-    if (cost < least) {
-      least = cost;
-      best = {parts, each};
+int64_t upper_tiles(int m, int tile_n) {
+  const int64_t tm = (m + kTile - 1) / kTile, tn = (m + tile_n - 1) / tile_n;
+  return tm * tn - tm * (tm - 1) / 2 * (kTile / tile_n);
+}
+
+// In units of a stage of a 256 x 256 tile (0.85 us): every round of tiles costs its
+// stages (those of a 256 x 128 tile 0.65 each: its loads bound it), a launch some 16
+// to start and to write both triangles, 11 with the smaller tile; cut along k, which keeps
+// pairs of SMs busy that would have no tile, some 10 (8) to write parts and 12 to join them.
+Cut cut_of(int m, uint64_t batch, int stages) {
+  Cut best = {256, 1, stages};
+  double least = 1e300;
+  for (int tile_n : {256, 128}) {
+    const int64_t tiles = upper_tiles(m, tile_n) * (int64_t)batch;
+    const double stage = tile_n == 256 ? 1 : 0.65;
+    const double whole = (double)((tiles + kPairs - 1) / kPairs) * stages * stage + (tile_n == 256 ? 16 : 11);
+    if (whole < least) {
+      least = whole;
+      best = {tile_n, 1, stages};
+    }
+    for (int s = 2; s <= stages && tiles * s <= kPairs; s++) {
+      const int each = (stages + s - 1) / s, parts = (stages + each - 1) / each;
+      const double cost = each * stage + (tile_n == 256 ? 22 : 20);
+      if (cost < least) {
+        least = cost;
+        best = {tile_n, parts, each};
+      }
     }
   }
   return best;
-}
-
-int64_t upper_tiles(int m) {
-  const int64_t t = (m + kTile - 1) / kTile;
-  return t * (t + 1) / 2;
 }
 
 // The workspace: X twice (a step reads one and writes the other), A, B, and
@@ -1213,11 +1229,15 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
   }
   if (d.steps > 1) l.x[1] = planes((int)d.rows, (int)d.cols);
   const int n = (int)(d.rows < d.cols ? d.cols : d.rows);
-  const int64_t tiles = upper_tiles(m) * (int64_t)d.batch;
-  l.gram = cut_of(tiles, (n + kBK - 1) / kBK);
-  l.poly = cut_of(tiles, (m + kBK - 1) / kBK);
-  const int most = l.gram.splits > l.poly.splits ? l.gram.splits : l.poly.splits;
-  l.sums = d.steps && most > 1 ? (float*)take((size_t)(tiles * most) * kTile * kTile * 4) : nullptr;
+  l.gram = cut_of(m, d.batch, (n + kBK - 1) / kBK);
+  l.poly = cut_of(m, d.batch, (m + kBK - 1) / kBK);
+  size_t sums = 0;
+  for (const Cut& c : {l.gram, l.poly})
+    if (c.splits > 1) {
+      const size_t bytes = (size_t)upper_tiles(m, c.tile_n) * d.batch * c.splits * kTile * c.tile_n * 4;
+      if (bytes > sums) sums = bytes;
+    }
+  l.sums = d.steps && sums ? (float*)take(sums) : nullptr;
   l.bytes = off;
   return l;
 }
@@ -1295,7 +1315,7 @@ int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out
 
 template <Mode MODE, bool P_MN, bool Q_MN>
 int gemm_run(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, cudaStream_t s) {
-  auto kernel = orth_gemm_kernel<MODE, P_MN, Q_MN>;
+  auto kernel = g.tile_n == 256 ? orth_gemm_kernel<MODE, P_MN, Q_MN, 256> : orth_gemm_kernel<MODE, P_MN, Q_MN, 128>;
   if (!prepare_smem((const void*)kernel, kGemmSmem)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
   return launch(kernel, dim3(2 * pairs), kGemmThreads, kGemmSmem, 2, s, p, q, g);
@@ -1304,7 +1324,9 @@ int gemm_run(const CUtensorMap& p, const CUtensorMap& q, const GemmArgs& g, cuda
 template <Mode MODE, bool P_MN, bool Q_MN>
 int gemm(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch, cudaStream_t s) {
   g.tiles_m = (g.m + kTile - 1) / kTile;
-  g.tiles_n = (g.n + kTile - 1) / kTile;
+  // Narrower tiles where they leave no pair a second one: less to write for each.
+  g.tile_n = (uint64_t)g.tiles_m * ((g.n + 127) / 128) * batch <= (uint64_t)kPairs ? 128 : 256;
+  g.tiles_n = (g.n + g.tile_n - 1) / g.tile_n;
   g.tiles = g.tiles_m * g.tiles_n;
   g.total = (int)(g.tiles * batch);
   return gemm_run<MODE, P_MN, Q_MN>(p, q, g, s);
@@ -1313,8 +1335,10 @@ int gemm(const CUtensorMap& p, const CUtensorMap& q, GemmArgs g, uint64_t batch,
 // A symmetric product, cut along k where that pays.
 template <Mode MODE, bool MN>
 int gemm_symmetric(const CUtensorMap& x, GemmArgs g, const Cut& cut, uint64_t batch, cudaStream_t s) {
-  g.tiles_m = g.tiles_n = (g.m + kTile - 1) / kTile;
-  g.tiles = (int)upper_tiles(g.m);
+  g.tile_n = cut.tile_n;
+  g.tiles_m = (g.m + kTile - 1) / kTile;
+  g.tiles_n = (g.m + g.tile_n - 1) / g.tile_n;
+  g.tiles = (int)upper_tiles(g.m, g.tile_n);
   g.total = (int)(g.tiles * batch);
   g.splits = cut.splits;
   g.split_k = cut.stages;
@@ -1322,7 +1346,7 @@ int gemm_symmetric(const CUtensorMap& x, GemmArgs g, const Cut& cut, uint64_t ba
   GemmArgs parts = g;
   parts.total *= cut.splits;
   if (int rc = gemm_run<PART, MN, MN>(x, x, parts, s)) return rc;
-  const int64_t warps = (int64_t)g.total * kTileBlocks;
+  const int64_t warps = (int64_t)g.total * (kTile / 32 * (g.tile_n / 32));
   return launch(orth_join_kernel<MODE>, dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps)), 32 * kJoinWarps, 0, 1, s, g);
 }
 
