@@ -899,6 +899,7 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       }
     }
   }
+  std::vector<std::unique_ptr<DeviceBuf>> works;  // workspaces, until the batch is done
   for (size_t i = 0; i < R; i++) {
     if (batched[i]) continue;
     FoldRequest& q = *reqs[i];
@@ -933,6 +934,28 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       case FoldRequest::SPLAT_SCAN:
         check(dcf_splat_check_async(l, q.lhs->es, q.lhs->n, st + i, s_), "splat scan");
         break;
+      case FoldRequest::BIAS:
+        check(dcf_position_bias_async(&q.bias, l, nullptr, outs[i]->ptr, s_), "position bias fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
+      case FoldRequest::BIAS_GRAD: {
+        size_t bytes = 0;
+        check(dcf_position_bias_grad_workspace(&q.bias, &bytes), "position bias gradient fold");
+        works.push_back(std::make_unique<DeviceBuf>(dev_, std::max<size_t>(bytes, 256)));
+        check(dcf_position_bias_grad_async(&q.bias, l, nullptr, outs[i]->ptr, works.back()->ptr, bytes, s_),
+              "position bias gradient fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
+      }
+      case FoldRequest::ORTH: {
+        size_t bytes = 0;
+        check(dcf_orthogonalize_workspace(&q.orth, &bytes), "orthogonalize fold");
+        works.push_back(std::make_unique<DeviceBuf>(dev_, std::max<size_t>(bytes, 256)));
+        check(dcf_orthogonalize_async(&q.orth, l, outs[i]->ptr, works.back()->ptr, bytes, st + i, s_),
+              "orthogonalize fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
+      }
       case FoldRequest::SELECT:
         check(dcf_select_async(oes, cs[i], q.cond->splat, l, q.lhs->splat, r, q.rhs->splat, q.n, outs[i]->ptr, st + i,
                                s_),

@@ -44,13 +44,15 @@ class DeviceBuf {
 // One element-level fold.  The greedy driver fills the inputs; the engine
 // fills the outcome.
 struct FoldRequest {
-  enum Kind { BINARY, CONVERT, RECIPROCAL, PERMUTE, SPLAT_SCAN, SELECT } kind = BINARY;
+  enum Kind { BINARY, CONVERT, RECIPROCAL, PERMUTE, SPLAT_SCAN, SELECT, BIAS, BIAS_GRAD, ORTH } kind = BINARY;
   int op = 0, dtype = 0, out_dtype = 0;
   uint32_t flags = 0;
   DenseP lhs, rhs;
   DenseP cond;                          // SELECT: i1 conditions; lhs / rhs are the values
   uint64_t n = 0;                       // result elements
   std::vector<int64_t> shape, perms;    // PERMUTE
+  dcf_bias_desc bias{};                 // BIAS, BIAS_GRAD: lhs is the table / the bias's gradient
+  dcf_orth_desc orth{};                 // ORTH
   TypeP out_ty;                         // attribute type of the result
   bool out_elements = true;
   // A second result over the same operands (the *_extended ops): a second

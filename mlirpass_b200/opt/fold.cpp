@@ -871,6 +871,158 @@ Plan layerwise_pattern(Module&, Op* op, Engine& eng) {
   return Plan::failed();
 }
 
+// ----------------------------------------- operators on learned tensors
+//
+// learned-constant-fold evaluates the operators of include/dcfold.h on
+// learned tensors where their operand is a constant:
+//   "dcf.position_bias"(%table)      tensor<BxHxT> -> tensor<HxQxKxT2>
+//   "dcf.position_bias_grad"(%grad)  tensor<[B x]HxQxKxT> -> tensor<BxHxf32>
+//       bidirectional, causal : bool, first_query, max_distance : i64
+//   "dcf.orthogonalize"(%w)          tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
+//       steps : i64, eps : f64, coef : array<f64: a, b, c> (or 3 per step)
+// An op whose types or properties the operator does not take stays as it is.
+
+bool bool_prop(const Op* op, const char* key, bool fallback, bool* ok) {
+  const std::string* p = op->prop(key);
+  if (!p) return fallback;
+  const std::string t = p->substr(0, p->find(' '));
+  if (t != "true" && t != "false") *ok = false;
+  return t == "true";
+}
+
+int64_t whole_prop(const Op* op, const char* key, int64_t fallback, bool* ok) {
+  const std::string* p = op->prop(key);
+  if (!p) return fallback;
+  bool read = false;
+  const int64_t v = parse_int_prop(*p, &read);
+  if (!read) *ok = false;
+  return v;
+}
+
+bool parse_number(const std::string& text, double* v) {
+  char* end = nullptr;
+  *v = strtod(text.c_str(), &end);
+  return end != text.c_str();
+}
+
+// The operand of a pattern as a constant with all of its values stored.
+DenseP whole_constant(const DenseP& k, Engine& eng) {
+  if (!k->splat) return k;
+  auto d = std::make_shared<DenseValue>();
+  d->ty = k->ty;
+  d->elements = k->elements;
+  d->dtype = k->dtype;
+  d->es = k->es;
+  d->n = (uint64_t)k->ty->count();
+  d->host.resize(d->n * d->es);
+  const uint64_t bits = eng.bits0_of(*k);
+  for (uint64_t i = 0; i < d->n; i++) memcpy(d->host.data() + i * d->es, &bits, d->es);
+  return d;
+}
+
+bool bias_properties(const Op* op, dcf_bias_desc* d) {
+  bool ok = true;
+  if (bool_prop(op, "bidirectional", true, &ok)) d->flags |= DCF_BIAS_BIDIRECTIONAL;
+  if (bool_prop(op, "causal", false, &ok)) d->flags |= DCF_BIAS_CAUSAL;
+  d->first_query = whole_prop(op, "first_query", 0, &ok);
+  const int64_t far = whole_prop(op, "max_distance", 128, &ok);
+  if (far < 0 || far > INT32_MAX) ok = false;
+  d->max_distance = (uint32_t)far;
+  size_t bytes;
+  return ok && dcf_position_bias_grad_workspace(d, &bytes) == 0;
+}
+
+bool fits32(std::initializer_list<int64_t> dims) {
+  for (int64_t d : dims)
+    if (d < 0 || d > INT32_MAX) return false;
+  return true;
+}
+
+Plan learned_pattern(Op* op, Engine& eng) {
+  if (op->dialect() != "dcf" || op->results.size() != 1 || op->operands.size() != 1) return Plan::failed();
+  const TypeP rty = op->results[0]->ty;
+  DenseP k = constant_of(op->operands[0]);
+  if (!k || k->poison || !k->elements || !k->ty->static_shape() || !rty->static_shape() || rty->kind != "tensor" ||
+      !rty->dtype || rty->count() == 0 || k->ty->count() == 0)
+    return Plan::failed();
+  const std::vector<int64_t>&in = k->ty->shape, &out = rty->shape;
+  auto q = std::make_unique<FoldRequest>();
+  if (op->name == "dcf.position_bias") {
+    if (in.size() != 2 || out.size() != 3 || in[1] != out[0] || !fits32({in[0], in[1], out[1], out[2]})) return Plan::failed();
+    dcf_bias_desc& d = q->bias;
+    d.dtype = (uint32_t)rty->dtype;
+    d.table_dtype = (uint32_t)k->dtype;
+    d.num_buckets = (uint32_t)in[0];
+    d.heads = (uint32_t)in[1];
+    d.batch = 1;
+    d.queries = (uint64_t)out[1];
+    d.keys = (uint64_t)out[2];
+    if (!bias_properties(op, &d)) return Plan::failed();
+    if (k->dtype != rty->dtype && !(k->dtype == DCF_F32 && (rty->dtype == DCF_F16 || rty->dtype == DCF_BF16)))
+      return Plan::failed();
+    q->kind = FoldRequest::BIAS;
+  } else if (op->name == "dcf.position_bias_grad") {
+    const size_t o = in.size() == 4 ? 1 : 0;
+    if (in.size() != 3 + o || out.size() != 2 || in[o] != out[1] ||
+        rty->dtype != (k->dtype == DCF_F64 ? DCF_F64 : DCF_F32) || !fits32({out[0], in[o], in[o + 1], in[o + 2], o ? in[0] : 1}))
+      return Plan::failed();
+    dcf_bias_desc& d = q->bias;
+    d.dtype = d.table_dtype = (uint32_t)k->dtype;
+    d.num_buckets = (uint32_t)out[0];
+    d.heads = (uint32_t)out[1];
+    d.batch = o ? (uint64_t)in[0] : 1;
+    d.queries = (uint64_t)in[o + 1];
+    d.keys = (uint64_t)in[o + 2];
+    if (!bias_properties(op, &d)) return Plan::failed();
+    q->kind = FoldRequest::BIAS_GRAD;
+  } else if (op->name == "dcf.orthogonalize") {
+    const size_t o = in.size() == 3 ? 1 : 0;
+    if (in.size() != 2 + o || in != out) return Plan::failed();
+    bool ok = true;
+    const int64_t steps = whole_prop(op, "steps", 5, &ok);
+    if (!ok || steps < 0 || steps > DCF_ORTH_MAX_STEPS) return Plan::failed();
+    dcf_orth_desc& d = q->orth;
+    d.dtype = (uint32_t)k->dtype;
+    d.out_dtype = (uint32_t)rty->dtype;
+    d.steps = (uint32_t)steps;
+    d.batch = o ? (uint64_t)in[0] : 1;
+    d.rows = (uint64_t)in[o];
+    d.cols = (uint64_t)in[o + 1];
+    d.eps = 1e-7;
+    if (const std::string* e = op->prop("eps"))
+      if (!parse_number(*e, &d.eps)) return Plan::failed();
+    std::vector<double> coef = {3.4445, -4.7750, 2.0315};
+    if (const std::string* c = op->prop("coef")) {
+      coef.clear();
+      const size_t from = c->find(':');
+      if (from == std::string::npos) return Plan::failed();
+      for (size_t at = from + 1; at < c->size();) {
+        double v;
+        if (!parse_number(c->substr(at), &v)) return Plan::failed();
+        coef.push_back(v);
+        at = c->find(',', at);
+        if (at == std::string::npos) break;
+        at++;
+      }
+    }
+    if (coef.size() != 3 && coef.size() != 3 * (size_t)steps) return Plan::failed();
+    for (int64_t i = 0; i < steps; i++)
+      for (int j = 0; j < 3; j++) d.coef[i][j] = coef[coef.size() == 3 ? (size_t)j : (size_t)(3 * i + j)];
+    size_t bytes;
+    if (dcf_orthogonalize_workspace(&d, &bytes) != 0) return Plan::failed();
+    q->kind = FoldRequest::ORTH;
+  } else {
+    return Plan::failed();
+  }
+  q->dtype = k->dtype;
+  q->out_dtype = rty->dtype;
+  q->lhs = whole_constant(k, eng);
+  q->n = (uint64_t)rty->count();
+  q->out_ty = rty;
+  q->out_elements = true;
+  return Plan::device(std::move(q));
+}
+
 bool commutative(const Op* op) {
   static const char* names[] = {"arith.addi", "arith.muli", "arith.andi", "arith.ori", "arith.xori",
                                 "arith.addf", "arith.mulf", "arith.maximumf", "arith.minimumf",
@@ -1191,8 +1343,8 @@ struct Greedy::Impl {
   }
 
   FoldRequest* try_patterns(Op* op) {
-    if (!cfg.layerwise || op->erased) return nullptr;
-    Plan p = layerwise_pattern(m, op, eng);
+    if ((!cfg.layerwise && !cfg.learned) || op->erased) return nullptr;
+    Plan p = cfg.learned ? learned_pattern(op, eng) : layerwise_pattern(m, op, eng);
     if (p.k == Plan::ATTR) {
       if (replace_with_attr(op, p.attr, "tosa")) changed = true;
       return nullptr;
@@ -1227,7 +1379,7 @@ struct Greedy::Impl {
         pend = nullptr;
         std::unique_ptr<FoldRequest> req = std::move(pend_req);
         if (pend_pattern) {
-          if (req->folded && replace_with_attr(op, req->out, "tosa")) changed = true;
+          if (req->folded && replace_with_attr(op, req->out, cfg.learned ? "arith" : "tosa")) changed = true;
           continue;
         }
         if (req->folded && req->op2) {
@@ -1317,6 +1469,10 @@ GreedyConfig config_for(const std::string& pass) {
   }
   if (pass == "tosa-layerwise-constant-fold") {
     c.layerwise = true;  // upstream greedy defaults: bottom-up
+    return c;
+  }
+  if (pass == "learned-constant-fold") {
+    c.learned = true;
     return c;
   }
   throw std::runtime_error("unknown pass `" + pass + "`");

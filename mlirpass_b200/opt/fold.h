@@ -12,8 +12,9 @@
 //                       and dedup, fold-then-patterns, replace_folded)
 // plus the two constant-fold patterns of the new tosa-layerwise-constant-fold
 // pass (upstream MLIR semantics: reciprocal and transpose of a constant with
-// a single use, or a splat).  The canonicalization *patterns* of the
-// reference are not restated: only folds run here.
+// a single use, or a splat), and those of learned-constant-fold (the dcf.*
+// operators on a model's learned tensors).  The canonicalization *patterns*
+// of the reference are not restated: only folds run here.
 //
 // The driver is resumable.  When a fold needs element work it hands back a
 // FoldRequest and stops; the scheduler runs the requests of many isolated
@@ -35,6 +36,7 @@ struct GreedyConfig {
   bool cse_constants = true;
   int max_iterations = 10;
   bool layerwise = false;  // add the tosa-layerwise-constant-fold patterns
+  bool learned = false;    // add the learned-constant-fold patterns
 };
 
 class Greedy {
@@ -60,7 +62,7 @@ struct PassStats {
 // Run a pass pipeline on the module.  Accepted forms:
 //   "canonicalize"                      (module-level, like --canonicalize)
 //   "builtin.module(func.func(P1,P2,...))" with P in
-//     {canonicalize, tosa-layerwise-constant-fold}
+//     {canonicalize, tosa-layerwise-constant-fold, learned-constant-fold}
 // Functions of a nested pipeline are spread over `engines` (one per GPU) and
 // their element folds are batched per round.
 void run_pipeline(Module& m, const std::string& pipeline, std::vector<Engine*>& engines, PassStats* stats);

@@ -1,0 +1,123 @@
+"""learned-constant-fold in the pass driver: the dcf.* operators on learned
+tensors fold where their operand is a constant, and stay as they are where
+their types or properties are not the operator's."""
+import numpy as np
+import pytest
+
+import learned_oracle as lo
+from mlir_text import parse_funcs
+from mlirpass_b200 import opt
+
+PIPELINE = "builtin.module(func.func(learned-constant-fold,canonicalize))"
+
+
+def hexed(a: np.ndarray) -> str:
+    return f'dense<"0x{a.tobytes().hex().upper()}">'
+
+
+def module(in_ty: str, literal: str, op: str, props: str, out_ty: str, name: str = "f") -> str:
+    return ('"builtin.module"() ({\n'
+            f'  "func.func"() <{{function_type = () -> {out_ty}, sym_name = "{name}"}}> ({{\n'
+            f'    %0 = "arith.constant"() <{{value = {literal} : {in_ty}}}> : () -> {in_ty}\n'
+            f'    %1 = "{op}"(%0){props} : ({in_ty}) -> {out_ty}\n'
+            f'    "func.return"(%1) : ({out_ty}) -> ()\n'
+            '  }) : () -> ()\n}) : () -> ()\n')
+
+
+def result(text: str, n_gpus: int = 1, name: str = "f"):
+    out, stats = opt.run(text, PIPELINE, n_gpus=n_gpus)
+    f = parse_funcs(out)[name]
+    return f.defs[f.ret.operands[0]], stats
+
+
+TABLE = np.arange(32 * 3, dtype=np.float32).reshape(32, 3) / 8
+
+
+@pytest.mark.parametrize("op,in_ty,props,out_ty", [
+    ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<4x5x6xf32>"),                       # heads differ
+    ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<3x5x6xi32>"),
+    ("dcf.position_bias", "tensor<32x3xf32>", " <{max_distance = 8 : i64}>", "tensor<3x5x6xf32>"),
+    ("dcf.position_bias", "tensor<32x3xf32>", " <{max_distance = -1 : i64}>", "tensor<3x5x6xf32>"),
+    ("dcf.position_bias", "tensor<32x3xf32>", " <{causal = 3 : i64}>", "tensor<3x5x6xf32>"),
+    ("dcf.position_bias", "tensor<96xf32>", "", "tensor<3x5x6xf32>"),
+    ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<3x5x?xf32>"),
+    ("dcf.position_bias_grad", "tensor<3x4x8xf32>", "", "tensor<32x3xbf16>"),
+    ("dcf.position_bias_grad", "tensor<32x3xf32>", "", "tensor<32x3xf32>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", "", "tensor<3x32xf32>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", "", "tensor<32x3xf64>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{steps = 17 : i64}>", "tensor<32x3xf32>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{coef = array<f64: 1.0, 2.0>}>", "tensor<32x3xf32>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{coef = array<f64: 9.0, 9.0, 9.0>}>", "tensor<32x3xf32>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{eps = -1.0 : f64}>", "tensor<32x3xf32>"),
+    ("dcf.unknown", "tensor<32x3xf32>", "", "tensor<32x3xf32>"),
+])
+def test_ops_that_stay(op, in_ty, props, out_ty):
+    d, stats = result(module(in_ty, hexed(TABLE), op, props, out_ty), n_gpus=0)
+    assert d.name == op and stats["folds"] == 0
+
+
+def test_other_passes_leave_them_alone():
+    text = module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", "", "tensor<3x5x6xf32>")
+    for pipeline in ("canonicalize", "builtin.module(func.func(tosa-layerwise-constant-fold,canonicalize))"):
+        out, stats = opt.run(text, pipeline, n_gpus=0)
+        assert '"dcf.position_bias"' in out and stats["folds"] == 0
+
+
+def test_element_work_needs_a_gpu():
+    text = module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", "", "tensor<3x5x6xf32>")
+    with pytest.raises(Exception):
+        opt.run(text, PIPELINE, n_gpus=0)
+
+
+@pytest.mark.gpu
+def test_bias_folds():
+    props = " <{bidirectional = false, causal = true, first_query = 3 : i64, max_distance = 64 : i64}>"
+    d, stats = result(module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", props, "tensor<3x9x12xf32>"))
+    q = lo.positions(9, 3)
+    want = np.where(lo.masked(q, 12), -np.inf, TABLE.T[:, lo.buckets(q, 12, 32, 64, False)]).astype(np.float32)
+    assert d.name == "arith.constant" and stats["folds"] == 1
+    assert np.array_equal(np.array(d.const.bits, np.uint32).reshape(3, 9, 12), want.view(np.uint32))
+
+
+@pytest.mark.gpu
+def test_bias_of_a_splat_table_is_a_splat_and_folds_on():
+    """The bias folds, then canonicalize folds what reads it."""
+    text = ('"builtin.module"() ({\n'
+            '  "func.func"() <{function_type = () -> tensor<3x40x50xf32>, sym_name = "f"}> ({\n'
+            '    %0 = "arith.constant"() <{value = dense<2.5> : tensor<32x3xf32>}> : () -> tensor<32x3xf32>\n'
+            '    %1 = "dcf.position_bias"(%0) : (tensor<32x3xf32>) -> tensor<3x40x50xf32>\n'
+            '    %2 = "arith.addf"(%1, %1) <{fastmath = #arith.fastmath<none>}> : (tensor<3x40x50xf32>, tensor<3x40x50xf32>) -> tensor<3x40x50xf32>\n'
+            '    "func.return"(%2) : (tensor<3x40x50xf32>) -> ()\n'
+            '  }) : () -> ()\n}) : () -> ()\n')
+    d, stats = result(text)
+    assert d.name == "arith.constant" and d.const.splat and stats["folds"] == 2
+    assert d.const.bits[0] == np.float32(5.0).view(np.uint32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [0, 2])
+def test_gradient_folds(batch):
+    rng = np.random.default_rng(1)
+    g = rng.standard_normal((max(batch, 1), 3, 20, 30)).astype(np.float32)
+    in_ty = "tensor<" + (f"{batch}x" if batch else "") + "3x20x30xf32>"
+    d, _ = result(module(in_ty, hexed(g), "dcf.position_bias_grad", "", "tensor<32x3xf32>"))
+    want, mag = lo.bias_grad(g, lo.buckets(lo.positions(20, 0), 30, 32, 128, True), 32)
+    got = np.array(d.const.bits, np.uint32).view(np.float32).reshape(32, 3)
+    assert d.name == "arith.constant"
+    assert (np.abs(got - want) <= lo.bias_grad_bound(mag, g.shape[0], 20, 30, 4, lo.U32)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,props,coef,steps", [
+    ((24, 40), "", (3.4445, -4.7750, 2.0315), 5),
+    ((2, 150, 140), " <{steps = 2 : i64, coef = array<f64: 1.5, -0.5, 0.0>, eps = 1.0e-3 : f64}>", (1.5, -0.5, 0.0), 2)])
+def test_orthogonalize_folds(shape, props, coef, steps):
+    x = np.random.default_rng(2).standard_normal(shape).astype(np.float32)
+    ty = "tensor<" + "x".join(map(str, shape)) + "xf32>"
+    d, _ = result(module(ty, hexed(x), "dcf.orthogonalize", props, ty))
+    got = np.array(d.const.bits, np.uint32).view(np.float32).reshape((-1,) + shape[-2:])
+    eps = 1e-3 if "eps" in props else 1e-7
+    for k, m in enumerate(x.reshape((-1,) + shape[-2:])):
+        want = lo.newton_schulz(m, [coef] * steps, eps)
+        tol = lo.orth_tolerance(m, [coef] * steps, eps) + lo.U32
+        assert np.linalg.norm(got[k] - want) <= tol * np.linalg.norm(want)
