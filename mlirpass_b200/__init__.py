@@ -585,7 +585,8 @@ def _own_stream(stream, t) -> int:
     """The given stream, or the current one of the tensor's device."""
     if stream is None:
         import torch
-        return torch.cuda.current_stream(t.device).cuda_stream
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object: 2 us less
+        return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 

@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
   __shared__ Near near;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int threads = p.warps * 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join waits for the whole grid
   uint16_t* offset = (uint16_t*)(acc + (size_t)p.warps * a.nb * 32);  // by distance + far: 32 x bucket
   const bool tabled = t.last <= kOffsets;
   const int far = max(t.last, 1);
@@ -459,6 +460,8 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
 template <class A>
 __global__ void __launch_bounds__(256) bias_grad_join_kernel(const A* __restrict__ part, int splits, int nb, int heads,
                                                              A* __restrict__ dtable, int add) {
+  // Launched as a programmatic dependent: its start overlaps the parts' end.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (e >= nb * heads) return;
   const int h = e / nb, v = e - h * nb;
@@ -581,9 +584,19 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
   note_launch();
   if (p.splits > 1) {
     const unsigned entries = d.num_buckets * d.heads;
-    bias_grad_join_kernel<A><<<(entries + 7) / 8, 256, 0, stream>>>((const A*)ws, p.splits, a.nb, a.heads, (A*)dtable,
-                                                                    add);
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3((entries + 7) / 8);
+    c.blockDim = dim3(256);
+    c.stream = stream;
+    cudaLaunchAttribute dependent[1];
+    dependent[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    dependent[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = dependent;
+    c.numAttrs = 1;
     note_launch();
+    if (cudaLaunchKernelEx(&c, bias_grad_join_kernel<A>, (const A*)ws, p.splits, a.nb, a.heads, (A*)dtable, add) !=
+        cudaSuccess)
+      return DCF_ECUDA;
   }
   return cudaPeekAtLastError() == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }

@@ -961,15 +961,18 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
         const uint32_t at0 = ab_at + (uint32_t)(r * 512 + (c4 ^ (r & 7)) * 16), at1 = ab_at + (uint32_t)(r * 512 + ((c4 + 1) ^ (r & 7)) * 16);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[u][j] = 0;
-        for (int k = 0; k < ctas; k += 2) {  // four loads in flight
-          float4 p[4];
+        for (int k = 0; k < ctas; k += 4) {  // eight loads in flight
+          float4 p[8];
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(p[e].x), "=f"(p[e].y), "=f"(p[e].z), "=f"(p[e].w)
-                         : "r"(remote(e & 1 ? at1 : at0, k + (e >> 1))));
+          for (int e = 0; e < 8; e++) {
+            p[e] = make_float4(0, 0, 0, 0);
+            if (k + (e >> 1) < ctas)
+              asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(p[e].x), "=f"(p[e].y), "=f"(p[e].z), "=f"(p[e].w)
+                           : "r"(remote(e & 1 ? at1 : at0, k + (e >> 1))));
+          }
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
+          for (int e = 0; e < 8; e++) {
             v[u][4 * (e & 1)] = __fadd_rn(v[u][4 * (e & 1)], p[e].x);
             v[u][4 * (e & 1) + 1] = __fadd_rn(v[u][4 * (e & 1) + 1], p[e].y);
             v[u][4 * (e & 1) + 2] = __fadd_rn(v[u][4 * (e & 1) + 2], p[e].z);
