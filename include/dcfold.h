@@ -484,7 +484,7 @@ typedef struct dcf_bias_desc {
   uint32_t flags;       /* DCF_BIAS_* */
   uint32_t heads;
   uint64_t batch;       /* gradient only: the bias is shared by the batch */
-  uint64_t queries, keys; /* < 2^31 each */
+  uint64_t queries, keys; /* < 2^31; keys <= 2^31 - 65536 */
   int64_t first_query;  /* position of query 0 where key 0 has position 0; |.| <= 2^40 */
   int64_t row_stride, head_stride, batch_stride;
 } dcf_bias_desc;
@@ -496,11 +496,13 @@ typedef struct dcf_bias_desc {
  * transposed): X = G / (||G||_F + eps), then per step, with the step's
  * coefficients (a, b, c),
  *     A = X X^T,  X <- a X + (b A + c A A) X,
- * which maps every singular value s of X to a s + b s^3 + c s^5.  The
- * iterate is kept in two fp16 halves of a scaled value (22 bits or more)
- * and products are accumulated in 32 bits; the norm is summed in 64.
- * The coefficients must keep every singular value from [0, 1] within
- * [-64, 64] (checked). */
+ * which maps every singular value s of X to a s + b s^3 + c s^5.  Every
+ * operand of a product is kept as two fp16 halves of a scaled value (22 bits
+ * or more), products are summed in 32 bits, the norm in 64; the result is
+ * rounded once.  The coefficients must keep every singular value from [0, 1]
+ * within [-64, 64] (checked).  A matrix with min(rows, cols) <= 128 and
+ * max(rows, cols) <= 2048 stays on the chip and needs no workspace.  No
+ * steps (steps = 0) give G / (||G||_F + eps). */
 typedef struct dcf_orth_desc {
   uint32_t dtype, out_dtype; /* DCF_F16, DCF_BF16 or DCF_F32 */
   uint32_t steps;            /* 0 .. DCF_ORTH_MAX_STEPS */

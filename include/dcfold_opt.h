@@ -7,9 +7,21 @@
  * rewrite driver (src/rewrite.rs:785-906), `canonicalize` as a bare flag
  * (src/pass.rs:693-695) and nested `func.func(...)` pipelines whose
  * functions the reference runs as parallel tasks (src/pass.rs:280-341), plus
- * the `tosa-layerwise-constant-fold` pass that the reference lacks.  Only
- * folds run: the reference's canonicalization rewrite patterns are not
- * restated.
+ * the `tosa-layerwise-constant-fold` pass that the reference lacks, and the
+ * `learned-constant-fold` pass, which evaluates operators on a model's
+ * learned tensors (dcf_position_bias, dcf_position_bias_grad and
+ * dcf_orthogonalize of dcfold.h) where their operand is a constant:
+ *   "dcf.position_bias"(%table)     tensor<BxHxT> -> tensor<HxQxKxT2>
+ *   "dcf.position_bias_grad"(%grad) tensor<[B x]HxQxKxT> -> tensor<BxHxf32>
+ *       (f64 from f64)
+ *     properties bidirectional (true), causal (false), first_query (0),
+ *     max_distance (128); buckets, heads, queries and keys are the types'
+ *   "dcf.orthogonalize"(%w)         tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
+ *     properties steps (5), eps (1e-7), coef (array<f64: a, b, c>, or three
+ *     for each step)
+ * An op whose types or properties its operator does not take is left as it
+ * is.  Only folds run: the reference's canonicalization rewrite patterns
+ * are not restated.
  */
 #ifndef DCFOLD_OPT_H
 #define DCFOLD_OPT_H
@@ -34,7 +46,8 @@ typedef struct dcf_opt_stats {
 } dcf_opt_stats;
 
 /* Run `pipeline` ("canonicalize", or "builtin.module(func.func(P,...))" with
- * P in canonicalize, tosa-layerwise-constant-fold) over the module `text`
+ * P in canonicalize, tosa-layerwise-constant-fold, learned-constant-fold)
+ * over the module `text`
  * on GPUs 0..n_gpus-1 (n_gpus < 0: every GPU).  n_gpus == 0 runs host-only:
  * parsing, printing and the folds decided without element work (shortcuts)
  * succeed, and any fold that needs element work fails with an error; there
