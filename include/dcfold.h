@@ -500,7 +500,7 @@ typedef struct dcf_bias_desc {
  * operand of a product is kept as two fp16 halves of a scaled value (22 bits
  * or more), products are summed in 32 bits, the norm in 64; the result is
  * rounded once.  The coefficients must keep every singular value from [0, 1]
- * within [-64, 64] (checked).  A matrix with min(rows, cols) <= 128 and
+ * within [-64, 64], and leave some of it (checked).  A matrix with min(rows, cols) <= 128 and
  * max(rows, cols) <= 2048 stays on the chip and needs no workspace.  No
  * steps (steps = 0) give G / (||G||_F + eps). */
 typedef struct dcf_orth_desc {
@@ -537,8 +537,9 @@ int dcf_position_bias_grad_async(const dcf_bias_desc* desc, const void* grad,
                                  const int32_t* positions, void* table_grad,
                                  void* workspace, size_t workspace_bytes,
                                  void* stream);
-/* `out` may be `in` (same strides and element type).  Kernels that give up a
- * bounded wait set status->error (reset it first; dcf_status_read). */
+/* `out` may be `in` (same strides and element type; anything else in place is
+ * refused) and must not overlap it otherwise.  Kernels that give up a bounded
+ * wait set status->error (reset it first; dcf_status_read). */
 int dcf_orthogonalize_workspace(const dcf_orth_desc* desc, size_t* bytes);
 int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in,
                             void* out, void* workspace,

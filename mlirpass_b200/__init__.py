@@ -604,6 +604,14 @@ def _need(t, what: str, elements: int, size: int) -> int:
     return t.data_ptr()
 
 
+def _positions(positions, queries: int):
+    if positions is None:
+        return None
+    if "int32" not in str(positions.dtype):
+        raise ValueError(f"positions: {positions.dtype}, int32 expected")
+    return _need(positions, "positions", queries, 4)
+
+
 def _bytes(workspace) -> int:
     if not workspace.is_contiguous():
         raise ValueError("workspace: not contiguous")
@@ -615,7 +623,7 @@ def position_bias_async(plan: BiasPlan, table, out, *, positions=None, stream=No
     first element; the plan's strides say where the rest lies."""
     _check(lib().dcf_position_bias_async(
         plan.ref, _need(table, "table", plan.entries, DTYPE_SIZE[plan.table_dtype]),
-        None if positions is None else _need(positions, "positions", plan.desc.queries, 4),
+        _positions(positions, plan.desc.queries),
         _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.dtype]), _own_stream(stream, out)))
 
 
@@ -630,7 +638,7 @@ def position_bias_grad_async(plan: BiasPlan, grad, out, workspace, *, positions=
     position_bias_grad_workspace says 0)."""
     _check(lib().dcf_position_bias_grad_async(
         plan.ref, _need(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype]),
-        None if positions is None else _need(positions, "positions", plan.desc.queries, 4),
+        _positions(positions, plan.desc.queries),
         _need(out, "out", plan.entries, 8 if plan.dtype == "f64" else 4), workspace.data_ptr(),
         _bytes(workspace), _own_stream(stream, out)))
 

@@ -1374,6 +1374,8 @@ int orth_desc_check(const dcf_orth_desc* d) {
     double q;
     step_bounds(d->coef[i], s, &s, &q);
     if (!(s <= kMostSingular)) return bad("orthogonalize: the coefficients let singular values grow past 64");
+    // below, powers of two that scale what is kept leave the range of fp32
+    if (!(q >= 1e-30) || !(s >= 1e-30)) return bad("orthogonalize: the coefficients leave nothing");
   }
   if (!d->batch || !d->rows || !d->cols) return DCF_OK;
   const uint64_t m = d->rows < d->cols ? d->rows : d->cols, n = d->rows < d->cols ? d->cols : d->rows;

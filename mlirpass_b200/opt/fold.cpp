@@ -880,7 +880,9 @@ Plan layerwise_pattern(Module&, Op* op, Engine& eng) {
 //       bidirectional, causal : bool, first_query, max_distance : i64
 //   "dcf.orthogonalize"(%w)          tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
 //       steps : i64, eps : f64, coef : array<f64: a, b, c> (or 3 per step)
-// An op whose types or properties the operator does not take stays as it is.
+// An op whose types or properties the operator does not take stays as it is,
+// and so does one whose operand or result is over 16 GiB: a module could not
+// hold it as a constant.
 
 bool bool_prop(const Op* op, const char* key, bool fallback, bool* ok) {
   const std::string* p = op->prop(key);
@@ -932,6 +934,16 @@ bool bias_properties(const Op* op, dcf_bias_desc* d) {
   return ok && dcf_position_bias_grad_workspace(d, &bytes) == 0;
 }
 
+bool fits_module(const TypeP& t) {
+  __int128 n = (__int128)dcf_dtype_size((dcf_dtype)t->dtype);
+  for (int64_t d : t->shape) {
+    if (d <= 0) return false;
+    n *= d;
+    if (n > ((__int128)1 << 34)) return false;
+  }
+  return true;
+}
+
 bool fits32(std::initializer_list<int64_t> dims) {
   for (int64_t d : dims)
     if (d < 0 || d > INT32_MAX) return false;
@@ -943,7 +955,7 @@ Plan learned_pattern(Op* op, Engine& eng) {
   const TypeP rty = op->results[0]->ty;
   DenseP k = constant_of(op->operands[0]);
   if (!k || k->poison || !k->elements || !k->ty->static_shape() || !rty->static_shape() || rty->kind != "tensor" ||
-      !rty->dtype || rty->count() == 0 || k->ty->count() == 0)
+      !rty->dtype || !fits_module(rty) || !fits_module(k->ty))
     return Plan::failed();
   const std::vector<int64_t>&in = k->ty->shape, &out = rty->shape;
   auto q = std::make_unique<FoldRequest>();

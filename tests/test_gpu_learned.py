@@ -369,6 +369,14 @@ def test_orth_scales(dcf, scale):
     check_orth(run_orth(dcf, x, "f32", eps=0.0), x, "f32", [COEF] * 5, eps=0.0)
 
 
+def test_orth_small_coefficients(dcf):
+    """Results far below the input's scale keep their precision."""
+    for shape in ((1, 40, 60), (1, 150, 170)):
+        x = randn(shape, "f32", 34)
+        coef = [(1e-12, 1e-13, -2e-13)] * 2
+        check_orth(run_orth(dcf, x, "f32", steps=2, coef=coef), x, "f32", coef)
+
+
 def test_orth_zero_and_not_finite(dcf):
     import torch
     x = randn((4, 33, 40), "f32", 28)
@@ -438,6 +446,10 @@ def test_device_pointer_checks(dcf):
         dcf.position_bias_async(plan, table.cuda(), out[1:])
     with pytest.raises(ValueError):
         dcf.position_bias_async(plan, table.cuda().double(), out)
+    with pytest.raises(ValueError):
+        dcf.position_bias_async(plan, table.cuda(), out, positions=torch.zeros(4, device="cuda"))
+    with pytest.raises(ValueError):          # one element shown many times is not room for many
+        dcf.position_bias_async(plan, table.cuda(), torch.zeros(1, device="cuda").expand(64))
     odd = torch.zeros(300, dtype=torch.uint8, device="cuda")[1:257].view(torch.uint8)
     with pytest.raises(dcf.DcfError):
         dcf._check(dcf.lib().dcf_position_bias_async(plan.ref, table.cuda().data_ptr(), None, odd.data_ptr(), None))

@@ -83,6 +83,7 @@ def test_bias_grad_workspace_and_its_checks():
     (dict(coef=(math.nan, 0, 0)), "coefficient"), (dict(coef=(1e5, 0, 0)), "coefficient"),
     (dict(coef=(3.0, 0, 0)), "past 64"),                    # 3^5 = 243
     (dict(coef=(3.4445, 4.7750, 2.0315)), "past 64"),
+    (dict(coef=(0, 0, 0)), "nothing"), (dict(coef=(1e-31, 0, 0)), "nothing"), (dict(coef=(1e-8, 0, 0), steps=5), "nothing"),
     (dict(rows=65536, cols=65536, batch=65535), "tiles"),
 ])
 def test_orth_plans_that_are_refused(kw, word):
@@ -115,6 +116,11 @@ def test_orth_calls_that_are_refused():
     bad = m.OrthDesc.from_buffer_copy(plan.desc)
     bad.reserved = 1
     assert call(ctypes.byref(bad), 256, 256, 256, plan.workspace, 256, None) == -1
+    # in place only where a matrix is written where it was read
+    for kw in (dict(out_dtype="bf16"), dict(out_row_stride=501), dict(batch=2, out_batch_stride=400 * 500 + 1)):
+        other = m.orthogonalize_plan("f32", 400, 500, **kw)
+        assert call(other.ref, 256, 256, 512, other.workspace, 1024, None) == -1
+        assert b"in place" in m.lib().dcf_last_error()
     bad = m.OrthDesc.from_buffer_copy(plan.desc)
     bad.steps = 17
     assert call(ctypes.byref(bad), 256, 256, 256, plan.workspace, 256, None) == -1

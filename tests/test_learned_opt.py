@@ -40,6 +40,8 @@ TABLE = np.arange(32 * 3, dtype=np.float32).reshape(32, 3) / 8
     ("dcf.position_bias", "tensor<32x3xf32>", " <{max_distance = -1 : i64}>", "tensor<3x5x6xf32>"),
     ("dcf.position_bias", "tensor<32x3xf32>", " <{causal = 3 : i64}>", "tensor<3x5x6xf32>"),
     ("dcf.position_bias", "tensor<96xf32>", "", "tensor<3x5x6xf32>"),
+    ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<3x200000x200000xf32>"),             # 480 GB
+    ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<3x0x6xf32>"),
     ("dcf.position_bias", "tensor<32x3xf32>", "", "tensor<3x5x?xf32>"),
     ("dcf.position_bias_grad", "tensor<3x4x8xf32>", "", "tensor<32x3xbf16>"),
     ("dcf.position_bias_grad", "tensor<32x3xf32>", "", "tensor<32x3xf32>"),
