@@ -265,6 +265,13 @@ __device__ __forceinline__ void put_row8(void* out, int dtype, int vectors, int6
 
 // Writes the block at row r0, column c0 of the result in the caller's type.
 __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* buf, int lane) {
+  if (!g.vectors) {  // element by element, a row at a time
+    int64_t at = (int64_t)z * g.out_bs + (int64_t)r0 * g.out_rs + c0 + lane;
+#pragma unroll 4
+    for (int row = 0; row < 32; row++, at += g.out_rs)
+      if (r0 + row < g.m && c0 + lane < g.n) store_typed(g.out, at, g.out_dtype, __fmul_rn(g.alpha, buf[place(lane, row)]));
+    return;
+  }
   const int o = (lane & 3) * 8, c = c0 + o;
 #pragma unroll 1
   for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
@@ -275,11 +282,13 @@ __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r
   }
 }
 
-// The same as planes; for GRAM and POLY on and above the diagonal, with
-// the mirror image strictly below it.
+// The same as planes.  Of a symmetric matrix, blocks right of the diagonal are
+// written with their mirror image, and one on it (blocks lie on multiples of
+// 32) takes its lower half from its upper.
 template <Mode MODE>
 __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int r0, int c0, float* buf, int lane) {
   constexpr bool sym = MODE == GRAM || MODE == POLY;
+  const bool on = sym && c0 == r0;
   const int o = (lane & 3) * 8, c = c0 + o;
   const size_t plane = (size_t)g.to.rows * g.to.ld;
 #pragma unroll 1
@@ -287,7 +296,7 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
     const int r = r0 + row;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[place(o + e, row)]);
+    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[on && o + e < row ? place(row, o + e) : place(o + e, row)]);
     if (MODE == POLY) {
       const __half* from = g.from.row(z, 0, r) + c;
       const uint4 x = *(const uint4*)from, y = *(const uint4*)(from + plane);
@@ -299,27 +308,23 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
         v[2 * e] = __fmaf_rn(g.beta, __fadd_rn(p.x, q.x), v[2 * e]);
         v[2 * e + 1] = __fmaf_rn(g.beta, __fadd_rn(p.y, q.y), v[2 * e + 1]);
       }
+      if (on) {
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (c + e == r) v[e] = __fadd_rn(v[e], g.diag);
+        for (int e = 0; e < 8; e++)
+          if (o + e == row) v[e] = __fadd_rn(v[e], g.diag);
+      }
     }
-    if (sym) {  // as the mirror image has them
+    if (sym && !on) {  // for the mirror image
 #pragma unroll
       for (int e = 0; e < 8; e++) buf[place(o + e, row)] = v[e];
     }
     uint4 hi, lo;
     split8(v, hi, lo);
     __half* to = g.to.row(z, 0, r) + c;  // rows are padded to 64 columns: whole vectors fit
-    const int left = sym ? r - c : 0;    // of the diagonal
-    if (left <= 0) {
-      *(uint4*)to = hi;
-      *(uint4*)(to + plane) = lo;
-    } else if (left < 8) {
-      put_some((uint16_t*)to, hi, left, 8);
-      put_some((uint16_t*)(to + plane), lo, left, 8);
-    }
+    *(uint4*)to = hi;
+    *(uint4*)(to + plane) = lo;
   }
-  if (!sym || c0 + 31 <= r0) return;
+  if (!sym || on) return;
   __syncwarp();
   const int r = r0 + o;  // eight rows of one column
   if (r >= g.m) return;
@@ -330,14 +335,8 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
     uint4 hi, lo;
     split8(v, hi, lo);
     __half* to = g.to.row(z, 0, c0 + col) + r;
-    const int above = c0 + col - r;
-    if (above >= 8) {
-      *(uint4*)to = hi;
-      *(uint4*)(to + plane) = lo;
-    } else if (above > 0) {
-      put_some((uint16_t*)to, hi, 0, above);
-      put_some((uint16_t*)(to + plane), lo, 0, above);
-    }
+    *(uint4*)to = hi;
+    *(uint4*)(to + plane) = lo;
   }
 }
 
