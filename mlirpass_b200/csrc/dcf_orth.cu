@@ -201,8 +201,8 @@ struct Tile {
 // A block of 32 rows x 32 columns on its way out: from rows in lanes, through
 // 4 KB of shared memory, to eight columns of a row, or eight rows of a column,
 // in each lane.  Groups of four rows are exchanged so that none of the three
-// has bank conflicts.  (The code is short on purpose: unrolled over a
-// warp's 128 columns it ran once per tile, and fetching it took 15 us.)
+// has bank conflicts.  (One block at a time on purpose: unrolled over a
+// warp's 128 columns the code ran once per tile, and fetching it took 15 us.)
 __device__ __forceinline__ uint32_t place(int col, int row) {
   return (uint32_t)(col * 32 + ((((row >> 2) ^ (col & 7) ^ ((col >> 2) & 6)) << 2) | (row & 3)));
 }
@@ -266,10 +266,17 @@ __device__ __forceinline__ void put_row8(void* out, int dtype, int vectors, int6
 // Writes the block at row r0, column c0 of the result in the caller's type.
 __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* buf, int lane) {
   if (!g.vectors) {  // element by element, a row at a time
-    int64_t at = (int64_t)z * g.out_bs + (int64_t)r0 * g.out_rs + c0 + lane;
-#pragma unroll 4
-    for (int row = 0; row < 32; row++, at += g.out_rs)
-      if (r0 + row < g.m && c0 + lane < g.n) store_typed(g.out, at, g.out_dtype, __fmul_rn(g.alpha, buf[place(lane, row)]));
+    const int64_t at = (int64_t)z * g.out_bs + (int64_t)r0 * g.out_rs + c0 + lane;
+    const int rows = c0 + lane < g.n ? min(32, g.m - r0) : 0;
+    auto each = [&](auto* out, auto cast) {
+      out += at;
+#pragma unroll 8
+      for (int row = 0; row < 32; row++, out += g.out_rs)
+        if (row < rows) *out = cast(__fmul_rn(g.alpha, buf[place(lane, row)]));
+    };
+    if (g.out_dtype == DCF_F32) each((float*)g.out, [](float v) { return v; });
+    else if (g.out_dtype == DCF_F16) each((__half*)g.out, [](float v) { return __float2half_rn(v); });
+    else each((__nv_bfloat16*)g.out, [](float v) { return __float2bfloat16_rn(v); });
     return;
   }
   const int o = (lane & 3) * 8, c = c0 + o;
@@ -291,7 +298,7 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
   const bool on = sym && c0 == r0;
   const int o = (lane & 3) * 8, c = c0 + o;
   const size_t plane = (size_t)g.to.rows * g.to.ld;
-#pragma unroll 1
+#pragma unroll 4
   for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
     const int r = r0 + row;
     float v[8];
@@ -328,7 +335,7 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
   __syncwarp();
   const int r = r0 + o;  // eight rows of one column
   if (r >= g.m) return;
-#pragma unroll 1
+#pragma unroll 4
   for (int col = lane >> 2; col < 32 && c0 + col < g.n; col += 8) {
     const float4 x = *(const float4*)&buf[place(col, o)], y = *(const float4*)&buf[place(col, o + 4)];
     const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
