@@ -153,7 +153,7 @@ struct GemmArgs {
   int tiles;                // per matrix (of a symmetric product: of the upper triangle)
   int total;                // work items: tiles of the batch, times splits
   int splits, split_k;      // PART: parts of k, stages of each
-  int sum;                  // stages that TMEM sums before registers do
+  int sum;                  // stages that TMEM sums before registers do; 0: half a stage
   float alpha, beta, diag;  // v = alpha acc [+ beta A + diag I]
   Planes to, from;          // result; POLY: A
   float* part;              // PART
@@ -369,7 +369,7 @@ __device__ __forceinline__ float* part_block(const GemmArgs& g, int64_t item, in
 // only (the two small products of a stage first, then the large one), in two
 // buffers in turn, and the eight warps add the sums in registers, rounding to
 // nearest: every stage where the result is f32 (3e-6 there; two stages: 6e-6,
-// and plain fp32 products 5e-6), 16 where it is rounded to 16 bits anyway (1e-5),
+// and plain fp32 products 5e-6; every half stage in A A of few rows), 16 where it is rounded to 16 bits anyway (1e-5),
 // which leaves the warps time to write a tile while the next is multiplied.
 template <Mode MODE, bool P_MN, bool Q_MN, int TN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
@@ -489,16 +489,33 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
           const uint64_t ph = smem_desc<P_MN>(at), pl = smem_desc<P_MN>(at + kPlane);
           const uint64_t qh = smem_desc<Q_MN>(at + 2 * kPlane), ql = smem_desc<Q_MN>(at + 3 * kPlane);
           constexpr uint32_t ps = kSlice<P_MN>, qs = kSlice<Q_MN>;
+          auto products = [&](uint32_t to, uint32_t from, uint32_t end, int in_sum) {
 #pragma unroll
-          for (uint32_t j = 0; j < kBK / 16; j++) {
-            pair_mma(to, ph + ps * j, ql + qs * j, idesc, in_sum | (int)j);
-            pair_mma(to, pl + ps * j, qh + qs * j, idesc, 1);
-          }
+            for (uint32_t j = 0; j < kBK / 16; j++)
+              if (j >= from && j < end) {
+                pair_mma(to, ph + ps * j, ql + qs * j, idesc, in_sum | (int)(j - from));
+                pair_mma(to, pl + ps * j, qh + qs * j, idesc, 1);
+              }
 #pragma unroll
-          for (uint32_t j = 0; j < kBK / 16; j++) pair_mma(to, ph + ps * j, qh + qs * j, idesc, 1);
-          pair_commit(&empty[s]);
-          if (++in_sum == g.sum || b == blocks - 1) {
+            for (uint32_t j = 0; j < kBK / 16; j++)
+              if (j >= from && j < end) pair_mma(to, ph + ps * j, qh + qs * j, idesc, 1);
+          };
+          if (g.sum == 0) {  // two sums of half a stage: one here, one below
+            products(to, 0, kBK / 32, 0);
             pair_commit(&sum_full[d]);
+            u++;
+            if (u >= 2 && !mbar_wait_bounded(&sum_empty[u & 1], (unsigned)((u / 2 - 1) & 1))) {
+              fail = true;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            products(tmem + (uint32_t)(u & 1) * kTile, kBK / 32, kBK / 16, 0);
+          } else {
+            products(to, 0, kBK / 16, in_sum);
+          }
+          pair_commit(&empty[s]);
+          if (++in_sum >= g.sum || b == blocks - 1) {
+            pair_commit(&sum_full[u & 1]);
             u++;
             in_sum = 0;
           }
@@ -514,7 +531,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     int64_t u = 0;  // sums so far
     for (int t = first; t < g.total && !fail; t += step) {
       const Tile at = tile_of(t);
-      const int sums = (count_of(t) + g.sum - 1) / g.sum;
+      const int sums = g.sum ? (count_of(t) + g.sum - 1) / g.sum : 2 * count_of(t);
       float acc[kMine];
 #pragma unroll
       for (int j = 0; j < kMine; j++) acc[j] = 0;
@@ -770,24 +787,27 @@ __device__ __forceinline__ Operand mn_major(uint32_t at, uint32_t plane, uint32_
   return {smem_desc<false>(at) + far, smem_desc<false>(at + plane) + far, 2048 >> 4, 4 * (2048 >> 4), 1};
 }
 
-// Each 64 k have an accumulator of their own, `pitch` columns after the last, and
-// the small products come first, while its sum is small: the tensor core truncates.
-__device__ __forceinline__ void one_product(uint32_t d, int pitch, Operand p, Operand q, int n, int chunks) {
+// Every PER slices of 16 k have an accumulator of their own, `pitch` columns after
+// the last, and the small products come first, while its sum is small: the tensor
+// core truncates.  Four slices, and two in A A where the result is f32 (from 64 bits, at
+// 79 x 249: 1.4e-6; with four 1.9e-6, with two in all products 1.3e-6 but 14 us of 38
+// more at 96 x 96; plain fp32 products 1.1e-6).
+template <int PER>
+__device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int from, int to) {
   const uint32_t idesc =
       (1u << 4) | (p.mn << 15) | (q.mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 #pragma unroll 1
-  for (int c = 0; c < chunks; c++, d += pitch) {
+  for (int s = from; s < to; s += PER, d += pitch) {  // a run of slices lies in one chunk of 64 k
+    const uint32_t po = (uint32_t)(s >> 2) * p.chunk + (uint32_t)(s & 3) * p.step;
+    const uint32_t qo = (uint32_t)(s >> 2) * q.chunk + (uint32_t)(s & 3) * q.step;
+    const uint64_t ph = p.hi + po, pl = p.lo + po, qh = q.hi + qo, ql = q.lo + qo;
 #pragma unroll
-    for (uint32_t s = 0; s < 4; s++) {
-      one_mma(d, p.hi + s * p.step, q.lo + s * q.step, idesc, s);
-      one_mma(d, p.lo + s * p.step, q.hi + s * q.step, idesc, 1);
+    for (uint32_t k = 0; k < PER; k++) {
+      one_mma(d, ph + k * p.step, ql + k * q.step, idesc, k);
+      one_mma(d, pl + k * p.step, qh + k * q.step, idesc, 1);
     }
 #pragma unroll
-    for (uint32_t s = 0; s < 4; s++) one_mma(d, p.hi + s * p.step, q.hi + s * q.step, idesc, 1);
-    p.hi += p.chunk;
-    p.lo += p.chunk;
-    q.hi += q.chunk;
-    q.lo += q.chunk;
+    for (uint32_t k = 0; k < PER; k++) one_mma(d, ph + k * p.step, qh + k * q.step, idesc, 1);
   }
 }
 
@@ -824,6 +844,7 @@ __device__ __forceinline__ void cluster_sync(int ctas) {
   else __syncthreads();
 }
 
+template <int PER>
 __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_constant__ FewArgs g) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);  // (a cast through an integer would make every access generic)
@@ -922,38 +943,32 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   for (int step = 0; step < g.steps; step++) {
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, 128, x_gram, x_gram, 128, g.slice / 64);
+      one_product<4>(tmem, 128, x_gram, x_gram, 128, 0, g.slice / 16);
       one_commit(&done);
     }
     after();
-    const float fa = g.fa[step];
     const int c = quarter * 32;
+    float sum[32];  // this thread's row, 32 columns
+    product_of(lanes + c, 128, g.slice / 64, sum);
+    const float fa = g.fa[step];
     if (ctas == 1) {
-      {
-        float x[32];
-        product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float v[8];
+      for (int k = 0; k < 4; k++) {
+        float v[8];
 #pragma unroll
-          for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fa, x[8 * k + j]);
-          uint4 hi, lo;
-          split8(v, hi, lo);
-          uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
-          *(uint4*)at = hi;
-          *(uint4*)(at + kFewPlane) = lo;
-        }
+        for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fa, sum[8 * k + j]);
+        uint4 hi, lo;
+        split8(v, hi, lo);
+        uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
+        *(uint4*)at = hi;
+        *(uint4*)(at + kFewPlane) = lo;
       }
     } else {
       // Parts as rows of 512 bytes, their 16-byte chunks exchanged by row.
-      {
-        float x[32];
-        product_of(lanes + c, 128, g.slice / 64, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-          *(float4*)(ab + row * 512 + (((c >> 2) + k) ^ (row & 7)) * 16) =
-              make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
-      }
+      for (int k = 0; k < 8; k++)
+        *(float4*)(ab + row * 512 + (((c >> 2) + k) ^ (row & 7)) * 16) =
+            make_float4(sum[4 * k], sum[4 * k + 1], sum[4 * k + 2], sum[4 * k + 3]);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       cluster_sync(ctas);
       // Rows rank * 128 / ctas on, eight columns at a time: 16 values a thread at most.
@@ -1011,14 +1026,14 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     }
     before();
     if (threadIdx.x == 0) {
-      one_product(tmem, 128, ab_k, ab_k, 128, 2);
+      one_product<PER>(tmem, 128, ab_k, ab_k, 128, 0, 8);
       one_commit(&done);
     }
     after();
     const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
     {
       float x[32];
-      product_of(lanes + c, 128, 2, x);
+      product_of(lanes + c, 128, 8 / PER, x);
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
@@ -1045,9 +1060,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     if (threadIdx.x == 0) {
       if (g.tall)
         for (int b = 0; b < g.slice / 128; b++)
-          one_product(tmem + b * 128, g.slice, k_major(x_at + (uint32_t)b * 128 * 128, plane, block), ab_k, 128, 2);
+          one_product<4>(tmem + b * 128, g.slice, k_major(x_at + (uint32_t)b * 128 * 128, plane, block), ab_k, 128, 0, 8);
       else
-        one_product(tmem, g.slice, ab_k, x_mn, g.slice, 2);
+        one_product<4>(tmem, g.slice, ab_k, x_mn, g.slice, 0, 8);
       one_commit(&done);
     }
     after();
@@ -1157,6 +1172,10 @@ int scale_of(double bound) {
 }
 
 constexpr double kMostSingular = 64;
+// Up to so many rows A A of a f32 result is summed every 32 k: there plain fp32 products
+// are as near to 64 bits as every 64 k leave it (258 x 131, six steps: 3.6e-6 and
+// 2.1e-6); at 2048 rows those are at 5.4e-6 and it is at 2.8e-6.
+constexpr int kFineRows = 1024;
 constexpr int kPairs = 74;  // pairs of SMs
 
 // Blocks of the norm's sum: 32 KB of a f32 matrix each, 256 at most.
@@ -1318,8 +1337,9 @@ int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out
   }
   int smem = 2 * (128 * g.slice * 2) + 2 * kFewPlane + 1024;
   if (smem < kFewLeast) smem = kFewLeast;
-  if (!prepare_smem((const void*)orth_few_kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
-  return launch(orth_few_kernel, dim3((unsigned)(d.batch * ctas)), kFewThreads, smem, ctas, s, g);
+  auto kernel = d.out_dtype == DCF_F32 ? orth_few_kernel<2> : orth_few_kernel<4>;
+  if (!prepare_smem((const void*)kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
+  return launch(kernel, dim3((unsigned)(d.batch * ctas)), kFewThreads, smem, ctas, s, g);
 }
 
 template <Mode MODE, bool P_MN, bool Q_MN>
@@ -1460,7 +1480,9 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
     g.to = l.b;
+    if (d.out_dtype == DCF_F32 && m <= kFineRows) g.sum = 0;
     if ((rc = gemm_symmetric<POLY, false>(ma, g, l.poly, d.batch, s))) return rc;
+    g.sum = d.out_dtype == DCF_F32 ? 1 : 16;
     g.m = rows;
     g.n = cols;
     if (i + 1 < d.steps) {
