@@ -15,8 +15,8 @@
 // against one table value or one addition.  What has to be kept small is the
 // work per element around that, above all finding its bucket: a row is
 // cut once into the two far ranges, which have one bucket each, and the near
-// columns between, whose buckets come from a table of distances in shared memory;
-// a thread owns one 16-byte vector, and in the bias its lookup serves all heads.
+// columns between, whose buckets come from a table of distances in shared
+// memory; a thread owns one 16-byte vector of a row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -136,7 +136,8 @@ template <class T, class S>
 __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a,
                                                            const S* __restrict__ table, T* __restrict__ out,
-                                                           uint32_t chunk, uint32_t chunks, uint64_t items, int turns, int team) {
+                                                           uint32_t chunk, uint32_t chunks, uint64_t items, int turns,
+                                                           int team) {
   constexpr int N = Vec<T>::N;
   __shared__ Near near;
   __shared__ T tab[kMaxB], value[2 * kTable];  // by bucket; by distance + last
@@ -235,8 +236,8 @@ BiasArgs args_of(const dcf_bias_desc& d, const int32_t* pos) {
 
 // How the gradient is split: `splits` CTAs per head, each with `warps`
 // warps, every warp taking items (`batch` entries of one row, or `chunk` steps of
-// 32 vectors of it) in turn.  Fixed by the sizes and strides alone, so sums keep
-// their order.
+// 32 vectors of it) in turn.  Fixed by the sizes and strides alone: sums keep
+// their order, as long as rows begin at the same places within 16 bytes.
 struct GradPlan {
   int warps, splits;
   uint32_t chunk, chunks, batches;
@@ -329,7 +330,8 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
   if (tabled) {
     for (int i = threadIdx.x; i <= 2 * far; i += threads) {
       const int d = i - far, n = d < 0 ? -d : t.both ? d : 0;
-      offset[i] = (uint16_t)(32 * ((t.both && d > 0 ? t.half : 0) + (n < kTable ? near.of[n] : search(near.start, t.half, n))));
+      const int bucket = n < kTable ? near.of[n] : search(near.start, t.half, n);
+      offset[i] = (uint16_t)(32 * ((t.both && d > 0 ? t.half : 0) + bucket));
     }
     __syncthreads();
   }
@@ -358,7 +360,8 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
     const Row r = row_of(t, a, row);
     // Near enough for every distance to fit 32 bits, far enough to change no bucket
     // that the table has.
-    const int query = clip(a.pos ? (int64_t)a.pos[row] : a.first + (int64_t)row, -kOffsets - 1, (int64_t)a.keys + kOffsets + 1);
+    const int64_t at = a.pos ? (int64_t)a.pos[row] : a.first + (int64_t)row;
+    const int query = clip(at, -kOffsets - 1, (int64_t)a.keys + kOffsets + 1);
     b *= p.batch;
     const uint64_t b_end = min(a.batch, b + p.batch);
     const T* line = g + (int64_t)b * a.bs + (int64_t)h * a.hs + (int64_t)row * a.rs;
@@ -432,7 +435,10 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
 #pragma unroll
         for (int k = 0; k < N; k++) {
           const int e = c + k;
-          mine[32 * (e <= r.left ? t.half - 1 : e >= r.right ? (t.both ? 2 * t.half - 1 : 0) : near_bucket(near, t, r, e))] += sum[k];
+          const int bucket = e <= r.left    ? t.half - 1
+                             : e >= r.right ? (t.both ? 2 * t.half - 1 : 0)
+                                            : near_bucket(near, t, r, e);
+          mine[32 * bucket] += sum[k];
         }
       }
     }
@@ -575,7 +581,8 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
   const BiasArgs a = args_of(d, pos);
   const GradPlan p = grad_plan(d);
   const int add = (d.flags & DCF_BIAS_ACCUMULATE) != 0;
-  const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A) + (t.last <= kOffsets ? (2 * (size_t)(t.last < 1 ? 1 : t.last) + 1) * 2 : 0);
+  const size_t offsets = t.last <= kOffsets ? 2 * (size_t)(t.last < 1 ? 1 : t.last) + 1 : 0;
+  const size_t smem = (size_t)p.warps * d.num_buckets * 32 * sizeof(A) + offsets * 2;
   if (smem > kAccBytes - 4096 &&
       cudaFuncSetAttribute(bias_grad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 << 10) != cudaSuccess)
     return DCF_ECUDA;

@@ -9,9 +9,13 @@
 // a value v scaled by a power of two is kept as two fp16 planes, hi = fp16(v)
 // and lo = fp16(v - hi), 22 bits or more, and a product is
 //     hi hi + hi lo + lo hi
-// accumulated in fp32 in TMEM (the dropped lo lo is 2^-22 of it).  The result
-// is closer to 64-bit arithmetic than products of fp32 values are, at three
-// fp16 products instead of fp32 arithmetic on the CUDA cores.
+// (the dropped lo lo is 2^-22 of it).  The tensor core truncates as it
+// accumulates, which over a long k costs more than the split does: TMEM sums
+// short runs of k (64, or 32 in A A, whose truncation the next step amplifies)
+// and fp32 registers, which round, add the runs.  Five steps end as near to
+// 64-bit arithmetic as with products of fp32 values (8192 x 2048: 2.8e-6 here,
+// 5.4e-6 there; 258 x 131, six steps: 2.4e-6 and 2.1e-6), at three fp16
+// products instead of fp32 arithmetic on the CUDA cores.
 //
 // Scales are powers of two from bounds the host computes: singular values of
 // X are in [0, 1] at the start, a step maps s to |a s + b s^3 + c s^5|, and
@@ -793,7 +797,8 @@ __device__ __forceinline__ Operand mn_major(uint32_t at, uint32_t plane, uint32_
 // 79 x 249: 1.4e-6; with four 1.9e-6, with two in all products 1.3e-6 but 14 us of 38
 // more at 96 x 96; plain fp32 products 1.1e-6).
 template <int PER>
-__device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int from, int to) {
+__device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int from,
+                                            int to) {
   const uint32_t idesc =
       (1u << 4) | (p.mn << 15) | (q.mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 #pragma unroll 1
@@ -979,7 +984,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
         const int i = u * kFewThreads + (int)threadIdx.x;
         if (i >= items) break;
         const int r = rank * share + i / 16, c4 = i % 16 * 2;
-        const uint32_t at0 = ab_at + (uint32_t)(r * 512 + (c4 ^ (r & 7)) * 16), at1 = ab_at + (uint32_t)(r * 512 + ((c4 + 1) ^ (r & 7)) * 16);
+        const uint32_t at0 = ab_at + (uint32_t)(r * 512 + (c4 ^ (r & 7)) * 16);
+        const uint32_t at1 = ab_at + (uint32_t)(r * 512 + ((c4 + 1) ^ (r & 7)) * 16);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[u][j] = 0;
         for (int k = 0; k < ctas; k += 4) {  // eight loads in flight
@@ -1086,8 +1092,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
           *(uint4*)at = hi;
           *(uint4*)(at + plane) = lo;
         } else if (row0 + lr < g.in.rows) {
-          put_row8(g.out, g.out_dtype, g.vectors, (int64_t)z * g.out_bs + (int64_t)(row0 + lr) * g.out_rs + col0 + lc + 8 * k,
-                   g.in.cols - (col0 + lc + 8 * k), v);
+          const int64_t at = (int64_t)z * g.out_bs + (int64_t)(row0 + lr) * g.out_rs + col0 + lc + 8 * k;
+          put_row8(g.out, g.out_dtype, g.vectors, at, g.in.cols - (col0 + lc + 8 * k), v);
         }
       }
     }
@@ -1376,7 +1382,8 @@ int gemm_symmetric(const CUtensorMap& x, GemmArgs g, const Cut& cut, uint64_t ba
   parts.total *= cut.splits;
   if (int rc = gemm_run<PART, MN, MN>(x, x, parts, s)) return rc;
   const int64_t warps = (int64_t)g.total * (kTile / 32 * (g.tile_n / 32));
-  return launch(orth_join_kernel<MODE>, dim3((unsigned)((warps + kJoinWarps - 1) / kJoinWarps)), 32 * kJoinWarps, 0, 1, s, g);
+  const unsigned blocks = (unsigned)((warps + kJoinWarps - 1) / kJoinWarps);
+  return launch(orth_join_kernel<MODE>, dim3(blocks), 32 * kJoinWarps, 0, 1, s, g);
 }
 
 }  // namespace
@@ -1441,12 +1448,14 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
   a.vectors = vectors(in, a.rs, a.bs, dtype_size(a.dtype));
   const int64_t out_rs = d.out_row_stride ? d.out_row_stride : (int64_t)d.cols;
   const int64_t out_bs = d.out_batch_stride ? d.out_batch_stride : (int64_t)d.rows * out_rs;
-  if (few_ctas(d)) return launch_few(d, a, out, out_rs, out_bs, vectors(out, out_rs, out_bs, dtype_size((int)d.out_dtype)), st, s);
+  const int whole = vectors(out, out_rs, out_bs, dtype_size((int)d.out_dtype));
+  if (few_ctas(d)) return launch_few(d, a, out, out_rs, out_bs, whole, st, s);
   int rc = launch(orth_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, 1, s, a, l.part);
   if (rc) return rc;
   int sx = d.steps ? scale_of(1) : 0;
   const uint64_t groups = (d.cols + 7) / 8 * d.rows, blocks = (groups + kNormThreads - 1) / kNormThreads;
-  rc = launch(orth_split_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch), kNormThreads, 0, 1, s, a,
+  const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch);
+  rc = launch(orth_split_kernel, grid, kNormThreads, 0, 1, s, a,
               (const double*)l.part, l.parts, d.eps, ldexp(1.0, sx), l.x[0], d.steps ? (void*)nullptr : out,
               (int)d.out_dtype, out_rs, out_bs);
   if (rc) return rc;
@@ -1493,7 +1502,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
       g.alpha = (float)ldexp(1.0, -sb - sx);
       g.out = out;
       g.out_dtype = (int)d.out_dtype;
-      g.vectors = vectors(out, out_rs, out_bs, dtype_size(g.out_dtype));
+      g.vectors = whole;
       g.out_rs = out_rs;
       g.out_bs = out_bs;
       rc = tall ? gemm<FINAL, false, false>(x, mb, g, d.batch, s) : gemm<FINAL, false, true>(mb, x, g, d.batch, s);

@@ -1381,7 +1381,8 @@ int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in, void* out
   if (!in || !out || !status || (ws && !workspace)) return set_err(DCF_EINVAL, "null pointer");
   if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
   if (in == out) {
-    const int64_t rs = q.row_stride ? q.row_stride : (int64_t)q.cols, os = q.out_row_stride ? q.out_row_stride : (int64_t)q.cols;
+    const int64_t rs = q.row_stride ? q.row_stride : (int64_t)q.cols;
+    const int64_t os = q.out_row_stride ? q.out_row_stride : (int64_t)q.cols;
     const int64_t bs = q.batch_stride ? q.batch_stride : (int64_t)q.rows * rs;
     const int64_t ob = q.out_batch_stride ? q.out_batch_stride : (int64_t)q.rows * os;
     if (q.dtype != q.out_dtype || rs != os || bs != ob)

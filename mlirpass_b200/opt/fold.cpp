@@ -960,7 +960,8 @@ Plan learned_pattern(Op* op, Engine& eng) {
   const std::vector<int64_t>&in = k->ty->shape, &out = rty->shape;
   auto q = std::make_unique<FoldRequest>();
   if (op->name == "dcf.position_bias") {
-    if (in.size() != 2 || out.size() != 3 || in[1] != out[0] || !fits32({in[0], in[1], out[1], out[2]})) return Plan::failed();
+    if (in.size() != 2 || out.size() != 3 || in[1] != out[0] || !fits32({in[0], in[1], out[1], out[2]}))
+      return Plan::failed();
     dcf_bias_desc& d = q->bias;
     d.dtype = (uint32_t)rty->dtype;
     d.table_dtype = (uint32_t)k->dtype;
@@ -976,7 +977,8 @@ Plan learned_pattern(Op* op, Engine& eng) {
   } else if (op->name == "dcf.position_bias_grad") {
     const size_t o = in.size() == 4 ? 1 : 0;
     if (in.size() != 3 + o || out.size() != 2 || in[o] != out[1] ||
-        rty->dtype != (k->dtype == DCF_F64 ? DCF_F64 : DCF_F32) || !fits32({out[0], in[o], in[o + 1], in[o + 2], o ? in[0] : 1}))
+        rty->dtype != (k->dtype == DCF_F64 ? DCF_F64 : DCF_F32) ||
+        !fits32({out[0], in[o], in[o + 1], in[o + 2], o ? in[0] : 1}))
       return Plan::failed();
     dcf_bias_desc& d = q->bias;
     d.dtype = d.table_dtype = (uint32_t)k->dtype;
