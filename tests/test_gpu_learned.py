@@ -161,6 +161,19 @@ def test_bias_past_32_bits_of_elements(dcf):
     assert int(flat[keys:row].count_nonzero()) == 0
 
 
+def test_bias_of_the_longest_row(dcf):
+    """Columns up to the largest count that is taken: offsets of columns near 2^31."""
+    import torch
+    keys = (1 << 31) - 65536
+    plan = dcf.position_bias_plan("f16", 1, 1, keys, first_query=keys - 200)
+    flat = torch.zeros(keys + 8, dtype=torch.float16, device="cuda")
+    table = randn((32, 1), "f16", 8)
+    dcf.position_bias_async(plan, table, flat)
+    ids = lo.buckets(lo.positions(1, 500), 700, 32, 128, True)
+    assert np.array_equal(values(flat[keys - 700:keys])[None, None], bias_want(values(table), ids, None))
+    assert (flat[:keys - 700] == table[15, 0]).all() and (flat[keys:] == 0).all()
+
+
 # -------------------------------------------------------------- gradient
 
 
@@ -262,6 +275,33 @@ def test_grad_of_nothing_is_zero(dcf, shape):
     assert (run_grad(dcf, g, "f32") == 0).all()
     out = torch.full((32, 2), 2.0, device="cuda")
     assert (run_grad(dcf, g, "f32", out=out) == 2.0).all()
+
+
+@pytest.mark.parametrize("keys,strides", [(19, (20, 20, (1 << 32) + 40)), (24, ((1 << 32) + 40, 48, 24)),
+                                          ((1 << 31) - 65536, ((1 << 31) - 65536,) * 3)])
+def test_grad_past_32_bits_of_elements(dcf, keys, strides):
+    """Offsets beyond 2^32 elements, and the longest row.  Powers of two: every sum is exact."""
+    import torch
+    rows = 1 if keys > 24 else 2
+    batch = 2 if keys == 24 else 1
+    n = (batch - 1) * strides[0] + (rows - 1) * strides[2] + keys
+    flat = torch.zeros(n, dtype=torch.float16, device="cuda")
+    g = flat.as_strided((batch, 1, rows, keys), strides + (1,))
+    want, ids = np.zeros((32, 1)), lo.buckets([10], 20, 32, 128, True)
+    first = keys - 10
+    for k in range(batch * rows):
+        for d, v in ((-9, 1.0), (-3, 2.0), (0, 4.0), (2, 8.0), (8, 16.0)):
+            b, r = divmod(k, rows)
+            place = first + r + d
+            if place >= keys:
+                continue
+            g[b, 0, r, place] = v * 8.0 ** k
+            want[ids[0, 10 + d], 0] += v * 8.0 ** k
+    if keys > 24:
+        g[0, 0, 0, 0] = 0.5
+        want[15, 0] += 0.5
+    got = run_grad(dcf, g, "f16", first_query=first)
+    assert np.array_equal(values(got), want)
 
 
 def test_grad_same_bits_every_time(dcf):
@@ -530,6 +570,59 @@ def test_another_stream_and_captured_graph(dcf):
     # and the step means what it says: the table's rows move against the gradient
     ids = lo.buckets(lo.positions(queries, 0), keys, 32, 128, True)
     check_grad(dtable, g, "f32", ids, None)
+
+
+def test_two_streams_at_once_and_graphs_that_share_a_workspace(dcf):
+    import torch
+    xs = [randn((3, 200, 333), "f32", 71), randn((12, 150, 140), "f32", 72)]
+    gs = [randn((2, 4, 300, 257), "bf16", 73), randn((1, 4, 300, 257), "bf16", 74)]
+    orth = [dcf.orthogonalize_plan("f32", *x.shape[1:], batch=x.shape[0]) for x in xs]
+    grad = [dcf.position_bias_plan("bf16", 4, 300, 257, batch=g.shape[0]) for g in gs]
+    want = [run_orth(dcf, x, "f32") for x in xs], [run_grad(dcf, g, "bf16") for g in gs]
+    got = [torch.empty_like(x) for x in xs], [torch.empty(32, 4, device="cuda") for _ in gs]
+    size = [dcf.orthogonalize_workspace(o) for o in orth], [dcf.position_bias_grad_workspace(p) for p in grad]
+    status = torch.empty(2, 2, dtype=torch.int64, device="cuda")
+    for k in range(2):
+        dcf.status_reset(status[k])
+
+    def run(k, w1, w2):
+        dcf.orthogonalize_async(orth[k], xs[k], got[0][k], w1, status[k])
+        dcf.position_bias_grad_async(grad[k], gs[k], got[1][k], w2)
+
+    def same():
+        torch.cuda.synchronize()
+        for a, b in zip(want[0] + want[1], got[0] + got[1]):
+            assert torch.equal(a, b)
+        for t in got[0] + got[1]:
+            t.fill_(float("nan"))
+
+    own = [[torch.empty(n[k] + 1, dtype=torch.uint8, device="cuda") for n in size] for k in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                run(k, *own[k])
+    same()
+    shared = [torch.empty(max(n) + 1, dtype=torch.uint8, device="cuda") for n in size]
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for k in range(2):
+        with torch.cuda.graph(graphs[k]):
+            run(k, *shared)
+    for order in ((0, 1), (1, 0), (0, 0, 1, 1)):
+        for k in order:
+            graphs[k].replay()
+        same()
+    assert all(dcf.status_read(status[k]).folded for k in range(2))
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(65535, 3, 5), (70, 130, 150), (300, 20, 2100)])
+def test_orth_many_matrices(dcf, batch, rows, cols):
+    x = randn((batch, rows, cols), "f32", 81)
+    got = run_orth(dcf, x, "f32")
+    at = [0, 1, batch // 2, batch - 2, batch - 1]
+    check_orth(got[at], x[at], "f32", [COEF] * 5)
+    assert bool(got.isfinite().all())
 
 
 @pytest.mark.parametrize("rows,cols,dtype", [(1601, 1550, "f32"), (1540, 1603, "bf16"), (1536, 2100, "f32")])
