@@ -258,7 +258,13 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
   const uint64_t n = 16 / es;
   p.warps = (int)(kAccBytes / (d.num_buckets * 32 * acc));
   p.warps = p.warps > 8 ? 8 : p.warps < 1 ? 1 : p.warps;
-  const uint64_t steps = (vectors_of_row(d.keys, n, false) + 31) / 32, rows = d.queries;
+  const int64_t rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
+  const int64_t hs = d.head_stride ? d.head_stride : (int64_t)d.queries * rs;
+  const int64_t bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * hs;
+  // (Where only the first row is not aligned, a row's last part takes the
+  // vector more that it may have.)
+  const bool aligned = rs % (int64_t)n == 0 && hs % (int64_t)n == 0 && bs % (int64_t)n == 0;
+  const uint64_t steps = (vectors_of_row(d.keys, n, aligned) + 31) / 32, rows = d.queries;
   const uint64_t ctas = d.heads ? (uint64_t)(kSms * 4 + d.heads - 1) / d.heads : 1;  // per head: four to an SM
   const uint64_t slots = ctas * p.warps;
   if (rows == 0 || d.batch == 0 || steps == 0) {
@@ -269,16 +275,15 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
     return p;
   }
   // Batch entries of a row share the buckets, as long as their rows are aligned
-  // alike; where that leaves fewer than three items per warp, rows are cut into
-  // parts, then the batch.
-  const int64_t rs = d.row_stride ? d.row_stride : (int64_t)d.keys;
-  const int64_t hs = d.head_stride ? d.head_stride : (int64_t)d.queries * rs;
-  const int64_t bs = d.batch_stride ? d.batch_stride : (int64_t)d.heads * hs;
+  // alike; where that leaves few items, rows are cut into parts, then the batch,
+  // as far as each warp has no more than three (8 x 12 x 512 x 512 bf16: 24.6 us
+  // with four to six smaller items, 19.8 us with three).
   uint64_t cuts = slots * 3 / rows;
   cuts = cuts < 1 ? 1 : cuts > steps ? steps : cuts;
   p.chunk = (uint32_t)((steps + cuts - 1) / cuts);
   p.chunks = (uint32_t)((steps + p.chunk - 1) / p.chunk);
-  uint64_t batches = (slots * 3 + rows * p.chunks - 1) / (rows * p.chunks);
+  uint64_t batches = slots * 3 / (rows * p.chunks);
+  if (batches < 1) batches = 1;
   if (batches > d.batch || bs % (int64_t)n) batches = d.batch;
   p.batch = (d.batch + batches - 1) / batches;
   p.batches = (uint32_t)((d.batch + p.batch - 1) / p.batch);
@@ -371,21 +376,28 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
     // Steps [l0, l1) lie in the left range, [r0, r1) in the right one.
     const int l0 = shift ? 1 : 0, l1 = (min(r.left + 1, r.end) + shift) / kStep;
     const int r0 = max(l0, (r.right + shift + kStep - 1) / kStep), r1 = (r.end + shift) / kStep;
-    const int stop = min((int)((cut + 1) * p.chunk), r.end > 0 ? (r.end + shift + kStep - 1) / kStep : 0);
+    int stop = r.end > 0 ? (r.end + shift + kStep - 1) / kStep : 0;
+    if (cut + 1 < p.chunks) stop = min(stop, (int)((cut + 1) * p.chunk));
     int i = (int)(cut * p.chunk);
     while (i < stop) {
       const bool left = i >= l0 && i < l1;
       if (left || (i >= r0 && i < r1)) {
         const int to = min(stop, left ? l1 : r1);
         A s = 0;
-        const T* at = lane_at;
-        for (int e = 0; e < entries; e++, at += a.bs) {
-          for (int j = i; j < to; j += 4) {  // four in flight, the last ones too
+        // Four loads in flight, the last ones too, along what is longer: the steps
+        // or the batch entries.
+        const bool across = entries > to - i;
+        const int fast = across ? entries : to - i, slow = across ? to - i : entries;
+        const int64_t fast_by = across ? a.bs : kStep, slow_by = across ? kStep : a.bs;
+        const T* at = lane_at + (int64_t)i * kStep;
+        for (int e = 0; e < slow; e++, at += slow_by) {
+          const T* from = at;
+          for (int j = 0; j < fast; j += 4, from += 4 * fast_by) {
             Vec<T> x[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
               *(uint4*)&x[k] = make_uint4(0, 0, 0, 0);
-              if (j + k < to) *(uint4*)&x[k] = __ldg((const uint4*)(at + (int64_t)(j + k) * kStep));
+              if (j + k < fast) *(uint4*)&x[k] = __ldg((const uint4*)(from + k * fast_by));
             }
             s += (sum_of(x[0]) + sum_of(x[1])) + (sum_of(x[2]) + sum_of(x[3]));
           }
