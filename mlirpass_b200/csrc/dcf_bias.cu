@@ -211,10 +211,18 @@ __global__ void __launch_bounds__(kFwdThreads) bias_kernel(const __grid_constant
 
 template <class T> struct AccOf { using type = float; };
 template <> struct AccOf<double> { using type = double; };
-__device__ __forceinline__ float widen(float x) { return x; }
-__device__ __forceinline__ double widen(double x) { return x; }
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+// s + x in the sum's type.  16-bit values are added by one instruction, exact but
+// for the sum's rounding, where a conversion and an addition are two.
+__device__ __forceinline__ float plus(float s, float x) { return s + x; }
+__device__ __forceinline__ double plus(double s, double x) { return s + x; }
+__device__ __forceinline__ float plus(float s, __half x) {
+  asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(s) : "h"(__half_as_ushort(x)));
+  return s;
+}
+__device__ __forceinline__ float plus(float s, __nv_bfloat16 x) {
+  asm("add.rn.f32.bf16 %0, %1, %0;" : "+f"(s) : "h"(__bfloat16_as_ushort(x)));
+  return s;
+}
 
 constexpr size_t kAccBytes = 48 << 10;
 constexpr int kOffsets = 2048;  // distances (each way) for which a block tables where their sums are
@@ -277,7 +285,7 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
   // Batch entries of a row share the buckets, as long as their rows are aligned
   // alike; where that leaves few items, rows are cut into parts, then the batch,
   // as far as each warp has no more than three (8 x 12 x 512 x 512 bf16: 24.6 us
-  // with four to six smaller items, 19.8 us with three).
+  // with up to six smaller items, 18.4 us with three).
   uint64_t cuts = slots * 3 / rows;
   cuts = cuts < 1 ? 1 : cuts > steps ? steps : cuts;
   p.chunk = (uint32_t)((steps + cuts - 1) / cuts);
@@ -295,11 +303,7 @@ GradPlan grad_plan(const dcf_bias_desc& d) {
   return p;
 }
 
-template <class T> __device__ __forceinline__ typename AccOf<T>::type sum_of(const Vec<T>& x) {
-  constexpr int N = Vec<T>::N;
-  typename AccOf<T>::type s[N];
-#pragma unroll
-  for (int k = 0; k < N; k++) s[k] = widen(x.e[k]);
+template <class A, int N> __device__ __forceinline__ A total(A (&s)[N]) {
 #pragma unroll
   for (int u = N / 2; u > 0; u >>= 1)
 #pragma unroll
@@ -308,10 +312,12 @@ template <class T> __device__ __forceinline__ typename AccOf<T>::type sum_of(con
 }
 
 // A warp walks along a row in steps of 32 vectors.  Steps that lie wholly in a
-// far range are only summed (18 instructions for 512 bytes of f16); the others
+// far range are only summed, one instruction per element; the others
 // are summed over the batch entries, then every element adds into its bucket's
 // sum, which each lane has for itself in shared memory, found by a table of
-// distances.
+// distances.  2 x 16 x 4001 x 4001 causal f16: 126 us, 4.1 TB/s; what it waits for
+// is its loads (half of the stalls).  Eight loads in flight per lane, or five CTAs
+// to an SM, need more registers than there are: 157 and 172 us.
 template <class T>
 __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant__ Buckets t,
                                                            const __grid_constant__ BiasArgs a, const T* __restrict__ g,
@@ -383,7 +389,9 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
       const bool left = i >= l0 && i < l1;
       if (left || (i >= r0 && i < r1)) {
         const int to = min(stop, left ? l1 : r1);
-        A s = 0;
+        A s[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) s[k] = 0;
         // Four loads in flight, the last ones too, along what is longer: the steps
         // or the batch entries.
         const bool across = entries > to - i;
@@ -399,11 +407,14 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
               *(uint4*)&x[k] = make_uint4(0, 0, 0, 0);
               if (j + k < fast) *(uint4*)&x[k] = __ldg((const uint4*)(from + k * fast_by));
             }
-            s += (sum_of(x[0]) + sum_of(x[1])) + (sum_of(x[2]) + sum_of(x[3]));
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+              for (int k = 0; k < N; k++) s[k] = plus(s[k], x[u].e[k]);
           }
         }
-        if (left) far_left += s;
-        else far_right += s;
+        if (left) far_left += total(s);
+        else far_right += total(s);
         i = to;
         continue;
       }
@@ -424,18 +435,26 @@ __global__ void __launch_bounds__(256, 4) bias_grad_kernel(const __grid_constant
           }
 #pragma unroll
           for (int k = 0; k < N; k++)
-            sum[k] += (widen(x[0].e[k]) + widen(x[1].e[k])) + (widen(x[2].e[k]) + widen(x[3].e[k]));
+#pragma unroll
+            for (int u = 0; u < 4; u++) sum[k] = plus(sum[k], x[u].e[k]);
         }
       } else {
         for (int e = 0; e < entries; e++, at += a.bs)
 #pragma unroll
           for (int k = 0; k < N; k++)
-            if (c + k >= 0 && c + k < r.end) sum[k] += widen(at[k]);
+            if (c + k >= 0 && c + k < r.end) sum[k] = plus(sum[k], at[k]);
       }
       if (c < 0 || c + N > r.end) {  // what lies outside adds nothing
 #pragma unroll
         for (int k = 0; k < N; k++)
           if (c + k < 0 || c + k >= r.end) sum[k] = 0;
+      }
+      // A first or last step that a far range covers as far as the row reaches.
+      const int from = i * kStep - kStep - shift;
+      if (from + kStep <= r.left + 1 || from >= r.right) {
+        if (from >= r.right) far_right += total(sum);
+        else far_left += total(sum);
+        continue;
       }
       // (Lanes in a far range add into its bucket the same way: a branch of
       // their own cost the warp more.)
