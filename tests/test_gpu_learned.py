@@ -255,6 +255,21 @@ def test_grad_strides(dcf, shape, strides, off, dtype):
     check_grad(got, g, dtype, lo.buckets(lo.positions(shape[2], 3), shape[3], 32, 128, True), None)
 
 
+@pytest.mark.parametrize("off", [0, 1, 7])
+@pytest.mark.parametrize("batch,queries,keys,first", [(2, 20, 512, 100), (8, 40, 512, -600), (5, 3, 1024, 900),
+                                                      (6, 700, 256, 0)])
+@pytest.mark.parametrize("dtype,causal", [("bf16", False), ("f16", True), ("f64", False)])
+def test_grad_whole_steps_from_any_start(dcf, off, batch, queries, keys, first, dtype, causal):
+    """Rows of whole steps, whose first element is off the boundary: the last
+    part of a row has a step more."""
+    n = batch * 2 * queries * keys
+    flat = randn((n + 8,), dtype, 19)
+    g = flat[off:off + n].view(batch, 2, queries, keys)
+    got = run_grad(dcf, g, dtype, first_query=first, bidirectional=not causal, causal=causal)
+    at = lo.positions(queries, first)
+    check_grad(got, g, dtype, lo.buckets(at, keys, 32, 128, not causal), lo.masked(at, keys) if causal else None)
+
+
 def test_grad_accumulates_and_overwrites(dcf):
     import torch
     g = randn((1, 2, 300, 300), "bf16", 16)
