@@ -11,8 +11,8 @@
 //     hi hi + hi lo + lo hi
 // (the dropped lo lo is 2^-22 of it).  The tensor core truncates as it
 // accumulates, which over a long k costs more than the split does: TMEM sums
-// short runs of k (64, or 32 in A A, whose truncation the next step amplifies)
-// and fp32 registers, which round, add the runs.  Five steps end as near to
+// short runs of k (32 to 128, see sums_of) and fp32 registers, which round, add
+// the runs.  Five steps end as near to
 // 64-bit arithmetic as with products of fp32 values (8192 x 2048: 2.8e-6 here,
 // 5.4e-6 there; 258 x 131, six steps: 2.4e-6 and 2.1e-6), at three fp16
 // products instead of fp32 arithmetic on the CUDA cores.
@@ -372,9 +372,7 @@ __device__ __forceinline__ float* part_block(const GemmArgs& g, int64_t item, in
 // instruction: 1e-4 in the result over k = 8192.  So TMEM sums `sum` stages
 // only (the two small products of a stage first, then the large one), in two
 // buffers in turn, and the eight warps add the sums in registers, rounding to
-// nearest: every stage where the result is f32 (3e-6 there; two stages: 6e-6,
-// and plain fp32 products 5e-6; every half stage in A A of few rows), 16 where it is rounded to 16 bits anyway (1e-5),
-// which leaves the warps time to write a tile while the next is multiplied.
+// nearest; sums_of says how many stages.
 template <Mode MODE, bool P_MN, bool Q_MN, int TN>
 __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid_constant__ CUtensorMap map_p,
                                                                     const __grid_constant__ CUtensorMap map_q,
@@ -793,9 +791,12 @@ __device__ __forceinline__ Operand mn_major(uint32_t at, uint32_t plane, uint32_
 
 // Every PER slices of 16 k have an accumulator of their own, `pitch` columns after
 // the last, and the small products come first, while its sum is small: the tensor
-// core truncates.  Four slices, and two in A A where the result is f32 (from 64 bits, at
+// core truncates.  Four slices, and two in A A (from 64 bits, f32 at
 // 79 x 249: 1.4e-6; with four 1.9e-6, with two in all products 1.3e-6 but 14 us of 38
-// more at 96 x 96; plain fp32 products 1.1e-6).
+// more at 96 x 96; plain fp32 products 1.1e-6).  Of few rows most of A's and B's k is
+// zero and left out, and the accumulators it would take halve the runs: up to 80 rows one
+// slice in A A, up to 64 two in B X (60 x 1000: 3.3e-6 -> 2.3e-6, plain fp32 products 2.0e-6;
+// 8 x 60 x 60: 30 -> 28 us).
 template <int PER>
 __device__ __forceinline__ void one_product(uint32_t d, int pitch, const Operand& p, const Operand& q, int n, int from,
                                             int to) {
@@ -849,7 +850,6 @@ __device__ __forceinline__ void cluster_sync(int ctas) {
   else __syncthreads();
 }
 
-template <int PER>
 __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_constant__ FewArgs g) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);  // (a cast through an integer would make every access generic)
@@ -930,6 +930,8 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   const Operand x_gram = g.tall ? x_mn : k_major(x_at, plane, block);
   const int part = warp & 3, quarter = warp >> 2, row = part * 32 + lane;  // TMEM lanes; columns
   const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16);
+  // A A: columns, and slices of 16 k that are not all zero.
+  const int square = m > 64 && m <= 80 ? 96 : 128, slices = m <= 64 ? 4 : m <= 80 ? 5 : 8;
   bool fail = false;
   unsigned phase = 0;
   auto before = [&]() {  // shared memory written so far is what the products read
@@ -1032,14 +1034,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     }
     before();
     if (threadIdx.x == 0) {
-      one_product<PER>(tmem, 128, ab_k, ab_k, 128, 0, 8);
+      if (m <= 80) one_product<1>(tmem, square, ab_k, ab_k, square, 0, slices);
+      else one_product<2>(tmem, square, ab_k, ab_k, square, 0, slices);
       one_commit(&done);
     }
     after();
     const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
     {
       float x[32];
-      product_of(lanes + c, 128, 8 / PER, x);
+      if (c < square) {
+        product_of(lanes + c, square, m <= 80 ? slices : slices / 2, x);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; j++) x[j] = 0;
+      }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         uint8_t* at = ab + few_offset(row, c + 8 * k, 128 * 128);
@@ -1064,11 +1072,15 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     }
     before();
     if (threadIdx.x == 0) {
-      if (g.tall)
-        for (int b = 0; b < g.slice / 128; b++)
-          one_product<4>(tmem + b * 128, g.slice, k_major(x_at + (uint32_t)b * 128 * 128, plane, block), ab_k, 128, 0, 8);
-      else
-        one_product<4>(tmem, g.slice, ab_k, x_mn, g.slice, 0, 8);
+      auto apply = [&](auto product, int to) {
+        if (g.tall)
+          for (int b = 0; b < g.slice / 128; b++)
+            product(tmem + b * 128, g.slice, k_major(x_at + (uint32_t)b * 128 * 128, plane, block), ab_k, 128, 0, to);
+        else
+          product(tmem, g.slice, ab_k, x_mn, g.slice, 0, to);
+      };
+      if (m <= 64) apply(one_product<2>, 4);
+      else apply(one_product<4>, 8);
       one_commit(&done);
     }
     after();
@@ -1178,10 +1190,28 @@ int scale_of(double bound) {
 }
 
 constexpr double kMostSingular = 64;
-// Up to so many rows A A of a f32 result is summed every 32 k: there plain fp32 products
-// are as near to 64 bits as every 64 k leave it (258 x 131, six steps: 3.6e-6 and
-// 2.1e-6); at 2048 rows those are at 5.4e-6 and it is at 2.8e-6.
-constexpr int kFineRows = 1024;
+
+// Stages of 64 k that TMEM sums before registers do, 0 for half a stage: few
+// enough for the result to be as near to 64 bits as with products of fp32 values.
+//
+// f32 results: every stage (8192 x 2048: 2.8e-6; two stages 6e-6, fp32 products
+// 5.4e-6), and every half stage in A A, whose truncation the next step amplifies, of up to
+// 1024 rows, where fp32 products are nearer (258 x 131, six steps: 3.6e-6 with whole
+// stages, 2.4e-6 with half ones, fp32 products 2.1e-6).
+//
+// 16-bit results hide less than that: the share of them that is not the 64-bit value
+// rounded is proportional to the error before the rounding.  Up to 768 rows as for
+// f32 (bf16 258 x 131, six steps: 0.21 % of the results, with two stages 0.58 %, fp32 products
+// 0.17 %; 520 x 530: two stages 0.33 %, fp32 products 0.20 %), above two stages (4096 x 4096:
+// 0.25 % and 3.6 ms, with 16 1.8 % and 3.4 ms, fp32 products 0.33 %), up to 1024 rows one in A A
+// (1024 x 4096: 0.2 %, with two 0.23 %, with 16 1.6 %, fp32 products 0.27 %; 770 x 1540: with two
+// 1.8 times as many as fp32 products).
+int sums_of(const dcf_orth_desc& d, int m, bool square) {
+  const bool f32 = d.out_dtype == DCF_F32;
+  if (square && m <= 1024) return f32 || m <= 768 ? 0 : 1;
+  return f32 || m <= 768 ? 1 : 2;
+}
+
 constexpr int kPairs = 74;  // pairs of SMs
 
 // Blocks of the norm's sum: 32 KB of a f32 matrix each, 256 at most.
@@ -1343,9 +1373,8 @@ int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out
   }
   int smem = 2 * (128 * g.slice * 2) + 2 * kFewPlane + 1024;
   if (smem < kFewLeast) smem = kFewLeast;
-  auto kernel = d.out_dtype == DCF_F32 ? orth_few_kernel<2> : orth_few_kernel<4>;
-  if (!prepare_smem((const void*)kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
-  return launch(kernel, dim3((unsigned)(d.batch * ctas)), kFewThreads, smem, ctas, s, g);
+  if (!prepare_smem((const void*)orth_few_kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
+  return launch(orth_few_kernel, dim3((unsigned)(d.batch * ctas)), kFewThreads, smem, ctas, s, g);
 }
 
 template <Mode MODE, bool P_MN, bool Q_MN>
@@ -1475,7 +1504,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     const CUtensorMap& x = mx[i & 1];
     GemmArgs g = {};
     g.st = st;
-    g.sum = d.out_dtype == DCF_F32 ? 1 : 16;
+    g.sum = sums_of(d, m, false);
     g.part = l.sums;
     g.m = g.n = m;
     g.k = n;
@@ -1489,9 +1518,9 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
     g.to = l.b;
-    if (d.out_dtype == DCF_F32 && m <= kFineRows) g.sum = 0;
+    g.sum = sums_of(d, m, true);
     if ((rc = gemm_symmetric<POLY, false>(ma, g, l.poly, d.batch, s))) return rc;
-    g.sum = d.out_dtype == DCF_F32 ? 1 : 16;
+    g.sum = sums_of(d, m, false);
     g.m = rows;
     g.n = cols;
     if (i + 1 < d.steps) {

@@ -645,3 +645,43 @@ def test_orth_large(dcf, rows, cols, dtype):
     """Sizes that pairs of CTAs take."""
     x = randn((1, rows, cols), dtype, 61)
     check_orth(run_orth(dcf, x, dtype, steps=2), x, dtype, [COEF] * 2)
+
+
+def fp32_form(x, steps):
+    """The iteration with products of fp32 values, rounded once to x's type."""
+    y = x.float() if x.shape[1] <= x.shape[2] else x.float().transpose(1, 2)
+    y = y / (y.square().sum((1, 2), keepdim=True).sqrt() + 1e-7)
+    a, b, c = COEF
+    for _ in range(steps):
+        gram = y @ y.transpose(1, 2)
+        y = a * y + (b * gram + c * (gram @ gram)) @ y
+    return (y if x.shape[1] <= x.shape[2] else y.transpose(1, 2)).to(x.dtype)
+
+
+def exact_form(x, steps):
+    import torch
+    y = x.double() if x.shape[1] <= x.shape[2] else x.double().transpose(1, 2)
+    y = y / (torch.linalg.vector_norm(y, dim=(1, 2), keepdim=True) + 1e-7)
+    a, b, c = COEF
+    for _ in range(steps):
+        gram = y @ y.transpose(1, 2)
+        y = a * y + (b * gram + c * (gram @ gram)) @ y
+    return y if x.shape[1] <= x.shape[2] else y.transpose(1, 2)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("batch,rows,cols", [(8, 96, 96), (8, 128, 128), (8, 128, 1000), (8, 1000, 60), (8, 70, 900), (8, 150, 180),
+                                             (8, 258, 131), (8, 260, 300), (1, 512, 2048), (1, 520, 530),
+                                             (1, 800, 810), (1, 1300, 1100), (1, 1024, 4096), (1, 4096, 300)])
+def test_orth_rounds_what_fp32_products_would(dcf, dtype, batch, rows, cols):
+    """Results of 16 bits come from sums as exact as those of fp32 products: a
+    result that is not the 64-bit value rounded lies within the sums' error of
+    a border, so the share of these is proportional to that error.  Half as many
+    again are allowed, and four times what counting them varies by."""
+    import torch
+    assert not torch.backends.cuda.matmul.allow_tf32
+    x = randn((batch, rows, cols), dtype, 91)
+    want = exact_form(x, 5).to(tdtype(dtype))
+    plain = float((fp32_form(x, 5) != want).double().mean())
+    here = float((run_orth(dcf, x, dtype) != want).double().mean())
+    assert here <= 1.5 * plain + 4 * (plain / want.numel()) ** 0.5, (here, plain)
