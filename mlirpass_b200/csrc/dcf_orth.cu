@@ -658,6 +658,11 @@ __device__ __forceinline__ void load_row8(const MatArgs& a, uint32_t z, int r, i
   }
 }
 
+// scale / (norm + eps); 0 for a matrix of zeros, which stays one however small eps is.
+__device__ __forceinline__ double factor_of(double norm, double eps, double scale) {
+  return norm == 0 && eps > 0 ? 0 : scale / (norm + eps);
+}
+
 constexpr int kNormThreads = 256;
 
 // Sums of squares in 64 bits (a f32 element's square can pass 32), one part
@@ -696,7 +701,7 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
     double s = 0;
     for (int i = threadIdx.x; i < parts; i += 32) s += part[(size_t)z * parts + i];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (threadIdx.x == 0) factor = scale / (sqrt(s) + eps);
+    if (threadIdx.x == 0) factor = factor_of(sqrt(s), eps, scale);
   }
   __syncthreads();
   const double f = factor;
@@ -910,7 +915,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(remote(smem_addr(&own), k)) : "memory");
     norm += part;
   }
-  const double factor = g.scale / (sqrt(norm) + g.eps);
+  const double factor = factor_of(sqrt(norm), g.eps, g.scale);
   for (int i = threadIdx.x; i < rows * groups; i += kFewThreads) {
     const int lr = i / groups, lc = i % groups * 8, r = row0 + lr, c = col0 + lc;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};

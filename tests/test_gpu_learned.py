@@ -685,3 +685,13 @@ def test_orth_rounds_what_fp32_products_would(dcf, dtype, batch, rows, cols):
     plain = float((fp32_form(x, 5) != want).double().mean())
     here = float((run_orth(dcf, x, dtype) != want).double().mean())
     assert here <= 1.5 * plain + 4 * (plain / want.numel()) ** 0.5, (here, plain)
+
+
+@pytest.mark.parametrize("shape", [(2, 30, 40), (2, 150, 140)])
+@pytest.mark.parametrize("steps", [0, 5])
+def test_orth_zeros_stay_zeros_beside_the_smallest_eps(dcf, shape, steps):
+    import torch
+    x = torch.zeros(shape, device="cuda")
+    for eps in (1e-7, 1e-300, 1e-306, 5e-324):
+        assert (run_orth(dcf, x, "f32", steps=steps, eps=eps) == 0).all(), eps
+    assert run_orth(dcf, x, "f32", steps=steps, eps=0.0).isnan().all()      # 0 / 0
