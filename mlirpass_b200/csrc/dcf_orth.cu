@@ -17,10 +17,13 @@
 // 5.4e-6 there; 258 x 131, six steps: 2.4e-6 and 2.1e-6), at three fp16
 // products instead of fp32 arithmetic on the CUDA cores.
 //
-// Scales are powers of two from bounds the host computes: singular values of
+// Scales are powers of two from bounds: singular values of
 // X are in [0, 1] at the start, a step maps s to |a s + b s^3 + c s^5|, and
 // no element of X, A = X X^T or B exceeds the largest singular value of its matrix.
-// So no plane overflows, whatever the data.
+// So no plane overflows, whatever the data.  The host computes the bounds; a matrix whose
+// norm eps exceeds starts from norm / (norm + eps) instead of 1, and its scales are
+// made on the device (set_factors): planes scaled for 1 would lose what fp16 has no
+// exponents for (norm 1e-12 beside an eps of 1e-7: 4e-4 of X).
 //
 // A and A A are symmetric: only tiles that touch the upper triangle are
 // computed, and their elements written to both sides.
@@ -131,6 +134,58 @@ template <bool MN> constexpr uint32_t kSlice = (MN ? 2048 : 32) >> 4;
 
 // -------------------------------------------------------------- planes
 
+// What a step's products are multiplied by on their way out, powers of two included.
+struct alignas(16) Factors {
+  float gram;       // A = gram acc
+  float b2, b1, b0; // B = b2 acc + b1 A + b0 I
+  float apply;      // X = apply acc
+};
+
+// From which set_factors makes a matrix's factors; `usual` are those of a bound of 1.
+struct Scaling {
+  int steps;
+  double eps;
+  double coef[DCF_ORTH_MAX_STEPS][3];
+  double bound[DCF_ORTH_MAX_STEPS + 1];  // of X's singular values before each step and after the last
+  double largest[DCF_ORTH_MAX_STEPS];    // of B's
+  Factors usual[DCF_ORTH_MAX_STEPS];
+};
+
+// The power of two that brings a bound to at most 2^13: a factor 8 below
+// fp16's largest value, for what rounding adds.  2^132 at most: what then falls off
+// fp16's smallest value is below fp32's, too.
+__host__ __device__ inline int scale_of(double bound) {
+  int e;
+  frexp(bound > 0x1p-120 ? bound : 0x1p-120, &e);  // bound < 2^e
+  return 13 - e;
+}
+
+// The factors of every step where singular values start in [0, s].
+__host__ __device__ inline void set_factors(const Scaling& k, double s, Factors* out) {
+  int sx = scale_of(s);
+  for (int i = 0; i < k.steps; i++) {
+    const double a = k.coef[i][0], b = k.coef[i][1], c = k.coef[i][2], t = s * s;
+    const double q = fmin(k.largest[i], fabs(a) + t * (fabs(b) + t * fabs(c)));
+    s = fmin(k.bound[i + 1], s * q);
+    const bool last = i + 1 == k.steps;
+    const int sa = scale_of(t), sn = last ? 0 : scale_of(s);
+    int sb = scale_of(q);
+    if (last && sb > 149 - sx) sb = 149 - sx;  // the factor stays a fp32 value; the result is below 2^-120
+    out[i].gram = (float)ldexp(1.0, sa - 2 * sx);
+    out[i].b2 = (float)ldexp(c, sb - 2 * sa);
+    out[i].b1 = (float)ldexp(b, sb - sa);
+    out[i].b0 = (float)ldexp(a, sb);
+    out[i].apply = (float)ldexp(1.0, sn - sb - sx);
+    sx = sn;
+  }
+}
+
+// The bound to start from, given a matrix's norm: 1 unless eps exceeds the norm.
+__host__ __device__ inline double start_of(double norm, double eps) {
+  const double s = norm / (norm + eps);
+  return s < 0.5 ? s : 1;
+}
+
 // One operand as the tensor map and the epilogue see it: per matrix two
 // planes (hi, lo) of `rows` rows of `ld` fp16 values.
 struct Planes {
@@ -158,7 +213,8 @@ struct GemmArgs {
   int total;                // work items: tiles of the batch, times splits
   int splits, split_k;      // PART: parts of k, stages of each
   int sum;                  // stages that TMEM sums before registers do; 0: half a stage
-  float alpha, beta, diag;  // v = alpha acc [+ beta A + diag I]
+  const Factors* factors;   // of this step, the first matrix's; `steps` on the next one's
+  int steps;
   Planes to, from;          // result; POLY: A
   float* part;              // PART
   void* out;
@@ -268,7 +324,8 @@ __device__ __forceinline__ void put_row8(void* out, int dtype, int vectors, int6
 }
 
 // Writes the block at row r0, column c0 of the result in the caller's type.
-__device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r0, int c0, const float* buf, int lane) {
+__device__ __forceinline__ void write_final(const GemmArgs& g, const Factors& f, uint32_t z, int r0, int c0, const float* buf,
+                                            int lane) {
   if (!g.vectors) {  // element by element, a row at a time
     const int64_t at = (int64_t)z * g.out_bs + (int64_t)r0 * g.out_rs + c0 + lane;
     const int rows = c0 + lane < g.n ? min(32, g.m - r0) : 0;
@@ -276,7 +333,7 @@ __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r
       out += at;
 #pragma unroll 8
       for (int row = 0; row < 32; row++, out += g.out_rs)
-        if (row < rows) *out = cast(__fmul_rn(g.alpha, buf[place(lane, row)]));
+        if (row < rows) *out = cast(__fmul_rn(f.apply, buf[place(lane, row)]));
     };
     if (g.out_dtype == DCF_F32) each((float*)g.out, [](float v) { return v; });
     else if (g.out_dtype == DCF_F16) each((__half*)g.out, [](float v) { return __float2half_rn(v); });
@@ -288,7 +345,7 @@ __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r
   for (int row = lane >> 2; row < 32 && r0 + row < g.m; row += 8) {
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[place(o + e, row)]);
+    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(f.apply, buf[place(o + e, row)]);
     put_row8(g.out, g.out_dtype, g.vectors, (int64_t)z * g.out_bs + (int64_t)(r0 + row) * g.out_rs + c, g.n - c, v);
   }
 }
@@ -297,8 +354,10 @@ __device__ __forceinline__ void write_final(const GemmArgs& g, uint32_t z, int r
 // written with their mirror image, and one on it (blocks lie on multiples of
 // 32) takes its lower half from its upper.
 template <Mode MODE>
-__device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int r0, int c0, float* buf, int lane) {
+__device__ __forceinline__ void write_planes(const GemmArgs& g, const Factors& f, uint32_t z, int r0, int c0, float* buf,
+                                             int lane) {
   constexpr bool sym = MODE == GRAM || MODE == POLY;
+  const float alpha = MODE == GRAM ? f.gram : MODE == POLY ? f.b2 : f.apply;
   const bool on = sym && c0 == r0;
   const int o = (lane & 3) * 8, c = c0 + o;
   const size_t plane = (size_t)g.to.rows * g.to.ld;
@@ -307,7 +366,7 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
     const int r = r0 + row;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(g.alpha, buf[on && o + e < row ? place(row, o + e) : place(o + e, row)]);
+    for (int e = 0; e < 8; e++) v[e] = __fmul_rn(alpha, buf[on && o + e < row ? place(row, o + e) : place(o + e, row)]);
     if (MODE == POLY) {
       const __half* from = g.from.row(z, 0, r) + c;
       const uint4 x = *(const uint4*)from, y = *(const uint4*)(from + plane);
@@ -316,13 +375,13 @@ __device__ __forceinline__ void write_planes(const GemmArgs& g, uint32_t z, int 
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const float2 p = __half22float2(h[e]), q = __half22float2(l[e]);
-        v[2 * e] = __fmaf_rn(g.beta, __fadd_rn(p.x, q.x), v[2 * e]);
-        v[2 * e + 1] = __fmaf_rn(g.beta, __fadd_rn(p.y, q.y), v[2 * e + 1]);
+        v[2 * e] = __fmaf_rn(f.b1, __fadd_rn(p.x, q.x), v[2 * e]);
+        v[2 * e + 1] = __fmaf_rn(f.b1, __fadd_rn(p.y, q.y), v[2 * e + 1]);
       }
       if (on) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          if (o + e == row) v[e] = __fadd_rn(v[e], g.diag);
+          if (o + e == row) v[e] = __fadd_rn(v[e], f.b0);
       }
     }
     if (sym && !on) {  // for the mirror image
@@ -533,6 +592,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     int64_t u = 0;  // sums so far
     for (int t = first; t < g.total && !fail; t += step) {
       const Tile at = tile_of(t);
+      Factors f = {};
+      if (MODE != PART) f = g.factors[(size_t)at.z * g.steps];
       const int sums = g.sum ? (count_of(t) + g.sum - 1) / g.sum : 2 * count_of(t);
       float acc[kMine];
 #pragma unroll
@@ -572,8 +633,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             for (int j = 0; j < 32; j++) p[j * 32] = acc[j];
           } else {
             block_in(buf, acc, lane);
-            if (MODE == FINAL) write_final(g, at.z, r0, c0, buf, lane);
-            else write_planes<MODE>(g, at.z, r0, c0, buf, lane);
+            if (MODE == FINAL) write_final(g, f, at.z, r0, c0, buf, lane);
+            else write_planes<MODE>(g, f, at.z, r0, c0, buf, lane);
           }
         }
 #pragma unroll
@@ -606,6 +667,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const GemmAr
   const Tile at(g, (int)item, true);
   const int r0 = at.row0 + block / wide * 32, c0 = at.col0 + block % wide * 32;
   if (r0 >= g.m || c0 >= g.n || c0 + 31 < r0) return;
+  const Factors f = g.factors[(size_t)at.z * g.steps];
   float v[32];
 #pragma unroll
   for (int j = 0; j < 32; j++) v[j] = 0;
@@ -616,7 +678,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) orth_join_kernel(const GemmAr
     for (int j = 0; j < 32; j++) v[j] = __fadd_rn(v[j], p[j * 32]);
   }
   block_in(buffers[warp], v, lane);
-  write_planes<MODE>(g, at.z, r0, c0, buffers[warp], lane);
+  write_planes<MODE>(g, f, at.z, r0, c0, buffers[warp], lane);
 }
 
 // ------------------------------------------------------- norm and split
@@ -688,12 +750,12 @@ __global__ void __launch_bounds__(kNormThreads) orth_norm_kernel(const __grid_co
   }
 }
 
-// X = G / (norm + eps) into its planes, or, with no steps to take, straight
-// to the result.  A thread takes eight columns of a row.
-__global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_constant__ MatArgs a, const double* part,
-                                                                  int parts, double eps, double scale, Planes x,
-                                                                  void* out, int out_dtype, int64_t out_rs,
-                                                                  int64_t out_bs) {
+// X = G / (norm + eps) into its planes and the matrix's factors beside them, or, with
+// no steps to take, straight to the result.  A thread takes eight columns of a row.
+__global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_constant__ MatArgs a,
+                                                                  const __grid_constant__ Scaling k, const double* part,
+                                                                  int parts, Planes x, Factors* factors, void* out,
+                                                                  int out_dtype, int64_t out_rs, int64_t out_bs) {
   __shared__ double factor;
   pdl_begin();
   const uint32_t z = blockIdx.y;
@@ -701,7 +763,13 @@ __global__ void __launch_bounds__(kNormThreads) orth_split_kernel(const __grid_c
     double s = 0;
     for (int i = threadIdx.x; i < parts; i += 32) s += part[(size_t)z * parts + i];
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (threadIdx.x == 0) factor = factor_of(sqrt(s), eps, scale);
+    const double norm = sqrt(s), start = start_of(norm, k.eps);
+    if (threadIdx.x == 0) factor = factor_of(norm, k.eps, k.steps ? ldexp(1.0, scale_of(start)) : 1.0);
+    if (blockIdx.x == 0 && threadIdx.x < k.steps) {
+      Factors* to = factors + (size_t)z * k.steps;
+      if (start == 1) to[threadIdx.x] = k.usual[threadIdx.x];
+      else if (threadIdx.x == 0) set_factors(k, start, to);
+    }
   }
   __syncthreads();
   const double f = factor;
@@ -757,12 +825,7 @@ struct FewArgs {
   int64_t out_rs, out_bs;
   int tall;                 // rows > cols: X^T is what lies in memory
   int slice;                // of the longer side per CTA: a multiple of 64 (128 where tall)
-  int steps;
-  double eps;
-  // per step: A = fa acc; B = fb2 acc + fb1 A + fb0 I; X = fx acc
-  float fa[DCF_ORTH_MAX_STEPS], fb2[DCF_ORTH_MAX_STEPS], fb1[DCF_ORTH_MAX_STEPS], fb0[DCF_ORTH_MAX_STEPS],
-      fx[DCF_ORTH_MAX_STEPS];
-  double scale;             // of X's planes at the start
+  Scaling k;
   dcf_status* st;
 };
 
@@ -861,6 +924,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
   __shared__ uint64_t done;
   __shared__ uint32_t tmem_at;
   __shared__ double sums[kFewThreads / 32], own;
+  __shared__ Factors factors[DCF_ORTH_MAX_STEPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int ctas, rank;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
@@ -915,7 +979,13 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(remote(smem_addr(&own), k)) : "memory");
     norm += part;
   }
-  const double factor = factor_of(sqrt(norm), g.eps, g.scale);
+  norm = sqrt(norm);
+  const double start = start_of(norm, g.k.eps), factor = factor_of(norm, g.k.eps, ldexp(1.0, scale_of(start)));
+  if (start == 1) {
+    if (threadIdx.x < g.k.steps) factors[threadIdx.x] = g.k.usual[threadIdx.x];
+  } else if (threadIdx.x == 0) {
+    set_factors(g.k, start, factors);
+  }
   for (int i = threadIdx.x; i < rows * groups; i += kFewThreads) {
     const int lr = i / groups, lc = i % groups * 8, r = row0 + lr, c = col0 + lc;
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -952,7 +1022,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   };
 
-  for (int step = 0; step < g.steps; step++) {
+  for (int step = 0; step < g.k.steps; step++) {
     before();
     if (threadIdx.x == 0) {
       one_product<4>(tmem, 128, x_gram, x_gram, 128, 0, g.slice / 16);
@@ -962,7 +1032,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     const int c = quarter * 32;
     float sum[32];  // this thread's row, 32 columns
     product_of(lanes + c, 128, g.slice / 64, sum);
-    const float fa = g.fa[step];
+    const float fa = factors[step].gram;
     if (ctas == 1) {
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -1044,7 +1114,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
       one_commit(&done);
     }
     after();
-    const float fb2 = g.fb2[step], fb1 = g.fb1[step], fb0 = g.fb0[step];
+    const float fb2 = factors[step].b2, fb1 = factors[step].b1, fb0 = factors[step].b0;
     {
       float x[32];
       if (c < square) {
@@ -1091,7 +1161,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
     after();
     // The accumulators: wide 128 rows x slice columns, tall slice / 128 blocks of
     // 128 x 128 beside each other.
-    const float fx = g.fx[step];
+    const float fx = factors[step].apply;
 #pragma unroll 1
     for (int at_col = quarter * 32; at_col < g.slice; at_col += 128) {
       const int lr = g.tall ? (at_col & ~127) + row : row, lc = g.tall ? at_col & 127 : at_col;
@@ -1102,7 +1172,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = __fmul_rn(fx, x[8 * k + j]);
-        if (step + 1 < g.steps) {
+        if (step + 1 < g.k.steps) {
           uint4 hi, lo;
           split8(v, hi, lo);
           uint8_t* at = base + few_offset(lr, lc + 8 * k, block);
@@ -1186,12 +1256,17 @@ void step_bounds(const double* k, double s, double* x, double* q) {
   }
 }
 
-// The power of two that brings a bound to at most 2^13: a factor 8 below
-// fp16's largest value, for what rounding adds.
-int scale_of(double bound) {
-  int e;
-  frexp(bound > 1e-30 ? bound : 1e-30, &e);  // bound < 2^e
-  return 13 - e;
+Scaling scaling_of(const dcf_orth_desc& d) {
+  Scaling k = {};
+  k.steps = (int)d.steps;
+  k.eps = d.eps;
+  k.bound[0] = 1;
+  for (int i = 0; i < k.steps; i++) {
+    for (int j = 0; j < 3; j++) k.coef[i][j] = d.coef[i][j];
+    step_bounds(k.coef[i], k.bound[i], &k.bound[i + 1], &k.largest[i]);
+  }
+  set_factors(k, 1, k.usual);
+  return k;
 }
 
 constexpr double kMostSingular = 64;
@@ -1271,6 +1346,7 @@ struct Layout {
   Cut gram, poly;
   double* part;
   int parts;
+  Factors* factors;
   size_t bytes;
 };
 
@@ -1290,6 +1366,7 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
   };
   l.parts = norm_parts(d);
   l.part = (double*)take(d.batch * l.parts * 8);
+  l.factors = d.steps ? (Factors*)take(d.batch * d.steps * sizeof(Factors)) : nullptr;
   l.x[0] = l.x[1] = l.a = l.b = Planes{nullptr, 0, 0};
   if (d.steps) {
     l.x[0] = planes((int)d.rows, (int)d.cols);
@@ -1357,25 +1434,8 @@ int launch_few(const dcf_orth_desc& d, const MatArgs& in, void* out, int64_t out
   g.tall = d.rows > d.cols;
   const int n = (int)(g.tall ? d.rows : d.cols), unit = g.tall ? 128 : 64;
   g.slice = ((n + ctas - 1) / ctas + unit - 1) / unit * unit;
-  g.steps = (int)d.steps;
-  g.eps = d.eps;
+  g.k = scaling_of(d);
   g.st = st;
-  double bound = 1;
-  int sx = scale_of(1);
-  g.scale = ldexp(1.0, sx);
-  for (uint32_t i = 0; i < d.steps; i++) {
-    const double* k = d.coef[i];
-    double next, q;
-    step_bounds(k, bound, &next, &q);
-    const int sa = scale_of(bound * bound), sb = scale_of(q), sn = scale_of(next);
-    g.fa[i] = (float)ldexp(1.0, sa - 2 * sx);
-    g.fb2[i] = (float)ldexp(k[2], sb - 2 * sa);
-    g.fb1[i] = (float)ldexp(k[1], sb - sa);
-    g.fb0[i] = (float)ldexp(k[0], sb);
-    g.fx[i] = (float)ldexp(1.0, (i + 1 < d.steps ? sn : 0) - sb - sx);
-    bound = next;
-    sx = sn;
-  }
   int smem = 2 * (128 * g.slice * 2) + 2 * kFewPlane + 1024;
   if (smem < kFewLeast) smem = kFewLeast;
   if (!prepare_smem((const void*)orth_few_kernel, 2 * (128 * kFewSlice * 2) + 2 * kFewPlane + 1024)) return DCF_ECUDA;
@@ -1486,11 +1546,10 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
   if (few_ctas(d)) return launch_few(d, a, out, out_rs, out_bs, whole, st, s);
   int rc = launch(orth_norm_kernel, dim3((unsigned)l.parts, (unsigned)d.batch), kNormThreads, 0, 1, s, a, l.part);
   if (rc) return rc;
-  int sx = d.steps ? scale_of(1) : 0;
   const uint64_t groups = (d.cols + 7) / 8 * d.rows, blocks = (groups + kNormThreads - 1) / kNormThreads;
   const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096), (unsigned)d.batch);
-  rc = launch(orth_split_kernel, grid, kNormThreads, 0, 1, s, a,
-              (const double*)l.part, l.parts, d.eps, ldexp(1.0, sx), l.x[0], d.steps ? (void*)nullptr : out,
+  rc = launch(orth_split_kernel, grid, kNormThreads, 0, 1, s, a, scaling_of(d),
+              (const double*)l.part, l.parts, l.x[0], l.factors, d.steps ? (void*)nullptr : out,
               (int)d.out_dtype, out_rs, out_bs);
   if (rc) return rc;
   if (!d.steps) return DCF_OK;
@@ -1500,12 +1559,7 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
   if (!encode(&mx[0], l.x[0], cols, d.batch) || !encode(&ma, l.a, m, d.batch) || !encode(&mb, l.b, m, d.batch) ||
       (d.steps > 1 && !encode(&mx[1], l.x[1], cols, d.batch)))
     return DCF_ECUDA;
-  double bound = 1;
   for (uint32_t i = 0; i < d.steps; i++) {
-    const double* k = d.coef[i];
-    double next, q;
-    step_bounds(k, bound, &next, &q);
-    const int sa = scale_of(bound * bound), sb = scale_of(q), sn = scale_of(next);
     const CUtensorMap& x = mx[i & 1];
     GemmArgs g = {};
     g.st = st;
@@ -1513,14 +1567,12 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.part = l.sums;
     g.m = g.n = m;
     g.k = n;
-    g.alpha = (float)ldexp(1.0, sa - 2 * sx);
+    g.factors = l.factors + i;
+    g.steps = (int)d.steps;
     g.to = l.a;
     rc = tall ? gemm_symmetric<GRAM, true>(x, g, l.gram, d.batch, s) : gemm_symmetric<GRAM, false>(x, g, l.gram, d.batch, s);
     if (rc) return rc;
     g.k = m;
-    g.alpha = (float)ldexp(k[2], sb - 2 * sa);
-    g.beta = (float)ldexp(k[1], sb - sa);
-    g.diag = (float)ldexp(k[0], sb);
     g.from = l.a;
     g.to = l.b;
     g.sum = sums_of(d, m, true);
@@ -1529,11 +1581,9 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
     g.m = rows;
     g.n = cols;
     if (i + 1 < d.steps) {
-      g.alpha = (float)ldexp(1.0, sn - sb - sx);
       g.to = l.x[(i + 1) & 1];
       rc = tall ? gemm<APPLY, false, false>(x, mb, g, d.batch, s) : gemm<APPLY, false, true>(mb, x, g, d.batch, s);
     } else {
-      g.alpha = (float)ldexp(1.0, -sb - sx);
       g.out = out;
       g.out_dtype = (int)d.out_dtype;
       g.vectors = whole;
@@ -1542,8 +1592,6 @@ int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void
       rc = tall ? gemm<FINAL, false, false>(x, mb, g, d.batch, s) : gemm<FINAL, false, true>(mb, x, g, d.batch, s);
     }
     if (rc) return rc;
-    bound = next;
-    sx = sn;
   }
   return DCF_OK;
 }

@@ -121,3 +121,34 @@ def orth_tolerance(g: np.ndarray, coef, eps: float, seed: int = 0) -> float:
         size = (3 * 2.0 ** -22 + math.sqrt(p.shape[1]) * 2.0 ** -23) * (np.abs(p) @ np.abs(q))
         return rng.uniform(-1, 1, size.shape) * size
     return 4 * max(np.linalg.norm(newton_schulz(g, coef, eps, wobble) - want) / norm for _ in range(3))
+
+
+def orth_quantum(g: np.ndarray, coef, eps: float, seed: int = 0) -> float:
+    """Error (2-norm) that the planes' smallest step may leave.
+
+    X, A and B are kept at powers of two that bring a bound on their singular values
+    to 2^13; a plane's smallest step is 2^-24 there, so every element is off by up to
+    half of that, 2^(e - 38) with the bound below 2^e, however small it is.  The bounds start
+    from norm / (norm + eps) where that is below a half, else from 1, and follow
+    the step's polynomial.  Its effect is taken as in orth_tolerance: the iteration with every
+    element moved at random within that, the worst of three, times four."""
+    rng = np.random.default_rng(seed)
+    x0 = g.astype(np.float64)
+    x0 = x0.T if x0.shape[0] > x0.shape[1] else x0
+    norm = math.sqrt(float((x0 * x0).sum()))
+    share = norm / (norm + eps) if norm else 1.0
+    eye, want = np.eye(x0.shape[0]), newton_schulz(x0, coef, eps)
+
+    def moved(v, bound):
+        return v + rng.uniform(-1, 1, v.shape) * 2.0 ** (math.frexp(max(bound, 2.0 ** -120))[1] - 38)
+
+    def run():
+        x, s = x0 / (norm + eps), share if share < 0.5 else 1.0
+        for a, b, c in coef:
+            t = np.linspace(0, s, 10001) ** 2
+            x = moved(x, s)
+            gram = moved(x @ x.T, s * s)
+            x = moved(a * eye + b * gram + c * gram @ gram, float(np.abs(a + t * (b + t * c)).max())) @ x
+            s = float((np.sqrt(t) * np.abs(a + t * (b + t * c))).max())
+        return x
+    return 4 * max(np.linalg.norm(run() - want) for _ in range(3)) if norm else 0.0

@@ -695,3 +695,52 @@ def test_orth_zeros_stay_zeros_beside_the_smallest_eps(dcf, shape, steps):
     for eps in (1e-7, 1e-300, 1e-306, 5e-324):
         assert (run_orth(dcf, x, "f32", steps=steps, eps=eps) == 0).all(), eps
     assert run_orth(dcf, x, "f32", steps=steps, eps=0.0).isnan().all()      # 0 / 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(60, 90), (500, 100), (150, 170), (300, 131)])
+def test_orth_norms_far_below_eps(dcf, rows, cols, dtype):
+    """The norm's share of norm + eps scales the planes: nothing is lost to a
+    fixed scale.  One batch of very different matrices, the first and last of usual norm."""
+    norms = [1.0, 1e-9, 1e-12, 1e-15, 1e-30, 0.0, 5e-8, 1e-7, 3.0]
+    x = randn((len(norms), rows, cols), "f32", 95)
+    for k, norm in enumerate(norms):
+        x[k] *= norm / float(x[k].double().norm())
+    x = x.to(tdtype(dtype))
+    got = run_orth(dcf, x, dtype)
+    assert (got[5] == 0).all()
+    some = [k for k in range(len(norms)) if k != 5]
+    check_orth(got[some], x[some], dtype, [COEF] * 5)
+
+
+def check_orth_f32(got, x, coef, eps):
+    """One f32 matrix whose results may be far smaller than the planes' bounds (odd powers
+    alone shrink what is below one), or lie below f32's normal range: there they round to
+    half of 2^-149 (and below that to zero), so a 2-norm is off by 2^-150 for each; as much
+    again is allowed."""
+    got, x = values(got)[0], values(x)[0]
+    want = lo.newton_schulz(x, coef, eps)
+    tol = lo.orth_tolerance(x, coef, eps) + lo.U32
+    err = np.linalg.norm(got - want)
+    assert err <= tol * np.linalg.norm(want) + lo.orth_quantum(x, coef, eps) + 2.0 ** -149 * np.sqrt(want.size), \
+        (err, np.linalg.norm(want), tol)
+
+
+@pytest.mark.parametrize("rows,cols", [(60, 90), (150, 170)])
+@pytest.mark.parametrize("coef", [(3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (0.0, 1.0, 0.0), (1e-3, 0.5, 0.25),
+                                  (2.0, 0.0, -1.0)])
+def test_orth_small_norms_with_other_coefficients(dcf, rows, cols, coef):
+    """Odd powers alone (a = 0) make results far smaller than X; eps beyond 1."""
+    for norm, eps, steps in ((1e-3, 1e-1, 2), (1e-5, 2.0, 3), (1e-2, 1e-2, 2)):
+        x = randn((1, rows, cols), "f32", 96)
+        x *= norm / float(x.double().norm())
+        check_orth_f32(run_orth(dcf, x, "f32", steps=steps, coef=coef, eps=eps), x, [coef] * steps, eps)
+
+
+@pytest.mark.parametrize("shape", [(1, 60, 90), (1, 150, 170)])
+def test_orth_results_at_the_end_of_f32(dcf, shape):
+    """norm / (norm + eps) of 2^-133, and a value that no f32 has."""
+    x = randn(shape, "f32", 97)
+    x *= 1e-30 / float(x.double().norm())
+    for eps in (1e10, 1e300):
+        check_orth_f32(run_orth(dcf, x, "f32", eps=eps), x, [COEF] * 5, eps)
