@@ -1231,7 +1231,9 @@ int round64(uint64_t v) { return (int)((v + 63) / 64 * 64); }
 
 // Bounds of one step on [0, s]: the largest |a s + b s^3 + c s^5| and
 // |a + b s^2 + c s^4|, from the ends and the points where the derivative is
-// zero.
+// zero, in t = s^2.  (The roots of a + 3 b t + 5 c t^2 in the form without
+// cancellation: a c that is nearly 0 puts one far away and leaves the other at
+// -a / 3 b.  A coefficient of 0 gives infinities or NaN, which lie outside.)
 void step_bounds(const double* k, double s, double* x, double* q) {
   const double a = k[0], b = k[1], c = k[2], t1 = s * s;
   auto at = [&](double t) {
@@ -1243,16 +1245,12 @@ void step_bounds(const double* k, double s, double* x, double* q) {
   *x = *q = 0;
   at(0);
   at(t1);
-  if (c != 0) at(-b / (2 * c));
-  // a + 3 b t + 5 c t^2 = 0
-  if (c == 0) {
-    if (b != 0) at(-a / (3 * b));
-  } else {
-    const double d = 9 * b * b - 20 * a * c;
-    if (d >= 0) {
-      at((-3 * b + sqrt(d)) / (10 * c));
-      at((-3 * b - sqrt(d)) / (10 * c));
-    }
+  at(-b / (2 * c));
+  const double d = 9 * b * b - 20 * a * c;
+  if (d >= 0) {
+    const double w = -(3 * b + copysign(sqrt(d), b)) / 2;
+    at(w / (5 * c));
+    at(a / w);
   }
 }
 

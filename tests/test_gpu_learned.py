@@ -744,3 +744,14 @@ def test_orth_results_at_the_end_of_f32(dcf, shape):
     x *= 1e-30 / float(x.double().norm())
     for eps in (1e10, 1e300):
         check_orth_f32(run_orth(dcf, x, "f32", eps=eps), x, [COEF] * 5, eps)
+
+
+@pytest.mark.parametrize("rows,cols", [(2, 2), (150, 170), (170, 150)])
+@pytest.mark.parametrize("c", [0.0, 5.5e-17, -5.5e-17])
+def test_orth_largest_value_inside_the_interval(dcf, rows, cols, c):
+    """2.6 s - 2.5 s^3 is 0.1 at 1 and 1.02 at 0.589: planes scaled for the first overflow."""
+    import torch
+    x = torch.zeros(1, rows, cols, device="cuda")
+    x[0, 0, 0], x[0, 1, 1] = 0.589, 0.808
+    coef = [(2.6, -2.5, c)] * 2
+    check_orth(run_orth(dcf, x, "f32", steps=2, coef=coef), x, "f32", coef)

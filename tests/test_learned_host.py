@@ -184,3 +184,34 @@ def test_oracle_starts_and_buckets_agree(num_buckets, max_distance, both):
     reach = max_distance + 30
     ids = lo.buckets([reach], 2 * reach + 1, num_buckets, max_distance, both)[0]
     assert list(ids) == [lo.bucket(d, num_buckets, max_distance, both) for d in range(-reach, reach + 1)]
+
+
+@pytest.mark.parametrize("c", [1e-17, -1e-17, 5.5e-17, 1e-300, -1e-300, 5e-324])
+def test_orth_bound_with_a_leftover_in_the_last_coefficient(c):
+    """What cancellation leaves of a zero changes no bound: the largest value inside the interval is found."""
+    assert "past 64" in refused(m.orthogonalize_plan, "f32", 8, 8, steps=4, coef=(4, -4, c))
+    m.orthogonalize_plan("f32", 8, 8, steps=2, coef=(4, -4, c))
+    m.orthogonalize_plan("f32", 8, 8, steps=2, coef=(3, -3, c))
+    m.orthogonalize_plan("f32", 8, 8, steps=5, coef=(1.5, -0.5, c))
+    m.orthogonalize_plan("f32", 8, 8, steps=2, coef=(c, 1, 1))
+    m.orthogonalize_plan("f32", 8, 8, steps=2, coef=(1, c, 1))
+
+
+def test_orth_bounds_against_a_fine_grid():
+    """Accepted or refused as the polynomial's values on a grid say, for coefficients of any sign."""
+    rng = np.random.default_rng(7)
+    for _ in range(400):
+        coef = [rng.choice([0.0, 1e-17, 1.0]) * rng.uniform(-8, 8) for _ in range(3)]
+        s, least = 1.0, math.inf
+        for _ in range(3):
+            t = np.linspace(0, s, 4001) ** 2
+            f = np.abs(coef[0] + t * (coef[1] + t * coef[2]))
+            least, s = min(least, f.max(), (np.sqrt(t) * f).max()), (np.sqrt(t) * f).max()
+            if s > 64:
+                break
+        if abs(s - 64) < 1 or 1e-40 < least < 1e-20:      # too near a border for a grid
+            continue
+        if s > 64 or least < 1e-30:
+            refused(m.orthogonalize_plan, "f32", 8, 8, steps=3, coef=coef)
+        else:
+            m.orthogonalize_plan("f32", 8, 8, steps=3, coef=coef)
