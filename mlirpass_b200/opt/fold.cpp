@@ -3,6 +3,9 @@
 #include "fold.h"
 
 #include <algorithm>
+#include <cctype>
+#include <charconv>
+#include <cstdlib>
 #include <cstring>
 #include <stdexcept>
 #include <thread>
@@ -901,10 +904,70 @@ int64_t whole_prop(const Op* op, const char* key, int64_t fallback, bool* ok) {
   return v;
 }
 
-bool parse_number(const std::string& text, double* v) {
-  char* end = nullptr;
-  *v = strtod(text.c_str(), &end);
-  return end != text.c_str();
+std::string trimmed(const std::string& s) {
+  const size_t a = s.find_first_not_of(" \t\r\n"), b = s.find_last_not_of(" \t\r\n");
+  return a == std::string::npos ? "" : s.substr(a, b - a + 1);
+}
+
+// The literal and the type of "literal : type" (the type empty where it has none).
+void split_type(const std::string& text, std::string* literal, std::string* type) {
+  const size_t colon = text.find(':');
+  *literal = trimmed(text.substr(0, colon));
+  *type = colon == std::string::npos ? "" : trimmed(text.substr(colon + 1));
+}
+
+// A float literal as MLIR writes it: decimal, or, with a type of `bits` bits (32 or
+// 64), 0x and the value's bits.  Nothing may follow it.
+bool parse_number(const std::string& text, int bits, double* v) {
+  if (bits && text.size() > 2 && text[0] == '0' && text[1] == 'x') {
+    if (text.size() > 2 + (size_t)bits / 4 || text.find_first_not_of("0123456789abcdefABCDEF", 2) != std::string::npos)
+      return false;
+    const uint64_t b = strtoull(text.c_str(), nullptr, 16);
+    if (bits == 64) {
+      memcpy(v, &b, 8);
+    } else {
+      float f;
+      const uint32_t w = (uint32_t)b;
+      memcpy(&f, &w, 4);
+      *v = f;
+    }
+    return true;
+  }
+  const size_t first = !text.empty() && text[0] == '-';
+  if (first >= text.size() || !isdigit((unsigned char)text[first]) ||
+      text.find_first_not_of("0123456789.eE+-", first) != std::string::npos)
+    return false;
+  const auto r = std::from_chars(text.data(), text.data() + text.size(), *v);
+  return r.ec == std::errc() && r.ptr == text.data() + text.size();
+}
+
+// A float property: f64, f32 (then its value is a f32) or a whole number.
+bool number_prop(const std::string& text, double* v) {
+  std::string literal, type;
+  split_type(text, &literal, &type);
+  const bool plain = literal.find_first_not_of("0123456789") == std::string::npos;
+  if (type == "f32") {
+    if (!parse_number(literal, 32, v)) return false;
+    *v = (float)*v;
+    return true;
+  }
+  if (type == "f64") return parse_number(literal, 64, v);
+  return (type.empty() || (plain && type == "i64")) && parse_number(literal, 0, v);
+}
+
+// array<f64: a, b, ...>
+bool number_list(const std::string& text, std::vector<double>* out) {
+  const std::string t = trimmed(text), head = "array<f64:";
+  if (t.size() <= head.size() || t.compare(0, head.size(), head) || t.back() != '>') return false;
+  for (size_t at = head.size(); at < t.size();) {
+    size_t end = t.find(',', at);
+    if (end == std::string::npos) end = t.size() - 1;
+    double v;
+    if (!parse_number(trimmed(t.substr(at, end - at)), 64, &v)) return false;
+    out->push_back(v);
+    at = end + 1;
+  }
+  return true;
 }
 
 // The operand of a pattern as a constant with all of its values stored.
@@ -1004,20 +1067,11 @@ Plan learned_pattern(Op* op, Engine& eng) {
     d.cols = (uint64_t)in[o + 1];
     d.eps = 1e-7;
     if (const std::string* e = op->prop("eps"))
-      if (!parse_number(*e, &d.eps)) return Plan::failed();
+      if (!number_prop(*e, &d.eps)) return Plan::failed();
     std::vector<double> coef = {3.4445, -4.7750, 2.0315};
     if (const std::string* c = op->prop("coef")) {
       coef.clear();
-      const size_t from = c->find(':');
-      if (from == std::string::npos) return Plan::failed();
-      for (size_t at = from + 1; at < c->size();) {
-        double v;
-        if (!parse_number(c->substr(at), &v)) return Plan::failed();
-        coef.push_back(v);
-        at = c->find(',', at);
-        if (at == std::string::npos) break;
-        at++;
-      }
+      if (!number_list(*c, &coef)) return Plan::failed();
     }
     if (coef.size() != 3 && coef.size() != 3 * (size_t)steps) return Plan::failed();
     for (int64_t i = 0; i < steps; i++)

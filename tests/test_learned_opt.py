@@ -123,3 +123,60 @@ def test_orthogonalize_folds(shape, props, coef, steps):
         want = lo.newton_schulz(m, [coef] * steps, eps)
         tol = lo.orth_tolerance(m, [coef] * steps, eps) + lo.U32
         assert np.linalg.norm(got[k] - want) <= tol * np.linalg.norm(want)
+
+
+def taken(props: str, op: str = "dcf.orthogonalize", out_ty: str = "tensor<32x3xf32>") -> bool:
+    """Whether the pass takes the op for folding (which fails here for want of a GPU) or leaves it."""
+    try:
+        d, _ = result(module("tensor<32x3xf32>", hexed(TABLE), op, props, out_ty), n_gpus=0)
+    except Exception as e:
+        assert "needs a GPU" in str(e)
+        return True
+    assert d.name == op
+    return False
+
+
+def f64_bits(v: float) -> str:
+    return f"0x{np.float64(v).view(np.uint64):016X}"
+
+
+@pytest.mark.parametrize("eps,is_eps", [
+    ("1.0e-7 : f64", True), ("1.0e-7", True), ("1.000000e-03 : f32", True), ("0.0 : f64", True), ("12.5E+1 : f64", True),
+    (f64_bits(1e-7) + " : f64", True), ("0x33D6BF95 : f32", True), (f64_bits(0.0) + " : f64", True), ("1 : i64", True),
+    (f64_bits(-1.0) + " : f64", False), (f64_bits(np.nan) + " : f64", False), (f64_bits(np.inf) + " : f64", False),
+    ("0xBF800000 : f32", False), (f64_bits(1e-7) + " : f32", False), ("0x7FC00000 : f32", False),
+    (f64_bits(1e-7), False), ("0x10 : i64", False), ("-0x1 : f64", False), ("0x : f64", False),
+    ("1e-3junk : f64", False), ("1.0e-3 junk", False), ("nan", False), ("inf : f64", False), ("1.0e-7 : f16", False),
+    ("1.0e-7 : tensor<f64>", False), ("0x1p-3 : f64", False), ("1.0e999 : f64", False), ("", False), ("-1.0 : f64", False),
+    ('"1.0"', False), (".5 : f64", False), ("1.0e : f64", False), ("--1.0 : f64", False)])
+def test_spellings_of_eps(eps, is_eps):
+    assert taken(f" <{{eps = {eps}}}>") == is_eps
+
+
+@pytest.mark.parametrize("coef,is_coef", [
+    ("array<f64: 1.5, -0.5, 0.0>", True), ("array<f64: 1.5,-5.0e-1,0.0>", True), ("array<f64: 1, 0, 0>", True),
+    (f"array<f64: {f64_bits(1.5)}, {f64_bits(-0.5)}, {f64_bits(0.0)}>", True),
+    ("array<f32: 1.5, -0.5, 0.0>", False), ("array<i64: 1, 0, 0>", False), ("array<f64: 1.5 junk, -0.5, 0.0>", False),
+    ("array<f64: 1.5, -0.5, 0.0> junk", False), ("array<f64: 1.5, -0.5, 0.0,>", False),
+    ("array<f64: , -0.5, 0.0>", False), ("array<f64>", False), ("dense<[1.5, -0.5, 0.0]> : tensor<3xf64>", False),
+    (f"array<f64: {f64_bits(np.nan)}, -0.5, 0.0>", False), ("array<f64: 0x3FF80000000000000, -0.5, 0.0>", False)])
+def test_spellings_of_coefficients(coef, is_coef):
+    assert taken(f" <{{coef = {coef}}}>") == is_coef
+
+
+def test_an_open_list_is_a_parse_error():
+    with pytest.raises(opt.OptError, match="parse error"):
+        result(module("tensor<32x3xf32>", hexed(TABLE), "dcf.orthogonalize", " <{coef = array<f64: 1.5, -0.5, 0.0}>",
+                      "tensor<32x3xf32>"), n_gpus=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps,same", [(f64_bits(1e-3) + " : f64", 1e-3), ("0x3A83126F : f32", float(np.float32(1e-3))),
+                                      ("1.0e-3 : f32", float(np.float32(1e-3)))])
+def test_eps_in_bits_means_its_value(eps, same):
+    ty = "tensor<8x8xf32>"
+    x = (np.random.default_rng(3).standard_normal((8, 8)) * 1e-3).astype(np.float32)
+    a, _ = result(module(ty, hexed(x), "dcf.orthogonalize", f" <{{steps = 0 : i64, eps = {eps}}}>", ty))
+    got = np.array(a.const.bits, np.uint32).view(np.float32).reshape(8, 8)
+    want = x.astype(np.float64) / (np.sqrt((x.astype(np.float64) ** 2).sum()) + same)
+    assert (np.abs(got - want) <= 2 * lo.U32 * np.abs(want)).all()
