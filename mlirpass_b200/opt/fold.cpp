@@ -887,23 +887,6 @@ Plan layerwise_pattern(Module&, Op* op, Engine& eng) {
 // and so does one whose operand or result is over 16 GiB: a module could not
 // hold it as a constant.
 
-bool bool_prop(const Op* op, const char* key, bool fallback, bool* ok) {
-  const std::string* p = op->prop(key);
-  if (!p) return fallback;
-  const std::string t = p->substr(0, p->find(' '));
-  if (t != "true" && t != "false") *ok = false;
-  return t == "true";
-}
-
-int64_t whole_prop(const Op* op, const char* key, int64_t fallback, bool* ok) {
-  const std::string* p = op->prop(key);
-  if (!p) return fallback;
-  bool read = false;
-  const int64_t v = parse_int_prop(*p, &read);
-  if (!read) *ok = false;
-  return v;
-}
-
 std::string trimmed(const std::string& s) {
   const size_t a = s.find_first_not_of(" \t\r\n"), b = s.find_last_not_of(" \t\r\n");
   return a == std::string::npos ? "" : s.substr(a, b - a + 1);
@@ -914,6 +897,49 @@ void split_type(const std::string& text, std::string* literal, std::string* type
   const size_t colon = text.find(':');
   *literal = trimmed(text.substr(0, colon));
   *type = colon == std::string::npos ? "" : trimmed(text.substr(colon + 1));
+}
+
+bool bool_prop(const Op* op, const char* key, bool fallback, bool* ok) {
+  const std::string* p = op->prop(key);
+  if (!p) return fallback;
+  const std::string t = trimmed(*p);
+  if (t != "true" && t != "false") *ok = false;
+  return t == "true";
+}
+
+// An integer property: decimal, or 0x and the bits of a value of its type (i64 where
+// it has none); iN, siN, uiN or index, of at most 64 bits, and within the type's range.
+int64_t whole_prop(const Op* op, const char* key, int64_t fallback, bool* ok) {
+  const std::string* p = op->prop(key);
+  if (!p) return fallback;
+  std::string literal, type;
+  split_type(*p, &literal, &type);
+  auto wrong = [&]() -> int64_t {
+    *ok = false;
+    return fallback;
+  };
+  auto digits = [](const std::string& s, size_t from, int base, uint64_t* v) {
+    const char* end = s.data() + s.size();
+    const auto r = std::from_chars(s.data() + from, end, *v, base);
+    return from < s.size() && r.ec == std::errc() && r.ptr == end;
+  };
+  uint64_t bits = 64, v = 0;
+  const bool unsigned_type = !type.empty() && type[0] == 'u';
+  if (!type.empty() && type != "index") {
+    const size_t i = type[0] == 's' || type[0] == 'u';
+    if (type[i] != 'i' || !digits(type, i + 1, 10, &bits) || bits < 1 || bits > 64) return wrong();
+  }
+  const uint64_t most = ~0ull >> (64 - bits);
+  if (literal.size() > 2 && literal[0] == '0' && literal[1] == 'x') {
+    if (!digits(literal, 2, 16, &v) || v > most) return wrong();
+    if (!unsigned_type && (v >> (bits - 1) & 1)) v |= ~most;
+    return unsigned_type && v > INT64_MAX ? wrong() : (int64_t)v;
+  }
+  const bool negative = !literal.empty() && literal[0] == '-';
+  if (!digits(literal, negative, 10, &v)) return wrong();
+  const uint64_t limit = unsigned_type ? std::min<uint64_t>(most, INT64_MAX) : (most >> 1) + negative;
+  if (v > limit || (negative && unsigned_type)) return wrong();
+  return negative ? (int64_t)(0 - v) : (int64_t)v;
 }
 
 // A float literal as MLIR writes it: decimal, or, with a type of `bits` bits (32 or

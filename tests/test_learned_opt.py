@@ -180,3 +180,29 @@ def test_eps_in_bits_means_its_value(eps, same):
     got = np.array(a.const.bits, np.uint32).view(np.float32).reshape(8, 8)
     want = x.astype(np.float64) / (np.sqrt((x.astype(np.float64) ** 2).sum()) + same)
     assert (np.abs(got - want) <= 2 * lo.U32 * np.abs(want)).all()
+
+
+@pytest.mark.parametrize("value,is_steps", [
+    ("3 : i64", True), ("3", True), ("0x3 : i64", True), ("3 : i32", True), ("3 : index", True), ("+3 : i64", False),
+    ("3.7 : i64", False), ("3.0 : f64", False), ("3junk : i64", False), ("3 junk", False), ("-1 : i64", False),
+    ("0x11 : i64", False), ("0xFFFFFFFFFFFFFFFD : i64", False), ("99999999999999999999 : i64", False), ("300 : i8", False),
+    ("0x : i64", False), ("", False), ("true", False), ("3 : tensor<i64>", False), ("3 : i0", False), ("3 : i65", False),
+    ("array<i64: 3>", False)])
+def test_spellings_of_whole_numbers(value, is_steps):
+    assert taken(f" <{{steps = {value}}}>") == is_steps
+
+
+@pytest.mark.parametrize("value,is_flag", [("true", True), ("false", True), ("true junk", False), ("truejunk", False),
+                                           ("1 : i1", False), ("unit", False), ("", False), ("false : i64", False)])
+def test_spellings_of_flags(value, is_flag):
+    assert taken(f" <{{causal = {value}}}>", "dcf.position_bias", "tensor<3x5x6xf32>") == is_flag
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first,value", [("0x10 : i64", 16), ("0xFFFFFFFFFFFFFFFE : i64", -2), ("0xFE : i8", -2),
+                                         ("-3 : i32", -3), ("250 : ui8", 250), ("0xFE : ui8", 254)])
+def test_whole_numbers_mean_their_value(first, value):
+    d, _ = result(module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", f" <{{first_query = {first}}}>",
+                         "tensor<3x5x20xf32>"))
+    want = TABLE.T[:, lo.buckets(lo.positions(5, value), 20, 32, 128, True)]
+    assert np.array_equal(np.array(d.const.bits, np.uint32).reshape(want.shape), want.view(np.uint32))
