@@ -19,8 +19,9 @@
  *   "dcf.orthogonalize"(%w)         tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
  *     properties steps (5), eps (1e-7), coef (array<f64: a, b, c>, or three
  *     for each step)
- * An op whose types or properties its operator does not take is left as it
- * is.  Only folds run: the reference's canonicalization rewrite patterns
+ * An op whose types or properties its operator does not take, or that has
+ * any other property or attribute (those of other dialects aside), is left as
+ * it is.  Only folds run: the reference's canonicalization rewrite patterns
  * are not restated.
  */
 #ifndef DCFOLD_OPT_H

@@ -883,9 +883,9 @@ Plan layerwise_pattern(Module&, Op* op, Engine& eng) {
 //       bidirectional, causal : bool, first_query, max_distance : i64
 //   "dcf.orthogonalize"(%w)          tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
 //       steps : i64, eps : f64, coef : array<f64: a, b, c> (or 3 per step)
-// An op whose types or properties the operator does not take stays as it is,
-// and so does one whose operand or result is over 16 GiB: a module could not
-// hold it as a constant.
+// An op whose types or properties the operator does not take, or that says more than
+// these properties (attributes of other dialects aside), stays as it is, and so does
+// one whose operand or result is over 16 GiB: a module could not hold it as a constant.
 
 std::string trimmed(const std::string& s) {
   const size_t a = s.find_first_not_of(" \t\r\n"), b = s.find_last_not_of(" \t\r\n");
@@ -996,6 +996,47 @@ bool number_list(const std::string& text, std::vector<double>* out) {
   return true;
 }
 
+// Whether every attribute of "{...}" belongs to a dialect ("some.mark"): one without a
+// dialect is an older spelling of a property.
+bool only_marks(const std::string& attrs) {
+  if (attrs.size() < 2) return attrs.empty();
+  size_t from = 1;
+  int depth = 0;
+  for (size_t i = 1; i < attrs.size(); i++) {
+    const char c = attrs[i];
+    if (c == '"') {
+      while (++i < attrs.size() && attrs[i] != '"')
+        if (attrs[i] == '\\') i++;
+      continue;
+    }
+    const bool end = i + 1 == attrs.size();
+    if ((c == ',' && depth == 0) || end) {
+      const std::string entry = attrs.substr(from, i - from), key = trimmed(entry.substr(0, entry.find('=')));
+      if (key.empty() ? !end : key.find('.') == std::string::npos) return false;
+      from = i + 1;
+    } else if (c == '-' && i + 1 < attrs.size() && attrs[i + 1] == '>') {
+      i++;
+    } else if (c == '<' || c == '(' || c == '[' || c == '{') {
+      depth++;
+    } else if (c == '>' || c == ')' || c == ']' || c == '}') {
+      depth--;
+    }
+  }
+  return true;
+}
+
+// Whether an op says nothing but these properties, each once.
+bool says_only(const Op* op, std::initializer_list<const char*> known) {
+  if (!op->regions.empty() || !op->successors.empty() || !only_marks(op->attrs)) return false;
+  for (size_t i = 0; i < op->props.size(); i++) {
+    const std::string& key = op->props[i].first;
+    if (std::find(known.begin(), known.end(), key) == known.end()) return false;
+    for (size_t j = 0; j < i; j++)
+      if (op->props[j].first == key) return false;
+  }
+  return true;
+}
+
 // The operand of a pattern as a constant with all of its values stored.
 DenseP whole_constant(const DenseP& k, Engine& eng) {
   if (!k->splat) return k;
@@ -1012,7 +1053,7 @@ DenseP whole_constant(const DenseP& k, Engine& eng) {
 }
 
 bool bias_properties(const Op* op, dcf_bias_desc* d) {
-  bool ok = true;
+  bool ok = says_only(op, {"bidirectional", "causal", "first_query", "max_distance"});
   if (bool_prop(op, "bidirectional", true, &ok)) d->flags |= DCF_BIAS_BIDIRECTIONAL;
   if (bool_prop(op, "causal", false, &ok)) d->flags |= DCF_BIAS_CAUSAL;
   d->first_query = whole_prop(op, "first_query", 0, &ok);
@@ -1081,7 +1122,7 @@ Plan learned_pattern(Op* op, Engine& eng) {
   } else if (op->name == "dcf.orthogonalize") {
     const size_t o = in.size() == 3 ? 1 : 0;
     if (in.size() != 2 + o || in != out) return Plan::failed();
-    bool ok = true;
+    bool ok = says_only(op, {"steps", "eps", "coef"});
     const int64_t steps = whole_prop(op, "steps", 5, &ok);
     if (!ok || steps < 0 || steps > DCF_ORTH_MAX_STEPS) return Plan::failed();
     dcf_orth_desc& d = q->orth;

@@ -206,3 +206,35 @@ def test_whole_numbers_mean_their_value(first, value):
                          "tensor<3x5x20xf32>"))
     want = TABLE.T[:, lo.buckets(lo.positions(5, value), 20, 32, 128, True)]
     assert np.array_equal(np.array(d.const.bits, np.uint32).reshape(want.shape), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("op,out_ty,props", [
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " <{casual = true}>"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " <{num_buckets = 64 : i64}>"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " <{causal}>"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " <{steps = 3 : i64}>"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " <{causal = true, causal = false}>"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " {causal = true}"),                  # not as a property
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " {some.mark = 1 : i64, causal = true}"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", ' {some.mark = "a, b", "causal" = true}'),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " {max_distance = 64 : i64}"),
+    ("dcf.position_bias", "tensor<3x5x6xf32>", " {unit}"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{step = 3 : i64}>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " <{steps = 3 : i64, causal = false}>"),
+    ("dcf.orthogonalize", "tensor<32x3xf32>", " {eps = 1.0e-3 : f64}"),
+])
+def test_properties_that_the_op_does_not_know(op, out_ty, props):
+    assert not taken(props, op, out_ty)
+
+
+@pytest.mark.parametrize("props", ["", " <{}>", " {}", " {some.mark = 1 : i64}", ' {some.mark = "causal = x, y", other.mark}',
+                                   " <{causal = true, first_query = 1 : i64, max_distance = 64 : i64, bidirectional = false}>",
+                                   ' <{causal = true}> {some.mark = {a = 1 : i64, b = [1, 2]}, "other.mark" = 2 : i64}'])
+def test_properties_and_marks_of_other_dialects_that_fold(props):
+    assert taken(props, "dcf.position_bias", "tensor<3x5x6xf32>")
+
+
+def test_an_op_with_a_region_stays():
+    out, stats = opt.run(module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", " ({\n    })", "tensor<3x5x6xf32>"),
+                         PIPELINE, n_gpus=0)
+    assert '"dcf.position_bias"' in out and stats["folds"] == 0
