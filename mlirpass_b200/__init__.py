@@ -14,6 +14,7 @@ CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from dataclasses import dataclass
 
@@ -494,6 +495,8 @@ class BiasPlan:
         self.out_elements = span                     # elements from a bias's first to its last
         self.grad_elements = span + (d.batch - 1) * batch if some and d.batch else 0
         self.entries = d.num_buckets * d.heads
+        self.out_layout = (d.heads, d.queries, d.keys), (head, row, 1)
+        self.grad_layout = (d.batch, d.heads, d.queries, d.keys), (batch, head, row, 1)
         ws = ctypes.c_size_t(0)
         _check(lib().dcf_position_bias_grad_workspace(self.ref, ctypes.byref(ws)))
         self.workspace = ws.value
@@ -596,11 +599,53 @@ def _room(t) -> int:
 
 
 def _need(t, what: str, elements: int, size: int) -> int:
-    """The tensor's pointer, once `elements` of `size` bytes are known to lie behind it."""
+    """The pointer of a dense tensor of at least `elements` of `size` bytes."""
     if t.element_size() != size:
         raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
-    if not (t.is_contiguous() and t.numel() >= elements) and _room(t) < elements:
-        raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
+    if elements and (not t.is_contiguous() or t.numel() < elements):
+        raise ValueError(f"{what}: {elements} contiguous elements expected, not {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr()
+
+
+def _memory(shape, strides) -> list:
+    """The (stride, size) pairs of a layout, the longest stride first, dims that join joined."""
+    dims = []
+    for stride, size in sorted(((t, n) for n, t in zip(shape, strides) if n > 1), reverse=True):
+        if dims and dims[-1][0] == stride * size:
+            dims[-1] = (stride, dims[-1][1] * size)
+        else:
+            dims.append((stride, size))
+    return dims
+
+
+def _lies_as(t, shape, strides) -> bool:
+    """Whether a tensor without all of a layout's elements in a row has them where the layout says:
+    it is the layout (or wider along some of its dims), or the same memory in another
+    order or number of dims, or a plain row that starts at its first element."""
+    have, at = list(t.shape), list(t.stride())
+    while len(have) > len(shape) and have[0] == 1:
+        have, at = have[1:], at[1:]
+    count = math.prod(shape)
+    if len(have) <= 1 and t.is_contiguous():
+        return t.numel() != count
+    rest = len(shape) - len(have)
+    if rest >= 0 and all(n == 1 for n in shape[:rest]):
+        if all(n <= 1 or (h >= n and a == s) for h, a, n, s in zip(have, at, shape[rest:], strides[rest:])):
+            return True
+        if tuple(have) == tuple(shape[rest:]):
+            return False
+    return _memory(have, at) == _memory(shape, strides)
+
+
+def _need_layout(t, what: str, elements: int, size: int, shape, strides) -> int:
+    """The pointer of a tensor in which the plan's layout, `elements` from its first to its last, lies."""
+    if t.element_size() != size:
+        raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
+    if elements and not (t.is_contiguous() and t.numel() >= elements):
+        if _room(t) < elements:
+            raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
+        if not _lies_as(t, shape, strides):
+            raise ValueError(f"{what}: {tuple(t.shape)} with strides {t.stride()}, the plan says {shape} with {strides}")
     return t.data_ptr()
 
 
@@ -619,12 +664,13 @@ def _bytes(workspace) -> int:
 
 
 def position_bias_async(plan: BiasPlan, table, out, *, positions=None, stream=None) -> None:
-    """Launch a position bias on device tensors.  `out` starts at the bias's
-    first element; the plan's strides say where the rest lies."""
+    """Launch a position bias on device tensors.  `table` and `positions` are dense;
+    `out` starts at the bias's first element and lies as the plan's strides say
+    (a tensor of the bias's shape with these strides, or the memory around it)."""
     _check(lib().dcf_position_bias_async(
         plan.ref, _need(table, "table", plan.entries, DTYPE_SIZE[plan.table_dtype]),
         _positions(positions, plan.desc.queries),
-        _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.dtype]), _own_stream(stream, out)))
+        _need_layout(out, "out", plan.out_elements, DTYPE_SIZE[plan.dtype], *plan.out_layout), _own_stream(stream, out)))
 
 
 def position_bias_grad_workspace(plan: BiasPlan) -> int:
@@ -633,11 +679,11 @@ def position_bias_grad_workspace(plan: BiasPlan) -> int:
 
 
 def position_bias_grad_async(plan: BiasPlan, grad, out, workspace, *, positions=None, stream=None) -> None:
-    """Launch the table gradient on device tensors: `out` is the dense
-    [num_buckets, heads] gradient, `workspace` uint8 (may be empty when
-    position_bias_grad_workspace says 0)."""
+    """Launch the table gradient on device tensors: `grad` lies as the plan's
+    strides say, `out` is the dense [num_buckets, heads] gradient, `workspace`
+    uint8 (may be empty when position_bias_grad_workspace says 0)."""
     _check(lib().dcf_position_bias_grad_async(
-        plan.ref, _need(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype]),
+        plan.ref, _need_layout(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype], *plan.grad_layout),
         _positions(positions, plan.desc.queries),
         _need(out, "out", plan.entries, 8 if plan.dtype == "f64" else 4), workspace.data_ptr(),
         _bytes(workspace), _own_stream(stream, out)))
@@ -657,6 +703,11 @@ class OrthPlan:
                 return 0
             row = row or d.cols
             return (d.rows - 1) * row + d.cols + (d.batch - 1) * (batch or d.rows * row)
+
+        def layout(row, batch):
+            row = row or d.cols
+            return (d.batch, d.rows, d.cols), (batch or d.rows * row, row, 1)
+        self.in_layout, self.out_layout = layout(d.row_stride, d.batch_stride), layout(d.out_row_stride, d.out_batch_stride)
         self.in_elements = span(d.row_stride, d.batch_stride)
         self.out_elements = span(d.out_row_stride, d.out_batch_stride)
         ws = ctypes.c_size_t(0)
@@ -709,9 +760,10 @@ def orthogonalize_workspace(plan: OrthPlan) -> int:
 
 
 def orthogonalize_async(plan: OrthPlan, x, out, workspace, status, *, stream=None) -> None:
-    """Launch an orthogonalisation on device tensors; `out` may be `x`.
+    """Launch an orthogonalisation on device tensors, which lie as the plan's strides
+    say; `out` may be `x`.
     `status` (16 bytes, reset first) takes a kernel's error report."""
     _check(lib().dcf_orthogonalize_async(
-        plan.ref, _need(x, "x", plan.in_elements, DTYPE_SIZE[plan.dtype]),
-        _need(out, "out", plan.out_elements, DTYPE_SIZE[plan.out_dtype]), workspace.data_ptr(),
+        plan.ref, _need_layout(x, "x", plan.in_elements, DTYPE_SIZE[plan.dtype], *plan.in_layout),
+        _need_layout(out, "out", plan.out_elements, DTYPE_SIZE[plan.out_dtype], *plan.out_layout), workspace.data_ptr(),
         _bytes(workspace), _need(status, "status", 2, 8), _own_stream(stream, out)))

@@ -215,3 +215,77 @@ def test_orth_bounds_against_a_fine_grid():
             refused(m.orthogonalize_plan, "f32", 8, 8, steps=3, coef=coef)
         else:
             m.orthogonalize_plan("f32", 8, 8, steps=3, coef=coef)
+
+
+def device_call(call, *args, **kw):
+    """A device form on CPU tensors: what the binding lets pass is refused by the library (host memory, or no GPU)."""
+    with pytest.raises((ValueError, m.DcfError)) as e:
+        call(*args, stream=0, **kw)
+    return "binding" if isinstance(e.value, ValueError) else "library"
+
+
+def test_tensors_without_strides_in_the_plan_are_contiguous():
+    import torch
+    plan = m.position_bias_plan("f32", 4, 10, 16)
+    table, out = torch.zeros(32, 4), torch.zeros(4, 10, 16)
+    grad, work = torch.zeros(1, 4, 10, 16), torch.zeros(m.position_bias_grad_workspace(plan) + 8, dtype=torch.uint8)
+    ids = torch.zeros(10, 2, dtype=torch.int32)
+    assert device_call(m.position_bias_async, plan, table, out) == "library"
+    assert device_call(m.position_bias_async, plan, torch.zeros(128), out) == "library"
+    assert device_call(m.position_bias_async, plan, torch.zeros(40, 4)[2:], out) == "library"
+    for t in (torch.zeros(4, 32).T, torch.zeros(32, 8)[:, :4], torch.zeros(64, 4)[::2], torch.zeros(1, 4).expand(32, 4),
+              torch.zeros(31, 4), torch.zeros(40, 4)[:31]):
+        assert device_call(m.position_bias_async, plan, t, out) == "binding"
+        assert device_call(m.position_bias_grad_async, plan, grad, t, work) == "binding"
+    assert device_call(m.position_bias_async, plan, table, out, positions=ids[:, 0].contiguous()) == "library"
+    for p in (ids[:, 0], ids[::2, :1], ids[:9, 0].contiguous(), torch.zeros(1, dtype=torch.int32).expand(10)):
+        assert device_call(m.position_bias_async, plan, table, out, positions=p) == "binding"
+        assert device_call(m.position_bias_grad_async, plan, grad, table, work, positions=p) == "binding"
+    orth, x = m.orthogonalize_plan("f32", 4, 4), torch.zeros(4, 4)
+    none = torch.zeros(0, dtype=torch.uint8)
+    status = torch.zeros(2, 2, dtype=torch.int64)
+    assert device_call(m.orthogonalize_async, orth, x, x, none, status[1]) == "library"
+    assert device_call(m.orthogonalize_async, orth, x, x, none, status[:, 0]) == "binding"
+
+
+def test_tensors_lie_as_the_plan_says():
+    import torch
+    work, status = torch.zeros(1 << 20, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64)
+
+    def orth(t, batch=2, rows=6, cols=8, **kw):
+        plan = m.orthogonalize_plan("f32", rows, cols, batch=batch, **kw)
+        keep = torch.zeros(4096)
+        got = {device_call(m.orthogonalize_async, plan, t, keep, work, status)}
+        plan = m.orthogonalize_plan("f32", rows, cols, batch=batch, **{"out_" + k: v for k, v in kw.items()})
+        return (got | {device_call(m.orthogonalize_async, plan, keep, t, work, status)}).pop()
+
+    square = torch.zeros(8, 8)
+    assert orth(torch.zeros(2, 6, 8)) == orth(torch.zeros(96)) == orth(torch.zeros(200)[7:]) == "library"
+    assert orth(torch.zeros(12, 8)) == orth(torch.zeros(1, 2, 6, 8)) == orth(torch.zeros(6, 8), batch=1) == "library"
+    wide = torch.zeros(2, 6, 11)
+    assert orth(wide[..., :8], row_stride=11) == orth(wide[..., 3:], row_stride=11) == "library"
+    assert orth(wide.view(12, 11)[:, 2:10], row_stride=11) == orth(wide[0, :, :8], batch=1, row_stride=11) == "library"
+    assert orth(wide[:, :, 1:], row_stride=11) == "library"               # wider than the plan's rows
+    assert orth(torch.zeros(6, 2, 8).transpose(0, 1), batch_stride=200) == "binding"
+    for t in (torch.zeros(2, 8, 6).transpose(1, 2), torch.zeros(2, 6, 11)[..., :8], torch.zeros(2, 6, 16)[..., ::2],
+              torch.zeros(4, 6, 8)[::2], torch.zeros(2, 12, 8)[:, ::2], torch.zeros(1, 6, 8).expand(2, 6, 8)):
+        assert orth(t) == "binding", t.stride()
+    assert orth(square.T, batch=1, rows=8) == "binding"
+    assert orth(torch.zeros(200)[:96].view(2, 6, 8), row_stride=11) == "binding"    # dense, with room behind
+
+    def bias(t, **kw):
+        plan = m.position_bias_plan("f32", 3, 5, 7, **kw)
+        got = {device_call(m.position_bias_async, plan, torch.zeros(32, 3), t)}
+        grad = device_call(m.position_bias_grad_async, plan, t, torch.zeros(32, 3), work)
+        assert got == {grad}
+        return grad
+
+    assert bias(torch.zeros(3, 5, 7)) == bias(torch.zeros(3, 5, 9)[..., :7], row_stride=9) == "library"
+    inside = dict(row_stride=27, head_stride=9)                                     # heads inside rows
+    buffer = torch.zeros(5, 3, 9)
+    assert bias(buffer[..., :7].transpose(0, 1), **inside) == bias(buffer[..., :7], **inside) == "library"
+    assert bias(buffer, **inside) == bias(buffer.view(-1), **inside) == "library"
+    for t in (torch.zeros(5, 3, 7).transpose(0, 1), torch.zeros(3, 7, 5).transpose(1, 2), torch.zeros(3, 5, 9)[..., :7],
+              torch.zeros(3, 5, 7)[:, :, :1].expand(3, 5, 7)):
+        assert bias(t) == "binding"
+    assert bias(torch.zeros(3, 5, 9)[..., :7], **inside) == "binding"
