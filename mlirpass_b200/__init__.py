@@ -598,10 +598,24 @@ def _room(t) -> int:
     return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
 
 
-def _need(t, what: str, elements: int, size: int) -> int:
-    """The pointer of a dense tensor of at least `elements` of `size` bytes."""
-    if t.element_size() != size:
-        raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
+_TORCH_TYPES: dict = {}
+
+
+def _typed(t, what: str, dtype: str) -> None:
+    """Refuse a tensor whose elements are not of the given type (another of the same size would be read as it)."""
+    if not _TORCH_TYPES:
+        import torch
+        _TORCH_TYPES.update(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32, f64=torch.float64, i32=torch.int32)
+    if t.dtype is not _TORCH_TYPES[dtype]:
+        raise ValueError(f"{what}: {t.dtype}, {dtype} expected")
+
+
+def _need(t, what: str, elements: int, dtype: str | None) -> int:
+    """The pointer of a dense tensor of at least `elements` of a type (None: any of 8 bytes)."""
+    if dtype:
+        _typed(t, what, dtype)
+    elif t.element_size() != 8:
+        raise ValueError(f"{what}: elements of {t.element_size()} bytes, 8 expected")
     if elements and (not t.is_contiguous() or t.numel() < elements):
         raise ValueError(f"{what}: {elements} contiguous elements expected, not {tuple(t.shape)} with strides {t.stride()}")
     return t.data_ptr()
@@ -637,10 +651,9 @@ def _lies_as(t, shape, strides) -> bool:
     return _memory(have, at) == _memory(shape, strides)
 
 
-def _need_layout(t, what: str, elements: int, size: int, shape, strides) -> int:
+def _need_layout(t, what: str, elements: int, dtype: str, shape, strides) -> int:
     """The pointer of a tensor in which the plan's layout, `elements` from its first to its last, lies."""
-    if t.element_size() != size:
-        raise ValueError(f"{what}: elements of {t.element_size()} bytes, {size} expected")
+    _typed(t, what, dtype)
     if elements and not (t.is_contiguous() and t.numel() >= elements):
         if _room(t) < elements:
             raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
@@ -652,9 +665,7 @@ def _need_layout(t, what: str, elements: int, size: int, shape, strides) -> int:
 def _positions(positions, queries: int):
     if positions is None:
         return None
-    if "int32" not in str(positions.dtype):
-        raise ValueError(f"positions: {positions.dtype}, int32 expected")
-    return _need(positions, "positions", queries, 4)
+    return _need(positions, "positions", queries, "i32")
 
 
 def _bytes(workspace) -> int:
@@ -668,9 +679,9 @@ def position_bias_async(plan: BiasPlan, table, out, *, positions=None, stream=No
     `out` starts at the bias's first element and lies as the plan's strides say
     (a tensor of the bias's shape with these strides, or the memory around it)."""
     _check(lib().dcf_position_bias_async(
-        plan.ref, _need(table, "table", plan.entries, DTYPE_SIZE[plan.table_dtype]),
+        plan.ref, _need(table, "table", plan.entries, plan.table_dtype),
         _positions(positions, plan.desc.queries),
-        _need_layout(out, "out", plan.out_elements, DTYPE_SIZE[plan.dtype], *plan.out_layout), _own_stream(stream, out)))
+        _need_layout(out, "out", plan.out_elements, plan.dtype, *plan.out_layout), _own_stream(stream, out)))
 
 
 def position_bias_grad_workspace(plan: BiasPlan) -> int:
@@ -683,9 +694,9 @@ def position_bias_grad_async(plan: BiasPlan, grad, out, workspace, *, positions=
     strides say, `out` is the dense [num_buckets, heads] gradient, `workspace`
     uint8 (may be empty when position_bias_grad_workspace says 0)."""
     _check(lib().dcf_position_bias_grad_async(
-        plan.ref, _need_layout(grad, "grad", plan.grad_elements, DTYPE_SIZE[plan.dtype], *plan.grad_layout),
+        plan.ref, _need_layout(grad, "grad", plan.grad_elements, plan.dtype, *plan.grad_layout),
         _positions(positions, plan.desc.queries),
-        _need(out, "out", plan.entries, 8 if plan.dtype == "f64" else 4), workspace.data_ptr(),
+        _need(out, "out", plan.entries, "f64" if plan.dtype == "f64" else "f32"), workspace.data_ptr(),
         _bytes(workspace), _own_stream(stream, out)))
 
 
@@ -764,6 +775,6 @@ def orthogonalize_async(plan: OrthPlan, x, out, workspace, status, *, stream=Non
     say; `out` may be `x`.
     `status` (16 bytes, reset first) takes a kernel's error report."""
     _check(lib().dcf_orthogonalize_async(
-        plan.ref, _need_layout(x, "x", plan.in_elements, DTYPE_SIZE[plan.dtype], *plan.in_layout),
-        _need_layout(out, "out", plan.out_elements, DTYPE_SIZE[plan.out_dtype], *plan.out_layout), workspace.data_ptr(),
-        _bytes(workspace), _need(status, "status", 2, 8), _own_stream(stream, out)))
+        plan.ref, _need_layout(x, "x", plan.in_elements, plan.dtype, *plan.in_layout),
+        _need_layout(out, "out", plan.out_elements, plan.out_dtype, *plan.out_layout), workspace.data_ptr(),
+        _bytes(workspace), _need(status, "status", 2, None), _own_stream(stream, out)))

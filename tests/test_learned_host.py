@@ -289,3 +289,35 @@ def test_tensors_lie_as_the_plan_says():
               torch.zeros(3, 5, 7)[:, :, :1].expand(3, 5, 7)):
         assert bias(t) == "binding"
     assert bias(torch.zeros(3, 5, 9)[..., :7], **inside) == "binding"
+
+
+def test_tensors_have_the_plans_types():
+    import torch
+    work, status = torch.zeros(1 << 20, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64)
+    types = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32, "f64": torch.float64}
+    others = [torch.float16, torch.bfloat16, torch.float32, torch.float64, torch.int16, torch.int32, torch.int64,
+              torch.complex64]
+    for name, own in types.items():
+        wide = torch.float64 if name == "f64" else torch.float32
+        plan = m.position_bias_plan(name, 4, 10, 16)
+        orth = m.orthogonalize_plan(name, 10, 16) if name != "f64" else None
+        back = m.orthogonalize_plan("f32", 10, 16, out_dtype=name) if name != "f64" else None
+        for t in others:
+            table, bias = torch.zeros(32, 4, dtype=t), torch.zeros(4, 10, 16, dtype=t)
+            x, f = torch.zeros(10, 16, dtype=t), torch.zeros(10, 16)
+            want = "library" if t == own else "binding"
+            assert device_call(m.position_bias_async, plan, table, torch.zeros(4, 10, 16, dtype=own)) == want
+            assert device_call(m.position_bias_async, plan, torch.zeros(32, 4, dtype=own), bias) == want
+            assert device_call(m.position_bias_grad_async, plan, bias, torch.zeros(32, 4, dtype=wide), work) == want
+            assert device_call(m.position_bias_grad_async, plan, torch.zeros(4, 10, 16, dtype=own), table, work) == \
+                ("library" if t == wide else "binding")
+            if orth:
+                assert device_call(m.orthogonalize_async, orth, x, torch.zeros(10, 16, dtype=own), work, status) == want
+                assert device_call(m.orthogonalize_async, back, f, x, work, status) == want
+    plan = m.position_bias_plan("bf16", 4, 10, 16, table_dtype="f32")
+    for t in others:
+        assert device_call(m.position_bias_async, plan, torch.zeros(32, 4, dtype=t), torch.zeros(4, 10, 16).bfloat16()) == \
+            ("library" if t == torch.float32 else "binding")
+    for t in (torch.int32, torch.uint32, torch.int64, torch.float32):
+        assert device_call(m.position_bias_async, plan, torch.zeros(32, 4), torch.zeros(4, 10, 16).bfloat16(),
+                           positions=torch.zeros(10, dtype=t)) == ("library" if t == torch.int32 else "binding")
