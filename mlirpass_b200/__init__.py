@@ -570,9 +570,15 @@ def position_bias_grad(plan: BiasPlan, grad, *, positions=None, out: np.ndarray 
 def _host_positions(positions, queries: int):
     if positions is None:
         return None
-    p = np.ascontiguousarray(positions, dtype=np.int32).reshape(-1)
-    if len(p) != queries:
-        raise ValueError(f"{len(p)} positions for {queries} queries")
+    given = np.asarray(positions).reshape(-1)
+    if len(given) != queries:
+        raise ValueError(f"{len(given)} positions for {queries} queries")
+    if given.dtype.kind not in "biuf":
+        raise ValueError(f"positions: {given.dtype}, whole numbers expected")
+    with np.errstate(invalid="ignore"):
+        p = np.ascontiguousarray(given, dtype=np.int32)
+    if not np.array_equal(p, given):                    # a cast wraps and cuts without a word
+        raise ValueError("positions: whole numbers of 32 bits expected")
     return p
 
 

@@ -321,3 +321,17 @@ def test_tensors_have_the_plans_types():
     for t in (torch.int32, torch.uint32, torch.int64, torch.float32):
         assert device_call(m.position_bias_async, plan, torch.zeros(32, 4), torch.zeros(4, 10, 16).bfloat16(),
                            positions=torch.zeros(10, dtype=t)) == ("library" if t == torch.int32 else "binding")
+
+
+def test_host_positions_keep_their_value():
+    plan = m.position_bias_plan("f32", 1, 3, 4)
+    for p in ([0, 1, 1 << 31], np.array([0, 1, (1 << 32) + 2]), np.array([0, 1, 1 << 63], np.uint64), [0, 1, 2.5],
+              [0, 1, math.nan], np.array([0.0, 1.0, 3e9]), [0, 1, -(1 << 31) - 1], ["0", "1", "2"], [0, 1]):
+        with pytest.raises(ValueError):
+            m.position_bias(plan, np.zeros((32, 1), np.float32), positions=p)
+        with pytest.raises(ValueError):
+            m.position_bias_grad(plan, np.zeros((1, 1, 3, 4), np.float32), positions=p)
+    for p in ([0, -5, (1 << 31) - 1], np.array([0, -(1 << 31), 7]), np.array([0.0, 1.0, 2.0]), np.arange(6, dtype=np.int16)[::2],
+              np.array([1, 2, 3], np.uint64), [True, False, True]):
+        assert m._host_positions(p, 3).tolist() == [int(v) for v in p]
+    assert len(m._host_positions([], 0)) == 0
