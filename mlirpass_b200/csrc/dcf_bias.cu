@@ -21,7 +21,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include "dcf_launch.h"
+#include "dcf_kernels.cuh"
 
 namespace dcf {
 
@@ -628,7 +628,7 @@ int launch_grad_t(const dcf_bias_desc& d, const void* g, const int32_t* pos, voi
     c.stream = stream;
     cudaLaunchAttribute dependent[1];
     dependent[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    dependent[0].val.programmaticStreamSerializationAllowed = 1;
+    dependent[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     c.attrs = dependent;
     c.numAttrs = 1;
     note_launch();

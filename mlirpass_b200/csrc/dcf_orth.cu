@@ -1386,8 +1386,8 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
   return l;
 }
 
-// Launches as a programmatic dependent: the kernel's start overlaps the end of
-// the one before it, whose results it reads only after griddepcontrol.wait.
+// Launches as a programmatic dependent (unless DCF_PDL=0): the kernel's start overlaps
+// the end of the one before it, whose results it reads only after griddepcontrol.wait.
 template <class... P, class... A>
 int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t c = {};
@@ -1397,7 +1397,7 @@ int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, 
   c.stream = s;
   cudaLaunchAttribute a[2];
   a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a[0].val.programmaticStreamSerializationAllowed = 1;
+  a[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
   a[1].id = cudaLaunchAttributeClusterDimension;
   a[1].val.clusterDim.x = (unsigned)cluster;
   a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;

@@ -755,3 +755,55 @@ def test_orth_largest_value_inside_the_interval(dcf, rows, cols, c):
     x[0, 0, 0], x[0, 1, 1] = 0.589, 0.808
     coef = [(2.6, -2.5, c)] * 2
     check_orth(run_orth(dcf, x, "f32", steps=2, coef=coef), x, "f32", coef)
+
+
+PROGRAMMATIC_EDGES = """
+import ctypes, sys
+import torch
+import mlirpass_b200 as dcf
+cu = ctypes.CDLL("libcuda.so.1")
+def check(rc):
+    assert rc == 0, rc
+torch.manual_seed(1)
+stream = torch.cuda.Stream()
+orth = dcf.orthogonalize_plan("f32", 150, 170)
+grad = dcf.position_bias_plan("f32", 8, 500, 500)
+x, g = torch.randn(150, 170, device="cuda"), torch.randn(1, 8, 500, 500, device="cuda")
+out, table = torch.empty_like(x), torch.empty(32, 8, device="cuda")
+work = torch.empty(orth.workspace + grad.workspace, dtype=torch.uint8, device="cuda")
+status = torch.empty(2, dtype=torch.int64, device="cuda")
+dcf.status_reset(status)
+def count(run):
+    run()
+    torch.cuda.synchronize()
+    graph, n = ctypes.c_void_p(), ctypes.c_size_t(0)
+    check(cu.cuStreamBeginCapture_v2(ctypes.c_void_p(stream.cuda_stream), 2))
+    run()
+    check(cu.cuStreamEndCapture(ctypes.c_void_p(stream.cuda_stream), ctypes.byref(graph)))
+    check(cu.cuGraphGetEdges_v2(graph, None, None, None, ctypes.byref(n)))
+    start, end, data = (ctypes.c_void_p * n.value)(), (ctypes.c_void_p * n.value)(), (ctypes.c_uint8 * (8 * n.value))()
+    check(cu.cuGraphGetEdges_v2(graph, start, end, data, ctypes.byref(n)))
+    check(cu.cuGraphDestroy(graph))
+    return n.value, sum(data[8 * i + 2] == 1 for i in range(n.value))
+a = count(lambda: dcf.orthogonalize_async(orth, x, out, work, status, stream=stream))
+b = count(lambda: dcf.position_bias_grad_async(grad, g, table, work, stream=stream))
+assert dcf.status_read(status).folded
+print(*a, *b, out.double().sum().item().hex(), table.double().sum().item().hex())
+"""
+
+
+def test_launches_as_programmatic_dependents_can_be_turned_off():
+    """DCF_PDL=0 reaches every launch of these operators: no programmatic edge in a captured graph, the same bits."""
+    import os
+    import subprocess
+    import sys
+    import conftest
+    got = {}
+    for value in ("1", "0"):
+        env = dict(os.environ, DCF_PDL=value, PYTHONPATH=conftest.ROOT)
+        run = subprocess.run([sys.executable, "-c", PROGRAMMATIC_EDGES], env=env, capture_output=True, text=True, timeout=300)
+        assert run.returncode == 0, run.stderr[-2000:]
+        got[value] = run.stdout.split()
+    assert got["1"][4:] == got["0"][4:] and got["1"][0::2][:2] == got["0"][0::2][:2]
+    assert int(got["1"][0]) >= 10 and int(got["1"][1]) >= 10 and int(got["1"][3]) == 1
+    assert got["0"][1] == got["0"][3] == "0"
