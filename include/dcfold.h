@@ -497,12 +497,16 @@ typedef struct dcf_bias_desc {
  * coefficients (a, b, c),
  *     A = X X^T,  X <- a X + (b A + c A A) X,
  * which maps every singular value s of X to a s + b s^3 + c s^5.  Every
- * operand of a product is kept as two fp16 halves of a scaled value (22 bits
- * or more), products are summed in 32 bits, the norm in 64; the result is
+ * operand of a product is kept as two fp16 halves of a value scaled by a
+ * power of two: to 22 bits, or to 2^-38 of a bound on the operand's largest singular
+ * value (the power of two above it) where that is more.  Bounds start from 1, or from
+ * ||G||_F / (||G||_F + eps) where eps exceeds the norm, and follow the
+ * coefficients.  Products are summed in 32 bits, the norm in 64; the result is
  * rounded once.  The coefficients must keep every singular value from [0, 1]
- * within [-64, 64], and leave some of it (checked).  A matrix with min(rows, cols) <= 128 and
- * max(rows, cols) <= 2048 stays on the chip and needs no workspace.  No
- * steps (steps = 0) give G / (||G||_F + eps). */
+ * within [-64, 64], and leave some of it (checked).  With at least one step a
+ * matrix with min(rows, cols) <= 128 and max(rows, cols) <= 2048 stays on the
+ * chip and needs no workspace.  No steps (steps = 0) give G / (||G||_F + eps),
+ * and need one. */
 typedef struct dcf_orth_desc {
   uint32_t dtype, out_dtype; /* DCF_F16, DCF_BF16 or DCF_F32 */
   uint32_t steps;            /* 0 .. DCF_ORTH_MAX_STEPS */

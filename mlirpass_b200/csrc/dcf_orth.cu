@@ -7,15 +7,16 @@
 // rounding of X leaves in its null space by several hundred: operands of 11
 // bits show as 4 % in a matrix of low rank.  Operands are therefore exact splits:
 // a value v scaled by a power of two is kept as two fp16 planes, hi = fp16(v)
-// and lo = fp16(v - hi), 22 bits or more, and a product is
+// and lo = fp16(v - hi): 22 bits, or, of what lies far below the scale, half of
+// fp16's smallest step, 2^-25 beside a bound of 2^13.  A product is
 //     hi hi + hi lo + lo hi
 // (the dropped lo lo is 2^-22 of it).  The tensor core truncates as it
 // accumulates, which over a long k costs more than the split does: TMEM sums
 // short runs of k (32 to 128, see sums_of) and fp32 registers, which round, add
-// the runs.  Five steps end as near to
-// 64-bit arithmetic as with products of fp32 values (8192 x 2048: 2.8e-6 here,
-// 5.4e-6 there; 258 x 131, six steps: 2.4e-6 and 2.1e-6), at three fp16
-// products instead of fp32 arithmetic on the CUDA cores.
+// the runs.  Five steps end about as near to
+// 64-bit arithmetic as with products of fp32 values (f32, 8 to 1200 rows, one to sixteen
+// times as many columns: 0.3 to 1.6 times their error, the more at few rows; 8192 x 2048: 2.8e-6
+// here, 5.4e-6 there), at three fp16 products instead of fp32 arithmetic on the CUDA cores.
 //
 // Scales are powers of two from bounds: singular values of
 // X are in [0, 1] at the start, a step maps s to |a s + b s^3 + c s^5|, and

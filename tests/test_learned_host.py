@@ -335,3 +335,15 @@ def test_host_positions_keep_their_value():
               np.array([1, 2, 3], np.uint64), [True, False, True]):
         assert m._host_positions(p, 3).tolist() == [int(v) for v in p]
     assert len(m._host_positions([], 0)) == 0
+
+
+def test_orth_workspace_without_steps():
+    """No workspace is for matrices that stay on the chip; without steps nothing does."""
+    call = m.lib().dcf_orthogonalize_async
+    for rows, cols in ((96, 96), (128, 2048), (1, 1)):
+        assert m.orthogonalize_plan("f32", rows, cols, steps=1).workspace == 0
+        plan = m.orthogonalize_plan("f32", rows, cols, steps=0)
+        assert plan.workspace > 0
+        assert call(plan.ref, 256, 256, None, 0, 256, None) == -1 and b"null" in m.lib().dcf_last_error()
+        assert call(plan.ref, 256, 256, 256, plan.workspace - 1, 256, None) == -1
+        assert b"workspace" in m.lib().dcf_last_error()
