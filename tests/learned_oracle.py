@@ -152,3 +152,9 @@ def orth_quantum(g: np.ndarray, coef, eps: float, seed: int = 0) -> float:
             s = float((np.sqrt(t) * np.abs(a + t * (b + t * c))).max())
         return x
     return 4 * max(np.linalg.norm(run() - want) for _ in range(3)) if norm else 0.0
+
+
+def whole_values(shape, seed: int) -> np.ndarray:
+    """1 .. 7 at random: exact in every type, and any sum of them below 2^24 is exact in
+    f32 whatever its order, so that a sum that lacks, repeats or misplaces one element differs."""
+    return np.random.default_rng(seed).integers(1, 8, shape).astype(np.float64)

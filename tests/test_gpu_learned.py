@@ -807,3 +807,85 @@ def test_launches_as_programmatic_dependents_can_be_turned_off():
     assert got["1"][4:] == got["0"][4:] and got["1"][0::2][:2] == got["0"][0::2][:2]
     assert int(got["1"][0]) >= 10 and int(got["1"][1]) >= 10 and int(got["1"][3]) == 1
     assert got["0"][1] == got["0"][3] == "0"
+
+
+# --------------------------------------- gradient sums that are exact
+
+
+def whole(shape, dtype, seed):
+    import torch
+    return torch.from_numpy(lo.whole_values(shape, seed)).cuda().to(tdtype(dtype))
+
+
+def check_exact(got, g, ids, hidden, num_buckets=32, start=0.0):
+    want, mag = lo.bias_grad(values(g), ids, num_buckets, hidden)
+    assert mag.max() + abs(start) < 2 ** 24
+    assert np.array_equal(values(got), want + start)
+
+
+@pytest.mark.parametrize("batch,queries,keys", [(1, 1, 1), (2, 1, 9), (1, 3, 40), (3, 17, 33), (1, 64, 64),
+                                                (9, 50, 131), (2, 257, 513), (1, 1, 5000), (40, 7, 65), (3, 1000, 12)])
+@pytest.mark.parametrize("both,causal", [(True, False), (False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16", "f64"])
+def test_grad_exact_sizes(dcf, batch, queries, keys, both, causal, dtype):
+    g = whole((batch, 3, queries, keys), dtype, 111)
+    first = max(0, keys - queries)
+    got = run_grad(dcf, g, dtype, bidirectional=both, causal=causal, first_query=first)
+    q = lo.positions(queries, first)
+    check_exact(got, g, lo.buckets(q, keys, 32, 128, both), lo.masked(q, keys) if causal else None)
+
+
+@pytest.mark.parametrize("off", [0, 1, 3, 7])
+@pytest.mark.parametrize("batch,queries,keys,first", [(2, 20, 512, 100), (8, 40, 512, -600), (5, 3, 1024, 900),
+                                                      (6, 700, 256, 0), (2, 30, 1023, 500), (1, 9, 4097, 8000)])
+@pytest.mark.parametrize("dtype,causal", [("bf16", False), ("f16", True), ("f16", False), ("f32", True), ("f64", False)])
+def test_grad_exact_from_any_start(dcf, off, batch, queries, keys, first, dtype, causal):
+    """Every step of every row counts once, wherever rows begin within 16 bytes."""
+    import torch
+    n = batch * 2 * queries * keys
+    flat = torch.zeros(n + 8, device="cuda", dtype=tdtype(dtype))
+    g = flat[off:off + n].view(batch, 2, queries, keys)
+    g.copy_(whole((batch, 2, queries, keys), dtype, 119))
+    got = run_grad(dcf, g, dtype, first_query=first, bidirectional=not causal, causal=causal)
+    at = lo.positions(queries, first)
+    check_exact(got, g, lo.buckets(at, keys, 32, 128, not causal), lo.masked(at, keys) if causal else None)
+
+
+@pytest.mark.parametrize("shape,strides,off", [((2, 3, 20, 45), (8000, 2000, 50, 1), 0), ((2, 3, 20, 45), (3 * 20 * 45 + 1, 45, 135, 1), 0),
+                                               ((1, 2, 30, 70), (9999, 2101, 70, 1), 3), ((3, 2, 11, 600), (20007, 9001, 640, 1), 5)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32", "f64"])
+def test_grad_exact_strides(dcf, shape, strides, off, dtype):
+    """What lies between rows (here NaN) is not summed."""
+    import torch
+    n = sum((s - 1) * t for s, t in zip(shape, strides)) + 1
+    flat = torch.full((n + off + 8,), float("nan"), device="cuda", dtype=tdtype(dtype))
+    g = flat[off:].as_strided(shape, strides, off)
+    g.copy_(whole(shape, dtype, 115))
+    got = run_grad(dcf, g, dtype, first_query=3)
+    check_exact(got, g, lo.buckets(lo.positions(shape[2], 3), shape[3], 32, 128, True), None)
+
+
+@pytest.mark.parametrize("num_buckets,max_distance,both", [(1, 1, False), (2, 1, True), (3, 2, True), (5, 3, False),
+                                                           (64, 300, True), (100, 3000, False), (128, 70, True), (256, 400, False)])
+@pytest.mark.parametrize("dtype", ["f16", "f32", "f64"])
+def test_grad_exact_buckets_and_positions(dcf, num_buckets, max_distance, both, dtype):
+    rng = np.random.default_rng(5)
+    given = [int(v) for v in rng.integers(-400, 900, 60)] + [0, 0, 299, -1, 300, 5000, -(1 << 31), (1 << 31) - 1]
+    g = whole((2, 2, len(given), 300), dtype, 112)
+    for causal in (False, True):
+        got = run_grad(dcf, g, dtype, given=given, num_buckets=num_buckets, max_distance=max_distance, bidirectional=both,
+                       causal=causal)
+        check_exact(got, g, lo.buckets(given, 300, num_buckets, max_distance, both),
+                    lo.masked(given, 300) if causal else None, num_buckets)
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 1, 3), (2, 2, 300, 300)])
+@pytest.mark.parametrize("dtype", ["bf16", "f64"])
+def test_grad_exact_accumulates(dcf, shape, dtype):
+    import torch
+    g = whole(shape, dtype, 116)
+    out = torch.full((32, 2), 5.0, device="cuda", dtype=torch.float64 if dtype == "f64" else torch.float32)
+    for k in range(3):
+        run_grad(dcf, g, dtype, out=out)
+    ids = lo.buckets(lo.positions(shape[2], 0), shape[3], 32, 128, True)
+    assert np.array_equal(values(out), 3 * lo.bias_grad(values(g), ids, 32)[0] + 5.0)

@@ -347,3 +347,22 @@ def test_orth_workspace_without_steps():
         assert call(plan.ref, 256, 256, None, 0, 256, None) == -1 and b"null" in m.lib().dcf_last_error()
         assert call(plan.ref, 256, 256, 256, plan.workspace - 1, 256, None) == -1
         assert b"workspace" in m.lib().dcf_last_error()
+
+
+@pytest.mark.parametrize("batch,queries,keys,first", [(6, 700, 256, 0), (8, 40, 512, -600), (2, 20, 512, 100), (1, 3, 9, 0)])
+def test_whole_values_show_what_is_missing(batch, queries, keys, first):
+    """One element, one step of 32 vectors, one row or one far range left out changes a sum."""
+    g = lo.whole_values((batch, 1, queries, keys), 1)
+    ids = lo.buckets(lo.positions(queries, first), keys, 32, 128, True)
+    want, mag = lo.bias_grad(g, ids, 32)
+    assert mag.max() < 2 ** 24 and np.array_equal(want, mag)
+    rng = np.random.default_rng(2)
+    for _ in range(5):
+        b, q, k = rng.integers(batch), rng.integers(queries), rng.integers(keys)
+        for cut in (np.s_[b, :, q, k], np.s_[b, :, q, k:k + 256], np.s_[b, :, q], np.s_[:, :, ids == ids[q, k]]):
+            less = g.copy()
+            less[cut] = 0
+            assert not np.array_equal(lo.bias_grad(less, ids, 32)[0], want)
+        more = g.copy()
+        more[b, 0, q, k] *= 2
+        assert not np.array_equal(lo.bias_grad(more, ids, 32)[0], want)
