@@ -889,3 +889,50 @@ def test_grad_exact_accumulates(dcf, shape, dtype):
         run_grad(dcf, g, dtype, out=out)
     ids = lo.buckets(lo.positions(shape[2], 0), shape[3], 32, 128, True)
     assert np.array_equal(values(out), 3 * lo.bias_grad(values(g), ids, 32)[0] + 5.0)
+
+
+# ------------------------------------------------- clusters, low rank, not finite
+
+
+@pytest.mark.parametrize("batch", [1, 150])
+@pytest.mark.parametrize("longer", [256, 257, 512, 513, 1024, 1025, 1100, 2048])
+@pytest.mark.parametrize("shorter", [30, 128])
+@pytest.mark.parametrize("tall", [False, True])
+def test_orth_clusters_of_one_to_eight(dcf, batch, longer, shorter, tall):
+    """A matrix takes a cluster of 1, 2, 4 or 8 CTAs by its longer side alone; the last CTAs may
+    hold few columns or none.  One matrix, and more of them than SMs."""
+    shape = (batch, longer, shorter) if tall else (batch, shorter, longer)
+    x = randn(shape, "f32", 133)
+    got = run_orth(dcf, x, "f32", steps=3)
+    some = sorted({0, batch // 2, batch - 1})
+    check_orth(got[some], x[some], "f32", [COEF] * 3)
+    assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,cols", [(60, 200), (100, 120), (200, 260), (700, 150)])
+def test_orth_low_rank_of_16_bits(dcf, rows, cols, dtype):
+    """Whole numbers of four directions: the rank is exact in 16 bits, the null space is amplified the most."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(125)
+    a = torch.randint(-3, 4, (1, rows, 4), device="cuda", generator=gen).float()
+    b = torch.randint(-3, 4, (1, 4, cols), device="cuda", generator=gen).float()
+    x = (a @ b).to(tdtype(dtype))
+    assert torch.linalg.matrix_rank(x[0].double()) == 4
+    check_orth(run_orth(dcf, x, dtype), x, dtype, [COEF] * 5)
+    check_orth(run_orth(dcf, x, dtype, out_dtype="f32"), x, "f32", [COEF] * 5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(33, 40), (40, 900), (150, 170), (300, 140)])
+def test_orth_not_finite_in_a_batch(dcf, rows, cols, dtype):
+    """NaN or an infinity makes its own matrix NaN and no other; zeros stay zeros."""
+    x = randn((6, rows, cols), dtype, 128)
+    x[0] = 0
+    x[2, 3, 3] = float("nan")
+    x[3, rows - 1, cols - 1] = float("inf")
+    x[4, 0, cols - 1] = float("-inf")
+    got = run_orth(dcf, x, dtype)
+    assert (got[0] == 0).all()
+    assert all(got[k].isnan().all() for k in (2, 3, 4))
+    check_orth(got[[1, 5]], x[[1, 5]], dtype, [COEF] * 5)
