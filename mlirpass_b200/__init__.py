@@ -660,7 +660,8 @@ def _lies_as(t, shape, strides) -> bool:
 def _need_layout(t, what: str, elements: int, dtype: str, shape, strides) -> int:
     """The pointer of a tensor in which the plan's layout, `elements` from its first to its last, lies."""
     _typed(t, what, dtype)
-    if elements and not (t.is_contiguous() and t.numel() >= elements):
+    own = t.is_contiguous() and t.numel() >= elements or t.stride() == strides and t.shape == shape
+    if elements and not own:
         if _room(t) < elements:
             raise ValueError(f"{what}: {_room(t)} elements behind the pointer, {elements} needed")
         if not _lies_as(t, shape, strides):
