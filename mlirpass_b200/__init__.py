@@ -481,7 +481,8 @@ ORTH_COEF = (3.4445, -4.7750, 2.0315)
 
 class BiasPlan:
     """The sizes, types and strides of one position bias: a dcf_bias_desc
-    that calls reuse.  Validated when made."""
+    that calls reuse.  What no call takes is refused when it is made; what the bias
+    alone does not take (rows that overlap, a table of another type, accumulation) by its call."""
 
     def __init__(self, desc: BiasDesc, dtype: str, table_dtype: str):
         self.desc, self.dtype, self.table_dtype = desc, dtype, table_dtype

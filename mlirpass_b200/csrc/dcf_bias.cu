@@ -28,6 +28,8 @@ namespace dcf {
 namespace {
 
 constexpr int kMaxB = DCF_BIAS_MAX_BUCKETS;
+// A B200's, for the sizes of grids and splits.  Not asked of the device: sums then split alike
+// wherever they run, and a workspace's size needs no device.  Any number of SMs runs them.
 constexpr int kSms = 148;
 constexpr int kTable = 256;  // distances whose bucket is looked up rather than searched
 

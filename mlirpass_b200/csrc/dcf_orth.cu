@@ -1283,15 +1283,17 @@ constexpr double kMostSingular = 64;
 // f32 (bf16 258 x 131, six steps: 0.21 % of the results, with two stages 0.58 %, fp32 products
 // 0.17 %; 520 x 530: two stages 0.33 %, fp32 products 0.20 %), above two stages (4096 x 4096:
 // 0.25 % and 3.6 ms, with 16 1.8 % and 3.4 ms, fp32 products 0.33 %), up to 1024 rows one in A A
-// (1024 x 4096: 0.2 %, with two 0.23 %, with 16 1.6 %, fp32 products 0.27 %; 770 x 1540: with two
-// 1.8 times as many as fp32 products).
+// (1024 x 4096: 0.16 % and 438 us, with two 0.23 % and 437 us, with 16 1.6 % and 427 us, fp32
+// products 0.27 %; 770 x 1540: with two 1.8 times as many as fp32 products).
 int sums_of(const dcf_orth_desc& d, int m, bool square) {
   const bool f32 = d.out_dtype == DCF_F32;
   if (square && m <= 1024) return f32 || m <= 768 ? 0 : 1;
   return f32 || m <= 768 ? 1 : 2;
 }
 
-constexpr int kPairs = 74;  // pairs of SMs
+// Pairs of SMs on a B200: not asked of the device, as a workspace's size needs none and
+// the parts of a sum are then the same everywhere.  Any number runs the persistent grids.
+constexpr int kPairs = 74;
 
 // Blocks of the norm's sum: 32 KB of a f32 matrix each, 256 at most.
 int norm_parts(const dcf_orth_desc& d) {
