@@ -899,7 +899,18 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       }
     }
   }
-  std::vector<std::unique_ptr<DeviceBuf>> works;  // workspaces, until the batch is done
+  // One workspace for all folds that need one: they run one after the other on s_.
+  std::vector<size_t> work_bytes(R, 0);
+  for (size_t i = 0; i < R; i++) {
+    const FoldRequest& q = *reqs[i];
+    if (q.kind == FoldRequest::BIAS_GRAD)
+      check(dcf_position_bias_grad_workspace(&q.bias, &work_bytes[i]), "position bias gradient fold");
+    if (q.kind == FoldRequest::ORTH) check(dcf_orthogonalize_workspace(&q.orth, &work_bytes[i]), "orthogonalize fold");
+  }
+  std::unique_ptr<DeviceBuf> work;
+  if (const size_t most = *std::max_element(work_bytes.begin(), work_bytes.end()))
+    work = std::make_unique<DeviceBuf>(dev_, most);
+  void* const ws = work ? work->ptr : nullptr;
   for (size_t i = 0; i < R; i++) {
     if (batched[i]) continue;
     FoldRequest& q = *reqs[i];
@@ -938,24 +949,15 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
         check(dcf_position_bias_async(&q.bias, l, nullptr, outs[i]->ptr, s_), "position bias fold");
         check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
         break;
-      case FoldRequest::BIAS_GRAD: {
-        size_t bytes = 0;
-        check(dcf_position_bias_grad_workspace(&q.bias, &bytes), "position bias gradient fold");
-        works.push_back(std::make_unique<DeviceBuf>(dev_, std::max<size_t>(bytes, 256)));
-        check(dcf_position_bias_grad_async(&q.bias, l, nullptr, outs[i]->ptr, works.back()->ptr, bytes, s_),
+      case FoldRequest::BIAS_GRAD:
+        check(dcf_position_bias_grad_async(&q.bias, l, nullptr, outs[i]->ptr, ws, work_bytes[i], s_),
               "position bias gradient fold");
         check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
         break;
-      }
-      case FoldRequest::ORTH: {
-        size_t bytes = 0;
-        check(dcf_orthogonalize_workspace(&q.orth, &bytes), "orthogonalize fold");
-        works.push_back(std::make_unique<DeviceBuf>(dev_, std::max<size_t>(bytes, 256)));
-        check(dcf_orthogonalize_async(&q.orth, l, outs[i]->ptr, works.back()->ptr, bytes, st + i, s_),
-              "orthogonalize fold");
+      case FoldRequest::ORTH:
+        check(dcf_orthogonalize_async(&q.orth, l, outs[i]->ptr, ws, work_bytes[i], st + i, s_), "orthogonalize fold");
         check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
         break;
-      }
       case FoldRequest::SELECT:
         check(dcf_select_async(oes, cs[i], q.cond->splat, l, q.lhs->splat, r, q.rhs->splat, q.n, outs[i]->ptr, st + i,
                                s_),

@@ -238,3 +238,64 @@ def test_an_op_with_a_region_stays():
     out, stats = opt.run(module("tensor<32x3xf32>", hexed(TABLE), "dcf.position_bias", " ({\n    })", "tensor<3x5x6xf32>"),
                          PIPELINE, n_gpus=0)
     assert '"dcf.position_bias"' in out and stats["folds"] == 0
+
+
+MEMORY_OF_MANY = """
+import sys
+import torch
+from mlirpass_b200 import opt
+def module(n):
+    ty = "tensor<1024x1024xbf16>"
+    return '"builtin.module"() ({\\n' + "".join(
+        f'  "func.func"() <{{function_type = () -> {ty}, sym_name = "f{k}"}}> ({{\\n'
+        f'    %0 = "arith.constant"() <{{value = dense<{k + 1}.0> : {ty}}}> : () -> {ty}\\n'
+        f'    %1 = "dcf.orthogonalize"(%0) <{{steps = 2 : i64}}> : ({ty}) -> {ty}\\n'
+        f'    "func.return"(%1) : ({ty}) -> ()\\n'
+        '  }) : () -> ()\\n' for k in range(n)) + '}) : () -> ()\\n'
+def used():
+    free, total = torch.cuda.mem_get_info()
+    return total - free
+pipeline = "builtin.module(func.func(learned-constant-fold,canonicalize))"
+out, stats = opt.run(module(1), pipeline, n_gpus=1)
+one = used()
+out, stats = opt.run(module(64), pipeline, n_gpus=1)
+assert stats["folds"] == 64 and "dcf.orthogonalize" not in out
+print(used() - one)
+"""
+
+
+@pytest.mark.gpu
+def test_folds_of_one_batch_share_a_workspace():
+    """64 functions, each with a matrix of 2 MB: operands and results (4 MB a function, at most
+    twice that in their size classes) stay on the device, a workspace of 16 MB or more each does not."""
+    import os
+    import subprocess
+    import sys
+    import conftest
+    run = subprocess.run([sys.executable, "-c", MEMORY_OF_MANY], env=dict(os.environ, PYTHONPATH=conftest.ROOT),
+                         capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+    assert int(run.stdout) <= 64 * 2 * (4 << 20) + (64 << 20)
+
+
+@pytest.mark.gpu
+def test_operators_of_different_sizes_in_one_batch():
+    """Functions whose workspaces differ, folded in one batch, each as it folds alone."""
+    rng = np.random.default_rng(9)
+    parts, alone = [], {}
+    for k, (op, shape, props, out) in enumerate([
+            ("dcf.orthogonalize", (150, 170), "", None), ("dcf.position_bias_grad", (2, 3, 300, 200), "", (32, 3)),
+            ("dcf.orthogonalize", (2, 30, 40), "", None), ("dcf.orthogonalize", (400, 131), " <{steps = 3 : i64}>", None),
+            ("dcf.position_bias", (32, 3), "", (3, 20, 30)), ("dcf.position_bias_grad", (1, 700, 700), " <{causal = true}>", (64, 1)),
+            ("dcf.orthogonalize", (64, 64), " <{steps = 0 : i64}>", None)]):
+        x = rng.standard_normal(shape).astype(np.float32)
+        ty, out_ty = ("tensor<" + "x".join(map(str, s)) + "xf32>" for s in (shape, out or shape))
+        text = module(ty, hexed(x), op, props, out_ty, f"f{k}")
+        alone[f"f{k}"] = result(text, name=f"f{k}")[0].const.bits
+        parts.append(text.split("\n", 1)[1].rsplit("}) : () -> ()", 1)[0])
+    out, stats = opt.run('"builtin.module"() ({\n' + "".join(parts) + "}) : () -> ()\n", PIPELINE, n_gpus=1)
+    assert stats["folds"] == len(alone)
+    funcs = parse_funcs(out)
+    for name, bits in alone.items():
+        f = funcs[name]
+        assert f.defs[f.ret.operands[0]].const.bits == bits
