@@ -591,12 +591,17 @@ def _host_out(out, n: int, dtype: str) -> np.ndarray:
     return out.reshape(-1)
 
 
+_CURRENT_STREAM: list = []
+
+
 def _own_stream(stream, t) -> int:
     """The given stream, or the current one of the tensor's device."""
     if stream is None:
-        import torch
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object: 2 us less
-        return raw(t.get_device()) if raw else torch.cuda.current_stream(t.device).cuda_stream
+        if not _CURRENT_STREAM:
+            import torch
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object: 2 us less
+            _CURRENT_STREAM.append(raw or (lambda device: torch.cuda.current_stream(device).cuda_stream))
+        return _CURRENT_STREAM[0](t.get_device())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
