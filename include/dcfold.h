@@ -550,6 +550,104 @@ int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in,
                             size_t workspace_bytes, dcf_status* status,
                             void* stream);
 
+/* ---- operators on 8-bit integers --------------------------------------
+ *
+ * Matrices as whole numbers from -127 to 127 with a f32 scale beside them: a
+ * learned weight, a layer's activations, the checkpoint that a training step
+ * keeps of them, and the products that read these.  They never refuse. */
+
+#define DCF_QUANT_ROWS 0u    /* a scale for each row */
+#define DCF_QUANT_COLUMNS 1u /* a scale for each column of each run of rows */
+#define DCF_QUANT_RUN 128    /* rows of a run; the last one may be shorter */
+
+/* A matrix and its 8-bit form.  With m the largest magnitude beside a value (of
+ * its row, or of its column in its run), and both quotients rounded to f32,
+ *     scale = m / 127,   q = the whole number nearest x * (127 / m)
+ * (the exact product, ties to even).  m below 2^-119 counts as 0: scale and
+ * whole numbers are 0.  Beside a NaN or an infinity the scale is NaN and the
+ * whole numbers are 0, so that all that is made from them is NaN.  Read back, a
+ * whole number is q * scale, rounded to f32 and from there to dtype.
+ * Scales are dense: [rows], or [ceil(rows / DCF_QUANT_RUN)][cols].  Strides are in
+ * elements, 0 means dense; columns are contiguous. */
+typedef struct dcf_quant_desc {
+  uint32_t dtype;       /* of the values: DCF_F16, BF16 or F32 */
+  uint32_t along;       /* DCF_QUANT_ROWS or DCF_QUANT_COLUMNS */
+  uint64_t rows, cols;  /* < 2^31; cols <= 2^31 - 65536 */
+  int64_t row_stride;   /* of the values */
+  int64_t q_row_stride; /* of the whole numbers */
+} dcf_quant_desc;
+
+#define DCF_INT8_MAX_DEPTH 131071
+
+/* The product of tokens a [tokens][depth] and a weight b [channels][depth]:
+ *     out[t][c] = (sum over k of a[t][k] * b[c][k]) * a_scale[t] * b_scale[c] + bias[c].
+ * Sums are exact; they are rounded to f32, and so is each step after that, in
+ * this order; the result is rounded once more to a 16-bit type.  Tokens of a
+ * float type are quantised by rows within the call, as dcf_quantize does.
+ * With out_dtype DCF_I32 the sums themselves are the result (a must be i8; no
+ * scales, no bias).  Whole numbers of a and b may be -128. */
+typedef struct dcf_int8_desc {
+  uint32_t a_dtype;   /* DCF_I8, or DCF_F16, BF16, F32 */
+  uint32_t out_dtype; /* DCF_F16, BF16, F32 or I32 */
+  uint64_t tokens, channels; /* <= 2^31 - 65536 */
+  uint64_t depth;            /* <= DCF_INT8_MAX_DEPTH */
+  int64_t a_row_stride, b_row_stride, out_row_stride; /* in elements; 0: dense */
+} dcf_int8_desc;
+
+#define DCF_CHECKPOINT_ACCUMULATE 1u /* add to what out (f32) holds */
+
+/* The gradient of a weight [channels][depth] whose layer's input was kept as a
+ * checkpoint (dcf_quantize with DCF_QUANT_COLUMNS) of [tokens][depth]:
+ *     out[c][k] = sum over t of grad[t][c] * (q[t][k] * scale[t / DCF_QUANT_RUN][k]).
+ * Products of the whole numbers are exact; a run's sum is multiplied by its scale
+ * and added in f32; the result is rounded once more to a 16-bit type.  Without
+ * tokens it is 0. */
+typedef struct dcf_checkpoint_desc {
+  uint32_t grad_dtype; /* DCF_F16 or BF16 */
+  uint32_t out_dtype;  /* DCF_F32, F16 or BF16 */
+  uint32_t flags;      /* DCF_CHECKPOINT_* */
+  uint32_t reserved;   /* 0 */
+  uint64_t tokens, channels, depth; /* <= 2^31 - 65536 */
+  int64_t grad_row_stride, q_row_stride, out_row_stride; /* in elements; 0: dense */
+} dcf_checkpoint_desc;
+
+/* Host forms: host pointers, dense tensors (strides 0). */
+int dcf_quantize(const dcf_quant_desc* desc, const void* in, int8_t* q,
+                 float* scale, dcf_result* res);
+int dcf_dequantize(const dcf_quant_desc* desc, const int8_t* q,
+                   const float* scale, void* out, dcf_result* res);
+int dcf_int8_matmul(const dcf_int8_desc* desc, const void* a,
+                    const float* a_scale, const int8_t* b,
+                    const float* b_scale, const float* bias, void* out,
+                    dcf_result* res);
+int dcf_checkpoint_grad(const dcf_checkpoint_desc* desc, const void* grad,
+                        const int8_t* q, const float* scale, void* out,
+                        dcf_result* res);
+
+/* Device forms: device pointers of one device, work queued on `stream` of
+ * that device, the caller's current device kept.  Elements between rows that a
+ * stride leaves out are not written.  Results must not overlap operands
+ * (checked).  a_scale is NULL where a is of a float type; bias may be NULL.
+ * Workspace and status are as for dcf_orthogonalize_async.  Sums run in a fixed
+ * order: the same call gives the same bits. */
+int dcf_quantize_async(const dcf_quant_desc* desc, const void* in, int8_t* q,
+                       float* scale, void* stream);
+int dcf_dequantize_async(const dcf_quant_desc* desc, const int8_t* q,
+                         const float* scale, void* out, void* stream);
+int dcf_int8_matmul_workspace(const dcf_int8_desc* desc, size_t* bytes);
+int dcf_int8_matmul_async(const dcf_int8_desc* desc, const void* a,
+                          const float* a_scale, const int8_t* b,
+                          const float* b_scale, const float* bias, void* out,
+                          void* workspace, size_t workspace_bytes,
+                          dcf_status* status, void* stream);
+int dcf_checkpoint_grad_workspace(const dcf_checkpoint_desc* desc,
+                                  size_t* bytes);
+int dcf_checkpoint_grad_async(const dcf_checkpoint_desc* desc,
+                              const void* grad, const int8_t* q,
+                              const float* scale, void* out, void* workspace,
+                              size_t workspace_bytes, dcf_status* status,
+                              void* stream);
+
 #ifdef __cplusplus
 }
 #endif

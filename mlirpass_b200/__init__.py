@@ -110,10 +110,29 @@ class OrthDesc(ctypes.Structure):
                 ("coef", (ctypes.c_double * 3) * ORTH_MAX_STEPS)]
 
 
+class QuantDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("along", ctypes.c_uint32), ("rows", ctypes.c_uint64),
+                ("cols", ctypes.c_uint64), ("row_stride", ctypes.c_int64), ("q_row_stride", ctypes.c_int64)]
+
+
+class Int8Desc(ctypes.Structure):
+    _fields_ = [("a_dtype", ctypes.c_uint32), ("out_dtype", ctypes.c_uint32), ("tokens", ctypes.c_uint64),
+                ("channels", ctypes.c_uint64), ("depth", ctypes.c_uint64), ("a_row_stride", ctypes.c_int64),
+                ("b_row_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64)]
+
+
+class CheckpointDesc(ctypes.Structure):
+    _fields_ = [("grad_dtype", ctypes.c_uint32), ("out_dtype", ctypes.c_uint32), ("flags", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32), ("tokens", ctypes.c_uint64), ("channels", ctypes.c_uint64),
+                ("depth", ctypes.c_uint64), ("grad_row_stride", ctypes.c_int64), ("q_row_stride", ctypes.c_int64),
+                ("out_row_stride", ctypes.c_int64)]
+
+
 # Every symbol include/dcfold.h declares, with its ctypes signature.
 _VP, _U64, _I, _U32, _SZ = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t
 _RP, _SP = ctypes.POINTER(Result), ctypes.POINTER(Status)
 _BP, _OP, _SZP = ctypes.POINTER(BiasDesc), ctypes.POINTER(OrthDesc), ctypes.POINTER(ctypes.c_size_t)
+_QP, _IP, _CP = ctypes.POINTER(QuantDesc), ctypes.POINTER(Int8Desc), ctypes.POINTER(CheckpointDesc)
 SIGNATURES = {
     "dcf_init": (_I, [_I]),
     "dcf_shutdown": (_I, []),
@@ -156,6 +175,16 @@ SIGNATURES = {
     "dcf_position_bias_grad_async": (_I, [_BP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "dcf_orthogonalize_workspace": (_I, [_OP, _SZP]),
     "dcf_orthogonalize_async": (_I, [_OP, _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dcf_quantize": (_I, [_QP, _VP, _VP, _VP, _RP]),
+    "dcf_dequantize": (_I, [_QP, _VP, _VP, _VP, _RP]),
+    "dcf_int8_matmul": (_I, [_IP, _VP, _VP, _VP, _VP, _VP, _VP, _RP]),
+    "dcf_checkpoint_grad": (_I, [_CP, _VP, _VP, _VP, _VP, _RP]),
+    "dcf_quantize_async": (_I, [_QP, _VP, _VP, _VP, _VP]),
+    "dcf_dequantize_async": (_I, [_QP, _VP, _VP, _VP, _VP]),
+    "dcf_int8_matmul_workspace": (_I, [_IP, _SZP]),
+    "dcf_int8_matmul_async": (_I, [_IP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP]),
+    "dcf_checkpoint_grad_workspace": (_I, [_CP, _SZP]),
+    "dcf_checkpoint_grad_async": (_I, [_CP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP, _VP]),
 }
 
 _lib = None
@@ -617,7 +646,7 @@ def _typed(t, what: str, dtype: str) -> None:
     """Refuse a tensor whose elements are not of the given type (another of the same size would be read as it)."""
     if not _TORCH_TYPES:
         import torch
-        _TORCH_TYPES.update(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32, f64=torch.float64, i32=torch.int32)
+        _TORCH_TYPES.update(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32, f64=torch.float64, i32=torch.int32, i8=torch.int8)
     if t.dtype is not _TORCH_TYPES[dtype]:
         raise ValueError(f"{what}: {t.dtype}, {dtype} expected")
 
@@ -791,3 +820,232 @@ def orthogonalize_async(plan: OrthPlan, x, out, workspace, status, *, stream=Non
         plan.ref, _need_layout(x, "x", plan.in_elements, plan.dtype, *plan.in_layout),
         _need_layout(out, "out", plan.out_elements, plan.out_dtype, *plan.out_layout), workspace.data_ptr(),
         _bytes(workspace), _need(status, "status", 2, None), _own_stream(stream, out)))
+
+
+# -------------------------------------------- operators on 8-bit integers
+
+QUANT_RUN = 128                                        # rows of a run that shares a scale for each column
+QUANT_ALONG = {"rows": 0, "columns": 1}
+INT8_MAX_DEPTH = 131071
+CHECKPOINT_ACCUMULATE = 1
+
+
+def _rows(rows: int, cols: int, stride: int) -> tuple:
+    """A matrix as (elements from its first to its last, shape, strides)."""
+    stride = stride or cols
+    return (rows - 1) * stride + cols if rows and cols else 0, (rows, cols), (stride, 1)
+
+
+def _fits(limit: int, **sizes) -> None:
+    for name, v in sizes.items():
+        if not 0 <= v < limit:
+            raise ValueError(f"{name} {v} out of range")
+
+
+def _vector(t, what: str, elements: int):
+    return None if t is None else _need(t, what, elements, "f32")
+
+
+class QuantPlan:
+    """The sizes, type and strides of a matrix and its 8-bit form: a
+    dcf_quant_desc that calls reuse."""
+
+    def __init__(self, desc: QuantDesc, dtype: str):
+        self.desc, self.dtype = desc, dtype
+        self.ref = ctypes.byref(desc)
+        self.values = _rows(desc.rows, desc.cols, desc.row_stride)
+        self.levels = _rows(desc.rows, desc.cols, desc.q_row_stride)
+        self.scale_shape = (desc.rows,) if desc.along == 0 else (-(-desc.rows // QUANT_RUN), desc.cols)
+        self.scales = math.prod(self.scale_shape)
+
+
+def quantize_plan(dtype: str, rows: int, cols: int, *, along: str = "rows", row_stride: int = 0,
+                  q_row_stride: int = 0) -> QuantPlan:
+    """Describe a matrix [rows, cols] of f16, bf16 or f32 and its 8-bit form
+    (dcf_quant_desc, include/dcfold.h).
+
+    `along` "rows" has a scale for each row, [rows]; "columns" one for each
+    column of each run of 128 rows, [ceil(rows / 128), cols]: a checkpoint of
+    activations.  Strides are in elements, 0 is dense.
+    """
+    _fits(1 << 31, rows=rows, cols=cols)
+    _fits(1 << 62, row_stride=row_stride, q_row_stride=q_row_stride)
+    plan = QuantPlan(QuantDesc(DTYPES[dtype], QUANT_ALONG[along], rows, cols, row_stride, q_row_stride), dtype)
+    if dtype not in ("f16", "bf16", "f32"):
+        raise ValueError(f"dtype {dtype}: f16, bf16 or f32 expected")
+    return plan
+
+
+def quantize(plan: QuantPlan, x) -> tuple:
+    """(Fold of int8 [rows, cols], f32 scales) of a matrix on host buffers."""
+    d = plan.desc
+    a = as_storage(x, plan.dtype)
+    if len(a) != d.rows * d.cols:
+        raise ValueError(f"input has {len(a)} elements, {d.rows * d.cols} expected")
+    q, scale, res = np.empty((d.rows, d.cols), np.int8), np.empty(plan.scale_shape, np.float32), Result()
+    _check(lib().dcf_quantize(plan.ref, _ptr(a), _ptr(q), _ptr(scale), ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), q), scale
+
+
+def dequantize(plan: QuantPlan, q, scale, *, out: np.ndarray | None = None) -> Fold:
+    """The values [rows, cols] that whole numbers and scales stand for, on host buffers."""
+    d = plan.desc
+    n = d.rows * d.cols
+    a, s = _host_array(q, "q", n, np.int8), _host_array(scale, "scale", plan.scales, np.float32)
+    out = _host_out(out, n, plan.dtype)
+    res = Result()
+    _check(lib().dcf_dequantize(plan.ref, _ptr(a), _ptr(s), _ptr(out), ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), out.reshape(d.rows, d.cols))
+
+
+def _host_array(x, what: str, n: int, dtype) -> np.ndarray:
+    a = np.ascontiguousarray(x).reshape(-1)
+    if a.dtype != dtype or a.size != n:
+        raise ValueError(f"{what}: {a.size} elements of {a.dtype}, {n} of {np.dtype(dtype)} expected")
+    return a
+
+
+def quantize_async(plan: QuantPlan, x, q, scale, *, stream=None) -> None:
+    """Launch a quantisation on device tensors: `x` and the int8 `q` lie as the
+    plan's strides say, the f32 `scale` is dense, of the plan's scale_shape."""
+    _check(lib().dcf_quantize_async(
+        plan.ref, _need_layout(x, "x", plan.values[0], plan.dtype, *plan.values[1:]),
+        _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]), _need(scale, "scale", plan.scales, "f32"),
+        _own_stream(stream, q)))
+
+
+def dequantize_async(plan: QuantPlan, q, scale, out, *, stream=None) -> None:
+    """Launch the reading back of what quantize_async wrote, into `out` as the plan's strides say."""
+    _check(lib().dcf_dequantize_async(
+        plan.ref, _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]),
+        _need(scale, "scale", plan.scales, "f32"),
+        _need_layout(out, "out", plan.values[0], plan.dtype, *plan.values[1:]), _own_stream(stream, out)))
+
+
+class Int8Plan:
+    """The sizes, types and strides of one 8-bit product: a dcf_int8_desc that
+    calls reuse.  Validated when made."""
+
+    def __init__(self, desc: Int8Desc, a_dtype: str, out_dtype: str):
+        self.desc, self.a_dtype, self.out_dtype = desc, a_dtype, out_dtype
+        self.ref = ctypes.byref(desc)
+        self.a = _rows(desc.tokens, desc.depth, desc.a_row_stride)
+        self.b = _rows(desc.channels, desc.depth, desc.b_row_stride)
+        self.out = _rows(desc.tokens, desc.channels, desc.out_row_stride)
+        ws = ctypes.c_size_t(0)
+        _check(lib().dcf_int8_matmul_workspace(self.ref, ctypes.byref(ws)))
+        self.workspace = ws.value
+
+
+def int8_matmul_plan(tokens: int, channels: int, depth: int, *, a_dtype: str = "i8", out_dtype: str = "bf16",
+                     a_row_stride: int = 0, b_row_stride: int = 0, out_row_stride: int = 0) -> Int8Plan:
+    """Describe the product of tokens [tokens, depth] and an int8 weight
+    [channels, depth] (dcf_int8_desc, include/dcfold.h).
+
+    Tokens are i8 with a scale each, or f16, bf16 or f32, which the call
+    quantises by rows.  The result [tokens, channels] is f16, bf16 or f32, or,
+    of i8 tokens, the i32 sums.  Strides are in elements, 0 is dense.
+    """
+    _fits(1 << 31, tokens=tokens, channels=channels, depth=depth)
+    _fits(1 << 62, a_row_stride=a_row_stride, b_row_stride=b_row_stride, out_row_stride=out_row_stride)
+    return Int8Plan(Int8Desc(DTYPES[a_dtype], DTYPES[out_dtype], tokens, channels, depth, a_row_stride, b_row_stride,
+                             out_row_stride), a_dtype, out_dtype)
+
+
+def int8_matmul(plan: Int8Plan, a, b, *, a_scale=None, b_scale=None, bias=None, out: np.ndarray | None = None) -> Fold:
+    """The product [tokens, channels] on host buffers."""
+    d = plan.desc
+    x = as_storage(a, plan.a_dtype)
+    if len(x) != d.tokens * d.depth:
+        raise ValueError(f"a has {len(x)} elements, {d.tokens * d.depth} expected")
+    w = _host_array(b, "b", d.channels * d.depth, np.int8)
+    given = [None if v is None else _host_array(v, what, n, np.float32)
+             for v, what, n in ((a_scale, "a_scale", d.tokens), (b_scale, "b_scale", d.channels), (bias, "bias", d.channels))]
+    sa, sb, add = (None if v is None else _ptr(v) for v in given)
+    out = _host_out(out, d.tokens * d.channels, plan.out_dtype)
+    res = Result()
+    _check(lib().dcf_int8_matmul(plan.ref, _ptr(x), sa, _ptr(w), sb, add, _ptr(out), ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), out.reshape(d.tokens, d.channels))
+
+
+def int8_matmul_workspace(plan: Int8Plan) -> int:
+    """Bytes of device workspace that a call of this plan needs."""
+    return plan.workspace
+
+
+def int8_matmul_async(plan: Int8Plan, a, b, out, workspace, status, *, a_scale=None, b_scale=None, bias=None,
+                      stream=None) -> None:
+    """Launch an 8-bit product on device tensors: `a`, the int8 weight `b` and
+    `out` lie as the plan's strides say; `a_scale` [tokens] (of i8 tokens),
+    `b_scale` and `bias` [channels] are dense f32.  `status` (16 bytes, reset
+    first) takes a kernel's error report."""
+    d = plan.desc
+    _check(lib().dcf_int8_matmul_async(
+        plan.ref, _need_layout(a, "a", plan.a[0], plan.a_dtype, *plan.a[1:]), _vector(a_scale, "a_scale", d.tokens),
+        _need_layout(b, "b", plan.b[0], "i8", *plan.b[1:]), _vector(b_scale, "b_scale", d.channels),
+        _vector(bias, "bias", d.channels), _need_layout(out, "out", plan.out[0], plan.out_dtype, *plan.out[1:]),
+        workspace.data_ptr(), _bytes(workspace), _need(status, "status", 2, None), _own_stream(stream, out)))
+
+
+class CheckpointPlan:
+    """The sizes, types and strides of one weight gradient from a checkpoint: a
+    dcf_checkpoint_desc that calls reuse.  Validated when made."""
+
+    def __init__(self, desc: CheckpointDesc, dtype: str, out_dtype: str):
+        self.desc, self.dtype, self.out_dtype = desc, dtype, out_dtype
+        self.ref = ctypes.byref(desc)
+        self.grad = _rows(desc.tokens, desc.channels, desc.grad_row_stride)
+        self.levels = _rows(desc.tokens, desc.depth, desc.q_row_stride)
+        self.out = _rows(desc.channels, desc.depth, desc.out_row_stride)
+        self.scale_shape = -(-desc.tokens // QUANT_RUN), desc.depth
+        self.scales = math.prod(self.scale_shape)
+        ws = ctypes.c_size_t(0)
+        _check(lib().dcf_checkpoint_grad_workspace(self.ref, ctypes.byref(ws)))
+        self.workspace = ws.value
+
+
+def checkpoint_grad_plan(dtype: str, tokens: int, channels: int, depth: int, *, out_dtype: str = "f32",
+                         grad_row_stride: int = 0, q_row_stride: int = 0, out_row_stride: int = 0,
+                         accumulate: bool = False) -> CheckpointPlan:
+    """Describe the gradient [channels, depth] of a weight from the f16 or bf16
+    gradient [tokens, channels] of its layer's output and the checkpoint
+    [tokens, depth] of its input, quantised along columns (dcf_checkpoint_desc,
+    include/dcfold.h).  Strides are in elements, 0 is dense.  `accumulate` adds
+    to what a f32 result holds.
+    """
+    _fits(1 << 31, tokens=tokens, channels=channels, depth=depth)
+    _fits(1 << 62, grad_row_stride=grad_row_stride, q_row_stride=q_row_stride, out_row_stride=out_row_stride)
+    flags = CHECKPOINT_ACCUMULATE if accumulate else 0
+    return CheckpointPlan(CheckpointDesc(DTYPES[dtype], DTYPES[out_dtype], flags, 0, tokens, channels, depth,
+                                         grad_row_stride, q_row_stride, out_row_stride), dtype, out_dtype)
+
+
+def checkpoint_grad(plan: CheckpointPlan, grad, q, scale, *, out: np.ndarray | None = None) -> Fold:
+    """The gradient [channels, depth] on host buffers.  With an accumulating plan `out` is added to."""
+    d = plan.desc
+    g = as_storage(grad, plan.dtype)
+    if len(g) != d.tokens * d.channels:
+        raise ValueError(f"gradient has {len(g)} elements, {d.tokens * d.channels} expected")
+    if out is None and d.flags & CHECKPOINT_ACCUMULATE:
+        raise ValueError("an accumulating plan needs `out`")
+    a, s = _host_array(q, "q", d.tokens * d.depth, np.int8), _host_array(scale, "scale", plan.scales, np.float32)
+    out = _host_out(out, d.channels * d.depth, plan.out_dtype)
+    res = Result()
+    _check(lib().dcf_checkpoint_grad(plan.ref, _ptr(g), _ptr(a), _ptr(s), _ptr(out), ctypes.byref(res)))
+    return Fold(bool(res.folded), bool(res.is_splat), int(res.first_fail_index), out.reshape(d.channels, d.depth))
+
+
+def checkpoint_grad_workspace(plan: CheckpointPlan) -> int:
+    """Bytes of device workspace that a call of this plan needs."""
+    return plan.workspace
+
+
+def checkpoint_grad_async(plan: CheckpointPlan, grad, q, scale, out, workspace, status, *, stream=None) -> None:
+    """Launch a weight gradient on device tensors: `grad`, the int8 `q` and `out`
+    lie as the plan's strides say, the f32 `scale` is dense, of the plan's
+    scale_shape.  `status` (16 bytes, reset first) takes a kernel's error report."""
+    _check(lib().dcf_checkpoint_grad_async(
+        plan.ref, _need_layout(grad, "grad", plan.grad[0], plan.dtype, *plan.grad[1:]),
+        _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]), _need(scale, "scale", plan.scales, "f32"),
+        _need_layout(out, "out", plan.out[0], plan.out_dtype, *plan.out[1:]), workspace.data_ptr(), _bytes(workspace),
+        _need(status, "status", 2, None), _own_stream(stream, out)))

@@ -115,6 +115,20 @@ size_t orth_workspace(const dcf_orth_desc& d);
 int launch_orthogonalize(const dcf_orth_desc& d, const void* in, void* out, void* ws, dcf_status* st,
                          cudaStream_t stream);
 
+// Operators on 8-bit integers, in the same manner.  `back`: for reading back, whose rows must not overlap.
+int quant_desc_check(const dcf_quant_desc* d, bool back);
+int launch_quantize(const dcf_quant_desc& d, const void* in, int8_t* q, float* scale, cudaStream_t stream);
+int launch_dequantize(const dcf_quant_desc& d, const int8_t* q, const float* scale, void* out, cudaStream_t stream);
+int int8_desc_check(const dcf_int8_desc* d);
+size_t int8_workspace(const dcf_int8_desc& d);
+int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_scale, const int8_t* b,
+                       const float* b_scale, const float* bias, void* out, void* ws, dcf_status* st,
+                       cudaStream_t stream);
+int checkpoint_desc_check(const dcf_checkpoint_desc* d);
+size_t checkpoint_workspace(const dcf_checkpoint_desc& d);
+int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const int8_t* q, const float* scale,
+                           void* out, void* ws, dcf_status* st, cudaStream_t stream);
+
 // Set the per-thread text dcf_last_error() returns; returns `code`.
 int record_error(int code, const char* msg);
 

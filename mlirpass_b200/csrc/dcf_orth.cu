@@ -33,9 +33,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include <mutex>
-
-#include "dcf_kernels.cuh"
+#include "dcf_tensor.cuh"
 
 namespace dcf {
 
@@ -60,61 +58,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
       ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
       : "memory");
-}
-
-// Products are made by pairs of CTAs (clusters of two): one instruction
-// multiplies what both have loaded, into the TMEM of both.
-__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Arrives on this barrier of both CTAs once the products issued before are done.
-__device__ __forceinline__ void pair_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_addr(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-
-__device__ __forceinline__ uint32_t pair_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-__device__ __forceinline__ void pair_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// Arrives on the first CTA's barrier, from either.
-__device__ __forceinline__ void arrive_first(uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(
-          smem_addr(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-}
-
-// Until the loads issued before have arrived; `r` is named so that no use of it moves ahead.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[j]));
 }
 
 // 384 threads start with 168 registers each; the first four warps keep 40 and
@@ -1198,24 +1141,6 @@ __global__ void __launch_bounds__(kFewThreads, 1) orth_few_kernel(const __grid_c
 
 // ---------------------------------------------------------------- host
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encoder() {
-  static EncodeTiled fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = (EncodeTiled)p;
-    cudaGetLastError();
-  });
-  return fn;
-}
-
 // Boxes of 64 columns x 64 rows of one plane; what lies beyond the matrix
 // reads as zero.
 bool encode(CUtensorMap* map, const Planes& x, int cols, uint64_t batch) {
@@ -1387,27 +1312,6 @@ Layout layout_of(const dcf_orth_desc& d, void* ws) {
   l.sums = d.steps && sums ? (float*)take(sums) : nullptr;
   l.bytes = off;
   return l;
-}
-
-// Launches as a programmatic dependent (unless DCF_PDL=0): the kernel's start overlaps
-// the end of the one before it, whose results it reads only after griddepcontrol.wait.
-template <class... P, class... A>
-int launch(void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster, cudaStream_t s, const A&... args) {
-  cudaLaunchConfig_t c = {};
-  c.gridDim = grid;
-  c.blockDim = dim3((unsigned)threads);
-  c.dynamicSmemBytes = (size_t)smem;
-  c.stream = s;
-  cudaLaunchAttribute a[2];
-  a[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
-  a[1].id = cudaLaunchAttributeClusterDimension;
-  a[1].val.clusterDim.x = (unsigned)cluster;
-  a[1].val.clusterDim.y = a[1].val.clusterDim.z = 1;
-  c.attrs = a;
-  c.numAttrs = cluster > 1 ? 2 : 1;
-  note_launch();
-  return cudaLaunchKernelEx(&c, kernel, args...) == cudaSuccess ? DCF_OK : DCF_ECUDA;
 }
 
 // CTAs of a cluster that take a matrix of few rows at once, 0 where it does not

@@ -1397,3 +1397,305 @@ int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in, void* out
 }
 
 }  // extern "C"
+
+// ------------------------------------------- operators on 8-bit integers
+
+namespace {
+
+// Bytes from the first element of rows to behind the last one, 0 without any.
+size_t rows_bytes(uint64_t rows, uint64_t cols, int64_t stride, size_t es) {
+  if (!rows || !cols) return 0;
+  return (size_t)((rows - 1) * (uint64_t)(stride ? stride : (int64_t)cols) + cols) * es;
+}
+
+struct Span {
+  const void* p;
+  size_t bytes;
+};
+
+// No result may share memory with an operand or another result.
+int apart(std::initializer_list<Span> results, std::initializer_list<Span> operands) {
+  auto meet = [](const Span& a, const Span& b) {
+    return a.bytes && b.bytes && (const char*)a.p < (const char*)b.p + b.bytes && (const char*)b.p < (const char*)a.p + a.bytes;
+  };
+  for (const Span* r = results.begin(); r != results.end(); r++) {
+    for (const Span& o : operands)
+      if (meet(*r, o)) return set_err(DCF_EINVAL, "a result overlaps an operand");
+    for (const Span* o = r + 1; o != results.end(); o++)
+      if (meet(*r, *o)) return set_err(DCF_EINVAL, "results overlap");
+  }
+  return DCF_OK;
+}
+
+uint64_t scale_count(const dcf_quant_desc& q) {
+  return q.along == DCF_QUANT_ROWS ? q.rows : (q.rows + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN * q.cols;
+}
+
+// Parts of one device buffer, each on a multiple of 256 bytes.
+struct Parts {
+  size_t total = 0;
+  size_t take(size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+int dcf_quantize_async(const dcf_quant_desc* desc, const void* in, int8_t* q, float* scale, void* stream) {
+  int rc = quant_desc_check(desc, false);
+  if (rc) return rc;
+  const dcf_quant_desc& d = *desc;
+  const uint64_t scales = scale_count(d);
+  if (!scales) return DCF_OK;
+  if (!scale || (d.cols && (!in || !q))) return set_err(DCF_EINVAL, "null pointer");
+  const size_t es = dtype_size((int)d.dtype);
+  if ((rc = apart({{q, rows_bytes(d.rows, d.cols, d.q_row_stride, 1)}, {scale, scales * 4}},
+                  {{in, rows_bytes(d.rows, d.cols, d.row_stride, es)}})))
+    return rc;
+  OnDevice on;
+  if ((rc = on.enter({{scale, 4}, {q, 1}, {in, es}}))) return rc;
+  rc = launch_quantize(d, in, q, scale, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "quantize") : DCF_OK;
+}
+
+int dcf_dequantize_async(const dcf_quant_desc* desc, const int8_t* q, const float* scale, void* out, void* stream) {
+  int rc = quant_desc_check(desc, true);
+  if (rc) return rc;
+  const dcf_quant_desc& d = *desc;
+  if (!d.rows || !d.cols) return DCF_OK;
+  if (!q || !scale || !out) return set_err(DCF_EINVAL, "null pointer");
+  const size_t es = dtype_size((int)d.dtype);
+  if ((rc = apart({{out, rows_bytes(d.rows, d.cols, d.row_stride, es)}},
+                  {{q, rows_bytes(d.rows, d.cols, d.q_row_stride, 1)}, {scale, scale_count(d) * 4}})))
+    return rc;
+  OnDevice on;
+  if ((rc = on.enter({{out, es}, {q, 1}, {scale, 4}}))) return rc;
+  rc = launch_dequantize(d, q, scale, out, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "dequantize") : DCF_OK;
+}
+
+int dcf_quantize(const dcf_quant_desc* desc, const void* in, int8_t* q, float* scale, dcf_result* res) {
+  int rc = quant_desc_check(desc, false);
+  if (rc) return rc;
+  const dcf_quant_desc& d = *desc;
+  if (!dense_strides({d.row_stride, d.q_row_stride})) return set_err(DCF_EINVAL, "quantize: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = d.rows * d.cols, scales = scale_count(d);
+  if (!scales) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if (!scale || (n && (!in || !q))) return set_err(DCF_EINVAL, "null buffer");
+  const size_t bytes = n * dtype_size((int)d.dtype);
+  Parts parts;
+  const size_t at_in = parts.take(bytes), at_q = parts.take(n), at_scale = parts.take(scales * 4);
+  Dev& dev = *g_devs[0];
+  std::lock_guard<std::mutex> g(dev.mu);
+  CK(cudaSetDevice(dev.id));
+  if ((rc = ensure_big(dev, 0, parts.total))) return rc;
+  cudaStream_t s = dev.s[0];
+  uint8_t* base = (uint8_t*)dev.big[0];
+  if ((rc = h2d_full(dev, base + at_in, in, bytes, s))) return rc;
+  if ((rc = launch_quantize(d, base + at_in, (int8_t*)base + at_q, (float*)(base + at_scale), s)))
+    return learned_launch_failed(rc, "quantize");
+  if ((rc = d2h_full(dev, q, base + at_q, n, s)) || (rc = d2h_full(dev, scale, base + at_scale, scales * 4, s))) return rc;
+  return learned_splat(dev, base + at_q, 1, n, s, res);
+}
+
+int dcf_dequantize(const dcf_quant_desc* desc, const int8_t* q, const float* scale, void* out, dcf_result* res) {
+  int rc = quant_desc_check(desc, true);
+  if (rc) return rc;
+  const dcf_quant_desc& d = *desc;
+  if (!dense_strides({d.row_stride, d.q_row_stride})) return set_err(DCF_EINVAL, "dequantize: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = d.rows * d.cols, scales = scale_count(d);
+  if (!n) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if (!q || !scale || !out) return set_err(DCF_EINVAL, "null buffer");
+  const size_t es = dtype_size((int)d.dtype);
+  Parts parts;
+  const size_t at_out = parts.take(n * es), at_q = parts.take(n), at_scale = parts.take(scales * 4);
+  Dev& dev = *g_devs[0];
+  std::lock_guard<std::mutex> g(dev.mu);
+  CK(cudaSetDevice(dev.id));
+  if ((rc = ensure_big(dev, 0, parts.total))) return rc;
+  cudaStream_t s = dev.s[0];
+  uint8_t* base = (uint8_t*)dev.big[0];
+  if ((rc = h2d_full(dev, base + at_q, q, n, s)) || (rc = h2d_full(dev, base + at_scale, scale, scales * 4, s))) return rc;
+  if ((rc = launch_dequantize(d, (int8_t*)base + at_q, (float*)(base + at_scale), base + at_out, s)))
+    return learned_launch_failed(rc, "dequantize");
+  if ((rc = d2h_full(dev, out, base + at_out, n * es, s))) return rc;
+  return learned_splat(dev, base + at_out, es, n, s, res);
+}
+
+}  // extern "C"
+
+namespace {
+
+// What a call of the 8-bit product needs beside its descriptor.
+int int8_pointers(const dcf_int8_desc& d, const void* a, const float* a_scale, const int8_t* b, const float* b_scale,
+                  const float* bias, const void* out) {
+  const bool sums = d.out_dtype == DCF_I32, ints = d.a_dtype == DCF_I8;
+  if (!out || (d.depth && (!a || !b)) || (!sums && !b_scale) || (!sums && ints && !a_scale))
+    return set_err(DCF_EINVAL, "null pointer");
+  if (sums && (a_scale || b_scale || bias)) return set_err(DCF_EINVAL, "int8 matmul: sums take no scales and no bias");
+  if (!ints && a_scale) return set_err(DCF_EINVAL, "int8 matmul: tokens that the call quantises have no scales yet");
+  return DCF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int dcf_int8_matmul_workspace(const dcf_int8_desc* desc, size_t* bytes) {
+  int rc = int8_desc_check(desc);
+  if (rc) return rc;
+  if (!bytes) return set_err(DCF_EINVAL, "null result");
+  *bytes = int8_workspace(*desc);
+  return DCF_OK;
+}
+
+int dcf_int8_matmul_async(const dcf_int8_desc* desc, const void* a, const float* a_scale, const int8_t* b,
+                          const float* b_scale, const float* bias, void* out, void* workspace, size_t workspace_bytes,
+                          dcf_status* status, void* stream) {
+  int rc = int8_desc_check(desc);
+  if (rc) return rc;
+  const dcf_int8_desc& d = *desc;
+  if (!d.tokens || !d.channels) return DCF_OK;
+  if ((rc = int8_pointers(d, a, a_scale, b, b_scale, bias, out))) return rc;
+  const size_t ws = int8_workspace(d), es = dtype_size((int)d.a_dtype), oes = dtype_size((int)d.out_dtype);
+  if (!status || (ws && !workspace)) return set_err(DCF_EINVAL, "null pointer");
+  if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
+  if ((rc = apart({{out, rows_bytes(d.tokens, d.channels, d.out_row_stride, oes)}, {workspace, ws}, {status, sizeof *status}},
+                  {{a, rows_bytes(d.tokens, d.depth, d.a_row_stride, es)},
+                   {b, rows_bytes(d.channels, d.depth, d.b_row_stride, 1)},
+                   {a_scale, a_scale ? d.tokens * 4 : 0},
+                   {b_scale, b_scale ? d.channels * 4 : 0},
+                   {bias, bias ? d.channels * 4 : 0}})))
+    return rc;
+  OnDevice on;
+  if ((rc = on.enter({{out, oes}, {a, es}, {b, 1}, {a_scale, 4}, {b_scale, 4}, {bias, 4}, {ws ? workspace : nullptr, 256},
+                      {status, 8}})))
+    return rc;
+  rc = launch_int8_matmul(d, a, a_scale, b, b_scale, bias, out, workspace, status, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "int8 matmul") : DCF_OK;
+}
+
+int dcf_int8_matmul(const dcf_int8_desc* desc, const void* a, const float* a_scale, const int8_t* b,
+                    const float* b_scale, const float* bias, void* out, dcf_result* res) {
+  int rc = int8_desc_check(desc);
+  if (rc) return rc;
+  const dcf_int8_desc& d = *desc;
+  if (!dense_strides({d.a_row_stride, d.b_row_stride, d.out_row_stride}))
+    return set_err(DCF_EINVAL, "int8 matmul: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = d.tokens * d.channels;
+  if (!n) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if ((rc = int8_pointers(d, a, a_scale, b, b_scale, bias, out))) return rc;
+  const size_t oes = dtype_size((int)d.out_dtype), ab = d.tokens * d.depth * dtype_size((int)d.a_dtype);
+  const size_t bb = d.channels * d.depth, ws = int8_workspace(d);
+  Parts parts;
+  const size_t at_a = parts.take(ab), at_b = parts.take(bb), at_as = parts.take(d.tokens * 4);
+  const size_t at_bs = parts.take(d.channels * 4), at_bias = parts.take(d.channels * 4), at_out = parts.take(n * oes);
+  const size_t at_ws = parts.take(ws);
+  Dev& dev = *g_devs[0];
+  std::lock_guard<std::mutex> g(dev.mu);
+  CK(cudaSetDevice(dev.id));
+  if ((rc = ensure_big(dev, 0, parts.total))) return rc;
+  cudaStream_t s = dev.s[0];
+  uint8_t* base = (uint8_t*)dev.big[0];
+  if ((rc = h2d_full(dev, base + at_a, a, ab, s)) || (rc = h2d_full(dev, base + at_b, b, bb, s))) return rc;
+  if (a_scale && (rc = h2d_full(dev, base + at_as, a_scale, d.tokens * 4, s))) return rc;
+  if (b_scale && (rc = h2d_full(dev, base + at_bs, b_scale, d.channels * 4, s))) return rc;
+  if (bias && (rc = h2d_full(dev, base + at_bias, bias, d.channels * 4, s))) return rc;
+  CK(cudaMemsetAsync(dev.st, 0xFF, sizeof(dcf_status), s));
+  rc = launch_int8_matmul(d, base + at_a, a_scale ? (float*)(base + at_as) : nullptr, (int8_t*)base + at_b,
+                          b_scale ? (float*)(base + at_bs) : nullptr, bias ? (float*)(base + at_bias) : nullptr,
+                          base + at_out, base + at_ws, dev.st, s);
+  if (rc) return learned_launch_failed(rc, "int8 matmul");
+  dcf_status st;
+  if ((rc = read_status(dev, s, &st))) return rc;
+  if ((rc = d2h_full(dev, out, base + at_out, n * oes, s))) return rc;
+  return learned_splat(dev, base + at_out, oes, n, s, res);
+}
+
+int dcf_checkpoint_grad_workspace(const dcf_checkpoint_desc* desc, size_t* bytes) {
+  int rc = checkpoint_desc_check(desc);
+  if (rc) return rc;
+  if (!bytes) return set_err(DCF_EINVAL, "null result");
+  *bytes = checkpoint_workspace(*desc);
+  return DCF_OK;
+}
+
+int dcf_checkpoint_grad_async(const dcf_checkpoint_desc* desc, const void* grad, const int8_t* q, const float* scale,
+                              void* out, void* workspace, size_t workspace_bytes, dcf_status* status, void* stream) {
+  int rc = checkpoint_desc_check(desc);
+  if (rc) return rc;
+  const dcf_checkpoint_desc& d = *desc;
+  if (!d.channels || !d.depth) return DCF_OK;
+  const size_t ws = checkpoint_workspace(d), es = dtype_size((int)d.grad_dtype), oes = dtype_size((int)d.out_dtype);
+  if (!out || !status || (d.tokens && (!grad || !q || !scale)) || (ws && !workspace))
+    return set_err(DCF_EINVAL, "null pointer");
+  if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
+  const uint64_t scales = (d.tokens + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN * d.depth;
+  if ((rc = apart({{out, rows_bytes(d.channels, d.depth, d.out_row_stride, oes)}, {workspace, ws}, {status, sizeof *status}},
+                  {{grad, rows_bytes(d.tokens, d.channels, d.grad_row_stride, es)},
+                   {q, rows_bytes(d.tokens, d.depth, d.q_row_stride, 1)},
+                   {scale, scales * 4}})))
+    return rc;
+  OnDevice on;
+  if ((rc = on.enter({{out, oes}, {grad, es}, {q, 1}, {scale, 4}, {ws ? workspace : nullptr, 256}, {status, 8}}))) return rc;
+  rc = launch_checkpoint_grad(d, grad, q, scale, out, workspace, status, (cudaStream_t)stream);
+  return rc ? learned_launch_failed(rc, "checkpoint grad") : DCF_OK;
+}
+
+int dcf_checkpoint_grad(const dcf_checkpoint_desc* desc, const void* grad, const int8_t* q, const float* scale,
+                        void* out, dcf_result* res) {
+  int rc = checkpoint_desc_check(desc);
+  if (rc) return rc;
+  const dcf_checkpoint_desc& d = *desc;
+  if (!dense_strides({d.grad_row_stride, d.q_row_stride, d.out_row_stride}))
+    return set_err(DCF_EINVAL, "checkpoint grad: host tensors are dense");
+  if ((rc = ensure_init())) return rc;
+  const uint64_t n = d.channels * d.depth;
+  if (!n) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
+  if (!out || (d.tokens && (!grad || !q || !scale))) return set_err(DCF_EINVAL, "null buffer");
+  const size_t oes = dtype_size((int)d.out_dtype), gb = d.tokens * d.channels * dtype_size((int)d.grad_dtype);
+  const size_t qb = d.tokens * d.depth, sb = (d.tokens + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN * d.depth * 4;
+  const size_t ws = checkpoint_workspace(d);
+  Parts parts;
+  const size_t at_g = parts.take(gb), at_q = parts.take(qb), at_s = parts.take(sb), at_out = parts.take(n * oes);
+  const size_t at_ws = parts.take(ws);
+  Dev& dev = *g_devs[0];
+  std::lock_guard<std::mutex> g(dev.mu);
+  CK(cudaSetDevice(dev.id));
+  if ((rc = ensure_big(dev, 0, parts.total))) return rc;
+  cudaStream_t s = dev.s[0];
+  uint8_t* base = (uint8_t*)dev.big[0];
+  if ((rc = h2d_full(dev, base + at_g, grad, gb, s)) || (rc = h2d_full(dev, base + at_q, q, qb, s)) ||
+      (rc = h2d_full(dev, base + at_s, scale, sb, s)))
+    return rc;
+  if ((d.flags & DCF_CHECKPOINT_ACCUMULATE) && (rc = h2d_full(dev, base + at_out, out, n * oes, s))) return rc;
+  CK(cudaMemsetAsync(dev.st, 0xFF, sizeof(dcf_status), s));
+  rc = launch_checkpoint_grad(d, base + at_g, (int8_t*)base + at_q, (float*)(base + at_s), base + at_out, base + at_ws,
+                              dev.st, s);
+  if (rc) return learned_launch_failed(rc, "checkpoint grad");
+  dcf_status st;
+  if ((rc = read_status(dev, s, &st))) return rc;
+  if ((rc = d2h_full(dev, out, base + at_out, n * oes, s))) return rc;
+  return learned_splat(dev, base + at_out, oes, n, s, res);
+}
+
+}  // extern "C"
