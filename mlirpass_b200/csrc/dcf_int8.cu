@@ -2,95 +2,515 @@
 // channel:
 //   out[t][c] = (sum over k of a[t][k] * b[c][k]) * a_scale[t] * b_scale[c] + bias[c]
 // Sums of whole numbers are exact in 32 bits (2^14 * 131071 < 2^31), in any
-// order, so a sum may be split and joined freely.
+// order, so a sum is split and joined wherever that helps.
 #include "dcf_quant.cuh"
 
 namespace dcf {
 
 namespace {
 
-struct Int8Args {
-  const int8_t* a;
-  const int8_t* b;
+constexpr int kSide = 128;                // channels of a CTA
+constexpr int kTileM = 2 * kSide;         // of a pair
+constexpr int kBK = 128;                  // k of a stage: one 128-byte swizzle row
+constexpr int kOutWarps = 8;
+constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+constexpr int kReaders = 128;             // threads that read a weight's rows where no tensor map describes them
+constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
+
+// What becomes of sums.
+struct Result {
   const float* a_scale;  // null: the sums themselves
   const float* b_scale;
   const float* bias;
   void* out;
   int out_dtype;
-  int tokens, channels, depth;
-  int64_t as, bs, os;
+  int pairs;             // two neighbours of a row of a 16-bit result make an aligned word
+  int tokens, channels;
+  int64_t stride;
 };
 
-__device__ __forceinline__ void put(const Int8Args& g, int64_t t, int64_t c, int sum) {
-  const int64_t at = t * g.os + c;
+__device__ __forceinline__ float scaled(int sum, float a, float b, float bias, bool add) {
+  const float v = __fmul_rn(__fmul_rn((float)sum, a), b);
+  return add ? __fadd_rn(v, bias) : v;
+}
+
+// The result of one token and channel.
+__device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int sum) {
+  const int64_t at = t * g.stride + c;
   if (g.out_dtype == DCF_I32) {
     ((int*)g.out)[at] = sum;
     return;
   }
-  float v = __fmul_rn(__fmul_rn((float)sum, g.a_scale[t]), g.b_scale[c]);
-  if (g.bias) v = __fadd_rn(v, g.bias[c]);
+  const float v = scaled(sum, g.a_scale[t], g.b_scale[c], g.bias ? g.bias[c] : 0.0f, g.bias != nullptr);
   if (g.out_dtype == DCF_F32) ((float*)g.out)[at] = v;
   else if (g.out_dtype == DCF_F16) ((__half*)g.out)[at] = __float2half_rn(v);
   else ((__nv_bfloat16*)g.out)[at] = __float2bfloat16_rn(v);
 }
 
-constexpr int kTile = 64, kDeep = 64;
+// ------------------------------------------------- tensor-core product
 
-// 64 x 64 results to a block of 256 threads, sixteen to a thread.
-__global__ void __launch_bounds__(256) int8_tile_kernel(const Int8Args g) {
-  __shared__ __align__(16) uint32_t a[kDeep / 4][kTile + 1], b[kDeep / 4][kTile + 1];
-  pdl_begin();
-  const int64_t tiles = ((int64_t)g.channels + kTile - 1) / kTile, total = tiles * (((int64_t)g.tokens + kTile - 1) / kTile);
-  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
-  for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
-    const int64_t t0 = i / tiles * kTile, c0 = i % tiles * kTile;
-    int sum[4][4] = {};
-    for (int k0 = 0; k0 < g.depth; k0 += kDeep) {
-      auto fill = [&](uint32_t (&to)[kDeep / 4][kTile + 1], const int8_t* from, int64_t row0, int rows, int64_t stride) {
-        for (int w = threadIdx.x; w < kTile * kDeep / 4; w += 256) {
-          const int r = w / (kDeep / 4), k = w % (kDeep / 4);
-          uint32_t v = 0;
-          for (int e = 0; e < 4; e++)
-            if (row0 + r < rows && k0 + 4 * k + e < g.depth)
-              v |= (uint32_t)(uint8_t)from[(row0 + r) * stride + k0 + 4 * k + e] << (8 * e);
-          to[k][r] = v;
-        }
-      };
-      __syncthreads();
-      fill(a, g.a, t0, g.tokens, g.as);
-      fill(b, g.b, c0, g.channels, g.bs);
-      __syncthreads();
+template <int TN> constexpr int kStage = (kSide + TN / 2) * kBK;
+template <int TN> constexpr int kStages = TN == 256 ? 6 : TN == 128 ? 8 : 10;
+template <int TN> constexpr int kGemmSmem = kStages<TN> * kStage<TN> + kOutWarps * (TN / 2) * 4 + 512 + 1024;
+
+struct GemmArgs {
+  Result to;
+  int blocks;              // stages along the whole depth
+  int tiles_m, tiles;      // tiles along the channels, in all
+  int splits, split_k;     // parts of the depth, stages of each
+  int64_t total;           // tiles times splits
+  int* part;               // sums of the parts, where there is more than one
+  const int8_t* b;         // the weight, where threads read it
+  int64_t b_stride;
+  int depth;
+  dcf_status* st;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void pair_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Rows of 128 bytes with the 128-byte swizzle; groups of eight lie 1024 bytes apart.
+__device__ __forceinline__ uint64_t row_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Sums of a part: [column of the tile][channel of the tile].
+template <int TN> __device__ __forceinline__ int* part_of(const GemmArgs& g, int64_t item) {
+  return g.part + item * (kTileM * TN);
+}
+
+// 32 columns (tokens from t0 on) of 32 channels, a channel in each lane, on their way out.
+__device__ __forceinline__ void write_block(const Result& g, const uint32_t (&r)[32], const float* scales, int64_t t0,
+                                            int64_t c, float b, float bias) {
+  const int there = (int)(g.tokens - t0 < 32 ? g.tokens - t0 : 32);
+  const bool mine = c < g.channels, add = g.bias != nullptr;
+  auto each = [&](auto* out, auto cast) {
+    out += t0 * g.stride + c;
 #pragma unroll
-      for (int k = 0; k < kDeep / 4; k++)
+    for (int j = 0; j < 32; j++)
+      if (mine && j < there) out[j * g.stride] = cast(r[j], scales ? scales[j] : 0.0f);
+  };
+  auto value = [&](uint32_t v, float a) { return scaled((int)v, a, b, bias, add); };
+  if (g.out_dtype == DCF_I32) {
+    each((int*)g.out, [](uint32_t v, float) { return (int)v; });
+  } else if (g.out_dtype == DCF_F32) {
+    each((float*)g.out, value);
+  } else if (g.pairs) {
+    // Lanes trade: an even one writes its token for two channels, an odd one the next token.
+    const int odd = threadIdx.x & 1;
+    uint16_t* out = (uint16_t*)g.out + (t0 + odd) * g.stride + (c & ~1ll);
+    const bool both = (c | 1) < g.channels, one = (c & ~1ll) < g.channels;
+    const bool half = g.out_dtype == DCF_F16;
 #pragma unroll
-        for (int m = 0; m < 4; m++)
-#pragma unroll
-          for (int n = 0; n < 4; n++) sum[m][n] = __dp4a((int)a[k][y + 16 * m], (int)b[k][x + 16 * n], sum[m][n]);
+    for (int j = 0; j < 32; j += 2) {
+      const float x = value(r[j], scales[j]), y = value(r[j + 1], scales[j + 1]);
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? x : y, 1);
+      const float lo = odd ? got : x, hi = odd ? y : got;
+      uint32_t w;
+      if (half) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        w = *(const uint32_t*)&h;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        w = *(const uint32_t*)&h;
+      }
+      if (j + odd < there) {
+        if (both) *(uint32_t*)(out + j * g.stride) = w;
+        else if (one) out[j * g.stride] = (uint16_t)w;
+      }
     }
-    for (int m = 0; m < 4; m++)
-      for (int n = 0; n < 4; n++)
-        if (t0 + y + 16 * m < g.tokens && c0 + x + 16 * n < g.channels) put(g, t0 + y + 16 * m, c0 + x + 16 * n, sum[m][n]);
+  } else if (g.out_dtype == DCF_F16) {
+    each((__half*)g.out, [&](uint32_t v, float a) { return __float2half_rn(value(v, a)); });
+  } else {
+    each((__nv_bfloat16*)g.out, [&](uint32_t v, float a) { return __float2bfloat16_rn(value(v, a)); });
   }
 }
 
-// The workspace: tokens of a float type as whole numbers, and their scales.
-struct Layout {
-  int64_t stride;
-  size_t q, scale, bytes;
+// Sixteen bytes of a row from k on, zeros behind its end, where the row may start
+// at any byte.  Eight neighbours in a warp read the row's 128 bytes of a stage
+// as the 16-byte vectors that hold them (all within the allocation that holds
+// the row), and take what they lack from each other.
+__device__ __forceinline__ void read_start(const int8_t* row, int k, int depth, int lane, uint4& own, uint4& next) {
+  const int8_t* p = row + k;
+  const int off = (int)((uintptr_t)p & 15);
+  own = next = make_uint4(0, 0, 0, 0);
+  if (!row) return;
+  if (k - off < depth) own = *(const uint4*)(p - off);
+  if (off && (lane & 7) == 7 && k + 16 - off < depth) next = *(const uint4*)(p - off + 16);
+}
+
+__device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, int lane, const uint4& own, uint4 next) {
+  const uint4 beside = make_uint4(__shfl_down_sync(0xFFFFFFFFu, own.x, 1), __shfl_down_sync(0xFFFFFFFFu, own.y, 1),
+                                  __shfl_down_sync(0xFFFFFFFFu, own.z, 1), __shfl_down_sync(0xFFFFFFFFu, own.w, 1));
+  if ((lane & 7) != 7) next = beside;
+  const int off = (int)((uintptr_t)(row + k) & 15), have = depth - k;
+  uint32_t w[8] = {own.x, own.y, own.z, own.w, next.x, next.y, next.z, next.w};
+  if (off & 8) {
+#pragma unroll
+    for (int j = 0; j < 6; j++) w[j] = w[j + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int j = 0; j < 5; j++) w[j] = w[j + 1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
+    const int here = have - 4 * j;  // bytes of this word in the row
+    if (here < 4) w[j] = here > 0 ? w[j] & (0xFFFFFFFFu >> (32 - 8 * here)) : 0u;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// D = B A^T in tiles of 256 channels x TN tokens by persistent pairs of CTAs:
+// each loads 128 channels and half of the tokens, one instruction multiplies
+// 32 k of both, and each keeps the sums of its channels in TMEM, in two
+// buffers, so that a tile is written while the next is summed.  Channels lie
+// in the lanes, so that a warp writes neighbours of a row.  Warp 0 keeps the
+// ring of stages full; one thread of the first CTA issues the products of
+// both; the second CTA reports its full stages to it.  READ: the weight's rows
+// lie off 16-byte boundaries, and four more warps read them.
+template <int TN, bool READ>
+__global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
+    int8_gemm_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
+                     const GemmArgs args) {
+  const GemmArgs g = args;  // a reference to the parameter itself would be read through memory
+  constexpr int kMine = TN / 2;  // columns of one out warp
+  constexpr int S = kStages<TN>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
+  float* scales = (float*)(base + S * kStage<TN>);
+  uint64_t* full = (uint64_t*)(scales + kOutWarps * kMine);
+  uint64_t* empty = full + S;
+  uint64_t* peer = empty + S;             // the first CTA's: the second's stage is full
+  uint64_t* sum_full = peer + S;
+  uint64_t* sum_empty = sum_full + 2;     // the first CTA's
+  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  auto begin_of = [&](int64_t t) { return (int)(t % g.splits) * g.split_k; };
+  auto count_of = [&](int64_t t) { return min(g.split_k, g.blocks - begin_of(t)); };
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < S; s++) {
+      mbar_init(&full[s], READ ? 1 + kReaders : 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&peer[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&sum_full[b], 1);
+      mbar_init(&sum_empty[b], 2 * kOutWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_at)), "r"(2 * TN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  pair_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t*)tmem_at;
+  if (threadIdx.x == 0) {
+    if (!READ) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_b) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_a) : "memory");
+  }
+  pdl_begin();
+
+  bool fail = false;
+  if (warp == 0) {
+    if (lane == 0) {
+      int64_t i = 0;  // stages so far
+      for (int64_t t = first; t < g.total && !fail; t += step) {
+        const int64_t tile = t / g.splits;
+        const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
+        const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
+        const int b0 = begin_of(t), blocks = count_of(t);
+        for (int b = 0; b < blocks; b++, i++) {
+          const int s = (int)(i % S);
+          if (i >= S && !mbar_wait_bounded(&empty[s], (unsigned)((i / S - 1) & 1))) {
+            fail = true;
+            break;
+          }
+          const uint32_t to = smem_addr(base + s * kStage<TN>);
+          mbar_expect_tx(&full[s], READ ? TN / 2 * kBK : kStage<TN>);
+          if (!READ) tma_load_2d(to, &map_b, (b0 + b) * kBK, row, &full[s]);
+          tma_load_2d(to + kSide * kBK, &map_a, (b0 + b) * kBK, col, &full[s]);
+        }
+      }
+      // Leave only with no copy of ours and no arrival for us left in flight.
+      for (int64_t j = i > S ? i - S : 0; j < i; j++) {
+        const unsigned turn = (unsigned)((j / S) & 1);
+        if (!mbar_wait_bounded(&full[j % S], turn)) fail = true;
+        if (!fail && !mbar_wait_bounded(&empty[j % S], turn)) fail = true;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
+      int64_t i = 0, u = 0;  // stages and items so far
+      for (int64_t t = first; t < g.total && !fail; t += step, u++) {
+        const int blocks = count_of(t), d = (int)(u & 1);
+        for (int b = 0; b < blocks; b++, i++) {
+          const int s = (int)(i % S);
+          const unsigned turn = (unsigned)((i / S) & 1);
+          if (!mbar_wait_bounded(&full[s], turn)) {
+            fail = true;
+            break;
+          }
+          if (rank) {
+            arrive_first(&peer[s]);
+            continue;
+          }
+          if (!mbar_wait_bounded(&peer[s], turn) ||
+              (b == 0 && u >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((u / 2 - 1) & 1)))) {
+            fail = true;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t at = smem_addr(base + s * kStage<TN>);
+          const uint64_t pb = row_desc(at), pa = row_desc(at + kSide * kBK);
+#pragma unroll
+          for (int j = 0; j < kBK / 32; j++) pair_mma_i8(tmem + d * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
+          pair_commit(&empty[s]);
+          if (b == blocks - 1) pair_commit(&sum_full[d]);
+        }
+      }
+    }
+  } else if (warp >= 4 + kOutWarps) {
+    const int at = threadIdx.x - kGemmThreads, chunk = at & 7;
+    int64_t i = 0;
+    for (int64_t t = first; t < g.total && !fail; t += step) {
+      const int64_t row0 = (t / g.splits) % g.tiles_m * kTileM + rank * kSide;
+      const int b0 = begin_of(t), blocks = count_of(t);
+      for (int b = 0; b < blocks; b++, i++) {
+        const int s = (int)(i % S), k = (b0 + b) * kBK + chunk * 16;
+        constexpr int kRows = kSide * 8 / kReaders;
+        uint4 own[kRows], next[kRows];
+        auto row_of = [&](int j) {
+          const int64_t r = row0 + at / 8 + j * (kReaders / 8);
+          return r < g.to.channels ? g.b + r * g.b_stride : nullptr;
+        };
+#pragma unroll
+        for (int j = 0; j < kRows; j++) read_start(row_of(j), k, g.depth, lane, own[j], next[j]);
+        if (__any_sync(0xFFFFFFFFu, i >= S && !mbar_wait_bounded(&empty[s], (unsigned)((i / S - 1) & 1)))) {
+          fail = true;
+          break;
+        }
+        uint8_t* to = base + s * kStage<TN>;
+#pragma unroll
+        for (int j = 0; j < kRows; j++) {
+          const int r = at / 8 + j * (kReaders / 8);
+          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end(row_of(j), k, g.depth, lane, own[j], next[j]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&full[s]);
+      }
+    }
+  } else if (warp >= 4) {
+    const int part = warp & 3;               // the 32 TMEM lanes this warp may read
+    const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
+    const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
+    float* mine = scales + (warp - 4) * kMine;
+    int64_t u = 0;  // items so far
+    for (int64_t t = first; t < g.total && !fail; t += step, u++) {
+      const int64_t tile = t / g.splits;
+      const int row = (int)rank * kSide + part * 32 + lane;  // of the tile
+      const int64_t c = (tile % g.tiles_m) * kTileM + row, t0 = tile / g.tiles_m * TN + col;
+      const bool whole = g.splits == 1;
+      float b = 0, bias = 0;
+      if (whole && g.to.b_scale) {
+        if (c < g.to.channels) {
+          b = g.to.b_scale[c];
+          if (g.to.bias) bias = g.to.bias[c];
+        }
+        __syncwarp();
+        for (int j = lane; j < kMine; j += 32) mine[j] = t0 + j < g.to.tokens ? g.to.a_scale[t0 + j] : 0.0f;
+        __syncwarp();
+      }
+      const int d = (int)(u & 1);
+      if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[d], (unsigned)((u >> 1) & 1)))) {
+        fail = true;
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+      for (int j = 0; j < kMine; j += 32) {
+        uint32_t r[32];
+        tmem_load32(lanes + d * TN + j, r);
+        tmem_wait(r);
+        if (j + 32 == kMine) {
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          if (lane == 0) arrive_first(&sum_empty[d]);
+        }
+        if (t0 + j >= g.to.tokens) continue;
+        if (whole) {
+          write_block(g.to, r, g.to.b_scale ? mine + j : nullptr, t0 + j, c, b, bias);
+        } else {
+          int* p = part_of<TN>(g, t) + (int64_t)(col + j) * kTileM + row;
+#pragma unroll
+          for (int k = 0; k < 32; k++) p[k * kTileM] = (int)r[k];
+        }
+      }
+    }
+  }
+  if (fail) atomicExch(&g.st->error, 1u);
+  __syncthreads();
+  pair_sync();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+  }
+}
+
+// Joins the parts of each sum; a thread takes a token and channel.  Also what
+// writes the result of a depth of 0, whose sums have no parts.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_constant__ GemmArgs g, int tile_n) {
+  pdl_begin();
+  const int64_t across = ((int64_t)g.to.channels + kJoinThreads - 1) / kJoinThreads, all = across * g.to.tokens;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const int64_t t = i / across, c = i % across * kJoinThreads + threadIdx.x;
+    if (c >= g.to.channels) continue;
+    int sum = 0;
+    if (g.splits) {
+      const int64_t tile = t / tile_n * g.tiles_m + c / kTileM, size = (int64_t)kTileM * tile_n;
+      const int* p = g.part + tile * g.splits * size + t % tile_n * kTileM + c % kTileM;
+      for (int s = 0; s < g.splits; s++) sum += p[s * size];
+    }
+    put(g.to, t, c, sum);
+  }
+}
+
+// Rows that no tensor map describes (a row that starts off a 16-byte boundary),
+// copied to rows of whole vectors; a thread writes 16 bytes.
+constexpr int kPackThreads = 256;
+__global__ void __launch_bounds__(kPackThreads) pack_kernel(const int8_t* from, int64_t stride, int64_t rows, int cols,
+                                                            int8_t* to, int64_t to_stride) {
+  pdl_begin();
+  const int64_t groups = (cols + 15) / 16, all = groups * rows;
+  for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kPackThreads) {
+    const int64_t r = i / groups;
+    const int c = (int)(i % groups) * 16, have = cols - c;
+    const int8_t* p = from + r * stride + c;
+    const int off = (int)((uintptr_t)p & 3);
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (have >= 20 && c >= 4) {  // the words around these bytes lie in the row
+      const uint32_t* a = (const uint32_t*)(p - off);
+      uint32_t v[5];
+#pragma unroll
+      for (int j = 0; j < 5; j++) v[j] = a[j];
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (e < have) w[e >> 2] |= (uint32_t)(uint8_t)p[e] << ((e & 3) * 8);
+    }
+    *(uint4*)(to + r * to_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+bool encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+int64_t stride_of(int64_t given, uint64_t cols) { return given ? given : (int64_t)cols; }
+
+// Whether a tensor map describes rows of bytes as they lie.
+bool mappable(const void* p, int64_t stride, uint64_t cols) {
+  return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride >= (int64_t)cols && stride < (1ll << 40);
+}
+
+// How a product is laid out: tokens of a tile, and the parts into which its
+// depth is cut, `stages` stages each.
+struct Cut {
+  int tile_n;
+  int64_t tiles_m, tiles;
+  int splits, stages;
 };
 
+Cut cut_of(const dcf_int8_desc& d) {
+  const int blocks = (int)((d.depth + kBK - 1) / kBK);
+  Cut best = {};
+  double least = 1e300;
+  for (int tn : {64, 128, 256}) {
+    const int64_t tm = (int64_t)(d.channels + kTileM - 1) / kTileM, tiles = tm * (int64_t)((d.tokens + tn - 1) / tn);
+    const double stage = tn == 256 ? 1 : tn == 128 ? 0.65 : 0.5;
+    for (int s = 1; s == 1 || (s <= blocks && tiles * s <= kPairs); s++) {
+      const int each = (blocks + s - 1) / s, parts = each ? (blocks + each - 1) / each : 1;
+      const double rounds = (double)((tiles * parts + kPairs - 1) / kPairs);
+      const double cost = rounds * each * stage + (parts > 1 ? 10 : 0) + 4 * stage;
+      if (cost < least) {
+        least = cost;
+        best = {tn, tm, tiles, parts, each};
+      }
+    }
+  }
+  return best;
+}
+
+// The workspace: tokens of a float type as whole numbers and their scales (or a
+// copy of whole numbers that no tensor map describes), a copy of a weight whose stride no
+// tensor map takes, and the parts of sums.
+struct Layout {
+  Cut cut;
+  int64_t stride;
+  bool copy_b;
+  size_t a, scale, b, part, bytes;
+};
+
+// A weight whose rows lie off 16-byte boundaries is read by threads as long as few tokens leave that hidden
+// behind HBM; many have it copied first.
 Layout layout_of(const dcf_int8_desc& d) {
   Layout l = {};
-  if (d.a_dtype == DCF_I8) return l;
   auto take = [&](size_t bytes) {
     const size_t at = l.bytes;
     l.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
+  l.cut = cut_of(d);
   l.stride = (int64_t)((d.depth + 15) / 16 * 16);
-  l.q = take((size_t)d.tokens * l.stride);
-  l.scale = take((size_t)d.tokens * 4);
+  l.a = take((size_t)d.tokens * l.stride);
+  l.scale = take(d.a_dtype != DCF_I8 ? (size_t)d.tokens * 4 : 0);
+  l.copy_b = l.cut.tile_n > 64 && d.channels > 1 && stride_of(d.b_row_stride, d.depth) % 16;
+  l.b = take(l.copy_b ? (size_t)d.channels * l.stride : 0);
+  l.part = take(l.cut.splits > 1 ? (size_t)l.cut.tiles * l.cut.splits * kTileM * l.cut.tile_n * 4 : 0);
   return l;
+}
+
+template <int TN, bool READ>
+int gemm(const CUtensorMap& mb, const CUtensorMap& ma, const GemmArgs& g, cudaStream_t s) {
+  if (!prepare_smem((const void*)int8_gemm_kernel<TN, READ>, kGemmSmem<TN>)) return DCF_ECUDA;
+  const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
+  return launch(int8_gemm_kernel<TN, READ>, dim3(2 * pairs), kGemmThreads + (READ ? kReaders : 0), kGemmSmem<TN>, 2, s, mb, ma, g);
 }
 
 }  // namespace
@@ -126,33 +546,66 @@ size_t int8_workspace(const dcf_int8_desc& d) {
 
 int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_scale, const int8_t* b,
                        const float* b_scale, const float* bias, void* out, void* ws, dcf_status* st, cudaStream_t s) {
-  (void)st;
-  Int8Args g;
-  g.a = (const int8_t*)a;
-  g.a_scale = a_scale;
-  g.as = d.a_row_stride ? d.a_row_stride : (int64_t)d.depth;
+  const Layout l = layout_of(d);
+  const Cut& cut = l.cut;
+  uint8_t* work = (uint8_t*)ws;
+  int64_t as = stride_of(d.a_row_stride, d.depth), bs = stride_of(d.b_row_stride, d.depth);
+  auto pack = [&](const int8_t** p, int64_t* stride, uint64_t rows, size_t at) {
+    const int64_t all = (l.stride / 16) * (int64_t)rows, blocks = (all + kPackThreads - 1) / kPackThreads;
+    const int rc = launch(pack_kernel, dim3((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30)), kPackThreads, 0, 1, s, *p,
+                          *stride, (int64_t)rows, (int)d.depth, (int8_t*)work + at, l.stride);
+    *p = (int8_t*)work + at;
+    *stride = l.stride;
+    return rc;
+  };
+  const int8_t* q = (const int8_t*)a;
+  int rc = DCF_OK;
   if (d.a_dtype != DCF_I8) {
-    const Layout l = layout_of(d);
-    int8_t* q = (int8_t*)ws + l.q;
-    float* scale = (float*)((uint8_t*)ws + l.scale);
-    const dcf_quant_desc tokens = {d.a_dtype, DCF_QUANT_ROWS, d.tokens, d.depth, g.as, l.stride};
-    if (int rc = launch_quantize(tokens, a, q, scale, s)) return rc;
-    g.a = q;
-    g.a_scale = scale;
-    g.as = l.stride;
+    const dcf_quant_desc tokens = {d.a_dtype, DCF_QUANT_ROWS, d.tokens, d.depth, as, l.stride};
+    q = (int8_t*)work + l.a;
+    a_scale = (float*)(work + l.scale);
+    as = l.stride;
+    if ((rc = launch_quantize(tokens, a, (int8_t*)q, (float*)a_scale, s))) return rc;
   }
-  g.b = b;
-  g.b_scale = b_scale;
-  g.bias = bias;
-  g.out = out;
-  g.out_dtype = (int)d.out_dtype;
-  g.tokens = (int)d.tokens;
-  g.channels = (int)d.channels;
-  g.depth = (int)d.depth;
-  g.bs = d.b_row_stride ? d.b_row_stride : (int64_t)d.depth;
-  g.os = d.out_row_stride ? d.out_row_stride : (int64_t)d.channels;
-  const int64_t total = (int64_t)((d.tokens + kTile - 1) / kTile) * (int64_t)((d.channels + kTile - 1) / kTile);
-  return launch(int8_tile_kernel, dim3((unsigned)(total < (1 << 30) ? total : 1 << 30)), 256, 0, 1, s, g);
+  GemmArgs g = {};
+  g.to.a_scale = a_scale;
+  g.to.b_scale = b_scale;
+  g.to.bias = bias;
+  g.to.out = out;
+  g.to.out_dtype = (int)d.out_dtype;
+  g.to.tokens = (int)d.tokens;
+  g.to.channels = (int)d.channels;
+  g.to.stride = stride_of(d.out_row_stride, d.channels);
+  g.to.pairs = (uintptr_t)out % 4 == 0 && (d.tokens == 1 || g.to.stride % 2 == 0);
+  g.blocks = (int)((d.depth + kBK - 1) / kBK);
+  g.tiles_m = (int)cut.tiles_m;
+  g.splits = d.depth ? cut.splits : 0;
+  g.split_k = cut.stages;
+  g.total = cut.tiles * cut.splits;
+  g.part = (int*)(work + l.part);
+  g.st = st;
+  if (d.depth) {
+    if (!mappable(q, as, d.depth) && (rc = pack(&q, &as, d.tokens, l.a))) return rc;
+    if (l.copy_b && (rc = pack(&b, &bs, d.channels, l.b))) return rc;
+    const bool read = !mappable(b, bs, d.depth);
+    g.b = b;
+    g.b_stride = bs;
+    g.depth = (int)d.depth;
+    if (!encoder()) return DCF_EUNSUPPORTED;
+    CUtensorMap ma, mb = {};
+    if ((!read && !encode_rows(&mb, b, (int64_t)d.channels, (int64_t)d.depth, bs, kSide)) ||
+        !encode_rows(&ma, q, (int64_t)d.tokens, (int64_t)d.depth, as, cut.tile_n / 2))
+      return DCF_ECUDA;
+    switch (cut.tile_n) {
+      case 64: rc = read ? gemm<64, true>(mb, ma, g, s) : gemm<64, false>(mb, ma, g, s); break;
+      case 128: rc = read ? gemm<128, true>(mb, ma, g, s) : gemm<128, false>(mb, ma, g, s); break;
+      default: rc = read ? gemm<256, true>(mb, ma, g, s) : gemm<256, false>(mb, ma, g, s);
+    }
+    if (rc || cut.splits == 1) return rc;
+  }
+  const int64_t joins = ((int64_t)d.channels + kJoinThreads - 1) / kJoinThreads * (int64_t)d.tokens;
+  return launch(int8_join_kernel, dim3((unsigned)(joins < (1 << 30) ? joins : 1 << 30)), kJoinThreads, 0, 1, s, g,
+                cut.tile_n);
 }
 
 }  // namespace dcf
