@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  const uint32_t stage0 = smem_addr(base);
   auto begin_of = [&](int64_t t) { return (int)(t % g.splits) * g.split_k; };
   auto count_of = [&](int64_t t) { return min(g.split_k, g.blocks - begin_of(t)); };
 
@@ -239,91 +240,94 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
   bool fail = false;
   if (warp == 0) {
     if (lane == 0) {
-      int64_t i = 0;  // stages so far
+      Ring<S> at;
+      int used = 0;  // stages filled, S at most
       for (int64_t t = first; t < g.total && !fail; t += step) {
         const int64_t tile = t / g.splits;
         const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
         const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
         const int b0 = begin_of(t), blocks = count_of(t);
-        for (int b = 0; b < blocks; b++, i++) {
-          const int s = (int)(i % S);
-          if (i >= S && !mbar_wait_bounded(&empty[s], (unsigned)((i / S - 1) & 1))) {
+        for (int k = b0 * kBK, end = (b0 + blocks) * kBK; k < end; k += kBK, at.next()) {
+          if (!mbar_wait_bounded(&empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
-          const uint32_t to = smem_addr(base + s * kStage<TN>);
-          mbar_expect_tx(&full[s], READ ? TN / 2 * kBK : kStage<TN>);
-          if (!READ) tma_load_2d(to, &map_b, (b0 + b) * kBK, row, &full[s]);
-          tma_load_2d(to + kSide * kBK, &map_a, (b0 + b) * kBK, col, &full[s]);
+          const uint32_t to = stage0 + at.s * kStage<TN>;
+          mbar_expect_tx(&full[at.s], READ ? TN / 2 * kBK : kStage<TN>);
+          if (!READ) tma_load_2d(to, &map_b, k, row, &full[at.s]);
+          tma_load_2d(to + kSide * kBK, &map_a, k, col, &full[at.s]);
+          used += used < S;
         }
       }
       // Leave only with no copy of ours and no arrival for us left in flight.
-      for (int64_t j = i > S ? i - S : 0; j < i; j++) {
-        const unsigned turn = (unsigned)((j / S) & 1);
-        if (!mbar_wait_bounded(&full[j % S], turn)) fail = true;
-        if (!fail && !mbar_wait_bounded(&empty[j % S], turn)) fail = true;
+      for (; used > 0; used--) {
+        const Ring<S> last = at.back(used);
+        if (!mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
+        if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
-      int64_t i = 0, u = 0;  // stages and items so far
-      for (int64_t t = first; t < g.total && !fail; t += step, u++) {
-        const int blocks = count_of(t), d = (int)(u & 1);
-        for (int b = 0; b < blocks; b++, i++) {
-          const int s = (int)(i % S);
-          const unsigned turn = (unsigned)((i / S) & 1);
-          if (!mbar_wait_bounded(&full[s], turn)) {
+      const uint64_t desc = row_desc(stage0);
+      Ring<S> at;
+      Ring<2> sum;
+      for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
+        const int blocks = count_of(t);
+        if (!rank && !mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1)) {
+          fail = true;
+          break;
+        }
+        for (int b = 0; b < blocks; b++, at.next()) {
+          if (!mbar_wait_bounded(&full[at.s], at.turn)) {
             fail = true;
             break;
           }
           if (rank) {
-            arrive_first(&peer[s]);
+            arrive_first(&peer[at.s]);
             continue;
           }
-          if (!mbar_wait_bounded(&peer[s], turn) ||
-              (b == 0 && u >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((u / 2 - 1) & 1)))) {
+          if (!mbar_wait_bounded(&peer[at.s], at.turn)) {
             fail = true;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t at = smem_addr(base + s * kStage<TN>);
-          const uint64_t pb = row_desc(at), pa = row_desc(at + kSide * kBK);
+          const uint64_t pb = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pa = pb + (kSide * kBK >> 4);
 #pragma unroll
-          for (int j = 0; j < kBK / 32; j++) pair_mma_i8(tmem + d * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
-          pair_commit(&empty[s]);
-          if (b == blocks - 1) pair_commit(&sum_full[d]);
+          for (int j = 0; j < kBK / 32; j++) pair_mma_i8(tmem + sum.s * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
+          pair_commit(&empty[at.s]);
         }
+        if (!rank && !fail) pair_commit(&sum_full[sum.s]);
       }
     }
   } else if (warp >= 4 + kOutWarps) {
-    const int at = threadIdx.x - kGemmThreads, chunk = at & 7;
-    int64_t i = 0;
+    const int id = threadIdx.x - kGemmThreads, chunk = id & 7;
+    Ring<S> at;
     for (int64_t t = first; t < g.total && !fail; t += step) {
       const int64_t row0 = (t / g.splits) % g.tiles_m * kTileM + rank * kSide;
       const int b0 = begin_of(t), blocks = count_of(t);
-      for (int b = 0; b < blocks; b++, i++) {
-        const int s = (int)(i % S), k = (b0 + b) * kBK + chunk * 16;
+      for (int b = 0; b < blocks; b++, at.next()) {
+        const int k = (b0 + b) * kBK + chunk * 16;
         constexpr int kRows = kSide * 8 / kReaders;
         uint4 own[kRows], next[kRows];
         auto row_of = [&](int j) {
-          const int64_t r = row0 + at / 8 + j * (kReaders / 8);
+          const int64_t r = row0 + id / 8 + j * (kReaders / 8);
           return r < g.to.channels ? g.b + r * g.b_stride : nullptr;
         };
 #pragma unroll
         for (int j = 0; j < kRows; j++) read_start(row_of(j), k, g.depth, lane, own[j], next[j]);
-        if (__any_sync(0xFFFFFFFFu, i >= S && !mbar_wait_bounded(&empty[s], (unsigned)((i / S - 1) & 1)))) {
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
         }
-        uint8_t* to = base + s * kStage<TN>;
+        uint8_t* to = base + at.s * kStage<TN>;
 #pragma unroll
         for (int j = 0; j < kRows; j++) {
-          const int r = at / 8 + j * (kReaders / 8);
+          const int r = id / 8 + j * (kReaders / 8);
           *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end(row_of(j), k, g.depth, lane, own[j], next[j]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&full[s]);
+        mbar_arrive(&full[at.s]);
       }
     }
   } else if (warp >= 4) {
@@ -331,8 +335,8 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
     const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     float* mine = scales + (warp - 4) * kMine;
-    int64_t u = 0;  // items so far
-    for (int64_t t = first; t < g.total && !fail; t += step, u++) {
+    Ring<2> sum;
+    for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
       const int64_t tile = t / g.splits;
       const int row = (int)rank * kSide + part * 32 + lane;  // of the tile
       const int64_t c = (tile % g.tiles_m) * kTileM + row, t0 = tile / g.tiles_m * TN + col;
@@ -347,8 +351,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
         for (int j = lane; j < kMine; j += 32) mine[j] = t0 + j < g.to.tokens ? g.to.a_scale[t0 + j] : 0.0f;
         __syncwarp();
       }
-      const int d = (int)(u & 1);
-      if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[d], (unsigned)((u >> 1) & 1)))) {
+      if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[sum.s], sum.turn))) {
         fail = true;
         break;
       }
@@ -356,11 +359,11 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
 #pragma unroll 1
       for (int j = 0; j < kMine; j += 32) {
         uint32_t r[32];
-        tmem_load32(lanes + d * TN + j, r);
+        tmem_load32(lanes + sum.s * TN + j, r);
         tmem_wait(r);
         if (j + 32 == kMine) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          if (lane == 0) arrive_first(&sum_empty[d]);
+          if (lane == 0) arrive_first(&sum_empty[sum.s]);
         }
         if (t0 + j >= g.to.tokens) continue;
         if (whole) {

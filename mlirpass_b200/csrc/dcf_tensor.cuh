@@ -65,6 +65,30 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
   for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[j]));
 }
 
+// A place in a ring of S stages and the parity of its turn.  Stepped, not
+// divided out: the one thread that issues products would spend as long on
+// that as four products take.
+template <int S> struct Ring {
+  int s = 0;
+  unsigned turn = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == S) {
+      s = 0;
+      turn ^= 1;
+    }
+  }
+  // The place n <= S steps before this one.
+  __device__ __forceinline__ Ring back(int n) const {
+    Ring r = *this;
+    r.s -= n;
+    if (r.s < 0) {
+      r.s += S;
+      r.turn ^= 1;
+    }
+    return r;
+  }
+};
+
 // ---------------------------------------------------------------- host
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
