@@ -66,15 +66,13 @@ struct GemmArgs {
   dcf_status* st;
 };
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+// Into this CTA's memory; the bytes are reported to a barrier of either CTA of the pair.
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
       : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 __device__ __forceinline__ void pair_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -183,8 +181,11 @@ __device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, i
 // buffers, so that a tile is written while the next is summed.  Channels lie
 // in the lanes, so that a warp writes neighbours of a row.  Warp 0 keeps the
 // ring of stages full; one thread of the first CTA issues the products of
-// both; the second CTA reports its full stages to it.  READ: the weight's rows
-// lie off 16-byte boundaries, and four more warps read them.
+// both: its barrier counts the bytes of both CTAs' loads, as each wait on
+// another costs that thread 160 cycles of the 512 that a stage's four products
+// take (probe: 136 cycles a product with one wait per stage, 176 with two).
+// READ: the weight's rows lie off 16-byte boundaries, and four more warps read
+// them.
 template <int TN, bool READ>
 __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
@@ -196,23 +197,23 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
   float* scales = (float*)(base + S * kStage<TN>);
   uint64_t* full = (uint64_t*)(scales + kOutWarps * kMine);
-  uint64_t* empty = full + S;
-  uint64_t* peer = empty + S;             // the first CTA's: the second's stage is full
-  uint64_t* sum_full = peer + S;
+  uint64_t* empty = full + S;             // (the first CTA's `full` counts what both have loaded)
+  uint64_t* sum_full = empty + S;
   uint64_t* sum_empty = sum_full + 2;     // the first CTA's
   uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
   const uint32_t stage0 = smem_addr(base);
+  uint32_t full0;  // the first CTA's
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(full0) : "r"(smem_addr(full)));
   auto begin_of = [&](int64_t t) { return (int)(t % g.splits) * g.split_k; };
   auto count_of = [&](int64_t t) { return min(g.split_k, g.blocks - begin_of(t)); };
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < S; s++) {
-      mbar_init(&full[s], READ ? 1 + kReaders : 1);
+      mbar_init(&full[s], READ ? 1 + 2 * kReaders : 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&peer[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
@@ -253,41 +254,34 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
             break;
           }
           const uint32_t to = stage0 + at.s * kStage<TN>;
-          mbar_expect_tx(&full[at.s], READ ? TN / 2 * kBK : kStage<TN>);
-          if (!READ) tma_load_2d(to, &map_b, k, row, &full[at.s]);
-          tma_load_2d(to + kSide * kBK, &map_a, k, col, &full[at.s]);
+          const uint32_t bar = full0 + at.s * 8;
+          if (!rank) mbar_expect_tx(&full[at.s], 2 * (READ ? TN / 2 * kBK : kStage<TN>));
+          if (!READ) pair_load_2d(to, &map_b, k, row, bar);
+          pair_load_2d(to + kSide * kBK, &map_a, k, col, bar);
           used += used < S;
         }
       }
       // Leave only with no copy of ours and no arrival for us left in flight.
       for (; used > 0; used--) {
         const Ring<S> last = at.back(used);
-        if (!mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
+        if (!rank && !mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
         if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && !rank) {
       constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTileM >> 4) << 24);
       const uint64_t desc = row_desc(stage0);
       Ring<S> at;
       Ring<2> sum;
       for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
         const int blocks = count_of(t);
-        if (!rank && !mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1)) {
+        if (!mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1)) {
           fail = true;
           break;
         }
         for (int b = 0; b < blocks; b++, at.next()) {
           if (!mbar_wait_bounded(&full[at.s], at.turn)) {
-            fail = true;
-            break;
-          }
-          if (rank) {
-            arrive_first(&peer[at.s]);
-            continue;
-          }
-          if (!mbar_wait_bounded(&peer[at.s], at.turn)) {
             fail = true;
             break;
           }
@@ -297,7 +291,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
           for (int j = 0; j < kBK / 32; j++) pair_mma_i8(tmem + sum.s * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
           pair_commit(&empty[at.s]);
         }
-        if (!rank && !fail) pair_commit(&sum_full[sum.s]);
+        if (!fail) pair_commit(&sum_full[sum.s]);
       }
     }
   } else if (warp >= 4 + kOutWarps) {
@@ -327,7 +321,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
           *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end(row_of(j), k, g.depth, lane, own[j], next[j]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&full[at.s]);
+        arrive_first(&full[at.s]);
       }
     }
   } else if (warp >= 4) {
