@@ -58,11 +58,20 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr));
 }
 
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
 // Until the loads issued before have arrived; `r` is named so that no use of it moves ahead.
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+template <int N> __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int j = 0; j < 32; j++) asm volatile("" : "+r"(r[j]));
+  for (int j = 0; j < N; j++) asm volatile("" : "+r"(r[j]));
 }
 
 // A place in a ring of S stages and the parity of its turn.  Stepped, not
