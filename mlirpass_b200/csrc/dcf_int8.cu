@@ -12,8 +12,8 @@ namespace {
 constexpr int kSide = 128;                // channels of a CTA
 constexpr int kTileM = 2 * kSide;         // of a pair
 constexpr int kBK = 128;                  // k of a stage: one 128-byte swizzle row
-constexpr int kOutWarps = 8;
-constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+template <bool READ> constexpr int kOutWarps = READ ? 8 : 16;  // warps that write results
+template <bool READ> constexpr int kGemmThreads = 128 + 32 * kOutWarps<READ>;  // warp 0 loads, warp 1 multiplies
 constexpr int kReaders = 128;             // threads that read a weight's rows where no tensor map describes them
 constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int s
 
 template <int TN> constexpr int kStage = (kSide + TN / 2) * kBK;
 template <int TN> constexpr int kStages = TN == 256 ? 6 : TN == 128 ? 8 : 10;
-template <int TN> constexpr int kGemmSmem = kStages<TN> * kStage<TN> + kOutWarps * (TN / 2) * 4 + 512 + 1024;
+template <int TN> constexpr int kGemmSmem = kStages<TN> * kStage<TN> + 4 * TN * 4 + 512 + 1024;
 
 struct GemmArgs {
   Result to;
@@ -92,37 +92,65 @@ template <int TN> __device__ __forceinline__ int* part_of(const GemmArgs& g, int
   return g.part + item * (kTileM * TN);
 }
 
+// Two f32 products by one instruction, each rounded as by itself.  (A packed sum
+// after it would be fused with it, whatever rounding is written.)
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
 // kBlock columns (tokens from t0 on) of 32 channels, a channel in each lane, on their way out.
-// (A short block on purpose: code that runs four times a tile is fetched about as
-// often as it runs.  32 columns at a time: 6.2 us a tile, 16: XX.)
+// A tile is as good as written once, so what counts is how few instructions and
+// how short a code do it (32 columns at a time by 8 warps and a predicate for
+// each: 6.2 us a tile of 256 x 256).
 constexpr int kBlock = 16;
+template <bool WHOLE>
 __device__ __forceinline__ void write_block(const Result& g, const uint32_t (&r)[kBlock], const float* scales, int64_t t0,
-                                            int64_t c, float b, float bias) {
-  const int there = (int)(g.tokens - t0 < kBlock ? g.tokens - t0 : kBlock);
+                                            int64_t c, uint64_t b, float bias) {
+  const int there = WHOLE ? kBlock : (int)(g.tokens - t0);
   const bool mine = c < g.channels;
-  auto value = [&](int j) { return __fadd_rn(__fmul_rn(__fmul_rn((float)(int)r[j], scales[j]), b), bias); };
+  const int64_t step = g.stride;
+  auto values = [&](int j) {
+    const float2 a = *(const float2*)&scales[j];
+    const float2 v = apart(mul2(mul2(two((float)(int)r[j], (float)(int)r[j + 1]), two(a.x, a.y)), b));
+    return make_float2(__fadd_rn(v.x, bias), __fadd_rn(v.y, bias));
+  };
   auto each = [&](auto* out, auto cast) {
-    out += t0 * g.stride + c;
+    out += t0 * step + c;
+    if (!mine) return;
 #pragma unroll
-    for (int j = 0; j < kBlock; j++, out += g.stride)
-      if (mine && j < there) *out = cast(j);
+    for (int j = 0; j < kBlock; j += 2, out += 2 * step) {
+      const auto v = cast(j);
+      if (WHOLE || j < there) out[0] = v.x;
+      if (WHOLE || j + 1 < there) out[step] = v.y;
+    }
   };
   if (g.out_dtype == DCF_I32) {
-    each((int*)g.out, [&](int j) { return (int)r[j]; });
+    each((int*)g.out, [&](int j) { return make_int2((int)r[j], (int)r[j + 1]); });
   } else if (g.out_dtype == DCF_F32) {
-    each((float*)g.out, value);
+    each((float*)g.out, values);
   } else if (g.pairs) {
     // Lanes trade: an even one writes its token for two channels, an odd one the next token.
     const int odd = threadIdx.x & 1;
-    uint16_t* out = (uint16_t*)g.out + (t0 + odd) * g.stride + (c & ~1ll);
+    uint16_t* out = (uint16_t*)g.out + (t0 + odd) * step + (c & ~1ll);
     const bool both = (c | 1) < g.channels, one = (c & ~1ll) < g.channels;
     const bool half = g.out_dtype == DCF_F16;
-    const int64_t step = 2 * g.stride;
 #pragma unroll
-    for (int j = 0; j < kBlock; j += 2, out += step) {
-      const float x = value(j), y = value(j + 1);
-      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? x : y, 1);
-      const float lo = odd ? got : x, hi = odd ? y : got;
+    for (int j = 0; j < kBlock; j += 2, out += 2 * step) {
+      const float2 v = values(j);
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v.x : v.y, 1);
+      const float lo = odd ? got : v.x, hi = odd ? v.y : got;
       uint32_t w;
       if (half) {
         const __half2 h = __floats2half2_rn(lo, hi);
@@ -131,15 +159,17 @@ __device__ __forceinline__ void write_block(const Result& g, const uint32_t (&r)
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         w = *(const uint32_t*)&h;
       }
-      if (j + odd < there) {
+      if (WHOLE) {
+        if (both) *(uint32_t*)out = w;
+      } else if (j + odd < there) {
         if (both) *(uint32_t*)out = w;
         else if (one) *out = (uint16_t)w;
       }
     }
   } else if (g.out_dtype == DCF_F16) {
-    each((__half*)g.out, [&](int j) { return __float2half_rn(value(j)); });
+    each((__half*)g.out, [&](int j) { return __float22half2_rn(values(j)); });
   } else {
-    each((__nv_bfloat16*)g.out, [&](int j) { return __float2bfloat16_rn(value(j)); });
+    each((__nv_bfloat16*)g.out, [&](int j) { return __float22bfloat162_rn(values(j)); });
   }
 }
 
@@ -191,16 +221,16 @@ __device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, i
 // READ: the weight's rows lie off 16-byte boundaries, and four more warps read
 // them.
 template <int TN, bool READ>
-__global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
+__global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
                      const GemmArgs args) {
   const GemmArgs g = args;  // a reference to the parameter itself would be read through memory
-  constexpr int kMine = TN / 2;  // columns of one out warp
+  constexpr int OW = kOutWarps<READ>, kMine = TN / (OW / 4);  // columns of one out warp
   constexpr int S = kStages<TN>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
   float* scales = (float*)(base + S * kStage<TN>);
-  uint64_t* full = (uint64_t*)(scales + kOutWarps * kMine);
+  uint64_t* full = (uint64_t*)(scales + OW * kMine);
   uint64_t* empty = full + S;             // (the first CTA's `full` counts what both have loaded)
   uint64_t* sum_full = empty + S;
   uint64_t* sum_empty = sum_full + 2;     // the first CTA's
@@ -221,7 +251,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
-      mbar_init(&sum_empty[b], 2 * kOutWarps);
+      mbar_init(&sum_empty[b], 2 * OW);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -298,8 +328,8 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
         if (!fail) pair_commit(&sum_full[sum.s]);
       }
     }
-  } else if (warp >= 4 + kOutWarps) {
-    const int id = threadIdx.x - kGemmThreads, chunk = id & 7;
+  } else if (warp >= 4 + OW) {
+    const int id = threadIdx.x - kGemmThreads<READ>, chunk = id & 7;
     Ring<S> at;
     for (int64_t t = first; t < g.total && !fail; t += step) {
       const int64_t row0 = (t / g.splits) % g.tiles_m * kTileM + rank * kSide;
@@ -330,7 +360,7 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
     }
   } else if (warp >= 4) {
     const int part = warp & 3;               // the 32 TMEM lanes this warp may read
-    const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
+    const int col = (warp - 4) / 4 * kMine;  // and its part of the columns
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     float* mine = scales + (warp - 4) * kMine;
     Ring<2> sum;
@@ -365,7 +395,12 @@ __global__ void __launch_bounds__(kGemmThreads + (READ ? kReaders : 0), 1)
         }
         if (t0 + j >= g.to.tokens) continue;
         if (whole) {
-          write_block(g.to, r, mine + j, t0 + j, c, b, bias);
+          const uint64_t b2 = two(b, b);
+          // (a block over the last channel takes the careful path when they are odd)
+          if (t0 + j + kBlock <= g.to.tokens && (c - lane + 32 <= g.to.channels || !g.to.pairs))
+            write_block<true>(g.to, r, mine + j, t0 + j, c, b2, bias);
+          else
+            write_block<false>(g.to, r, mine + j, t0 + j, c, b2, bias);
         } else {
           int* p = part_of<TN>(g, t) + (int64_t)(col + j) * kTileM + row;
 #pragma unroll
@@ -511,7 +546,7 @@ template <int TN, bool READ>
 int gemm(const CUtensorMap& mb, const CUtensorMap& ma, const GemmArgs& g, cudaStream_t s) {
   if (!prepare_smem((const void*)int8_gemm_kernel<TN, READ>, kGemmSmem<TN>)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
-  return launch(int8_gemm_kernel<TN, READ>, dim3(2 * pairs), kGemmThreads + (READ ? kReaders : 0), kGemmSmem<TN>, 2, s, mb, ma, g);
+  return launch(int8_gemm_kernel<TN, READ>, dim3(2 * pairs), kGemmThreads<READ> + (READ ? kReaders : 0), kGemmSmem<TN>, 2, s, mb, ma, g);
 }
 
 }  // namespace
