@@ -35,13 +35,13 @@ __device__ __forceinline__ float scaled(int sum, float a, float b, float bias, b
 }
 
 // The result of one token and channel.
-__device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int sum) {
+__device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int sum, float a_scale) {
   const int64_t at = t * g.stride + c;
   if (g.out_dtype == DCF_I32) {
     ((int*)g.out)[at] = sum;
     return;
   }
-  const float v = scaled(sum, g.a_scale[t], g.b_scale[c], g.bias ? g.bias[c] : 0.0f, g.bias != nullptr);
+  const float v = scaled(sum, a_scale, g.b_scale[c], g.bias ? g.bias[c] : 0.0f, g.bias != nullptr);
   if (g.out_dtype == DCF_F32) ((float*)g.out)[at] = v;
   else if (g.out_dtype == DCF_F16) ((__half*)g.out)[at] = __float2half_rn(v);
   else ((__nv_bfloat16*)g.out)[at] = __float2bfloat16_rn(v);
@@ -174,22 +174,24 @@ __device__ __forceinline__ void write_block(const Result& g, const uint32_t (&r)
 }
 
 // Sixteen bytes of a row from k on, zeros behind its end, where the row may start
-// at any byte.  Eight neighbours in a warp read the row's 128 bytes of a stage
+// at any byte.  L neighbours in a warp read 16 L bytes of the row
 // as the 16-byte vectors that hold them (all within the allocation that holds
 // the row), and take what they lack from each other.
+template <int L>
 __device__ __forceinline__ void read_start(const int8_t* row, int k, int depth, int lane, uint4& own, uint4& next) {
   const int8_t* p = row + k;
   const int off = (int)((uintptr_t)p & 15);
   own = next = make_uint4(0, 0, 0, 0);
   if (!row) return;
   if (k - off < depth) own = *(const uint4*)(p - off);
-  if (off && (lane & 7) == 7 && k + 16 - off < depth) next = *(const uint4*)(p - off + 16);
+  if (off && (lane & (L - 1)) == L - 1 && k + 16 - off < depth) next = *(const uint4*)(p - off + 16);
 }
 
+template <int L>
 __device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, int lane, const uint4& own, uint4 next) {
   const uint4 beside = make_uint4(__shfl_down_sync(0xFFFFFFFFu, own.x, 1), __shfl_down_sync(0xFFFFFFFFu, own.y, 1),
                                   __shfl_down_sync(0xFFFFFFFFu, own.z, 1), __shfl_down_sync(0xFFFFFFFFu, own.w, 1));
-  if ((lane & 7) != 7) next = beside;
+  if ((lane & (L - 1)) != L - 1) next = beside;
   const int off = (int)((uintptr_t)(row + k) & 15), have = depth - k;
   uint32_t w[8] = {own.x, own.y, own.z, own.w, next.x, next.y, next.z, next.w};
   if (off & 8) {
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
           return r < g.to.channels ? g.b + r * g.b_stride : nullptr;
         };
 #pragma unroll
-        for (int j = 0; j < kRows; j++) read_start(row_of(j), k, g.depth, lane, own[j], next[j]);
+        for (int j = 0; j < kRows; j++) read_start<8>(row_of(j), k, g.depth, lane, own[j], next[j]);
         if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
 #pragma unroll
         for (int j = 0; j < kRows; j++) {
           const int r = id / 8 + j * (kReaders / 8);
-          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end(row_of(j), k, g.depth, lane, own[j], next[j]);
+          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end<8>(row_of(j), k, g.depth, lane, own[j], next[j]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_co
       const int* p = g.part + tile * g.splits * size + t % tile_n * kTileM + c % kTileM;
       for (int s = 0; s < g.splits; s++) sum += p[s * size];
     }
-    put(g.to, t, c, sum);
+    put(g.to, t, c, sum, g.to.a_scale ? g.to.a_scale[t] : 0.0f);
   }
 }
 
@@ -463,6 +465,166 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const int8_t* from, 
         if (e < have) w[e >> 2] |= (uint32_t)(uint8_t)p[e] << ((e & 3) * 8);
     }
     *(uint4*)(to + r * to_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// -------------------------------------------------------- few tokens
+
+// Up to eight tokens are bound by the weight's bytes.  A block takes a few
+// channels, its warps take 512 bytes of their rows in turn, so that everything
+// there is to load is under way at once (4096 x 4096: one load of each of eight rows
+// for each lane); the tokens are in shared memory, where a block quantises one or two by
+// itself.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int kFewTokens = 8;
+constexpr int kFewSmem = 96 << 10;
+constexpr int kFewOwn = 8192;            // values of tokens that each block quantises for itself
+template <int T> constexpr int kFewChannels = T <= 4 ? 8 : 4;
+
+struct FewArgs {
+  Result to;
+  const void* a;
+  int a_dtype, a_vectors;  // vectors: rows of the tokens start on 16-byte boundaries
+  int64_t a_stride;
+  const int8_t* b;
+  int64_t b_stride;
+  int depth, padded;       // to whole turns of a warp
+  int early;               // only the kernel that quantised the tokens ran since the weight may have changed
+};
+
+// Tokens as whole numbers in shared memory, zeros behind them.
+template <class V, int E, int T>
+__device__ __forceinline__ void few_quantise(const FewArgs& g, int8_t* x, float* scales, uint32_t* keys) {
+  const int groups = (g.depth + E - 1) / E;
+#pragma unroll 1
+  for (int t = 0; t < g.to.tokens; t++) {
+    const V* in = (const V*)g.a + t * g.a_stride;
+    uint32_t key = 0;
+    for (int c = threadIdx.x; c < groups; c += kFewThreads) {
+      Group<V, E> v;
+      load_group(v, in + c * E, g.depth - c * E);
+      key = group_key(v, key);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) key = key_max<V>(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) keys[threadIdx.x / 32] = key;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kFewWarps; j++) key = key_max<V>(key, keys[j]);
+    const Scale s(key_value<V>(key));
+    if (threadIdx.x == 0) scales[t] = s.scale;
+    for (int c = threadIdx.x; c < groups; c += kFewThreads) {
+      Group<V, E> v;
+      load_group(v, in + c * E, g.depth - c * E);
+      uint32_t w[E > 4 ? 2 : 1];
+      quantise_group(v, s, w);
+      store_levels<E>(x + t * g.padded + c * E, w, g.depth - c * E);
+    }
+  }
+}
+
+template <int T, bool READ>
+__global__ void __launch_bounds__(kFewThreads) int8_few_kernel(const __grid_constant__ FewArgs g) {
+  constexpr int C = kFewChannels<T>;
+  extern __shared__ __align__(16) int8_t x[];
+  __shared__ float scales[T];
+  __shared__ uint32_t keys[kFewWarps];
+  __shared__ int parts[kFewWarps][C * T];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = (int64_t)blockIdx.x * C;
+  const int8_t* b = g.b;
+  auto row_of = [&](int j) { return c0 + j < g.to.channels ? b + (c0 + j) * g.b_stride : nullptr; };
+  uint4 own[C], next[READ ? C : 1];
+  auto load = [&](int k) {
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+      const int8_t* row = row_of(j);
+      if (READ) {
+        read_start<32>(row, k, g.depth, lane, own[j], next[READ ? j : 0]);
+      } else {
+        own[j] = make_uint4(0, 0, 0, 0);
+        if (row && k < g.depth) own[j] = *(const uint4*)(row + k);  // what lies behind the row meets zeros
+      }
+    }
+  };
+  if (!g.early) pdl_begin();
+  load(warp * 512 + lane * 16);
+  if (g.early) pdl_begin();
+
+  for (int i = threadIdx.x * 16; i < T * g.padded; i += kFewThreads * 16) *(uint4*)(x + i) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  if (T <= 2 && g.a_dtype != DCF_I8) {
+    if constexpr (T <= 2) {
+      if (g.a_dtype == DCF_F32) g.a_vectors ? few_quantise<float, 4, T>(g, x, scales, keys) : few_quantise<float, 1, T>(g, x, scales, keys);
+      else if (g.a_dtype == DCF_F16) g.a_vectors ? few_quantise<__half, 8, T>(g, x, scales, keys) : few_quantise<__half, 1, T>(g, x, scales, keys);
+      else g.a_vectors ? few_quantise<__nv_bfloat16, 8, T>(g, x, scales, keys) : few_quantise<__nv_bfloat16, 1, T>(g, x, scales, keys);
+    }
+  } else {
+    for (int t = 0; t < g.to.tokens; t++) {
+      const int8_t* in = (const int8_t*)g.a + t * g.a_stride;
+      if (g.a_vectors) {
+        for (int k = threadIdx.x * 16; k < g.depth; k += kFewThreads * 16) {
+          uint4 v = *(const uint4*)(in + k);
+          uint32_t* w = (uint32_t*)&v;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int here = g.depth - k - 4 * e;
+            if (here < 4) w[e] = here > 0 ? w[e] & (0xFFFFFFFFu >> (32 - 8 * here)) : 0u;
+          }
+          *(uint4*)(x + t * g.padded + k) = v;
+        }
+      } else {
+        for (int k = threadIdx.x; k < g.depth; k += kFewThreads) x[t * g.padded + k] = in[k];
+      }
+    }
+    if (threadIdx.x < g.to.tokens && g.to.a_scale) scales[threadIdx.x] = g.to.a_scale[threadIdx.x];
+  }
+  __syncthreads();
+
+  int sum[C][T];
+#pragma unroll
+  for (int j = 0; j < C; j++)
+#pragma unroll
+    for (int t = 0; t < T; t++) sum[j][t] = 0;
+  for (int k0 = warp * 512; k0 < g.depth; k0 += kFewWarps * 512) {
+    const int k = k0 + lane * 16;
+    uint4 w[C];
+#pragma unroll
+    for (int j = 0; j < C; j++) {
+      if constexpr (READ) w[j] = read_end<32>(row_of(j), k, g.depth, lane, own[j], next[j]);
+      else w[j] = own[j];
+    }
+    if (k0 + kFewWarps * 512 < g.depth) load(k + kFewWarps * 512);
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const uint4 v = *(const uint4*)(x + t * g.padded + k);
+#pragma unroll
+      for (int j = 0; j < C; j++) {
+        sum[j][t] = __dp4a((int)w[j].x, (int)v.x, sum[j][t]);
+        sum[j][t] = __dp4a((int)w[j].y, (int)v.y, sum[j][t]);
+        sum[j][t] = __dp4a((int)w[j].z, (int)v.z, sum[j][t]);
+        sum[j][t] = __dp4a((int)w[j].w, (int)v.w, sum[j][t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < C; j++)
+#pragma unroll
+    for (int t = 0; t < T; t++) {
+      const int all = __reduce_add_sync(0xFFFFFFFFu, sum[j][t]);
+      if (lane == (t * C + j) % 32) parts[warp][t * C + j] = all;
+    }
+  __syncthreads();
+  if (threadIdx.x < C * T) {
+    const int t = threadIdx.x / C;
+    const int64_t c = c0 + threadIdx.x % C;
+    if (t < g.to.tokens && c < g.to.channels) {
+      int all = 0;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; w++) all += parts[w][threadIdx.x];
+      put(g.to, t, c, all, scales[t]);
+    }
   }
 }
 
@@ -517,11 +679,18 @@ Cut cut_of(const dcf_int8_desc& d) {
 // copy of whole numbers that no tensor map describes), a copy of a weight whose stride no
 // tensor map takes, and the parts of sums.
 struct Layout {
+  bool few, own;           // few tokens; each block quantises them
   Cut cut;
   int64_t stride;
   bool copy_b;
   size_t a, scale, b, part, bytes;
 };
+
+int few_padded(const dcf_int8_desc& d) { return (int)((d.depth + 511) / 512 * 512); }
+int few_bucket(const dcf_int8_desc& d) { return d.tokens <= 1 ? 1 : d.tokens <= 2 ? 2 : d.tokens <= 4 ? 4 : 8; }
+bool few(const dcf_int8_desc& d) {
+  return d.tokens <= kFewTokens && d.depth && few_bucket(d) * few_padded(d) <= kFewSmem;
+}
 
 // A weight whose rows lie off 16-byte boundaries is read by threads as long as few tokens leave that hidden
 // behind HBM; many have it copied first.
@@ -532,14 +701,36 @@ Layout layout_of(const dcf_int8_desc& d) {
     l.bytes += (bytes + 255) / 256 * 256;
     return at;
   };
-  l.cut = cut_of(d);
   l.stride = (int64_t)((d.depth + 15) / 16 * 16);
+  l.few = few(d);
+  if (l.few) {
+    l.own = d.a_dtype == DCF_I8 || (d.tokens <= 2 && d.tokens * d.depth <= kFewOwn);
+    l.a = take(l.own ? 0 : (size_t)d.tokens * l.stride);
+    l.scale = take(l.own ? 0 : (size_t)d.tokens * 4);
+    return l;
+  }
+  l.cut = cut_of(d);
   l.a = take((size_t)d.tokens * l.stride);
   l.scale = take(d.a_dtype != DCF_I8 ? (size_t)d.tokens * 4 : 0);
   l.copy_b = l.cut.tile_n > 64 && d.channels > 1 && stride_of(d.b_row_stride, d.depth) % 16;
   l.b = take(l.copy_b ? (size_t)d.channels * l.stride : 0);
   l.part = take(l.cut.splits > 1 ? (size_t)l.cut.tiles * l.cut.splits * kTileM * l.cut.tile_n * 4 : 0);
   return l;
+}
+
+template <int T, bool READ> int few_run(const FewArgs& g, cudaStream_t s) {
+  if (!prepare_smem((const void*)int8_few_kernel<T, READ>, kFewSmem)) return DCF_ECUDA;
+  const unsigned blocks = (unsigned)(((int64_t)g.to.channels + kFewChannels<T> - 1) / kFewChannels<T>);
+  return launch(int8_few_kernel<T, READ>, dim3(blocks), kFewThreads, T * g.padded, 1, s, g);
+}
+
+template <bool READ> int few_product(int bucket, const FewArgs& g, cudaStream_t s) {
+  switch (bucket) {
+    case 1: return few_run<1, READ>(g, s);
+    case 2: return few_run<2, READ>(g, s);
+    case 4: return few_run<4, READ>(g, s);
+    default: return few_run<8, READ>(g, s);
+  }
 }
 
 template <int TN, bool READ>
@@ -594,25 +785,46 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     *stride = l.stride;
     return rc;
   };
-  const int8_t* q = (const int8_t*)a;
   int rc = DCF_OK;
-  if (d.a_dtype != DCF_I8) {
+  const bool ours = d.a_dtype != DCF_I8 && !l.own;  // tokens to quantise first
+  if (ours) {
     const dcf_quant_desc tokens = {d.a_dtype, DCF_QUANT_ROWS, d.tokens, d.depth, as, l.stride};
-    q = (int8_t*)work + l.a;
     a_scale = (float*)(work + l.scale);
     as = l.stride;
-    if ((rc = launch_quantize(tokens, a, (int8_t*)q, (float*)a_scale, s))) return rc;
+    if ((rc = launch_quantize(tokens, a, (int8_t*)work + l.a, (float*)a_scale, s))) return rc;
+    a = work + l.a;
   }
+  Result to;
+  to.a_scale = a_scale;
+  to.b_scale = b_scale;
+  to.bias = bias;
+  to.out = out;
+  to.out_dtype = (int)d.out_dtype;
+  to.tokens = (int)d.tokens;
+  to.channels = (int)d.channels;
+  to.stride = stride_of(d.out_row_stride, d.channels);
+  to.pairs = (uintptr_t)out % 4 == 0 && (d.tokens == 1 || to.stride % 2 == 0);
+  auto on16 = [&](const void* p, int64_t stride, uint64_t rows, size_t es) {
+    return (uintptr_t)p % 16 == 0 && (rows == 1 || stride * (int64_t)es % 16 == 0);
+  };
+  if (l.few) {
+    FewArgs g = {};
+    g.to = to;
+    g.a = a;
+    g.a_dtype = (int)(ours ? (uint32_t)DCF_I8 : d.a_dtype);
+    g.a_stride = as;
+    g.a_vectors = on16(a, as, d.tokens, dtype_size(g.a_dtype));
+    g.b = b;
+    g.b_stride = bs;
+    g.depth = (int)d.depth;
+    g.padded = few_padded(d);
+    g.early = ours;
+    const int bucket = few_bucket(d);
+    return on16(b, bs, d.channels, 1) ? few_product<false>(bucket, g, s) : few_product<true>(bucket, g, s);
+  }
+  const int8_t* q = (const int8_t*)a;
   GemmArgs g = {};
-  g.to.a_scale = a_scale;
-  g.to.b_scale = b_scale;
-  g.to.bias = bias;
-  g.to.out = out;
-  g.to.out_dtype = (int)d.out_dtype;
-  g.to.tokens = (int)d.tokens;
-  g.to.channels = (int)d.channels;
-  g.to.stride = stride_of(d.out_row_stride, d.channels);
-  g.to.pairs = (uintptr_t)out % 4 == 0 && (d.tokens == 1 || g.to.stride % 2 == 0);
+  g.to = to;
   g.blocks = (int)((d.depth + kBK - 1) / kBK);
   g.tiles_m = (int)cut.tiles_m;
   g.splits = d.depth ? cut.splits : 0;

@@ -68,17 +68,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const QuantAr
     if (at == 0) a.scale[r] = s.scale;
     int8_t* q = a.q + r * a.qs;
     auto write = [&](Group<T, E>& v, int c) {
-#pragma unroll
-      for (int j = 0; j < Group<T, E>::kWords; j++) v.w[j] &= s.keep;
       uint32_t w[E > 4 ? 2 : 1];
-      if constexpr (E == 1) {
-        w[0] = level(group_value(v, 0), s.factor);
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; j += 4)
-          w[j / 4] = pack4(level(group_value(v, j), s.factor), level(group_value(v, j + 1), s.factor),
-                           level(group_value(v, j + 2), s.factor), level(group_value(v, j + 3), s.factor));
-      }
+      quantise_group(v, s, w);
       store_levels<E>(q + (int64_t)c * E, w, a.cols - c * E);
     };
     for (int c = at; c < first; c += TPR) {

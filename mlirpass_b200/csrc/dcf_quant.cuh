@@ -105,6 +105,21 @@ template <class T, int E> __device__ __forceinline__ float group_value(const Gro
   else return __uint_as_float(j & 1 ? g.w[j >> 1] & 0xFFFF0000u : g.w[j >> 1] << 16);
 }
 
+// The whole numbers of a group, all beside the same largest magnitude.
+template <class T, int E>
+__device__ __forceinline__ void quantise_group(Group<T, E>& v, const Scale& s, uint32_t (&w)[E > 4 ? 2 : 1]) {
+#pragma unroll
+  for (int j = 0; j < Group<T, E>::kWords; j++) v.w[j] &= s.keep;
+  if constexpr (E == 1) {
+    w[0] = level(group_value(v, 0), s.factor);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; j += 4)
+      w[j / 4] = pack4(level(group_value(v, j), s.factor), level(group_value(v, j + 1), s.factor),
+                       level(group_value(v, j + 2), s.factor), level(group_value(v, j + 3), s.factor));
+  }
+}
+
 // The first `have` bytes of q's words to p, which vectors of E bytes divide.
 template <int E> __device__ __forceinline__ void store_levels(int8_t* p, const uint32_t* w, int have) {
   if constexpr (E == 1) {
