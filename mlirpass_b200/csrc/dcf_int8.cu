@@ -14,7 +14,7 @@ constexpr int kTileM = 2 * kSide;         // of a pair
 constexpr int kBK = 128;                  // k of a stage: one 128-byte swizzle row
 template <bool READ> constexpr int kOutWarps = READ ? 8 : 16;  // warps that write results
 template <bool READ> constexpr int kGemmThreads = 128 + 32 * kOutWarps<READ>;  // warp 0 loads, warp 1 multiplies
-constexpr int kReaders = 128;             // threads that read a weight's rows where no tensor map describes them
+constexpr int kReaders = 256;             // threads that read a weight's rows where no tensor map describes them
 constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
 
 // What becomes of sums.
@@ -29,19 +29,15 @@ struct Result {
   int64_t stride;
 };
 
-__device__ __forceinline__ float scaled(int sum, float a, float b, float bias, bool add) {
-  const float v = __fmul_rn(__fmul_rn((float)sum, a), b);
-  return add ? __fadd_rn(v, bias) : v;
-}
-
-// The result of one token and channel.
-__device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int sum, float a_scale) {
+// The result of one token and channel; a bias of -0 adds nothing to any value.
+__device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int sum, float a_scale, float b_scale,
+                                    float bias) {
   const int64_t at = t * g.stride + c;
   if (g.out_dtype == DCF_I32) {
     ((int*)g.out)[at] = sum;
     return;
   }
-  const float v = scaled(sum, a_scale, g.b_scale[c], g.bias ? g.bias[c] : 0.0f, g.bias != nullptr);
+  const float v = __fadd_rn(__fmul_rn(__fmul_rn((float)sum, a_scale), b_scale), bias);
   if (g.out_dtype == DCF_F32) ((float*)g.out)[at] = v;
   else if (g.out_dtype == DCF_F16) ((__half*)g.out)[at] = __float2half_rn(v);
   else ((__nv_bfloat16*)g.out)[at] = __float2bfloat16_rn(v);
@@ -332,20 +328,38 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     }
   } else if (warp >= 4 + OW) {
     const int id = threadIdx.x - kGemmThreads<READ>, chunk = id & 7;
-    Ring<S> at;
-    for (int64_t t = first; t < g.total && !fail; t += step) {
-      const int64_t row0 = (t / g.splits) % g.tiles_m * kTileM + rank * kSide;
-      const int b0 = begin_of(t), blocks = count_of(t);
-      for (int b = 0; b < blocks; b++, at.next()) {
-        const int k = (b0 + b) * kBK + chunk * 16;
-        constexpr int kRows = kSide * 8 / kReaders;
-        uint4 own[kRows], next[kRows];
-        auto row_of = [&](int j) {
-          const int64_t r = row0 + id / 8 + j * (kReaders / 8);
-          return r < g.to.channels ? g.b + r * g.b_stride : nullptr;
-        };
+    constexpr int kRows = kSide * 8 / kReaders;
+    uint4 own[kRows], next[kRows];
+    const int8_t* rows[kRows];
+    auto rows_of = [&](int64_t t) {
 #pragma unroll
-        for (int j = 0; j < kRows; j++) read_start<8>(row_of(j), k, g.depth, lane, own[j], next[j]);
+      for (int j = 0; j < kRows; j++) {
+        const int64_t r = (t / g.splits) % g.tiles_m * kTileM + rank * kSide + id / 8 + j * (kReaders / 8);
+        rows[j] = r < g.to.channels ? g.b + r * g.b_stride : nullptr;
+      }
+    };
+    auto read = [&](int k) {
+#pragma unroll
+      for (int j = 0; j < kRows; j++) read_start<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
+    };
+    Ring<S> at;
+    if (first < g.total) {
+      rows_of(first);
+      read(begin_of(first) * kBK);
+    }
+    for (int64_t t = first; t < g.total && !fail; t += step) {
+      const int k0 = begin_of(t) * kBK, end = k0 + count_of(t) * kBK;
+      for (int k = k0; k < end; k += kBK, at.next()) {
+        uint4 v[kRows];
+#pragma unroll
+        for (int j = 0; j < kRows; j++) v[j] = read_end<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
+        // The next stage is on its way while this one waits for room.
+        if (k + kBK < end) {
+          read(k + kBK);
+        } else if (t + step < g.total) {
+          rows_of(t + step);
+          read(begin_of(t + step) * kBK);
+        }
         if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
@@ -354,7 +368,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
 #pragma unroll
         for (int j = 0; j < kRows; j++) {
           const int r = id / 8 + j * (kReaders / 8);
-          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = read_end<8>(row_of(j), k, g.depth, lane, own[j], next[j]);
+          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = v[j];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
@@ -435,7 +449,9 @@ __global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_co
       const int* p = g.part + tile * g.splits * size + t % tile_n * kTileM + c % kTileM;
       for (int s = 0; s < g.splits; s++) sum += p[s * size];
     }
-    put(g.to, t, c, sum, g.to.a_scale ? g.to.a_scale[t] : 0.0f);
+    const bool scaled = g.to.b_scale != nullptr;
+    put(g.to, t, c, sum, scaled ? g.to.a_scale[t] : 0.0f, scaled ? g.to.b_scale[c] : 0.0f,
+        g.to.bias ? g.to.bias[c] : -0.0f);
   }
 }
 
@@ -470,16 +486,23 @@ __global__ void __launch_bounds__(kPackThreads) pack_kernel(const int8_t* from, 
 
 // -------------------------------------------------------- few tokens
 
-// Up to eight tokens are bound by the weight's bytes.  A block takes a few
-// channels, its warps take 512 bytes of their rows in turn, so that everything
-// there is to load is under way at once (4096 x 4096: one load of each of eight rows
-// for each lane); the tokens are in shared memory, where a block quantises one or two by
-// itself.
+// Up to four tokens are bound by the weight's bytes.  A group of warps takes
+// eight channels, its warps 32 vectors of 16 bytes of their rows in turn (eight
+// loads in each lane, the next eight under way while these are multiplied).
+// More than one warp to a group only where there are too few channels: joining
+// their sums makes warps wait for each other.  The tokens are in shared memory,
+// where a block quantises them itself while that is little work.  One wave of
+// blocks takes all channels in turns.
+//
+// A weight off 16-byte boundaries is read as the vectors that hold its rows
+// (all within the allocation that holds the row), and each lane makes up its sixteen
+// bytes from its vector and its neighbour's; the last lane lends its vector only.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
-constexpr int kFewTokens = 8;
-constexpr int kFewSmem = 96 << 10;
+constexpr int kFewTokens = 4, kFewChannels = 8;
+constexpr int kFewResident = 2;          // blocks to an SM
+template <bool READ> constexpr int kFewBytes = READ ? 31 * 16 : 32 * 16;  // of a row that a warp takes
+constexpr int kFewSmem = 64 << 10;
 constexpr int kFewOwn = 8192;            // values of tokens that each block quantises for itself
-template <int T> constexpr int kFewChannels = T <= 4 ? 8 : 4;
 
 struct FewArgs {
   Result to;
@@ -488,78 +511,94 @@ struct FewArgs {
   int64_t a_stride;
   const int8_t* b;
   int64_t b_stride;
-  int depth, padded;       // to whole turns of a warp
+  int depth, padded;       // padded: to whole turns of a warp, and a vector of zeros
+  int across;              // warps along the depth
   int early;               // only the kernel that quantised the tokens ran since the weight may have changed
 };
 
-// Tokens as whole numbers in shared memory, zeros behind them.
+// Sixteen bytes from byte `off` of a lane's vector and the next lane's on.
+__device__ __forceinline__ uint4 shifted_down(const uint4& own, int off) {
+  uint32_t w[8] = {own.x, own.y, own.z, own.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[4 + j] = __shfl_down_sync(0xFFFFFFFFu, w[j], 1);
+  if (off & 8) {
+#pragma unroll
+    for (int j = 0; j < 6; j++) w[j] = w[j + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int j = 0; j < 5; j++) w[j] = w[j + 1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Tokens as whole numbers in shared memory, zeros behind them; warps share a token.
 template <class V, int E, int T>
 __device__ __forceinline__ void few_quantise(const FewArgs& g, int8_t* x, float* scales, uint32_t* keys) {
-  const int groups = (g.depth + E - 1) / E;
-#pragma unroll 1
-  for (int t = 0; t < g.to.tokens; t++) {
-    const V* in = (const V*)g.a + t * g.a_stride;
-    uint32_t key = 0;
-    for (int c = threadIdx.x; c < groups; c += kFewThreads) {
+  constexpr int kShare = kFewThreads / T;  // threads to a token
+  const int groups = (g.depth + E - 1) / E, t = threadIdx.x / kShare, first = threadIdx.x % kShare;
+  const V* in = (const V*)g.a + t * g.a_stride;
+  const bool there = t < g.to.tokens;
+  uint32_t key = 0;
+  if (there) {
+    for (int c = first; c < groups; c += kShare) {
       Group<V, E> v;
       load_group(v, in + c * E, g.depth - c * E);
       key = group_key(v, key);
     }
+  }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) key = key_max<V>(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) keys[threadIdx.x / 32] = key;
-    __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) key = key_max<V>(key, __shfl_xor_sync(0xFFFFFFFFu, key, o));
+  if (threadIdx.x % 32 == 0) keys[threadIdx.x / 32] = key;
+  __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kFewWarps; j++) key = key_max<V>(key, keys[j]);
-    const Scale s(key_value<V>(key));
-    if (threadIdx.x == 0) scales[t] = s.scale;
-    for (int c = threadIdx.x; c < groups; c += kFewThreads) {
-      Group<V, E> v;
-      load_group(v, in + c * E, g.depth - c * E);
-      uint32_t w[E > 4 ? 2 : 1];
-      quantise_group(v, s, w);
-      store_levels<E>(x + t * g.padded + c * E, w, g.depth - c * E);
-    }
+  for (int j = 0; j < kShare / 32; j++) key = key_max<V>(key, keys[t * (kShare / 32) + j]);
+  const Scale s(key_value<V>(key));
+  if (!there) return;
+  if (first == 0) scales[t] = s.scale;
+  for (int c = first; c < groups; c += kShare) {
+    Group<V, E> v;
+    load_group(v, in + c * E, g.depth - c * E);
+    uint32_t w[E > 4 ? 2 : 1];
+    quantise_group(v, s, w);
+    store_levels<E>(x + t * g.padded + c * E, w, g.depth - c * E);
   }
 }
 
 template <int T, bool READ>
-__global__ void __launch_bounds__(kFewThreads) int8_few_kernel(const __grid_constant__ FewArgs g) {
-  constexpr int C = kFewChannels<T>;
+__global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(const __grid_constant__ FewArgs args) {
+  const FewArgs g = args;
+  constexpr int C = kFewChannels;
   extern __shared__ __align__(16) int8_t x[];
   __shared__ float scales[T];
   __shared__ uint32_t keys[kFewWarps];
-  __shared__ int parts[kFewWarps][C * T];
+  __shared__ int parts[2][kFewWarps][C * T];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t c0 = (int64_t)blockIdx.x * C;
-  const int8_t* b = g.b;
-  auto row_of = [&](int j) { return c0 + j < g.to.channels ? b + (c0 + j) * g.b_stride : nullptr; };
-  uint4 own[C], next[READ ? C : 1];
-  auto load = [&](int k) {
-#pragma unroll
-    for (int j = 0; j < C; j++) {
-      const int8_t* row = row_of(j);
-      if (READ) {
-        read_start<32>(row, k, g.depth, lane, own[j], next[READ ? j : 0]);
-      } else {
-        own[j] = make_uint4(0, 0, 0, 0);
-        if (row && k < g.depth) own[j] = *(const uint4*)(row + k);  // what lies behind the row meets zeros
-      }
-    }
+  const int groups = kFewWarps / g.across, start = warp % g.across * kFewBytes<READ>, turn = g.across * kFewBytes<READ>;
+  const int64_t step = (int64_t)gridDim.x * groups * C;
+  int64_t c0 = ((int64_t)blockIdx.x * groups + warp / g.across) * C;
+  uint4 own[C];
+  auto load = [&](int j, int64_t c, int k) {  // row c + j
+    const int8_t* p = g.b + (c + j) * g.b_stride + k + lane * 16;
+    const int off = READ ? (int)((uintptr_t)p & 15) : 0;  // bytes before the row, or the end of the vector before
+    own[j] = make_uint4(0, 0, 0, 0);
+    if (c + j < g.to.channels && k + lane * 16 - off < g.depth) own[j] = *(const uint4*)(p - off);  // what else they hold meets zeros
   };
   if (!g.early) pdl_begin();
-  load(warp * 512 + lane * 16);
+#pragma unroll
+  for (int j = 0; j < C; j++) load(j, c0, start);
   if (g.early) pdl_begin();
 
   for (int i = threadIdx.x * 16; i < T * g.padded; i += kFewThreads * 16) *(uint4*)(x + i) = make_uint4(0, 0, 0, 0);
   __syncthreads();
-  if (T <= 2 && g.a_dtype != DCF_I8) {
-    if constexpr (T <= 2) {
-      if (g.a_dtype == DCF_F32) g.a_vectors ? few_quantise<float, 4, T>(g, x, scales, keys) : few_quantise<float, 1, T>(g, x, scales, keys);
-      else if (g.a_dtype == DCF_F16) g.a_vectors ? few_quantise<__half, 8, T>(g, x, scales, keys) : few_quantise<__half, 1, T>(g, x, scales, keys);
-      else g.a_vectors ? few_quantise<__nv_bfloat16, 8, T>(g, x, scales, keys) : few_quantise<__nv_bfloat16, 1, T>(g, x, scales, keys);
-    }
+  if (g.a_dtype == DCF_F32) {
+    g.a_vectors ? few_quantise<float, 4, T>(g, x, scales, keys) : few_quantise<float, 1, T>(g, x, scales, keys);
+  } else if (g.a_dtype == DCF_F16) {
+    g.a_vectors ? few_quantise<__half, 8, T>(g, x, scales, keys) : few_quantise<__half, 1, T>(g, x, scales, keys);
+  } else if (g.a_dtype == DCF_BF16) {
+    g.a_vectors ? few_quantise<__nv_bfloat16, 8, T>(g, x, scales, keys) : few_quantise<__nv_bfloat16, 1, T>(g, x, scales, keys);
   } else {
     for (int t = 0; t < g.to.tokens; t++) {
       const int8_t* in = (const int8_t*)g.a + t * g.a_stride;
@@ -582,49 +621,61 @@ __global__ void __launch_bounds__(kFewThreads) int8_few_kernel(const __grid_cons
   }
   __syncthreads();
 
-  int sum[C][T];
+  for (int buffer = 0; c0 < g.to.channels; c0 += step, buffer ^= 1) {
+    int sum[C][T];
 #pragma unroll
-  for (int j = 0; j < C; j++)
+    for (int j = 0; j < C; j++)
 #pragma unroll
-    for (int t = 0; t < T; t++) sum[j][t] = 0;
-  for (int k0 = warp * 512; k0 < g.depth; k0 += kFewWarps * 512) {
-    const int k = k0 + lane * 16;
-    uint4 w[C];
-#pragma unroll
-    for (int j = 0; j < C; j++) {
-      if constexpr (READ) w[j] = read_end<32>(row_of(j), k, g.depth, lane, own[j], next[j]);
-      else w[j] = own[j];
+      for (int t = 0; t < T; t++) sum[j][t] = 0;
+    // What the result of this lane, token lane / C of channel lane % C, is multiplied by.
+    const int id = lane % (C * T);
+    const int64_t c = c0 + id % C;
+    const bool mine = lane < C * T && c < g.to.channels && id / C < g.to.tokens;
+    float b = 0, bias = -0.0f;
+    if (mine && g.to.b_scale) {
+      b = g.to.b_scale[c];
+      if (g.to.bias) bias = g.to.bias[c];
     }
-    if (k0 + kFewWarps * 512 < g.depth) load(k + kFewWarps * 512);
-#pragma unroll
-    for (int t = 0; t < T; t++) {
-      const uint4 v = *(const uint4*)(x + t * g.padded + k);
+    for (int k0 = start; k0 < g.depth; k0 += turn) {
+      uint4 w[C];
 #pragma unroll
       for (int j = 0; j < C; j++) {
-        sum[j][t] = __dp4a((int)w[j].x, (int)v.x, sum[j][t]);
-        sum[j][t] = __dp4a((int)w[j].y, (int)v.y, sum[j][t]);
-        sum[j][t] = __dp4a((int)w[j].z, (int)v.z, sum[j][t]);
-        sum[j][t] = __dp4a((int)w[j].w, (int)v.w, sum[j][t]);
+        w[j] = own[j];
+        if (READ) w[j] = shifted_down(w[j], (int)((uintptr_t)(g.b + (c0 + j) * g.b_stride) & 15));
+      }
+      const bool more = k0 + turn < g.depth;
+#pragma unroll
+      for (int j = 0; j < C; j++) load(j, more ? c0 : c0 + step, more ? k0 + turn : start);
+      const int k = READ && lane == 31 ? g.padded - 16 : k0 + lane * 16;
+#pragma unroll
+      for (int t = 0; t < T; t++) {
+        const uint4 v = *(const uint4*)(x + t * g.padded + k);
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+          sum[j][t] = __dp4a((int)w[j].x, (int)v.x, sum[j][t]);
+          sum[j][t] = __dp4a((int)w[j].y, (int)v.y, sum[j][t]);
+          sum[j][t] = __dp4a((int)w[j].z, (int)v.z, sum[j][t]);
+          sum[j][t] = __dp4a((int)w[j].w, (int)v.w, sum[j][t]);
+        }
       }
     }
-  }
+    int all = 0;
 #pragma unroll
-  for (int j = 0; j < C; j++)
+    for (int j = 0; j < C; j++)
 #pragma unroll
-    for (int t = 0; t < T; t++) {
-      const int all = __reduce_add_sync(0xFFFFFFFFu, sum[j][t]);
-      if (lane == (t * C + j) % 32) parts[warp][t * C + j] = all;
+      for (int t = 0; t < T; t++) {
+        const int one = __reduce_add_sync(0xFFFFFFFFu, sum[j][t]);
+        if (lane == t * C + j) all = one;
+      }
+    if (g.across > 1) {
+      const int group = warp / g.across;
+      if (lane < C * T) parts[buffer][warp][id] = all;
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(g.across * 32) : "memory");
+      if (warp % g.across) continue;
+      all = 0;
+      for (int w = 0; w < g.across; w++) all += parts[buffer][warp + w][id];
     }
-  __syncthreads();
-  if (threadIdx.x < C * T) {
-    const int t = threadIdx.x / C;
-    const int64_t c = c0 + threadIdx.x % C;
-    if (t < g.to.tokens && c < g.to.channels) {
-      int all = 0;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; w++) all += parts[w][threadIdx.x];
-      put(g.to, t, c, all, scales[t]);
-    }
+    if (mine) put(g.to, id / C, c, all, scales[id / C], b, bias);
   }
 }
 
@@ -686,8 +737,9 @@ struct Layout {
   size_t a, scale, b, part, bytes;
 };
 
-int few_padded(const dcf_int8_desc& d) { return (int)((d.depth + 511) / 512 * 512); }
-int few_bucket(const dcf_int8_desc& d) { return d.tokens <= 1 ? 1 : d.tokens <= 2 ? 2 : d.tokens <= 4 ? 4 : 8; }
+// (Room for the turns of either width: 496 bytes reach less than 512 past the depth, too.)
+int few_padded(const dcf_int8_desc& d) { return (int)((d.depth + 511) / 512 * 512) + 512; }
+int few_bucket(const dcf_int8_desc& d) { return d.tokens <= 1 ? 1 : d.tokens <= 2 ? 2 : 4; }
 bool few(const dcf_int8_desc& d) {
   return d.tokens <= kFewTokens && d.depth && few_bucket(d) * few_padded(d) <= kFewSmem;
 }
@@ -704,7 +756,7 @@ Layout layout_of(const dcf_int8_desc& d) {
   l.stride = (int64_t)((d.depth + 15) / 16 * 16);
   l.few = few(d);
   if (l.few) {
-    l.own = d.a_dtype == DCF_I8 || (d.tokens <= 2 && d.tokens * d.depth <= kFewOwn);
+    l.own = d.a_dtype == DCF_I8 || d.tokens * d.depth <= kFewOwn;
     l.a = take(l.own ? 0 : (size_t)d.tokens * l.stride);
     l.scale = take(l.own ? 0 : (size_t)d.tokens * 4);
     return l;
@@ -720,16 +772,16 @@ Layout layout_of(const dcf_int8_desc& d) {
 
 template <int T, bool READ> int few_run(const FewArgs& g, cudaStream_t s) {
   if (!prepare_smem((const void*)int8_few_kernel<T, READ>, kFewSmem)) return DCF_ECUDA;
-  const unsigned blocks = (unsigned)(((int64_t)g.to.channels + kFewChannels<T> - 1) / kFewChannels<T>);
-  return launch(int8_few_kernel<T, READ>, dim3(blocks), kFewThreads, T * g.padded, 1, s, g);
+  const int smem = T * g.padded, each = kFewWarps / g.across * kFewChannels;
+  const int64_t blocks = ((int64_t)g.to.channels + each - 1) / each, wave = 2 * kPairs * kFewResident;
+  return launch(int8_few_kernel<T, READ>, dim3((unsigned)(blocks < wave ? blocks : wave)), kFewThreads, smem, 1, s, g);
 }
 
 template <bool READ> int few_product(int bucket, const FewArgs& g, cudaStream_t s) {
   switch (bucket) {
     case 1: return few_run<1, READ>(g, s);
     case 2: return few_run<2, READ>(g, s);
-    case 4: return few_run<4, READ>(g, s);
-    default: return few_run<8, READ>(g, s);
+    default: return few_run<4, READ>(g, s);
   }
 }
 
@@ -819,8 +871,13 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     g.depth = (int)d.depth;
     g.padded = few_padded(d);
     g.early = ours;
+    const int64_t groups = ((int64_t)d.channels + kFewChannels - 1) / kFewChannels;
+    for (g.across = 1; g.across < kFewWarps && g.across * 512 < (int)d.depth &&
+                       groups * g.across < 2 * kPairs * kFewResident * kFewWarps * 3 / 4;)
+      g.across *= 2;
     const int bucket = few_bucket(d);
-    return on16(b, bs, d.channels, 1) ? few_product<false>(bucket, g, s) : few_product<true>(bucket, g, s);
+    const bool read = !on16(b, bs, d.channels, 1);
+    return !read ? few_product<false>(bucket, g, s) : few_product<true>(bucket, g, s);
   }
   const int8_t* q = (const int8_t*)a;
   GemmArgs g = {};
