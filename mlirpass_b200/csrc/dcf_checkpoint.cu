@@ -1,23 +1,88 @@
 // dcf_checkpoint.cu — the gradient of a weight from a checkpoint of its
 // layer's input:
 //   out[c][k] = sum over runs r of scale[r][k] * (sum over t in r of grad[t][c] * q[t][k])
-// A whole number of 8 bits is exact in f16 and bf16, so the products of the
-// inner sum are exact in f32; the scale comes after it.
+// A whole number of 8 bits is exact in f16 and bf16, so the tensor cores
+// multiply it by the gradient as it is, and the products are exact in f32.  A
+// run's scale comes after its sum: TMEM sums the 128 tokens of a run, and
+// registers multiply that by the scale and add it, rounding to nearest.  (The
+// tensor core truncates as it accumulates; longer sums in TMEM would be further
+// from 64 bits than fp32 products are.)
 #include "dcf_quant.cuh"
 
 namespace dcf {
 
 namespace {
 
+constexpr int kSide = 128;                // k of a CTA
+constexpr int kTileM = 2 * kSide;         // of a pair
+constexpr int kReaders = 128;             // threads that turn whole numbers into the gradient's type
+constexpr int kOutWarps = 8;
+constexpr int kThreads_ = 128 + kReaders + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
+
+// A stage is a run: 128 tokens of 128 k and of TN / 2 channels in two bytes each, in
+// blocks of 64 that have a 128-byte row for each token.
+constexpr int kBlockBytes = kRun * 128;
+template <int TN> constexpr int kStage = (kSide + TN / 2) * kRun * 2;
+template <int TN> constexpr int kStages = TN == 256 ? 3 : 4;
+template <int TN> constexpr int kSmem = kStages<TN> * kStage<TN> + 256 + 1024;
+
 struct GradArgs {
-  const void* grad;
   const int8_t* q;
   const float* scale;
   void* out;
   int out_dtype, add;
+  int pairs;               // two neighbours of a row of a 16-bit result make an aligned word
   int tokens, channels, depth;
-  int64_t gs, qs, os;
+  int skip;                // columns of the gradient's map before its first channel
+  int64_t qs, os;
+  int runs, tiles_m;       // tiles along k
+  int splits, split_runs;  // parts of the runs, runs of each
+  int64_t total;           // tiles times splits
+  float* part;             // sums of the parts, where there is more than one
+  uint32_t idesc;
+  dcf_status* st;
 };
+
+__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+// An operand whose memory runs along it: blocks of 64 lie kBlockBytes apart,
+// groups of eight tokens 1024 bytes.
+__device__ __forceinline__ uint64_t block_desc(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kBlockBytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Two of a word's signed bytes (the low ones of its halves) in a 16-bit type.
+template <class T> __device__ __forceinline__ uint32_t to_halves(uint32_t h) {
+  if constexpr (std::is_same<T, __half>::value) {
+    // a byte, its sign turned, under the exponent of 1024: 1024 + 128 + q
+    const uint32_t m = (h ^ 0x00800080u) | 0x64006400u, c = 0x64806480u;
+    const __half2 r = __hsub2(*(const __half2*)&m, *(const __half2*)&c);
+    return *(const uint32_t*)&r;
+  } else {
+    // seven bits under the exponent of 128, less 128 or, beside the sign, 256
+    const uint32_t m = (h & 0x007F007Fu) | 0x43004300u, c = (h & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*(const __nv_bfloat162*)&m, *(const __nv_bfloat162*)&c);
+    return *(const uint32_t*)&r;
+  }
+}
+
+template <class T> __device__ __forceinline__ uint4 to_eight(uint32_t a, uint32_t b) {
+  return make_uint4(to_halves<T>(__byte_perm(a, 0, 0x4140)), to_halves<T>(__byte_perm(a, 0, 0x4342)),
+                    to_halves<T>(__byte_perm(b, 0, 0x4140)), to_halves<T>(__byte_perm(b, 0, 0x4342)));
+}
+
+// 512 threads start with 128 registers each; warps 0 to 3 keep 32, the four
+// that read 96, and the eight that add up get 192: 128 * 32 + 128 * 96 + 256 * 192 = 512 * 128.
+__device__ __forceinline__ void control_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 32;"); }
+__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 96;"); }
+__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); }
 
 __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, float v) {
   const int64_t at = c * g.os + k;
@@ -26,45 +91,378 @@ __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, flo
   else ((__nv_bfloat16*)g.out)[at] = __float2bfloat16_rn(v);
 }
 
-constexpr int kTile = 64, kDeep = 32;
-
-// 64 channels x 64 k to a block of 256 threads, sixteen results to a thread.
-template <class T> __global__ void __launch_bounds__(256) grad_tile_kernel(const GradArgs g) {
-  __shared__ float a[kDeep][kTile], b[kDeep][kTile];
-  pdl_begin();
-  const int64_t tiles = ((int64_t)g.depth + kTile - 1) / kTile, total = tiles * (((int64_t)g.channels + kTile - 1) / kTile);
-  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
-  for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
-    const int64_t c0 = i / tiles * kTile, k0 = i % tiles * kTile;
-    float sum[4][4] = {};
-    for (int64_t r0 = 0; r0 < g.tokens; r0 += kRun) {
-      float part[4][4] = {};
-      for (int64_t t0 = r0; t0 < r0 + kRun && t0 < g.tokens; t0 += kDeep) {
-        __syncthreads();
-        for (int w = threadIdx.x; w < kTile * kDeep; w += 256) {
-          const int64_t t = t0 + w / kTile, c = c0 + w % kTile, k = k0 + w % kTile;
-          a[w / kTile][w % kTile] =
-              t < g.tokens && c < g.channels ? value_of<T>(bits_of((const T*)g.grad + t * g.gs + c)) : 0.0f;
-          b[w / kTile][w % kTile] = t < g.tokens && k < g.depth ? (float)g.q[t * g.qs + k] : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int t = 0; t < kDeep; t++)
+// 16 columns (channels from c0 on) of 32 k, a k in each lane.
+__device__ __forceinline__ void write_block(const GradArgs& g, const float* v, int64_t c0, int64_t k) {
+  if (g.out_dtype == DCF_F32) {
+    if (k >= g.depth) return;
+    float* out = (float*)g.out + c0 * g.os + k;
 #pragma unroll
-          for (int m = 0; m < 4; m++)
+    for (int j = 0; j < 16; j++, out += g.os)
+      if (c0 + j >= 0 && c0 + j < g.channels) *out = g.add ? __fadd_rn(*out, v[j]) : v[j];
+  } else if (g.pairs) {
+    // Lanes trade: an even one writes its channel for two k, an odd one the next channel.
+    const int odd = threadIdx.x & 1;
+    uint16_t* out = (uint16_t*)g.out + (c0 + odd) * g.os + (k & ~1ll);
+    const bool both = (k | 1) < g.depth, one = (k & ~1ll) < g.depth, half = g.out_dtype == DCF_F16;
 #pragma unroll
-            for (int n = 0; n < 4; n++) part[m][n] = __fmaf_rn(a[t][y + 16 * m], b[t][x + 16 * n], part[m][n]);
+    for (int j = 0; j < 16; j += 2, out += 2 * g.os) {
+      const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
+      const float lo = odd ? got : v[j], hi = odd ? v[j + 1] : got;
+      uint32_t w;
+      if (half) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        w = *(const uint32_t*)&h;
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        w = *(const uint32_t*)&h;
       }
-      for (int n = 0; n < 4; n++) {
-        const int64_t k = k0 + x + 16 * n;
-        const float s = k < g.depth ? g.scale[r0 / kRun * g.depth + k] : 0.0f;
-        for (int m = 0; m < 4; m++) sum[m][n] = __fmaf_rn(s, part[m][n], sum[m][n]);
+      const int64_t c = c0 + j + odd;
+      if (c >= 0 && c < g.channels) {
+        if (both) *(uint32_t*)out = w;
+        else if (one) *out = (uint16_t)w;
       }
     }
-    for (int m = 0; m < 4; m++)
-      for (int n = 0; n < 4; n++)
-        if (c0 + y + 16 * m < g.channels && k0 + x + 16 * n < g.depth) put(g, c0 + y + 16 * m, k0 + x + 16 * n, sum[m][n]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (c0 + j >= 0 && c0 + j < g.channels && k < g.depth) put(g, c0 + j, k, v[j]);
   }
+}
+
+// Sums of a part: [column of the tile][k of the tile].
+template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, int64_t item) {
+  return g.part + item * (kTileM * TN);
+}
+
+// D = q^T grad of each run in tiles of 256 k x TN channels by persistent pairs
+// of CTAs, each with 128 k and half of the channels.  Warp 0 loads the gradient; four
+// warps read whole numbers, a run ahead, and write them as operands of the
+// gradient's type; one thread of the first CTA issues the eight products of a
+// run for both; eight warps take a run's sums out of one of two buffers of TMEM while
+// the other is filled.  k lies in the lanes: a lane needs one scale a run, and
+// a warp writes neighbours of a row.  READ: rows of whole numbers lie off
+// 16-byte boundaries; they are read as the 16-byte vectors that hold them, and
+// neighbours in a warp make up what they lack from each other.
+template <class T, int TN, bool READ>
+__global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constant__ CUtensorMap map_g, const GradArgs args) {
+  const GradArgs g = args;  // a reference to the parameter itself would be read through memory
+  constexpr int S = kStages<TN>, kMine = TN / 2;  // columns of one out warp
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
+  uint64_t* full = (uint64_t*)(base + S * kStage<TN>);  // the first CTA's counts what both have
+  uint64_t* empty = full + S;
+  uint64_t* sum_full = empty + S;
+  uint64_t* sum_empty = sum_full + 2;  // the first CTA's
+  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  const uint32_t stage0 = smem_addr(base);
+  uint32_t full0;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(full0) : "r"(smem_addr(full)));
+  auto begin_of = [&](int64_t t) { return (int)(t % g.splits) * g.split_runs; };
+  auto count_of = [&](int64_t t) { return min(g.split_runs, g.runs - begin_of(t)); };
+
+  if (warp == 0 && lane == 0) {
+    for (int s = 0; s < S; s++) {
+      mbar_init(&full[s], 1 + 2 * kReaders);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&sum_full[b], 1);
+      mbar_init(&sum_empty[b], 2 * kOutWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_at)), "r"(2 * TN)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  pair_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *(volatile uint32_t*)tmem_at;
+  if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_g) : "memory");
+  pdl_begin();
+
+  bool fail = false;
+  if (warp < 4) control_registers();
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring<S> at;
+      int used = 0;  // stages filled, S at most
+      for (int64_t t = first; t < g.total && !fail; t += step) {
+        const int col = (int)(t / g.splits / g.tiles_m) * TN + (int)rank * (TN / 2);
+        const int r0 = begin_of(t), count = count_of(t);
+        for (int r = 0; r < count; r++, at.next()) {
+          if (!mbar_wait_bounded(&empty[at.s], at.turn ^ 1)) {
+            fail = true;
+            break;
+          }
+          const uint32_t to = stage0 + at.s * kStage<TN> + kSide * kRun * 2, bar = full0 + at.s * 8;
+          if (!rank) mbar_expect_tx(&full[at.s], TN * kRun * 2);
+          pair_load_2d(to, &map_g, col, (r0 + r) * kRun, bar);
+          if (TN == 256) pair_load_2d(to + kBlockBytes, &map_g, col + 64, (r0 + r) * kRun, bar);
+          used += used < S;
+        }
+      }
+      // Leave only with no copy of ours and no arrival for us left in flight.
+      for (; used > 0; used--) {
+        const Ring<S> last = at.back(used);
+        if (!rank && !mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
+        if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && !rank) {
+      const uint64_t desc = block_desc(stage0);
+      Ring<S> at;
+      Ring<2> sum;
+      for (int64_t t = first; t < g.total && !fail; t += step) {
+        const int count = count_of(t);
+        for (int r = 0; r < count; r++, at.next(), sum.next()) {
+          if (!mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1) || !mbar_wait_bounded(&full[at.s], at.turn)) {
+            fail = true;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t pq = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pg = pq + (kSide * kRun * 2 >> 4);
+#pragma unroll
+          for (int j = 0; j < kRun / 16; j++)
+            pair_mma(tmem + sum.s * TN, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
+          pair_commit(&empty[at.s]);
+          pair_commit(&sum_full[sum.s]);
+        }
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    reader_registers();
+    // Eight neighbours store four vectors of two rows, which the swizzle puts into different banks.
+    const int chunk = (lane >> 3 & 1) * 4 + (lane & 3);
+    const int row = (warp - 4) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
+    const int beside = (lane & 3) < 3 ? lane + 1 : (lane + 5) & 31;  // who has the next vector of the row
+    constexpr int kRows = 8, kHalf = READ ? 4 : 8;  // loads of a run, and at a time
+    auto from = [&](int64_t t, int r, int j) {
+      const int64_t token = (int64_t)r * kRun + row + j * 16;
+      const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16;
+      return token < g.tokens ? g.q + token * g.qs + k : nullptr;
+    };
+    auto read = [&](const int8_t* p, int64_t t, uint4& own, uint4& next) {
+      const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16;
+      const int off = READ ? (int)((uintptr_t)p & 15) : 0;
+      own = make_uint4(0, 0, 0, 0);
+      if (p && k - off < g.depth) own = *(const uint4*)(p - off);  // what lies behind the row is not written out
+      if (READ) {
+        next = make_uint4(0, 0, 0, 0);
+        if (p && off && chunk == 7 && k + 16 - off < g.depth) next = *(const uint4*)(p - off + 16);
+      }
+    };
+    uint4 own[kRows], next[READ ? kRows : 1];
+    Ring<S> at;
+    if (first < g.total) {
+#pragma unroll
+      for (int j = 0; j < kHalf; j++) read(from(first, begin_of(first), j), first, own[j], next[READ ? j : 0]);
+    }
+    for (int64_t t = first; t < g.total && !fail; t += step) {
+      const int r0 = begin_of(t), count = count_of(t);
+      for (int r = 0; r < count; r++, at.next()) {
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+          fail = true;
+          break;
+        }
+        uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes;
+        const bool more = r + 1 < count;
+        const int64_t then = more ? t : t + step;
+        const int then_r = more ? r0 + r + 1 : then < g.total ? begin_of(then) : 0;
+#pragma unroll
+        for (int half = 0; half < kRows; half += kHalf) {
+#pragma unroll
+          for (int i = 0; i < kHalf; i++) {
+            const int j = half + i, line = row + j * 16;
+            uint4 v = own[i];
+            if (READ) {
+              const int8_t* p = from(t, r0 + r, j);
+              uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, v.x, beside), __shfl_sync(0xFFFFFFFFu, v.y, beside),
+                                        __shfl_sync(0xFFFFFFFFu, v.z, beside), __shfl_sync(0xFFFFFFFFu, v.w, beside));
+              if (chunk == 7) beyond = next[READ ? i : 0];
+              v = bytes_from(v, beyond, p ? (int)((uintptr_t)p & 15) : 0);
+            }
+            // the next of this register: the second half of this run, or the next run
+            if (half + kHalf < kRows) read(from(t, r0 + r, j + kHalf), t, own[i], next[READ ? i : 0]);
+            else if (then < g.total) read(from(then, then_r, i), then, own[i], next[READ ? i : 0]);
+            const int c = (chunk & 3) * 2;
+            *(uint4*)(to + line * 128 + ((c ^ (line & 7)) << 4)) = to_eight<T>(v.x, v.y);
+            *(uint4*)(to + line * 128 + (((c + 1) ^ (line & 7)) << 4)) = to_eight<T>(v.z, v.w);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive_first(&full[at.s]);
+      }
+    }
+  } else if (warp >= 8) {
+    adder_registers();
+    const int part = warp & 3;               // the 32 TMEM lanes this warp may read
+    const int col = (warp - 8) / 4 * kMine;  // and the half of the columns it takes
+    const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
+    Ring<2> sum;
+    for (int64_t t = first; t < g.total && !fail; t += step) {
+      const int64_t tile = t / g.splits;
+      const int row = (int)rank * kSide + part * 32 + lane;  // of the tile
+      const int64_t k = tile % g.tiles_m * kTileM + row, c0 = tile / g.tiles_m * TN + col - g.skip;
+      const int r0 = begin_of(t), count = count_of(t);
+      const float* scale = g.scale + (int64_t)r0 * g.depth + k;
+      float acc[kMine], s = k < g.depth ? *scale : 0.0f;
+#pragma unroll
+      for (int j = 0; j < kMine; j++) acc[j] = 0;
+      for (int r = 0; r < count; r++, sum.next()) {
+        scale += g.depth;
+        const float then = k < g.depth && r + 1 < count ? *scale : 0.0f;
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[sum.s], sum.turn))) {
+          fail = true;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t x[2][16];  // one part is added while the next arrives
+        tmem_load16(lanes + sum.s * TN, x[0]);
+#pragma unroll
+        for (int c = 0; c < kMine; c += 16) {
+          tmem_wait(x[c / 16 & 1]);
+          if (c + 16 < kMine) {
+            tmem_load16(lanes + sum.s * TN + c + 16, x[(c / 16 + 1) & 1]);
+          } else {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (lane == 0) arrive_first(&sum_empty[sum.s]);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) acc[c + j] = __fmaf_rn(s, __uint_as_float(x[c / 16 & 1][j]), acc[c + j]);
+        }
+        s = then;
+      }
+      if (fail) break;
+#pragma unroll 1
+      for (int c = 0; c < kMine; c += 16) {
+        if (c0 + c < g.channels) {
+          if (g.splits > 1) {
+            float* p = part_of<TN>(g, t) + (int64_t)(col + c) * kTileM + row;
+#pragma unroll
+            for (int j = 0; j < 16; j++) p[j * kTileM] = acc[j];
+          } else {
+            write_block(g, acc, c0 + c, k);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kMine - 16; j++) acc[j] = acc[j + 16];
+      }
+    }
+  }
+  if (fail) atomicExch(&g.st->error, 1u);
+  __syncthreads();
+  pair_sync();
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TN) : "memory");
+  }
+}
+
+// Joins the parts of each sum, always in the same order; a thread takes a k
+// and channel.  Also what writes the gradient of no tokens, whose sums have no parts.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_constant__ GradArgs g, int tile_n) {
+  pdl_begin();
+  const int64_t across = ((int64_t)g.depth + kJoinThreads - 1) / kJoinThreads, all = across * g.channels;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const int64_t c = i / across, k = i % across * kJoinThreads + threadIdx.x, col = c + g.skip;
+    if (k >= g.depth) continue;
+    float sum = 0;
+    if (g.splits) {
+      const int64_t tile = col / tile_n * g.tiles_m + k / kTileM, size = (int64_t)kTileM * tile_n;
+      const float* p = g.part + tile * g.splits * size + col % tile_n * kTileM + k % kTileM;
+      for (int s = 0; s < g.splits; s++) sum = __fadd_rn(sum, p[s * size]);
+    }
+    put(g, c, k, sum);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+// The gradient as boxes of 64 channels x 128 tokens.
+bool encode_grad(CUtensorMap* map, const void* p, bool bf16, int64_t channels, int64_t tokens, int64_t stride) {
+  const cuuint64_t dims[2] = {(cuuint64_t)channels, (cuuint64_t)tokens};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  const cuuint32_t boxes[2] = {64, kRun};
+  const cuuint32_t estr[2] = {1, 1};
+  return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)p, dims,
+                   strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t stride_of(int64_t given, uint64_t cols) { return given ? given : (int64_t)cols; }
+
+// How a gradient is laid out: channels of a tile, and the parts into which its
+// runs are cut.
+struct Cut {
+  int tile_n;
+  int64_t tiles_m, tiles;
+  int splits, runs;        // runs of a part
+};
+
+Cut cut_of(const dcf_checkpoint_desc& d, int skip) {
+  const int runs = (int)((d.tokens + kRun - 1) / kRun);
+  Cut best = {};
+  double least = 1e300;
+  for (int tn : {128, 256}) {
+    const int64_t tm = ((int64_t)d.depth + kTileM - 1) / kTileM;
+    const int64_t tiles = tm * (((int64_t)d.channels + skip + tn - 1) / tn);
+    const double run = tn == 256 ? 1 : 0.65;
+    for (int s = 1; s == 1 || (s <= runs && tiles * s <= kPairs); s++) {
+      const int each = (runs + s - 1) / s, parts = each ? (runs + each - 1) / each : 1;
+      const double rounds = (double)((tiles * parts + kPairs - 1) / kPairs);
+      const double cost = rounds * (each + 3) * run + (parts > 1 ? 6 : 0);
+      if (cost < least) {
+        least = cost;
+        best = {tn, tm, tiles, parts, each};
+      }
+    }
+  }
+  return best;
+}
+
+// The workspace: a copy of a gradient whose stride no tensor map takes, and the parts of sums.
+struct Layout {
+  Cut cut;
+  bool copy;
+  int64_t stride;          // of the copy, in elements
+  size_t grad, part, bytes;
+};
+
+Layout layout_of(const dcf_checkpoint_desc& d, int skip) {
+  Layout l = {};
+  auto take = [&](size_t bytes) {
+    const size_t at = l.bytes;
+    l.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  l.cut = cut_of(d, skip);
+  const int64_t gs = stride_of(d.grad_row_stride, d.channels);
+  l.copy = d.tokens > 1 && (gs % 8 || gs < (int64_t)d.channels || gs >= 1ll << 38);
+  l.stride = (int64_t)((d.channels + 7) / 8 * 8);
+  l.grad = take(l.copy ? (size_t)d.tokens * l.stride * 2 : 0);
+  l.part = take(l.cut.splits > 1 ? (size_t)l.cut.tiles * l.cut.splits * kTileM * l.cut.tile_n * 4 : 0);
+  return l;
+}
+
+template <class T, int TN, bool READ> int run(const CUtensorMap& map, const GradArgs& g, cudaStream_t s) {
+  if (!prepare_smem((const void*)grad_kernel<T, TN, READ>, kSmem<TN>)) return DCF_ECUDA;
+  const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
+  return launch(grad_kernel<T, TN, READ>, dim3(2 * pairs), kThreads_, kSmem<TN>, 2, s, map, g);
+}
+
+template <class T> int run_typed(int tile_n, bool read, const CUtensorMap& map, const GradArgs& g, cudaStream_t s) {
+  if (tile_n == 256) return read ? run<T, 256, true>(map, g, s) : run<T, 256, false>(map, g, s);
+  return read ? run<T, 128, true>(map, g, s) : run<T, 128, false>(map, g, s);
 }
 
 }  // namespace
@@ -97,16 +495,15 @@ int checkpoint_desc_check(const dcf_checkpoint_desc* d) {
 }
 
 size_t checkpoint_workspace(const dcf_checkpoint_desc& d) {
-  (void)d;
-  return 0;
+  if (!d.tokens || !d.channels || !d.depth) return 0;
+  // The gradient may start 0 to 7 elements into a vector: as many tiles as with none, or as with seven.
+  const Layout none = layout_of(d, 0), most = layout_of(d, 7);
+  return none.copy || none.bytes > most.bytes ? none.bytes : most.bytes;
 }
 
 int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const int8_t* q, const float* scale,
                            void* out, void* ws, dcf_status* st, cudaStream_t s) {
-  (void)ws;
-  (void)st;
-  GradArgs g;
-  g.grad = grad;
+  GradArgs g = {};
   g.q = q;
   g.scale = scale;
   g.out = out;
@@ -115,13 +512,45 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
   g.tokens = (int)d.tokens;
   g.channels = (int)d.channels;
   g.depth = (int)d.depth;
-  g.gs = d.grad_row_stride ? d.grad_row_stride : (int64_t)d.channels;
-  g.qs = d.q_row_stride ? d.q_row_stride : (int64_t)d.depth;
-  g.os = d.out_row_stride ? d.out_row_stride : (int64_t)d.depth;
-  const int64_t total = (int64_t)((d.channels + kTile - 1) / kTile) * (int64_t)((d.depth + kTile - 1) / kTile);
-  const dim3 grid((unsigned)(total < (1 << 30) ? total : 1 << 30));
-  return d.grad_dtype == DCF_F16 ? launch(grad_tile_kernel<__half>, grid, 256, 0, 1, s, g)
-                                 : launch(grad_tile_kernel<__nv_bfloat16>, grid, 256, 0, 1, s, g);
+  g.qs = stride_of(d.q_row_stride, d.depth);
+  g.os = stride_of(d.out_row_stride, d.depth);
+  g.pairs = (uintptr_t)out % 4 == 0 && (d.channels == 1 || g.os % 2 == 0);
+  g.st = st;
+  int tile_n = 0;
+  if (d.tokens) {
+    Layout l = layout_of(d, 0);
+    int64_t gs = d.tokens > 1 ? stride_of(d.grad_row_stride, d.channels) : l.stride + 8;
+    int rc;
+    if (l.copy) {
+      uint8_t* to = (uint8_t*)ws + l.grad;
+      if ((rc = launch_pack_rows(grad, gs * 2, (int64_t)d.tokens, (int64_t)d.channels * 2, to, l.stride * 2, s))) return rc;
+      grad = to;
+      gs = l.stride;
+    }
+    // A map starts on a 16-byte boundary; the columns before the first channel are left out again.
+    g.skip = (int)((uintptr_t)grad % 16 / 2);
+    if (g.skip) l = layout_of(d, g.skip);
+    const bool bf16 = d.grad_dtype == DCF_BF16;
+    if (!encoder()) return DCF_EUNSUPPORTED;
+    CUtensorMap map;
+    tile_n = l.cut.tile_n;
+    const int64_t wide = (int64_t)d.channels + g.skip;
+    if (!encode_grad(&map, (const uint8_t*)grad - g.skip * 2, bf16, wide, (int64_t)d.tokens, gs)) return DCF_ECUDA;
+    g.runs = (int)((d.tokens + kRun - 1) / kRun);
+    g.tiles_m = (int)l.cut.tiles_m;
+    g.splits = l.cut.splits;
+    g.split_runs = l.cut.runs;
+    g.total = l.cut.tiles * l.cut.splits;
+    g.part = (float*)((uint8_t*)ws + l.part);
+    g.idesc = (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | ((uint32_t)(tile_n >> 3) << 17) |
+              ((uint32_t)(kTileM >> 4) << 24);
+    const bool read = (uintptr_t)q % 16 || (d.tokens > 1 && g.qs % 16);
+    rc = bf16 ? run_typed<__nv_bfloat16>(tile_n, read, map, g, s) : run_typed<__half>(tile_n, read, map, g, s);
+    if (rc || g.splits == 1) return rc;
+  }
+  const int64_t joins = ((int64_t)d.depth + kJoinThreads - 1) / kJoinThreads * (int64_t)d.channels;
+  return launch(grad_join_kernel, dim3((unsigned)(joins < (1 << 30) ? joins : 1 << 30)), kJoinThreads, 0, 1, s, g,
+                tile_n ? tile_n : 1);
 }
 
 }  // namespace dcf

@@ -188,23 +188,15 @@ __device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, i
   const uint4 beside = make_uint4(__shfl_down_sync(0xFFFFFFFFu, own.x, 1), __shfl_down_sync(0xFFFFFFFFu, own.y, 1),
                                   __shfl_down_sync(0xFFFFFFFFu, own.z, 1), __shfl_down_sync(0xFFFFFFFFu, own.w, 1));
   if ((lane & (L - 1)) != L - 1) next = beside;
-  const int off = (int)((uintptr_t)(row + k) & 15), have = depth - k;
-  uint32_t w[8] = {own.x, own.y, own.z, own.w, next.x, next.y, next.z, next.w};
-  if (off & 8) {
-#pragma unroll
-    for (int j = 0; j < 6; j++) w[j] = w[j + 2];
-  }
-  if (off & 4) {
-#pragma unroll
-    for (int j = 0; j < 5; j++) w[j] = w[j + 1];
-  }
+  uint4 v = bytes_from(own, next, (int)((uintptr_t)(row + k) & 15));
+  uint32_t* w = (uint32_t*)&v;
+  const int have = depth - k;
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
     const int here = have - 4 * j;  // bytes of this word in the row
     if (here < 4) w[j] = here > 0 ? w[j] & (0xFFFFFFFFu >> (32 - 8 * here)) : 0u;
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return v;
 }
 
 // D = B A^T in tiles of 256 channels x TN tokens by persistent pairs of CTAs:
@@ -455,35 +447,6 @@ __global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_co
   }
 }
 
-// Rows that no tensor map describes (a row that starts off a 16-byte boundary),
-// copied to rows of whole vectors; a thread writes 16 bytes.
-constexpr int kPackThreads = 256;
-__global__ void __launch_bounds__(kPackThreads) pack_kernel(const int8_t* from, int64_t stride, int64_t rows, int cols,
-                                                            int8_t* to, int64_t to_stride) {
-  pdl_begin();
-  const int64_t groups = (cols + 15) / 16, all = groups * rows;
-  for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kPackThreads) {
-    const int64_t r = i / groups;
-    const int c = (int)(i % groups) * 16, have = cols - c;
-    const int8_t* p = from + r * stride + c;
-    const int off = (int)((uintptr_t)p & 3);
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (have >= 20 && c >= 4) {  // the words around these bytes lie in the row
-      const uint32_t* a = (const uint32_t*)(p - off);
-      uint32_t v[5];
-#pragma unroll
-      for (int j = 0; j < 5; j++) v[j] = a[j];
-#pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (e < have) w[e >> 2] |= (uint32_t)(uint8_t)p[e] << ((e & 3) * 8);
-    }
-    *(uint4*)(to + r * to_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
 // -------------------------------------------------------- few tokens
 
 // Up to four tokens are bound by the weight's bytes.  A group of warps takes
@@ -518,20 +481,9 @@ struct FewArgs {
 
 // Sixteen bytes from byte `off` of a lane's vector and the next lane's on.
 __device__ __forceinline__ uint4 shifted_down(const uint4& own, int off) {
-  uint32_t w[8] = {own.x, own.y, own.z, own.w};
-#pragma unroll
-  for (int j = 0; j < 4; j++) w[4 + j] = __shfl_down_sync(0xFFFFFFFFu, w[j], 1);
-  if (off & 8) {
-#pragma unroll
-    for (int j = 0; j < 6; j++) w[j] = w[j + 2];
-  }
-  if (off & 4) {
-#pragma unroll
-    for (int j = 0; j < 5; j++) w[j] = w[j + 1];
-  }
-#pragma unroll
-  for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  const uint4 beside = make_uint4(__shfl_down_sync(0xFFFFFFFFu, own.x, 1), __shfl_down_sync(0xFFFFFFFFu, own.y, 1),
+                                  __shfl_down_sync(0xFFFFFFFFu, own.z, 1), __shfl_down_sync(0xFFFFFFFFu, own.w, 1));
+  return bytes_from(own, beside, off);
 }
 
 // Tokens as whole numbers in shared memory, zeros behind them; warps share a token.
@@ -830,9 +782,7 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
   uint8_t* work = (uint8_t*)ws;
   int64_t as = stride_of(d.a_row_stride, d.depth), bs = stride_of(d.b_row_stride, d.depth);
   auto pack = [&](const int8_t** p, int64_t* stride, uint64_t rows, size_t at) {
-    const int64_t all = (l.stride / 16) * (int64_t)rows, blocks = (all + kPackThreads - 1) / kPackThreads;
-    const int rc = launch(pack_kernel, dim3((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30)), kPackThreads, 0, 1, s, *p,
-                          *stride, (int64_t)rows, (int)d.depth, (int8_t*)work + at, l.stride);
+    const int rc = launch_pack_rows(*p, *stride, (int64_t)rows, (int64_t)d.depth, work + at, l.stride, s);
     *p = (int8_t*)work + at;
     *stride = l.stride;
     return rc;

@@ -247,6 +247,32 @@ __global__ void __launch_bounds__(kQuantThreads) dequant_kernel(const QuantArgs 
   }
 }
 
+// A thread writes 16 bytes of a row.
+__global__ void __launch_bounds__(kQuantThreads) pack_kernel(const uint8_t* from, int64_t stride, int64_t rows,
+                                                             int64_t bytes, uint8_t* to, int64_t to_stride) {
+  pdl_begin();
+  const int64_t groups = (bytes + 15) / 16, all = groups * rows;
+  for (int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kQuantThreads) {
+    const int64_t r = i / groups, c = i % groups * 16, have = bytes - c;
+    const uint8_t* p = from + r * stride + c;
+    const int off = (int)((uintptr_t)p & 3);
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (have >= 20 && c >= 4) {  // the words around these bytes lie in the row
+      const uint32_t* a = (const uint32_t*)(p - off);
+      uint32_t v[5];
+#pragma unroll
+      for (int j = 0; j < 5; j++) v[j] = a[j];
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (e < have) w[e >> 2] |= (uint32_t)p[e] << ((e & 3) * 8);
+    }
+    *(uint4*)(to + r * to_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 unsigned blocks_of(int64_t n) { return (unsigned)(n < (1 << 30) ? n : 1 << 30); }
 
 QuantArgs quant_args(const dcf_quant_desc& d, const void* in, int8_t* q, float* scale) {
@@ -309,6 +335,13 @@ template <class F> int by_type(uint32_t dtype, const QuantArgs& a, const void* v
 }
 
 }  // namespace
+
+int launch_pack_rows(const void* from, int64_t stride, int64_t rows, int64_t bytes, void* to, int64_t to_stride,
+                     cudaStream_t s) {
+  const int64_t all = (bytes + 15) / 16 * rows;
+  return launch(pack_kernel, blocks_of((all + kQuantThreads - 1) / kQuantThreads), kQuantThreads, 0, 1, s,
+                (const uint8_t*)from, stride, rows, bytes, (uint8_t*)to, to_stride);
+}
 
 int quant_desc_check(const dcf_quant_desc* d, bool back) {
   auto bad = [](const char* m) { return record_error(DCF_EINVAL, m); };

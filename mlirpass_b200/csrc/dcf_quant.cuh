@@ -136,6 +136,27 @@ template <int E> __device__ __forceinline__ void store_levels(int8_t* p, const u
   }
 }
 
+// Sixteen bytes from byte `off` of two neighbouring vectors on.
+__device__ __forceinline__ uint4 bytes_from(const uint4& own, const uint4& next, int off) {
+  uint32_t w[8] = {own.x, own.y, own.z, own.w, next.x, next.y, next.z, next.w};
+  if (off & 8) {
+#pragma unroll
+    for (int j = 0; j < 6; j++) w[j] = w[j + 2];
+  }
+  if (off & 4) {
+#pragma unroll
+    for (int j = 0; j < 5; j++) w[j] = w[j + 1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 3) * 8);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Copies rows that no tensor map describes (they start off 16-byte boundaries)
+// to rows of whole vectors; sizes and strides in bytes.
+int launch_pack_rows(const void* from, int64_t stride, int64_t rows, int64_t bytes, void* to, int64_t to_stride,
+                     cudaStream_t s);
+
 // The signed byte j of a word as a float: a byte (its sign turned) under the
 // exponent of 2^23 is 2^23 + 128 + q.
 __device__ __forceinline__ float byte_value(uint32_t turned, int j) {

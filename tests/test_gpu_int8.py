@@ -337,7 +337,8 @@ def test_grad_of_whole_numbers_is_exact(dcf, tokens, channels, depth, dtype, out
 
 @pytest.mark.parametrize("pads,offsets", [((8, 16, 4), (0, 0, 0)), ((3, 0, 0), (0, 0, 0)), ((0, 3, 0), (0, 0, 0)),
                                           ((0, 0, 1), (0, 0, 0)), ((8, 16, 4), (1, 0, 0)), ((8, 16, 4), (0, 5, 0)),
-                                          ((8, 16, 4), (0, 0, 1)), ((8, 16, 4), (8, 16, 4)), ((1, 1, 1), (1, 1, 1))])
+                                          ((8, 16, 4), (0, 0, 1)), ((8, 16, 4), (8, 16, 4)), ((1, 1, 1), (1, 1, 1)),
+                                          ((0, 0, 0), (3, 0, 0)), ((0, 0, 0), (7, 9, 3))])
 @pytest.mark.parametrize("out", ["f32", "bf16"])
 def test_grad_strides_and_what_lies_between(dcf, pads, offsets, out):
     g, q, scale = exact_inputs(300, 136, 160, "bf16", 4)
