@@ -245,59 +245,68 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     const int row = (warp - 4) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
     const int beside = (lane & 3) < 3 ? lane + 1 : (lane + 5) & 31;  // who has the next vector of the row
     constexpr int kRows = 8, kHalf = READ ? 4 : 8;  // loads of a run, and at a time
-    auto from = [&](int64_t t, int r, int j) {
-      const int64_t token = (int64_t)r * kRun + row + j * 16;
-      const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16;
-      return token < g.tokens ? g.q + token * g.qs + k : nullptr;
+    // The vectors of a run: k of this thread's, and the place of its first row.
+    struct Run {
+      int k, rows;  // rows: of this thread's first one, how many are left of it
+      const int8_t* p;
     };
-    auto read = [&](const int8_t* p, int64_t t, uint4& own, uint4& next) {
-      const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16;
+    auto run_of = [&](int k, int r) {
+      const int64_t token = (int64_t)r * kRun + row;
+      return Run{k, (int)min((int64_t)kRun, g.tokens - token), g.q + token * g.qs + k};
+    };
+    auto k_of = [&](int64_t t) { return (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16; };
+    auto read = [&](const Run& u, int j, uint4& own, uint4& next) {
+      const int8_t* p = u.p + j * 16 * g.qs;
       const int off = READ ? (int)((uintptr_t)p & 15) : 0;
+      const bool there = j * 16 < u.rows;
       own = make_uint4(0, 0, 0, 0);
-      if (p && k - off < g.depth) own = *(const uint4*)(p - off);  // what lies behind the row is not written out
+      if (there && u.k - off < g.depth) own = *(const uint4*)(p - off);  // what lies behind the row is not written out
       if (READ) {
         next = make_uint4(0, 0, 0, 0);
-        if (p && off && chunk == 7 && k + 16 - off < g.depth) next = *(const uint4*)(p - off + 16);
+        if (there && off && chunk == 7 && u.k + 16 - off < g.depth) next = *(const uint4*)(p - off + 16);
       }
     };
     uint4 own[kRows], next[READ ? kRows : 1];
     Ring<S> at;
+    Run now = {};
     if (first < g.total) {
+      now = run_of(k_of(first), begin_of(first));
 #pragma unroll
-      for (int j = 0; j < kHalf; j++) read(from(first, begin_of(first), j), first, own[j], next[READ ? j : 0]);
+      for (int j = 0; j < kHalf; j++) read(now, j, own[j], next[READ ? j : 0]);
     }
     for (int64_t t = first; t < g.total && !fail; t += step) {
       const int r0 = begin_of(t), count = count_of(t);
       for (int r = 0; r < count; r++, at.next()) {
+        Run then = now;
+        if (r + 1 < count) then = run_of(now.k, r0 + r + 1);
+        else if (t + step < g.total) then = run_of(k_of(t + step), begin_of(t + step));
+        else then.rows = 0;
         if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
         }
-        uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes;
-        const bool more = r + 1 < count;
-        const int64_t then = more ? t : t + step;
-        const int then_r = more ? r0 + r + 1 : then < g.total ? begin_of(then) : 0;
+        uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes + row * 128;
 #pragma unroll
         for (int half = 0; half < kRows; half += kHalf) {
 #pragma unroll
           for (int i = 0; i < kHalf; i++) {
-            const int j = half + i, line = row + j * 16;
+            const int j = half + i;
             uint4 v = own[i];
             if (READ) {
-              const int8_t* p = from(t, r0 + r, j);
               uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, v.x, beside), __shfl_sync(0xFFFFFFFFu, v.y, beside),
                                         __shfl_sync(0xFFFFFFFFu, v.z, beside), __shfl_sync(0xFFFFFFFFu, v.w, beside));
               if (chunk == 7) beyond = next[READ ? i : 0];
-              v = bytes_from(v, beyond, p ? (int)((uintptr_t)p & 15) : 0);
+              v = bytes_from(v, beyond, (int)((uintptr_t)(now.p + j * 16 * g.qs) & 15));
             }
-            // the next of this register: the second half of this run, or the next run
-            if (half + kHalf < kRows) read(from(t, r0 + r, j + kHalf), t, own[i], next[READ ? i : 0]);
-            else if (then < g.total) read(from(then, then_r, i), then, own[i], next[READ ? i : 0]);
-            const int c = (chunk & 3) * 2;
-            *(uint4*)(to + line * 128 + ((c ^ (line & 7)) << 4)) = to_eight<T>(v.x, v.y);
-            *(uint4*)(to + line * 128 + (((c + 1) ^ (line & 7)) << 4)) = to_eight<T>(v.z, v.w);
+            // the next of this register: of the second half of this run, or of the next run
+            if (half + kHalf < kRows) read(now, j + kHalf, own[i], next[READ ? i : 0]);
+            else read(then, i, own[i], next[READ ? i : 0]);
+            const int c = (chunk & 3) * 2, turn = row & 7;  // 16 rows on, the swizzle is the same
+            *(uint4*)(to + j * 2048 + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
+            *(uint4*)(to + j * 2048 + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
           }
         }
+        now = then;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
       }
