@@ -15,7 +15,7 @@ namespace {
 
 constexpr int kSide = 128;                // k of a CTA
 constexpr int kTileM = 2 * kSide;         // of a pair
-constexpr int kReaders = 128;             // threads that turn whole numbers into the gradient's type
+constexpr int kReaders = 256;             // threads that turn whole numbers into the gradient's type
 constexpr int kOutWarps = 8;
 constexpr int kThreads_ = 128 + kReaders + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
 constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
@@ -78,11 +78,11 @@ template <class T> __device__ __forceinline__ uint4 to_eight(uint32_t a, uint32_
                     to_halves<T>(__byte_perm(b, 0, 0x4140)), to_halves<T>(__byte_perm(b, 0, 0x4342)));
 }
 
-// 512 threads start with 128 registers each; warps 0 to 3 keep 32, the four
-// that read 96, and the eight that add up get 192: 128 * 32 + 128 * 96 + 256 * 192 = 512 * 128.
+// 640 threads start with 96 registers each; warps 0 to 3 keep 32, the eight
+// that read 56, and the eight that add up get 168: 128 * 32 + 256 * 56 + 256 * 168 = 640 * 96.
 __device__ __forceinline__ void control_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 32;"); }
-__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 96;"); }
-__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 192;"); }
+__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
 
 __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, float v) {
   const int64_t at = c * g.os + k;
@@ -135,7 +135,7 @@ template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, i
 }
 
 // D = q^T grad of each run in tiles of 256 k x TN channels by persistent pairs
-// of CTAs, each with 128 k and half of the channels.  Warp 0 loads the gradient; four
+// of CTAs, each with 128 k and half of the channels.  Warp 0 loads the gradient; eight
 // warps read whole numbers, a run ahead, and write them as operands of the
 // gradient's type; one thread of the first CTA issues the eight products of a
 // run for both; eight warps take a run's sums out of one of two buffers of TMEM while
@@ -238,13 +238,13 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         }
       }
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp >= 4 && warp < 4 + kReaders / 32) {
     reader_registers();
     // Eight neighbours store four vectors of two rows, which the swizzle puts into different banks.
     const int chunk = (lane >> 3 & 1) * 4 + (lane & 3);
     const int row = (warp - 4) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
     const int beside = (lane & 3) < 3 ? lane + 1 : (lane + 5) & 31;  // who has the next vector of the row
-    constexpr int kRows = 8, kHalf = READ ? 4 : 8;  // loads of a run, and at a time
+    constexpr int kStep = kReaders / 8, kRows = kRun / kStep, kHalf = READ ? kRows / 2 : kRows;  // loads of a run, and at a time
     // The vectors of a run: k of this thread's, and the place of its first row.
     struct Run {
       int k, rows;  // rows: of this thread's first one, how many are left of it
@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     };
     auto k_of = [&](int64_t t) { return (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16; };
     auto read = [&](const Run& u, int j, uint4& own, uint4& next) {
-      const int8_t* p = u.p + j * 16 * g.qs;
+      const int8_t* p = u.p + j * kStep * g.qs;
       const int off = READ ? (int)((uintptr_t)p & 15) : 0;
-      const bool there = j * 16 < u.rows;
+      const bool there = j * kStep < u.rows;
       own = make_uint4(0, 0, 0, 0);
       if (there && u.k - off < g.depth) own = *(const uint4*)(p - off);  // what lies behind the row is not written out
       if (READ) {
@@ -296,14 +296,14 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
               uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, v.x, beside), __shfl_sync(0xFFFFFFFFu, v.y, beside),
                                         __shfl_sync(0xFFFFFFFFu, v.z, beside), __shfl_sync(0xFFFFFFFFu, v.w, beside));
               if (chunk == 7) beyond = next[READ ? i : 0];
-              v = bytes_from(v, beyond, (int)((uintptr_t)(now.p + j * 16 * g.qs) & 15));
+              v = bytes_from(v, beyond, (int)((uintptr_t)(now.p + j * kStep * g.qs) & 15));
             }
             // the next of this register: of the second half of this run, or of the next run
             if (half + kHalf < kRows) read(now, j + kHalf, own[i], next[READ ? i : 0]);
             else read(then, i, own[i], next[READ ? i : 0]);
-            const int c = (chunk & 3) * 2, turn = row & 7;  // 16 rows on, the swizzle is the same
-            *(uint4*)(to + j * 2048 + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
-            *(uint4*)(to + j * 2048 + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
+            const int c = (chunk & 3) * 2, turn = row & 7;  // kStep rows on, the swizzle is the same
+            *(uint4*)(to + j * kStep * 128 + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
+            *(uint4*)(to + j * kStep * 128 + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
           }
         }
         now = then;
@@ -311,10 +311,10 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         arrive_first(&full[at.s]);
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 4 + kReaders / 32) {
     adder_registers();
     const int part = warp & 3;               // the 32 TMEM lanes this warp may read
-    const int col = (warp - 8) / 4 * kMine;  // and the half of the columns it takes
+    const int col = (warp - 4 - kReaders / 32) / 4 * kMine;  // and the half of the columns it takes
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     Ring<2> sum;
     for (int64_t t = first; t < g.total && !fail; t += step) {
@@ -334,19 +334,19 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t x[2][16];  // one part is added while the next arrives
-        tmem_load16(lanes + sum.s * TN, x[0]);
+        uint32_t x[2][8];  // one part is added while the next arrives
+        tmem_load8(lanes + sum.s * TN, x[0]);
 #pragma unroll
-        for (int c = 0; c < kMine; c += 16) {
-          tmem_wait(x[c / 16 & 1]);
-          if (c + 16 < kMine) {
-            tmem_load16(lanes + sum.s * TN + c + 16, x[(c / 16 + 1) & 1]);
+        for (int c = 0; c < kMine; c += 8) {
+          tmem_wait(x[c / 8 & 1]);
+          if (c + 8 < kMine) {
+            tmem_load8(lanes + sum.s * TN + c + 8, x[(c / 8 + 1) & 1]);
           } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) arrive_first(&sum_empty[sum.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 16; j++) acc[c + j] = __fmaf_rn(s, __uint_as_float(x[c / 16 & 1][j]), acc[c + j]);
+          for (int j = 0; j < 8; j++) acc[c + j] = __fmaf_rn(s, __uint_as_float(x[c / 8 & 1][j]), acc[c + j]);
         }
         s = then;
       }
