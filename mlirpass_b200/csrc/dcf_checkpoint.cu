@@ -323,9 +323,10 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       const int64_t k = tile % g.tiles_m * kTileM + row, c0 = tile / g.tiles_m * TN + col - g.skip;
       const int r0 = begin_of(t), count = count_of(t);
       const float* scale = g.scale + (int64_t)r0 * g.depth + k;
-      float acc[kMine], s = k < g.depth ? *scale : 0.0f;
+      float s = k < g.depth ? *scale : 0.0f;
+      uint64_t acc[kMine / 2];  // two columns each
 #pragma unroll
-      for (int j = 0; j < kMine; j++) acc[j] = 0;
+      for (int j = 0; j < kMine / 2; j++) acc[j] = 0;
       for (int r = 0; r < count; r++, sum.next()) {
         scale += g.depth;
         const float then = k < g.depth && r + 1 < count ? *scale : 0.0f;
@@ -346,7 +347,8 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
             if (lane == 0) arrive_first(&sum_empty[sum.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 8; j++) acc[c + j] = __fmaf_rn(s, __uint_as_float(x[c / 8 & 1][j]), acc[c + j]);
+          for (int j = 0; j < 8; j += 2)
+            acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(x[c / 8 & 1][j]), __uint_as_float(x[c / 8 & 1][j + 1])), acc[(c + j) / 2]);
         }
         s = then;
       }
@@ -354,16 +356,22 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
 #pragma unroll 1
       for (int c = 0; c < kMine; c += 16) {
         if (c0 + c < g.channels) {
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 f = apart(acc[j / 2]);
+            v[j] = f.x, v[j + 1] = f.y;
+          }
           if (g.splits > 1) {
             float* p = part_of<TN>(g, t) + (int64_t)(col + c) * kTileM + row;
 #pragma unroll
-            for (int j = 0; j < 16; j++) p[j * kTileM] = acc[j];
+            for (int j = 0; j < 16; j++) p[j * kTileM] = v[j];
           } else {
-            write_block(g, acc, c0 + c, k);
+            write_block(g, v, c0 + c, k);
           }
         }
 #pragma unroll
-        for (int j = 0; j < kMine - 16; j++) acc[j] = acc[j + 16];
+        for (int j = 0; j < kMine / 2 - 8; j++) acc[j] = acc[j + 8];
       }
     }
   }

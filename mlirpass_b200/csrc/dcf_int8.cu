@@ -88,24 +88,6 @@ template <int TN> __device__ __forceinline__ int* part_of(const GemmArgs& g, int
   return g.part + item * (kTileM * TN);
 }
 
-// Two f32 products by one instruction, each rounded as by itself.  (A packed sum
-// after it would be fused with it, whatever rounding is written.)
-__device__ __forceinline__ uint64_t two(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float2 apart(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-
 // kBlock columns (tokens from t0 on) of 32 channels, a channel in each lane, on their way out.
 // A tile is as good as written once, so what counts is how few instructions and
 // how short a code do it (32 columns at a time by 8 warps and a predicate for
