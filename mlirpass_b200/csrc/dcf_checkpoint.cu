@@ -25,7 +25,9 @@ constexpr int kPairs = 74;                // of SMs on a B200; any number runs t
 constexpr int kBlockBytes = kRun * 128;
 template <int TN> constexpr int kStage = (kSide + TN / 2) * kRun * 2;
 template <int TN> constexpr int kStages = TN == 256 ? 3 : 4;
-template <int TN> constexpr int kSmem = kStages<TN> * kStage<TN> + 256 + 1024;
+// Whole numbers on their way to their operand: two runs of 128 k.
+constexpr int kRaw = kSide * kRun, kRaws = 2;
+template <int TN> constexpr int kSmem = kStages<TN> * kStage<TN> + kRaws * kRaw + 256 + 1024;
 
 struct GradArgs {
   const int8_t* q;
@@ -50,6 +52,17 @@ __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* ma
       "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 // An operand whose memory runs along it: blocks of 64 lie kBlockBytes apart,
@@ -144,16 +157,20 @@ template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, i
 // 16-byte boundaries; they are read as the 16-byte vectors that hold them, and
 // neighbours in a warp make up what they lack from each other.
 template <class T, int TN, bool READ>
-__global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constant__ CUtensorMap map_g, const GradArgs args) {
+__global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_q,
+                                                            const GradArgs args) {
   const GradArgs g = args;  // a reference to the parameter itself would be read through memory
   constexpr int S = kStages<TN>, kMine = TN / 2;  // columns of one out warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
-  uint64_t* full = (uint64_t*)(base + S * kStage<TN>);  // the first CTA's counts what both have
+  uint8_t* raw = base + S * kStage<TN>;
+  uint64_t* full = (uint64_t*)(raw + kRaws * kRaw);  // the first CTA's counts what both have
   uint64_t* empty = full + S;
   uint64_t* sum_full = empty + S;
   uint64_t* sum_empty = sum_full + 2;  // the first CTA's
-  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
+  uint64_t* raw_full = sum_empty + 2;
+  uint64_t* raw_empty = raw_full + kRaws;
+  uint32_t* tmem_at = (uint32_t*)(raw_empty + kRaws);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -172,6 +189,10 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       mbar_init(&sum_full[b], 1);
       mbar_init(&sum_empty[b], 2 * kOutWarps);
     }
+    for (int b = 0; b < kRaws; b++) {
+      mbar_init(&raw_full[b], 1);
+      mbar_init(&raw_empty[b], kReaders / 32);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -185,7 +206,10 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
   pair_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t*)tmem_at;
-  if (threadIdx.x == 0) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_g) : "memory");
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_g) : "memory");
+    if (!READ) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_q) : "memory");
+  }
   pdl_begin();
 
   bool fail = false;
@@ -216,6 +240,27 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
       }
     }
+  } else if (warp == 2) {
+    if (!READ && lane == 0) {
+      Ring<kRaws> at;
+      int used = 0;
+      for (int64_t t = first; t < g.total && !fail; t += step) {
+        const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide, r0 = begin_of(t), count = count_of(t);
+        for (int r = 0; r < count; r++, at.next()) {
+          if (!mbar_wait_bounded(&raw_empty[at.s], at.turn ^ 1)) {
+            fail = true;
+            break;
+          }
+          mbar_expect_tx(&raw_full[at.s], kRaw);
+          load_2d(smem_addr(raw + at.s * kRaw), &map_q, k, (r0 + r) * kRun, &raw_full[at.s]);
+          used += used < kRaws;
+        }
+      }
+      for (; used > 0; used--) {
+        const Ring<kRaws> last = at.back(used);
+        if (!mbar_wait_bounded(&raw_full[last.s], last.turn)) fail = true;
+      }
+    }
   } else if (warp == 1) {
     if (lane == 0 && !rank) {
       const uint64_t desc = block_desc(stage0);
@@ -240,12 +285,13 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     }
   } else if (warp >= 4 && warp < 4 + kReaders / 32) {
     reader_registers();
-    // Eight neighbours store four vectors of two rows, which the swizzle puts into different banks.
-    const int chunk = (lane >> 3 & 1) * 4 + (lane & 3);
+    // Eight neighbours store four vectors each of a row's first half and of the next
+    // row's second one, or the other way round: the swizzle puts them into different banks, and so they lie as read.
+    const int chunk = ((lane >> 3 ^ lane >> 2) & 1) * 4 + (lane & 3);
     const int row = (warp - 4) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
-    const int beside = (lane & 3) < 3 ? lane + 1 : (lane + 5) & 31;  // who has the next vector of the row
+    const int beside = (lane & 3) < 3 ? lane + 1 : (lane ^ 8) - 3;  // who has the next vector of the row
     constexpr int kStep = kReaders / 8, kRows = kRun / kStep, kHalf = READ ? kRows / 2 : kRows;  // loads of a run, and at a time
-    // The vectors of a run: k of this thread's, and the place of its first row.
+    // READ.  The vectors of a run: k of this thread's, and the place of its first row.
     struct Run {
       int k, rows;  // rows: of this thread's first one, how many are left of it
       const int8_t* p;
@@ -266,8 +312,39 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         if (there && off && chunk == 7 && u.k + 16 - off < g.depth) next = *(const uint4*)(p - off + 16);
       }
     };
-    uint4 own[kRows], next[READ ? kRows : 1];
     Ring<S> at;
+    const int c = (chunk & 3) * 2, turn = row & 7;  // kStep rows on, the swizzle is the same
+    auto store = [&](int j, const uint4& v) {
+      uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes + (row + j * kStep) * 128;
+      *(uint4*)(to + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
+      *(uint4*)(to + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
+    };
+    if constexpr (!READ) {
+      Ring<kRaws> from;
+      for (int64_t t = first; t < g.total && !fail; t += step) {
+        const int count = count_of(t);
+        for (int r = 0; r < count; r++, at.next(), from.next()) {
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&raw_full[from.s], from.turn))) {
+            fail = true;
+            break;
+          }
+          uint4 v[kRows];
+#pragma unroll
+          for (int j = 0; j < kRows; j++) v[j] = *(const uint4*)(raw + from.s * kRaw + (row + j * kStep) * kSide + chunk * 16);
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+            fail = true;
+            break;
+          }
+#pragma unroll
+          for (int j = 0; j < kRows; j++) store(j, v[j]);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&raw_empty[from.s]);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          arrive_first(&full[at.s]);
+        }
+      }
+    } else {
+    uint4 own[kRows], next[READ ? kRows : 1];
     Run now = {};
     if (first < g.total) {
       now = run_of(k_of(first), begin_of(first));
@@ -285,7 +362,6 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           fail = true;
           break;
         }
-        uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes + row * 128;
 #pragma unroll
         for (int half = 0; half < kRows; half += kHalf) {
 #pragma unroll
@@ -301,15 +377,14 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
             // the next of this register: of the second half of this run, or of the next run
             if (half + kHalf < kRows) read(now, j + kHalf, own[i], next[READ ? i : 0]);
             else read(then, i, own[i], next[READ ? i : 0]);
-            const int c = (chunk & 3) * 2, turn = row & 7;  // kStep rows on, the swizzle is the same
-            *(uint4*)(to + j * kStep * 128 + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
-            *(uint4*)(to + j * kStep * 128 + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
+            store(j, v);
           }
         }
         now = then;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
       }
+    }
     }
   } else if (warp >= 4 + kReaders / 32) {
     adder_registers();
@@ -416,6 +491,17 @@ bool encode_grad(CUtensorMap* map, const void* p, bool bf16, int64_t channels, i
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Whole numbers as boxes of 128 k x 128 tokens.
+bool encode_levels(CUtensorMap* map, const int8_t* p, int64_t depth, int64_t tokens, int64_t stride) {
+  const cuuint64_t dims[2] = {(cuuint64_t)depth, (cuuint64_t)tokens};
+  const cuuint64_t strides[1] = {(cuuint64_t)stride};
+  const cuuint32_t boxes[2] = {kSide, kRun};
+  const cuuint32_t estr[2] = {1, 1};
+  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
 int64_t stride_of(int64_t given, uint64_t cols) { return given ? given : (int64_t)cols; }
 
 // How a gradient is laid out: channels of a tile, and the parts into which its
@@ -471,15 +557,15 @@ Layout layout_of(const dcf_checkpoint_desc& d, int skip) {
   return l;
 }
 
-template <class T, int TN, bool READ> int run(const CUtensorMap& map, const GradArgs& g, cudaStream_t s) {
+template <class T, int TN, bool READ> int run(const CUtensorMap& map, const CUtensorMap& map_q, const GradArgs& g, cudaStream_t s) {
   if (!prepare_smem((const void*)grad_kernel<T, TN, READ>, kSmem<TN>)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
-  return launch(grad_kernel<T, TN, READ>, dim3(2 * pairs), kThreads_, kSmem<TN>, 2, s, map, g);
+  return launch(grad_kernel<T, TN, READ>, dim3(2 * pairs), kThreads_, kSmem<TN>, 2, s, map, map_q, g);
 }
 
-template <class T> int run_typed(int tile_n, bool read, const CUtensorMap& map, const GradArgs& g, cudaStream_t s) {
-  if (tile_n == 256) return read ? run<T, 256, true>(map, g, s) : run<T, 256, false>(map, g, s);
-  return read ? run<T, 128, true>(map, g, s) : run<T, 128, false>(map, g, s);
+template <class T> int run_typed(int tile_n, bool read, const CUtensorMap& map, const CUtensorMap& map_q, const GradArgs& g, cudaStream_t s) {
+  if (tile_n == 256) return read ? run<T, 256, true>(map, map_q, g, s) : run<T, 256, false>(map, map_q, g, s);
+  return read ? run<T, 128, true>(map, map_q, g, s) : run<T, 128, false>(map, map_q, g, s);
 }
 
 }  // namespace
@@ -561,8 +647,11 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     g.part = (float*)((uint8_t*)ws + l.part);
     g.idesc = (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | ((uint32_t)(tile_n >> 3) << 17) |
               ((uint32_t)(kTileM >> 4) << 24);
-    const bool read = (uintptr_t)q % 16 || (d.tokens > 1 && g.qs % 16);
-    rc = bf16 ? run_typed<__nv_bfloat16>(tile_n, read, map, g, s) : run_typed<__half>(tile_n, read, map, g, s);
+    const int64_t qs = d.tokens > 1 ? g.qs : ((int64_t)d.depth + 15) / 16 * 16;
+    const bool read = (uintptr_t)q % 16 || qs % 16 || qs < (int64_t)d.depth || qs >= 1ll << 40;
+    CUtensorMap map_q = {};
+    if (!read && !encode_levels(&map_q, q, (int64_t)d.depth, (int64_t)d.tokens, qs)) return DCF_ECUDA;
+    rc = bf16 ? run_typed<__nv_bfloat16>(tile_n, read, map, map_q, g, s) : run_typed<__half>(tile_n, read, map, map_q, g, s);
     if (rc || g.splits == 1) return rc;
   }
   const int64_t joins = ((int64_t)d.depth + kJoinThreads - 1) / kJoinThreads * (int64_t)d.channels;
