@@ -16,6 +16,7 @@ namespace {
 constexpr int kSide = 128;                // k of a CTA
 constexpr int kTileM = 2 * kSide;         // of a pair
 constexpr int kReaders = 256;             // threads that turn whole numbers into the gradient's type
+constexpr int kTeam = kReaders / 2;       // of them, for one run; two teams take runs in turn
 constexpr int kOutWarps = 8;
 constexpr int kThreads_ = 128 + kReaders + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
 constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < S; s++) {
-      mbar_init(&full[s], 1 + 2 * kReaders);
+      mbar_init(&full[s], 1 + 2 * kTeam);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; b++) {
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     }
     for (int b = 0; b < kRaws; b++) {
       mbar_init(&raw_full[b], 1);
-      mbar_init(&raw_empty[b], kReaders / 32);
+      mbar_init(&raw_empty[b], kTeam / 32);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -288,30 +289,9 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     // Eight neighbours store four vectors each of a row's first half and of the next
     // row's second one, or the other way round: the swizzle puts them into different banks, and so they lie as read.
     const int chunk = ((lane >> 3 ^ lane >> 2) & 1) * 4 + (lane & 3);
-    const int row = (warp - 4) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
+    const int team = (warp - 4) / (kTeam / 32), row = (warp - 4) % (kTeam / 32) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
     const int beside = (lane & 3) < 3 ? lane + 1 : (lane ^ 8) - 3;  // who has the next vector of the row
-    constexpr int kStep = kReaders / 8, kRows = kRun / kStep, kHalf = READ ? kRows / 2 : kRows;  // loads of a run, and at a time
-    // READ.  The vectors of a run: k of this thread's, and the place of its first row.
-    struct Run {
-      int k, rows;  // rows: of this thread's first one, how many are left of it
-      const int8_t* p;
-    };
-    auto run_of = [&](int k, int r) {
-      const int64_t token = (int64_t)r * kRun + row;
-      return Run{k, (int)min((int64_t)kRun, g.tokens - token), g.q + token * g.qs + k};
-    };
-    auto k_of = [&](int64_t t) { return (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16; };
-    auto read = [&](const Run& u, int j, uint4& own, uint4& next) {
-      const int8_t* p = u.p + j * kStep * g.qs;
-      const int off = READ ? (int)((uintptr_t)p & 15) : 0;
-      const bool there = j * kStep < u.rows;
-      own = make_uint4(0, 0, 0, 0);
-      if (there && u.k - off < g.depth) own = *(const uint4*)(p - off);  // what lies behind the row is not written out
-      if (READ) {
-        next = make_uint4(0, 0, 0, 0);
-        if (there && off && chunk == 7 && u.k + 16 - off < g.depth) next = *(const uint4*)(p - off + 16);
-      }
-    };
+    constexpr int kStep = kTeam / 8, kRows = kRun / kStep, kHalf = kRows / 2;  // rows of a run, and at a time
     Ring<S> at;
     const int c = (chunk & 3) * 2, turn = row & 7;  // kStep rows on, the swizzle is the same
     auto store = [&](int j, const uint4& v) {
@@ -319,72 +299,64 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       *(uint4*)(to + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
       *(uint4*)(to + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
     };
-    if constexpr (!READ) {
-      Ring<kRaws> from;
-      for (int64_t t = first; t < g.total && !fail; t += step) {
-        const int count = count_of(t);
-        for (int r = 0; r < count; r++, at.next(), from.next()) {
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&raw_full[from.s], from.turn))) {
-            fail = true;
-            break;
-          }
-          uint4 v[kRows];
-#pragma unroll
-          for (int j = 0; j < kRows; j++) v[j] = *(const uint4*)(raw + from.s * kRaw + (row + j * kStep) * kSide + chunk * 16);
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
-            fail = true;
-            break;
-          }
-#pragma unroll
-          for (int j = 0; j < kRows; j++) store(j, v[j]);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[from.s]);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          arrive_first(&full[at.s]);
-        }
-      }
-    } else {
-    uint4 own[kRows], next[READ ? kRows : 1];
-    Run now = {};
-    if (first < g.total) {
-      now = run_of(k_of(first), begin_of(first));
-#pragma unroll
-      for (int j = 0; j < kHalf; j++) read(now, j, own[j], next[READ ? j : 0]);
-    }
+    int mine = team;  // runs until this team's next one
+    Ring<kRaws> from;
     for (int64_t t = first; t < g.total && !fail; t += step) {
       const int r0 = begin_of(t), count = count_of(t);
-      for (int r = 0; r < count; r++, at.next()) {
-        Run then = now;
-        if (r + 1 < count) then = run_of(now.k, r0 + r + 1);
-        else if (t + step < g.total) then = run_of(k_of(t + step), begin_of(t + step));
-        else then.rows = 0;
-        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
-          fail = true;
-          break;
-        }
+      const int k = READ ? (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16 : 0;
+      for (int r = 0; r < count; r++, at.next(), from.next(), mine ^= 1) {
+        if (mine) continue;
+        if (READ) {
+          const int64_t token = (int64_t)(r0 + r) * kRun + row;
+          const int8_t* p = g.q + token * g.qs + k;
+          bool waited = false;
 #pragma unroll
-        for (int half = 0; half < kRows; half += kHalf) {
+          for (int half = 0; half < kRows; half += kHalf) {
+            uint4 own[kHalf], next[kHalf];
 #pragma unroll
-          for (int i = 0; i < kHalf; i++) {
-            const int j = half + i;
-            uint4 v = own[i];
-            if (READ) {
-              uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, v.x, beside), __shfl_sync(0xFFFFFFFFu, v.y, beside),
-                                        __shfl_sync(0xFFFFFFFFu, v.z, beside), __shfl_sync(0xFFFFFFFFu, v.w, beside));
-              if (chunk == 7) beyond = next[READ ? i : 0];
-              v = bytes_from(v, beyond, (int)((uintptr_t)(now.p + j * kStep * g.qs) & 15));
+            for (int i = 0; i < kHalf; i++) {
+              const int8_t* line = p + (half + i) * kStep * g.qs;
+              const int off = (int)((uintptr_t)line & 15);
+              const bool there = token + (half + i) * kStep < g.tokens;
+              own[i] = next[i] = make_uint4(0, 0, 0, 0);
+              if (there && k - off < g.depth) own[i] = *(const uint4*)(line - off);  // what lies behind the row is not written out
+              if (there && off && chunk == 7 && k + 16 - off < g.depth) next[i] = *(const uint4*)(line - off + 16);
             }
-            // the next of this register: of the second half of this run, or of the next run
-            if (half + kHalf < kRows) read(now, j + kHalf, own[i], next[READ ? i : 0]);
-            else read(then, i, own[i], next[READ ? i : 0]);
-            store(j, v);
+            if (!waited && __any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+              fail = true;
+              break;
+            }
+            waited = true;
+#pragma unroll
+            for (int i = 0; i < kHalf; i++) {
+              uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, own[i].x, beside), __shfl_sync(0xFFFFFFFFu, own[i].y, beside),
+                                        __shfl_sync(0xFFFFFFFFu, own[i].z, beside), __shfl_sync(0xFFFFFFFFu, own[i].w, beside));
+              if (chunk == 7) beyond = next[i];
+              store(half + i, bytes_from(own[i], beyond, (int)((uintptr_t)(p + (half + i) * kStep * g.qs) & 15)));
+            }
           }
+          if (fail) break;
+        } else {
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&raw_full[from.s], from.turn) ||
+                                          !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+            fail = true;
+            break;
+          }
+          const uint8_t* in = raw + from.s * kRaw + row * kSide + chunk * 16;
+#pragma unroll
+          for (int half = 0; half < kRows; half += kHalf) {
+            uint4 v[kHalf];
+#pragma unroll
+            for (int i = 0; i < kHalf; i++) v[i] = *(const uint4*)(in + (half + i) * kStep * kSide);
+#pragma unroll
+            for (int i = 0; i < kHalf; i++) store(half + i, v[i]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&raw_empty[from.s]);
         }
-        now = then;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
       }
-    }
     }
   } else if (warp >= 4 + kReaders / 32) {
     adder_registers();
