@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         const int col = (int)(t / g.splits / g.tiles_m) * TN + (int)rank * (TN / 2);
         const int r0 = begin_of(t), count = count_of(t);
         for (int r = 0; r < count; r++, at.next()) {
-          if (!mbar_wait_bounded(&empty[at.s], at.turn ^ 1)) {
+          if (!mbar_wait_parked(&empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       // Leave only with no copy of ours and no arrival for us left in flight.
       for (; used > 0; used--) {
         const Ring<S> last = at.back(used);
-        if (!rank && !mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
-        if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
+        if (!rank && !mbar_wait_parked(&full[last.s], last.turn)) fail = true;
+        if (!fail && !mbar_wait_parked(&empty[last.s], last.turn)) fail = true;
       }
     }
   } else if (warp == 2) {
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       for (int64_t t = first; t < g.total && !fail; t += step) {
         const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide, r0 = begin_of(t), count = count_of(t);
         for (int r = 0; r < count; r++, at.next()) {
-          if (!mbar_wait_bounded(&raw_empty[at.s], at.turn ^ 1)) {
+          if (!mbar_wait_parked(&raw_empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       }
       for (; used > 0; used--) {
         const Ring<kRaws> last = at.back(used);
-        if (!mbar_wait_bounded(&raw_full[last.s], last.turn)) fail = true;
+        if (!mbar_wait_parked(&raw_full[last.s], last.turn)) fail = true;
       }
     }
   } else if (warp == 1) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       for (int64_t t = first; t < g.total && !fail; t += step) {
         const int count = count_of(t);
         for (int r = 0; r < count; r++, at.next(), sum.next()) {
-          if (!mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1) || !mbar_wait_bounded(&full[at.s], at.turn)) {
+          if (!mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1) || !mbar_wait_parked(&full[at.s], at.turn)) {
             fail = true;
             break;
           }
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
               if (there && k - off < g.depth) own[i] = *(const uint4*)(line - off);  // what lies behind the row is not written out
               if (there && off && chunk == 7 && k + 16 - off < g.depth) next[i] = *(const uint4*)(line - off + 16);
             }
-            if (!waited && __any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+            if (!waited && __any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
               fail = true;
               break;
             }
@@ -337,8 +337,8 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           }
           if (fail) break;
         } else {
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&raw_full[from.s], from.turn) ||
-                                          !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&raw_full[from.s], from.turn) ||
+                                          !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
             fail = true;
             break;
           }
@@ -377,25 +377,22 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
       for (int r = 0; r < count; r++, sum.next()) {
         scale += g.depth;
         const float then = k < g.depth && r + 1 < count ? *scale : 0.0f;
-        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[sum.s], sum.turn))) {
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&sum_full[sum.s], sum.turn))) {
           fail = true;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t x[2][8];  // one part is added while the next arrives
-        tmem_load8(lanes + sum.s * TN, x[0]);
 #pragma unroll
-        for (int c = 0; c < kMine; c += 8) {
-          tmem_wait(x[c / 8 & 1]);
-          if (c + 8 < kMine) {
-            tmem_load8(lanes + sum.s * TN + c + 8, x[(c / 8 + 1) & 1]);
-          } else {
+        for (int c = 0; c < kMine; c += 16) {
+          uint32_t x[16];
+          tmem_read16(lanes + sum.s * TN + c, x);
+          if (c + 16 == kMine) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) arrive_first(&sum_empty[sum.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 8; j += 2)
-            acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(x[c / 8 & 1][j]), __uint_as_float(x[c / 8 & 1][j + 1])), acc[(c + j) / 2]);
+          for (int j = 0; j < 16; j += 2)
+            acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), acc[(c + j) / 2]);
         }
         s = then;
       }

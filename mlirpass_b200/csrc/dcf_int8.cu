@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
         const int b0 = begin_of(t), blocks = count_of(t);
         for (int k = b0 * kBK, end = (b0 + blocks) * kBK; k < end; k += kBK, at.next()) {
-          if (!mbar_wait_bounded(&empty[at.s], at.turn ^ 1)) {
+          if (!mbar_wait_parked(&empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
@@ -270,8 +270,8 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
       // Leave only with no copy of ours and no arrival for us left in flight.
       for (; used > 0; used--) {
         const Ring<S> last = at.back(used);
-        if (!rank && !mbar_wait_bounded(&full[last.s], last.turn)) fail = true;
-        if (!fail && !mbar_wait_bounded(&empty[last.s], last.turn)) fail = true;
+        if (!rank && !mbar_wait_parked(&full[last.s], last.turn)) fail = true;
+        if (!fail && !mbar_wait_parked(&empty[last.s], last.turn)) fail = true;
       }
     }
   } else if (warp == 1) {
@@ -282,12 +282,12 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
       Ring<2> sum;
       for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
         const int blocks = count_of(t);
-        if (!mbar_wait_bounded(&sum_empty[sum.s], sum.turn ^ 1)) {
+        if (!mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) {
           fail = true;
           break;
         }
         for (int b = 0; b < blocks; b++, at.next()) {
-          if (!mbar_wait_bounded(&full[at.s], at.turn)) {
+          if (!mbar_wait_parked(&full[at.s], at.turn)) {
             fail = true;
             break;
           }
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
           rows_of(t + step);
           read(begin_of(t + step) * kBK);
         }
-        if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&empty[at.s], at.turn ^ 1))) {
+        if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
         }
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         for (int j = lane; j < kMine; j += 32) mine[j] = t0 + j < g.to.tokens ? g.to.a_scale[t0 + j] : 0.0f;
         __syncwarp();
       }
-      if (__any_sync(0xFFFFFFFFu, !mbar_wait_bounded(&sum_full[sum.s], sum.turn))) {
+      if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&sum_full[sum.s], sum.turn))) {
         fail = true;
         break;
       }

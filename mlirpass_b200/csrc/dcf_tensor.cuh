@@ -58,10 +58,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr));
 }
 
-__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
+// Sixteen columns, arrived.  (As one statement: loads whose wait names their registers again cost a move each.)
+__device__ __forceinline__ void tmem_read16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
 }
 
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
@@ -79,13 +85,6 @@ template <int N> __device__ __forceinline__ void tmem_wait(uint32_t (&r)[N]) {
 #pragma unroll
   for (int j = 0; j < N; j++) asm volatile("" : "+r"(r[j]));
 }
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-               :
-               : "memory");
-}
-
 // Two f32 values to an instruction, each rounded as by itself.  (A packed sum
 // after a packed product would be fused with it, whatever rounding is written.)
 __device__ __forceinline__ uint64_t two(float a, float b) {
@@ -107,6 +106,24 @@ __device__ __forceinline__ float2 apart(uint64_t v) {
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
+}
+
+// Bounded wait for phase `parity` of `bar`, like mbar_wait_bounded, but the
+// thread sleeps for up to a microsecond at a time: warps that look again at
+// once take issue slots from those that have something to do.
+constexpr int kParkLimit = 1 << 21;
+__device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, unsigned parity) {
+  const uint32_t at = smem_addr(bar);
+  for (int turns = 0; turns < kParkLimit; turns++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(1000)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
 }
 
 // A place in a ring of S stages and the parity of its turn.  Stepped, not
