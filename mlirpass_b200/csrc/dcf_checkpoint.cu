@@ -264,24 +264,34 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
     }
   } else if (warp == 1) {
     if (lane == 0 && !rank) {
+      // The tensor core has one or two products in hand at most, so a look at a barrier after the last one (160
+      // cycles) leaves it without: whether the next run is there is asked before this one's last products.
       const uint64_t desc = block_desc(stage0);
       Ring<S> at;
       Ring<2> sum;
-      for (int64_t t = first; t < g.total && !fail; t += step) {
-        const int count = count_of(t);
-        for (int r = 0; r < count; r++, at.next(), sum.next()) {
-          if (!mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1) || !mbar_wait_parked(&full[at.s], at.turn)) {
-            fail = true;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t pq = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pg = pq + (kSide * kRun * 2 >> 4);
-#pragma unroll
-          for (int j = 0; j < kRun / 16; j++)
-            pair_mma(tmem + sum.s * TN, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
-          pair_commit(&empty[at.s]);
-          pair_commit(&sum_full[sum.s]);
+      int64_t left = 0;  // runs of this pair
+      for (int64_t t = first; t < g.total; t += step) left += count_of(t);
+      bool room = false, there = false;
+      for (; left > 0; left--) {
+        if ((!room && !mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) || (!there && !mbar_wait_parked(&full[at.s], at.turn))) {
+          fail = true;
+          break;
         }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint64_t pq = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pg = pq + (kSide * kRun * 2 >> 4);
+        uint64_t* const done = &empty[at.s];
+        uint64_t* const summed = &sum_full[sum.s];
+        const uint32_t to = tmem + sum.s * TN;
+        at.next();
+        sum.next();
+#pragma unroll
+        for (int j = 0; j < kRun / 16; j++) {
+          pair_mma(to, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
+          if (j == 3) room = mbar_test(&sum_empty[sum.s], sum.turn ^ 1);
+          if (j == 5) there = mbar_test(&full[at.s], at.turn);
+        }
+        pair_commit(summed);
+        pair_commit(done);
       }
     }
   } else if (warp >= 4 && warp < 4 + kReaders / 32) {

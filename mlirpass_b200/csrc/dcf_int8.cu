@@ -280,22 +280,28 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
       const uint64_t desc = row_desc(stage0);
       Ring<S> at;
       Ring<2> sum;
+      bool there = false;
       for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
         const int blocks = count_of(t);
         if (!mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) {
           fail = true;
           break;
         }
-        for (int b = 0; b < blocks; b++, at.next()) {
-          if (!mbar_wait_parked(&full[at.s], at.turn)) {
+        for (int b = 0; b < blocks; b++) {
+          if (!there && !mbar_wait_parked(&full[at.s], at.turn)) {
             fail = true;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           const uint64_t pb = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pa = pb + (kSide * kBK >> 4);
+          uint64_t* const done = &empty[at.s];
+          at.next();
 #pragma unroll
-          for (int j = 0; j < kBK / 32; j++) pair_mma_i8(tmem + sum.s * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
-          pair_commit(&empty[at.s]);
+          for (int j = 0; j < kBK / 32; j++) {
+            pair_mma_i8(tmem + sum.s * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
+            if (j == 1) there = mbar_test(&full[at.s], at.turn);  // before the tensor core runs out of products
+          }
+          pair_commit(done);
         }
         if (!fail) pair_commit(&sum_full[sum.s]);
       }

@@ -111,7 +111,7 @@ __device__ __forceinline__ float2 apart(uint64_t v) {
 // Bounded wait for phase `parity` of `bar`, like mbar_wait_bounded, but the
 // thread sleeps for up to a microsecond at a time: warps that look again at
 // once take issue slots from those that have something to do.
-constexpr int kParkLimit = 1 << 21;
+constexpr int kParkLimit = 1 << 20;
 __device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, unsigned parity) {
   const uint32_t at = smem_addr(bar);
   for (int turns = 0; turns < kParkLimit; turns++) {
@@ -124,6 +124,17 @@ __device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, unsigned parity)
     if (ok) return true;
   }
   return false;
+}
+
+// Whether phase `parity` of `bar` is over.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, unsigned parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 
 // A place in a ring of S stages and the parity of its turn.  Stepped, not
