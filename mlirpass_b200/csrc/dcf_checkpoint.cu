@@ -93,10 +93,10 @@ template <class T> __device__ __forceinline__ uint4 to_eight(uint32_t a, uint32_
 }
 
 // 640 threads start with 96 registers each; warps 0 to 3 keep 32, the eight
-// that read 56, and the eight that add up get 168: 128 * 32 + 256 * 56 + 256 * 168 = 640 * 96.
+// that read 64, and the eight that add up get 160: 128 * 32 + 256 * 64 + 256 * 160 = 640 * 96.
 __device__ __forceinline__ void control_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 32;"); }
-__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
-__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 168;"); }
+__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
+__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 160;"); }
 
 __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, float v) {
   const int64_t at = c * g.os + k;
@@ -347,22 +347,23 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           }
           if (fail) break;
         } else {
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&raw_full[from.s], from.turn) ||
-                                          !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&raw_full[from.s], from.turn))) {
             fail = true;
             break;
           }
+          // All of it into registers at once: the place is free for the run after the next.
           const uint8_t* in = raw + from.s * kRaw + row * kSide + chunk * 16;
+          uint4 v[kRows];
 #pragma unroll
-          for (int half = 0; half < kRows; half += kHalf) {
-            uint4 v[kHalf];
-#pragma unroll
-            for (int i = 0; i < kHalf; i++) v[i] = *(const uint4*)(in + (half + i) * kStep * kSide);
-#pragma unroll
-            for (int i = 0; i < kHalf; i++) store(half + i, v[i]);
-          }
+          for (int j = 0; j < kRows; j++) v[j] = *(const uint4*)(in + j * kStep * kSide);
           __syncwarp();
           if (lane == 0) mbar_arrive(&raw_empty[from.s]);
+          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
+            fail = true;
+            break;
+          }
+#pragma unroll
+          for (int j = 0; j < kRows; j++) store(j, v[j]);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
