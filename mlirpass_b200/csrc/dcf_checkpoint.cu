@@ -7,6 +7,12 @@
 // registers multiply that by the scale and add it, rounding to nearest.  (The
 // tensor core truncates as it accumulates; longer sums in TMEM would be further
 // from 64 bits than fp32 products are.)
+//
+// Whole numbers become 16-bit values in a pass of their own (three bytes of
+// memory each).  Made on their way into each tile instead, by eight warps
+// between the copy and the product, they cost 270 us at 8192 x 4096 x 4096
+// against XX: every tile makes them again, and what they are copied, read and
+// written in shared memory there (384 KB a microsecond) is what the operands of the products need.
 #include "dcf_quant.cuh"
 
 namespace dcf {
@@ -15,10 +21,8 @@ namespace {
 
 constexpr int kSide = 128;                // k of a CTA
 constexpr int kTileM = 2 * kSide;         // of a pair
-constexpr int kReaders = 256;             // threads that turn whole numbers into the gradient's type
-constexpr int kTeam = kReaders / 2;       // of them, for one run; two teams take runs in turn
 constexpr int kOutWarps = 8;
-constexpr int kThreads_ = 128 + kReaders + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies
+constexpr int kGemmThreads = 128 + 32 * kOutWarps;  // warp 0 loads, warp 1 multiplies, 2 and 3 lend their registers
 constexpr int kPairs = 74;                // of SMs on a B200; any number runs the persistent grid
 
 // A stage is a run: 128 tokens of 128 k and of TN / 2 channels in two bytes each, in
@@ -26,19 +30,16 @@ constexpr int kPairs = 74;                // of SMs on a B200; any number runs t
 constexpr int kBlockBytes = kRun * 128;
 template <int TN> constexpr int kStage = (kSide + TN / 2) * kRun * 2;
 template <int TN> constexpr int kStages = TN == 256 ? 3 : 4;
-// Whole numbers on their way to their operand: two runs of 128 k.
-constexpr int kRaw = kSide * kRun, kRaws = 2;
-template <int TN> constexpr int kSmem = kStages<TN> * kStage<TN> + kRaws * kRaw + 256 + 1024;
+template <int TN> constexpr int kSmem = kStages<TN> * kStage<TN> + 256 + 1024;
 
 struct GradArgs {
-  const int8_t* q;
   const float* scale;
   void* out;
   int out_dtype, add;
   int pairs;               // two neighbours of a row of a 16-bit result make an aligned word
   int tokens, channels, depth;
   int skip;                // columns of the gradient's map before its first channel
-  int64_t qs, os;
+  int64_t os;
   int runs, tiles_m;       // tiles along k
   int splits, split_runs;  // parts of the runs, runs of each
   int64_t total;           // tiles times splits
@@ -55,21 +56,21 @@ __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* ma
       : "memory");
 }
 
-__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+// The low half of an operand's descriptor, whose memory runs along it: blocks of 64
+// lie kBlockBytes apart.  The high half says that groups of eight tokens lie
+// 1024 bytes apart, and the 128-byte swizzle.  (In halves because the thread that issues
+// has few registers, and waits for none.)
+__device__ __forceinline__ uint32_t block_desc(uint32_t addr) {
+  return ((addr >> 4) & 0x3FFF) | (uint32_t)(kBlockBytes >> 4) << 16;
+}
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+
+__device__ __forceinline__ void pair_mma_low(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(smem_addr(bar))
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
-}
-
-// An operand whose memory runs along it: blocks of 64 lie kBlockBytes apart,
-// groups of eight tokens 1024 bytes.
-__device__ __forceinline__ uint64_t block_desc(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kBlockBytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // Two of a word's signed bytes (the low ones of its halves) in a 16-bit type.
@@ -91,12 +92,6 @@ template <class T> __device__ __forceinline__ uint4 to_eight(uint32_t a, uint32_
   return make_uint4(to_halves<T>(__byte_perm(a, 0, 0x4140)), to_halves<T>(__byte_perm(a, 0, 0x4342)),
                     to_halves<T>(__byte_perm(b, 0, 0x4140)), to_halves<T>(__byte_perm(b, 0, 0x4342)));
 }
-
-// 640 threads start with 96 registers each; warps 0 to 3 keep 32, the eight
-// that read 64, and the eight that add up get 160: 128 * 32 + 256 * 64 + 256 * 160 = 640 * 96.
-__device__ __forceinline__ void control_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 32;"); }
-__device__ __forceinline__ void reader_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 64;"); }
-__device__ __forceinline__ void adder_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 160;"); }
 
 __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, float v) {
   const int64_t at = c * g.os + k;
@@ -149,29 +144,24 @@ template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, i
 }
 
 // D = q^T grad of each run in tiles of 256 k x TN channels by persistent pairs
-// of CTAs, each with 128 k and half of the channels.  Warp 0 loads the gradient; eight
-// warps read whole numbers, a run ahead, and write them as operands of the
-// gradient's type; one thread of the first CTA issues the eight products of a
-// run for both; eight warps take a run's sums out of one of two buffers of TMEM while
-// the other is filled.  k lies in the lanes: a lane needs one scale a run, and
-// a warp writes neighbours of a row.  READ: rows of whole numbers lie off
-// 16-byte boundaries; they are read as the 16-byte vectors that hold them, and
-// neighbours in a warp make up what they lack from each other.
-template <class T, int TN, bool READ>
-__global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_q,
-                                                            const GradArgs args) {
+// of CTAs, each with 128 k and half of the channels.  Warp 0 loads; one thread
+// of the first CTA issues the eight products of a run for both; eight warps
+// take a run's sums out of one of two buffers of TMEM while the other is
+// filled.  k lies in the lanes: a lane needs one scale a run, and a warp writes
+// neighbours of a row.
+template <int TN>
+__global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_constant__ CUtensorMap map_q,
+                                                               const __grid_constant__ CUtensorMap map_g,
+                                                               const GradArgs args) {
   const GradArgs g = args;  // a reference to the parameter itself would be read through memory
   constexpr int S = kStages<TN>, kMine = TN / 2;  // columns of one out warp
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
-  uint8_t* raw = base + S * kStage<TN>;
-  uint64_t* full = (uint64_t*)(raw + kRaws * kRaw);  // the first CTA's counts what both have
+  uint64_t* full = (uint64_t*)(base + S * kStage<TN>);  // the first CTA's counts what both have
   uint64_t* empty = full + S;
   uint64_t* sum_full = empty + S;
   uint64_t* sum_empty = sum_full + 2;  // the first CTA's
-  uint64_t* raw_full = sum_empty + 2;
-  uint64_t* raw_empty = raw_full + kRaws;
-  uint32_t* tmem_at = (uint32_t*)(raw_empty + kRaws);
+  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -183,16 +173,12 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < S; s++) {
-      mbar_init(&full[s], 1 + 2 * kTeam);
+      mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
       mbar_init(&sum_empty[b], 2 * kOutWarps);
-    }
-    for (int b = 0; b < kRaws; b++) {
-      mbar_init(&raw_full[b], 1);
-      mbar_init(&raw_empty[b], kTeam / 32);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -208,29 +194,34 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *(volatile uint32_t*)tmem_at;
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_g) : "memory");
-    if (!READ) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_q) : "memory");
   }
   pdl_begin();
 
   bool fail = false;
-  if (warp < 4) control_registers();
+  if (warp < 4) shrink_registers();
   if (warp == 0) {
     if (lane == 0) {
       Ring<S> at;
       int used = 0;  // stages filled, S at most
       for (int64_t t = first; t < g.total && !fail; t += step) {
-        const int col = (int)(t / g.splits / g.tiles_m) * TN + (int)rank * (TN / 2);
+        const int64_t tile = t / g.splits;
+        const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
+        const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
         const int r0 = begin_of(t), count = count_of(t);
         for (int r = 0; r < count; r++, at.next()) {
           if (!mbar_wait_parked(&empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
-          const uint32_t to = stage0 + at.s * kStage<TN> + kSide * kRun * 2, bar = full0 + at.s * 8;
-          if (!rank) mbar_expect_tx(&full[at.s], TN * kRun * 2);
-          pair_load_2d(to, &map_g, col, (r0 + r) * kRun, bar);
-          if (TN == 256) pair_load_2d(to + kBlockBytes, &map_g, col + 64, (r0 + r) * kRun, bar);
+          const uint32_t to = stage0 + at.s * kStage<TN>, bar = full0 + at.s * 8;
+          const int token = (r0 + r) * kRun;
+          if (!rank) mbar_expect_tx(&full[at.s], 2 * kStage<TN>);
+          pair_load_2d(to, &map_q, row, token, bar);
+          pair_load_2d(to + kBlockBytes, &map_q, row + 64, token, bar);
+          pair_load_2d(to + 2 * kBlockBytes, &map_g, col, token, bar);
+          if (TN == 256) pair_load_2d(to + 3 * kBlockBytes, &map_g, col + 64, token, bar);
           used += used < S;
         }
       }
@@ -241,32 +232,11 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         if (!fail && !mbar_wait_parked(&empty[last.s], last.turn)) fail = true;
       }
     }
-  } else if (warp == 2) {
-    if (!READ && lane == 0) {
-      Ring<kRaws> at;
-      int used = 0;
-      for (int64_t t = first; t < g.total && !fail; t += step) {
-        const int k = (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide, r0 = begin_of(t), count = count_of(t);
-        for (int r = 0; r < count; r++, at.next()) {
-          if (!mbar_wait_parked(&raw_empty[at.s], at.turn ^ 1)) {
-            fail = true;
-            break;
-          }
-          mbar_expect_tx(&raw_full[at.s], kRaw);
-          load_2d(smem_addr(raw + at.s * kRaw), &map_q, k, (r0 + r) * kRun, &raw_full[at.s]);
-          used += used < kRaws;
-        }
-      }
-      for (; used > 0; used--) {
-        const Ring<kRaws> last = at.back(used);
-        if (!mbar_wait_parked(&raw_full[last.s], last.turn)) fail = true;
-      }
-    }
   } else if (warp == 1) {
     if (lane == 0 && !rank) {
       // The tensor core has one or two products in hand at most, so a look at a barrier after the last one (160
       // cycles) leaves it without: whether the next run is there is asked before this one's last products.
-      const uint64_t desc = block_desc(stage0);
+      const uint32_t desc = block_desc(stage0);
       Ring<S> at;
       Ring<2> sum;
       int64_t left = 0;  // runs of this pair
@@ -278,7 +248,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint64_t pq = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pg = pq + (kSide * kRun * 2 >> 4);
+        const uint32_t pq = desc + (uint32_t)(at.s * (kStage<TN> >> 4)), pg = pq + (kSide * kRun * 2 >> 4);
         uint64_t* const done = &empty[at.s];
         uint64_t* const summed = &sum_full[sum.s];
         const uint32_t to = tmem + sum.s * TN;
@@ -286,7 +256,7 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         sum.next();
 #pragma unroll
         for (int j = 0; j < kRun / 16; j++) {
-          pair_mma(to, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
+          pair_mma_low(to, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
           if (j == 3) room = mbar_test(&sum_empty[sum.s], sum.turn ^ 1);
           if (j == 5) there = mbar_test(&full[at.s], at.turn);
         }
@@ -294,85 +264,10 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
         pair_commit(done);
       }
     }
-  } else if (warp >= 4 && warp < 4 + kReaders / 32) {
-    reader_registers();
-    // Eight neighbours store four vectors each of a row's first half and of the next
-    // row's second one, or the other way round: the swizzle puts them into different banks, and so they lie as read.
-    const int chunk = ((lane >> 3 ^ lane >> 2) & 1) * 4 + (lane & 3);
-    const int team = (warp - 4) / (kTeam / 32), row = (warp - 4) % (kTeam / 32) * 4 + (lane >> 4) * 2 + (lane >> 2 & 1);
-    const int beside = (lane & 3) < 3 ? lane + 1 : (lane ^ 8) - 3;  // who has the next vector of the row
-    constexpr int kStep = kTeam / 8, kRows = kRun / kStep, kHalf = kRows / 2;  // rows of a run, and at a time
-    Ring<S> at;
-    const int c = (chunk & 3) * 2, turn = row & 7;  // kStep rows on, the swizzle is the same
-    auto store = [&](int j, const uint4& v) {
-      uint8_t* to = base + at.s * kStage<TN> + (chunk >> 2) * kBlockBytes + (row + j * kStep) * 128;
-      *(uint4*)(to + ((c ^ turn) << 4)) = to_eight<T>(v.x, v.y);
-      *(uint4*)(to + (((c + 1) ^ turn) << 4)) = to_eight<T>(v.z, v.w);
-    };
-    int mine = team;  // runs until this team's next one
-    Ring<kRaws> from;
-    for (int64_t t = first; t < g.total && !fail; t += step) {
-      const int r0 = begin_of(t), count = count_of(t);
-      const int k = READ ? (int)(t / g.splits % g.tiles_m) * kTileM + (int)rank * kSide + chunk * 16 : 0;
-      for (int r = 0; r < count; r++, at.next(), from.next(), mine ^= 1) {
-        if (mine) continue;
-        if (READ) {
-          const int64_t token = (int64_t)(r0 + r) * kRun + row;
-          const int8_t* p = g.q + token * g.qs + k;
-          bool waited = false;
-#pragma unroll
-          for (int half = 0; half < kRows; half += kHalf) {
-            uint4 own[kHalf], next[kHalf];
-#pragma unroll
-            for (int i = 0; i < kHalf; i++) {
-              const int8_t* line = p + (half + i) * kStep * g.qs;
-              const int off = (int)((uintptr_t)line & 15);
-              const bool there = token + (half + i) * kStep < g.tokens;
-              own[i] = next[i] = make_uint4(0, 0, 0, 0);
-              if (there && k - off < g.depth) own[i] = *(const uint4*)(line - off);  // what lies behind the row is not written out
-              if (there && off && chunk == 7 && k + 16 - off < g.depth) next[i] = *(const uint4*)(line - off + 16);
-            }
-            if (!waited && __any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
-              fail = true;
-              break;
-            }
-            waited = true;
-#pragma unroll
-            for (int i = 0; i < kHalf; i++) {
-              uint4 beyond = make_uint4(__shfl_sync(0xFFFFFFFFu, own[i].x, beside), __shfl_sync(0xFFFFFFFFu, own[i].y, beside),
-                                        __shfl_sync(0xFFFFFFFFu, own[i].z, beside), __shfl_sync(0xFFFFFFFFu, own[i].w, beside));
-              if (chunk == 7) beyond = next[i];
-              store(half + i, bytes_from(own[i], beyond, (int)((uintptr_t)(p + (half + i) * kStep * g.qs) & 15)));
-            }
-          }
-          if (fail) break;
-        } else {
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&raw_full[from.s], from.turn))) {
-            fail = true;
-            break;
-          }
-          // All of it into registers at once: the place is free for the run after the next.
-          const uint8_t* in = raw + from.s * kRaw + row * kSide + chunk * 16;
-          uint4 v[kRows];
-#pragma unroll
-          for (int j = 0; j < kRows; j++) v[j] = *(const uint4*)(in + j * kStep * kSide);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&raw_empty[from.s]);
-          if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
-            fail = true;
-            break;
-          }
-#pragma unroll
-          for (int j = 0; j < kRows; j++) store(j, v[j]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        arrive_first(&full[at.s]);
-      }
-    }
-  } else if (warp >= 4 + kReaders / 32) {
-    adder_registers();
+  } else if (warp >= 4) {
+    grow_registers();
     const int part = warp & 3;               // the 32 TMEM lanes this warp may read
-    const int col = (warp - 4 - kReaders / 32) / 4 * kMine;  // and the half of the columns it takes
+    const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     Ring<2> sum;
     for (int64_t t = first; t < g.total && !fail; t += step) {
@@ -393,17 +288,21 @@ __global__ void __launch_bounds__(kThreads_, 1) grad_kernel(const __grid_constan
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        uint32_t x[2][32];  // one part is added while the next arrives
+        tmem_load32(lanes + sum.s * TN, x[0]);
 #pragma unroll
-        for (int c = 0; c < kMine; c += 16) {
-          uint32_t x[16];
-          tmem_read16(lanes + sum.s * TN + c, x);
-          if (c + 16 == kMine) {
+        for (int c = 0; c < kMine; c += 32) {
+          uint32_t(&y)[32] = x[c / 32 & 1];
+          tmem_wait(y);
+          if (c + 32 < kMine) {
+            tmem_load32(lanes + sum.s * TN + c + 32, x[(c / 32 + 1) & 1]);
+          } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) arrive_first(&sum_empty[sum.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 16; j += 2)
-            acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(x[j]), __uint_as_float(x[j + 1])), acc[(c + j) / 2]);
+          for (int j = 0; j < 32; j += 2)
+            acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), acc[(c + j) / 2]);
         }
         s = then;
       }
@@ -458,28 +357,33 @@ __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_co
   }
 }
 
+// Whole numbers as values of T, rows of whole vectors; a thread makes sixteen.
+constexpr int kLevelThreads = 256;
+template <class T>
+__global__ void __launch_bounds__(kLevelThreads) levels_kernel(const int8_t* q, int64_t stride, int64_t rows, int64_t cols,
+                                                               T* to, int64_t to_stride) {
+  pdl_begin();
+  const int64_t groups = (cols + 15) / 16, all = groups * rows;
+  for (int64_t i = (int64_t)blockIdx.x * kLevelThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kLevelThreads) {
+    const int64_t r = i / groups, c = i % groups * 16;
+    const uint4 v = row_bytes((const uint8_t*)q + r * stride, c, cols);
+    uint4* out = (uint4*)(to + r * to_stride + c);
+    out[0] = to_eight<T>(v.x, v.y);
+    out[1] = to_eight<T>(v.z, v.w);
+  }
+}
+
 // ---------------------------------------------------------------- host
 
-// The gradient as boxes of 64 channels x 128 tokens.
-bool encode_grad(CUtensorMap* map, const void* p, bool bf16, int64_t channels, int64_t tokens, int64_t stride) {
-  const cuuint64_t dims[2] = {(cuuint64_t)channels, (cuuint64_t)tokens};
+// An operand as boxes of 64 columns x 128 tokens.
+bool encode_operand(CUtensorMap* map, const void* p, bool bf16, int64_t cols, int64_t tokens, int64_t stride) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)tokens};
   const cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
   const cuuint32_t boxes[2] = {64, kRun};
   const cuuint32_t estr[2] = {1, 1};
   return encoder()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, (void*)p, dims,
                    strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Whole numbers as boxes of 128 k x 128 tokens.
-bool encode_levels(CUtensorMap* map, const int8_t* p, int64_t depth, int64_t tokens, int64_t stride) {
-  const cuuint64_t dims[2] = {(cuuint64_t)depth, (cuuint64_t)tokens};
-  const cuuint64_t strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t boxes[2] = {kSide, kRun};
-  const cuuint32_t estr[2] = {1, 1};
-  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
-         CUDA_SUCCESS;
 }
 
 int64_t stride_of(int64_t given, uint64_t cols) { return given ? given : (int64_t)cols; }
@@ -513,12 +417,13 @@ Cut cut_of(const dcf_checkpoint_desc& d, int skip) {
   return best;
 }
 
-// The workspace: a copy of a gradient whose stride no tensor map takes, and the parts of sums.
+// The workspace: whole numbers as 16-bit values, a copy of a gradient whose stride no tensor map takes,
+// and the parts of sums.
 struct Layout {
   Cut cut;
   bool copy;
-  int64_t stride;          // of the copy, in elements
-  size_t grad, part, bytes;
+  int64_t stride, level_stride;  // of the copies, in elements
+  size_t levels, grad, part, bytes;
 };
 
 Layout layout_of(const dcf_checkpoint_desc& d, int skip) {
@@ -532,20 +437,17 @@ Layout layout_of(const dcf_checkpoint_desc& d, int skip) {
   const int64_t gs = stride_of(d.grad_row_stride, d.channels);
   l.copy = d.tokens > 1 && (gs % 8 || gs < (int64_t)d.channels || gs >= 1ll << 38);
   l.stride = (int64_t)((d.channels + 7) / 8 * 8);
+  l.level_stride = (int64_t)((d.depth + 15) / 16 * 16);
+  l.levels = take((size_t)d.tokens * l.level_stride * 2);
   l.grad = take(l.copy ? (size_t)d.tokens * l.stride * 2 : 0);
   l.part = take(l.cut.splits > 1 ? (size_t)l.cut.tiles * l.cut.splits * kTileM * l.cut.tile_n * 4 : 0);
   return l;
 }
 
-template <class T, int TN, bool READ> int run(const CUtensorMap& map, const CUtensorMap& map_q, const GradArgs& g, cudaStream_t s) {
-  if (!prepare_smem((const void*)grad_kernel<T, TN, READ>, kSmem<TN>)) return DCF_ECUDA;
+template <int TN> int run(const CUtensorMap& map_q, const CUtensorMap& map_g, const GradArgs& g, cudaStream_t s) {
+  if (!prepare_smem((const void*)grad_kernel<TN>, kSmem<TN>)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
-  return launch(grad_kernel<T, TN, READ>, dim3(2 * pairs), kThreads_, kSmem<TN>, 2, s, map, map_q, g);
-}
-
-template <class T> int run_typed(int tile_n, bool read, const CUtensorMap& map, const CUtensorMap& map_q, const GradArgs& g, cudaStream_t s) {
-  if (tile_n == 256) return read ? run<T, 256, true>(map, map_q, g, s) : run<T, 256, false>(map, map_q, g, s);
-  return read ? run<T, 128, true>(map, map_q, g, s) : run<T, 128, false>(map, map_q, g, s);
+  return launch(grad_kernel<TN>, dim3(2 * pairs), kGemmThreads, kSmem<TN>, 2, s, map_q, map_g, g);
 }
 
 }  // namespace
@@ -587,7 +489,6 @@ size_t checkpoint_workspace(const dcf_checkpoint_desc& d) {
 int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const int8_t* q, const float* scale,
                            void* out, void* ws, dcf_status* st, cudaStream_t s) {
   GradArgs g = {};
-  g.q = q;
   g.scale = scale;
   g.out = out;
   g.out_dtype = (int)d.out_dtype;
@@ -595,7 +496,6 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
   g.tokens = (int)d.tokens;
   g.channels = (int)d.channels;
   g.depth = (int)d.depth;
-  g.qs = stride_of(d.q_row_stride, d.depth);
   g.os = stride_of(d.out_row_stride, d.depth);
   g.pairs = (uintptr_t)out % 4 == 0 && (d.channels == 1 || g.os % 2 == 0);
   g.st = st;
@@ -615,10 +515,19 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     if (g.skip) l = layout_of(d, g.skip);
     const bool bf16 = d.grad_dtype == DCF_BF16;
     if (!encoder()) return DCF_EUNSUPPORTED;
-    CUtensorMap map;
+    void* levels = (uint8_t*)ws + l.levels;
+    const int64_t all = l.level_stride / 16 * (int64_t)d.tokens, blocks = (all + kLevelThreads - 1) / kLevelThreads;
+    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30));
+    const int64_t qs = stride_of(d.q_row_stride, d.depth), rows = (int64_t)d.tokens, cols = (int64_t)d.depth;
+    rc = bf16 ? launch(levels_kernel<__nv_bfloat16>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__nv_bfloat16*)levels,
+                       l.level_stride)
+              : launch(levels_kernel<__half>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__half*)levels, l.level_stride);
+    if (rc) return rc;
+    CUtensorMap map_q, map_g;
     tile_n = l.cut.tile_n;
-    const int64_t wide = (int64_t)d.channels + g.skip;
-    if (!encode_grad(&map, (const uint8_t*)grad - g.skip * 2, bf16, wide, (int64_t)d.tokens, gs)) return DCF_ECUDA;
+    if (!encode_operand(&map_q, levels, bf16, cols, rows, l.level_stride) ||
+        !encode_operand(&map_g, (const uint8_t*)grad - g.skip * 2, bf16, (int64_t)d.channels + g.skip, rows, gs))
+      return DCF_ECUDA;
     g.runs = (int)((d.tokens + kRun - 1) / kRun);
     g.tiles_m = (int)l.cut.tiles_m;
     g.splits = l.cut.splits;
@@ -627,11 +536,7 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     g.part = (float*)((uint8_t*)ws + l.part);
     g.idesc = (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | ((uint32_t)(tile_n >> 3) << 17) |
               ((uint32_t)(kTileM >> 4) << 24);
-    const int64_t qs = d.tokens > 1 ? g.qs : ((int64_t)d.depth + 15) / 16 * 16;
-    const bool read = (uintptr_t)q % 16 || qs % 16 || qs < (int64_t)d.depth || qs >= 1ll << 40;
-    CUtensorMap map_q = {};
-    if (!read && !encode_levels(&map_q, q, (int64_t)d.depth, (int64_t)d.tokens, qs)) return DCF_ECUDA;
-    rc = bf16 ? run_typed<__nv_bfloat16>(tile_n, read, map, map_q, g, s) : run_typed<__half>(tile_n, read, map, map_q, g, s);
+    rc = tile_n == 256 ? run<256>(map_q, map_g, g, s) : run<128>(map_q, map_g, g, s);
     if (rc || g.splits == 1) return rc;
   }
   const int64_t joins = ((int64_t)d.depth + kJoinThreads - 1) / kJoinThreads * (int64_t)d.channels;

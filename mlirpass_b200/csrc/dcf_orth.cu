@@ -60,11 +60,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-// 384 threads start with 168 registers each; the first four warps keep 40 and
-// the eight that add up get 232: 128 * 40 + 256 * 232 = 384 * 168.
-__device__ __forceinline__ void shrink_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
-__device__ __forceinline__ void grow_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
-
 // Shared-memory descriptor of one plane of an operand with the 128-byte
 // swizzle: groups of eight 128-byte rows lie 1024 bytes apart.  A K-major
 // plane has a row of 64 k for each of 128 rows of the operand; one whose rows

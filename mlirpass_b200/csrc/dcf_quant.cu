@@ -253,23 +253,8 @@ __global__ void __launch_bounds__(kQuantThreads) pack_kernel(const uint8_t* from
   pdl_begin();
   const int64_t groups = (bytes + 15) / 16, all = groups * rows;
   for (int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kQuantThreads) {
-    const int64_t r = i / groups, c = i % groups * 16, have = bytes - c;
-    const uint8_t* p = from + r * stride + c;
-    const int off = (int)((uintptr_t)p & 3);
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (have >= 20 && c >= 4) {  // the words around these bytes lie in the row
-      const uint32_t* a = (const uint32_t*)(p - off);
-      uint32_t v[5];
-#pragma unroll
-      for (int j = 0; j < 5; j++) v[j] = a[j];
-#pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; e++)
-        if (e < have) w[e >> 2] |= (uint32_t)p[e] << ((e & 3) * 8);
-    }
-    *(uint4*)(to + r * to_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    const int64_t r = i / groups, c = i % groups * 16;
+    *(uint4*)(to + r * to_stride + c) = row_bytes(from + r * stride, c, bytes);
   }
 }
 

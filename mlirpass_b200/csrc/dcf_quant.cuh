@@ -152,6 +152,28 @@ __device__ __forceinline__ uint4 bytes_from(const uint4& own, const uint4& next,
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Sixteen bytes of a row of `bytes` from byte c (a multiple of 16) on, zeros behind its end; the row may start anywhere.
+__device__ __forceinline__ uint4 row_bytes(const uint8_t* row, int64_t c, int64_t bytes) {
+  const uint8_t* p = row + c;
+  const int64_t have = bytes - c;
+  if (have >= 16 && (uintptr_t)p % 16 == 0) return *(const uint4*)p;
+  const int off = (int)((uintptr_t)p & 3);
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (have >= 20 && c >= 4) {  // the words around these bytes lie in the row
+    const uint32_t* a = (const uint32_t*)(p - off);
+    uint32_t v[5];
+#pragma unroll
+    for (int j = 0; j < 5; j++) v[j] = a[j];
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(v[j], v[j + 1], off * 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (e < have) w[e >> 2] |= (uint32_t)p[e] << ((e & 3) * 8);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // Copies rows that no tensor map describes (they start off 16-byte boundaries)
 // to rows of whole vectors; sizes and strides in bytes.
 int launch_pack_rows(const void* from, int64_t stride, int64_t rows, int64_t bytes, void* to, int64_t to_stride,

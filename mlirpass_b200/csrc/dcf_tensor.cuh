@@ -58,18 +58,6 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr));
 }
 
-// Sixteen columns, arrived.  (As one statement: loads whose wait names their registers again cost a move each.)
-__device__ __forceinline__ void tmem_read16(uint32_t addr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr)
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -107,6 +95,11 @@ __device__ __forceinline__ float2 apart(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
+
+// 384 threads start with 168 registers each; the first four warps keep 40 and
+// the eight that add up get 232: 128 * 40 + 256 * 232 = 384 * 168.
+__device__ __forceinline__ void shrink_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
+__device__ __forceinline__ void grow_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
 
 // Bounded wait for phase `parity` of `bar`, like mbar_wait_bounded, but the
 // thread sleeps for up to a microsecond at a time: warps that look again at
