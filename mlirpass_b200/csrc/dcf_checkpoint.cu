@@ -42,7 +42,7 @@ struct GradArgs {
   int64_t os;
   int runs, tiles_m;       // tiles along k
   int splits, split_runs;  // parts of the runs, runs of each
-  int64_t total;           // tiles times splits
+  int total;               // tiles times splits
   float* part;             // sums of the parts, where there is more than one
   uint32_t idesc;
   dcf_status* st;
@@ -101,18 +101,18 @@ __device__ __forceinline__ void put(const GradArgs& g, int64_t c, int64_t k, flo
 }
 
 // 16 columns (channels from c0 on) of 32 k, a k in each lane.
-__device__ __forceinline__ void write_block(const GradArgs& g, const float* v, int64_t c0, int64_t k) {
+__device__ __forceinline__ void write_block(const GradArgs& g, const float* v, int c0, int k) {
   if (g.out_dtype == DCF_F32) {
     if (k >= g.depth) return;
-    float* out = (float*)g.out + c0 * g.os + k;
+    float* out = (float*)g.out + (int64_t)c0 * g.os + k;
 #pragma unroll
     for (int j = 0; j < 16; j++, out += g.os)
       if (c0 + j >= 0 && c0 + j < g.channels) *out = g.add ? __fadd_rn(*out, v[j]) : v[j];
   } else if (g.pairs) {
     // Lanes trade: an even one writes its channel for two k, an odd one the next channel.
     const int odd = threadIdx.x & 1;
-    uint16_t* out = (uint16_t*)g.out + (c0 + odd) * g.os + (k & ~1ll);
-    const bool both = (k | 1) < g.depth, one = (k & ~1ll) < g.depth, half = g.out_dtype == DCF_F16;
+    uint16_t* out = (uint16_t*)g.out + (int64_t)(c0 + odd) * g.os + (k & ~1);
+    const bool both = (k | 1) < g.depth, one = (k & ~1) < g.depth, half = g.out_dtype == DCF_F16;
 #pragma unroll
     for (int j = 0; j < 16; j += 2, out += 2 * g.os) {
       const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
@@ -125,7 +125,7 @@ __device__ __forceinline__ void write_block(const GradArgs& g, const float* v, i
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         w = *(const uint32_t*)&h;
       }
-      const int64_t c = c0 + j + odd;
+      const int c = c0 + j + odd;
       if (c >= 0 && c < g.channels) {
         if (both) *(uint32_t*)out = w;
         else if (one) *out = (uint16_t)w;
@@ -139,8 +139,8 @@ __device__ __forceinline__ void write_block(const GradArgs& g, const float* v, i
 }
 
 // Sums of a part: [column of the tile][k of the tile].
-template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, int64_t item) {
-  return g.part + item * (kTileM * TN);
+template <int TN> __device__ __forceinline__ float* part_of(const GradArgs& g, int item) {
+  return g.part + (int64_t)item * (kTileM * TN);
 }
 
 // D = q^T grad of each run in tiles of 256 k x TN channels by persistent pairs
@@ -164,12 +164,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
   uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
-  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
+  const int first = (int)(blockIdx.x / 2), step = (int)(gridDim.x / 2);
   const uint32_t stage0 = smem_addr(base);
   uint32_t full0;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(full0) : "r"(smem_addr(full)));
-  auto begin_of = [&](int64_t t) { return (int)(t % g.splits) * g.split_runs; };
-  auto count_of = [&](int64_t t) { return min(g.split_runs, g.runs - begin_of(t)); };
+  auto begin_of = [&](int t) { return t % g.splits * g.split_runs; };
+  auto count_of = [&](int t) { return min(g.split_runs, g.runs - begin_of(t)); };
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < S; s++) {
@@ -205,10 +205,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
     if (lane == 0) {
       Ring<S> at;
       int used = 0;  // stages filled, S at most
-      for (int64_t t = first; t < g.total && !fail; t += step) {
-        const int64_t tile = t / g.splits;
-        const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
-        const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
+      for (int t = first; t < g.total && !fail; t += step) {
+        const int tile = t / g.splits;
+        const int row = (tile % g.tiles_m) * kTileM + (int)rank * kSide;
+        const int col = tile / g.tiles_m * TN + (int)rank * (TN / 2);
         const int r0 = begin_of(t), count = count_of(t);
         for (int r = 0; r < count; r++, at.next()) {
           if (!mbar_wait_parked(&empty[at.s], at.turn ^ 1)) {
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
       const uint32_t desc = block_desc(stage0);
       Ring<S> at;
       Ring<2> sum;
-      int64_t left = 0;  // runs of this pair
-      for (int64_t t = first; t < g.total; t += step) left += count_of(t);
+      int left = 0;  // runs of this pair
+      for (int t = first; t < g.total; t += step) left += count_of(t);
       bool room = false, there = false;
       for (; left > 0; left--) {
         if ((!room && !mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) || (!there && !mbar_wait_parked(&full[at.s], at.turn))) {
@@ -270,10 +270,10 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
     const int col = (warp - 4) / 4 * kMine;  // and the half of the columns it takes
     const uint32_t lanes = tmem + ((uint32_t)(part * 32) << 16) + col;
     Ring<2> sum;
-    for (int64_t t = first; t < g.total && !fail; t += step) {
-      const int64_t tile = t / g.splits;
+    for (int t = first; t < g.total && !fail; t += step) {
+      const int tile = t / g.splits;
       const int row = (int)rank * kSide + part * 32 + lane;  // of the tile
-      const int64_t k = tile % g.tiles_m * kTileM + row, c0 = tile / g.tiles_m * TN + col - g.skip;
+      const int k = tile % g.tiles_m * kTileM + row, c0 = tile / g.tiles_m * TN + col - g.skip;
       const int r0 = begin_of(t), count = count_of(t);
       const float* scale = g.scale + (int64_t)r0 * g.depth + k;
       float s = k < g.depth ? *scale : 0.0f;
@@ -288,25 +288,48 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        uint32_t x[2][32];  // one part is added while the next arrives
-        tmem_load32(lanes + sum.s * TN, x[0]);
+        uint32_t x[2][16];  // one part is added while the next arrives
+        tmem_load16(lanes + sum.s * TN, x[0]);
 #pragma unroll
-        for (int c = 0; c < kMine; c += 32) {
-          uint32_t(&y)[32] = x[c / 32 & 1];
+        for (int c = 0; c < kMine; c += 16) {
+          uint32_t(&y)[16] = x[c / 16 & 1];
           tmem_wait(y);
-          if (c + 32 < kMine) {
-            tmem_load32(lanes + sum.s * TN + c + 32, x[(c / 32 + 1) & 1]);
+          if (c + 16 < kMine) {
+            tmem_load16(lanes + sum.s * TN + c + 16, x[(c / 16 + 1) & 1]);
           } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (lane == 0) arrive_first(&sum_empty[sum.s]);
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 2)
+          for (int j = 0; j < 16; j += 2)
             acc[(c + j) / 2] = fma2(two(s, s), two(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), acc[(c + j) / 2]);
         }
         s = then;
       }
       if (fail) break;
+      // The products wait while a tile is written, so the usual ways out are straight: sums of parts, and whole
+      // f32 tiles (17000 cycles a tile by the general way below).
+      const bool inside = c0 >= 0 && c0 + kMine <= g.channels && k - lane + 32 <= g.depth;
+      if (g.splits > 1) {
+        float* p = part_of<TN>(g, t) + (int64_t)col * kTileM + row;
+#pragma unroll
+        for (int j = 0; j < kMine / 2; j++) {
+          const float2 f = apart(acc[j]);
+          p[2 * j * kTileM] = f.x;
+          p[(2 * j + 1) * kTileM] = f.y;
+        }
+        continue;
+      }
+      if (inside && g.out_dtype == DCF_F32 && !g.add) {
+        float* p = (float*)g.out + (int64_t)c0 * g.os + k;
+#pragma unroll
+        for (int j = 0; j < kMine / 2; j++, p += 2 * g.os) {
+          const float2 f = apart(acc[j]);
+          p[0] = f.x;
+          p[g.os] = f.y;
+        }
+        continue;
+      }
 #pragma unroll 1
       for (int c = 0; c < kMine; c += 16) {
         if (c0 + c < g.channels) {
@@ -316,13 +339,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
             const float2 f = apart(acc[j / 2]);
             v[j] = f.x, v[j + 1] = f.y;
           }
-          if (g.splits > 1) {
-            float* p = part_of<TN>(g, t) + (int64_t)(col + c) * kTileM + row;
-#pragma unroll
-            for (int j = 0; j < 16; j++) p[j * kTileM] = v[j];
-          } else {
-            write_block(g, v, c0 + c, k);
-          }
+          write_block(g, v, c0 + c, k);
         }
 #pragma unroll
         for (int j = 0; j < kMine / 2 - 8; j++) acc[j] = acc[j + 8];
@@ -357,19 +374,23 @@ __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_co
   }
 }
 
-// Whole numbers as values of T, rows of whole vectors; a thread makes sixteen.
+// Whole numbers as values of T, rows of whole vectors; a thread makes sixteen,
+// 2^wide threads a row.
 constexpr int kLevelThreads = 256;
 template <class T>
 __global__ void __launch_bounds__(kLevelThreads) levels_kernel(const int8_t* q, int64_t stride, int64_t rows, int64_t cols,
-                                                               T* to, int64_t to_stride) {
+                                                               T* to, int64_t to_stride, int wide) {
   pdl_begin();
-  const int64_t groups = (cols + 15) / 16, all = groups * rows;
-  for (int64_t i = (int64_t)blockIdx.x * kLevelThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kLevelThreads) {
-    const int64_t r = i / groups, c = i % groups * 16;
-    const uint4 v = row_bytes((const uint8_t*)q + r * stride, c, cols);
-    uint4* out = (uint4*)(to + r * to_stride + c);
-    out[0] = to_eight<T>(v.x, v.y);
-    out[1] = to_eight<T>(v.z, v.w);
+  const int64_t first = threadIdx.x & ((1 << wide) - 1), across = (int64_t)1 << wide;
+  for (int64_t r = (int64_t)blockIdx.x * (kLevelThreads >> wide) + (threadIdx.x >> wide); r < rows;
+       r += (int64_t)gridDim.x * (kLevelThreads >> wide)) {
+    const uint8_t* row = (const uint8_t*)q + r * stride;
+    for (int64_t c = first * 16; c < cols; c += across * 16) {
+      const uint4 v = row_bytes(row, c, cols);
+      uint4* out = (uint4*)(to + r * to_stride + c);
+      out[0] = to_eight<T>(v.x, v.y);
+      out[1] = to_eight<T>(v.z, v.w);
+    }
   }
 }
 
@@ -476,6 +497,7 @@ int checkpoint_desc_check(const dcf_checkpoint_desc* d) {
     if (k == 2 && rows[k] > 1 && rs < (__int128)cols[k])
       return bad("checkpoint grad: strides make rows of the result overlap");
   }
+  if ((d->channels / 128 + 2) * (d->depth / kTileM + 1) >= 1ull << 30) return bad("checkpoint grad: too many tiles");
   return DCF_OK;
 }
 
@@ -516,12 +538,15 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     const bool bf16 = d.grad_dtype == DCF_BF16;
     if (!encoder()) return DCF_EUNSUPPORTED;
     void* levels = (uint8_t*)ws + l.levels;
-    const int64_t all = l.level_stride / 16 * (int64_t)d.tokens, blocks = (all + kLevelThreads - 1) / kLevelThreads;
-    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30));
     const int64_t qs = stride_of(d.q_row_stride, d.depth), rows = (int64_t)d.tokens, cols = (int64_t)d.depth;
+    int wide = 0;
+    while (wide < 8 && (16 << wide) < cols) wide++;
+    const int64_t blocks = (rows + (kLevelThreads >> wide) - 1) / (kLevelThreads >> wide);
+    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30));
     rc = bf16 ? launch(levels_kernel<__nv_bfloat16>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__nv_bfloat16*)levels,
-                       l.level_stride)
-              : launch(levels_kernel<__half>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__half*)levels, l.level_stride);
+                       l.level_stride, wide)
+              : launch(levels_kernel<__half>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__half*)levels, l.level_stride,
+                       wide);
     if (rc) return rc;
     CUtensorMap map_q, map_g;
     tile_n = l.cut.tile_n;
@@ -532,7 +557,7 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     g.tiles_m = (int)l.cut.tiles_m;
     g.splits = l.cut.splits;
     g.split_runs = l.cut.runs;
-    g.total = l.cut.tiles * l.cut.splits;
+    g.total = (int)(l.cut.tiles * l.cut.splits);
     g.part = (float*)((uint8_t*)ws + l.part);
     g.idesc = (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) | ((uint32_t)(tile_n >> 3) << 17) |
               ((uint32_t)(kTileM >> 4) << 24);
