@@ -37,6 +37,7 @@ struct GradArgs {
   void* out;
   int out_dtype, add;
   int pairs;               // two neighbours of a row of a 16-bit result make an aligned word
+  int vectors;             // four neighbours of a row make an aligned vector
   int tokens, channels, depth;
   int skip;                // columns of the gradient's map before its first channel
   int64_t os;
@@ -355,22 +356,45 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
   }
 }
 
-// Joins the parts of each sum, always in the same order; a thread takes a k
-// and channel.  Also what writes the gradient of no tokens, whose sums have no parts.
-constexpr int kJoinThreads = 256;
+// Joins the parts of each sum, always in the same order; a thread takes four
+// neighbouring k of a channel, a block 512.  Also what writes the gradient of no tokens, whose
+// sums have no parts.
+constexpr int kJoinThreads = 128;
 __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_constant__ GradArgs g, int tile_n) {
   pdl_begin();
-  const int64_t across = ((int64_t)g.depth + kJoinThreads - 1) / kJoinThreads, all = across * g.channels;
+  const int across = (g.depth + 4 * kJoinThreads - 1) / (4 * kJoinThreads);
+  const int64_t all = (int64_t)across * g.channels;
   for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
-    const int64_t c = i / across, k = i % across * kJoinThreads + threadIdx.x, col = c + g.skip;
+    const int c = (int)(i / across), k = ((int)(i - (int64_t)c * across) * kJoinThreads + (int)threadIdx.x) * 4;
     if (k >= g.depth) continue;
-    float sum = 0;
+    float4 sum = make_float4(0, 0, 0, 0);
     if (g.splits) {
-      const int64_t tile = col / tile_n * g.tiles_m + k / kTileM, size = (int64_t)kTileM * tile_n;
-      const float* p = g.part + tile * g.splits * size + col % tile_n * kTileM + k % kTileM;
-      for (int s = 0; s < g.splits; s++) sum = __fadd_rn(sum, p[s * size]);
+      const int col = c + g.skip, tile = col / tile_n * g.tiles_m + k / kTileM;
+      const int64_t size = (int64_t)kTileM * tile_n;
+      const float* p = g.part + tile * g.splits * size + (int64_t)(col % tile_n) * kTileM + k % kTileM;
+#pragma unroll 4
+      for (int s = 0; s < g.splits; s++, p += size) {
+        const float4 v = *(const float4*)p;
+        sum = make_float4(__fadd_rn(sum.x, v.x), __fadd_rn(sum.y, v.y), __fadd_rn(sum.z, v.z), __fadd_rn(sum.w, v.w));
+      }
     }
-    put(g, c, k, sum);
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (g.vectors && k + 4 <= g.depth && !g.add) {
+      const int64_t at = (int64_t)c * g.os + k;
+      if (g.out_dtype == DCF_F32) {
+        *(float4*)((float*)g.out + at) = sum;
+      } else if (g.out_dtype == DCF_F16) {
+        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+        *(uint2*)((__half*)g.out + at) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+      } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+        *(uint2*)((__nv_bfloat16*)g.out + at) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (k + e < g.depth) put(g, c, k + e, v[e]);
+    }
   }
 }
 
@@ -520,6 +544,8 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
   g.depth = (int)d.depth;
   g.os = stride_of(d.out_row_stride, d.depth);
   g.pairs = (uintptr_t)out % 4 == 0 && (d.channels == 1 || g.os % 2 == 0);
+  const int four = 4 * (int)dtype_size(g.out_dtype);
+  g.vectors = (uintptr_t)out % four == 0 && (d.channels == 1 || g.os % 4 == 0);
   g.st = st;
   int tile_n = 0;
   if (d.tokens) {
@@ -564,7 +590,7 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     rc = tile_n == 256 ? run<256>(map_q, map_g, g, s) : run<128>(map_q, map_g, g, s);
     if (rc || g.splits == 1) return rc;
   }
-  const int64_t joins = ((int64_t)d.depth + kJoinThreads - 1) / kJoinThreads * (int64_t)d.channels;
+  const int64_t joins = ((int64_t)d.depth + 4 * kJoinThreads - 1) / (4 * kJoinThreads) * (int64_t)d.channels;
   return launch(grad_join_kernel, dim3((unsigned)(joins < (1 << 30) ? joins : 1 << 30)), kJoinThreads, 0, 1, s, g,
                 tile_n ? tile_n : 1);
 }

@@ -414,24 +414,33 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
   }
 }
 
-// Joins the parts of each sum; a thread takes a token and channel.  Also what
-// writes the result of a depth of 0, whose sums have no parts.
-constexpr int kJoinThreads = 256;
+// Joins the parts of each sum; a thread takes four neighbouring channels of a
+// token, a block 512.  Also what writes the result of a depth of 0, whose sums have no parts.
+constexpr int kJoinThreads = 128;
 __global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_constant__ GemmArgs g, int tile_n) {
   pdl_begin();
-  const int64_t across = ((int64_t)g.to.channels + kJoinThreads - 1) / kJoinThreads, all = across * g.to.tokens;
+  const int across = (g.to.channels + 4 * kJoinThreads - 1) / (4 * kJoinThreads);
+  const int64_t all = (int64_t)across * g.to.tokens;
+  const bool scaled = g.to.b_scale != nullptr;
   for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
-    const int64_t t = i / across, c = i % across * kJoinThreads + threadIdx.x;
+    const int t = (int)(i / across), c = ((int)(i - (int64_t)t * across) * kJoinThreads + (int)threadIdx.x) * 4;
     if (c >= g.to.channels) continue;
-    int sum = 0;
+    int4 sum = make_int4(0, 0, 0, 0);
     if (g.splits) {
-      const int64_t tile = t / tile_n * g.tiles_m + c / kTileM, size = (int64_t)kTileM * tile_n;
-      const int* p = g.part + tile * g.splits * size + t % tile_n * kTileM + c % kTileM;
-      for (int s = 0; s < g.splits; s++) sum += p[s * size];
+      const int64_t size = (int64_t)kTileM * tile_n, tile = (int64_t)(t / tile_n) * g.tiles_m + c / kTileM;
+      const int* p = g.part + tile * g.splits * size + (int64_t)(t % tile_n) * kTileM + c % kTileM;
+#pragma unroll 4
+      for (int s = 0; s < g.splits; s++, p += size) {
+        const int4 v = *(const int4*)p;
+        sum = make_int4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+      }
     }
-    const bool scaled = g.to.b_scale != nullptr;
-    put(g.to, t, c, sum, scaled ? g.to.a_scale[t] : 0.0f, scaled ? g.to.b_scale[c] : 0.0f,
-        g.to.bias ? g.to.bias[c] : -0.0f);
+    const int v[4] = {sum.x, sum.y, sum.z, sum.w};
+    const float a = scaled ? g.to.a_scale[t] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (c + e < g.to.channels)
+        put(g.to, t, c + e, v[e], a, scaled ? g.to.b_scale[c + e] : 0.0f, g.to.bias ? g.to.bias[c + e] : -0.0f);
   }
 }
 
@@ -846,7 +855,7 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     }
     if (rc || cut.splits == 1) return rc;
   }
-  const int64_t joins = ((int64_t)d.channels + kJoinThreads - 1) / kJoinThreads * (int64_t)d.tokens;
+  const int64_t joins = ((int64_t)d.channels + 4 * kJoinThreads - 1) / (4 * kJoinThreads) * (int64_t)d.tokens;
   return launch(int8_join_kernel, dim3((unsigned)(joins < (1 << 30) ? joins : 1 << 30)), kJoinThreads, 0, 1, s, g,
                 cut.tile_n);
 }
