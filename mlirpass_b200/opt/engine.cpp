@@ -808,6 +808,8 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       if (q->lhs && !q->lhs->splat) ins.push_back(q->lhs.get());
       if (q->rhs && !q->rhs->splat) ins.push_back(q->rhs.get());
       if (q->cond && !q->cond->splat) ins.push_back(q->cond.get());
+      for (const DenseP& o : q->more)
+        if (o) ins.push_back(o.get());
     }
     to_device_all(ins);
   }
@@ -854,7 +856,7 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
     cs[i] = q.cond ? operand(*q.cond, cpos[i]) : nullptr;
     if (q.kind != FoldRequest::SPLAT_SCAN)
       outs[i] = std::make_shared<DeviceBuf>(dev_, q.n * dcf_dtype_size((dcf_dtype)q.out_dtype));
-    if (q.op2) outs2[i] = std::make_shared<DeviceBuf>(dev_, q.n * dcf_dtype_size((dcf_dtype)q.out2_dtype));
+    if (q.op2) outs2[i] = std::make_shared<DeviceBuf>(dev_, q.second() * dcf_dtype_size((dcf_dtype)q.out2_dtype));
   }
   // Many small folds of one kind (one per isolated function, say) go out as
   // one launch per group through the batched kernel.
@@ -906,6 +908,9 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
     if (q.kind == FoldRequest::BIAS_GRAD)
       check(dcf_position_bias_grad_workspace(&q.bias, &work_bytes[i]), "position bias gradient fold");
     if (q.kind == FoldRequest::ORTH) check(dcf_orthogonalize_workspace(&q.orth, &work_bytes[i]), "orthogonalize fold");
+    if (q.kind == FoldRequest::INT8_MATMUL) check(dcf_int8_matmul_workspace(&q.int8, &work_bytes[i]), "int8 matmul fold");
+    if (q.kind == FoldRequest::CHECKPOINT_GRAD)
+      check(dcf_checkpoint_grad_workspace(&q.checkpoint, &work_bytes[i]), "checkpoint gradient fold");
   }
   std::unique_ptr<DeviceBuf> work;
   if (const size_t most = *std::max_element(work_bytes.begin(), work_bytes.end()))
@@ -916,6 +921,11 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
     FoldRequest& q = *reqs[i];
     const void* l = ls[i];
     const void* r = rs[i];
+    auto further = [&](size_t k) -> const void* {
+      if (k >= q.more.size() || !q.more[k]) return nullptr;
+      to_device(*q.more[k]);
+      return q.more[k]->dev->ptr;
+    };
     set_device();
     const size_t oes = dcf_dtype_size((dcf_dtype)q.out_dtype);
     switch (q.kind) {
@@ -958,6 +968,27 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
         check(dcf_orthogonalize_async(&q.orth, l, outs[i]->ptr, ws, work_bytes[i], st + i, s_), "orthogonalize fold");
         check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
         break;
+      case FoldRequest::QUANTIZE:
+        check(dcf_quantize_async(&q.quant, l, (int8_t*)outs[i]->ptr, (float*)outs2[i]->ptr, s_), "quantize fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        check(dcf_splat_check_async(outs2[i]->ptr, 4, q.n2, st + R + i, s_), "splat scan");
+        break;
+      case FoldRequest::DEQUANTIZE:
+        check(dcf_dequantize_async(&q.quant, (const int8_t*)l, (const float*)r, outs[i]->ptr, s_), "dequantize fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
+      case FoldRequest::INT8_MATMUL:
+        check(dcf_int8_matmul_async(&q.int8, l, (const float*)further(0), (const int8_t*)r, (const float*)further(1),
+                                    (const float*)further(2), outs[i]->ptr, ws, work_bytes[i], st + i, s_),
+              "int8 matmul fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
+      case FoldRequest::CHECKPOINT_GRAD:
+        check(dcf_checkpoint_grad_async(&q.checkpoint, l, (const int8_t*)r, (const float*)further(0), outs[i]->ptr, ws,
+                                        work_bytes[i], st + i, s_),
+              "checkpoint gradient fold");
+        check(dcf_splat_check_async(outs[i]->ptr, oes, q.n, st + i, s_), "splat scan");
+        break;
       case FoldRequest::SELECT:
         check(dcf_select_async(oes, cs[i], q.cond->splat, l, q.lhs->splat, r, q.rhs->splat, q.n, outs[i]->ptr, st + i,
                                s_),
@@ -981,7 +1012,7 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       sizes[i].es = dcf_dtype_size((dcf_dtype)q.out_dtype);
       if (q.op2) {
         hb[R + i] = outs2[i];
-        sizes[R + i].n = q.n;
+        sizes[R + i].n = q.second();
         sizes[R + i].es = dcf_dtype_size((dcf_dtype)q.out2_dtype);
       }
     }
@@ -1016,7 +1047,7 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
   // A folded result: one element if the kernel saw all values equal (as
   // MLIR stores a splat), else the device buffer.
   auto result = [&](const FoldRequest& q, const dcf_status& h, const std::shared_ptr<DeviceBuf>& buf, int dtype,
-                    const TypeP& ty, uint64_t first_bits) {
+                    const TypeP& ty, uint64_t first_bits, uint64_t n) {
     auto d = std::make_shared<DenseValue>();
     d->ty = ty;
     d->elements = q.out_elements;
@@ -1028,7 +1059,7 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
       d->host.resize(d->es);
       memcpy(d->host.data(), &first_bits, d->es);
     } else {
-      d->n = q.n;
+      d->n = n;
       d->dev = buf;
       // The kernel's splat test already said the values differ.
       if (q.kind != FoldRequest::PERMUTE) d->all_equal = 0;
@@ -1047,13 +1078,13 @@ void Engine::execute(const std::vector<FoldRequest*>& reqs) {
     if (q.op2 && hst[R + i].first_fail < q.first_fail) q.first_fail = hst[R + i].first_fail;
     q.folded = q.first_fail == ~0ull;
     if (!q.folded) continue;
-    q.out = result(q, hst[i], outs[i], q.out_dtype, q.out_ty, first[i]);
+    q.out = result(q, hst[i], outs[i], q.out_dtype, q.out_ty, first[i], q.n);
     if (q.out->dev) {
       q.out->hash = rh[i];
       q.out->hashed = true;
     }
     if (q.op2) {
-      q.out2 = result(q, hst[R + i], outs2[i], q.out2_dtype, q.out2_ty, first[R + i]);
+      q.out2 = result(q, hst[R + i], outs2[i], q.out2_dtype, q.out2_ty, first[R + i], q.second());
       if (q.out2->dev) {
         q.out2->hash = rh[R + i];
         q.out2->hashed = true;

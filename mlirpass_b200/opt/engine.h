@@ -44,7 +44,8 @@ class DeviceBuf {
 // One element-level fold.  The greedy driver fills the inputs; the engine
 // fills the outcome.
 struct FoldRequest {
-  enum Kind { BINARY, CONVERT, RECIPROCAL, PERMUTE, SPLAT_SCAN, SELECT, BIAS, BIAS_GRAD, ORTH } kind = BINARY;
+  enum Kind { BINARY, CONVERT, RECIPROCAL, PERMUTE, SPLAT_SCAN, SELECT, BIAS, BIAS_GRAD, ORTH,
+              QUANTIZE, DEQUANTIZE, INT8_MATMUL, CHECKPOINT_GRAD } kind = BINARY;
   int op = 0, dtype = 0, out_dtype = 0;
   uint32_t flags = 0;
   DenseP lhs, rhs;
@@ -53,14 +54,21 @@ struct FoldRequest {
   std::vector<int64_t> shape, perms;    // PERMUTE
   dcf_bias_desc bias{};                 // BIAS, BIAS_GRAD: lhs is the table / the bias's gradient
   dcf_orth_desc orth{};                 // ORTH
+  dcf_quant_desc quant{};               // QUANTIZE, DEQUANTIZE (lhs whole numbers, rhs scales)
+  dcf_int8_desc int8{};                 // INT8_MATMUL: lhs a, rhs b, more: a_scale, b_scale, bias (null where not given)
+  dcf_checkpoint_desc checkpoint{};     // CHECKPOINT_GRAD: lhs the gradient, rhs whole numbers, more: scales
+  std::vector<DenseP> more;             // further operands, none of them a splat
   TypeP out_ty;                         // attribute type of the result
   bool out_elements = true;
   // A second result over the same operands (the *_extended ops): a second
-  // binary kernel `op2` writing out2_dtype elements of type out2_ty.
+  // binary kernel `op2` writing out2_dtype elements of type out2_ty.  QUANTIZE
+  // writes both results by itself (op2 = 1), n2 scales.
   int op2 = 0, out2_dtype = 0;
+  uint64_t n2 = 0;                      // elements of the second result where they are not n
   uint32_t flags2 = 0;
   TypeP out2_ty;
   DenseP out2;
+  uint64_t second() const { return n2 ? n2 : n; }
   // outcome
   bool folded = false;
   uint64_t first_fail = ~0ull;

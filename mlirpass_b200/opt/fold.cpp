@@ -883,6 +883,14 @@ Plan layerwise_pattern(Module&, Op* op, Engine& eng) {
 //       bidirectional, causal : bool, first_query, max_distance : i64
 //   "dcf.orthogonalize"(%w)          tensor<[N x]RxCxT> -> tensor<[N x]RxCxT2>
 //       steps : i64, eps : f64, coef : array<f64: a, b, c> (or 3 per step)
+// and its operators on 8-bit integers where all of their operands are:
+//   "dcf.quantize"(%x)               tensor<RxCxT> -> (tensor<RxCxi8>, tensor<Rxf32>), or with
+//       columns : bool               -> (tensor<RxCxi8>, tensor<NxCxf32>), N = ceil(R / 128)
+//   "dcf.dequantize"(%q, %scale)     the other way round (columns : bool)
+//   "dcf.int8_matmul"(%a, %b)                        tensor<TxKxi8>, tensor<CxKxi8> -> tensor<TxCxi32>
+//   "dcf.int8_matmul"(%a, %as, %b, %bs[, %bias])     scales tensor<Txf32>, tensor<Cxf32> -> tensor<TxCxT2>
+//   "dcf.int8_matmul"(%a, %b, %bs[, %bias])          tensor<TxKxT>, quantised by rows first
+//   "dcf.checkpoint_grad"(%g, %q, %scale)            tensor<TxCxT>, tensor<TxKxi8>, tensor<NxKxf32> -> tensor<CxKxT2>
 // An op whose types or properties the operator does not take, or that says more than
 // these properties (attributes of other dialects aside), stays as it is, and so does
 // one whose operand or result is over 16 GiB: a module could not hold it as a constant.
@@ -1080,7 +1088,106 @@ bool fits32(std::initializer_list<int64_t> dims) {
   return true;
 }
 
+// The operators on 8-bit integers.
+Plan integer_pattern(Op* op, Engine& eng) {
+  std::vector<DenseP> in;
+  for (Value* v : op->operands) {
+    DenseP k = constant_of(v);
+    if (!k || k->poison || !k->elements || !k->ty->static_shape() || !fits_module(k->ty)) return Plan::failed();
+    for (int64_t d : k->ty->shape)
+      if (d > INT32_MAX - 65535) return Plan::failed();
+    in.push_back(k);
+  }
+  for (Value* r : op->results) {
+    const TypeP t = r->ty;
+    if (!t->static_shape() || t->kind != "tensor" || !t->dtype || !fits_module(t)) return Plan::failed();
+  }
+  if (in.empty() || op->results.empty()) return Plan::failed();
+  const TypeP rty = op->results[0]->ty;
+  const std::vector<int64_t>& out = rty->shape;
+  auto is = [](const TypeP& t, int dtype, const std::vector<int64_t>& shape) { return t->dtype == dtype && t->shape == shape; };
+  auto real = [](int dtype) { return dtype == DCF_F16 || dtype == DCF_BF16 || dtype == DCF_F32; };
+  auto q = std::make_unique<FoldRequest>();
+  const std::vector<int64_t>& a = in[0]->ty->shape;
+  if (a.size() != 2 || out.size() != 2) return Plan::failed();
+  size_t bytes;
+  bool ok = true;
+  if (op->name == "dcf.quantize" || op->name == "dcf.dequantize") {
+    const bool back = op->name == "dcf.dequantize";
+    ok = says_only(op, {"columns"});
+    const bool columns = bool_prop(op, "columns", false, &ok);
+    if (!ok || in.size() != (back ? 2u : 1u) || op->results.size() != (back ? 1u : 2u)) return Plan::failed();
+    const std::vector<int64_t> scales = columns ? std::vector<int64_t>{(a[0] + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN, a[1]}
+                                                : std::vector<int64_t>{a[0]};
+    const TypeP values = back ? rty : in[0]->ty, levels = back ? in[0]->ty : rty, scale = back ? in[1]->ty : op->results[1]->ty;
+    if (!real(values->dtype) || out != a || !is(levels, DCF_I8, a) || !is(scale, DCF_F32, scales)) return Plan::failed();
+    q->quant.dtype = (uint32_t)values->dtype;
+    q->quant.along = columns ? DCF_QUANT_COLUMNS : DCF_QUANT_ROWS;
+    q->quant.rows = (uint64_t)a[0];
+    q->quant.cols = (uint64_t)a[1];
+    q->kind = back ? FoldRequest::DEQUANTIZE : FoldRequest::QUANTIZE;
+    if (back) {
+      q->rhs = whole_constant(in[1], eng);
+    } else {
+      q->op2 = 1;
+      q->out2_dtype = DCF_F32;
+      q->out2_ty = scale;
+      q->n2 = (uint64_t)scale->count();
+    }
+  } else if (op->name == "dcf.int8_matmul") {
+    if (!says_only(op, {}) || op->results.size() != 1) return Plan::failed();
+    const bool sums = rty->dtype == DCF_I32, ints = in[0]->dtype == DCF_I8;
+    const size_t at = ints && !sums ? 2 : 1;  // of b
+    const size_t least = sums ? 2 : at + 2;
+    if (in.size() < least || in.size() > (sums ? least : least + 1)) return Plan::failed();
+    const std::vector<int64_t>& b = in[at]->ty->shape;
+    if (in[at]->dtype != DCF_I8 || b.size() != 2 || b[1] != a[1] || out[0] != a[0] || out[1] != b[0]) return Plan::failed();
+    if (at == 2 && !is(in[1]->ty, DCF_F32, {a[0]})) return Plan::failed();
+    for (size_t k = at + 1; k < in.size(); k++)
+      if (!is(in[k]->ty, DCF_F32, {b[0]})) return Plan::failed();
+    dcf_int8_desc& d = q->int8;
+    d.a_dtype = (uint32_t)in[0]->dtype;
+    d.out_dtype = (uint32_t)rty->dtype;
+    d.tokens = (uint64_t)a[0];
+    d.channels = (uint64_t)b[0];
+    d.depth = (uint64_t)a[1];
+    if (dcf_int8_matmul_workspace(&d, &bytes) != 0) return Plan::failed();
+    q->kind = FoldRequest::INT8_MATMUL;
+    q->rhs = whole_constant(in[at], eng);
+    q->more = {at == 2 ? whole_constant(in[1], eng) : nullptr, sums ? nullptr : whole_constant(in[at + 1], eng),
+               in.size() > at + 2 ? whole_constant(in[at + 2], eng) : nullptr};
+  } else if (op->name == "dcf.checkpoint_grad") {
+    if (!says_only(op, {}) || op->results.size() != 1 || in.size() != 3) return Plan::failed();
+    const std::vector<int64_t>& b = in[1]->ty->shape;
+    if (in[1]->dtype != DCF_I8 || b.size() != 2 || b[0] != a[0] || out[0] != a[1] || out[1] != b[1] ||
+        !is(in[2]->ty, DCF_F32, {(a[0] + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN, b[1]}))
+      return Plan::failed();
+    dcf_checkpoint_desc& d = q->checkpoint;
+    d.grad_dtype = (uint32_t)in[0]->dtype;
+    d.out_dtype = (uint32_t)rty->dtype;
+    d.tokens = (uint64_t)a[0];
+    d.channels = (uint64_t)a[1];
+    d.depth = (uint64_t)b[1];
+    if (dcf_checkpoint_grad_workspace(&d, &bytes) != 0) return Plan::failed();
+    q->kind = FoldRequest::CHECKPOINT_GRAD;
+    q->rhs = whole_constant(in[1], eng);
+    q->more = {whole_constant(in[2], eng)};
+  } else {
+    return Plan::failed();
+  }
+  q->dtype = in[0]->dtype;
+  q->out_dtype = rty->dtype;
+  q->lhs = whole_constant(in[0], eng);
+  q->n = (uint64_t)rty->count();
+  q->out_ty = rty;
+  q->out_elements = true;
+  return Plan::device(std::move(q));
+}
+
 Plan learned_pattern(Op* op, Engine& eng) {
+  if (op->dialect() == "dcf" && (op->name == "dcf.quantize" || op->name == "dcf.dequantize" ||
+                                 op->name == "dcf.int8_matmul" || op->name == "dcf.checkpoint_grad"))
+    return integer_pattern(op, eng);
   if (op->dialect() != "dcf" || op->results.size() != 1 || op->operands.size() != 1) return Plan::failed();
   const TypeP rty = op->results[0]->ty;
   DenseP k = constant_of(op->operands[0]);
@@ -1443,7 +1550,7 @@ struct Greedy::Impl {
   // replace_folded for several results: each part is a value or an
   // attribute that is materialised as a constant; nothing changes unless
   // every attribute materialises.
-  bool replace_with_parts(Op* op, const std::vector<std::pair<Value*, DenseP>>& parts) {
+  bool replace_with_parts(Op* op, const std::vector<std::pair<Value*, DenseP>>& parts, const std::string& dialect) {
     if (parts.size() != op->results.size()) return false;
     std::vector<Op*> made;
     std::vector<Value*> vals;
@@ -1452,7 +1559,7 @@ struct Greedy::Impl {
         vals.push_back(parts[i].first);
         continue;
       }
-      Op* c = materialize(m, op->dialect(), parts[i].second, op->results[i]->ty);
+      Op* c = materialize(m, dialect, parts[i].second, op->results[i]->ty);
       if (!c) return false;
       c->loc = op->loc;
       made.push_back(c);
@@ -1513,12 +1620,16 @@ struct Greedy::Impl {
         Op* op = pend;
         pend = nullptr;
         std::unique_ptr<FoldRequest> req = std::move(pend_req);
+        if (pend_pattern && req->op2) {
+          if (req->folded && replace_with_parts(op, {{nullptr, req->out}, {nullptr, req->out2}}, "arith")) changed = true;
+          continue;
+        }
         if (pend_pattern) {
           if (req->folded && replace_with_attr(op, req->out, cfg.learned ? "arith" : "tosa")) changed = true;
           continue;
         }
         if (req->folded && req->op2) {
-          if (replace_with_parts(op, {{nullptr, req->out}, {nullptr, req->out2}})) changed = true;
+          if (replace_with_parts(op, {{nullptr, req->out}, {nullptr, req->out2}}, op->dialect())) changed = true;
           continue;
         }
         if (req->folded && replace_with_attr(op, req->out, op->dialect())) {
@@ -1562,7 +1673,7 @@ struct Greedy::Impl {
           changed = true;
           continue;
         }
-        if (p.k == Plan::MULTI && replace_with_parts(op, p.parts)) {
+        if (p.k == Plan::MULTI && replace_with_parts(op, p.parts, op->dialect())) {
           changed = true;
           continue;
         }

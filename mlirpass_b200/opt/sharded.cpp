@@ -235,6 +235,8 @@ void ShardedEngine::execute(const std::vector<FoldRequest*>& reqs) {
     }
     for (DenseP* o : {&q->lhs, &q->rhs, &q->cond})
       if (*o && !(*o)->parts.empty() && (*o)->hex.empty()) to_host(**o);
+    for (DenseP& o : q->more)
+      if (o && !o->parts.empty() && o->hex.empty()) to_host(*o);
     whole.push_back(q);
   }
   // Per GPU, one sub-request per split request over that GPU's range;
