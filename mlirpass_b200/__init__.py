@@ -642,11 +642,16 @@ def _room(t) -> int:
 _TORCH_TYPES: dict = {}
 
 
+def _load_torch_types() -> None:
+    import torch
+    _TORCH_TYPES.update(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32, f64=torch.float64, i32=torch.int32,
+                        i8=torch.int8)
+
+
 def _typed(t, what: str, dtype: str) -> None:
     """Refuse a tensor whose elements are not of the given type (another of the same size would be read as it)."""
     if not _TORCH_TYPES:
-        import torch
-        _TORCH_TYPES.update(f16=torch.float16, bf16=torch.bfloat16, f32=torch.float32, f64=torch.float64, i32=torch.int32, i8=torch.int8)
+        _load_torch_types()
     if t.dtype is not _TORCH_TYPES[dtype]:
         raise ValueError(f"{what}: {t.dtype}, {dtype} expected")
 
@@ -836,6 +841,27 @@ def _rows(rows: int, cols: int, stride: int) -> tuple:
     return (rows - 1) * stride + cols if rows and cols else 0, (rows, cols), (stride, 1)
 
 
+def _torch_type(dtype: str):
+    if not _TORCH_TYPES:
+        _load_torch_types()
+    return _TORCH_TYPES[dtype]
+
+
+def _at(t, what: str, dtype: str, rows: tuple) -> int:
+    """The pointer of a tensor in which a matrix of _rows lies; one with exactly its shape and strides needs no
+    further look."""
+    if t.dtype is _torch_type(dtype) and t.stride() == rows[2] and t.shape == rows[1]:
+        return t.data_ptr()
+    return _need_layout(t, what, rows[0], dtype, *rows[1:])
+
+
+def _floats(t, what: str, elements: int) -> int:
+    """The pointer of a dense f32 tensor of at least `elements`."""
+    if t.dtype is _torch_type("f32") and t.is_contiguous() and t.numel() >= elements:
+        return t.data_ptr()
+    return _need(t, what, elements, "f32")
+
+
 def _fits(limit: int, **sizes) -> None:
     for name, v in sizes.items():
         if not 0 <= v < limit:
@@ -843,7 +869,7 @@ def _fits(limit: int, **sizes) -> None:
 
 
 def _vector(t, what: str, elements: int):
-    return None if t is None else _need(t, what, elements, "f32")
+    return None if t is None else _floats(t, what, elements)
 
 
 class QuantPlan:
@@ -857,6 +883,7 @@ class QuantPlan:
         self.levels = _rows(desc.rows, desc.cols, desc.q_row_stride)
         self.scale_shape = (desc.rows,) if desc.along == 0 else (-(-desc.rows // QUANT_RUN), desc.cols)
         self.scales = math.prod(self.scale_shape)
+        self.quantize, self.dequantize = lib().dcf_quantize_async, lib().dcf_dequantize_async
 
 
 def quantize_plan(dtype: str, rows: int, cols: int, *, along: str = "rows", row_stride: int = 0,
@@ -870,10 +897,9 @@ def quantize_plan(dtype: str, rows: int, cols: int, *, along: str = "rows", row_
     """
     _fits(1 << 31, rows=rows, cols=cols)
     _fits(1 << 62, row_stride=row_stride, q_row_stride=q_row_stride)
-    plan = QuantPlan(QuantDesc(DTYPES[dtype], QUANT_ALONG[along], rows, cols, row_stride, q_row_stride), dtype)
     if dtype not in ("f16", "bf16", "f32"):
         raise ValueError(f"dtype {dtype}: f16, bf16 or f32 expected")
-    return plan
+    return QuantPlan(QuantDesc(DTYPES[dtype], QUANT_ALONG[along], rows, cols, row_stride, q_row_stride), dtype)
 
 
 def quantize(plan: QuantPlan, x) -> tuple:
@@ -908,18 +934,14 @@ def _host_array(x, what: str, n: int, dtype) -> np.ndarray:
 def quantize_async(plan: QuantPlan, x, q, scale, *, stream=None) -> None:
     """Launch a quantisation on device tensors: `x` and the int8 `q` lie as the
     plan's strides say, the f32 `scale` is dense, of the plan's scale_shape."""
-    _check(lib().dcf_quantize_async(
-        plan.ref, _need_layout(x, "x", plan.values[0], plan.dtype, *plan.values[1:]),
-        _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]), _need(scale, "scale", plan.scales, "f32"),
-        _own_stream(stream, q)))
+    _check(plan.quantize(plan.ref, _at(x, "x", plan.dtype, plan.values), _at(q, "q", "i8", plan.levels),
+                         _floats(scale, "scale", plan.scales), _own_stream(stream, q)))
 
 
 def dequantize_async(plan: QuantPlan, q, scale, out, *, stream=None) -> None:
     """Launch the reading back of what quantize_async wrote, into `out` as the plan's strides say."""
-    _check(lib().dcf_dequantize_async(
-        plan.ref, _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]),
-        _need(scale, "scale", plan.scales, "f32"),
-        _need_layout(out, "out", plan.values[0], plan.dtype, *plan.values[1:]), _own_stream(stream, out)))
+    _check(plan.dequantize(plan.ref, _at(q, "q", "i8", plan.levels), _floats(scale, "scale", plan.scales),
+                           _at(out, "out", plan.dtype, plan.values), _own_stream(stream, out)))
 
 
 class Int8Plan:
@@ -935,6 +957,7 @@ class Int8Plan:
         ws = ctypes.c_size_t(0)
         _check(lib().dcf_int8_matmul_workspace(self.ref, ctypes.byref(ws)))
         self.workspace = ws.value
+        self.tokens, self.channels, self.call = desc.tokens, desc.channels, lib().dcf_int8_matmul_async
 
 
 def int8_matmul_plan(tokens: int, channels: int, depth: int, *, a_dtype: str = "i8", out_dtype: str = "bf16",
@@ -979,12 +1002,11 @@ def int8_matmul_async(plan: Int8Plan, a, b, out, workspace, status, *, a_scale=N
     `out` lie as the plan's strides say; `a_scale` [tokens] (of i8 tokens),
     `b_scale` and `bias` [channels] are dense f32.  `status` (16 bytes, reset
     first) takes a kernel's error report."""
-    d = plan.desc
-    _check(lib().dcf_int8_matmul_async(
-        plan.ref, _need_layout(a, "a", plan.a[0], plan.a_dtype, *plan.a[1:]), _vector(a_scale, "a_scale", d.tokens),
-        _need_layout(b, "b", plan.b[0], "i8", *plan.b[1:]), _vector(b_scale, "b_scale", d.channels),
-        _vector(bias, "bias", d.channels), _need_layout(out, "out", plan.out[0], plan.out_dtype, *plan.out[1:]),
-        workspace.data_ptr(), _bytes(workspace), _need(status, "status", 2, None), _own_stream(stream, out)))
+    _check(plan.call(
+        plan.ref, _at(a, "a", plan.a_dtype, plan.a), _vector(a_scale, "a_scale", plan.tokens),
+        _at(b, "b", "i8", plan.b), _vector(b_scale, "b_scale", plan.channels), _vector(bias, "bias", plan.channels),
+        _at(out, "out", plan.out_dtype, plan.out), workspace.data_ptr(), _bytes(workspace),
+        _need(status, "status", 2, None), _own_stream(stream, out)))
 
 
 class CheckpointPlan:
@@ -1002,6 +1024,7 @@ class CheckpointPlan:
         ws = ctypes.c_size_t(0)
         _check(lib().dcf_checkpoint_grad_workspace(self.ref, ctypes.byref(ws)))
         self.workspace = ws.value
+        self.call = lib().dcf_checkpoint_grad_async
 
 
 def checkpoint_grad_plan(dtype: str, tokens: int, channels: int, depth: int, *, out_dtype: str = "f32",
@@ -1044,8 +1067,7 @@ def checkpoint_grad_async(plan: CheckpointPlan, grad, q, scale, out, workspace, 
     """Launch a weight gradient on device tensors: `grad`, the int8 `q` and `out`
     lie as the plan's strides say, the f32 `scale` is dense, of the plan's
     scale_shape.  `status` (16 bytes, reset first) takes a kernel's error report."""
-    _check(lib().dcf_checkpoint_grad_async(
-        plan.ref, _need_layout(grad, "grad", plan.grad[0], plan.dtype, *plan.grad[1:]),
-        _need_layout(q, "q", plan.levels[0], "i8", *plan.levels[1:]), _need(scale, "scale", plan.scales, "f32"),
-        _need_layout(out, "out", plan.out[0], plan.out_dtype, *plan.out[1:]), workspace.data_ptr(), _bytes(workspace),
-        _need(status, "status", 2, None), _own_stream(stream, out)))
+    _check(plan.call(
+        plan.ref, _at(grad, "grad", plan.dtype, plan.grad), _at(q, "q", "i8", plan.levels),
+        _floats(scale, "scale", plan.scales), _at(out, "out", plan.out_dtype, plan.out), workspace.data_ptr(),
+        _bytes(workspace), _need(status, "status", 2, None), _own_stream(stream, out)))

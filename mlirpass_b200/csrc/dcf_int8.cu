@@ -59,6 +59,7 @@ struct GemmArgs {
   const int8_t* b;         // the weight, where threads read it
   int64_t b_stride;
   int depth;
+  int early;               // only the kernel that quantised the tokens ran since the weight may have changed
   dcf_status* st;
 };
 
@@ -242,13 +243,25 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     if (!READ) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_b) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)&map_a) : "memory");
   }
-  pdl_begin();
+  // What reads the weight alone need not wait for the tokens.
+  if (!g.early || (warp != 0 && warp < 4 + OW)) pdl_begin();
 
   bool fail = false;
   if (warp == 0) {
     if (lane == 0) {
       Ring<S> at;
       int used = 0;  // stages filled, S at most
+      int ahead = 0; // stages whose weight is on its way
+      if (g.early) {
+        if (!READ && first < g.total) {
+          const int row = (int)(first / g.splits % g.tiles_m) * kTileM + (int)rank * kSide;
+          for (const int end = min(S, count_of(first)); ahead < end; ahead++) {
+            if (!rank) mbar_expect_tx(&full[ahead], 2 * kStage<TN>);
+            pair_load_2d(stage0 + ahead * kStage<TN>, &map_b, (begin_of(first) + ahead) * kBK, row, full0 + ahead * 8);
+          }
+        }
+        pdl_begin();
+      }
       for (int64_t t = first; t < g.total && !fail; t += step) {
         const int64_t tile = t / g.splits;
         const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
@@ -261,8 +274,12 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
           }
           const uint32_t to = stage0 + at.s * kStage<TN>;
           const uint32_t bar = full0 + at.s * 8;
-          if (!rank) mbar_expect_tx(&full[at.s], 2 * (READ ? TN / 2 * kBK : kStage<TN>));
-          if (!READ) pair_load_2d(to, &map_b, k, row, bar);
+          if (ahead > 0) {
+            ahead--;
+          } else {
+            if (!rank) mbar_expect_tx(&full[at.s], 2 * (READ ? TN / 2 * kBK : kStage<TN>));
+            if (!READ) pair_load_2d(to, &map_b, k, row, bar);
+          }
           pair_load_2d(to + kSide * kBK, &map_a, k, col, bar);
           used += used < S;
         }
@@ -843,6 +860,7 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     g.b = b;
     g.b_stride = bs;
     g.depth = (int)d.depth;
+    g.early = ours && !l.copy_b;
     if (!encoder()) return DCF_EUNSUPPORTED;
     CUtensorMap ma, mb = {};
     if ((!read && !encode_rows(&mb, b, (int64_t)d.channels, (int64_t)d.depth, bs, kSide)) ||
