@@ -1402,22 +1402,31 @@ int dcf_orthogonalize_async(const dcf_orth_desc* desc, const void* in, void* out
 
 namespace {
 
-// Bytes from the first element of rows to behind the last one, 0 without any.
-size_t rows_bytes(uint64_t rows, uint64_t cols, int64_t stride, size_t es) {
-  if (!rows || !cols) return 0;
-  return (size_t)((rows - 1) * (uint64_t)(stride ? stride : (int64_t)cols) + cols) * es;
-}
-
+// Memory as rows of `width` bytes, `stride` apart (one row: plain bytes).
 struct Span {
   const void* p;
-  size_t bytes;
+  size_t width;
+  uint64_t rows = 1;
+  size_t stride = 0;
+  size_t bytes() const { return width && rows ? (rows - 1) * stride + width : 0; }
 };
+
+Span rows_at(const void* p, uint64_t rows, uint64_t cols, int64_t stride, size_t es) {
+  return {p, cols * es, rows, (size_t)(stride ? stride : (int64_t)cols) * es};
+}
+
+// Whether two spans share a byte.  Rows the same stride apart may lie between each other's (two
+// parts of one wide tensor); of other strides their whole reach counts.
+bool meet(const Span& a, const Span& b) {
+  const char *x = (const char*)a.p, *y = (const char*)b.p;
+  if (!a.bytes() || !b.bytes() || x >= y + b.bytes() || y >= x + a.bytes()) return false;
+  if (a.rows == 1 || b.rows == 1 || a.stride != b.stride || a.width > a.stride || b.width > b.stride) return true;
+  const size_t behind = y >= x ? (size_t)(y - x) % a.stride : (a.stride - (size_t)(x - y) % a.stride) % a.stride;
+  return behind < a.width || behind + b.width > a.stride;
+}
 
 // No result may share memory with an operand or another result.
 int apart(std::initializer_list<Span> results, std::initializer_list<Span> operands) {
-  auto meet = [](const Span& a, const Span& b) {
-    return a.bytes && b.bytes && (const char*)a.p < (const char*)b.p + b.bytes && (const char*)b.p < (const char*)a.p + a.bytes;
-  };
   for (const Span* r = results.begin(); r != results.end(); r++) {
     for (const Span& o : operands)
       if (meet(*r, o)) return set_err(DCF_EINVAL, "a result overlaps an operand");
@@ -1453,8 +1462,8 @@ int dcf_quantize_async(const dcf_quant_desc* desc, const void* in, int8_t* q, fl
   if (!scales) return DCF_OK;
   if (!scale || (d.cols && (!in || !q))) return set_err(DCF_EINVAL, "null pointer");
   const size_t es = dtype_size((int)d.dtype);
-  if ((rc = apart({{q, rows_bytes(d.rows, d.cols, d.q_row_stride, 1)}, {scale, scales * 4}},
-                  {{in, rows_bytes(d.rows, d.cols, d.row_stride, es)}})))
+  if ((rc = apart({rows_at(q, d.rows, d.cols, d.q_row_stride, 1), {scale, scales * 4}},
+                  {rows_at(in, d.rows, d.cols, d.row_stride, es)})))
     return rc;
   OnDevice on;
   if ((rc = on.enter({{scale, 4}, {q, 1}, {in, es}}))) return rc;
@@ -1469,8 +1478,8 @@ int dcf_dequantize_async(const dcf_quant_desc* desc, const int8_t* q, const floa
   if (!d.rows || !d.cols) return DCF_OK;
   if (!q || !scale || !out) return set_err(DCF_EINVAL, "null pointer");
   const size_t es = dtype_size((int)d.dtype);
-  if ((rc = apart({{out, rows_bytes(d.rows, d.cols, d.row_stride, es)}},
-                  {{q, rows_bytes(d.rows, d.cols, d.q_row_stride, 1)}, {scale, scale_count(d) * 4}})))
+  if ((rc = apart({rows_at(out, d.rows, d.cols, d.row_stride, es)},
+                  {rows_at(q, d.rows, d.cols, d.q_row_stride, 1), {scale, scale_count(d) * 4}})))
     return rc;
   OnDevice on;
   if ((rc = on.enter({{out, es}, {q, 1}, {scale, 4}}))) return rc;
@@ -1572,9 +1581,9 @@ int dcf_int8_matmul_async(const dcf_int8_desc* desc, const void* a, const float*
   const size_t ws = int8_workspace(d), es = dtype_size((int)d.a_dtype), oes = dtype_size((int)d.out_dtype);
   if (!status || (ws && !workspace)) return set_err(DCF_EINVAL, "null pointer");
   if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
-  if ((rc = apart({{out, rows_bytes(d.tokens, d.channels, d.out_row_stride, oes)}, {workspace, ws}, {status, sizeof *status}},
-                  {{a, rows_bytes(d.tokens, d.depth, d.a_row_stride, es)},
-                   {b, rows_bytes(d.channels, d.depth, d.b_row_stride, 1)},
+  if ((rc = apart({rows_at(out, d.tokens, d.channels, d.out_row_stride, oes), {workspace, ws}, {status, sizeof *status}},
+                  {rows_at(a, d.tokens, d.depth, d.a_row_stride, es),
+                   rows_at(b, d.channels, d.depth, d.b_row_stride, 1),
                    {a_scale, a_scale ? d.tokens * 4 : 0},
                    {b_scale, b_scale ? d.channels * 4 : 0},
                    {bias, bias ? d.channels * 4 : 0}})))
@@ -1647,9 +1656,9 @@ int dcf_checkpoint_grad_async(const dcf_checkpoint_desc* desc, const void* grad,
     return set_err(DCF_EINVAL, "null pointer");
   if (workspace_bytes < ws) return set_err(DCF_EINVAL, "workspace of %zu bytes, %zu needed", workspace_bytes, ws);
   const uint64_t scales = (d.tokens + DCF_QUANT_RUN - 1) / DCF_QUANT_RUN * d.depth;
-  if ((rc = apart({{out, rows_bytes(d.channels, d.depth, d.out_row_stride, oes)}, {workspace, ws}, {status, sizeof *status}},
-                  {{grad, rows_bytes(d.tokens, d.channels, d.grad_row_stride, es)},
-                   {q, rows_bytes(d.tokens, d.depth, d.q_row_stride, 1)},
+  if ((rc = apart({rows_at(out, d.channels, d.depth, d.out_row_stride, oes), {workspace, ws}, {status, sizeof *status}},
+                  {rows_at(grad, d.tokens, d.channels, d.grad_row_stride, es),
+                   rows_at(q, d.tokens, d.depth, d.q_row_stride, 1),
                    {scale, scales * 4}})))
     return rc;
   OnDevice on;

@@ -462,3 +462,184 @@ def test_layer_forward_checkpoint_backward_and_step(dcf):
     dcf.dequantize_async(cplan, q, s, values)
     half = wide(s).repeat(io.RUN, 0)[:tokens] / 2
     assert (np.abs(wide(values) - wide(x)) <= half * (1 + 2.0 ** -20) + np.abs(wide(values)) * 2.0 ** -8).all()
+
+
+# ------------------------------------- streams, graphs, large offsets, many rows
+
+
+def calls_of(dcf, seed, tokens=300, channels=200, depth=264):
+    """Every operator once, on buffers of its own: (inputs, outputs, a function that queues all of them)."""
+    import torch
+    x, w = randn((tokens, depth), "bf16", seed), randn((channels, depth), "bf16", seed + 1, 0.05)
+    cplan, wplan = dcf.quantize_plan("bf16", tokens, depth, along="columns"), dcf.quantize_plan("bf16", channels, depth)
+    mm, gp = dcf.int8_matmul_plan(tokens, channels, depth, a_dtype="bf16"), dcf.checkpoint_grad_plan("bf16", tokens, channels, depth)
+    status = new_status(dcf)
+    room = {n: torch.empty(s, dtype=t, device="cuda") for n, s, t in (
+        ("wq", (channels, depth), torch.int8), ("ws", (channels,), torch.float32), ("q", (tokens, depth), torch.int8),
+        ("s", cplan.scale_shape, torch.float32), ("y", (tokens, channels), torch.bfloat16), ("dw", (channels, depth), torch.float32),
+        ("back", (tokens, depth), torch.bfloat16), ("work", (max(mm.workspace, gp.workspace),), torch.uint8))}
+
+    def queue(stream=None):
+        dcf.quantize_async(wplan, w, room["wq"], room["ws"], stream=stream)
+        dcf.int8_matmul_async(mm, x, room["wq"], room["y"], room["work"], status, b_scale=room["ws"], stream=stream)
+        dcf.quantize_async(cplan, x, room["q"], room["s"], stream=stream)
+        dcf.dequantize_async(cplan, room["q"], room["s"], room["back"], stream=stream)
+        dcf.checkpoint_grad_async(gp, room["y"], room["q"], room["s"], room["dw"], room["work"], status, stream=stream)
+
+    return (x, w), room, queue
+
+
+def results(room):
+    return [room[n].clone() for n in ("wq", "ws", "q", "s", "back", "y", "dw")]
+
+
+def equal(a, b) -> bool:
+    import torch
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_equal_calls_give_equal_bits_on_two_streams_at_once(dcf):
+    import torch
+    sets = [calls_of(dcf, 10 * k, depth=264 if k else 4096, tokens=300 + 77 * k) for k in range(2)]
+    want = []
+    for _, room, queue in sets:
+        queue()
+        torch.cuda.synchronize()
+        want.append(results(room))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(20):
+        for (_, _, queue), stream in zip(sets, streams):
+            queue(stream)
+    torch.cuda.synchronize()
+    for (_, room, _), w in zip(sets, want):
+        assert equal(results(room), w)
+
+
+def test_captured_and_replayed_on_new_inputs(dcf):
+    import torch
+    (x, w), room, queue = calls_of(dcf, 3)
+    (x2, w2), room2, queue2 = calls_of(dcf, 50)
+    queue2()
+    torch.cuda.synchronize()
+    want = results(room2)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        queue()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            queue()
+    x.copy_(x2)
+    w.copy_(w2)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert equal(results(room), want)
+
+
+def test_graphs_that_share_a_workspace_one_after_the_other(dcf):
+    import torch
+    one, two = calls_of(dcf, 4), calls_of(dcf, 60, tokens=1000)
+    two[1]["work"] = one[1]["work"] = torch.empty(max(one[1]["work"].numel(), two[1]["work"].numel()), dtype=torch.uint8, device="cuda")
+    graphs, want = [], []
+    stream = torch.cuda.Stream()
+    for _, room, queue in (one, two):
+        with torch.cuda.stream(stream):
+            queue()
+            torch.cuda.synchronize()
+            want.append(results(room))
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                queue()
+            graphs.append(g)
+    for _ in range(5):
+        graphs[0].replay()
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    assert equal(results(one[1]), want[0]) and equal(results(two[1]), want[1])
+
+
+def test_rows_past_32_bits_of_elements(dcf):
+    """Two rows 2^31 and some elements apart, in every operand that has rows."""
+    import torch
+    far = (1 << 31) + 16
+    big = torch.empty(far + 4096, dtype=torch.bfloat16, device="cuda")
+    bytes_ = torch.empty(far + 4096, dtype=torch.int8, device="cuda")
+    x, b = randn((2, 256), "bf16", 1), whole((2, 256), 2)
+    values, levels = big.as_strided((2, 256), (far, 1)), bytes_.as_strided((2, 256), (far, 1))
+    values.copy_(x)
+    for along in ("rows", "columns"):
+        plan = dcf.quantize_plan("bf16", 2, 256, along=along, row_stride=far, q_row_stride=far)
+        scale = torch.empty(*plan.scale_shape, device="cuda")
+        dcf.quantize_async(plan, values, levels, scale)
+        want_q, want_s = io.quantize(wide(x), along)
+        assert np.array_equal(levels.cpu().numpy(), want_q) and np.array_equal(scale.cpu().numpy(), want_s)
+        back = big[512:].as_strided((2, 256), (far, 1))
+        dcf.dequantize_async(plan, levels, scale, back)
+        assert same(back, rounded(io.values(want_q, want_s, along), "bf16"))
+    levels.copy_(b)
+    tokens = whole((40, 256), 3)
+    # the weight's rows, and a result's
+    for a in (tokens, tokens[:2]):
+        n = len(a)
+        p = dcf.int8_matmul_plan(n, 2, 256, out_dtype="i32", b_row_stride=far)
+        out, work, st = torch.empty(n, 2, dtype=torch.int32, device="cuda"), torch.empty(p.workspace, dtype=torch.uint8, device="cuda"), new_status(dcf)
+        dcf.int8_matmul_async(p, a, levels, out, work, st)
+        assert np.array_equal(out.cpu().numpy(), io.matmul(a.cpu().numpy(), None, b.cpu().numpy(), None, None))
+    p = dcf.int8_matmul_plan(2, 40, 256, out_dtype="bf16", a_row_stride=far, out_row_stride=far)
+    sa, sb, _ = scales_for(2, 40, 4)
+    work = torch.empty(p.workspace, dtype=torch.uint8, device="cuda")
+    to = big[1024:].as_strided((2, 40), (far, 1))
+    dcf.int8_matmul_async(p, levels, tokens, to, work, st, a_scale=sa, b_scale=sb)
+    assert same(to, rounded(io.matmul(b.cpu().numpy(), sa.cpu().numpy(), tokens.cpu().numpy(), sb.cpu().numpy(), None), "bf16"))
+    # a gradient's rows, a checkpoint's, and a result's
+    g, q, scale = exact_inputs(2, 2, 256, "bf16", 5)
+    values[:, :2].copy_(g)
+    levels.copy_(q)
+    p = dcf.checkpoint_grad_plan("bf16", 2, 2, 256, out_dtype="bf16", grad_row_stride=far, q_row_stride=far, out_row_stride=far)
+    work, to = torch.empty(p.workspace, dtype=torch.uint8, device="cuda"), big[2048:].as_strided((2, 256), (far, 1))
+    dcf.checkpoint_grad_async(p, values[:, :2], levels, scale, to, work, st)
+    want, _ = io.grad(wide(g), q.cpu().numpy(), scale.cpu().numpy())
+    assert same(to, rounded(want.astype(np.float32), "bf16"))
+    assert dcf.status_read(st).folded
+
+
+def test_many_rows(dcf):
+    """More rows, tokens and runs than a grid's second dimension has blocks."""
+    rows = 9_000_000
+    x = randn((rows, 2), "bf16", 1)
+    check_quantize(dcf, x, "bf16", "rows")
+    check_quantize(dcf, x, "bf16", "columns")
+    check_matmul(dcf, 300_000, 3, 5, "f32", seed=1)
+    check_matmul(dcf, 3, 300_000, 5, "bf16", seed=2)
+    check_matmul(dcf, 70, 70_001, 16, "i32", seed=3)
+    for tokens, channels, depth in ((30_000, 3, 5), (5, 70_001, 3), (130, 2, 70_001)):
+        g, q, scale = exact_inputs(tokens, channels, depth, "bf16", tokens)
+        want, _ = io.grad(wide(g), q.cpu().numpy(), scale.cpu().numpy())
+        assert same(run_grad(dcf, g, q, scale, "bf16"), rounded(want.astype(np.float32), "f32"))
+
+
+def test_host_forms(dcf):
+    x = randn((140, 40), "f32", 1).cpu().numpy()
+    for along in ("rows", "columns"):
+        plan = dcf.quantize_plan("f32", 140, 40, along=along)
+        fold, scale = dcf.quantize(plan, x)
+        q, s = io.quantize(x.astype(np.float64), along)
+        assert fold.folded and not fold.is_splat and np.array_equal(fold.out, q) and np.array_equal(scale, s)
+        back = dcf.dequantize(plan, q, s)
+        assert np.array_equal(back.out.view(np.float32), io.values(q, s, along))
+    rng = np.random.default_rng(2)
+    a, b = rng.integers(-127, 128, (50, 40)).astype(np.int8), rng.integers(-127, 128, (9, 40)).astype(np.int8)
+    sa, sb, add = (rng.random(n).astype(np.float32) for n in (50, 9, 9))
+    got = dcf.int8_matmul(dcf.int8_matmul_plan(50, 9, 40, out_dtype="f32"), a, b, a_scale=sa, b_scale=sb, bias=add)
+    assert np.array_equal(got.out.view(np.float32), io.matmul(a, sa, b, sb, add))
+    got = dcf.int8_matmul(dcf.int8_matmul_plan(50, 9, 40, out_dtype="i32"), a, b)
+    assert np.array_equal(got.out.view(np.int32), io.matmul(a, None, b, None, None))
+    got = dcf.int8_matmul(dcf.int8_matmul_plan(140, 9, 40, a_dtype="f32", out_dtype="f32"), x, b, b_scale=sb)
+    assert np.array_equal(got.out.view(np.float32), io.matmul(*io.quantize(x.astype(np.float64), "rows"), b, sb, None))
+    g, q, scale = (t.cpu().numpy() for t in exact_inputs(300, 7, 40, "f16", 3))
+    onto = np.ones((7, 40), np.float32)
+    want, _ = io.grad(g.astype(np.float64), q, scale)
+    assert np.array_equal(dcf.checkpoint_grad(dcf.checkpoint_grad_plan("f16", 300, 7, 40), g, q, scale).out.view(np.float32), want)
+    got = dcf.checkpoint_grad(dcf.checkpoint_grad_plan("f16", 300, 7, 40, accumulate=True), g, q, scale, out=onto)
+    assert np.array_equal(got.out, want + 1)

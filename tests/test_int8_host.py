@@ -67,6 +67,21 @@ def test_quantize_pointers_that_are_refused():
     assert L.dcf_dequantize_async(ctypes.byref(quant_desc(cols=0)), None, None, None, None) == 0
 
 
+def test_parts_of_one_wide_tensor_do_not_overlap():
+    """Rows of a result between the rows of an operand, the same stride apart: only what they share is refused."""
+    L = m.lib()
+    d = quant_desc(dtype=m.DTYPES["f32"], row_stride=64, q_row_stride=256)          # rows of 64 and 16 bytes, 256 apart
+    r = ctypes.byref(d)
+    for q, meets in ((A + 64, False), (A + 240, False), (A + 63, True), (A + 241, True), (A, True), (A + 256 + 64, False),
+                     (A - 256 + 64, False), (A - 16, False), (A - 15, True), (A + 256 * 7 + 63, True), (A + 256 * 7 + 64, False)):
+        assert L.dcf_quantize_async(r, A, q, C, None) == -1            # no such memory, at the latest
+        assert ("overlap" in last()) == meets, hex(q - A)
+        assert L.dcf_dequantize_async(r, q, C, A, None) == -1
+        assert ("overlap" in last()) == meets, hex(q - A)
+    d.q_row_stride = 255                                                # another stride: any reach into it is refused
+    assert L.dcf_quantize_async(r, A, A + 64, C, None) == -1 and "overlap" in last()
+
+
 def test_quantize_plans():
     for kw in (dict(rows=-1), dict(cols=1 << 31), dict(row_stride=-1)):
         with pytest.raises(ValueError):
