@@ -527,7 +527,7 @@ __device__ __forceinline__ void few_quantise(const FewArgs& g, int8_t* x, float*
   for (int c = first; c < groups; c += kShare) {
     Group<V, E> v;
     load_group(v, in + c * E, g.depth - c * E);
-    uint32_t w[E > 4 ? 2 : 1];
+    uint32_t w[kLevelWords<E>];
     quantise_group(v, s, w);
     store_levels<E>(x + t * g.padded + c * E, w, g.depth - c * E);
   }

@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_rows_kernel(const QuantAr
     if (at == 0) a.scale[r] = s.scale;
     int8_t* q = a.q + r * a.qs;
     auto write = [&](Group<T, E>& v, int c) {
-      uint32_t w[E > 4 ? 2 : 1];
+      uint32_t w[kLevelWords<E>];
       quantise_group(v, s, w);
       store_levels<E>(q + (int64_t)c * E, w, a.cols - c * E);
     };
@@ -147,15 +147,8 @@ __global__ void __launch_bounds__(kQuantThreads) quant_columns_kernel(const Quan
       if (y + j * R >= rows) break;
 #pragma unroll
       for (int k = 0; k < kWords; k++) g[j].w[k] &= keep[k];
-      uint32_t w[E > 4 ? 2 : 1];
-      if constexpr (E == 1) {
-        w[0] = level(group_value(g[j], 0), f[0]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; e += 4)
-          w[e / 4] = pack4(level(group_value(g[j], e), f[e]), level(group_value(g[j], e + 1), f[e + 1]),
-                           level(group_value(g[j], e + 2), f[e + 2]), level(group_value(g[j], e + 3), f[e + 3]));
-      }
+      uint32_t w[kLevelWords<E>];
+      pack_levels<E>(w, [&](int e) { return level(group_value(g[j], e), f[e]); });
       store_levels<E>(q + (y + j * R) * a.qs, w, have);
     }
     __syncthreads();
@@ -192,7 +185,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequant_kernel(const QuantArgs 
     const int rows = (int)(a.rows - run * kRun < kRun ? a.rows - run * kRun : kRun);
     if (have <= 0) continue;
     const int8_t* q = a.q + run * kRun * a.qs + c;
-    uint32_t w[S][E > 4 ? 2 : 1];
+    uint32_t w[S][kLevelWords<E>];
 #pragma unroll
     for (int j = 0; j < S; j++) {
       const int8_t* p = q + (y + j * R) * a.qs;
@@ -203,12 +196,14 @@ __global__ void __launch_bounds__(kQuantThreads) dequant_kernel(const QuantArgs 
         if constexpr (E == 8) {
           const uint2 v = *(const uint2*)p;
           w[j][0] = v.x, w[j][E > 4] = v.y;
-        } else {
+        } else if constexpr (E == 4) {
           w[j][0] = *(const uint32_t*)p;
+        } else {
+          w[j][0] = *(const uint16_t*)p;
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < (E > 4 ? 2 : 1); k++) w[j][k] = 0;
+        for (int k = 0; k < kLevelWords<E>; k++) w[j][k] = 0;
 #pragma unroll
         for (int e = 0; e < E; e++)
           if (e < have) w[j][e >> 2] |= (uint32_t)(uint8_t)p[e] << ((e & 3) * 8);
@@ -238,6 +233,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequant_kernel(const QuantArgs 
                                    two_values<T>(v[6], v[7]));
         else if constexpr (E == 4)
           *(float4*)to = make_float4(v[0], v[1], v[2], v[3]);
+        else if constexpr (E == 2)
+          *(uint32_t*)to = two_values<T>(v[0], v[1]);
       } else {
 #pragma unroll
         for (int e = 0; e < E; e++)
@@ -274,14 +271,15 @@ QuantArgs quant_args(const dcf_quant_desc& d, const void* in, int8_t* q, float* 
 
 // Whether rows of values and of whole numbers divide into whole vectors of E.
 template <class T, int E> bool vectors(const QuantArgs& a, const void* values) {
-  return (uintptr_t)values % 16 == 0 && (uintptr_t)a.q % E == 0 &&
-         (a.rows == 1 || (a.rs * (int64_t)sizeof(T) % 16 == 0 && a.qs % E == 0));
+  constexpr int kBytes = E * (int)sizeof(T);
+  return (uintptr_t)values % kBytes == 0 && (uintptr_t)a.q % E == 0 &&
+         (a.rows == 1 || (a.rs * (int64_t)sizeof(T) % kBytes == 0 && a.qs % E == 0));
 }
 
 // Rows to a warp while that keeps them in registers, then to a block that holds as little as
 // it can: more blocks to an SM have more on its way (f32, 8192 x 4096: 38 us with room for twice the row, XX us so).
 template <class T, int E> int quantize_rows(const QuantArgs& a, cudaStream_t s) {
-  constexpr int kUnit = E == 1 ? 4 : 1;
+  constexpr int kUnit = E <= 2 ? 4 : 1;
   const int64_t groups = (a.cols + E - 1) / E;
   auto run = [&](auto kernel, int64_t blocks) { return launch(kernel, blocks_of(blocks), kQuantThreads, 0, 1, s, a); };
   if (groups <= 32 * 4 * kUnit)
@@ -291,7 +289,7 @@ template <class T, int E> int quantize_rows(const QuantArgs& a, cudaStream_t s) 
   return run(quant_rows_kernel<T, E, 8 * kUnit, kQuantThreads>, a.rows);
 }
 
-template <int E> constexpr int kWide = E == 1 ? 64 : 16;  // groups of a tile's row
+template <int E> constexpr int kWide = E == 1 ? 64 : E == 2 ? 32 : 16;  // groups of a tile's row
 
 template <class T, int E, int W> int64_t run_tiles(const QuantArgs& a) {
   constexpr int kCols = RunTile<T, E, W>::kCols;
@@ -310,13 +308,18 @@ template <class T, int E> int dequantize_t(const dcf_quant_desc& d, const QuantA
                                    : launch(dequant_kernel<T, E, W, true>, blocks, kQuantThreads, 0, 1, s, a, (T*)out);
 }
 
-// Calls f<T, E>() of the type and of whole vectors or single values.
+// Calls f<T, E>() of the type and of the widest vectors that rows divide into (16-bit values, rows of odd numbers
+// of words: two at a time, 3728 x 3186 35 -> XX us).
 template <class F> int by_type(uint32_t dtype, const QuantArgs& a, const void* values, F f) {
+  auto half = [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (vectors<T, 8>(a, values)) return f(t, std::integral_constant<int, 8>());
+    if (vectors<T, 2>(a, values)) return f(t, std::integral_constant<int, 2>());
+    return f(t, std::integral_constant<int, 1>());
+  };
   switch (dtype) {
-    case DCF_F16: return vectors<__half, 8>(a, values) ? f((__half*)0, std::integral_constant<int, 8>())
-                                                       : f((__half*)0, std::integral_constant<int, 1>());
-    case DCF_BF16: return vectors<__nv_bfloat16, 8>(a, values) ? f((__nv_bfloat16*)0, std::integral_constant<int, 8>())
-                                                               : f((__nv_bfloat16*)0, std::integral_constant<int, 1>());
+    case DCF_F16: return half((__half*)0);
+    case DCF_BF16: return half((__nv_bfloat16*)0);
     case DCF_F32: return vectors<float, 4>(a, values) ? f((float*)0, std::integral_constant<int, 4>())
                                                       : f((float*)0, std::integral_constant<int, 1>());
     default: return DCF_EUNSUPPORTED;

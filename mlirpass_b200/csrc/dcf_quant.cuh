@@ -19,7 +19,8 @@ constexpr int kRun = DCF_QUANT_RUN;
 constexpr float kLeastMagnitude = 0x1p-119f;  // 127 / m is finite from here on, and m / 127 a normal number
 constexpr float kRounder = 12582912.0f;       // 1.5 * 2^23
 
-// Bits of E values of T: one 16-byte vector, or a single value in the low bits.
+// Bits of E values of T: one 16-byte vector, or, of rows that are none, a word of two 16-bit values, or a single
+// value in the low bits.
 template <class T, int E> struct Group {
   static constexpr int kWords = E > 1 ? E * (int)sizeof(T) / 4 : 1;
   uint32_t w[kWords];
@@ -36,11 +37,15 @@ template <class T, int E> __device__ __forceinline__ void load_group(Group<T, E>
     g.w[0] = have > 0 ? bits_of(p) : 0;
   } else {
     if (have >= E) {
-      const uint4 v = *(const uint4*)p;
-      g.w[0] = v.x, g.w[1] = v.y, g.w[2] = v.z, g.w[3] = v.w;
+      if constexpr (E == 2) {
+        g.w[0] = *(const uint32_t*)p;
+      } else {
+        const uint4 v = *(const uint4*)p;
+        g.w[0] = v.x, g.w[1] = v.y, g.w[2] = v.z, g.w[3] = v.w;
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; j++) g.w[j] = 0;
+      for (int j = 0; j < Group<T, E>::kWords; j++) g.w[j] = 0;
 #pragma unroll
       for (int j = 0; j < E; j++)
         if (j < have) g.w[j * sizeof(T) / 4] |= bits_of(p + j) << (j * sizeof(T) % 4 * 8);
@@ -98,6 +103,21 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// Bytes of E whole numbers.
+template <int E> constexpr int kLevelWords = E > 4 ? 2 : 1;
+
+// E whole numbers from the values that a group and the factors beside them give.
+template <int E, class F> __device__ __forceinline__ void pack_levels(uint32_t (&w)[kLevelWords<E>], F at) {
+  if constexpr (E == 1) {
+    w[0] = at(0);
+  } else if constexpr (E == 2) {
+    w[0] = __byte_perm(at(0), at(1), 0x0040);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; j += 4) w[j / 4] = pack4(at(j), at(j + 1), at(j + 2), at(j + 3));
+  }
+}
+
 // Value j of a group.
 template <class T, int E> __device__ __forceinline__ float group_value(const Group<T, E>& g, int j) {
   if constexpr (sizeof(T) == 4 || E == 1) return value_of<T>(g.w[j]);
@@ -107,17 +127,10 @@ template <class T, int E> __device__ __forceinline__ float group_value(const Gro
 
 // The whole numbers of a group, all beside the same largest magnitude.
 template <class T, int E>
-__device__ __forceinline__ void quantise_group(Group<T, E>& v, const Scale& s, uint32_t (&w)[E > 4 ? 2 : 1]) {
+__device__ __forceinline__ void quantise_group(Group<T, E>& v, const Scale& s, uint32_t (&w)[kLevelWords<E>]) {
 #pragma unroll
   for (int j = 0; j < Group<T, E>::kWords; j++) v.w[j] &= s.keep;
-  if constexpr (E == 1) {
-    w[0] = level(group_value(v, 0), s.factor);
-  } else {
-#pragma unroll
-    for (int j = 0; j < E; j += 4)
-      w[j / 4] = pack4(level(group_value(v, j), s.factor), level(group_value(v, j + 1), s.factor),
-                       level(group_value(v, j + 2), s.factor), level(group_value(v, j + 3), s.factor));
-  }
+  pack_levels<E>(w, [&](int j) { return level(group_value(v, j), s.factor); });
 }
 
 // The first `have` bytes of q's words to p, which vectors of E bytes divide.
@@ -127,7 +140,8 @@ template <int E> __device__ __forceinline__ void store_levels(int8_t* p, const u
   } else {
     if (have >= E) {
       if constexpr (E == 8) *(uint2*)p = make_uint2(w[0], w[1]);
-      else *(uint32_t*)p = w[0];
+      else if constexpr (E == 4) *(uint32_t*)p = w[0];
+      else *(uint16_t*)p = (uint16_t)w[0];
     } else {
 #pragma unroll
       for (int j = 0; j < E; j++)
