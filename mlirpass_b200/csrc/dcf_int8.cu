@@ -11,7 +11,7 @@ namespace {
 
 constexpr int kSide = 128;                // channels of a CTA
 constexpr int kTileM = 2 * kSide;         // of a pair
-constexpr int kBK = 128;                  // k of a stage: one 128-byte swizzle row
+constexpr int kAtom = 128;                // k of a 128-byte swizzle row
 template <bool READ> constexpr int kOutWarps = READ ? 8 : 16;  // warps that write results
 template <bool READ> constexpr int kGemmThreads = 128 + 32 * kOutWarps<READ>;  // warp 0 loads, warp 1 multiplies
 constexpr int kReaders = 256;             // threads that read a weight's rows where no tensor map describes them
@@ -45,9 +45,13 @@ __device__ __forceinline__ void put(const Result& g, int64_t t, int64_t c, int s
 
 // ------------------------------------------------- tensor-core product
 
-template <int TN> constexpr int kStage = (kSide + TN / 2) * kBK;
-template <int TN> constexpr int kStages = TN == 256 ? 6 : TN == 128 ? 8 : 10;
-template <int TN> constexpr int kGemmSmem = kStages<TN> * kStage<TN> + 4 * TN * 4 + 512 + 1024;
+// k of a stage: two swizzle rows, so that half as many waits come between the
+// products and memory is read 256 bytes of a row at a time; one where threads read the weight.
+template <bool READ> constexpr int kAtoms = READ ? 1 : 2;
+template <bool READ> constexpr int kBK = kAtoms<READ> * kAtom;
+template <int TN, bool READ> constexpr int kStage = (kSide + TN / 2) * kBK<READ>;
+template <int TN, bool READ> constexpr int kStages = (TN == 256 ? 6 : TN == 128 ? 8 : 10) / kAtoms<READ>;
+template <int TN, bool READ> constexpr int kGemmSmem = kStages<TN, READ> * kStage<TN, READ> + 4 * TN * 4 + 512 + 1024;
 
 struct GemmArgs {
   Result to;
@@ -199,10 +203,10 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
                      const GemmArgs args) {
   const GemmArgs g = args;  // a reference to the parameter itself would be read through memory
   constexpr int OW = kOutWarps<READ>, kMine = TN / (OW / 4);  // columns of one out warp
-  constexpr int S = kStages<TN>;
+  constexpr int S = kStages<TN, READ>, BK = kBK<READ>, kSize = kStage<TN, READ>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);
-  float* scales = (float*)(base + S * kStage<TN>);
+  float* scales = (float*)(base + S * kSize);
   uint64_t* full = (uint64_t*)(scales + OW * kMine);
   uint64_t* empty = full + S;             // (the first CTA's `full` counts what both have loaded)
   uint64_t* sum_full = empty + S;
@@ -256,8 +260,11 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         if (!READ && first < g.total) {
           const int row = (int)(first / g.splits % g.tiles_m) * kTileM + (int)rank * kSide;
           for (const int end = min(S, count_of(first)); ahead < end; ahead++) {
-            if (!rank) mbar_expect_tx(&full[ahead], 2 * kStage<TN>);
-            pair_load_2d(stage0 + ahead * kStage<TN>, &map_b, (begin_of(first) + ahead) * kBK, row, full0 + ahead * 8);
+            if (!rank) mbar_expect_tx(&full[ahead], 2 * kSize);
+#pragma unroll
+            for (int h = 0; h < kAtoms<READ>; h++)
+              pair_load_2d(stage0 + ahead * kSize + h * (kSide * kAtom), &map_b, (begin_of(first) + ahead) * BK + h * kAtom, row,
+                           full0 + ahead * 8);
           }
         }
         pdl_begin();
@@ -267,20 +274,24 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         const int row = (int)(tile % g.tiles_m) * kTileM + (int)rank * kSide;
         const int col = (int)(tile / g.tiles_m) * TN + (int)rank * (TN / 2);
         const int b0 = begin_of(t), blocks = count_of(t);
-        for (int k = b0 * kBK, end = (b0 + blocks) * kBK; k < end; k += kBK, at.next()) {
+        for (int k = b0 * BK, end = (b0 + blocks) * BK; k < end; k += BK, at.next()) {
           if (!mbar_wait_parked(&empty[at.s], at.turn ^ 1)) {
             fail = true;
             break;
           }
-          const uint32_t to = stage0 + at.s * kStage<TN>;
+          const uint32_t to = stage0 + at.s * kSize;
           const uint32_t bar = full0 + at.s * 8;
           if (ahead > 0) {
             ahead--;
           } else {
-            if (!rank) mbar_expect_tx(&full[at.s], 2 * (READ ? TN / 2 * kBK : kStage<TN>));
-            if (!READ) pair_load_2d(to, &map_b, k, row, bar);
+            if (!rank) mbar_expect_tx(&full[at.s], 2 * (READ ? TN / 2 * BK : kSize));
+#pragma unroll
+            for (int h = 0; h < kAtoms<READ>; h++)
+              if (!READ) pair_load_2d(to + h * (kSide * kAtom), &map_b, k + h * kAtom, row, bar);
           }
-          pair_load_2d(to + kSide * kBK, &map_a, k, col, bar);
+#pragma unroll
+          for (int h = 0; h < kAtoms<READ>; h++)
+            pair_load_2d(to + kSide * BK + h * (TN / 2 * kAtom), &map_a, k + h * kAtom, col, bar);
           used += used < S;
         }
       }
@@ -310,13 +321,14 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t pb = desc + (uint64_t)(at.s * (kStage<TN> >> 4)), pa = pb + (kSide * kBK >> 4);
+          const uint64_t pb = desc + (uint64_t)(at.s * (kSize >> 4)), pa = pb + (kSide * BK >> 4);
           uint64_t* const done = &empty[at.s];
           at.next();
 #pragma unroll
-          for (int j = 0; j < kBK / 32; j++) {
-            pair_mma_i8(tmem + sum.s * TN, pb + 2 * j, pa + 2 * j, idesc, b | j);
-            if (j == 1) there = mbar_test(&full[at.s], at.turn);  // before the tensor core runs out of products
+          for (int j = 0; j < BK / 32; j++) {
+            const int h = j / 4, at32 = j % 4 * 2;  // the swizzle row, and 32 bytes in it
+            pair_mma_i8(tmem + sum.s * TN, pb + h * (kSide * kAtom >> 4) + at32, pa + h * (TN / 2 * kAtom >> 4) + at32, idesc, b | j);
+            if (j == BK / 32 - 3) there = mbar_test(&full[at.s], at.turn);  // before the tensor core runs out of products
           }
           pair_commit(done);
         }
@@ -342,30 +354,30 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     Ring<S> at;
     if (first < g.total) {
       rows_of(first);
-      read(begin_of(first) * kBK);
+      read(begin_of(first) * BK);
     }
     for (int64_t t = first; t < g.total && !fail; t += step) {
-      const int k0 = begin_of(t) * kBK, end = k0 + count_of(t) * kBK;
-      for (int k = k0; k < end; k += kBK, at.next()) {
+      const int k0 = begin_of(t) * BK, end = k0 + count_of(t) * BK;
+      for (int k = k0; k < end; k += BK, at.next()) {
         uint4 v[kRows];
 #pragma unroll
         for (int j = 0; j < kRows; j++) v[j] = read_end<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
         // The next stage is on its way while this one waits for room.
-        if (k + kBK < end) {
-          read(k + kBK);
+        if (k + BK < end) {
+          read(k + BK);
         } else if (t + step < g.total) {
           rows_of(t + step);
-          read(begin_of(t + step) * kBK);
+          read(begin_of(t + step) * BK);
         }
         if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
           fail = true;
           break;
         }
-        uint8_t* to = base + at.s * kStage<TN>;
+        uint8_t* to = base + at.s * kSize;
 #pragma unroll
         for (int j = 0; j < kRows; j++) {
           const int r = id / 8 + j * (kReaders / 8);
-          *(uint4*)(to + r * kBK + ((chunk ^ (r & 7)) << 4)) = v[j];
+          *(uint4*)(to + r * BK + ((chunk ^ (r & 7)) << 4)) = v[j];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         arrive_first(&full[at.s]);
@@ -650,7 +662,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(con
 bool encode_rows(CUtensorMap* map, const int8_t* p, int64_t rows, int64_t cols, int64_t stride, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)stride};
-  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {kAtom, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
@@ -673,7 +685,7 @@ struct Cut {
 };
 
 Cut cut_of(const dcf_int8_desc& d) {
-  const int blocks = (int)((d.depth + kBK - 1) / kBK);
+  const int blocks = (int)((d.depth + kBK<false> - 1) / kBK<false>);
   Cut best = {};
   double least = 1e300;
   for (int tn : {64, 128, 256}) {
@@ -753,9 +765,9 @@ template <bool READ> int few_product(int bucket, const FewArgs& g, cudaStream_t 
 
 template <int TN, bool READ>
 int gemm(const CUtensorMap& mb, const CUtensorMap& ma, const GemmArgs& g, cudaStream_t s) {
-  if (!prepare_smem((const void*)int8_gemm_kernel<TN, READ>, kGemmSmem<TN>)) return DCF_ECUDA;
+  if (!prepare_smem((const void*)int8_gemm_kernel<TN, READ>, kGemmSmem<TN, READ>)) return DCF_ECUDA;
   const unsigned pairs = (unsigned)(g.total < kPairs ? g.total : kPairs);
-  return launch(int8_gemm_kernel<TN, READ>, dim3(2 * pairs), kGemmThreads<READ> + (READ ? kReaders : 0), kGemmSmem<TN>, 2, s, mb, ma, g);
+  return launch(int8_gemm_kernel<TN, READ>, dim3(2 * pairs), kGemmThreads<READ> + (READ ? kReaders : 0), kGemmSmem<TN, READ>, 2, s, mb, ma, g);
 }
 
 }  // namespace
@@ -846,10 +858,8 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
   const int8_t* q = (const int8_t*)a;
   GemmArgs g = {};
   g.to = to;
-  g.blocks = (int)((d.depth + kBK - 1) / kBK);
   g.tiles_m = (int)cut.tiles_m;
   g.splits = d.depth ? cut.splits : 0;
-  g.split_k = cut.stages;
   g.total = cut.tiles * cut.splits;
   g.part = (int*)(work + l.part);
   g.st = st;
@@ -857,6 +867,9 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     if (!mappable(q, as, d.depth) && (rc = pack(&q, &as, d.tokens, l.a))) return rc;
     if (l.copy_b && (rc = pack(&b, &bs, d.channels, l.b))) return rc;
     const bool read = !mappable(b, bs, d.depth);
+    const int bk = read ? kBK<true> : kBK<false>;
+    g.blocks = (int)((d.depth + bk - 1) / bk);
+    g.split_k = cut.stages * (kBK<false> / bk);
     g.b = b;
     g.b_stride = bs;
     g.depth = (int)d.depth;
