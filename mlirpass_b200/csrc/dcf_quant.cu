@@ -5,7 +5,10 @@
 // All four are bound by HBM: a value is read once, held in registers until the
 // largest magnitude beside it is known, and its byte written; reading back is
 // the same way round.  Some five instructions per value (dcf_quant.cuh) keep
-// the arithmetic behind that.
+// the arithmetic behind that.  Measured (bytes read and written over the
+// kernel's time): 8192 x 4096 f32 by rows 32 us and back 28 us (5.3, 6.0 TB/s),
+// bf16 by columns 20 us and back 17 us (4.9, 5.9 TB/s; one after the other they
+// take 33 us, as what is read back is still in L2).
 #include <math.h>
 
 #include "dcf_quant.cuh"
@@ -277,7 +280,7 @@ template <class T, int E> bool vectors(const QuantArgs& a, const void* values) {
 }
 
 // Rows to a warp while that keeps them in registers, then to a block that holds as little as
-// it can: more blocks to an SM have more on its way (f32, 8192 x 4096: 38 us with room for twice the row, XX us so).
+// it can: more blocks to an SM have more on its way (f32, 8192 x 4096: 38 us with room for twice the row, 32 us so).
 template <class T, int E> int quantize_rows(const QuantArgs& a, cudaStream_t s) {
   constexpr int kUnit = E <= 2 ? 4 : 1;
   const int64_t groups = (a.cols + E - 1) / E;
@@ -309,7 +312,7 @@ template <class T, int E> int dequantize_t(const dcf_quant_desc& d, const QuantA
 }
 
 // Calls f<T, E>() of the type and of the widest vectors that rows divide into (16-bit values, rows of odd numbers
-// of words: two at a time, 3728 x 3186 35 -> XX us).
+// of words: two at a time; 3728 x 3186 there and back 35 us by single values, 27 us so).
 template <class F> int by_type(uint32_t dtype, const QuantArgs& a, const void* values, F f) {
   auto half = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
