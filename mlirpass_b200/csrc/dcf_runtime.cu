@@ -1512,6 +1512,10 @@ int dcf_quantize(const dcf_quant_desc* desc, const void* in, int8_t* q, float* s
   if ((rc = launch_quantize(d, base + at_in, (int8_t*)base + at_q, (float*)(base + at_scale), s)))
     return learned_launch_failed(rc, "quantize");
   if ((rc = d2h_full(dev, q, base + at_q, n, s)) || (rc = d2h_full(dev, scale, base + at_scale, scales * 4, s))) return rc;
+  if (!n) {
+    learned_result(res, true);
+    return DCF_OK;
+  }
   return learned_splat(dev, base + at_q, 1, n, s, res);
 }
 

@@ -393,6 +393,29 @@ def test_grad_is_the_differences_of_the_layer(dcf):
         assert loss(w + step) - loss(w) == grad[c, k]
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_grad_of_every_whole_number(dcf, dtype):
+    """All 256 bytes, -128 among them, each picked out by a token of its own."""
+    import torch
+    g = torch.eye(256, device="cuda").to(tdtype(dtype))
+    q = torch.arange(-128, 128, device="cuda").to(torch.int8)[:, None].repeat(1, 20)
+    scale = torch.tensor([[1.0], [0.5]], device="cuda").repeat(1, 20)
+    got = run_grad(dcf, g, q, scale, dtype)
+    want = q.float() * scale.repeat_interleave(128, 0)
+    assert torch.equal(got, want)
+
+
+def test_matmul_of_no_depth(dcf):
+    """Float tokens without a single value: nothing but the bias is left."""
+    import torch
+    for tokens in (2, 40):
+        x, b = torch.empty(tokens, 0, dtype=torch.bfloat16, device="cuda"), torch.empty(6, 0, dtype=torch.int8, device="cuda")
+        _, sb, add = scales_for(tokens, 6, 1)
+        assert torch.equal(run_matmul(dcf, x, b, a_dtype="bf16", out="f32", b_scale=sb, bias=add), add.repeat(tokens, 1))
+    fold, scale = dcf.quantize(dcf.quantize_plan("f32", 5, 0), np.empty((5, 0), np.float32))
+    assert fold.folded and (scale == 0).all()
+
+
 def test_grad_adds_to_what_is_there(dcf):
     g, q, scale = exact_inputs(300, 70, 90, "f16", 6)
     onto = whole((70, 90), 9).float()
