@@ -406,22 +406,39 @@ __global__ void __launch_bounds__(kJoinThreads) grad_join_kernel(const __grid_co
   }
 }
 
-// Whole numbers as values of T, rows of whole vectors; a thread makes sixteen,
-// 2^wide threads a row.
-constexpr int kLevelThreads = 256;
+// What the products read, in rows of whole vectors: whole numbers as values of T, and, in a second row of
+// blocks, a gradient whose rows no tensor map describes.  A thread makes sixteen values, or copies sixteen
+// bytes; 2^wide threads take a row.
+constexpr int kOperandThreads = 256;
+struct Rows {
+  const uint8_t* from;
+  int64_t stride, bytes;  // in bytes
+  uint8_t* to;
+  int64_t to_stride;
+  int wide;
+};
 template <class T>
-__global__ void __launch_bounds__(kLevelThreads) levels_kernel(const int8_t* q, int64_t stride, int64_t rows, int64_t cols,
-                                                               T* to, int64_t to_stride, int wide) {
+__global__ void __launch_bounds__(kOperandThreads) operands_kernel(const __grid_constant__ Rows levels,
+                                                                   const __grid_constant__ Rows grad, int64_t rows) {
   pdl_begin();
-  const int64_t first = threadIdx.x & ((1 << wide) - 1), across = (int64_t)1 << wide;
-  for (int64_t r = (int64_t)blockIdx.x * (kLevelThreads >> wide) + (threadIdx.x >> wide); r < rows;
-       r += (int64_t)gridDim.x * (kLevelThreads >> wide)) {
-    const uint8_t* row = (const uint8_t*)q + r * stride;
-    for (int64_t c = first * 16; c < cols; c += across * 16) {
-      const uint4 v = row_bytes(row, c, cols);
-      uint4* out = (uint4*)(to + r * to_stride + c);
-      out[0] = to_eight<T>(v.x, v.y);
-      out[1] = to_eight<T>(v.z, v.w);
+  const bool copy = blockIdx.y;
+  const int64_t stride = copy ? grad.stride : levels.stride, bytes = copy ? grad.bytes : levels.bytes;
+  const int64_t to_stride = copy ? grad.to_stride : levels.to_stride;
+  const uint8_t* from = copy ? grad.from : levels.from;
+  uint8_t* to = copy ? grad.to : levels.to;
+  const int wide = copy ? grad.wide : levels.wide, first = threadIdx.x & ((1 << wide) - 1);
+  const int64_t step = (int64_t)gridDim.x * (kOperandThreads >> wide);
+  for (int64_t r = (int64_t)blockIdx.x * (kOperandThreads >> wide) + (threadIdx.x >> wide); r < rows; r += step) {
+    const uint8_t* row = from + r * stride;
+    for (int64_t c = (int64_t)first * 16; c < bytes; c += (int64_t)16 << wide) {
+      const uint4 v = row_bytes(row, c, bytes);
+      if (copy) {
+        *(uint4*)(to + r * to_stride + c) = v;
+      } else {
+        uint4* out = (uint4*)(to + r * to_stride + 2 * c);
+        out[0] = to_eight<T>(v.x, v.y);
+        out[1] = to_eight<T>(v.z, v.w);
+      }
     }
   }
 }
@@ -563,10 +580,15 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     Layout l = layout_of(d, 0);
     int64_t gs = d.tokens > 1 ? stride_of(d.grad_row_stride, d.channels) : l.stride + 8;
     int rc;
-    if (l.copy) {
-      uint8_t* to = (uint8_t*)ws + l.grad;
-      if ((rc = launch_pack_rows(grad, gs * 2, (int64_t)d.tokens, (int64_t)d.channels * 2, to, l.stride * 2, s))) return rc;
-      grad = to;
+    auto rows_of = [](const void* from, int64_t stride, int64_t bytes, void* to, int64_t to_stride) {
+      Rows r = {(const uint8_t*)from, stride, bytes, (uint8_t*)to, to_stride, 0};
+      while (r.wide < 8 && (16ll << r.wide) < bytes) r.wide++;
+      return r;
+    };
+    const Rows copy = rows_of(grad, gs * 2, (int64_t)d.channels * 2, (uint8_t*)ws + l.grad, l.stride * 2);
+    const bool copied = l.copy;
+    if (copied) {
+      grad = copy.to;
       gs = l.stride;
     }
     // A map starts on a 16-byte boundary; the columns before the first channel are left out again.
@@ -574,20 +596,17 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
     if (g.skip) l = layout_of(d, g.skip);
     const bool bf16 = d.grad_dtype == DCF_BF16;
     if (!encoder()) return DCF_EUNSUPPORTED;
-    void* levels = (uint8_t*)ws + l.levels;
-    const int64_t qs = stride_of(d.q_row_stride, d.depth), rows = (int64_t)d.tokens, cols = (int64_t)d.depth;
-    int wide = 0;
-    while (wide < 8 && (16 << wide) < cols) wide++;
-    const int64_t blocks = (rows + (kLevelThreads >> wide) - 1) / (kLevelThreads >> wide);
-    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30));
-    rc = bf16 ? launch(levels_kernel<__nv_bfloat16>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__nv_bfloat16*)levels,
-                       l.level_stride, wide)
-              : launch(levels_kernel<__half>, grid, kLevelThreads, 0, 1, s, q, qs, rows, cols, (__half*)levels, l.level_stride,
-                       wide);
+    const int64_t rows = (int64_t)d.tokens, cols = (int64_t)d.depth;
+    const Rows levels = rows_of(q, stride_of(d.q_row_stride, d.depth), cols, (uint8_t*)ws + l.levels, l.level_stride * 2);
+    const int across = kOperandThreads >> (copied && copy.wide > levels.wide ? copy.wide : levels.wide);
+    const int64_t blocks = (rows + across - 1) / across;
+    const dim3 grid((unsigned)(blocks < (1 << 30) ? blocks : 1 << 30), copied ? 2 : 1);
+    rc = bf16 ? launch(operands_kernel<__nv_bfloat16>, grid, kOperandThreads, 0, 1, s, levels, copy, rows)
+              : launch(operands_kernel<__half>, grid, kOperandThreads, 0, 1, s, levels, copy, rows);
     if (rc) return rc;
     CUtensorMap map_q, map_g;
     tile_n = l.cut.tile_n;
-    if (!encode_operand(&map_q, levels, bf16, cols, rows, l.level_stride) ||
+    if (!encode_operand(&map_q, levels.to, bf16, cols, rows, l.level_stride) ||
         !encode_operand(&map_g, (const uint8_t*)grad - g.skip * 2, bf16, (int64_t)d.channels + g.skip, rows, gs))
       return DCF_ECUDA;
     g.runs = (int)((d.tokens + kRun - 1) / kRun);
