@@ -114,9 +114,12 @@ __device__ __forceinline__ void write_block(const GradArgs& g, const float* v, i
   if (g.out_dtype == DCF_F32) {
     if (k >= g.depth) return;
     float* out = (float*)g.out + (int64_t)c0 * g.os + k;
+    float old[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) old[j] = g.add && c0 + j >= 0 && c0 + j < g.channels ? out[j * g.os] : 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; j++, out += g.os)
-      if (c0 + j >= 0 && c0 + j < g.channels) *out = g.add ? __fadd_rn(*out, v[j]) : v[j];
+      if (c0 + j >= 0 && c0 + j < g.channels) *out = g.add ? __fadd_rn(old[j], v[j]) : v[j];
   } else if (g.pairs) {
     // Lanes trade: an even one writes its channel for two k, an odd one the next channel.
     const int odd = threadIdx.x & 1;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
       }
       if (fail) break;
       // The products wait while a tile is written, so the usual ways out are straight: sums of parts, and whole
-      // f32 tiles (17000 cycles a tile by the general way below).
+      // tiles (17000 cycles a tile by the general way below).
       const bool inside = c0 >= 0 && c0 + kMine <= g.channels && k - lane + 32 <= g.depth;
       if (g.splits > 1) {
         float* p = part_of<TN>(g, t) + (int64_t)col * kTileM + row;
@@ -329,14 +332,46 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
         }
         continue;
       }
-      if (inside && g.out_dtype == DCF_F32 && !g.add) {
+      if (inside && g.out_dtype == DCF_F32) {
         float* p = (float*)g.out + (int64_t)c0 * g.os + k;
+        if (g.add) {
 #pragma unroll
-        for (int j = 0; j < kMine / 2; j++, p += 2 * g.os) {
-          const float2 f = apart(acc[j]);
-          p[0] = f.x;
-          p[g.os] = f.y;
+          for (int c = 0; c < kMine; c += 16) {  // what is there is read sixteen at a time
+            float old[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) old[j] = p[j * g.os];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2, p += 2 * g.os) {
+              const float2 f = apart(acc[(c + j) / 2]);
+              p[0] = __fadd_rn(old[j], f.x);
+              p[g.os] = __fadd_rn(old[j + 1], f.y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kMine / 2; j++, p += 2 * g.os) {
+            const float2 f = apart(acc[j]);
+            p[0] = f.x;
+            p[g.os] = f.y;
+          }
         }
+        continue;
+      }
+      if (inside && g.pairs) {
+        // As in write_block, every lane with both of its k.
+        const int odd = lane & 1;
+        uint16_t* p = (uint16_t*)g.out + (int64_t)(c0 + odd) * g.os + (k & ~1);
+        auto each = [&](auto cast) {
+#pragma unroll
+          for (int j = 0; j < kMine / 2; j++, p += 2 * g.os) {
+            const float2 f = apart(acc[j]);
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? f.x : f.y, 1);
+            const auto h = cast(odd ? got : f.x, odd ? f.y : got);
+            *(uint32_t*)p = *(const uint32_t*)&h;
+          }
+        };
+        if (g.out_dtype == DCF_F16) each([](float a, float b) { return __floats2half2_rn(a, b); });
+        else each([](float a, float b) { return __floats2bfloat162_rn(a, b); });
         continue;
       }
 #pragma unroll 1

@@ -416,9 +416,10 @@ def test_matmul_of_no_depth(dcf):
     assert fold.folded and (scale == 0).all()
 
 
-def test_grad_adds_to_what_is_there(dcf):
-    g, q, scale = exact_inputs(300, 70, 90, "f16", 6)
-    onto = whole((70, 90), 9).float()
+@pytest.mark.parametrize("tokens,channels,depth", [(300, 70, 90), (300, 256, 256), (130, 600, 520), (6000, 128, 40), (2, 400, 33)])
+def test_grad_adds_to_what_is_there(dcf, tokens, channels, depth):
+    g, q, scale = exact_inputs(tokens, channels, depth, "f16", 6)
+    onto = whole((channels, depth), 9).float()
     want, _ = io.grad(wide(g), q.cpu().numpy(), scale.cpu().numpy())
     assert same(run_grad(dcf, g, q, scale, "f16", onto=onto), rounded((want + wide(onto)).astype(np.float32), "f32"))
     none = run_grad(dcf, g[:0], q[:0], scale[:0], "f16", onto=onto)
