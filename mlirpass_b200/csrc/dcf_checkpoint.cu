@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
       for (int t = first; t < g.total; t += step) left += count_of(t);
       bool room = false, there = false;
       for (; left > 0; left--) {
-        if ((!room && !mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) || (!there && !mbar_wait_parked(&full[at.s], at.turn))) {
+        if ((!room && !pair_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) || (!there && !mbar_wait_parked(&full[at.s], at.turn))) {
           fail = true;
           break;
         }
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
 #pragma unroll
         for (int j = 0; j < kRun / 16; j++) {
           pair_mma_low(to, pq + j * (2048 >> 4), pg + j * (2048 >> 4), g.idesc, j);
-          if (j == 3) room = mbar_test(&sum_empty[sum.s], sum.turn ^ 1);
+          if (j == 3) room = pair_test(&sum_empty[sum.s], sum.turn ^ 1);
           if (j == 5) there = mbar_test(&full[at.s], at.turn);
         }
         pair_commit(summed);
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) grad_kernel(const __grid_cons
             tmem_load16(lanes + sum.s * TN + c + 16, x[(c / 16 + 1) & 1]);
           } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) arrive_first(&sum_empty[sum.s]);
+            if (lane == 0) arrive_first<false>(&sum_empty[sum.s]);
           }
 #pragma unroll
           for (int j = 0; j < 16; j += 2)

@@ -220,7 +220,9 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
   uint64_t* empty = full + S;             // (the first CTA's `full` counts what both have loaded)
   uint64_t* sum_full = empty + S;
   uint64_t* sum_empty = sum_full + 2;     // the first CTA's
-  uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
+  uint64_t* read = sum_empty + 2;         // READ: this CTA's part of the weight is in its memory
+  uint64_t* peer = read + S;              // and the second's is, the first CTA's
+  uint32_t* tmem_at = (uint32_t*)(peer + S);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2;
@@ -232,8 +234,10 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
 
   if (warp == 0 && lane == 0) {
     for (int s = 0; s < S; s++) {
-      mbar_init(&full[s], READ ? 1 + 2 * kReaders : 1);
+      mbar_init(&full[s], READ ? 2 : 1);
       mbar_init(&empty[s], 1);
+      if (READ) mbar_init(&read[s], kReaders);
+      if (READ) mbar_init(&peer[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
       bool there = false;
       for (int64_t t = first; t < g.total && !fail; t += step, sum.next()) {
         const int blocks = count_of(t);
-        if (!mbar_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) {
+        if (!pair_wait_parked(&sum_empty[sum.s], sum.turn ^ 1)) {
           fail = true;
           break;
         }
@@ -344,6 +348,21 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         if (!fail) pair_commit(&sum_full[sum.s]);
       }
     }
+  } else if (READ && warp == 2) {
+    // Passes on that a stage's weight is there, so that neither the readers, who have loads on their way, nor the
+    // thread that issues products spend time on the other CTA.
+    if (lane == 0) {
+      Ring<S> at;
+      for (int64_t t = first; t < g.total && !fail; t += step)
+        for (int left = count_of(t); left > 0; left--, at.next()) {
+          if (!mbar_wait_parked(&read[at.s], at.turn) || (!rank && !pair_acquire(&peer[at.s], at.turn))) {
+            fail = true;
+            break;
+          }
+          if (rank) arrive_first<true>(&peer[at.s]);
+          else mbar_arrive(&full[at.s]);
+        }
+    }
   } else if (warp >= 4 + OW) {
     const int id = threadIdx.x - kGemmThreads<READ>, chunk = id & 7;
     constexpr int kRows = kSide * 8 / kReaders;
@@ -356,14 +375,14 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         rows[j] = r < g.to.channels ? g.b + r * g.b_stride : nullptr;
       }
     };
-    auto read = [&](int k) {
+    auto start = [&](int k) {
 #pragma unroll
       for (int j = 0; j < kRows; j++) read_start<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
     };
     Ring<S> at;
     if (first < g.total) {
       rows_of(first);
-      read(begin_of(first) * BK);
+      start(begin_of(first) * BK);
     }
     for (int64_t t = first; t < g.total && !fail; t += step) {
       const int k0 = begin_of(t) * BK, end = k0 + count_of(t) * BK;
@@ -373,10 +392,10 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         for (int j = 0; j < kRows; j++) v[j] = read_end<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
         // The next stage is on its way while this one waits for room.
         if (k + BK < end) {
-          read(k + BK);
+          start(k + BK);
         } else if (t + step < g.total) {
           rows_of(t + step);
-          read(begin_of(t + step) * BK);
+          start(begin_of(t + step) * BK);
         }
         if (__any_sync(0xFFFFFFFFu, !mbar_wait_parked(&empty[at.s], at.turn ^ 1))) {
           fail = true;
@@ -389,7 +408,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
           *(uint4*)(to + r * BK + ((chunk ^ (r & 7)) << 4)) = v[j];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        arrive_first(&full[at.s]);
+        mbar_arrive(&read[at.s]);
       }
     }
   } else if (warp >= 4) {
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
         tmem_wait(r);
         if (j + kBlock == kMine) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          if (lane == 0) arrive_first(&sum_empty[sum.s]);
+          if (lane == 0) arrive_first<false>(&sum_empty[sum.s]);
         }
         if (t0 + j >= g.to.tokens) continue;
         if (whole) {

@@ -53,10 +53,12 @@ constexpr int kGemmSmem = kOrthStages * kStage + kOutWarps * kBuffer + 256 + 102
 
 // ------------------------------------------------------- PTX wrappers
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+// Into this CTA's memory; the bytes are reported to a barrier of either CTA of the pair.
+__device__ __forceinline__ void pair_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
 
@@ -381,15 +383,16 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* base = smem_raw + (-smem_addr(smem_raw) & 1023);  // (a cast through an integer would make every access generic)
   uint8_t* buffers = base + kOrthStages * kStage;
-  uint64_t* full = (uint64_t*)(buffers + kOutWarps * kBuffer);
+  uint64_t* full = (uint64_t*)(buffers + kOutWarps * kBuffer);  // the first CTA's counts what both have loaded
   uint64_t* empty = full + kOrthStages;
-  uint64_t* peer = empty + kOrthStages;   // the first CTA's: the second's stage is full
-  uint64_t* sum_full = peer + kOrthStages;
+  uint64_t* sum_full = empty + kOrthStages;
   uint64_t* sum_empty = sum_full + 2;     // the first CTA's
   uint32_t* tmem_at = (uint32_t*)(sum_empty + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
   const int first = (int)(blockIdx.x / 2), step = (int)(gridDim.x / 2);
+  uint32_t full0;  // the first CTA's
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(full0) : "r"(smem_addr(full)));
   const int all = (g.k + kBK - 1) / kBK;
   // The stages of a work item.
   auto begin_of = [&](int t) { return MODE == PART ? t % g.splits * g.split_k : 0; };
@@ -400,7 +403,6 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
     for (int s = 0; s < kOrthStages; s++) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
-      mbar_init(&peer[s], 1);
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sum_full[b], 1);
@@ -441,27 +443,28 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             break;
           }
           const uint32_t to = smem_addr(base + s * kStage);
-          mbar_expect_tx(&full[s], 2 * (kSide + TN / 2) * kBK * 2);
+          const uint32_t bar = full0 + s * 8;
+          if (!rank) mbar_expect_tx(&full[s], 2 * 2 * (kSide + TN / 2) * kBK * 2);
 #pragma unroll
           for (int half = 0; half < 2; half++)
 #pragma unroll
             for (int p = 0; p < 2; p++) {
               const uint32_t at = to + p * kPlane + half * (kPlane / 2);
               const int r = row + half * 64, c = col + half * 64, k = (b0 + b) * kBK;
-              tma_load_3d(at, &map_p, P_MN ? r : k, P_MN ? k : r, z + p, &full[s]);
-              if (half * 128 < TN) tma_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, &full[s]);
+              pair_load_3d(at, &map_p, P_MN ? r : k, P_MN ? k : r, z + p, bar);
+              if (half * 128 < TN) pair_load_3d(at + 2 * kPlane, &map_q, Q_MN ? c : k, Q_MN ? k : c, z + p, bar);
             }
         }
       }
       // Leave only with no copy of ours and no arrival for us left in flight.
       for (int64_t j = i > kOrthStages ? i - kOrthStages : 0; j < i; j++) {
         const unsigned turn = (unsigned)((j / kOrthStages) & 1);
-        if (!mbar_wait_bounded(&full[j % kOrthStages], turn)) fail = true;
+        if (!rank && !mbar_wait_bounded(&full[j % kOrthStages], turn)) fail = true;
         if (!fail && !mbar_wait_bounded(&empty[j % kOrthStages], turn)) fail = true;
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && !rank) {
       const uint32_t idesc = (1u << 4) | ((uint32_t)P_MN << 15) | ((uint32_t)Q_MN << 16) |
                              ((uint32_t)(TN >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
       int64_t i = 0, u = 0;  // stages and sums so far
@@ -471,16 +474,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
         for (int b = 0; b < blocks; b++, i++) {
           const int s = (int)(i % kOrthStages), d = (int)(u & 1);
           const unsigned turn = (unsigned)((i / kOrthStages) & 1);
-          if (!mbar_wait_bounded(&full[s], turn)) {
-            fail = true;
-            break;
-          }
-          if (rank) {
-            arrive_first(&peer[s]);
-            continue;
-          }
-          if (!mbar_wait_bounded(&peer[s], turn) ||
-              (in_sum == 0 && u >= 2 && !mbar_wait_bounded(&sum_empty[d], (unsigned)((u / 2 - 1) & 1)))) {
+          if (!mbar_wait_bounded(&full[s], turn) ||
+              (in_sum == 0 && u >= 2 && !pair_wait(&sum_empty[d], (unsigned)((u / 2 - 1) & 1)))) {
             fail = true;
             break;
           }
@@ -504,7 +499,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             products(to, 0, kBK / 32, 0);
             pair_commit(&sum_full[d]);
             u++;
-            if (u >= 2 && !mbar_wait_bounded(&sum_empty[u & 1], (unsigned)((u / 2 - 1) & 1))) {
+            if (u >= 2 && !pair_wait(&sum_empty[u & 1], (unsigned)((u / 2 - 1) & 1))) {
               fail = true;
               break;
             }
@@ -553,7 +548,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1) orth_gemm_kernel(const __grid
             tmem_load32(lanes + d * kTile + c + 32, x[(c / 32 + 1) & 1]);
           } else {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            if (lane == 0) arrive_first(&sum_empty[d]);
+            if (lane == 0) arrive_first<false>(&sum_empty[d]);
           }
 #pragma unroll
           for (int j = 0; j < 32; j++) acc[c + j] = __fadd_rn(acc[c + j], __uint_as_float(x[c / 32 & 1][j]));

@@ -38,12 +38,44 @@ __device__ __forceinline__ void pair_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Arrives on the first CTA's barrier, from either.
-__device__ __forceinline__ void arrive_first(uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(
-          smem_addr(bar))
-      : "memory");
+// Arrives on the first CTA's barrier, from either.  A barrier operation that names no scope orders within its own
+// CTA only, so these, and the waits for them, name the cluster.  Tensor memory is ordered by the tcgen05 fences
+// around them and needs no more.  What shared memory holds (PUBLISH) is released here and acquired by pair_acquire,
+// for which a thread waits: warps that have nothing else to do take that on themselves.  (48 x 16384 x 4095 with
+// a weight that threads read: 51 us where each of them releases and the thread that issues products acquires, 34 us
+// so; the gradient of 8192 x 4096 x 4096, where TMEM alone is handed over: 402 and 275 us.)
+template <bool PUBLISH> __device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  const uint32_t at = smem_addr(bar);
+  if constexpr (PUBLISH)
+    asm volatile(
+        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n"
+        " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}\n" ::"r"(at)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, 0;\n"
+        " mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [r];\n}\n" ::"r"(at)
+        : "memory");
+}
+
+// Bounded wait for phase `parity` of a barrier at which both CTAs arrive, like mbar_wait_bounded.
+__device__ __forceinline__ bool pair_wait(uint64_t* bar, unsigned parity) {
+  const uint32_t at = smem_addr(bar);
+  for (long spins = 0; spins <= kWaitLimit; spins++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(at), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
@@ -119,6 +151,37 @@ __device__ __forceinline__ bool mbar_wait_parked(uint64_t* bar, unsigned parity)
   return false;
 }
 
+// The same for barriers at which both CTAs arrive; pair_acquire sees what was published.
+__device__ __forceinline__ bool pair_wait_parked(uint64_t* bar, unsigned parity) {
+  const uint32_t at = smem_addr(bar);
+  for (int turns = 0; turns < kParkLimit; turns++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(1000)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ bool pair_acquire(uint64_t* bar, unsigned parity) {
+  const uint32_t at = smem_addr(bar);
+  for (int turns = 0; turns < kParkLimit; turns++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(1000)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
 // Whether phase `parity` of `bar` is over.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, unsigned parity) {
   uint32_t ok;
@@ -126,6 +189,19 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, unsigned parity) {
       "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
       : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The same for a barrier at which both CTAs arrive.
+__device__ __forceinline__ bool pair_test(uint64_t* bar, unsigned parity) {
+  const uint32_t at = smem_addr(bar);
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(at), "r"(parity)
       : "memory");
   return ok != 0;
 }
