@@ -627,8 +627,9 @@ int dcf_checkpoint_grad(const dcf_checkpoint_desc* desc, const void* grad,
 /* Device forms: device pointers of one device, work queued on `stream` of
  * that device, the caller's current device kept.  Elements between rows that a
  * stride leaves out are not written.  Results must not overlap operands
- * (checked; rows between each other's, the same stride apart, do not).  a_scale
- * is NULL where a is of a float type; bias may be NULL.  Workspaces hold tokens
+ * (checked; rows between each other's, the same stride apart, do not).  Operands
+ * may be read from the 16-byte boundary before a row on, never behind their last
+ * element.  a_scale is NULL where a is of a float type; bias may be NULL.  Workspaces hold tokens
  * quantised in the call, copies of operands whose rows lie off 16-byte
  * boundaries, the 16-bit form of a checkpoint, and parts of sums; they and the
  * status are as for dcf_orthogonalize_async.  Sums run in a fixed

@@ -71,6 +71,7 @@ struct GemmArgs {
   int* part;               // sums of the parts, where there is more than one
   const int8_t* b;         // the weight, where threads read it
   int64_t b_stride;
+  int whole;               // rows whose last vector lies in the weight's memory
   int depth;
   int early;               // only the kernel that quantised the tokens ran since the weight may have changed
   dcf_status* st;
@@ -165,18 +166,39 @@ __device__ __forceinline__ void write_block(const Result& g, const uint32_t (&r)
   }
 }
 
+// A row's vectors may start before it, in the allocation that holds it, and hold what follows it, but for the last rows
+// (all but `whole`), behind which the memory may end: the ends of these are left out at first and read by bytes before
+// they are used.  Of the rows up to `whole` and `rows`, the number whose vector with `have` bytes up to the row's
+// end is read at once (asked for a row's last turn only; with all of this at each load 48 x 16384 x 4095 took 43 us
+// instead of 34):
+__device__ __forceinline__ int read_at_once(int have, int whole, int rows) {
+  return have >= 16 ? rows : have > 0 ? whole : 0;
+}
+
+__device__ __forceinline__ void last_bytes(uint4& v, const int8_t* p, int have) {
+  if (have > 0 && have < 16) v = first_bytes(p, have);
+}
+
 // Sixteen bytes of a row from k on, zeros behind its end, where the row may start
 // at any byte.  L neighbours in a warp read 16 L bytes of the row
-// as the 16-byte vectors that hold them (all within the allocation that holds
-// the row), and take what they lack from each other.
-template <int L>
-__device__ __forceinline__ void read_start(const int8_t* row, int k, int depth, int lane, uint4& own, uint4& next) {
+// as the 16-byte vectors that hold them, and take what they lack from each other.
+template <int L, bool LAST>
+__device__ __forceinline__ void read_start(const int8_t* row, int k, int depth, bool there, bool whole, int lane, uint4& own,
+                                           uint4& next) {
   const int8_t* p = row + k;
-  const int off = (int)((uintptr_t)p & 15);
+  const int off = (int)((uintptr_t)p & 15), have = depth - k + off;
   own = next = make_uint4(0, 0, 0, 0);
-  if (!row) return;
-  if (k - off < depth) own = *(const uint4*)(p - off);
-  if (off && (lane & (L - 1)) == L - 1 && k + 16 - off < depth) next = *(const uint4*)(p - off + 16);
+  if (LAST ? read_at_once(have, whole, there) : there) own = *(const uint4*)(p - off);
+  if (off && (lane & (L - 1)) == L - 1 && (LAST ? read_at_once(have - 16, whole, there) : there))
+    next = *(const uint4*)(p - off + 16);
+}
+
+template <int L>
+__device__ __forceinline__ void read_last(const int8_t* row, int k, int depth, int lane, uint4& own, uint4& next) {
+  const int8_t* p = row + k;
+  const int off = (int)((uintptr_t)p & 15), have = depth - k + off;
+  last_bytes(own, p - off, have);
+  if (off && (lane & (L - 1)) == L - 1) last_bytes(next, p - off + 16, have - 16);
 }
 
 template <int L>
@@ -368,16 +390,26 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     constexpr int kRows = kSide * 8 / kReaders;
     uint4 own[kRows], next[kRows];
     const int8_t* rows[kRows];
+    bool there[kRows], whole[kRows];
     auto rows_of = [&](int64_t t) {
 #pragma unroll
       for (int j = 0; j < kRows; j++) {
         const int64_t r = (t / g.splits) % g.tiles_m * kTileM + rank * kSide + id / 8 + j * (kReaders / 8);
-        rows[j] = r < g.to.channels ? g.b + r * g.b_stride : nullptr;
+        rows[j] = g.b + r * g.b_stride;
+        there[j] = r < g.to.channels;
+        whole[j] = r < g.whole;
       }
     };
     auto start = [&](int k) {
+      if (k + BK + 16 <= g.depth) {
 #pragma unroll
-      for (int j = 0; j < kRows; j++) read_start<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
+        for (int j = 0; j < kRows; j++)
+          read_start<8, false>(rows[j], k + chunk * 16, g.depth, there[j], whole[j], lane, own[j], next[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kRows; j++)
+          read_start<8, true>(rows[j], k + chunk * 16, g.depth, there[j], whole[j], lane, own[j], next[j]);
+      }
     };
     Ring<S> at;
     if (first < g.total) {
@@ -388,6 +420,11 @@ __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
       const int k0 = begin_of(t) * BK, end = k0 + count_of(t) * BK;
       for (int k = k0; k < end; k += BK, at.next()) {
         uint4 v[kRows];
+        if (k + BK + 16 > g.depth) {
+#pragma unroll
+          for (int j = 0; j < kRows; j++)
+            if (there[j] && !whole[j]) read_last<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
+        }
 #pragma unroll
         for (int j = 0; j < kRows; j++) v[j] = read_end<8>(rows[j], k + chunk * 16, g.depth, lane, own[j], next[j]);
         // The next stage is on its way while this one waits for room.
@@ -511,9 +548,9 @@ __global__ void __launch_bounds__(kJoinThreads) int8_join_kernel(const __grid_co
 // where a block quantises them itself while that is little work.  One wave of
 // blocks takes all channels in turns.
 //
-// A weight off 16-byte boundaries is read as the vectors that hold its rows
-// (all within the allocation that holds the row), and each lane makes up its sixteen
-// bytes from its vector and its neighbour's; the last lane lends its vector only.
+// A weight off 16-byte boundaries is read as the vectors that hold its rows,
+// and each lane makes up its sixteen bytes from its vector and its neighbour's; the last
+// lane lends its vector only.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int kFewTokens = 4, kFewChannels = 8;
 constexpr int kFewResident = 2;          // blocks to an SM
@@ -528,6 +565,7 @@ struct FewArgs {
   int64_t a_stride;
   const int8_t* b;
   int64_t b_stride;
+  int whole;               // rows whose last vector lies in the weight's memory
   int depth, padded;       // padded: to whole turns of a warp, and a vector of zeros
   int across;              // warps along the depth
   int early;               // only the kernel that quantised the tokens ran since the weight may have changed
@@ -586,15 +624,22 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(con
   const int64_t step = (int64_t)gridDim.x * groups * C;
   int64_t c0 = ((int64_t)blockIdx.x * groups + warp / g.across) * C;
   uint4 own[C];
-  auto load = [&](int j, int64_t c, int k) {  // row c + j
-    const int8_t* p = g.b + (c + j) * g.b_stride + k + lane * 16;
-    const int off = READ ? (int)((uintptr_t)p & 15) : 0;  // bytes before the row, or the end of the vector before
-    own[j] = make_uint4(0, 0, 0, 0);
-    if (c + j < g.to.channels && k + lane * 16 - off < g.depth) own[j] = *(const uint4*)(p - off);  // what else they hold meets zeros
+  auto load = [&](int64_t c, int k) {
+    const int have = g.depth - k - lane * 16, whole = (int)(g.whole - c), rows = (int)(g.to.channels - c);
+    const int8_t* p = g.b + c * g.b_stride + k + lane * 16;
+    auto each = [&](auto at_once) {
+#pragma unroll
+      for (int j = 0; j < C; j++, p += g.b_stride) {
+        const int off = READ ? (int)((uintptr_t)p & 15) : 0;  // bytes before the row, or the end of the vector before
+        own[j] = make_uint4(0, 0, 0, 0);
+        if (j < at_once(off)) own[j] = *(const uint4*)(p - off);  // what else they hold meets zeros
+      }
+    };
+    if (k + 512 <= g.depth) each([&](int) { return rows; });
+    else each([&](int off) { return read_at_once(have + off, whole, rows); });
   };
   if (!g.early) pdl_begin();
-#pragma unroll
-  for (int j = 0; j < C; j++) load(j, c0, start);
+  load(c0, start);
   if (g.early) pdl_begin();
 
   for (int i = threadIdx.x * 16; i < T * g.padded; i += kFewThreads * 16) *(uint4*)(x + i) = make_uint4(0, 0, 0, 0);
@@ -609,16 +654,10 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(con
     for (int t = 0; t < g.to.tokens; t++) {
       const int8_t* in = (const int8_t*)g.a + t * g.a_stride;
       if (g.a_vectors) {
-        for (int k = threadIdx.x * 16; k < g.depth; k += kFewThreads * 16) {
-          uint4 v = *(const uint4*)(in + k);
-          uint32_t* w = (uint32_t*)&v;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int here = g.depth - k - 4 * e;
-            if (here < 4) w[e] = here > 0 ? w[e] & (0xFFFFFFFFu >> (32 - 8 * here)) : 0u;
-          }
-          *(uint4*)(x + t * g.padded + k) = v;
-        }
+        for (int k = threadIdx.x * 16; k + 16 <= g.depth; k += kFewThreads * 16)
+          *(uint4*)(x + t * g.padded + k) = *(const uint4*)(in + k);
+        const int k = g.depth / 16 * 16 + threadIdx.x;
+        if (k < g.depth) x[t * g.padded + k] = in[k];
       } else {
         for (int k = threadIdx.x; k < g.depth; k += kFewThreads) x[t * g.padded + k] = in[k];
       }
@@ -643,6 +682,14 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(con
       if (g.to.bias) bias = g.to.bias[c];
     }
     for (int k0 = start; k0 < g.depth; k0 += turn) {
+      if (c0 + C > g.whole && k0 + 512 > g.depth) {
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+          const int8_t* p = g.b + (c0 + j) * g.b_stride + k0 + lane * 16;
+          const int off = READ ? (int)((uintptr_t)p & 15) : 0;
+          if (c0 + j >= g.whole && c0 + j < g.to.channels) last_bytes(own[j], p - off, g.depth - k0 - lane * 16 + off);
+        }
+      }
       uint4 w[C];
 #pragma unroll
       for (int j = 0; j < C; j++) {
@@ -650,8 +697,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewResident) int8_few_kernel(con
         if (READ) w[j] = shifted_down(w[j], (int)((uintptr_t)(g.b + (c0 + j) * g.b_stride) & 15));
       }
       const bool more = k0 + turn < g.depth;
-#pragma unroll
-      for (int j = 0; j < C; j++) load(j, more ? c0 : c0 + step, more ? k0 + turn : start);
+      load(more ? c0 : c0 + step, more ? k0 + turn : start);
       const int k = READ && lane == 31 ? g.padded - 16 : k0 + lane * 16;
 #pragma unroll
       for (int t = 0; t < T; t++) {
@@ -702,6 +748,12 @@ int64_t stride_of(int64_t given, uint64_t cols) { return given ? given : (int64_
 // Whether a tensor map describes rows of bytes as they lie.
 bool mappable(const void* p, int64_t stride, uint64_t cols) {
   return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride >= (int64_t)cols && stride < (1ll << 40);
+}
+
+// The rows of a weight that are followed by another 15 bytes of it.
+int whole_rows(uint64_t rows, int64_t stride) {
+  const int64_t last = (15 + stride - 1) / stride;
+  return (int64_t)rows > last ? (int)((int64_t)rows - last) : 0;
 }
 
 // How a product is laid out: tokens of a tile, and the parts into which its
@@ -875,6 +927,7 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     g.a_vectors = on16(a, as, d.tokens, dtype_size(g.a_dtype));
     g.b = b;
     g.b_stride = bs;
+    g.whole = whole_rows(d.channels, bs);
     g.depth = (int)d.depth;
     g.padded = few_padded(d);
     g.early = ours;
@@ -903,6 +956,7 @@ int launch_int8_matmul(const dcf_int8_desc& d, const void* a, const float* a_sca
     g.split_k = cut.stages * (kBK<false> / bk);
     g.b = b;
     g.b_stride = bs;
+    g.whole = whole_rows(d.channels, bs);
     g.depth = (int)d.depth;
     g.early = ours && !l.copy_b;
     if (!encoder()) return DCF_EUNSUPPORTED;

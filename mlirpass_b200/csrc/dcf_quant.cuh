@@ -166,6 +166,18 @@ __device__ __forceinline__ uint4 bytes_from(const uint4& own, const uint4& next,
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The vector at p (a 16-byte boundary), of which the first `have` bytes (1 to 15) are there, zeros behind them.
+__device__ __forceinline__ uint4 first_bytes(const void* at, int have) {
+  const uint8_t* p = (const uint8_t*)at;
+  const int n8 = have & 8, n4 = have & 4, n2 = have & 2;
+  const uint64_t eight = n8 ? *(const uint64_t*)p : 0;
+  uint64_t rest = n4 ? *(const uint32_t*)(p + n8) : 0;
+  rest |= (uint64_t)(n2 ? *(const uint16_t*)(p + n8 + n4) : 0) << (8 * n4);
+  rest |= (uint64_t)(have & 1 ? p[have - 1] : 0) << (8 * (n4 + n2));
+  const uint64_t lo = n8 ? eight : rest, hi = n8 ? rest : 0;
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
 // Sixteen bytes of a row of `bytes` from byte c (a multiple of 16) on, zeros behind its end; the row may start anywhere.
 __device__ __forceinline__ uint4 row_bytes(const uint8_t* row, int64_t c, int64_t bytes) {
   const uint8_t* p = row + c;
