@@ -46,7 +46,7 @@ struct GradArgs {
   int out_dtype, add;
   int pairs;               // two neighbours of a row of a 16-bit result make an aligned word
   int vectors;             // four neighbours of a row make an aligned vector
-  int tokens, channels, depth;
+  int channels, depth;
   int skip;                // columns of the gradient's map before its first channel
   int64_t os;
   int runs, tiles_m;       // tiles along k
@@ -56,14 +56,6 @@ struct GradArgs {
   uint32_t idesc;
   dcf_status* st;
 };
-
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
 
 // The low half of an operand's descriptor, whose memory runs along it: blocks of 64
 // lie kBlockBytes apart.  The high half says that groups of eight tokens lie
@@ -602,7 +594,6 @@ int launch_checkpoint_grad(const dcf_checkpoint_desc& d, const void* grad, const
   g.out = out;
   g.out_dtype = (int)d.out_dtype;
   g.add = (d.flags & DCF_CHECKPOINT_ACCUMULATE) != 0;
-  g.tokens = (int)d.tokens;
   g.channels = (int)d.channels;
   g.depth = (int)d.depth;
   g.os = stride_of(d.out_row_stride, d.depth);

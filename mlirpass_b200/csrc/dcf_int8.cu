@@ -65,7 +65,7 @@ template <int TN, bool READ> constexpr int kGemmSmem = kStages<TN, READ> * kStag
 struct GemmArgs {
   Result to;
   int blocks;              // stages along the whole depth
-  int tiles_m, tiles;      // tiles along the channels, in all
+  int tiles_m;             // tiles along the channels
   int splits, split_k;     // parts of the depth, stages of each
   int64_t total;           // tiles times splits
   int* part;               // sums of the parts, where there is more than one
@@ -76,15 +76,6 @@ struct GemmArgs {
   int early;               // only the kernel that quantised the tokens ran since the weight may have changed
   dcf_status* st;
 };
-
-// Into this CTA's memory; the bytes are reported to a barrier of either CTA of the pair.
-__device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-      "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
 
 __device__ __forceinline__ void pair_mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -224,10 +215,9 @@ __device__ __forceinline__ uint4 read_end(const int8_t* row, int k, int depth, i
 // in the lanes, so that a warp writes neighbours of a row.  Warp 0 keeps the
 // ring of stages full; one thread of the first CTA issues the products of
 // both: its barrier counts the bytes of both CTAs' loads, as each wait on
-// another costs that thread 160 cycles of the 512 that a stage's four products
-// take (probe: 136 cycles a product with one wait per stage, 176 with two).
-// READ: the weight's rows lie off 16-byte boundaries, and four more warps read
-// them.
+// another costs that thread 160 cycles, and four products take 512 (probe: 136
+// cycles a product with one wait between four of them, 176 with two).
+// READ: no tensor map describes the weight, and eight more warps read it.
 template <int TN, bool READ>
 __global__ void __launch_bounds__(kGemmThreads<READ> + (READ ? kReaders : 0), 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a,
