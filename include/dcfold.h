@@ -629,11 +629,13 @@ int dcf_checkpoint_grad(const dcf_checkpoint_desc* desc, const void* grad,
  * stride leaves out are not written.  Results must not overlap operands
  * (checked; rows between each other's, the same stride apart, do not).  Operands
  * may be read from the 16-byte boundary before a row on, never behind their last
- * element.  a_scale is NULL where a is of a float type; bias may be NULL.  Workspaces hold tokens
- * quantised in the call, copies of operands whose rows lie off 16-byte
- * boundaries, the 16-bit form of a checkpoint, and parts of sums; they and the
- * status are as for dcf_orthogonalize_async.  Sums run in a fixed
- * order: the same call gives the same bits. */
+ * element.  a_scale is NULL where a is of a float type; bias may be NULL.
+ * Workspaces hold tokens quantised in the call or room for a copy of 8-bit ones
+ * (made where their rows lie off 16-byte boundaries), a copy of a weight or a
+ * gradient whose rows are no multiple of 16 bytes apart (of a weight only where tokens
+ * are many), a checkpoint as 16-bit values (two bytes an element), and parts of sums;
+ * they and the status are as for dcf_orthogonalize_async.  Sums run in a
+ * fixed order: the same call gives the same bits. */
 int dcf_quantize_async(const dcf_quant_desc* desc, const void* in, int8_t* q,
                        float* scale, void* stream);
 int dcf_dequantize_async(const dcf_quant_desc* desc, const int8_t* q,

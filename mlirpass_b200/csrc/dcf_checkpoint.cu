@@ -9,15 +9,16 @@
 // from 64 bits than fp32 products are.)
 //
 // Whole numbers become 16-bit values in a pass of their own (three bytes of
-// memory each: 20 us of 8192 x 4096).  Made on their way into each tile instead,
-// by eight warps between the copy and the product, the gradient of 4096
-// channels took 270 us against 220 now: every tile makes them again, and copying,
+// memory each, two of them in the workspace: 20 us of 8192 x 4096).  Made on their way into each
+// tile instead, by eight warps between the copy and the product, the gradient of 4096
+// channels took 270 us against 220 (bursts): every tile makes them again, and copying,
 // reading and writing them in shared memory takes a quarter of what its banks
 // move, which the operands of the products need.
 //
 // What bounds it: at 8192 x 4096 x 4096 the products take 340000 cycles of which
-// the tensor cores are active in 68 % (210 us at the 1.6 GHz that the power
-// limit leaves; 256 tiles on 74 pairs of CTAs are 3.5 rounds of work in 4).
+// the tensor cores are active in 68 %; 256 tiles on 74 pairs of CTAs are 3.5 rounds of work
+// in 4.  With the 16-bit values 210 us in a burst, 240 us in a long run at the power
+// limit (SM at 1.65 GHz; 278 us with inputs that change).
 // Registers that spilt in the one thread that issues products cost more than
 // anything else measured here (317 us): it waits for each, and the tensor core
 // has no more than two products in hand.

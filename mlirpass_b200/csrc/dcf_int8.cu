@@ -5,13 +5,14 @@
 // order, so a sum is split and joined wherever that helps.
 //
 // Three ways, by what bounds them:
-//   up to four tokens       the weight's bytes: int8_few_kernel, on the CUDA cores (4096 x 4096, one bf16
-//                           token: 5.2 us, 2.6 us of bytes; 16384 x 8192: 31 us, 20.5 us of bytes)
+//   up to four tokens       the weight's bytes: int8_few_kernel, on the CUDA cores (one bf16 token, 4096 x 4096 in
+//                           L2: 4.6 us, 2.6 us of bytes at HBM's rate; 16384 x 8192: 30 us, 20.5 us of bytes)
 //   some tens of tokens     the weight's bytes: int8_gemm_kernel with tiles of 64 tokens, the depth cut in parts
 //                           where channels are few (48 x 16384 x 4096: 17 us, 10.5 us of bytes)
-//   more                    the tensor cores: tiles of 128 and 256 tokens (8192 x 8192 x 8192: 334 us, 3290 Tops/s,
-//                           98 % of twice the measured bf16 rate; 4096 x 4096 x 4096: 50 us, 41 us at that rate:
-//                           256 tiles on 74 pairs of CTAs are 3.5 rounds of work in 4)
+//   more                    the tensor cores: tiles of 128 and 256 tokens (bursts of thirty, and long runs at the
+//                           power limit: 8192 x 8192 x 8192 365 and 454 us, the SM at 1.1 GHz, 328 us at twice the
+//                           measured bf16 burst rate; 4096 x 4096 x 4096 48 and 54 us at 1.57 GHz, 41 us at that
+//                           rate: 256 tiles on 74 pairs of CTAs are 3.5 rounds of work in 4)
 #include "dcf_quant.cuh"
 
 namespace dcf {
@@ -795,8 +796,9 @@ bool few(const dcf_int8_desc& d) {
   return d.tokens <= kFewTokens && d.depth && few_bucket(d) * few_padded(d) <= kFewSmem;
 }
 
-// A weight whose rows lie off 16-byte boundaries is read by threads as long as few tokens leave that hidden
-// behind HBM; many have it copied first.
+// A weight whose rows are no multiple of 16 bytes apart is copied first where tiles are wider than 64 tokens. In
+// narrower ones, which read it once or twice, and where only its start lies off a boundary, which is not known before
+// the launch, it is read by threads (1001 x 2048 x 1536: 16 us, 7.4 us by map and some 6 us for a copy).
 Layout layout_of(const dcf_int8_desc& d) {
   Layout l = {};
   auto take = [&](size_t bytes) {

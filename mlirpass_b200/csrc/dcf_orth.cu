@@ -1198,7 +1198,7 @@ constexpr double kMostSingular = 64;
 // f32 (bf16 258 x 131, six steps: 0.21 % of the results, with two stages 0.58 %, fp32 products
 // 0.17 %; 520 x 530: two stages 0.33 %, fp32 products 0.20 %), above two stages (4096 x 4096:
 // 0.25 % and 3.6 ms, with 16 1.8 % and 3.4 ms, fp32 products 0.33 %), up to 1024 rows one in A A
-// (1024 x 4096: 0.16 % and 438 us, with two 0.23 % and 437 us, with 16 1.6 % and 427 us, fp32
+// (1024 x 4096: 0.16 %, with two 0.23 % and 1 us less, with 16 1.6 % and 11 us less of 438, fp32
 // products 0.27 %; 770 x 1540: with two 1.8 times as many as fp32 products).
 int sums_of(const dcf_orth_desc& d, int m, bool square) {
   const bool f32 = d.out_dtype == DCF_F32;
